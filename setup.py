@@ -1,4 +1,5 @@
 """Builds the sm_100a extension in place: python setup.py build_ext --inplace"""
+import ctypes.util
 import glob
 import os
 
@@ -18,11 +19,17 @@ nvcc_flags = [
 if os.environ.get("TGO_PTXAS_VERBOSE"):
     nvcc_flags.append("-Xptxas=-v")
 
+# torch's C++ streams and exceptions cross this extension's border, so both must use one C++ runtime: the shared one comes
+# before a toolchain's own static copy (with two, a refusal whose message holds a number crashes in the stream's locale).
+shared_cxx = ctypes.util.find_library("stdc++")
+link_args = [f"-l:{shared_cxx}"] if shared_cxx else []
+
 setup(
     name="trenowanie_generatora_obrazkow_b200",
     ext_modules=[CUDAExtension(
         name="trenowanie_generatora_obrazkow_b200._C",
         sources=sources,
+        extra_link_args=link_args,
         extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": nvcc_flags},
     )],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},
