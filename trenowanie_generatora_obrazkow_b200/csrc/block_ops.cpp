@@ -1,0 +1,411 @@
+// Torch-facing wrappers of the routed block's kernels (block_ops.h): argument checks, outputs, launches on the current
+// stream. Registered in the extension module by ops.cpp.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <cmath>
+
+#include "block_ops.h"
+#include "kernels.h"
+
+namespace tgo {
+
+void count_launches(int n);  // ops.cpp
+
+namespace {
+
+using OptT = c10::optional<at::Tensor>;
+
+#define BLOCK_LAUNCH(expr, n)                                                         \
+  do {                                                                                \
+    cudaError_t _e = (expr);                                                          \
+    TORCH_CHECK(_e == cudaSuccess, "kernel launch failed: ", cudaGetErrorString(_e)); \
+    count_launches(n);                                                                \
+  } while (0)
+
+int elem_of(const at::Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return ELEM_BF16;
+    case at::kHalf: return ELEM_F16;
+    case at::kFloat: return ELEM_F32;
+    default: TORCH_CHECK(false, what, ": bf16, fp16 or fp32 expected, got ", t.scalar_type());
+  }
+  return -1;
+}
+bool given(const OptT& t) { return t.has_value() && t->defined(); }
+void same_device(const at::Tensor& t, const at::Tensor& as, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == as.device(), what, ": a tensor on ", as.device(), " expected");
+}
+const float* vec_f32(const OptT& t, int64_t n, const at::Tensor& as, const char* what) {
+  if (!given(t)) return nullptr;
+  same_device(*t, as, what);
+  TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == n, what, ": contiguous fp32 [", n,
+              "] expected");
+  return t->data_ptr<float>();
+}
+float* acc_f32(const OptT& t, int64_t n, const at::Tensor& as, const char* what) {
+  return const_cast<float*>(vec_f32(t, n, as, what));
+}
+
+// ---------------------------------------------------------------------------------------------------------- routing
+RouteParams route_params(const at::Tensor& logits, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups,
+                         bool renorm, double scale) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, "route: logits [N, E] with contiguous rows");
+  const int64_t N = logits.size(0), E = logits.size(1);
+  TORCH_CHECK(N < (1ll << 31) && E >= 1 && E <= kRouteMaxExperts, "route: 1 to ", kRouteMaxExperts, " experts");
+  TORCH_CHECK(groups >= 1 && groups <= kRouteMaxGroups && E % groups == 0, "route: groups must divide the experts (at most ",
+              kRouteMaxGroups, ")");
+  TORCH_CHECK(top_groups >= 1 && top_groups <= groups, "route: 1 <= top_groups <= groups");
+  TORCH_CHECK(k >= 1 && k <= kRouteMaxK && k <= top_groups * (E / groups), "route: k between 1 and ", kRouteMaxK,
+              " and at most the experts of the kept groups");
+  TORCH_CHECK(std::isfinite(scale) && scale != 0.0, "route: scale must be finite and not zero");
+  RouteParams p{};
+  p.logits = logits.data_ptr();
+  p.ld = logits.stride(0);
+  p.N = (int)N;
+  p.E = (int)E;
+  p.k = (int)k;
+  p.groups = (int)groups;
+  p.top_groups = (int)top_groups;
+  p.group_size = (int)(E / groups);
+  p.group_magic = (unsigned)(((1u << 22) + p.group_size - 1) / p.group_size);
+  p.sigmoid = sigmoid;
+  p.renorm = renorm;
+  p.scale = (float)scale;
+  return p;
+}
+
+std::tuple<at::Tensor, at::Tensor> route_fwd(at::Tensor logits, OptT bias, OptT valid, int64_t k, bool sigmoid,
+                                             int64_t groups, int64_t top_groups, bool renorm, double scale) {
+  RouteParams p = route_params(logits, k, sigmoid, groups, top_groups, renorm, scale);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  p.bias = vec_f32(bias, p.E, logits, "route: bias");
+  if (given(valid)) {
+    same_device(*valid, logits, "route: valid");
+    TORCH_CHECK(valid->scalar_type() == at::kBool && valid->is_contiguous() && valid->numel() == p.N,
+                "route: valid bool [N]");
+    p.valid = valid->data_ptr<bool>();
+  }
+  at::Tensor w = at::empty({p.N, k}, logits.options().dtype(at::kFloat));
+  at::Tensor idx = at::empty({p.N, k}, logits.options().dtype(at::kInt));
+  p.w = w.data_ptr<float>();
+  p.idx = idx.data_ptr<int>();
+  BLOCK_LAUNCH(route_fwd_launch(p, elem_of(logits, "route"), at::cuda::getCurrentCUDAStream()), p.N > 0);
+  return {w, idx};
+}
+
+at::Tensor route_bwd(at::Tensor logits, at::Tensor w, at::Tensor idx, at::Tensor dw, bool sigmoid, bool renorm,
+                     double scale) {
+  RouteParams p = route_params(logits, w.size(1), sigmoid, 1, 1, renorm, scale);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  same_device(idx, logits, "route_bwd: idx");
+  TORCH_CHECK(idx.scalar_type() == at::kInt && idx.is_contiguous() && idx.sizes() == w.sizes() && w.size(0) == p.N,
+              "route_bwd: idx int32 [N, k]");
+  p.w = const_cast<float*>(vec_f32(w, w.numel(), logits, "route_bwd: w"));
+  p.idx = idx.data_ptr<int>();
+  const float* g = vec_f32(dw, w.numel(), logits, "route_bwd: dw");
+  at::Tensor d = at::empty({p.N, p.E}, logits.options());
+  BLOCK_LAUNCH(route_bwd_launch(p, g, d.data_ptr(), elem_of(logits, "route_bwd"), at::cuda::getCurrentCUDAStream()),
+               p.N > 0);
+  return d;
+}
+
+// ------------------------------------------------------------------------------------------ plan, dispatch, combine
+std::tuple<at::Tensor, at::Tensor, at::Tensor> expert_plan(at::Tensor idx, int64_t experts, int64_t capacity) {
+  TORCH_CHECK(idx.is_cuda() && idx.dim() == 2 && idx.scalar_type() == at::kInt && idx.is_contiguous(),
+              "expert_plan: idx int32 [N, k], contiguous");
+  TORCH_CHECK(experts >= 1 && experts <= kRouteMaxExperts, "expert_plan: 1 to ", kRouteMaxExperts, " experts");
+  TORCH_CHECK(capacity >= 0 && capacity * experts < (1ll << 31) && idx.numel() < (1ll << 31) - 65536,
+              "expert_plan: too many rows");
+  const c10::cuda::CUDAGuard guard(idx.device());
+  PlanParams p{};
+  p.idx = idx.data_ptr<int>();
+  p.A = (int)idx.numel();
+  p.E = (int)experts;
+  p.capacity = (int)capacity;
+  at::Tensor slot = at::empty_like(idx);
+  at::Tensor offsets = at::empty({experts + 1}, idx.options());
+  at::Tensor counts = at::empty({experts}, idx.options());
+  p.slot = slot.data_ptr<int>();
+  p.offsets = offsets.data_ptr<int>();
+  p.counts = counts.data_ptr<int>();
+  BLOCK_LAUNCH(plan_launch(p, at::cuda::getCurrentCUDAStream()), 1);
+  return {slot, offsets, counts};
+}
+
+ExpertRows expert_rows(const at::Tensor& slot, const at::Tensor& offsets, const at::Tensor& counts, int64_t capacity,
+                       int64_t rows, int64_t D, const at::Tensor& as) {
+  same_device(slot, as, "expert rows: slot");
+  same_device(offsets, as, "expert rows: offsets");
+  same_device(counts, as, "expert rows: counts");
+  TORCH_CHECK(slot.scalar_type() == at::kInt && slot.dim() == 2 && slot.is_contiguous() &&
+                  offsets.scalar_type() == at::kInt && offsets.is_contiguous() && counts.scalar_type() == at::kInt &&
+                  counts.is_contiguous() && offsets.numel() == counts.numel() + 1,
+              "expert rows: int32 slot [N, k], offsets [E + 1], counts [E]");
+  ExpertRows r{};
+  r.slot = slot.data_ptr<int>();
+  r.offsets = offsets.data_ptr<int>();
+  r.counts = counts.data_ptr<int>();
+  r.N = (int)slot.size(0);
+  r.k = (int)slot.size(1);
+  r.D = (int)D;
+  r.E = (int)counts.numel();
+  r.capacity = (int)capacity;
+  r.rows = rows;
+  TORCH_CHECK(r.k <= kRouteMaxK, "expert rows: at most ", kRouteMaxK, " choices per token");
+  TORCH_CHECK(rows == (capacity > 0 ? capacity * r.E : slot.numel()), "expert rows: row count");
+  return r;
+}
+
+at::Tensor expert_dispatch(at::Tensor x, at::Tensor slot, at::Tensor offsets, at::Tensor counts, int64_t capacity,
+                           int64_t rows) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(0) == slot.size(0) && (x.size(1) <= 1 || x.stride(1) == 1),
+              "expert_dispatch: x [N, D] with contiguous rows, one per planned token");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const ExpertRows r = expert_rows(slot, offsets, counts, capacity, rows, x.size(1), x);
+  at::Tensor xs = at::empty({rows, x.size(1)}, x.options());
+  BLOCK_LAUNCH(dispatch_launch(r, x.data_ptr(), x.stride(0), xs.data_ptr(), elem_of(x, "expert_dispatch"),
+                               at::cuda::getCurrentCUDAStream()), 1);
+  return xs;
+}
+
+at::Tensor expert_combine(at::Tensor y, OptT w, at::Tensor slot, at::Tensor offsets, at::Tensor counts,
+                          int64_t capacity) {
+  TORCH_CHECK(y.is_cuda() && y.dim() == 2 && y.is_contiguous(), "expert_combine: y [rows, D], contiguous");
+  const c10::cuda::CUDAGuard guard(y.device());
+  const ExpertRows r = expert_rows(slot, offsets, counts, capacity, y.size(0), y.size(1), y);
+  const float* wp = vec_f32(w, slot.numel(), y, "expert_combine: w");
+  at::Tensor out = at::empty({r.N, y.size(1)}, y.options());
+  BLOCK_LAUNCH(combine_launch(r, y.data_ptr(), wp, out.data_ptr(), elem_of(y, "expert_combine"),
+                              at::cuda::getCurrentCUDAStream()), 1);
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> expert_combine_bwd(at::Tensor y, at::Tensor w, at::Tensor dout, at::Tensor slot,
+                                                      at::Tensor offsets, at::Tensor counts, int64_t capacity) {
+  TORCH_CHECK(y.is_cuda() && y.dim() == 2 && y.is_contiguous(), "expert_combine_bwd: y [rows, D], contiguous");
+  TORCH_CHECK(dout.dim() == 2 && dout.size(0) == slot.size(0) && dout.size(1) == y.size(1) &&
+                  dout.scalar_type() == y.scalar_type() && (dout.size(1) <= 1 || dout.stride(1) == 1),
+              "expert_combine_bwd: dout [N, D] with contiguous rows, in y's type");
+  same_device(dout, y, "expert_combine_bwd: dout");
+  const c10::cuda::CUDAGuard guard(y.device());
+  const ExpertRows r = expert_rows(slot, offsets, counts, capacity, y.size(0), y.size(1), y);
+  const float* wp = vec_f32(w, slot.numel(), y, "expert_combine_bwd: w");
+  at::Tensor dy = at::empty_like(y), dw = at::empty({r.N, r.k}, y.options().dtype(at::kFloat));
+  BLOCK_LAUNCH(combine_bwd_launch(r, y.data_ptr(), wp, dout.data_ptr(), dout.stride(0), dy.data_ptr(),
+                                  dw.data_ptr<float>(), elem_of(y, "expert_combine_bwd"),
+                                  at::cuda::getCurrentCUDAStream()), 1);
+  return {dy, dw};
+}
+
+// ---------------------------------------------------------------------------------------------------- sandwich norm
+// [B, D] rows of one value per sample and channel, in x's type, channels contiguous
+const void* sample_rows(const OptT& t, int64_t B, int64_t D, const at::Tensor& x, long long* stride, const char* what) {
+  if (!given(t)) return nullptr;
+  same_device(*t, x, what);
+  TORCH_CHECK(t->dim() == 2 && t->size(0) == B && t->size(1) == D && t->scalar_type() == x.scalar_type() &&
+                  (D <= 1 || t->stride(1) == 1),
+              what, ": [", B, ", ", D, "] rows in x's type with contiguous channels expected");
+  *stride = B > 1 ? t->stride(0) : 0;
+  return t->data_ptr();
+}
+
+SandwichParams sandwich_params(const at::Tensor& x, const at::Tensor& y, const OptT& gate, const OptT& post_w,
+                               const OptT& w, const OptT& shift, const OptT& scale, double res_scale, double eps) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 3 && x.is_contiguous(), "sandwich_norm: x [B, T, D], contiguous");
+  TORCH_CHECK(y.is_contiguous() && y.sizes() == x.sizes() && y.scalar_type() == x.scalar_type(),
+              "sandwich_norm: y as x");
+  same_device(y, x, "sandwich_norm: y");
+  const int64_t B = x.size(0), T = x.size(1), D = x.size(2);
+  TORCH_CHECK(D >= 1 && D <= 16384 && B * T < (1ll << 31), "sandwich_norm: at most 16384 channels");
+  TORCH_CHECK(given(shift) == given(scale), "sandwich_norm: shift and scale together");
+  TORCH_CHECK(given(w) || !given(scale), "sandwich_norm: shift and scale need w (the norm they modulate)");
+  SandwichParams p{};
+  p.x = x.data_ptr();
+  p.y = y.data_ptr();
+  p.gate = sample_rows(gate, B, D, x, &p.gate_bs, "sandwich_norm: gate");
+  p.scale = sample_rows(scale, B, D, x, &p.mod_bs, "sandwich_norm: scale");
+  long long shift_bs = 0;
+  p.shift = sample_rows(shift, B, D, x, &shift_bs, "sandwich_norm: shift");
+  TORCH_CHECK(shift_bs == p.mod_bs, "sandwich_norm: shift and scale must share a row stride");
+  p.post_w = vec_f32(post_w, D, x, "sandwich_norm: post_w");
+  p.w = vec_f32(w, D, x, "sandwich_norm: w");
+  p.res_scale = (float)res_scale;
+  p.eps = (float)eps;
+  p.M = (int)(B * T);
+  p.D = (int)D;
+  p.T = (int)std::max<int64_t>(T, 1);
+  return p;
+}
+
+std::vector<at::Tensor> sandwich_fwd(at::Tensor x, at::Tensor y, OptT gate, OptT post_w, OptT w, OptT shift, OptT scale,
+                                     double res_scale, double eps) {
+  SandwichParams p = sandwich_params(x, y, gate, post_w, w, shift, scale, res_scale, eps);
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor x_new = at::empty_like(x), h, ry, rx;
+  p.x_new = x_new.data_ptr();
+  auto f32 = x.options().dtype(at::kFloat);
+  if (p.post_w != nullptr) {
+    ry = at::empty({p.M}, f32);
+    p.rstd_y = ry.data_ptr<float>();
+  }
+  if (p.w != nullptr) {
+    h = at::empty_like(x);
+    rx = at::empty({p.M}, f32);
+    p.h = h.data_ptr();
+    p.rstd_x = rx.data_ptr<float>();
+  }
+  BLOCK_LAUNCH(sandwich_fwd_launch(p, elem_of(x, "sandwich_norm"), at::cuda::getCurrentCUDAStream()), p.M > 0);
+  return {x_new, h, ry, rx};
+}
+
+// -> dx, dy, dgate, dshift, dscale; dpost_w and dw are accumulated (+=)
+std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Tensor y, OptT gate, OptT post_w, OptT w,
+                                     OptT shift, OptT scale, OptT ry, OptT rx, OptT dpost_w, OptT dw, double res_scale,
+                                     double eps) {
+  SandwichParams p = sandwich_params(x, y, gate, post_w, w, shift, scale, res_scale, eps);
+  const c10::cuda::CUDAGuard guard(x.device());
+  p.rstd_y = acc_f32(ry, p.M, x, "sandwich_bwd: ry");
+  p.rstd_x = acc_f32(rx, p.M, x, "sandwich_bwd: rx");
+  TORCH_CHECK((p.rstd_y != nullptr || p.post_w == nullptr) && (p.rstd_x != nullptr || p.w == nullptr),
+              "sandwich_bwd: the forward's statistics");
+  SandwichBwdParams q{};
+  auto grad_in = [&](const OptT& t, const char* what) -> const void* {
+    if (!given(t)) return nullptr;
+    same_device(*t, x, what);
+    TORCH_CHECK(t->is_contiguous() && t->sizes() == x.sizes() && t->scalar_type() == x.scalar_type(), what, ": as x");
+    return t->data_ptr();
+  };
+  q.dx_new = grad_in(dx_new, "sandwich_bwd: dx_new");
+  q.dh = grad_in(dh, "sandwich_bwd: dh");
+  at::Tensor dx = at::empty_like(x), dy = at::empty_like(x), dgate, dshift, dscale;
+  q.dx = dx.data_ptr();
+  q.dy = dy.data_ptr();
+  const int64_t B = x.size(0), D = x.size(2);
+  if (p.gate != nullptr) {
+    dgate = at::empty({B, D}, x.options());
+    q.dgate = dgate.data_ptr();
+  }
+  if (p.scale != nullptr) {
+    at::Tensor both = at::empty({2, B, D}, x.options());
+    dshift = both[0];
+    dscale = both[1];
+    q.dshift = dshift.data_ptr();
+    q.dscale = dscale.data_ptr();
+  }
+  q.dpost_w = acc_f32(dpost_w, D, x, "sandwich_bwd: dpost_w");
+  q.dw = acc_f32(dw, D, x, "sandwich_bwd: dw");
+  if (p.M == 0) {
+    if (dgate.defined()) dgate.zero_();
+    if (dshift.defined()) dshift.zero_(), dscale.zero_();
+    return {dx, dy, dgate, dshift, dscale};
+  }
+  const int elem = elem_of(x, "sandwich_bwd");
+  sandwich_bwd_plan(p, elem, &q);
+  const int64_t entries = q.ctas + B, floats = entries * 3 * D + (int64_t)q.groups * 2 * D;
+  at::Tensor scratch = at::empty({floats}, x.options().dtype(at::kFloat));
+  q.partial = scratch.data_ptr<float>();
+  q.wpart = q.partial + entries * 3 * D;
+  BLOCK_LAUNCH(sandwich_bwd_launch(p, q, elem, at::cuda::getCurrentCUDAStream()), 3);
+  return {dx, dy, dgate, dshift, dscale};
+}
+
+// -------------------------------------------------------------------------------------------------- multi-axis rotary
+RopeAxesParams rope_params(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& freq,
+                           const at::Tensor& axis, const OptT& q_w, const OptT& k_w, bool interleaved, double eps) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3, "rope_axes: q [M, Hq, d], k [M, Hkv, d]");
+  same_device(k, q, "rope_axes: k");
+  same_device(pos, q, "rope_axes: pos");
+  same_device(freq, q, "rope_axes: freq");
+  same_device(axis, q, "rope_axes: axis");
+  const int64_t M = q.size(0), hd = q.size(2);
+  TORCH_CHECK(k.size(0) == M && k.size(2) == hd && k.scalar_type() == q.scalar_type(), "rope_axes: k as q");
+  auto heads_ok = [&](const at::Tensor& t) {
+    return (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) == hd);
+  };
+  TORCH_CHECK(heads_ok(q) && heads_ok(k), "rope_axes: the heads of a token must be contiguous");
+  TORCH_CHECK(hd >= 2 && hd <= 1024 && M < (1ll << 31), "rope_axes: head dim 2 to 1024");
+  TORCH_CHECK(pos.dim() == 2 && pos.size(0) == M && pos.is_contiguous() && pos.size(1) >= 1 &&
+                  pos.size(1) <= kRopeMaxAxes && (pos.scalar_type() == at::kInt || pos.scalar_type() == at::kFloat),
+              "rope_axes: pos int32 or fp32 [M, axes], at most ", kRopeMaxAxes, " axes");
+  TORCH_CHECK(freq.scalar_type() == at::kFloat && freq.is_contiguous() && freq.dim() == 2 && freq.size(0) == 2 &&
+                  axis.scalar_type() == at::kInt && axis.is_contiguous() && axis.numel() == freq.size(1) &&
+                  2 * freq.size(1) <= hd,
+              "rope_axes: freq fp32 [2, pairs], axis int32 [pairs], at most d / 2 pairs");
+  RopeAxesParams p{};
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.q_ts = q.stride(0);
+  p.k_ts = k.stride(0);
+  p.pos = pos.data_ptr();
+  p.pos_f32 = pos.scalar_type() == at::kFloat;
+  p.freq = freq.data_ptr<float>();
+  p.axis = axis.data_ptr<int>();
+  p.q_w = vec_f32(q_w, hd, q, "rope_axes: q_w");
+  p.k_w = vec_f32(k_w, hd, q, "rope_axes: k_w");
+  TORCH_CHECK((p.q_w == nullptr) == (p.k_w == nullptr), "rope_axes: q and k norm weights both or neither");
+  p.eps = (float)eps;
+  p.M = (int)M;
+  p.axes = (int)pos.size(1);
+  p.hq = (int)q.size(1);
+  p.hkv = (int)k.size(1);
+  p.hd = (int)hd;
+  p.rot = (int)(2 * freq.size(1));
+  p.interleaved = interleaved;
+  return p;
+}
+
+std::tuple<at::Tensor, at::Tensor> rope_axes_fwd(at::Tensor q, at::Tensor k, at::Tensor pos, at::Tensor freq,
+                                                 at::Tensor axis, OptT q_w, OptT k_w, bool interleaved, double eps) {
+  RopeAxesParams p = rope_params(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  p.q_out = qo.data_ptr();
+  p.k_out = ko.data_ptr();
+  BLOCK_LAUNCH(rope_axes_fwd_launch(p, elem_of(q, "rope_axes"), at::cuda::getCurrentCUDAStream()), p.M > 0);
+  return {qo, ko};
+}
+
+// -> dq_in, dk_in; dq_w and dk_w (both or neither) are accumulated (+=)
+std::tuple<at::Tensor, at::Tensor> rope_axes_bwd(at::Tensor dq, at::Tensor dk, at::Tensor q, at::Tensor k,
+                                                 at::Tensor pos, at::Tensor freq, at::Tensor axis, OptT q_w, OptT k_w,
+                                                 OptT dq_w, OptT dk_w, bool interleaved, double eps) {
+  RopeAxesParams p = rope_params(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto grad_ok = [&](const at::Tensor& g, const at::Tensor& t) {
+    return g.is_contiguous() && g.sizes() == t.sizes() && g.scalar_type() == t.scalar_type() &&
+           g.device() == t.device();
+  };
+  TORCH_CHECK(grad_ok(dq, q) && grad_ok(dk, k), "rope_axes_bwd: dq / dk contiguous, as q / k");
+  at::Tensor dqi = at::empty_like(dq), dki = at::empty_like(dk), partial;
+  float* gq = acc_f32(dq_w, p.hd, q, "rope_axes_bwd: dq_w");
+  float* gk = acc_f32(dk_w, p.hd, q, "rope_axes_bwd: dk_w");
+  TORCH_CHECK((gq == nullptr) == (gk == nullptr) && (gq == nullptr || p.q_w != nullptr),
+              "rope_axes_bwd: dq_w and dk_w both or neither, with the norm weights");
+  if (p.M == 0) return {dqi, dki};
+  if (gq != nullptr)
+    partial = at::empty({rope_axes_bwd_ctas(p), 2, p.hd}, q.options().dtype(at::kFloat));
+  BLOCK_LAUNCH(rope_axes_bwd_launch(p, dq.data_ptr(), dk.data_ptr(), dqi.data_ptr(), dki.data_ptr(),
+                                    gq != nullptr ? partial.data_ptr<float>() : nullptr, gq, gk,
+                                    elem_of(q, "rope_axes_bwd"), at::cuda::getCurrentCUDAStream()),
+               gq != nullptr ? 2 : 1);
+  return {dqi, dki};
+}
+
+}  // namespace
+
+void bind_block_ops(pybind11::module_& m) {
+  m.def("route_fwd", &route_fwd, "expert scores, group-limited top-k and weights of every token");
+  m.def("route_bwd", &route_bwd, "gradient of the chosen experts' weights to the router's logits");
+  m.def("expert_plan", &expert_plan, "stable row of every assignment in expert order, offsets and counts");
+  m.def("expert_dispatch", &expert_dispatch, "token rows into expert order");
+  m.def("expert_combine", &expert_combine, "weighted sum of a token's rows from expert order");
+  m.def("expert_combine_bwd", &expert_combine_bwd, "gradient of expert_combine to the rows and the weights");
+  m.def("sandwich_fwd", &sandwich_fwd, "x + r gate rmsnorm(y) post_w, then rmsnorm, w, scale and shift");
+  m.def("sandwich_bwd", &sandwich_bwd, "backward of sandwich_fwd");
+  m.def("rope_axes_fwd", &rope_axes_fwd, "q/k RMSNorm and rotary positions with several axes");
+  m.def("rope_axes_bwd", &rope_axes_bwd, "backward of rope_axes_fwd");
+}
+
+}  // namespace tgo

@@ -139,3 +139,124 @@ def swiglu(ab):
 def valid_to_len(valid):
     """Boolean key mask [B, L] (a prefix per row, captions are right-padded) -> int32 lengths [B]."""
     return valid.sum(dim=1).to(torch.int32)
+
+
+def route_experts(logits, k, score="softmax", bias=None, groups=1, top_groups=1, renorm=True, scale=1.0, valid=None):
+    """Expert choice and weights (see ops/routing.py); NaN scores come last."""
+    l = logits.float() if logits.dtype in (torch.bfloat16, torch.float16) else logits
+    n, e = l.shape
+    if score == "softmax":
+        p = torch.softmax(torch.where((l == -math.inf).all(-1, keepdim=True), torch.zeros_like(l), l), -1)
+        p = torch.where((l == -math.inf), torch.zeros_like(p), p)
+        key = l.detach()
+    else:
+        p = torch.sigmoid(l)
+        key = p.detach()
+    if bias is not None:
+        key = key + bias
+    live = torch.ones_like(key, dtype=torch.bool)
+    nan = key.isnan()
+    key = key.masked_fill(nan, -math.inf)
+    if groups > 1:
+        by = key.view(n, groups, -1).sort(dim=-1, descending=True).values
+        worth = by[..., 0] if score == "softmax" or by.shape[-1] == 1 else by[..., 0] + by[..., 1]
+        worth = worth.masked_fill(worth.isnan(), -math.inf)
+        kept = worth.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups]
+        on = torch.zeros(n, groups, device=l.device, dtype=torch.bool).scatter_(1, kept, True)
+        live = on.repeat_interleave(e // groups, 1)
+    order = key.sort(dim=-1, descending=True, stable=True).indices
+    late = 2 * (~live).to(torch.int8) + nan.to(torch.int8)  # kept numbers, kept NaNs, then dropped groups
+    idx = order.gather(1, late.gather(1, order).sort(dim=-1, stable=True).indices)[:, :k]
+    w = p.gather(1, idx)
+    if renorm:
+        w = w / (w.sum(-1, keepdim=True) + 1e-20)
+    w, idx = w * scale, idx.to(torch.int32)
+    if valid is not None:
+        w, idx = w * valid[:, None], idx.masked_fill(~valid[:, None], -1)
+    return w, idx
+
+
+def expert_plan(idx, experts, capacity=0):
+    """(slot [N, k], offsets [E + 1], counts [E]), int32: a stable counting sort of the assignments by expert."""
+    flat = idx.reshape(-1).long()
+    flat = torch.where((flat >= 0) & (flat < experts), flat, torch.full_like(flat, -1))
+    hit = flat[:, None] == torch.arange(experts, device=flat.device)
+    rank = (hit.cumsum(0) - 1).gather(1, flat.clamp(min=0)[:, None])[:, 0]
+    counts = hit.sum(0)
+    if capacity:
+        offsets = torch.arange(experts + 1, device=flat.device) * capacity
+        ok = (flat >= 0) & (rank < capacity)
+    else:
+        offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+        ok = flat >= 0
+    slot = torch.where(ok, offsets[flat.clamp(min=0)] + rank, torch.full_like(flat, -1))
+    i32 = torch.int32
+    return slot.view(idx.shape).to(i32), offsets.to(i32), counts.to(i32)
+
+
+def expert_dispatch(x, plan):
+    """x [N, D] -> [rows, D] (unused rows zero)."""
+    k = plan.slot.shape[1]
+    slot = plan.slot.reshape(-1).long()
+    at = torch.where(slot >= 0, slot, torch.full_like(slot, plan.rows))
+    return x.new_zeros(plan.rows + 1, x.shape[1]).index_copy(0, at, x.repeat_interleave(k, 0))[:plan.rows]
+
+
+def expert_combine(y, w, plan):
+    """y [rows, D], w [N, k] -> [N, D]."""
+    n, k = plan.slot.shape
+    slot = plan.slot.reshape(-1).long()
+    rows = torch.cat([y, y.new_zeros(1, y.shape[1])])[torch.where(slot >= 0, slot, torch.full_like(slot, plan.rows))]
+    keep = (slot >= 0).view(n, k, 1)
+    wide = torch.promote_types(y.dtype, torch.float32)
+    return torch.where(keep, rows.view(n, k, -1).to(wide) * w[..., None].to(wide), torch.zeros((), dtype=wide)).sum(
+        1).to(y.dtype)
+
+
+def sandwich_norm(x, y, gate=None, post_w=None, w=None, shift=None, scale=None, res_scale=1.0, eps=EPS):
+    """x_new = x + res_scale gate rmsnorm(y) post_w; h = rmsnorm(x_new) w (1 + scale) + shift (see ops/fused.py)."""
+    wide = torch.promote_types(x.dtype, torch.float32)
+    norm = lambda a: a * torch.rsqrt(a.square().mean(-1, keepdim=True) + eps)
+    u = y.to(wide)
+    if post_w is not None:
+        u = norm(u) * post_w
+    if gate is not None:
+        u = u * gate.to(wide)[:, None]
+    x_new = x.to(wide) + res_scale * u
+    if w is None:
+        return x_new.to(x.dtype), None
+    h = norm(x_new) * w
+    if scale is not None:
+        h = h * (1 + scale.to(wide)[:, None]) + shift.to(wide)[:, None]
+    return x_new.to(x.dtype), h.to(x.dtype)
+
+
+def axes_frequencies(axes, theta=10000.0):
+    """Angle per position of every rotated pair (fp64 [sum(axes) / 2]) and its position axis: axis a turns the pairs
+    m < axes[a] / 2 by theta_a^(-2 m / axes[a])."""
+    thetas = [theta] * len(axes) if isinstance(theta, (int, float)) else list(theta)
+    freq = torch.cat([float(th) ** (-torch.arange(0, d, 2, dtype=torch.float64) / d) for d, th in zip(axes, thetas)])
+    return freq, torch.cat([torch.full((d // 2,), a, dtype=torch.int32) for a, d in enumerate(axes)])
+
+
+def rope_axes(q, k, pos, axes, theta=10000.0, q_w=None, k_w=None, interleaved=True, eps=EPS):
+    """q [B, T, Hq, d], k [B, T, Hkv, d], pos [B, T, len(axes)] -> rotated (and normalised) q, k (see ops/fused.py)."""
+    freq, axis = axes_frequencies(axes, theta)
+    wide = torch.promote_types(q.dtype, torch.float32)
+    ang = (pos.double()[..., axis.long()] * freq.to(pos.device))[:, :, None]
+    cos, sin = ang.cos().to(wide), ang.sin().to(wide)
+    half = freq.numel()
+
+    def turn(x, w):
+        x = x.to(wide)
+        if w is not None:
+            x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * w
+        rot, rest = x[..., :2 * half], x[..., 2 * half:]
+        if interleaved:
+            rot = torch.stack((rot[..., 0::2] * cos - rot[..., 1::2] * sin,
+                               rot[..., 1::2] * cos + rot[..., 0::2] * sin), dim=-1).flatten(-2)
+        else:
+            a, b = rot[..., :half], rot[..., half:]
+            rot = torch.cat((a * cos - b * sin, b * cos + a * sin), dim=-1)
+        return torch.cat((rot, rest), dim=-1)
+    return turn(q, q_w).to(q.dtype), turn(k, k_w).to(k.dtype)

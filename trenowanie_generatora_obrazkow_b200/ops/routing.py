@@ -1,0 +1,144 @@
+"""Routing of tokens to experts and the way of their rows there and back (csrc/route.cu, csrc/dispatch.cu).
+
+    w, idx = route_experts(logits, k, score="sigmoid", bias=bias, groups=8, top_groups=4)
+    plan   = expert_plan(idx, experts)                    # or capacity=C: static [experts * C] rows, overflow dropped
+    xs     = expert_dispatch(x, plan)                     # [rows, D], experts' rows contiguous
+    y      = ... the experts' products (ops/gemm.py: gemm_grouped(xs, w, plan.offsets), or a batched gemm) ...
+    out    = expert_combine(y, w, plan)                   # [N, D]
+
+Differentiable in the logits, x, y and w; nothing here synchronises with the host. CUDA tensors run the sm_100a
+kernels, CPU tensors the fp32 definitions of ``reference.py`` under ordinary autograd.
+"""
+from typing import NamedTuple
+
+import torch
+
+from . import reference as R
+from ._ext import ext
+
+MAX_EXPERTS, MAX_CHOICES, MAX_GROUPS = 512, 32, 32
+
+
+class ExpertPlan(NamedTuple):
+    """Rows of the assignments in expert order: slot int32 [N, k] (-1: no row), offsets int32 [E + 1] (expert e owns rows
+    offsets[e]..offsets[e + 1]), counts int32 [E] (assignments per expert, dropped ones included), capacity (0: packed)
+    and the number of rows (N k packed, E capacity otherwise)."""
+    slot: torch.Tensor
+    offsets: torch.Tensor
+    counts: torch.Tensor
+    capacity: int
+    rows: int
+
+
+class _RouteFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale):
+        w, idx = ext().route_fwd(logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale)
+        ctx.mark_non_differentiable(idx)
+        ctx.save_for_backward(logits, w, idx)
+        ctx.how = (sigmoid, renorm, scale)
+        return w, idx
+
+    @staticmethod
+    def backward(ctx, dw, _):
+        logits, w, idx = ctx.saved_tensors
+        return (ext().route_bwd(logits, w, idx, dw.contiguous(), *ctx.how),) + (None,) * 8
+
+
+def route_experts(logits, k, score="softmax", bias=None, groups=1, top_groups=1, renorm=True, scale=1.0, valid=None):
+    """Choose k experts for every token: logits [N, E] (fp32, bf16 or fp16) -> (w fp32 [N, k], idx int32 [N, k]).
+
+    Scores are softmax(logits) or sigmoid(logits). The choice goes by the logits (softmax) or the scores (sigmoid), plus
+    ``bias`` [E] fp32 (for balance: it moves the choice, not the weights), in descending order, ties to the lowest
+    index. groups > 1: only the ``top_groups`` best of the ``groups`` equal runs of experts take part, a group's worth
+    being its best expert (softmax) or the sum of its two best (sigmoid). renorm divides the weights by their sum
+    (+ 1e-20); ``scale`` multiplies them. valid [N] bool: False rows get w 0 and idx -1. The gradient reaches the logits
+    through the weights."""
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"route_experts: score is 'softmax' or 'sigmoid', not {score!r}")
+    if logits.dim() != 2:
+        raise ValueError("route_experts: logits [N, E] expected")
+    E = logits.shape[1]
+    if not (1 <= E <= MAX_EXPERTS and 1 <= groups <= MAX_GROUPS and E % groups == 0 and 1 <= top_groups <= groups
+            and 1 <= k <= min(MAX_CHOICES, top_groups * (E // groups))):
+        raise ValueError(f"route_experts: {E} experts, groups={groups}, top_groups={top_groups}, k={k} (at most "
+                         f"{MAX_EXPERTS} experts in equal groups, k at most {MAX_CHOICES} and the kept groups' experts)")
+    if not logits.is_cuda:
+        return R.route_experts(logits, k, score, bias, groups, top_groups, renorm, scale, valid)
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    args = (logits, bias, valid, k, score == "sigmoid", groups, top_groups, renorm, float(scale))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _RouteFn.apply(*args)
+    return ext().route_fwd(*args)
+
+
+def expert_plan(idx, experts, capacity=None):
+    """Rows of the assignments idx int [N, k] (< 0: none) in expert order, token order within an expert. capacity: every
+    expert owns that many rows and later assignments are dropped (their slot is -1); None: packed without gaps."""
+    if idx.dim() != 2 or not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError(f"expert_plan: idx [N, k] and 1 to {MAX_EXPERTS} experts")
+    if capacity is not None and capacity < 1:
+        raise ValueError("expert_plan: capacity of at least 1 row")
+    cap = int(capacity or 0)
+    idx = idx.detach()
+    if not idx.is_cuda:
+        slot, offsets, counts = R.expert_plan(idx, experts, cap)
+    else:
+        slot, offsets, counts = ext().expert_plan(idx.to(torch.int32).contiguous(), experts, cap)
+    return ExpertPlan(slot, offsets, counts, cap, experts * cap if cap else idx.numel())
+
+
+class _DispatchFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, plan):
+        ctx.save_for_backward(plan.slot, plan.offsets, plan.counts)
+        ctx.capacity = plan.capacity
+        return ext().expert_dispatch(x, plan.slot, plan.offsets, plan.counts, plan.capacity, plan.rows)
+
+    @staticmethod
+    def backward(ctx, dxs):
+        return ext().expert_combine(dxs.contiguous(), None, *ctx.saved_tensors, ctx.capacity), None
+
+
+def expert_dispatch(x, plan):
+    """x [N, D] -> [plan.rows, D]: the row of every assignment's token at its slot, zeros in unused rows."""
+    if x.dim() != 2 or x.shape[0] != plan.slot.shape[0]:
+        raise ValueError(f"expert_dispatch: x [{plan.slot.shape[0]}, D] expected, got {tuple(x.shape)}")
+    if not x.is_cuda:
+        return R.expert_dispatch(x, plan)
+    if x.stride(1) != 1:
+        x = x.contiguous()
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _DispatchFn.apply(x, plan)
+    return ext().expert_dispatch(x, plan.slot, plan.offsets, plan.counts, plan.capacity, plan.rows)
+
+
+class _CombineFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, w, plan):
+        ctx.save_for_backward(y, w, plan.slot, plan.offsets, plan.counts)
+        ctx.capacity = plan.capacity
+        return ext().expert_combine(y, w, plan.slot, plan.offsets, plan.counts, plan.capacity)
+
+    @staticmethod
+    def backward(ctx, dout):
+        y, w, *rows = ctx.saved_tensors
+        if dout.stride(1) != 1:
+            dout = dout.contiguous()
+        dy, dw = ext().expert_combine_bwd(y, w, dout, *rows, ctx.capacity)
+        return dy, dw, None
+
+
+def expert_combine(y, w, plan):
+    """y [plan.rows, D], w fp32 [N, k] -> [N, D]: the weighted sum of every token's rows (fp32 sum, one rounding);
+    dropped assignments add nothing."""
+    if y.dim() != 2 or y.shape[0] != plan.rows or w.shape != plan.slot.shape:
+        raise ValueError(f"expert_combine: y [{plan.rows}, D] and w {tuple(plan.slot.shape)} expected, got "
+                         f"{tuple(y.shape)} and {tuple(w.shape)}")
+    if not y.is_cuda:
+        return R.expert_combine(y, w, plan)
+    y, w = y.contiguous(), w.float().contiguous()
+    if torch.is_grad_enabled() and (y.requires_grad or w.requires_grad):
+        return _CombineFn.apply(y, w, plan)
+    return ext().expert_combine(y, w, plan.slot, plan.offsets, plan.counts, plan.capacity)
