@@ -385,7 +385,7 @@ std::tuple<at::Tensor, at::Tensor> rope_axes_bwd(at::Tensor dq, at::Tensor dk, a
               "rope_axes_bwd: dq_w and dk_w both or neither, with the norm weights");
   if (p.M == 0) return {dqi, dki};
   if (gq != nullptr)
-    partial = at::empty({rope_axes_bwd_ctas(p), 2, p.hd}, q.options().dtype(at::kFloat));
+    partial = at::empty({rope_axes_bwd_ctas(), 2, p.hd}, q.options().dtype(at::kFloat));
   BLOCK_LAUNCH(rope_axes_bwd_launch(p, dq.data_ptr(), dk.data_ptr(), dqi.data_ptr(), dki.data_ptr(),
                                     gq != nullptr ? partial.data_ptr<float>() : nullptr, gq, gk,
                                     elem_of(q, "rope_axes_bwd"), at::cuda::getCurrentCUDAStream()),

@@ -109,8 +109,8 @@ struct RopeAxesParams {
 };
 cudaError_t rope_axes_fwd_launch(const RopeAxesParams& p, int elem, cudaStream_t s);
 // dq / dk [M, h, hd] contiguous -> dq_in / dk_in [M, h, hd] contiguous; dq_w / dk_w [hd] accumulated through partials
-// [rope_axes_bwd_ctas()][2][hd]
-int rope_axes_bwd_ctas(const RopeAxesParams& p);
+// [rope_axes_bwd_ctas()][2][hd] (the most CTAs of any launch)
+int rope_axes_bwd_ctas();
 cudaError_t rope_axes_bwd_launch(const RopeAxesParams& p, const void* dq, const void* dk, void* dq_in, void* dk_in,
                                  float* partial, float* dq_w, float* dk_w, int elem, cudaStream_t s);
 

@@ -8,9 +8,8 @@
 // Backward: the transposed rotation, then the norm's gradient with x and its rstd recomputed from q / k:
 //     n = x r, gn = w g:   dx = r (gn - n mean(gn n)),   dw = sum over tokens and heads of g n.
 //
-// Bound by memory: one warp per token, LPH lanes of 8 channels per head; the angles and norm weights of a token are
-// set up once in registers and used for all of its q and k heads.
 #include <algorithm>
+#include <initializer_list>
 
 #include "block_ops.h"
 #include "common.cuh"
@@ -47,6 +46,229 @@ __device__ __forceinline__ void turn_of(const RopeAxesParams& p, long long tok, 
 
 }  // namespace
 
+// ------------------------------------------------------------------------------------------------------------------
+// Vector form: head dims of whole 16-byte vectors up to 256 channels. LPH lanes of 8 channels per head (the next power of
+// two: a head dim of 96 leaves 4 of 16 lanes idle), 32 / LPH heads per pass, UNROLL passes' loads issued together.
+// A rotation is out[c] = x[c] A[c] + x[partner(c)] B[c] with A = w cos, B = -+ w sin of the channel's pair: 16 registers
+// that a token sets up once for its q heads and once for its k heads. The pairs' cos / sin are computed once per warp
+// (rot / 2 of them over 32 lanes) and shared through shared memory. The partner is the neighbour in the lane
+// (interleaved) or the same element of the lane rot / 16 further (half-split, rot % 16 == 0): its raw words are shuffled.
+// ------------------------------------------------------------------------------------------------------------------
+namespace {
+
+constexpr int ROPE_UNROLL = 4;
+constexpr int ROPE_MAX_VEC_HD = 256;
+
+// this lane's cos and signed sin: out[c] = x[c] cs[c] + x[partner] sn[c]
+template <bool INTER>
+__device__ __forceinline__ void lane_turns(const RopeAxesParams& p, long long tok, float2* sh, int e0, float (&cs)[8],
+                                           float (&sn)[8]) {
+  const int half = p.rot / 2;
+  __syncwarp();
+  for (int i = lane_id(); i < half; i += 32) {
+    float c, s;
+    turn_of(p, tok, i, c, s);
+    sh[i] = make_float2(c, s);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int c = e0 + j;
+    float2 t = make_float2(1.f, 0.f);
+    if (c < p.rot) {
+      t = sh[INTER ? c >> 1 : (c < half ? c : c - half)];
+      if (INTER ? (j & 1) == 0 : c < half) t.y = -t.y;
+    }
+    cs[j] = t.x;
+    sn[j] = t.y;
+  }
+}
+
+template <typename T, bool INTER>
+__device__ __forceinline__ void partner_of(const Raw<T, 8>& own, int src_lane, float (&f)[8]) {
+  if constexpr (INTER) {
+    float o[8];
+    own.get(o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = o[j ^ 1];
+  } else {
+    Raw<T, 8> r;
+    const uint32_t* a = reinterpret_cast<const uint32_t*>(own.u);
+    uint32_t* b = reinterpret_cast<uint32_t*>(r.u);
+#pragma unroll
+    for (int i = 0; i < 4 * Raw<T, 8>::W; ++i) b[i] = __shfl_sync(0xffffffffu, a[i], src_lane);
+    r.get(f);
+  }
+}
+
+// lane (of the warp) that holds the partner channels of this lane's 8 channels, half-split form
+__device__ __forceinline__ int partner_lane(const RopeAxesParams& p, int lane, int e0) {
+  const int step = p.rot / 16;
+  if (e0 < p.rot / 2) return lane + step;
+  return e0 < p.rot ? lane - step : lane;
+}
+
+}  // namespace
+
+template <typename T, int LPH, bool INTER>
+__global__ void __launch_bounds__(ROPE_WARPS * 32) rope_axes_kernel(RopeAxesParams p) {
+  constexpr int HPP = 32 / LPH, U = ROPE_UNROLL;
+  __shared__ float2 turns[ROPE_WARPS][ROPE_MAX_VEC_HD / 2];
+  const int lane = lane_id(), sub = lane / LPH, e0 = (lane % LPH) * 8;
+  const bool on = e0 < p.hd;
+  const int src = INTER ? lane : partner_lane(p, lane, e0);
+  const int ep = (src % LPH) * 8;  // first partner channel (half-split)
+  const bool norm = p.q_w != nullptr;
+  const float inv_hd = 1.f / p.hd;
+  for (long long tok = (long long)blockIdx.x * ROPE_WARPS + warp_id(); tok < p.M; tok += (long long)gridDim.x * ROPE_WARPS) {
+    float cs[8], sn[8];
+    lane_turns<INTER>(p, tok, turns[warp_id()], e0, cs, sn);
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {  // q heads, then k heads
+      const int heads = which == 0 ? p.hq : p.hkv;
+      const T* in = which == 0 ? reinterpret_cast<const T*>(p.q) + tok * p.q_ts
+                               : reinterpret_cast<const T*>(p.k) + tok * p.k_ts;
+      T* out = (which == 0 ? reinterpret_cast<T*>(p.q_out) : reinterpret_cast<T*>(p.k_out)) + tok * heads * p.hd;
+      const float* w = which == 0 ? p.q_w : p.k_w;
+      float A[8], B[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        A[j] = cs[j];
+        B[j] = sn[j];
+        if (norm && on) {
+          A[j] *= w[e0 + j];
+          B[j] *= w[INTER ? e0 + (j ^ 1) : ep + j];
+        }
+      }
+#pragma unroll 1
+      for (int h0 = sub; h0 - sub < heads; h0 += U * HPP) {
+        Raw<T, 8> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * HPP;
+          if (on && h < heads) x[u].load(in + h * p.hd + e0);
+          else x[u].zero();
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * HPP;
+          if (h - sub >= heads) break;  // warp-uniform
+          float f[8], g[8];
+          x[u].get(f);
+          partner_of<T, INTER>(x[u], src, g);
+          float r = 1.f;
+          if (norm) {
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
+            r = rsqrtf(head_sum<LPH>(ss) * inv_hd + p.eps);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = r * fmaf(f[j], A[j], g[j] * B[j]);
+          if (on && h < heads) store_vec<T, 8>(out + h * p.hd + e0, f);
+        }
+      }
+    }
+  }
+}
+
+// Backward, same layout. dw partials stay in registers over the whole grid-stride loop (a lane's channels are the same
+// for every head and token).
+template <typename T, int LPH, bool INTER>
+__global__ void __launch_bounds__(ROPE_WARPS * 32, 2) rope_axes_bwd_kernel(RopeAxesParams p, const T* __restrict__ dq,
+                                                                        const T* __restrict__ dk,
+                                                                        T* __restrict__ dq_in, T* __restrict__ dk_in,
+                                                                        float* __restrict__ partial) {
+  constexpr int HPP = 32 / LPH, U = sizeof(T) == 4 ? 2 : ROPE_UNROLL;
+  __shared__ float2 turns[ROPE_WARPS][ROPE_MAX_VEC_HD / 2];
+  __shared__ float dw[ROPE_WARPS][2][LPH * 8];
+  const int lane = lane_id(), sub = lane / LPH, e0 = (lane % LPH) * 8;
+  const bool on = e0 < p.hd;
+  const int src = INTER ? lane : partner_lane(p, lane, e0);
+  const bool norm = p.q_w != nullptr;
+  const float inv_hd = 1.f / p.hd;
+  float acc[2][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[0][j] = acc[1][j] = 0.f;
+  for (long long tok = (long long)blockIdx.x * ROPE_WARPS + warp_id(); tok < p.M; tok += (long long)gridDim.x * ROPE_WARPS) {
+    float cs[8], sn[8];
+    lane_turns<INTER>(p, tok, turns[warp_id()], e0, cs, sn);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const int heads = which == 0 ? p.hq : p.hkv;
+      const T* in = which == 0 ? reinterpret_cast<const T*>(p.q) + tok * p.q_ts
+                               : reinterpret_cast<const T*>(p.k) + tok * p.k_ts;
+      const T* grad = (which == 0 ? dq : dk) + tok * heads * p.hd;
+      T* out = (which == 0 ? dq_in : dk_in) + tok * heads * p.hd;
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = norm && on ? (which == 0 ? p.q_w : p.k_w)[e0 + j] : 0.f;
+#pragma unroll 1
+      for (int h0 = sub; h0 - sub < heads; h0 += U * HPP) {
+        Raw<T, 8> g[U], x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * HPP;
+          const bool ok = on && h < heads;
+          if (ok) g[u].load(grad + h * p.hd + e0);
+          else g[u].zero();
+          if (ok && norm) x[u].load(in + h * p.hd + e0);
+          else x[u].zero();
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * HPP;
+          if (h - sub >= heads) break;
+          float gf[8], gp[8];
+          g[u].get(gf);
+          partner_of<T, INTER>(g[u], src, gp);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) gf[j] = fmaf(gf[j], cs[j], -gp[j] * sn[j]);
+          if (norm) {
+            float xf[8], ss = 0.f, dot = 0.f;
+            x[u].get(xf);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              ss = fmaf(xf[j], xf[j], ss);
+              dot = fmaf(gf[j] * w[j], xf[j], dot);
+            }
+            ss = head_sum<LPH>(ss);
+            dot = head_sum<LPH>(dot);
+            const float r = rsqrtf(ss * inv_hd + p.eps);
+            const float m = dot * r * r * inv_hd;  // n mean(gn n) = x r (r dot / hd)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              acc[which][j] = fmaf(gf[j] * xf[j], r, acc[which][j]);
+              gf[j] = r * fmaf(gf[j], w[j], -xf[j] * m);
+            }
+          }
+          if (on && h < heads) store_vec<T, 8>(out + h * p.hd + e0, gf);
+        }
+      }
+    }
+  }
+  if (partial == nullptr) return;
+  // sums over the warp's heads groups, then over the warps, in a fixed order
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v = acc[which][j];
+#pragma unroll
+      for (int o = 16; o >= LPH; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (sub == 0) dw[warp_id()][which][e0 + j] = v;
+    }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * p.hd; c += blockDim.x) {
+    const int which = c >= p.hd, e = c - which * p.hd;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < ROPE_WARPS; ++i) s += dw[i][which][e];
+    partial[(long long)blockIdx.x * 2 * p.hd + c] = s;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
 // Any head dim, stride and alignment: one warp per (token, head), channels strided over the lanes.
 template <typename T>
 __global__ void __launch_bounds__(ROPE_WARPS * 32) rope_axes_any_kernel(RopeAxesParams p) {
@@ -183,16 +405,66 @@ __global__ void rope_weights_kernel(const float* __restrict__ partial, int ctas,
 
 namespace {
 
-int rope_grid(const RopeAxesParams& p) {
-  const long long units = (long long)p.M * (p.hq + p.hkv);
+// The vector form needs whole 16-byte vectors at 16-byte addresses, and in the half-split form partners at the same
+// element of another lane.
+bool rope_vectors(const RopeAxesParams& p, int elem, std::initializer_list<const void*> more = {}) {
+  const int per = elem == ELEM_F32 ? 4 : 8;  // elements of a 16-byte word
+  if (p.hd % 8 != 0 || p.hd > ROPE_MAX_VEC_HD || p.q_ts % per != 0 || p.k_ts % per != 0) return false;
+  if (!p.interleaved && p.rot % 16 != 0) return false;
+  uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) |
+                   reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_out);
+  for (const void* m : more) bits |= reinterpret_cast<uintptr_t>(m);
+  return (bits & 15) == 0;
+}
+
+// CTAs of the grid-stride kernels: a warp per token (vector form) or per token and head, at most 8 blocks per SM
+int rope_grid(const RopeAxesParams& p, bool vectors) {
+  const long long units = vectors ? p.M : (long long)p.M * (p.hq + p.hkv);
   return (int)std::min<long long>((units + ROPE_WARPS - 1) / ROPE_WARPS, (long long)num_sms() * 8);
+}
+
+template <typename T, int LPH>
+void rope_fwd_vec(const RopeAxesParams& p, cudaStream_t s) {
+  const long long grid = ((long long)p.M + ROPE_WARPS - 1) / ROPE_WARPS;
+  if (p.interleaved) rope_axes_kernel<T, LPH, true><<<(unsigned)grid, ROPE_WARPS * 32, 0, s>>>(p);
+  else rope_axes_kernel<T, LPH, false><<<(unsigned)grid, ROPE_WARPS * 32, 0, s>>>(p);
+}
+template <typename T, int LPH>
+void rope_bwd_vec(const RopeAxesParams& p, const T* dq, const T* dk, T* dqi, T* dki, float* partial, int grid,
+                  cudaStream_t s) {
+  if (p.interleaved)
+    rope_axes_bwd_kernel<T, LPH, true><<<grid, ROPE_WARPS * 32, 0, s>>>(p, dq, dk, dqi, dki, partial);
+  else
+    rope_axes_bwd_kernel<T, LPH, false><<<grid, ROPE_WARPS * 32, 0, s>>>(p, dq, dk, dqi, dki, partial);
+}
+
+template <typename T>
+cudaError_t rope_fwd_run(const RopeAxesParams& p, int elem, cudaStream_t s) {
+  if (!rope_vectors(p, elem)) rope_axes_any_kernel<T><<<rope_grid(p, false), ROPE_WARPS * 32, 0, s>>>(p);
+  else if (p.hd <= 32) rope_fwd_vec<T, 4>(p, s);
+  else if (p.hd <= 64) rope_fwd_vec<T, 8>(p, s);
+  else if (p.hd <= 128) rope_fwd_vec<T, 16>(p, s);
+  else rope_fwd_vec<T, 32>(p, s);
+  return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t rope_bwd_run(const RopeAxesParams& p, const void* dq, const void* dk, void* dq_in, void* dk_in,
-                         float* partial, cudaStream_t s) {
-  rope_axes_bwd_any_kernel<T><<<rope_grid(p), ROPE_WARPS * 32, sizeof(float) * ROPE_WARPS * 2 * p.hd, s>>>(
-      p, static_cast<const T*>(dq), static_cast<const T*>(dk), static_cast<T*>(dq_in), static_cast<T*>(dk_in), partial);
+                         float* partial, float* dq_w, float* dk_w, int elem, cudaStream_t s) {
+  const T *gq = static_cast<const T*>(dq), *gk = static_cast<const T*>(dk);
+  T *iq = static_cast<T*>(dq_in), *ik = static_cast<T*>(dk_in);
+  const bool vec = rope_vectors(p, elem, {dq, dk, dq_in, dk_in});
+  const int grid = rope_grid(p, vec);
+  if (!vec)
+    rope_axes_bwd_any_kernel<T><<<grid, ROPE_WARPS * 32, sizeof(float) * ROPE_WARPS * 2 * p.hd, s>>>(p, gq, gk, iq, ik,
+                                                                                                   partial);
+  else if (p.hd <= 32) rope_bwd_vec<T, 4>(p, gq, gk, iq, ik, partial, grid, s);
+  else if (p.hd <= 64) rope_bwd_vec<T, 8>(p, gq, gk, iq, ik, partial, grid, s);
+  else if (p.hd <= 128) rope_bwd_vec<T, 16>(p, gq, gk, iq, ik, partial, grid, s);
+  else rope_bwd_vec<T, 32>(p, gq, gk, iq, ik, partial, grid, s);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || partial == nullptr) return e;
+  rope_weights_kernel<<<(2 * p.hd + 31) / 32, dim3(32, 8), 0, s>>>(partial, grid, p.hd, dq_w, dk_w);
   return cudaGetLastError();
 }
 
@@ -200,31 +472,25 @@ cudaError_t rope_bwd_run(const RopeAxesParams& p, const void* dq, const void* dk
 
 cudaError_t rope_axes_fwd_launch(const RopeAxesParams& p, int elem, cudaStream_t s) {
   if (p.M <= 0) return cudaSuccess;
-  const int grid = rope_grid(p);
   switch (elem) {
-    case ELEM_BF16: rope_axes_any_kernel<__nv_bfloat16><<<grid, ROPE_WARPS * 32, 0, s>>>(p); break;
-    case ELEM_F16: rope_axes_any_kernel<__half><<<grid, ROPE_WARPS * 32, 0, s>>>(p); break;
-    case ELEM_F32: rope_axes_any_kernel<float><<<grid, ROPE_WARPS * 32, 0, s>>>(p); break;
-    default: return cudaErrorInvalidValue;
+    case ELEM_BF16: return rope_fwd_run<__nv_bfloat16>(p, elem, s);
+    case ELEM_F16: return rope_fwd_run<__half>(p, elem, s);
+    case ELEM_F32: return rope_fwd_run<float>(p, elem, s);
   }
-  return cudaGetLastError();
+  return cudaErrorInvalidValue;
 }
 
-int rope_axes_bwd_ctas(const RopeAxesParams& p) { return rope_grid(p); }
+int rope_axes_bwd_ctas() { return num_sms() * 8; }
 
 cudaError_t rope_axes_bwd_launch(const RopeAxesParams& p, const void* dq, const void* dk, void* dq_in, void* dk_in,
                                  float* partial, float* dq_w, float* dk_w, int elem, cudaStream_t s) {
   if (p.M <= 0) return cudaSuccess;
-  cudaError_t e;
   switch (elem) {
-    case ELEM_BF16: e = rope_bwd_run<__nv_bfloat16>(p, dq, dk, dq_in, dk_in, partial, s); break;
-    case ELEM_F16: e = rope_bwd_run<__half>(p, dq, dk, dq_in, dk_in, partial, s); break;
-    case ELEM_F32: e = rope_bwd_run<float>(p, dq, dk, dq_in, dk_in, partial, s); break;
-    default: return cudaErrorInvalidValue;
+    case ELEM_BF16: return rope_bwd_run<__nv_bfloat16>(p, dq, dk, dq_in, dk_in, partial, dq_w, dk_w, elem, s);
+    case ELEM_F16: return rope_bwd_run<__half>(p, dq, dk, dq_in, dk_in, partial, dq_w, dk_w, elem, s);
+    case ELEM_F32: return rope_bwd_run<float>(p, dq, dk, dq_in, dk_in, partial, dq_w, dk_w, elem, s);
   }
-  if (e != cudaSuccess || partial == nullptr) return e;
-  rope_weights_kernel<<<(2 * p.hd + 31) / 32, dim3(32, 8), 0, s>>>(partial, rope_grid(p), p.hd, dq_w, dk_w);
-  return cudaGetLastError();
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace tgo
