@@ -338,8 +338,14 @@ def test_sandwich_norm_noncontiguous_and_repeatable():
     b = Fz.sandwich_norm(**{**ins, "x": wide[..., :512], "shift": ins["shift"].contiguous()})
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     off = torch.empty(2 * 64 * 512 + 1, device="cuda", dtype=BF16)[1:].view(2, 64, 512).copy_(ins["x"])  # 2-byte aligned
-    c = Fz.sandwich_norm(**{**ins, "x": off})
-    check(c[1], a[1].double(), 4 * a[1].double().abs(), "misaligned")
+    c = Fz.sandwich_norm(**{**ins, "x": off})  # another kernel: held to the 64-bit values by the rule above
+    d = {n: t.double() for n, t in ins.items()}
+    xn64, h64 = R.sandwich_norm(**d)
+    yn = d["y"].abs() * (d["y"].square().mean(-1, keepdim=True) + 1e-6) ** -0.5
+    mag = d["x"].abs() + d["gate"].abs()[:, None] * d["post_w"].abs() * yn
+    n = mag * (xn64.square().mean(-1, keepdim=True) + 1e-6) ** -0.5
+    check(c[0], xn64, mag, "misaligned x_new")
+    check(c[1], h64, n * d["w"].abs() * (1 + d["scale"].abs()[:, None]) + d["shift"].abs()[:, None], "misaligned h")
     grads = []
     for _ in range(2):
         leaf = {n: t.detach().requires_grad_() for n, t in ins.items()}

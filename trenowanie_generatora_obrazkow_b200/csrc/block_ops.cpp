@@ -48,6 +48,12 @@ float* acc_f32(const OptT& t, int64_t n, const at::Tensor& as, const char* what)
   return const_cast<float*>(vec_f32(t, n, as, what));
 }
 
+int* err_word(const at::Tensor& err, const at::Tensor& as) {
+  same_device(err, as, "err");
+  TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() >= 1, "err: int32 error word");
+  return err.data_ptr<int>();
+}
+
 // ---------------------------------------------------------------------------------------------------------- routing
 RouteParams route_params(const at::Tensor& logits, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups,
                          bool renorm, double scale) {
@@ -240,7 +246,7 @@ SandwichParams sandwich_params(const at::Tensor& x, const at::Tensor& y, const O
 }
 
 std::vector<at::Tensor> sandwich_fwd(at::Tensor x, at::Tensor y, OptT gate, OptT post_w, OptT w, OptT shift, OptT scale,
-                                     double res_scale, double eps) {
+                                     double res_scale, double eps, at::Tensor err) {
   SandwichParams p = sandwich_params(x, y, gate, post_w, w, shift, scale, res_scale, eps);
   const c10::cuda::CUDAGuard guard(x.device());
   at::Tensor x_new = at::empty_like(x), h, ry, rx;
@@ -256,14 +262,15 @@ std::vector<at::Tensor> sandwich_fwd(at::Tensor x, at::Tensor y, OptT gate, OptT
     p.h = h.data_ptr();
     p.rstd_x = rx.data_ptr<float>();
   }
-  BLOCK_LAUNCH(sandwich_fwd_launch(p, elem_of(x, "sandwich_norm"), at::cuda::getCurrentCUDAStream()), p.M > 0);
+  BLOCK_LAUNCH(sandwich_fwd_launch(p, elem_of(x, "sandwich_norm"), err_word(err, x),
+                                   at::cuda::getCurrentCUDAStream()), p.M > 0);
   return {x_new, h, ry, rx};
 }
 
 // -> dx, dy, dgate, dshift, dscale; dpost_w and dw are accumulated (+=)
 std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Tensor y, OptT gate, OptT post_w, OptT w,
                                      OptT shift, OptT scale, OptT ry, OptT rx, OptT dpost_w, OptT dw, double res_scale,
-                                     double eps) {
+                                     double eps, at::Tensor err) {
   SandwichParams p = sandwich_params(x, y, gate, post_w, w, shift, scale, res_scale, eps);
   const c10::cuda::CUDAGuard guard(x.device());
   p.rstd_y = acc_f32(ry, p.M, x, "sandwich_bwd: ry");
@@ -307,7 +314,7 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
   at::Tensor scratch = at::empty({floats}, x.options().dtype(at::kFloat));
   q.partial = scratch.data_ptr<float>();
   q.wpart = q.partial + entries * 3 * D;
-  BLOCK_LAUNCH(sandwich_bwd_launch(p, q, elem, at::cuda::getCurrentCUDAStream()), 3);
+  BLOCK_LAUNCH(sandwich_bwd_launch(p, q, elem, err_word(err, x), at::cuda::getCurrentCUDAStream()), 3);
   return {dx, dy, dgate, dshift, dscale};
 }
 

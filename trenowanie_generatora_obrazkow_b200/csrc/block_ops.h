@@ -84,11 +84,12 @@ struct SandwichBwdParams {
   void* dscale;
   float* dpost_w;        // [D], accumulated
   float* dw;             // [D], accumulated
-  int ctas, rows_per_cta, groups;
+  int ctas, rows_per_cta, groups;  // units of rows (see sandwich.cu), groups of samples of the reduction
 };
-cudaError_t sandwich_fwd_launch(const SandwichParams& p, int elem, cudaStream_t s);
-void sandwich_bwd_plan(const SandwichParams& p, int elem, SandwichBwdParams* q);  // ctas, rows_per_cta, groups
-cudaError_t sandwich_bwd_launch(const SandwichParams& p, const SandwichBwdParams& q, int elem, cudaStream_t s);
+// err: device error word of the kernels' bounded waits
+cudaError_t sandwich_fwd_launch(const SandwichParams& p, int elem, int* err, cudaStream_t s);
+void sandwich_bwd_plan(const SandwichParams& p, int elem, SandwichBwdParams* q);  // sets ctas, rows_per_cta, groups
+cudaError_t sandwich_bwd_launch(const SandwichParams& p, const SandwichBwdParams& q, int elem, int* err, cudaStream_t s);
 
 // ---------------------------------------------------------------- rotary positions with several axes (rope_axes.cu)
 constexpr int kRopeMaxAxes = 4;

@@ -57,7 +57,15 @@ __device__ __forceinline__ void turn_of(const RopeAxesParams& p, long long tok, 
 namespace {
 
 constexpr int ROPE_UNROLL = 4;
+
 constexpr int ROPE_MAX_VEC_HD = 256;
+
+// Table of a warp's token in shared memory: (cos, sin) of pair i at [i], and the identity from rot / 2 on, where the
+// lanes of the channels past rot (and idle lanes) look: written once, no token touches it.
+template <int SIZE>
+__device__ __forceinline__ void identity_turns(const RopeAxesParams& p, float2 (&sh)[SIZE]) {
+  for (int i = p.rot / 2 + lane_id(); i < SIZE; i += 32) sh[i] = make_float2(1.f, 0.f);
+}
 
 // this lane's cos and signed sin: out[c] = x[c] cs[c] + x[partner] sn[c]
 template <bool INTER>
@@ -71,16 +79,25 @@ __device__ __forceinline__ void lane_turns(const RopeAxesParams& p, long long to
     sh[i] = make_float2(c, s);
   }
   __syncwarp();
+  const int at = INTER ? e0 / 2 : (e0 < half ? e0 : e0 - half);
+  const float4* t = reinterpret_cast<const float4*>(sh + at);
+  if constexpr (INTER) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int c = e0 + j;
-    float2 t = make_float2(1.f, 0.f);
-    if (c < p.rot) {
-      t = sh[INTER ? c >> 1 : (c < half ? c : c - half)];
-      if (INTER ? (j & 1) == 0 : c < half) t.y = -t.y;
+    for (int j = 0; j < 2; ++j) {
+      const float4 v = t[j];
+      cs[4 * j] = cs[4 * j + 1] = v.x;
+      cs[4 * j + 2] = cs[4 * j + 3] = v.z;
+      sn[4 * j] = -v.y, sn[4 * j + 1] = v.y;
+      sn[4 * j + 2] = -v.w, sn[4 * j + 3] = v.w;
     }
-    cs[j] = t.x;
-    sn[j] = t.y;
+  } else {
+    const float sign = e0 < half ? -1.f : 1.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 v = t[j];
+      cs[2 * j] = v.x, cs[2 * j + 1] = v.z;
+      sn[2 * j] = sign * v.y, sn[2 * j + 1] = sign * v.w;
+    }
   }
 }
 
@@ -111,15 +128,16 @@ __device__ __forceinline__ int partner_lane(const RopeAxesParams& p, int lane, i
 }  // namespace
 
 template <typename T, int LPH, bool INTER>
-__global__ void __launch_bounds__(ROPE_WARPS * 32) rope_axes_kernel(RopeAxesParams p) {
+__global__ void __launch_bounds__(ROPE_WARPS * 32, 3) rope_axes_kernel(RopeAxesParams p) {
   constexpr int HPP = 32 / LPH, U = ROPE_UNROLL;
-  __shared__ float2 turns[ROPE_WARPS][ROPE_MAX_VEC_HD / 2];
+  __shared__ __align__(16) float2 turns[ROPE_WARPS][INTER ? LPH * 4 : LPH * 8];
   const int lane = lane_id(), sub = lane / LPH, e0 = (lane % LPH) * 8;
   const bool on = e0 < p.hd;
   const int src = INTER ? lane : partner_lane(p, lane, e0);
   const int ep = (src % LPH) * 8;  // first partner channel (half-split)
   const bool norm = p.q_w != nullptr;
   const float inv_hd = 1.f / p.hd;
+  identity_turns(p, turns[warp_id()]);
   for (long long tok = (long long)blockIdx.x * ROPE_WARPS + warp_id(); tok < p.M; tok += (long long)gridDim.x * ROPE_WARPS) {
     float cs[8], sn[8];
     lane_turns<INTER>(p, tok, turns[warp_id()], e0, cs, sn);
@@ -132,13 +150,13 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) rope_axes_kernel(RopeAxesPara
       const float* w = which == 0 ? p.q_w : p.k_w;
       float A[8], B[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        A[j] = cs[j];
-        B[j] = sn[j];
-        if (norm && on) {
-          A[j] *= w[e0 + j];
-          B[j] *= w[INTER ? e0 + (j ^ 1) : ep + j];
-        }
+      for (int j = 0; j < 8; ++j) A[j] = cs[j], B[j] = sn[j];
+      if (norm && on) {
+        float a[8], b[8];
+        load_vec<float, 8>(w + e0, a);
+        load_vec<float, 8>(w + (INTER ? e0 : ep), b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) A[j] *= a[j], B[j] *= b[INTER ? j ^ 1 : j];
       }
 #pragma unroll 1
       for (int h0 = sub; h0 - sub < heads; h0 += U * HPP) {
@@ -180,7 +198,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 2) rope_axes_bwd_kernel(RopeA
                                                                         T* __restrict__ dq_in, T* __restrict__ dk_in,
                                                                         float* __restrict__ partial) {
   constexpr int HPP = 32 / LPH, U = sizeof(T) == 4 ? 2 : ROPE_UNROLL;
-  __shared__ float2 turns[ROPE_WARPS][ROPE_MAX_VEC_HD / 2];
+  __shared__ __align__(16) float2 turns[ROPE_WARPS][INTER ? LPH * 4 : LPH * 8];
   __shared__ float dw[ROPE_WARPS][2][LPH * 8];
   const int lane = lane_id(), sub = lane / LPH, e0 = (lane % LPH) * 8;
   const bool on = e0 < p.hd;
@@ -190,6 +208,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 2) rope_axes_bwd_kernel(RopeA
   float acc[2][8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[0][j] = acc[1][j] = 0.f;
+  identity_turns(p, turns[warp_id()]);
   for (long long tok = (long long)blockIdx.x * ROPE_WARPS + warp_id(); tok < p.M; tok += (long long)gridDim.x * ROPE_WARPS) {
     float cs[8], sn[8];
     lane_turns<INTER>(p, tok, turns[warp_id()], e0, cs, sn);
@@ -200,9 +219,8 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 2) rope_axes_bwd_kernel(RopeA
                                : reinterpret_cast<const T*>(p.k) + tok * p.k_ts;
       const T* grad = (which == 0 ? dq : dk) + tok * heads * p.hd;
       T* out = (which == 0 ? dq_in : dk_in) + tok * heads * p.hd;
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = norm && on ? (which == 0 ? p.q_w : p.k_w)[e0 + j] : 0.f;
+      float w[8] = {};
+      if (norm && on) load_vec<float, 8>((which == 0 ? p.q_w : p.k_w) + e0, w);
 #pragma unroll 1
       for (int h0 = sub; h0 - sub < heads; h0 += U * HPP) {
         Raw<T, 8> g[U], x[U];
@@ -412,7 +430,8 @@ bool rope_vectors(const RopeAxesParams& p, int elem, std::initializer_list<const
   if (p.hd % 8 != 0 || p.hd > ROPE_MAX_VEC_HD || p.q_ts % per != 0 || p.k_ts % per != 0) return false;
   if (!p.interleaved && p.rot % 16 != 0) return false;
   uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) |
-                   reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_out);
+                   reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_out) |
+                   reinterpret_cast<uintptr_t>(p.q_w) | reinterpret_cast<uintptr_t>(p.k_w);
   for (const void* m : more) bits |= reinterpret_cast<uintptr_t>(m);
   return (bits & 15) == 0;
 }

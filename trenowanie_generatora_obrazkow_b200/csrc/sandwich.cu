@@ -12,9 +12,9 @@
 //     mean(a g yn) = mean(a yn (dx' + rx dh cw)) - rx m mean(a yn n),    m = mean(dh cw n).
 // Statistics and sums are fp32; x' is rounded only when it is stored, so h comes from the unrounded sum.
 //
-// Column sums: a CTA owns a contiguous span of rows and writes one partial row (three sums per channel) per sample it
-// meets. Entry cta + sample is unique (along the spans both only grow), so ctas + samples entries hold them all; two
-// small kernels add them in a fixed order.
+// Column sums: a unit (a CTA, or a group of its threads) owns a contiguous span of rows and writes one partial row (three
+// sums per channel) per sample it meets. Entry unit + sample is unique (along the spans both only grow), so
+// units + samples entries hold them all; two small kernels add them in a fixed order.
 #include <algorithm>
 
 #include "block_ops.h"
@@ -165,6 +165,363 @@ __global__ void __launch_bounds__(SW_THREADS) sandwich_bwd_any_kernel(SandwichPa
   }
 }
 
+// ------------------------------------------------------------------------------------------------------------------
+// Vector form: rows of whole 16-byte vectors, up to 4096 channels.
+//
+// A group of tpg = D / 8 threads (rounded up to warps) owns 8 channels per thread and walks a contiguous span of rows, R
+// rows per step; a block holds several groups when rows are short. Rows arrive through untiled bulk copies into a ring of
+// SW_STAGES steps: one thread issues them, so the loads of the next steps stay in flight across the block barriers of the
+// row reductions, without registers. Modulation, gate and weights of the group's sample stay in registers, and so do the
+// backward's column sums.
+// ------------------------------------------------------------------------------------------------------------------
+namespace {
+
+constexpr int SW_STAGES = 3;
+constexpr int SW_MAX_VEC_D = 4096;
+
+struct SwGeom {
+  int tpg, groups;      // threads per group, groups per block
+  int span;             // rows per group
+  int steps;            // of every group (R rows each)
+};
+
+// ring slot of (stage, tensor, group): [SW_STAGES][tensors][groups][R][D]
+template <typename T, int R, int TENSORS>
+struct SwRing {
+  uint64_t* full;
+  uint8_t* base;
+  long long step_bytes, tensor_bytes, group_bytes;  // strides
+  __device__ __forceinline__ SwRing(uint8_t* smem, const SwGeom& g, int D) {
+    full = reinterpret_cast<uint64_t*>(smem);
+    base = smem + 128;
+    group_bytes = (long long)R * D * sizeof(T);
+    tensor_bytes = group_bytes * g.groups;
+    step_bytes = tensor_bytes * TENSORS;
+  }
+  __device__ __forceinline__ const T* row(int stage, int tensor, int group, int r, int D) const {
+    return reinterpret_cast<const T*>(base + stage * step_bytes + tensor * tensor_bytes + group * group_bytes) +
+           (long long)r * D;
+  }
+};
+
+__device__ __forceinline__ int span_rows(int M, long long row0, int span, int done, int R) {
+  const long long left = min((long long)M, row0 + span) - (row0 + done);
+  return (int)max(0ll, min((long long)R, left));
+}
+
+// one thread: the rows of step i of every group of this block, all tensors
+template <typename T, int R, int TENSORS>
+__device__ __forceinline__ void sw_load(const SwRing<T, R, TENSORS>& ring, const SwGeom& g, int M, int D, int i,
+                                        const void* const (&src)[TENSORS]) {
+  const int stage = i % SW_STAGES;
+  uint32_t bytes = 0;
+  for (int k = 0; k < g.groups; ++k) {
+    const long long row0 = ((long long)blockIdx.x * g.groups + k) * g.span;
+    bytes += (uint32_t)(span_rows(M, row0, g.span, i * R, R) * D * sizeof(T));
+  }
+  uint32_t present = 0;
+#pragma unroll
+  for (int t = 0; t < TENSORS; ++t) present += src[t] != nullptr;
+  mbar_expect_tx(&ring.full[stage], bytes * present);
+  for (int k = 0; k < g.groups; ++k) {
+    const long long row0 = ((long long)blockIdx.x * g.groups + k) * g.span;
+    const int n = span_rows(M, row0, g.span, i * R, R);
+    if (n <= 0) continue;
+#pragma unroll
+    for (int t = 0; t < TENSORS; ++t)
+      if (src[t] != nullptr)
+        bulk_load(const_cast<T*>(ring.row(stage, t, k, 0, D)),
+                  reinterpret_cast<const T*>(src[t]) + (row0 + (long long)i * R) * D, (uint32_t)(n * D * sizeof(T)),
+                  &ring.full[stage]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_row8(const void* base, long long off, float (&f)[8]) {
+  load_vec<T, 8>(reinterpret_cast<const T*>(base) + off, f);
+}
+
+// K per-row values of R rows summed over a group. red: [R * K][warps of the block]; the caller's barrier sits between the
+// two halves.
+template <int N>
+__device__ __forceinline__ void group_put(const float (&v)[N], float* red, int warps) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float t = warp_total(v[i]);
+    if (lane_id() == 0) red[i * warps + warp_id()] = t;
+  }
+}
+template <int N>
+__device__ __forceinline__ void group_get(float (&v)[N], const float* red, int warps, int first, int count) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float s = 0.f;
+    for (int w = first; w < first + count; ++w) s += red[i * warps + w];
+    v[i] = s;
+  }
+}
+
+}  // namespace
+
+template <typename T, int R>
+__global__ void __launch_bounds__(512) sandwich_fwd_kernel(SandwichParams p, SwGeom g, int* err) {
+  extern __shared__ __align__(128) uint8_t sw_smem[];
+  __shared__ float red[2][R * 16];
+  const int group = threadIdx.x / g.tpg, c0 = (threadIdx.x % g.tpg) * 8;
+  const bool on = c0 < p.D;
+  const int warps = blockDim.x >> 5, wpg = g.tpg >> 5, w0 = group * wpg;
+  const long long row0 = ((long long)blockIdx.x * g.groups + group) * g.span;
+  const bool per_sample = samples_of(p) > 1;
+  const SwRing<T, R, 2> ring(sw_smem, g, p.D);
+  const void* const src[2] = {p.x, p.y};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SW_STAGES; ++s) mbar_init(&ring.full[s], 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    for (int i = 0; i < SW_STAGES && i < g.steps; ++i) sw_load<T, R, 2>(ring, g, p.M, p.D, i, src);
+  }
+  __syncthreads();
+  float a[8], cw[8], sh[8];
+  int cur = -1;
+  auto sample = [&](int b) {  // constants of sample b: a = res_scale gate post_w, cw = w (1 + scale), shift
+    if (b == cur || !on) return;
+    cur = b;
+    float t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = p.res_scale, cw[j] = 0.f, sh[j] = 0.f;
+    if (p.post_w != nullptr) {
+      load_vec<float, 8>(p.post_w + c0, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] *= t[j];
+    }
+    if (p.gate != nullptr) {
+      load_row8<T>(p.gate, b * p.gate_bs + c0, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] *= t[j];
+    }
+    if (p.w != nullptr) load_vec<float, 8>(p.w + c0, cw);
+    if (p.scale != nullptr) {
+      load_row8<T>(p.scale, b * p.mod_bs + c0, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cw[j] = fmaf(cw[j], t[j], cw[j]);
+      load_row8<T>(p.shift, b * p.mod_bs + c0, sh);
+    }
+  };
+  for (int i = 0; i < g.steps; ++i) {
+    const int stage = i % SW_STAGES;
+    const int n = span_rows(p.M, row0, g.span, i * R, R);
+    const long long row = row0 + (long long)i * R;
+    mbar_wait(&ring.full[stage], (i / SW_STAGES) & 1, err, ERR_MBAR_TIMEOUT_PRODUCER);
+    Raw<T, 8> x[R], y[R];
+    float s[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[r] = 0.f;
+      if (on && r < n) {
+        x[r].load(ring.row(stage, 0, group, r, p.D) + c0);
+        y[r].load(ring.row(stage, 1, group, r, p.D) + c0);
+        if (p.post_w != nullptr) {
+          float f[8];
+          y[r].get(f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[r] = fmaf(f[j], f[j], s[r]);
+        }
+      } else {
+        x[r].zero();
+        y[r].zero();
+      }
+    }
+    group_put<R>(s, red[0], warps);
+    __syncthreads();  // every thread has taken its rows out of the stage: refill it
+    if (threadIdx.x == 0 && i + SW_STAGES < g.steps) sw_load<T, R, 2>(ring, g, p.M, p.D, i + SW_STAGES, src);
+    float xn[R][8];
+    float ry[R];
+    if (p.post_w != nullptr) {
+      group_get<R>(ry, red[0], warps, w0, wpg);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        ry[r] = rsqrtf(ry[r] / p.D + p.eps);
+        if (c0 == 0 && r < n) p.rstd_y[row + r] = ry[r];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[r] = 0.f;
+      if (r >= n) continue;
+      sample(per_sample ? (int)((row + r) / p.T) : 0);
+      if (!on) continue;
+      float f[8];
+      x[r].get(xn[r]);
+      y[r].get(f);
+      const float q = p.post_w != nullptr ? ry[r] : 1.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        xn[r][j] = fmaf(f[j] * q, a[j], xn[r][j]);
+        s[r] = fmaf(xn[r][j], xn[r][j], s[r]);
+      }
+      store_vec<T, 8>(reinterpret_cast<T*>(p.x_new) + (row + r) * p.D + c0, xn[r]);
+    }
+    if (p.w != nullptr) {
+      group_put<R>(s, red[1], warps);
+      __syncthreads();
+      float rx[R];
+      group_get<R>(rx, red[1], warps, w0, wpg);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r >= n) continue;
+        rx[r] = rsqrtf(rx[r] / p.D + p.eps);
+        if (c0 == 0) p.rstd_x[row + r] = rx[r];
+        sample(per_sample ? (int)((row + r) / p.T) : 0);
+        if (!on) continue;
+        float h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = fmaf(xn[r][j] * rx[r], cw[j], sh[j]);
+        store_vec<T, 8>(reinterpret_cast<T*>(p.h) + (row + r) * p.D + c0, h);
+      }
+    } else {
+      __syncthreads();  // red[0] is written again
+    }
+  }
+}
+
+template <typename T, int R>
+__global__ void __launch_bounds__(512) sandwich_bwd_kernel(SandwichParams p, SandwichBwdParams q, SwGeom g, int* err) {
+  extern __shared__ __align__(128) uint8_t sw_smem[];
+  __shared__ float red[2][3 * R * 16];
+  const int group = threadIdx.x / g.tpg, c0 = (threadIdx.x % g.tpg) * 8;
+  const bool on = c0 < p.D;
+  const int warps = blockDim.x >> 5, wpg = g.tpg >> 5, w0 = group * wpg;
+  const int unit = blockIdx.x * g.groups + group;
+  const long long row0 = (long long)unit * g.span;
+  const bool per_sample = samples_of(p) > 1;
+  const SwRing<T, R, 4> ring(sw_smem, g, p.D);
+  const void* const src[4] = {p.x, p.y, q.dh, q.dx_new};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SW_STAGES; ++s) mbar_init(&ring.full[s], 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    for (int i = 0; i < SW_STAGES && i < g.steps; ++i) sw_load<T, R, 4>(ring, g, p.M, p.D, i, src);
+  }
+  __syncthreads();
+  float a[8], cw[8], acc[3][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[0][j] = acc[1][j] = acc[2][j] = 0.f;
+  int cur = -1, acc_b = -1;
+  auto sample = [&](int b) {
+    if (b == cur || !on) return;
+    cur = b;
+    float t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = p.res_scale, cw[j] = 0.f;
+    if (p.post_w != nullptr) {
+      load_vec<float, 8>(p.post_w + c0, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] *= t[j];
+    }
+    if (p.gate != nullptr) {
+      load_row8<T>(p.gate, b * p.gate_bs + c0, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] *= t[j];
+    }
+    if (p.w != nullptr) load_vec<float, 8>(p.w + c0, cw);
+    if (p.scale != nullptr) {
+      load_row8<T>(p.scale, b * p.mod_bs + c0, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cw[j] = fmaf(cw[j], t[j], cw[j]);
+    }
+  };
+  auto flush = [&]() {  // the column sums of sample acc_b
+    if (acc_b >= 0 && on) {
+      float* dst = q.partial + (long long)(unit + acc_b) * 3 * p.D + c0;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        store_vec<float, 8>(dst + (long long)i * p.D, acc[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+      }
+    }
+  };
+  for (int i = 0; i < g.steps; ++i) {
+    const int stage = i % SW_STAGES;
+    const int n = span_rows(p.M, row0, g.span, i * R, R);
+    const long long row = row0 + (long long)i * R;
+    float ry[R], rx[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      ry[r] = p.post_w != nullptr && r < n ? p.rstd_y[row + r] : 1.f;
+      rx[r] = p.w != nullptr && r < n ? p.rstd_x[row + r] : 0.f;
+    }
+    mbar_wait(&ring.full[stage], (i / SW_STAGES) & 1, err, ERR_MBAR_TIMEOUT_PRODUCER);
+    Raw<T, 8> x[R], y[R], dh[R], e[R];
+    float s[3 * R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[3 * r] = s[3 * r + 1] = s[3 * r + 2] = 0.f;
+      dh[r].zero();
+      e[r].zero();
+      if (r >= n || !on) {
+        x[r].zero();
+        y[r].zero();
+        continue;
+      }
+      sample(per_sample ? (int)((row + r) / p.T) : 0);
+      x[r].load(ring.row(stage, 0, group, r, p.D) + c0);
+      y[r].load(ring.row(stage, 1, group, r, p.D) + c0);
+      if (q.dh != nullptr) dh[r].load(ring.row(stage, 2, group, r, p.D) + c0);
+      if (q.dx_new != nullptr) e[r].load(ring.row(stage, 3, group, r, p.D) + c0);
+      float xf[8], yf[8], gf[8], ef[8];
+      x[r].get(xf);
+      y[r].get(yf);
+      dh[r].get(gf);
+      e[r].get(ef);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float ay = a[j] * (yf[j] * ry[r]);
+        const float nn = (xf[j] + ay) * rx[r];
+        const float c = gf[j] * cw[j];
+        s[3 * r] = fmaf(c, nn, s[3 * r]);
+        s[3 * r + 1] = fmaf(ay, fmaf(rx[r], c, ef[j]), s[3 * r + 1]);
+        s[3 * r + 2] = fmaf(ay, nn, s[3 * r + 2]);
+      }
+    }
+    group_put<3 * R>(s, red[i & 1], warps);
+    __syncthreads();
+    if (threadIdx.x == 0 && i + SW_STAGES < g.steps) sw_load<T, R, 4>(ring, g, p.M, p.D, i + SW_STAGES, src);
+    group_get<3 * R>(s, red[i & 1], warps, w0, wpg);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r >= n || !on) continue;
+      const int b = per_sample ? (int)((row + r) / p.T) : 0;
+      if (b != acc_b) {
+        flush();
+        acc_b = b;
+      }
+      sample(b);
+      const float m = s[3 * r] / p.D;
+      const float m2 = p.post_w != nullptr ? (s[3 * r + 1] - rx[r] * m * s[3 * r + 2]) / p.D : 0.f;
+      float xf[8], yf[8], gf[8], ef[8];
+      x[r].get(xf);
+      y[r].get(yf);
+      dh[r].get(gf);
+      e[r].get(ef);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float yn = yf[j] * ry[r];
+        const float nn = fmaf(a[j], yn, xf[j]) * rx[r];
+        const float gx = fmaf(rx[r], fmaf(gf[j], cw[j], -nn * m), ef[j]);
+        acc[0][j] += gf[j];
+        acc[1][j] = fmaf(gf[j], nn, acc[1][j]);
+        acc[2][j] = fmaf(gx, yn, acc[2][j]);
+        xf[j] = gx;
+        yf[j] = ry[r] * fmaf(a[j], gx, -yn * m2);
+      }
+      store_vec<T, 8>(reinterpret_cast<T*>(q.dx) + (row + r) * p.D + c0, xf);
+      store_vec<T, 8>(reinterpret_cast<T*>(q.dy) + (row + r) * p.D + c0, yf);
+    }
+  }
+  flush();
+}
+
 // Sums of a sample's partial rows -> its dshift / dscale / dgate rows, and the weights' sums over this block's samples.
 constexpr int RED_ROWS = 8;
 template <typename T>
@@ -232,23 +589,87 @@ __global__ void sandwich_weights_kernel(SandwichParams p, SandwichBwdParams q) {
 
 namespace {
 
+// rows of the vector form per step and group: two 16-bit rows or one fp32 row
 template <typename T>
-cudaError_t fwd_run(const SandwichParams& p, cudaStream_t s) {
-  sandwich_fwd_any_kernel<T><<<std::min(p.M, num_sms() * 8), SW_THREADS, 0, s>>>(p);
+struct SwRows {
+  static constexpr int R = sizeof(T) == 2 ? 2 : 1;
+};
+int sw_rows(int elem) { return elem == ELEM_F32 ? SwRows<float>::R : SwRows<__half>::R; }
+
+bool sw_vectors(const SandwichParams& p, const SandwichBwdParams* q) {
+  if (p.D % 8 != 0 || p.D > SW_MAX_VEC_D || p.gate_bs % 8 != 0 || p.mod_bs % 8 != 0) return false;
+  uintptr_t bits = 0;
+  for (const void* t : {p.x, p.y, p.gate, p.shift, p.scale, (const void*)p.post_w, (const void*)p.w,
+                        (const void*)p.x_new, (const void*)p.h})
+    bits |= reinterpret_cast<uintptr_t>(t);
+  if (q != nullptr)
+    for (const void* t : {q->dx_new, q->dh, (const void*)q->dx, (const void*)q->dy}) bits |= reinterpret_cast<uintptr_t>(t);
+  return (bits & 15) == 0;
+}
+
+// groups of a block: about 256 threads; spans that fill every SM with the blocks that its shared memory holds (at most 2)
+int sw_smem(const SandwichParams& p, const SwGeom& g, int R, int tensors, int es) {
+  return 128 + SW_STAGES * tensors * g.groups * R * p.D * es;
+}
+SwGeom sw_geom(const SandwichParams& p, int R, int tensors, int es) {
+  SwGeom g;
+  g.tpg = (p.D / 8 + 31) / 32 * 32;
+  g.groups = std::max(1, 256 / g.tpg);
+  const int fit = 226 * 1024 / (sw_smem(p, g, R, tensors, es) + 2048);
+  const int units = num_sms() * std::max(1, std::min(fit, 2)) * g.groups;
+  g.span = (p.M + units - 1) / units;
+  g.span = (g.span + R - 1) / R * R;
+  g.steps = g.span / R;
+  return g;
+}
+int sw_blocks(const SandwichParams& p, const SwGeom& g) {
+  const int units = (p.M + g.span - 1) / g.span;
+  return (units + g.groups - 1) / g.groups;
+}
+
+template <typename K>
+cudaError_t sw_smem_limit(K kernel, int smem, int* allowed) {
+  if (smem <= *allowed) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) *allowed = smem;
+  return e;
+}
+
+template <typename T>
+cudaError_t fwd_run(const SandwichParams& p, int* err, cudaStream_t s) {
+  constexpr int R = SwRows<T>::R;
+  if (sw_vectors(p, nullptr)) {
+    const SwGeom g = sw_geom(p, R, 2, sizeof(T));
+    const int smem = sw_smem(p, g, R, 2, sizeof(T));
+    static int allowed = 46 * 1024;
+    cudaError_t e = sw_smem_limit(sandwich_fwd_kernel<T, R>, smem, &allowed);
+    if (e != cudaSuccess) return e;
+    sandwich_fwd_kernel<T, R><<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, g, err);
+  } else {
+    sandwich_fwd_any_kernel<T><<<std::min(p.M, num_sms() * 8), SW_THREADS, 0, s>>>(p);
+  }
   return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t bwd_run(const SandwichParams& p, const SandwichBwdParams& q, cudaStream_t s) {
-  const int smem = 3 * p.D * (int)sizeof(float);
-  static int allowed = 47 * 1024;  // beside the static shared memory
-  if (smem > allowed) {
-    cudaError_t e = cudaFuncSetAttribute(sandwich_bwd_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+cudaError_t bwd_run(const SandwichParams& p, const SandwichBwdParams& q, int* err, cudaStream_t s) {
+  cudaError_t e;
+  if (sw_vectors(p, &q)) {
+    constexpr int R = SwRows<T>::R;
+    const SwGeom g = sw_geom(p, R, 4, sizeof(T));
+    const int smem = sw_smem(p, g, R, 4, sizeof(T));
+    static int allowed = 46 * 1024;
+    e = sw_smem_limit(sandwich_bwd_kernel<T, R>, smem, &allowed);
     if (e != cudaSuccess) return e;
-    allowed = smem;
+    sandwich_bwd_kernel<T, R><<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, q, g, err);
+  } else {
+    const int smem = 3 * p.D * (int)sizeof(float);
+    static int allowed = 46 * 1024;
+    e = sw_smem_limit(sandwich_bwd_any_kernel<T>, smem, &allowed);
+    if (e != cudaSuccess) return e;
+    sandwich_bwd_any_kernel<T><<<q.ctas, SW_THREADS, smem, s>>>(p, q);
   }
-  sandwich_bwd_any_kernel<T><<<q.ctas, SW_THREADS, smem, s>>>(p, q);
-  cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   sandwich_reduce_kernel<T><<<dim3((p.D + 31) / 32, q.groups), dim3(32, RED_ROWS), 0, s>>>(p, q);
   e = cudaGetLastError();
@@ -260,29 +681,35 @@ cudaError_t bwd_run(const SandwichParams& p, const SandwichBwdParams& q, cudaStr
 
 }  // namespace
 
-cudaError_t sandwich_fwd_launch(const SandwichParams& p, int elem, cudaStream_t s) {
+cudaError_t sandwich_fwd_launch(const SandwichParams& p, int elem, int* err, cudaStream_t s) {
   if (p.M <= 0 || p.D <= 0) return cudaSuccess;
   switch (elem) {
-    case ELEM_BF16: return fwd_run<__nv_bfloat16>(p, s);
-    case ELEM_F16: return fwd_run<__half>(p, s);
-    case ELEM_F32: return fwd_run<float>(p, s);
+    case ELEM_BF16: return fwd_run<__nv_bfloat16>(p, err, s);
+    case ELEM_F16: return fwd_run<__half>(p, err, s);
+    case ELEM_F32: return fwd_run<float>(p, err, s);
   }
   return cudaErrorInvalidValue;
 }
 
 void sandwich_bwd_plan(const SandwichParams& p, int elem, SandwichBwdParams* q) {
-  const int most = num_sms() * 4;
-  q->rows_per_cta = std::max(1, (p.M + most - 1) / most);
+  if (sw_vectors(p, q)) {
+    const SwGeom g = sw_geom(p, sw_rows(elem), 4, elem == ELEM_F32 ? 4 : 2);
+    q->rows_per_cta = g.span;
+  } else {
+    const int most = num_sms() * 4;
+    q->rows_per_cta = std::max(1, (p.M + most - 1) / most);
+  }
   q->ctas = (p.M + q->rows_per_cta - 1) / q->rows_per_cta;
   q->groups = std::min(samples_of(p), 64);
 }
 
-cudaError_t sandwich_bwd_launch(const SandwichParams& p, const SandwichBwdParams& q, int elem, cudaStream_t s) {
+cudaError_t sandwich_bwd_launch(const SandwichParams& p, const SandwichBwdParams& q, int elem, int* err,
+                                cudaStream_t s) {
   if (p.M <= 0 || p.D <= 0) return cudaSuccess;
   switch (elem) {
-    case ELEM_BF16: return bwd_run<__nv_bfloat16>(p, q, s);
-    case ELEM_F16: return bwd_run<__half>(p, q, s);
-    case ELEM_F32: return bwd_run<float>(p, q, s);
+    case ELEM_BF16: return bwd_run<__nv_bfloat16>(p, q, err, s);
+    case ELEM_F16: return bwd_run<__half>(p, q, err, s);
+    case ELEM_F32: return bwd_run<float>(p, q, err, s);
   }
   return cudaErrorInvalidValue;
 }

@@ -342,7 +342,7 @@ def adanorm(x, y, gate, w, shift=None, scale=None, eps=R.EPS):
 class _SandwichFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, post_w, w, shift, scale, res_scale, eps):
-        x_new, h, ry, rx = ext().sandwich_fwd(x, y, gate, post_w, w, shift, scale, res_scale, eps)
+        x_new, h, ry, rx = ext().sandwich_fwd(x, y, gate, post_w, w, shift, scale, res_scale, eps, err_buf(x.device))
         ctx.save_for_backward(x, y, gate, post_w, w, shift, scale, ry, rx)
         ctx.how = (res_scale, eps)
         ctx.params = (post_w, w)
@@ -357,7 +357,7 @@ class _SandwichFn(torch.autograd.Function):
         dw, w_direct = _weight_grad_target(wp) if wp is not None and wp.requires_grad else (None, False)
         dx, dy, dgate, dshift, dscale = ext().sandwich_bwd(
             None if dx_new is None else dx_new.contiguous(), None if dh is None else dh.contiguous(), x, y, gate,
-            post_w, w, shift, scale, ry, rx, dpost, dw, *ctx.how)
+            post_w, w, shift, scale, ry, rx, dpost, dw, *ctx.how, err_buf(x.device))
         return (dx, dy, dgate, None if dpost is None else _weight_grad_done(pp, p_direct, dpost),
                 None if dw is None else _weight_grad_done(wp, w_direct, dw), dshift, dscale, None, None)
 
@@ -381,12 +381,12 @@ def sandwich_norm(x, y, gate=None, post_w=None, w=None, shift=None, scale=None, 
         shift, scale = shift.contiguous(), scale.contiguous()
     args = (x, y, gate, post_w, w, shift, scale, float(res_scale), float(eps))
     if not torch.is_grad_enabled():
-        x_new, h = ext().sandwich_fwd(*args)[:2]
+        x_new, h = ext().sandwich_fwd(*args, err_buf(x.device))[:2]
         return x_new, h
     x_new, h = _SandwichFn.apply(*args)
     if _SAC_ACTIVE[0] and h is not None:  # h is rebuilt from the tensors that the backward keeps anyway
         again = tuple(a.detach() if isinstance(a, torch.Tensor) else a for a in args)
-        _tag(h, _Recipe(lambda: (ext().sandwich_fwd(*again)[1],)))
+        _tag(h, _Recipe(lambda: (ext().sandwich_fwd(*again, err_buf(again[0].device))[1],)))
     return x_new, h
 
 
