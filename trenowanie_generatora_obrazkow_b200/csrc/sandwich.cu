@@ -176,7 +176,10 @@ __global__ void __launch_bounds__(SW_THREADS) sandwich_bwd_any_kernel(SandwichPa
 // ------------------------------------------------------------------------------------------------------------------
 namespace {
 
-constexpr int SW_STAGES = 3;
+#ifndef STAGES
+#define STAGES 3
+#endif
+constexpr int SW_STAGES = STAGES;
 constexpr int SW_MAX_VEC_D = 4096;
 
 struct SwGeom {
@@ -237,43 +240,114 @@ __device__ __forceinline__ void sw_load(const SwRing<T, R, TENSORS>& ring, const
 }
 
 template <typename T>
-__device__ __forceinline__ void load_row8(const void* base, long long off, float (&f)[8]) {
-  load_vec<T, 8>(reinterpret_cast<const T*>(base) + off, f);
+__device__ __forceinline__ void load_row8(const void* base, long long off, f32x2 (&v)[4]) {
+  Raw<T, 8> r;
+  r.load(reinterpret_cast<const T*>(base) + off);
+  unpack_x2<T>(r, v);
+}
+__device__ __forceinline__ void load_w8(const float* p, f32x2 (&v)[4]) {
+  Raw<float, 8> r;
+  r.load(p);
+  unpack_x2<float>(r, v);
 }
 
-// K per-row values of R rows summed over a group. red: [R * K][warps of the block]; the caller's barrier sits between the
-// two halves.
+// N sums over a group's warps. Step 1 (group_put): the lanes' values are summed over the warp while their number is
+// halved (a lane pair exchanges the halves that the other keeps), so N values cost about N + 5 shuffles instead of 5 N;
+// one lane per value writes it to red[value][group's slot of this warp]. Step 2 (group_get), after the caller's barrier:
+// every thread adds the group's slots (padded with zeros to float4s).
+constexpr int RED_PITCH = 32;
 template <int N>
-__device__ __forceinline__ void group_put(const float (&v)[N], float* red, int warps) {
+__device__ __forceinline__ void group_put(float (&v)[N], float* red, int slot) {
+  static_assert(N == 1 || N == 2 || N == 4 || N == 8, "a power of two");
+  int keep = 0, bit = 16;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float t = warp_total(v[i]);
-    if (lane_id() == 0) red[i * warps + warp_id()] = t;
+  for (int h = N / 2; h >= 1; h >>= 1) {
+    const bool up = lane_id() & bit;
+#pragma unroll
+    for (int i = 0; i < h; ++i) {
+      const float give = up ? v[i] : v[i + h], mine = up ? v[i + h] : v[i];
+      v[i] = mine + __shfl_xor_sync(0xffffffffu, give, bit);
+    }
+    keep += up ? h : 0;
+    bit >>= 1;
   }
+  float t = v[0];
+#pragma unroll
+  for (int o = 16 / N; o >= 1; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if ((lane_id() & (32 / N - 1)) == 0) red[keep * RED_PITCH + slot] = t;
 }
 template <int N>
-__device__ __forceinline__ void group_get(float (&v)[N], const float* red, int warps, int first, int count) {
+__device__ __forceinline__ void group_get(float (&v)[N], const float* red, int first, int quads) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    float s = 0.f;
-    for (int w = first; w < first + count; ++w) s += red[i * warps + w];
-    v[i] = s;
+    const float4* q = reinterpret_cast<const float4*>(red + i * RED_PITCH + first);
+    float4 t = q[0];
+    for (int k = 1; k < quads; ++k) {
+      const float4 u = q[k];
+      t.x += u.x, t.y += u.y, t.z += u.z, t.w += u.w;
+    }
+    v[i] = (t.x + t.y) + (t.z + t.w);
+  }
+}
+
+// Position of a unit in its samples, advanced step by step (no division in the row loop). R divides T, so a step never
+// straddles two samples.
+struct SwSample {
+  int b, t, T;
+  __device__ __forceinline__ SwSample(const SandwichParams& p, bool per_sample, long long row) {
+    T = per_sample ? p.T : 0x7fffffff;
+    b = per_sample ? (int)(row / p.T) : 0;
+    t = per_sample ? (int)(row - (long long)b * p.T) : 0;
+  }
+  __device__ __forceinline__ bool next(int rows) {  // true: a new sample begins
+    t += rows;
+    if (t < T) return false;
+    t = 0;
+    ++b;
+    return true;
+  }
+};
+
+// a = res_scale gate post_w and cw = w (1 + scale) of sample b, channels c0 .. c0 + 7
+template <typename T>
+__device__ __forceinline__ void sw_constants(const SandwichParams& p, int b, int c0, f32x2 (&a)[4], f32x2 (&cw)[4]) {
+  f32x2 t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) a[j] = x2(p.res_scale), cw[j] = x2(0.f);
+  if (p.post_w != nullptr) {
+    load_w8(p.post_w + c0, t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = x2_mul(a[j], t[j]);
+  }
+  if (p.gate != nullptr) {
+    load_row8<T>(p.gate, b * p.gate_bs + c0, t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = x2_mul(a[j], t[j]);
+  }
+  if (p.w != nullptr) load_w8(p.w + c0, cw);
+  if (p.scale != nullptr) {
+    load_row8<T>(p.scale, b * p.mod_bs + c0, t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) cw[j] = x2_fma(cw[j], t[j], cw[j]);
   }
 }
 
 }  // namespace
 
-template <typename T, int R>
-__global__ void __launch_bounds__(512) sandwich_fwd_kernel(SandwichParams p, SwGeom g, int* err) {
+// Threads past the last channel of a row (D / 8 not a multiple of 32) work on channel 0's values and keep their sums at 0.
+template <typename T, int R, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) sandwich_fwd_kernel(SandwichParams p, SwGeom g, int* err) {
   extern __shared__ __align__(128) uint8_t sw_smem[];
-  __shared__ float red[2][R * 16];
-  const int group = threadIdx.x / g.tpg, c0 = (threadIdx.x % g.tpg) * 8;
-  const bool on = c0 < p.D;
-  const int warps = blockDim.x >> 5, wpg = g.tpg >> 5, w0 = group * wpg;
+  __shared__ __align__(16) float red[2][R * RED_PITCH];
+  const int group = threadIdx.x / g.tpg, tc = (threadIdx.x % g.tpg) * 8;
+  const bool on = tc < p.D, lead = tc == 0;
+  const int c0 = on ? tc : 0;
+  const int wpg = g.tpg >> 5, quads = (wpg + 3) >> 2, first = group * quads * 4, slot = first + warp_id() - group * wpg;
   const long long row0 = ((long long)blockIdx.x * g.groups + group) * g.span;
-  const bool per_sample = samples_of(p) > 1;
+  const float inv_d = 1.f / p.D;
   const SwRing<T, R, 2> ring(sw_smem, g, p.D);
   const void* const src[2] = {p.x, p.y};
+  for (int i = threadIdx.x; i < 2 * R * RED_PITCH; i += blockDim.x) (&red[0][0])[i] = 0.f;
   if (threadIdx.x == 0) {
     for (int s = 0; s < SW_STAGES; ++s) mbar_init(&ring.full[s], 1);
     fence_barrier_init();
@@ -281,121 +355,102 @@ __global__ void __launch_bounds__(512) sandwich_fwd_kernel(SandwichParams p, SwG
     for (int i = 0; i < SW_STAGES && i < g.steps; ++i) sw_load<T, R, 2>(ring, g, p.M, p.D, i, src);
   }
   __syncthreads();
-  float a[8], cw[8], sh[8];
-  int cur = -1;
-  auto sample = [&](int b) {  // constants of sample b: a = res_scale gate post_w, cw = w (1 + scale), shift
-    if (b == cur || !on) return;
-    cur = b;
-    float t[8];
+  const int rows = (int)max(0ll, min((long long)g.span, p.M - row0));
+  SwSample at(p, samples_of(p) > 1, row0);
+  const bool post = p.post_w != nullptr, pre = p.w != nullptr;
+  f32x2 a[4], cw[4], sh[4];
+  auto sample = [&]() {
+    sw_constants<T>(p, at.b, c0, a, cw);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = p.res_scale, cw[j] = 0.f, sh[j] = 0.f;
-    if (p.post_w != nullptr) {
-      load_vec<float, 8>(p.post_w + c0, t);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] *= t[j];
-    }
-    if (p.gate != nullptr) {
-      load_row8<T>(p.gate, b * p.gate_bs + c0, t);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] *= t[j];
-    }
-    if (p.w != nullptr) load_vec<float, 8>(p.w + c0, cw);
-    if (p.scale != nullptr) {
-      load_row8<T>(p.scale, b * p.mod_bs + c0, t);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) cw[j] = fmaf(cw[j], t[j], cw[j]);
-      load_row8<T>(p.shift, b * p.mod_bs + c0, sh);
-    }
+    for (int j = 0; j < 4; ++j) sh[j] = x2(0.f);
+    if (p.scale != nullptr) load_row8<T>(p.shift, at.b * p.mod_bs + c0, sh);
   };
+  if (rows > 0) sample();
+  const T* slots = ring.row(0, 0, group, 0, p.D) + c0;
+  const int to_y = (int)(ring.tensor_bytes / sizeof(T)), to_stage = (int)(ring.step_bytes / sizeof(T));
+  T* out_x = reinterpret_cast<T*>(p.x_new) + row0 * p.D + c0;
+  T* out_h = reinterpret_cast<T*>(p.h) + row0 * p.D + c0;
+  float *st_y = p.rstd_y + row0, *st_x = p.rstd_x + row0;
+  int stage = 0, phase = 0, left = rows;  // left <= 0: only the barriers
   for (int i = 0; i < g.steps; ++i) {
-    const int stage = i % SW_STAGES;
-    const int n = span_rows(p.M, row0, g.span, i * R, R);
-    const long long row = row0 + (long long)i * R;
-    mbar_wait(&ring.full[stage], (i / SW_STAGES) & 1, err, ERR_MBAR_TIMEOUT_PRODUCER);
+    mbar_wait(&ring.full[stage], phase, err, ERR_MBAR_TIMEOUT_PRODUCER);
     Raw<T, 8> x[R], y[R];
     float s[R];
+    const T* in = slots + stage * to_stage;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      s[r] = 0.f;
-      if (on && r < n) {
-        x[r].load(ring.row(stage, 0, group, r, p.D) + c0);
-        y[r].load(ring.row(stage, 1, group, r, p.D) + c0);
-        if (p.post_w != nullptr) {
-          float f[8];
-          y[r].get(f);
+    for (int r = 0; r < R; ++r) {  // a missing last row reads what its slot held: its results go nowhere
+      x[r].load(in + r * p.D);
+      y[r].load(in + to_y + r * p.D);
+      f32x2 q = x2(0.f), f[4];
+      unpack_x2<T>(y[r], f);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) s[r] = fmaf(f[j], f[j], s[r]);
-        }
-      } else {
-        x[r].zero();
-        y[r].zero();
-      }
+      for (int j = 0; j < 4; ++j) q = x2_fma(f[j], f[j], q);
+      s[r] = on ? x2_sum(q) : 0.f;
     }
-    group_put<R>(s, red[0], warps);
+    group_put<R>(s, red[0], slot);
     __syncthreads();  // every thread has taken its rows out of the stage: refill it
     if (threadIdx.x == 0 && i + SW_STAGES < g.steps) sw_load<T, R, 2>(ring, g, p.M, p.D, i + SW_STAGES, src);
-    float xn[R][8];
-    float ry[R];
-    if (p.post_w != nullptr) {
-      group_get<R>(ry, red[0], warps, w0, wpg);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        ry[r] = rsqrtf(ry[r] / p.D + p.eps);
-        if (c0 == 0 && r < n) p.rstd_y[row + r] = ry[r];
-      }
-    }
+    if (++stage == SW_STAGES) stage = 0, phase ^= 1;
+    group_get<R>(s, red[0], first, quads);
+    f32x2 xn[R][4];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      s[r] = 0.f;
-      if (r >= n) continue;
-      sample(per_sample ? (int)((row + r) / p.T) : 0);
-      if (!on) continue;
-      float f[8];
-      x[r].get(xn[r]);
-      y[r].get(f);
-      const float q = p.post_w != nullptr ? ry[r] : 1.f;
+      const float ry = post ? rsqrtf(fmaf(s[r], inv_d, p.eps)) : 1.f;
+      if (lead && post && r < left) st_y[r] = ry;
+      f32x2 f[4], q = x2(0.f);
+      const f32x2 ry2 = x2(ry);
+      unpack_x2<T>(x[r], xn[r]);
+      unpack_x2<T>(y[r], f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        xn[r][j] = fmaf(f[j] * q, a[j], xn[r][j]);
-        s[r] = fmaf(xn[r][j], xn[r][j], s[r]);
+      for (int j = 0; j < 4; ++j) {
+        xn[r][j] = x2_fma(x2_mul(f[j], ry2), a[j], xn[r][j]);
+        q = x2_fma(xn[r][j], xn[r][j], q);
       }
-      store_vec<T, 8>(reinterpret_cast<T*>(p.x_new) + (row + r) * p.D + c0, xn[r]);
+      s[r] = on ? x2_sum(q) : 0.f;
+      if (on && r < left) store_x2<T>(out_x + r * p.D, xn[r]);
     }
-    if (p.w != nullptr) {
-      group_put<R>(s, red[1], warps);
-      __syncthreads();
-      float rx[R];
-      group_get<R>(rx, red[1], warps, w0, wpg);
+    group_put<R>(s, red[1], slot);
+    __syncthreads();
+    if (pre) {
+      group_get<R>(s, red[1], first, quads);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        if (r >= n) continue;
-        rx[r] = rsqrtf(rx[r] / p.D + p.eps);
-        if (c0 == 0) p.rstd_x[row + r] = rx[r];
-        sample(per_sample ? (int)((row + r) / p.T) : 0);
-        if (!on) continue;
-        float h[8];
+        const float rx = rsqrtf(fmaf(s[r], inv_d, p.eps));
+        const f32x2 rx2 = x2(rx);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = fmaf(xn[r][j] * rx[r], cw[j], sh[j]);
-        store_vec<T, 8>(reinterpret_cast<T*>(p.h) + (row + r) * p.D + c0, h);
+        for (int j = 0; j < 4; ++j) xn[r][j] = x2_fma(x2_mul(xn[r][j], rx2), cw[j], sh[j]);
+        if (r < left) {
+          if (lead) st_x[r] = rx;
+          if (on) store_x2<T>(out_h + r * p.D, xn[r]);
+        }
       }
-    } else {
-      __syncthreads();  // red[0] is written again
     }
+    out_x += R * p.D;
+    out_h += R * p.D;
+    st_y += R;
+    st_x += R;
+    left -= R;
+    if (at.next(R) && left > 0) sample();
   }
 }
 
-template <typename T, int R>
-__global__ void __launch_bounds__(512) sandwich_bwd_kernel(SandwichParams p, SandwichBwdParams q, SwGeom g, int* err) {
+// One barrier per step: what the second half needs of a row is kept as fp32 (w1 = dx' + rx dh cw, n, yn).
+template <typename T, int R, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) sandwich_bwd_kernel(SandwichParams p, SandwichBwdParams q, SwGeom g,
+                                                                  int* err) {
+  constexpr int N = R == 1 ? 4 : 8;  // three sums per row
   extern __shared__ __align__(128) uint8_t sw_smem[];
-  __shared__ float red[2][3 * R * 16];
-  const int group = threadIdx.x / g.tpg, c0 = (threadIdx.x % g.tpg) * 8;
-  const bool on = c0 < p.D;
-  const int warps = blockDim.x >> 5, wpg = g.tpg >> 5, w0 = group * wpg;
+  __shared__ __align__(16) float red[2][N * RED_PITCH];
+  const int group = threadIdx.x / g.tpg, tc = (threadIdx.x % g.tpg) * 8;
+  const bool on = tc < p.D;
+  const int c0 = on ? tc : 0;
+  const int wpg = g.tpg >> 5, quads = (wpg + 3) >> 2, first = group * quads * 4, slot = first + warp_id() - group * wpg;
   const int unit = blockIdx.x * g.groups + group;
   const long long row0 = (long long)unit * g.span;
-  const bool per_sample = samples_of(p) > 1;
+  const float inv_d = 1.f / p.D;
   const SwRing<T, R, 4> ring(sw_smem, g, p.D);
   const void* const src[4] = {p.x, p.y, q.dh, q.dx_new};
+  for (int i = threadIdx.x; i < 2 * N * RED_PITCH; i += blockDim.x) (&red[0][0])[i] = 0.f;
   if (threadIdx.x == 0) {
     for (int s = 0; s < SW_STAGES; ++s) mbar_init(&ring.full[s], 1);
     fence_barrier_init();
@@ -403,123 +458,111 @@ __global__ void __launch_bounds__(512) sandwich_bwd_kernel(SandwichParams p, San
     for (int i = 0; i < SW_STAGES && i < g.steps; ++i) sw_load<T, R, 4>(ring, g, p.M, p.D, i, src);
   }
   __syncthreads();
-  float a[8], cw[8], acc[3][8];
+  const int rows = (int)max(0ll, min((long long)g.span, p.M - row0));
+  SwSample at(p, samples_of(p) > 1, row0);
+  const bool post = p.post_w != nullptr, pre = p.w != nullptr;
+  f32x2 a[4], cw[4], acc[3][4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[0][j] = acc[1][j] = acc[2][j] = 0.f;
-  int cur = -1, acc_b = -1;
-  auto sample = [&](int b) {
-    if (b == cur || !on) return;
-    cur = b;
-    float t[8];
+  for (int j = 0; j < 4; ++j) acc[0][j] = acc[1][j] = acc[2][j] = x2(0.f);
+  if (rows > 0) sw_constants<T>(p, at.b, c0, a, cw);
+  const T* slots = ring.row(0, 0, group, 0, p.D) + c0;
+  const int to_next = (int)(ring.tensor_bytes / sizeof(T)), to_stage = (int)(ring.step_bytes / sizeof(T));
+  T* out_x = reinterpret_cast<T*>(q.dx) + row0 * p.D + c0;
+  T* out_y = reinterpret_cast<T*>(q.dy) + row0 * p.D + c0;
+  const float *st_y = p.rstd_y + row0, *st_x = p.rstd_x + row0;
+  float ry[R], rx[R];
+  int stage = 0, phase = 0, left = rows;
+  auto stats = [&](int first_row) {  // the forward's statistics of a step's rows
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = p.res_scale, cw[j] = 0.f;
-    if (p.post_w != nullptr) {
-      load_vec<float, 8>(p.post_w + c0, t);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] *= t[j];
-    }
-    if (p.gate != nullptr) {
-      load_row8<T>(p.gate, b * p.gate_bs + c0, t);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] *= t[j];
-    }
-    if (p.w != nullptr) load_vec<float, 8>(p.w + c0, cw);
-    if (p.scale != nullptr) {
-      load_row8<T>(p.scale, b * p.mod_bs + c0, t);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) cw[j] = fmaf(cw[j], t[j], cw[j]);
+    for (int r = 0; r < R; ++r) {
+      ry[r] = post && first_row + r < rows ? st_y[first_row + r] : 1.f;
+      rx[r] = pre && first_row + r < rows ? st_x[first_row + r] : 0.f;
     }
   };
-  auto flush = [&]() {  // the column sums of sample acc_b
-    if (acc_b >= 0 && on) {
-      float* dst = q.partial + (long long)(unit + acc_b) * 3 * p.D + c0;
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        store_vec<float, 8>(dst + (long long)i * p.D, acc[i]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
-      }
-    }
-  };
+  stats(0);
   for (int i = 0; i < g.steps; ++i) {
-    const int stage = i % SW_STAGES;
-    const int n = span_rows(p.M, row0, g.span, i * R, R);
-    const long long row = row0 + (long long)i * R;
-    float ry[R], rx[R];
+    mbar_wait(&ring.full[stage], phase, err, ERR_MBAR_TIMEOUT_PRODUCER);
+    f32x2 w1[R][4], nn[R][4], yn[R][4];
+    float s[N], ky[R];
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k] = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      ry[r] = p.post_w != nullptr && r < n ? p.rstd_y[row + r] : 1.f;
-      rx[r] = p.w != nullptr && r < n ? p.rstd_x[row + r] : 0.f;
-    }
-    mbar_wait(&ring.full[stage], (i / SW_STAGES) & 1, err, ERR_MBAR_TIMEOUT_PRODUCER);
-    Raw<T, 8> x[R], y[R], dh[R], e[R];
-    float s[3 * R];
+      ky[r] = ry[r];
+      if (r < left && on) {
+        const T* in = slots + stage * to_stage + r * p.D;
+        Raw<T, 8> x, y, gh, e;
+        x.load(in);
+        y.load(in + to_next);
+        if (q.dh != nullptr) gh.load(in + 2 * to_next);
+        else gh.zero();
+        if (q.dx_new != nullptr) e.load(in + 3 * to_next);
+        else e.zero();
+        f32x2 gf[4];
+        unpack_x2<T>(x, nn[r]);
+        unpack_x2<T>(y, yn[r]);
+        unpack_x2<T>(gh, gf);
+        unpack_x2<T>(e, w1[r]);
+        const f32x2 ry2 = x2(ry[r]), rx2 = x2(rx[r]);
+        f32x2 s0 = x2(0.f), s1 = x2(0.f), s2 = x2(0.f);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      s[3 * r] = s[3 * r + 1] = s[3 * r + 2] = 0.f;
-      dh[r].zero();
-      e[r].zero();
-      if (r >= n || !on) {
-        x[r].zero();
-        y[r].zero();
-        continue;
-      }
-      sample(per_sample ? (int)((row + r) / p.T) : 0);
-      x[r].load(ring.row(stage, 0, group, r, p.D) + c0);
-      y[r].load(ring.row(stage, 1, group, r, p.D) + c0);
-      if (q.dh != nullptr) dh[r].load(ring.row(stage, 2, group, r, p.D) + c0);
-      if (q.dx_new != nullptr) e[r].load(ring.row(stage, 3, group, r, p.D) + c0);
-      float xf[8], yf[8], gf[8], ef[8];
-      x[r].get(xf);
-      y[r].get(yf);
-      dh[r].get(gf);
-      e[r].get(ef);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float ay = a[j] * (yf[j] * ry[r]);
-        const float nn = (xf[j] + ay) * rx[r];
-        const float c = gf[j] * cw[j];
-        s[3 * r] = fmaf(c, nn, s[3 * r]);
-        s[3 * r + 1] = fmaf(ay, fmaf(rx[r], c, ef[j]), s[3 * r + 1]);
-        s[3 * r + 2] = fmaf(ay, nn, s[3 * r + 2]);
+        for (int j = 0; j < 4; ++j) {
+          yn[r][j] = x2_mul(yn[r][j], ry2);
+          const f32x2 ay = x2_mul(a[j], yn[r][j]);
+          nn[r][j] = x2_mul(x2_add(nn[r][j], ay), rx2);
+          const f32x2 c = x2_mul(gf[j], cw[j]);
+          w1[r][j] = x2_fma(rx2, c, w1[r][j]);
+          s0 = x2_fma(c, nn[r][j], s0);
+          s1 = x2_fma(ay, w1[r][j], s1);
+          s2 = x2_fma(ay, nn[r][j], s2);
+          acc[0][j] = x2_add(acc[0][j], gf[j]);
+          acc[1][j] = x2_fma(gf[j], nn[r][j], acc[1][j]);
+        }
+        s[3 * r] = x2_sum(s0) * rx[r];  // rx m D
+        s[3 * r + 1] = x2_sum(s1);
+        s[3 * r + 2] = x2_sum(s2);
       }
     }
-    group_put<3 * R>(s, red[i & 1], warps);
+    group_put<N>(s, red[i & 1], slot);
+    stats((i + 1) * R);  // in flight across the barrier
     __syncthreads();
     if (threadIdx.x == 0 && i + SW_STAGES < g.steps) sw_load<T, R, 4>(ring, g, p.M, p.D, i + SW_STAGES, src);
-    group_get<3 * R>(s, red[i & 1], warps, w0, wpg);
+    if (++stage == SW_STAGES) stage = 0, phase ^= 1;
+    float sum[3 * R];
+    group_get<3 * R>(sum, red[i & 1], first, quads);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (r >= n || !on) continue;
-      const int b = per_sample ? (int)((row + r) / p.T) : 0;
-      if (b != acc_b) {
-        flush();
-        acc_b = b;
-      }
-      sample(b);
-      const float m = s[3 * r] / p.D;
-      const float m2 = p.post_w != nullptr ? (s[3 * r + 1] - rx[r] * m * s[3 * r + 2]) / p.D : 0.f;
-      float xf[8], yf[8], gf[8], ef[8];
-      x[r].get(xf);
-      y[r].get(yf);
-      dh[r].get(gf);
-      e[r].get(ef);
+      if (r < left && on) {
+        const float m = sum[3 * r] * inv_d;
+        const float m2 = post ? ky[r] * (sum[3 * r + 1] - m * sum[3 * r + 2]) * inv_d : 0.f;
+        const f32x2 ry2 = x2(ky[r]), nm = x2(-m), nm2 = x2(-m2);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float yn = yf[j] * ry[r];
-        const float nn = fmaf(a[j], yn, xf[j]) * rx[r];
-        const float gx = fmaf(rx[r], fmaf(gf[j], cw[j], -nn * m), ef[j]);
-        acc[0][j] += gf[j];
-        acc[1][j] = fmaf(gf[j], nn, acc[1][j]);
-        acc[2][j] = fmaf(gx, yn, acc[2][j]);
-        xf[j] = gx;
-        yf[j] = ry[r] * fmaf(a[j], gx, -yn * m2);
+        for (int j = 0; j < 4; ++j) {
+          w1[r][j] = x2_fma(nm, nn[r][j], w1[r][j]);
+          acc[2][j] = x2_fma(w1[r][j], yn[r][j], acc[2][j]);
+          yn[r][j] = x2_fma(nm2, yn[r][j], x2_mul(ry2, x2_mul(a[j], w1[r][j])));
+        }
+        store_x2<T>(out_x + r * p.D, w1[r]);
+        store_x2<T>(out_y + r * p.D, yn[r]);
       }
-      store_vec<T, 8>(reinterpret_cast<T*>(q.dx) + (row + r) * p.D + c0, xf);
-      store_vec<T, 8>(reinterpret_cast<T*>(q.dy) + (row + r) * p.D + c0, yf);
     }
+    out_x += R * p.D;
+    out_y += R * p.D;
+    const bool had = left > 0;
+    left -= R;
+    const int b = at.b;
+    const bool turn = at.next(R);
+    if (had && on && (turn || left <= 0)) {  // the sample's or the unit's last step: its column sums go out
+      float* dst = q.partial + (long long)(unit + b) * 3 * p.D + c0;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        store_x2<float>(dst + (long long)k * p.D, acc[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[k][j] = x2(0.f);
+      }
+    }
+    if (turn && left > 0) sw_constants<T>(p, at.b, c0, a, cw);
   }
-  flush();
 }
 
 // Sums of a sample's partial rows -> its dshift / dscale / dgate rows, and the weights' sums over this block's samples.
@@ -589,12 +632,16 @@ __global__ void sandwich_weights_kernel(SandwichParams p, SandwichBwdParams q) {
 
 namespace {
 
-// rows of the vector form per step and group: two 16-bit rows or one fp32 row
-template <typename T>
-struct SwRows {
-  static constexpr int R = sizeof(T) == 2 ? 2 : 1;
-};
-int sw_rows(int elem) { return elem == ELEM_F32 ? SwRows<float>::R : SwRows<__half>::R; }
+#ifndef FWD_R
+#define FWD_R 2
+#define BWD_R 2
+#define FWD_B 2
+#define BWD_B 2
+#endif
+// rows per step and group: two rows share a barrier where a sample's rows come in pairs (16-bit types)
+int sw_rows(const SandwichParams& p, int es, int most) {
+  return es == 2 && most == 2 && (samples_of(p) == 1 || p.T % 2 == 0) ? 2 : 1;
+}
 
 bool sw_vectors(const SandwichParams& p, const SandwichBwdParams* q) {
   if (p.D % 8 != 0 || p.D > SW_MAX_VEC_D || p.gate_bs % 8 != 0 || p.mod_bs % 8 != 0) return false;
@@ -607,16 +654,16 @@ bool sw_vectors(const SandwichParams& p, const SandwichBwdParams* q) {
   return (bits & 15) == 0;
 }
 
-// groups of a block: about 256 threads; spans that fill every SM with the blocks that its shared memory holds (at most 2)
+// groups of a block: about 256 threads; spans that fill every SM with the blocks that its shared memory holds, up to `blocks`
 int sw_smem(const SandwichParams& p, const SwGeom& g, int R, int tensors, int es) {
   return 128 + SW_STAGES * tensors * g.groups * R * p.D * es;
 }
-SwGeom sw_geom(const SandwichParams& p, int R, int tensors, int es) {
+SwGeom sw_geom(const SandwichParams& p, int R, int tensors, int es, int blocks) {
   SwGeom g;
   g.tpg = (p.D / 8 + 31) / 32 * 32;
   g.groups = std::max(1, 256 / g.tpg);
   const int fit = 226 * 1024 / (sw_smem(p, g, R, tensors, es) + 2048);
-  const int units = num_sms() * std::max(1, std::min(fit, 2)) * g.groups;
+  const int units = num_sms() * std::max(1, std::min(fit, blocks)) * g.groups;
   g.span = (p.M + units - 1) / units;
   g.span = (g.span + R - 1) / R * R;
   g.steps = g.span / R;
@@ -635,42 +682,68 @@ cudaError_t sw_smem_limit(K kernel, int smem, int* allowed) {
   return e;
 }
 
+template <typename T, int R, int MAXT, int MINB>
+cudaError_t fwd_vec(const SandwichParams& p, const SwGeom& g, int* err, cudaStream_t s) {
+  const int smem = sw_smem(p, g, R, 2, sizeof(T));
+  static int allowed = 44 * 1024;
+  cudaError_t e = sw_smem_limit(sandwich_fwd_kernel<T, R, MAXT, MINB>, smem, &allowed);
+  if (e != cudaSuccess) return e;
+  sandwich_fwd_kernel<T, R, MAXT, MINB><<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, g, err);
+  return cudaGetLastError();
+}
+template <typename T, int R, int MAXT, int MINB>
+cudaError_t bwd_vec(const SandwichParams& p, const SandwichBwdParams& q, const SwGeom& g, int* err, cudaStream_t s) {
+  const int smem = sw_smem(p, g, R, 4, sizeof(T));
+  static int allowed = 44 * 1024;
+  cudaError_t e = sw_smem_limit(sandwich_bwd_kernel<T, R, MAXT, MINB>, smem, &allowed);
+  if (e != cudaSuccess) return e;
+  sandwich_bwd_kernel<T, R, MAXT, MINB><<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, q, g, err);
+  return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t fwd_run(const SandwichParams& p, int* err, cudaStream_t s) {
-  constexpr int R = SwRows<T>::R;
-  if (sw_vectors(p, nullptr)) {
-    const SwGeom g = sw_geom(p, R, 2, sizeof(T));
-    const int smem = sw_smem(p, g, R, 2, sizeof(T));
-    static int allowed = 46 * 1024;
-    cudaError_t e = sw_smem_limit(sandwich_fwd_kernel<T, R>, smem, &allowed);
-    if (e != cudaSuccess) return e;
-    sandwich_fwd_kernel<T, R><<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, g, err);
-  } else {
+  if (!sw_vectors(p, nullptr)) {
     sandwich_fwd_any_kernel<T><<<std::min(p.M, num_sms() * 8), SW_THREADS, 0, s>>>(p);
+    return cudaGetLastError();
   }
-  return cudaGetLastError();
+  const int R = sw_rows(p, sizeof(T), FWD_R);
+  const SwGeom g = sw_geom(p, R, 2, sizeof(T), FWD_B);
+  const bool narrow = g.tpg * g.groups <= 256;
+  if constexpr (sizeof(T) == 2) {
+    if (R == 2) return narrow ? fwd_vec<T, 2, 256, FWD_B>(p, g, err, s) : fwd_vec<T, 2, 512, 1>(p, g, err, s);
+  }
+  return narrow ? fwd_vec<T, 1, 256, FWD_B>(p, g, err, s) : fwd_vec<T, 1, 512, 1>(p, g, err, s);
+}
+
+template <typename T>
+cudaError_t bwd_rows(const SandwichParams& p, const SandwichBwdParams& q, int* err, cudaStream_t s) {
+  const int R = sw_rows(p, sizeof(T), BWD_R);
+  const SwGeom g = sw_geom(p, R, 4, sizeof(T), BWD_B);
+  const bool narrow = g.tpg * g.groups <= 256;
+#if BWD_R == 2
+  if constexpr (sizeof(T) == 2) {
+    if (R == 2) return narrow ? bwd_vec<T, 2, 256, BWD_B>(p, q, g, err, s) : bwd_vec<T, 2, 512, 1>(p, q, g, err, s);
+  }
+#endif
+  return narrow ? bwd_vec<T, 1, 256, BWD_B>(p, q, g, err, s) : bwd_vec<T, 1, 512, 1>(p, q, g, err, s);
 }
 
 template <typename T>
 cudaError_t bwd_run(const SandwichParams& p, const SandwichBwdParams& q, int* err, cudaStream_t s) {
   cudaError_t e;
   if (sw_vectors(p, &q)) {
-    constexpr int R = SwRows<T>::R;
-    const SwGeom g = sw_geom(p, R, 4, sizeof(T));
-    const int smem = sw_smem(p, g, R, 4, sizeof(T));
-    static int allowed = 46 * 1024;
-    e = sw_smem_limit(sandwich_bwd_kernel<T, R>, smem, &allowed);
+    e = bwd_rows<T>(p, q, err, s);
     if (e != cudaSuccess) return e;
-    sandwich_bwd_kernel<T, R><<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, q, g, err);
   } else {
     const int smem = 3 * p.D * (int)sizeof(float);
     static int allowed = 46 * 1024;
     e = sw_smem_limit(sandwich_bwd_any_kernel<T>, smem, &allowed);
     if (e != cudaSuccess) return e;
     sandwich_bwd_any_kernel<T><<<q.ctas, SW_THREADS, smem, s>>>(p, q);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
   }
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   sandwich_reduce_kernel<T><<<dim3((p.D + 31) / 32, q.groups), dim3(32, RED_ROWS), 0, s>>>(p, q);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
@@ -693,7 +766,8 @@ cudaError_t sandwich_fwd_launch(const SandwichParams& p, int elem, int* err, cud
 
 void sandwich_bwd_plan(const SandwichParams& p, int elem, SandwichBwdParams* q) {
   if (sw_vectors(p, q)) {
-    const SwGeom g = sw_geom(p, sw_rows(elem), 4, elem == ELEM_F32 ? 4 : 2);
+    const int es = elem == ELEM_F32 ? 4 : 2;
+    const SwGeom g = sw_geom(p, sw_rows(p, es, BWD_R), 4, es, BWD_B);
     q->rows_per_cta = g.span;
   } else {
     const int most = num_sms() * 4;

@@ -84,6 +84,60 @@ struct Raw {
     }
   }
 };
+// Pairs of fp32 in one 64-bit register: sm_100 issues one instruction for both (f32x2).
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 x2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 x2(float a) { return x2(a, a); }
+__device__ __forceinline__ float2 x2_split(f32x2 r) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r));
+  return f;
+}
+__device__ __forceinline__ f32x2 x2_fma(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 x2_mul(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 x2_add(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float x2_sum(f32x2 r) {
+  const float2 f = x2_split(r);
+  return f.x + f.y;
+}
+
+// 8 stored elements as 4 fp32 pairs, and back
+template <typename T>
+__device__ __forceinline__ void unpack_x2(const Raw<T, 8>& r, f32x2 (&v)[4]) {
+  float f[8];
+  r.get(f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = x2(f[2 * i], f[2 * i + 1]);
+}
+template <typename T>
+__device__ __forceinline__ void store_x2(T* p, const f32x2 (&v)[4]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = x2_split(v[i]);
+    f[2 * i] = t.x, f[2 * i + 1] = t.y;
+  }
+  Raw<T, 8> r;
+  r.put(f);
+  r.store(p);
+}
+
 template <typename T>
 struct Raw<T, 1> {
   T e;
