@@ -309,7 +309,7 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
     return {dx, dy, dgate, dshift, dscale};
   }
   const int elem = elem_of(x, "sandwich_bwd");
-  sandwich_bwd_plan(p, elem, &q);
+  BLOCK_LAUNCH(sandwich_bwd_plan(p, elem, &q), 0);
   const int64_t entries = q.ctas + B, floats = entries * 3 * D + (int64_t)q.groups * 2 * D;
   at::Tensor scratch = at::empty({floats}, x.options().dtype(at::kFloat));
   q.partial = scratch.data_ptr<float>();

@@ -88,7 +88,7 @@ struct SandwichBwdParams {
 };
 // err: device error word of the kernels' bounded waits
 cudaError_t sandwich_fwd_launch(const SandwichParams& p, int elem, int* err, cudaStream_t s);
-void sandwich_bwd_plan(const SandwichParams& p, int elem, SandwichBwdParams* q);  // sets ctas, rows_per_cta, groups
+cudaError_t sandwich_bwd_plan(const SandwichParams& p, int elem, SandwichBwdParams* q);  // sets ctas, rows_per_cta, groups
 cudaError_t sandwich_bwd_launch(const SandwichParams& p, const SandwichBwdParams& q, int elem, int* err, cudaStream_t s);
 
 // ---------------------------------------------------------------- rotary positions with several axes (rope_axes.cu)

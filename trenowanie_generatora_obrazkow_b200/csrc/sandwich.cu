@@ -176,11 +176,9 @@ __global__ void __launch_bounds__(SW_THREADS) sandwich_bwd_any_kernel(SandwichPa
 // ------------------------------------------------------------------------------------------------------------------
 namespace {
 
-#ifndef STAGES
-#define STAGES 3
-#endif
-constexpr int SW_STAGES = STAGES;
+constexpr int SW_STAGES = 2;
 constexpr int SW_MAX_VEC_D = 4096;
+constexpr int SW_MAX_GROUPS = 8;  // 256 threads of 32 each
 
 struct SwGeom {
   int tpg, groups;      // threads per group, groups per block
@@ -207,35 +205,31 @@ struct SwRing {
   }
 };
 
-__device__ __forceinline__ int span_rows(int M, long long row0, int span, int done, int R) {
-  const long long left = min((long long)M, row0 + span) - (row0 + done);
-  return (int)max(0ll, min((long long)R, left));
+// rows of a step that starts at `row` with `left` rows of its span to go
+__device__ __forceinline__ int step_rows(int M, long long row, int left, int R) {
+  return max(0, min(min(R, left), (int)min((long long)R, M - row)));
 }
 
 // one thread: the rows of step i of every group of this block, all tensors
 template <typename T, int R, int TENSORS>
 __device__ __forceinline__ void sw_load(const SwRing<T, R, TENSORS>& ring, const SwGeom& g, int M, int D, int i,
-                                        const void* const (&src)[TENSORS]) {
-  const int stage = i % SW_STAGES;
-  uint32_t bytes = 0;
+                                        int stage, const void* const (&src)[TENSORS]) {
+  const int present = TENSORS == 2 ? 2 : 2 + (src[2] != nullptr) + (src[TENSORS - 1] != nullptr);
+  const long long row0 = (long long)blockIdx.x * g.groups * g.span + i * R;
+  const int row_bytes = D * (int)sizeof(T);
+  uint8_t* slot = ring.base + stage * ring.step_bytes;
+  int total = 0;
+  for (int k = 0; k < g.groups; ++k) total += step_rows(M, row0 + (long long)k * g.span, g.span - i * R, R);
+  mbar_expect_tx(&ring.full[stage], (uint32_t)(total * row_bytes * present));
   for (int k = 0; k < g.groups; ++k) {
-    const long long row0 = ((long long)blockIdx.x * g.groups + k) * g.span;
-    bytes += (uint32_t)(span_rows(M, row0, g.span, i * R, R) * D * sizeof(T));
-  }
-  uint32_t present = 0;
-#pragma unroll
-  for (int t = 0; t < TENSORS; ++t) present += src[t] != nullptr;
-  mbar_expect_tx(&ring.full[stage], bytes * present);
-  for (int k = 0; k < g.groups; ++k) {
-    const long long row0 = ((long long)blockIdx.x * g.groups + k) * g.span;
-    const int n = span_rows(M, row0, g.span, i * R, R);
-    if (n <= 0) continue;
+    const long long row = row0 + (long long)k * g.span;
+    const int bytes = step_rows(M, row, g.span - i * R, R) * row_bytes;
+    if (bytes <= 0) continue;
 #pragma unroll
     for (int t = 0; t < TENSORS; ++t)
-      if (src[t] != nullptr)
-        bulk_load(const_cast<T*>(ring.row(stage, t, k, 0, D)),
-                  reinterpret_cast<const T*>(src[t]) + (row0 + (long long)i * R) * D, (uint32_t)(n * D * sizeof(T)),
-                  &ring.full[stage]);
+      if (t < 2 || src[t] != nullptr)
+        bulk_load(slot + t * ring.tensor_bytes + k * ring.group_bytes,
+                  reinterpret_cast<const T*>(src[t]) + row * D, (uint32_t)bytes, &ring.full[stage]);
   }
 }
 
@@ -251,17 +245,17 @@ __device__ __forceinline__ void load_w8(const float* p, f32x2 (&v)[4]) {
   unpack_x2<float>(r, v);
 }
 
-// N sums over a group's warps. Step 1 (group_put): the lanes' values are summed over the warp while their number is
-// halved (a lane pair exchanges the halves that the other keeps), so N values cost about N + 5 shuffles instead of 5 N;
-// one lane per value writes it to red[value][group's slot of this warp]. Step 2 (group_get), after the caller's barrier:
-// every thread adds the group's slots (padded with zeros to float4s).
-constexpr int RED_PITCH = 32;
-template <int N>
-__device__ __forceinline__ void group_put(float (&v)[N], float* red, int slot) {
-  static_assert(N == 1 || N == 2 || N == 4 || N == 8, "a power of two");
+// V sums over a group's warps (P slots, wpg <= P of them used, the others hold zeros).
+// group_put: the lanes' values are summed over the warp while their number is halved (a lane pair exchanges the halves
+// that the other keeps), so V values cost about V + 5 shuffles instead of 5 V; one lane per value writes red[v P + slot].
+// group_total, after the caller's barrier: lane l of every warp takes the entries l, l + 32, ... and the P slots of a value,
+// which sit in neighbouring lanes, are added by shuffles. Value v is then in every lane of its P, of register v P / 32.
+template <int V, int P>
+__device__ __forceinline__ void group_put(float (&v)[V], float* red, int slot) {
+  static_assert(V == 1 || V == 2 || V == 4 || V == 8, "a power of two");
   int keep = 0, bit = 16;
 #pragma unroll
-  for (int h = N / 2; h >= 1; h >>= 1) {
+  for (int h = V / 2; h >= 1; h >>= 1) {
     const bool up = lane_id() & bit;
 #pragma unroll
     for (int i = 0; i < h; ++i) {
@@ -273,22 +267,24 @@ __device__ __forceinline__ void group_put(float (&v)[N], float* red, int slot) {
   }
   float t = v[0];
 #pragma unroll
-  for (int o = 16 / N; o >= 1; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  if ((lane_id() & (32 / N - 1)) == 0) red[keep * RED_PITCH + slot] = t;
+  for (int o = 16 / V; o >= 1; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if ((lane_id() & (32 / V - 1)) == 0) red[keep * P + slot] = t;
 }
-template <int N>
-__device__ __forceinline__ void group_get(float (&v)[N], const float* red, int first, int quads) {
+template <int V, int P>
+struct Totals {
+  static constexpr int K = (V * P + 31) / 32;
+  float t[K];
+  __device__ __forceinline__ explicit Totals(const float* red) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float4* q = reinterpret_cast<const float4*>(red + i * RED_PITCH + first);
-    float4 t = q[0];
-    for (int k = 1; k < quads; ++k) {
-      const float4 u = q[k];
-      t.x += u.x, t.y += u.y, t.z += u.z, t.w += u.w;
+    for (int k = 0; k < K; ++k) {
+      const int i = k * 32 + lane_id();
+      t[k] = V * P >= 32 || i < V * P ? red[i] : 0.f;
+#pragma unroll
+      for (int o = 1; o < P; o <<= 1) t[k] += __shfl_xor_sync(0xffffffffu, t[k], o);
     }
-    v[i] = (t.x + t.y) + (t.z + t.w);
   }
-}
+  __device__ __forceinline__ float get(int v) const { return __shfl_sync(0xffffffffu, t[v * P / 32], v * P % 32); }
+};
 
 // Position of a unit in its samples, advanced step by step (no division in the row loop). R divides T, so a step never
 // straddles two samples.
@@ -335,24 +331,25 @@ __device__ __forceinline__ void sw_constants(const SandwichParams& p, int b, int
 }  // namespace
 
 // Threads past the last channel of a row (D / 8 not a multiple of 32) work on channel 0's values and keep their sums at 0.
-template <typename T, int R, int MAXT, int MINB>
+template <typename T, int R, int P, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) sandwich_fwd_kernel(SandwichParams p, SwGeom g, int* err) {
   extern __shared__ __align__(128) uint8_t sw_smem[];
-  __shared__ __align__(16) float red[2][R * RED_PITCH];
+  __shared__ float reds[2][SW_MAX_GROUPS * R * P];
   const int group = threadIdx.x / g.tpg, tc = (threadIdx.x % g.tpg) * 8;
-  const bool on = tc < p.D, lead = tc == 0;
+  const bool on = tc < p.D;
   const int c0 = on ? tc : 0;
-  const int wpg = g.tpg >> 5, quads = (wpg + 3) >> 2, first = group * quads * 4, slot = first + warp_id() - group * wpg;
+  const int slot = warp_id() - group * (g.tpg >> 5);
   const long long row0 = ((long long)blockIdx.x * g.groups + group) * g.span;
   const float inv_d = 1.f / p.D;
   const SwRing<T, R, 2> ring(sw_smem, g, p.D);
   const void* const src[2] = {p.x, p.y};
-  for (int i = threadIdx.x; i < 2 * R * RED_PITCH; i += blockDim.x) (&red[0][0])[i] = 0.f;
+  for (int i = threadIdx.x; i < 2 * SW_MAX_GROUPS * R * P; i += blockDim.x) (&reds[0][0])[i] = 0.f;
+  float* const red[2] = {reds[0] + group * R * P, reds[1] + group * R * P};
   if (threadIdx.x == 0) {
     for (int s = 0; s < SW_STAGES; ++s) mbar_init(&ring.full[s], 1);
     fence_barrier_init();
     fence_proxy_async_smem();
-    for (int i = 0; i < SW_STAGES && i < g.steps; ++i) sw_load<T, R, 2>(ring, g, p.M, p.D, i, src);
+    for (int i = 0; i < SW_STAGES && i < g.steps; ++i) sw_load<T, R, 2>(ring, g, p.M, p.D, i, i, src);
   }
   __syncthreads();
   const int rows = (int)max(0ll, min((long long)g.span, p.M - row0));
@@ -387,16 +384,22 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_fwd_kernel(SandwichParams
       for (int j = 0; j < 4; ++j) q = x2_fma(f[j], f[j], q);
       s[r] = on ? x2_sum(q) : 0.f;
     }
-    group_put<R>(s, red[0], slot);
+    group_put<R, P>(s, red[0], slot);
     __syncthreads();  // every thread has taken its rows out of the stage: refill it
-    if (threadIdx.x == 0 && i + SW_STAGES < g.steps) sw_load<T, R, 2>(ring, g, p.M, p.D, i + SW_STAGES, src);
+    if (threadIdx.x == 0 && i + SW_STAGES < g.steps) sw_load<T, R, 2>(ring, g, p.M, p.D, i + SW_STAGES, stage, src);
     if (++stage == SW_STAGES) stage = 0, phase ^= 1;
-    group_get<R>(s, red[0], first, quads);
+    // the lanes that hold row r's sum turn it into its statistic once
+    Totals<R, P> ty(red[0]);
+#pragma unroll
+    for (int k = 0; k < Totals<R, P>::K; ++k) {
+      ty.t[k] = post ? rsqrtf(fmaf(ty.t[k], inv_d, p.eps)) : 1.f;
+      const int r = (k * 32 + lane_id()) / P;
+      if (post && slot == 0 && lane_id() % P == 0 && r < R && r < left) st_y[r] = ty.t[k];
+    }
     f32x2 xn[R][4];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float ry = post ? rsqrtf(fmaf(s[r], inv_d, p.eps)) : 1.f;
-      if (lead && post && r < left) st_y[r] = ry;
+      const float ry = ty.get(r);
       f32x2 f[4], q = x2(0.f);
       const f32x2 ry2 = x2(ry);
       unpack_x2<T>(x[r], xn[r]);
@@ -409,20 +412,22 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_fwd_kernel(SandwichParams
       s[r] = on ? x2_sum(q) : 0.f;
       if (on && r < left) store_x2<T>(out_x + r * p.D, xn[r]);
     }
-    group_put<R>(s, red[1], slot);
+    group_put<R, P>(s, red[1], slot);
     __syncthreads();
     if (pre) {
-      group_get<R>(s, red[1], first, quads);
+      Totals<R, P> tx(red[1]);
+#pragma unroll
+      for (int k = 0; k < Totals<R, P>::K; ++k) {
+        tx.t[k] = rsqrtf(fmaf(tx.t[k], inv_d, p.eps));
+        const int r = (k * 32 + lane_id()) / P;
+        if (slot == 0 && lane_id() % P == 0 && r < R && r < left) st_x[r] = tx.t[k];
+      }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float rx = rsqrtf(fmaf(s[r], inv_d, p.eps));
-        const f32x2 rx2 = x2(rx);
+        const f32x2 rx2 = x2(tx.get(r));
 #pragma unroll
         for (int j = 0; j < 4; ++j) xn[r][j] = x2_fma(x2_mul(xn[r][j], rx2), cw[j], sh[j]);
-        if (r < left) {
-          if (lead) st_x[r] = rx;
-          if (on) store_x2<T>(out_h + r * p.D, xn[r]);
-        }
+        if (on && r < left) store_x2<T>(out_h + r * p.D, xn[r]);
       }
     }
     out_x += R * p.D;
@@ -435,27 +440,28 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_fwd_kernel(SandwichParams
 }
 
 // One barrier per step: what the second half needs of a row is kept as fp32 (w1 = dx' + rx dh cw, n, yn).
-template <typename T, int R, int MAXT, int MINB>
+template <typename T, int R, int P, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) sandwich_bwd_kernel(SandwichParams p, SandwichBwdParams q, SwGeom g,
                                                                   int* err) {
   constexpr int N = R == 1 ? 4 : 8;  // three sums per row
   extern __shared__ __align__(128) uint8_t sw_smem[];
-  __shared__ __align__(16) float red[2][N * RED_PITCH];
+  __shared__ float reds[2][SW_MAX_GROUPS * N * P];
   const int group = threadIdx.x / g.tpg, tc = (threadIdx.x % g.tpg) * 8;
   const bool on = tc < p.D;
   const int c0 = on ? tc : 0;
-  const int wpg = g.tpg >> 5, quads = (wpg + 3) >> 2, first = group * quads * 4, slot = first + warp_id() - group * wpg;
+  const int slot = warp_id() - group * (g.tpg >> 5);
   const int unit = blockIdx.x * g.groups + group;
   const long long row0 = (long long)unit * g.span;
   const float inv_d = 1.f / p.D;
   const SwRing<T, R, 4> ring(sw_smem, g, p.D);
   const void* const src[4] = {p.x, p.y, q.dh, q.dx_new};
-  for (int i = threadIdx.x; i < 2 * N * RED_PITCH; i += blockDim.x) (&red[0][0])[i] = 0.f;
+  for (int i = threadIdx.x; i < 2 * SW_MAX_GROUPS * N * P; i += blockDim.x) (&reds[0][0])[i] = 0.f;
+  float* const red0 = reds[0] + group * N * P;
   if (threadIdx.x == 0) {
     for (int s = 0; s < SW_STAGES; ++s) mbar_init(&ring.full[s], 1);
     fence_barrier_init();
     fence_proxy_async_smem();
-    for (int i = 0; i < SW_STAGES && i < g.steps; ++i) sw_load<T, R, 4>(ring, g, p.M, p.D, i, src);
+    for (int i = 0; i < SW_STAGES && i < g.steps; ++i) sw_load<T, R, 4>(ring, g, p.M, p.D, i, i, src);
   }
   __syncthreads();
   const int rows = (int)max(0ll, min((long long)g.span, p.M - row0));
@@ -523,18 +529,20 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_bwd_kernel(SandwichParams
         s[3 * r + 2] = x2_sum(s2);
       }
     }
-    group_put<N>(s, red[i & 1], slot);
+    group_put<N, P>(s, red0 + (i & 1) * (SW_MAX_GROUPS * N * P), slot);
     stats((i + 1) * R);  // in flight across the barrier
     __syncthreads();
-    if (threadIdx.x == 0 && i + SW_STAGES < g.steps) sw_load<T, R, 4>(ring, g, p.M, p.D, i + SW_STAGES, src);
+    if (threadIdx.x == 0 && i + SW_STAGES < g.steps) sw_load<T, R, 4>(ring, g, p.M, p.D, i + SW_STAGES, stage, src);
     if (++stage == SW_STAGES) stage = 0, phase ^= 1;
+    const Totals<N, P> sums(red0 + (i & 1) * (SW_MAX_GROUPS * N * P));
     float sum[3 * R];
-    group_get<3 * R>(sum, red[i & 1], first, quads);
+#pragma unroll
+    for (int k = 0; k < 3 * R; ++k) sum[k] = sums.get(k) * inv_d;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       if (r < left && on) {
-        const float m = sum[3 * r] * inv_d;
-        const float m2 = post ? ky[r] * (sum[3 * r + 1] - m * sum[3 * r + 2]) * inv_d : 0.f;
+        const float m = sum[3 * r];
+        const float m2 = post ? ky[r] * (sum[3 * r + 1] - m * sum[3 * r + 2]) : 0.f;
         const f32x2 ry2 = x2(ky[r]), nm = x2(-m), nm2 = x2(-m2);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -565,38 +573,49 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_bwd_kernel(SandwichParams
   }
 }
 
-// Sums of a sample's partial rows -> its dshift / dscale / dgate rows, and the weights' sums over this block's samples.
-constexpr int RED_ROWS = 8;
+// Sums of a sample's partial rows -> its dshift / dscale / dgate rows, and the weights' sums over this block's samples. A
+// block owns 32 channels (lane = channel) and 32 warps: `wps` warps share a sample's rows, so few samples with many rows
+// (no modulation: one sample) and many samples with few rows both fill the block.
+constexpr int RED_WARPS = 32;
 template <typename T>
-__global__ void __launch_bounds__(32 * RED_ROWS) sandwich_reduce_kernel(SandwichParams p, SandwichBwdParams q) {
-  __shared__ float part[RED_ROWS][3][32];
+__global__ void __launch_bounds__(32 * RED_WARPS) sandwich_reduce_kernel(SandwichParams p, SandwichBwdParams q,
+                                                                         int wps) {
+  __shared__ float part[RED_WARPS][3][32];
   const int samples = samples_of(p);
   const int T_rows = samples > 1 ? p.T : p.M;
-  const int c = blockIdx.x * 32 + threadIdx.x;
+  const int lane = lane_id(), warp = warp_id(), share = warp % wps;
+  const int c = blockIdx.x * 32 + lane;
   const bool ok = c < p.D;
-  const int per = (samples + gridDim.y - 1) / gridDim.y;
+  const int per = (samples + gridDim.y - 1) / gridDim.y, at_once = RED_WARPS / wps;
   const int b0 = blockIdx.y * per, b1 = min(samples, b0 + per);
   const float w = ok && p.w != nullptr ? p.w[c] : 0.f;
   const float pw = ok && p.post_w != nullptr ? p.post_w[c] : 1.f;
   float sum_w = 0.f, sum_p = 0.f;
-  for (int b = b0; b < b1; ++b) {
-    const int first = (int)((long long)b * T_rows / q.rows_per_cta);
-    const int last = (int)(((long long)(b + 1) * T_rows - 1) / q.rows_per_cta);
+  for (int bb = b0; bb < b1; bb += at_once) {
+    const int b = bb + warp / wps;
+    const bool live = b < b1 && ok;
     float s[3] = {0.f, 0.f, 0.f};
-    if (ok)
-      for (int k = first + threadIdx.y; k <= last; k += RED_ROWS) {
+    if (live) {
+      const int first = (int)((long long)b * T_rows / q.rows_per_cta);
+      const int last = (int)(((long long)(b + 1) * T_rows - 1) / q.rows_per_cta);
+#pragma unroll 4
+      for (int k = first + share; k <= last; k += wps) {
         const float* src = q.partial + (long long)(k + b) * 3 * p.D + c;
 #pragma unroll
         for (int i = 0; i < 3; ++i) s[i] += src[(long long)i * p.D];
       }
+    }
+    if (wps > 1) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) part[threadIdx.y][i][threadIdx.x] = s[i];
-    __syncthreads();
-    if (threadIdx.y == 0 && ok) {
+      for (int i = 0; i < 3; ++i) part[warp][i][lane] = s[i];
+      __syncthreads();
+      if (share == 0)
+        for (int k = 1; k < wps; ++k)
 #pragma unroll
-      for (int k = 1; k < RED_ROWS; ++k)
-#pragma unroll
-        for (int i = 0; i < 3; ++i) s[i] += part[k][i][threadIdx.x];
+          for (int i = 0; i < 3; ++i) s[i] += part[warp + k][i][lane];
+      __syncthreads();
+    }
+    if (live && share == 0) {
       float sc = 1.f, g = p.res_scale;
       if (p.scale != nullptr) {
         sc += to_f<T>(reinterpret_cast<const T*>(p.scale)[b * p.mod_bs + c]);
@@ -610,38 +629,43 @@ __global__ void __launch_bounds__(32 * RED_ROWS) sandwich_reduce_kernel(Sandwich
       sum_w = fmaf(sc, s[1], sum_w);
       sum_p = fmaf(g, s[2], sum_p);
     }
-    __syncthreads();
   }
-  if (threadIdx.y == 0 && ok) {
-    q.wpart[(long long)blockIdx.y * 2 * p.D + c] = sum_w;
-    q.wpart[((long long)blockIdx.y * 2 + 1) * p.D + c] = sum_p;
+  part[warp][0][lane] = sum_w;
+  part[warp][1][lane] = sum_p;
+  __syncthreads();
+  if (warp < 2 && ok) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < RED_WARPS; ++k) t += part[k][warp][lane];
+    float* dst = warp == 0 ? q.dw : q.dpost_w;
+    if (gridDim.y > 1) q.wpart[((long long)blockIdx.y * 2 + warp) * p.D + c] = t;
+    else if (dst != nullptr) dst[c] += t;
   }
 }
 
-__global__ void sandwich_weights_kernel(SandwichParams p, SandwichBwdParams q) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= p.D) return;
-  float a = 0.f, b = 0.f;
-  for (int g = 0; g < q.groups; ++g) {
-    a += q.wpart[(long long)g * 2 * p.D + c];
-    b += q.wpart[((long long)g * 2 + 1) * p.D + c];
-  }
-  if (q.dw != nullptr) q.dw[c] += a;
-  if (q.dpost_w != nullptr) q.dpost_w[c] += b;
+// dw / dpost_w += the groups' sums (only with more than one group of samples)
+__global__ void __launch_bounds__(256) sandwich_weights_kernel(SandwichParams p, SandwichBwdParams q) {
+  __shared__ float part[8][32];
+  const int lane = lane_id(), c = blockIdx.x * 32 + lane;
+  float* dst = blockIdx.y == 0 ? q.dw : q.dpost_w;
+  float s = 0.f;
+  if (c < p.D)
+    for (int g = warp_id(); g < q.groups; g += 8) s += q.wpart[((long long)g * 2 + blockIdx.y) * p.D + c];
+  part[warp_id()][lane] = s;
+  __syncthreads();
+  if (warp_id() != 0 || c >= p.D || dst == nullptr) return;
+  for (int i = 1; i < 8; ++i) s += part[i][lane];
+  dst[c] += s;
 }
 
 namespace {
 
-#ifndef FWD_R
-#define FWD_R 2
-#define BWD_R 2
-#define FWD_B 2
-#define BWD_B 2
-#endif
-// rows per step and group: two rows share a barrier where a sample's rows come in pairs (16-bit types)
-int sw_rows(const SandwichParams& p, int es, int most) {
-  return es == 2 && most == 2 && (samples_of(p) == 1 || p.T % 2 == 0) ? 2 : 1;
-}
+// Rows per step and group (16-bit and fp32 rows). 32 x 1024 x 2048 bf16: forward 1 / 2 / 4 rows 139 / 96 / 100 us, backward
+// 1 / 2 rows 181 / 175 us; fp32 32 x 1024 x 1024 backward 2 rows spill (165 us against 155 us).
+template <typename T>
+struct SwRows {
+  static constexpr int FWD = 2, BWD = sizeof(T) == 2 ? 2 : 1;
+};
 
 bool sw_vectors(const SandwichParams& p, const SandwichBwdParams* q) {
   if (p.D % 8 != 0 || p.D > SW_MAX_VEC_D || p.gate_bs % 8 != 0 || p.mod_bs % 8 != 0) return false;
@@ -654,51 +678,63 @@ bool sw_vectors(const SandwichParams& p, const SandwichBwdParams* q) {
   return (bits & 15) == 0;
 }
 
-// groups of a block: about 256 threads; spans that fill every SM with the blocks that its shared memory holds, up to `blocks`
-int sw_smem(const SandwichParams& p, const SwGeom& g, int R, int tensors, int es) {
-  return 128 + SW_STAGES * tensors * g.groups * R * p.D * es;
-}
-SwGeom sw_geom(const SandwichParams& p, int R, int tensors, int es, int blocks) {
-  SwGeom g;
-  g.tpg = (p.D / 8 + 31) / 32 * 32;
-  g.groups = std::max(1, 256 / g.tpg);
-  const int fit = 226 * 1024 / (sw_smem(p, g, R, tensors, es) + 2048);
-  const int units = num_sms() * std::max(1, std::min(fit, blocks)) * g.groups;
-  g.span = (p.M + units - 1) / units;
-  g.span = (g.span + R - 1) / R * R;
-  g.steps = g.span / R;
-  return g;
+int sw_threads(const SandwichParams& p, SwGeom* g) {  // groups of a block: about 256 threads
+  g->tpg = (p.D / 8 + 31) / 32 * 32;
+  g->groups = std::max(1, 256 / g->tpg);
+  return g->tpg * g->groups;
 }
 int sw_blocks(const SandwichParams& p, const SwGeom& g) {
   const int units = (p.M + g.span - 1) / g.span;
   return (units + g.groups - 1) / g.groups;
 }
 
-template <typename K>
-cudaError_t sw_smem_limit(K kernel, int smem, int* allowed) {
-  if (smem <= *allowed) return cudaSuccess;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) *allowed = smem;
-  return e;
+// Calls f(kernel, R, tensors, element size) with the variant for p: R rows per step, as many as divide a sample's rows;
+// threads up to 256 (8 slots of the group sums), 320 and 512 (16 slots).
+template <typename T, int R, typename F>
+auto sw_fwd_width(const SandwichParams& p, F f) {
+  SwGeom g;
+  const int threads = sw_threads(p, &g);
+  if (threads <= 256) return f(sandwich_fwd_kernel<T, R, 8, 256, 2>, R, 2, (int)sizeof(T));
+  if (threads <= 320) return f(sandwich_fwd_kernel<T, R, 16, 320, 2>, R, 2, (int)sizeof(T));
+  return f(sandwich_fwd_kernel<T, R, 16, 512, 1>, R, 2, (int)sizeof(T));
+}
+template <typename T, int R, typename F>
+auto sw_bwd_width(const SandwichParams& p, F f) {
+  SwGeom g;
+  const int threads = sw_threads(p, &g);
+  if (threads <= 256) return f(sandwich_bwd_kernel<T, R, 8, 256, 2>, R, 4, (int)sizeof(T));
+  if (threads <= 320) return f(sandwich_bwd_kernel<T, R, 16, 320, 2>, R, 4, (int)sizeof(T));
+  return f(sandwich_bwd_kernel<T, R, 16, 512, 1>, R, 4, (int)sizeof(T));
+}
+template <typename T, int R, typename F>
+auto sw_fwd_pick(const SandwichParams& p, F f) {
+  if constexpr (R > 1) {
+    if (samples_of(p) > 1 && p.T % R != 0) return sw_fwd_pick<T, R / 2>(p, f);
+  }
+  return sw_fwd_width<T, R>(p, f);
+}
+template <typename T, int R, typename F>
+auto sw_bwd_pick(const SandwichParams& p, F f) {
+  if constexpr (R > 1) {
+    if (samples_of(p) > 1 && p.T % R != 0) return sw_bwd_pick<T, R / 2>(p, f);
+  }
+  return sw_bwd_width<T, R>(p, f);
 }
 
-template <typename T, int R, int MAXT, int MINB>
-cudaError_t fwd_vec(const SandwichParams& p, const SwGeom& g, int* err, cudaStream_t s) {
-  const int smem = sw_smem(p, g, R, 2, sizeof(T));
-  static int allowed = 44 * 1024;
-  cudaError_t e = sw_smem_limit(sandwich_fwd_kernel<T, R, MAXT, MINB>, smem, &allowed);
+// Spans that fill every SM with the blocks that it holds; allows the kernel its shared memory.
+template <typename K>
+cudaError_t sw_geom(K kernel, const SandwichParams& p, int R, int tensors, int es, SwGeom* g, int* smem) {
+  const int threads = sw_threads(p, g);
+  *smem = 128 + SW_STAGES * tensors * g->groups * R * p.D * es;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, *smem);
   if (e != cudaSuccess) return e;
-  sandwich_fwd_kernel<T, R, MAXT, MINB><<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, g, err);
-  return cudaGetLastError();
-}
-template <typename T, int R, int MAXT, int MINB>
-cudaError_t bwd_vec(const SandwichParams& p, const SandwichBwdParams& q, const SwGeom& g, int* err, cudaStream_t s) {
-  const int smem = sw_smem(p, g, R, 4, sizeof(T));
-  static int allowed = 44 * 1024;
-  cudaError_t e = sw_smem_limit(sandwich_bwd_kernel<T, R, MAXT, MINB>, smem, &allowed);
+  int blocks = 0;
+  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, *smem);
   if (e != cudaSuccess) return e;
-  sandwich_bwd_kernel<T, R, MAXT, MINB><<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, q, g, err);
-  return cudaGetLastError();
+  const int units = num_sms() * std::max(1, blocks) * g->groups;
+  g->span = ((p.M + units - 1) / units + R - 1) / R * R;
+  g->steps = g->span / R;
+  return cudaSuccess;
 }
 
 template <typename T>
@@ -707,48 +743,55 @@ cudaError_t fwd_run(const SandwichParams& p, int* err, cudaStream_t s) {
     sandwich_fwd_any_kernel<T><<<std::min(p.M, num_sms() * 8), SW_THREADS, 0, s>>>(p);
     return cudaGetLastError();
   }
-  const int R = sw_rows(p, sizeof(T), FWD_R);
-  const SwGeom g = sw_geom(p, R, 2, sizeof(T), FWD_B);
-  const bool narrow = g.tpg * g.groups <= 256;
-  if constexpr (sizeof(T) == 2) {
-    if (R == 2) return narrow ? fwd_vec<T, 2, 256, FWD_B>(p, g, err, s) : fwd_vec<T, 2, 512, 1>(p, g, err, s);
-  }
-  return narrow ? fwd_vec<T, 1, 256, FWD_B>(p, g, err, s) : fwd_vec<T, 1, 512, 1>(p, g, err, s);
+  return sw_fwd_pick<T, SwRows<T>::FWD>(p, [&](auto kernel, int R, int tensors, int es) {
+    SwGeom g;
+    int smem;
+    cudaError_t e = sw_geom(kernel, p, R, tensors, es, &g, &smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, g, err);
+    return cudaGetLastError();
+  });
 }
 
 template <typename T>
-cudaError_t bwd_rows(const SandwichParams& p, const SandwichBwdParams& q, int* err, cudaStream_t s) {
-  const int R = sw_rows(p, sizeof(T), BWD_R);
-  const SwGeom g = sw_geom(p, R, 4, sizeof(T), BWD_B);
-  const bool narrow = g.tpg * g.groups <= 256;
-#if BWD_R == 2
-  if constexpr (sizeof(T) == 2) {
-    if (R == 2) return narrow ? bwd_vec<T, 2, 256, BWD_B>(p, q, g, err, s) : bwd_vec<T, 2, 512, 1>(p, q, g, err, s);
-  }
-#endif
-  return narrow ? bwd_vec<T, 1, 256, BWD_B>(p, q, g, err, s) : bwd_vec<T, 1, 512, 1>(p, q, g, err, s);
+cudaError_t bwd_span(const SandwichParams& p, int* span) {
+  return sw_bwd_pick<T, SwRows<T>::BWD>(p, [&](auto kernel, int R, int tensors, int es) {
+    SwGeom g;
+    int smem;
+    cudaError_t e = sw_geom(kernel, p, R, tensors, es, &g, &smem);
+    *span = g.span;
+    return e;
+  });
 }
 
 template <typename T>
 cudaError_t bwd_run(const SandwichParams& p, const SandwichBwdParams& q, int* err, cudaStream_t s) {
   cudaError_t e;
   if (sw_vectors(p, &q)) {
-    e = bwd_rows<T>(p, q, err, s);
-    if (e != cudaSuccess) return e;
+    e = sw_bwd_pick<T, SwRows<T>::BWD>(p, [&](auto kernel, int R, int tensors, int es) {
+      SwGeom g;
+      int smem;
+      cudaError_t e = sw_geom(kernel, p, R, tensors, es, &g, &smem);
+      if (e != cudaSuccess) return e;
+      if (g.span != q.rows_per_cta) return cudaErrorInvalidValue;  // the partial sums were laid out for this span
+      kernel<<<sw_blocks(p, g), g.tpg * g.groups, smem, s>>>(p, q, g, err);
+      return cudaGetLastError();
+    });
   } else {
     const int smem = 3 * p.D * (int)sizeof(float);
-    static int allowed = 46 * 1024;
-    e = sw_smem_limit(sandwich_bwd_any_kernel<T>, smem, &allowed);
+    e = cudaFuncSetAttribute(sandwich_bwd_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     sandwich_bwd_any_kernel<T><<<q.ctas, SW_THREADS, smem, s>>>(p, q);
     e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
   }
-  sandwich_reduce_kernel<T><<<dim3((p.D + 31) / 32, q.groups), dim3(32, RED_ROWS), 0, s>>>(p, q);
-  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  if (q.dw != nullptr || q.dpost_w != nullptr)
-    sandwich_weights_kernel<<<(p.D + 127) / 128, 128, 0, s>>>(p, q);
+  int wps = 1;
+  while (wps < RED_WARPS && wps * samples_of(p) < RED_WARPS) wps *= 2;
+  const int tiles = (p.D + 31) / 32;
+  sandwich_reduce_kernel<T><<<dim3(tiles, q.groups), 32 * RED_WARPS, 0, s>>>(p, q, wps);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || q.groups == 1 || (q.dw == nullptr && q.dpost_w == nullptr)) return e;
+  sandwich_weights_kernel<<<dim3(tiles, 2), 256, 0, s>>>(p, q);
   return cudaGetLastError();
 }
 
@@ -764,17 +807,19 @@ cudaError_t sandwich_fwd_launch(const SandwichParams& p, int elem, int* err, cud
   return cudaErrorInvalidValue;
 }
 
-void sandwich_bwd_plan(const SandwichParams& p, int elem, SandwichBwdParams* q) {
+cudaError_t sandwich_bwd_plan(const SandwichParams& p, int elem, SandwichBwdParams* q) {
   if (sw_vectors(p, q)) {
-    const int es = elem == ELEM_F32 ? 4 : 2;
-    const SwGeom g = sw_geom(p, sw_rows(p, es, BWD_R), 4, es, BWD_B);
-    q->rows_per_cta = g.span;
+    cudaError_t e = elem == ELEM_F32    ? bwd_span<float>(p, &q->rows_per_cta)
+                    : elem == ELEM_BF16 ? bwd_span<__nv_bfloat16>(p, &q->rows_per_cta)
+                                        : bwd_span<__half>(p, &q->rows_per_cta);
+    if (e != cudaSuccess) return e;
   } else {
     const int most = num_sms() * 4;
     q->rows_per_cta = std::max(1, (p.M + most - 1) / most);
   }
   q->ctas = (p.M + q->rows_per_cta - 1) / q->rows_per_cta;
-  q->groups = std::min(samples_of(p), 64);
+  q->groups = std::min((samples_of(p) + 255) / 256, 64);  // more than 256 samples: a block would walk them too long
+  return cudaSuccess;
 }
 
 cudaError_t sandwich_bwd_launch(const SandwichParams& p, const SandwichBwdParams& q, int elem, int* err,
