@@ -24,6 +24,7 @@ struct RouteParams {
   unsigned group_magic;    // ceil(2^22 / group_size): e / group_size == (e * magic) >> 22 for e < 512
   int sigmoid, renorm;
   float scale;
+  int vec, group_lanes;    // set by the launchers (route.cu)
 };
 cudaError_t route_fwd_launch(const RouteParams& p, int elem, cudaStream_t s);
 // dlogits [N, E] contiguous, in the logits' type; p.w and p.idx are read

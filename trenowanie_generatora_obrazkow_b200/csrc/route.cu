@@ -10,10 +10,11 @@
 //     softmax           dl_i = [i chosen] w_i dw_i - scale p_i m      sigmoid           dl_j = scale dw_j s_j'
 // s' = s (1 - s), S = sum of the chosen s. The selection and the bias take no gradient.
 //
-// L lanes hold one token, EPL consecutive experts each, so a row is read once with wide loads and every later step
-// works on registers. c is mapped to an unsigned key of the same order (NaN lowest, -0 as +0), and each of the k steps
-// is a maximum over the lane's keys and over the L lanes; the lowest lane that holds the maximum wins (its experts have
-// the lowest indices) and takes the expert out.
+// L lanes hold one token, EPL consecutive experts each, so a row is read once with wide loads and every later step works on
+// registers. c is mapped to an unsigned key of the same order (NaN lowest, -0 as +0). Each lane sorts its keys (stable, so
+// equal keys keep their index order), then each of the k steps takes the largest head of the L lists; the lowest lane
+// that holds it wins (its experts have the lowest indices) and drops its head. What the weights need beyond the choice
+// is computed for the k chosen alone, from logits read again (they are in the cache).
 #include "block_ops.h"
 #include "common.cuh"
 #include "vec.cuh"
@@ -60,11 +61,24 @@ __device__ __forceinline__ unsigned lanes_or(unsigned v) {
   return v;
 }
 
+// EPL logits from expert e0 on; vec: E, the row stride and the base allow 16-byte loads of 8 logits
 template <typename T, int EPL>
 __device__ __forceinline__ void load_logits(const RouteParams& p, long long n, int e0, float (&l)[EPL]) {
   const T* row = reinterpret_cast<const T*>(p.logits) + n * p.ld;
+  if (p.vec) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) l[j] = e0 + j < p.E ? to_f<T>(row[e0 + j]) : -INFINITY;
+    for (int v = 0; v < EPL; v += 8) {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = -INFINITY;
+      if (e0 + v < p.E) load_vec<T, 8>(row + e0 + v, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) l[v + j] = f[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) l[j] = e0 + j < p.E ? to_f<T>(row[e0 + j]) : -INFINITY;
+  }
 }
 
 // sigmoid from e = exp(-|l|) <= 1: no overflow, small scores keep their relative precision
@@ -76,18 +90,17 @@ template <typename T, int L, int EPL>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_fwd_kernel(RouteParams p) {
   constexpr int TOKENS = ROUTE_WARPS * 32 / L;  // per block
   extern __shared__ uint8_t route_smem[];
-  // chosen scores and experts [TOKENS][k]; with groups also the selection scores [TOKENS][E] and group scores
-  float* sc = reinterpret_cast<float*>(route_smem);
-  int* si = reinterpret_cast<int*>(sc + TOKENS * p.k);
+  // chosen experts [TOKENS][k]; for groups that do not fall on whole lanes also selection and group scores
+  int* si = reinterpret_cast<int*>(route_smem);
   float* cs = reinterpret_cast<float*>(si + TOKENS * p.k);
   float* gsc = cs + TOKENS * p.E;
   const int lane = lane_id(), li = lane % L, tok = threadIdx.x / L;
   const long long n = (long long)blockIdx.x * TOKENS + tok;
   const bool in = n < p.N;
   const int e0 = li * EPL;
-  float s[EPL];
+  const bool whole = !p.sigmoid && (p.bias != nullptr || !p.renorm);  // softmax: the sum over all experts matters
   unsigned key[EPL];
-  float z = 1.f;
+  float z = 1.f, mx = 0.f;
   {
     float l[EPL];
     if (in) {
@@ -96,38 +109,69 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_fwd_kernel(RouteParams
 #pragma unroll
       for (int j = 0; j < EPL; ++j) l[j] = 0.f;
     }
-    if (!p.sigmoid) {
-      float mx = -INFINITY;
+    if (whole) {
+      mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < EPL; ++j) mx = fmaxf(mx, l[j]);
       mx = lanes_max<L>(mx);
-      if (mx == -INFINITY) mx = 0.f;  // a token with every expert at -inf: all s are 0, and so are its weights
+      if (mx == -INFINITY) mx = 0.f;  // every expert at -inf: all s are 0, and so are the weights
       z = 0.f;
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) {
-        s[j] = e0 + j < p.E ? expf(l[j] - mx) : 0.f;
-        z += s[j];
-      }
+      for (int j = 0; j < EPL; ++j) z += e0 + j < p.E ? expf(l[j] - mx) : 0.f;
       z = fmaxf(lanes_sum<L>(z), 1e-20f);
-    } else {
+    }
+    if (p.sigmoid) {
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) {
-        s[j] = sigmoid_of(l[j], expf(-fabsf(l[j])));
-        l[j] = s[j];
+      for (int j = 0; j < EPL; ++j) l[j] = sigmoid_of(l[j], expf(-fabsf(l[j])));
+    }
+    if (p.bias != nullptr) {
+      if (p.vec) {
+#pragma unroll
+        for (int v = 0; v < EPL; v += 8) {
+          float f[8] = {};
+          if (e0 + v < p.E) load_vec<float, 8>(p.bias + e0 + v, f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) l[v + j] += f[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j)
+          if (e0 + j < p.E) l[j] += p.bias[e0 + j];
       }
     }
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      const int e = e0 + j;
-      if (p.bias != nullptr && e < p.E) l[j] += p.bias[e];
-      key[j] = e < p.E ? order_key(l[j]) : 0u;
-      if (p.groups > 1 && e < p.E) cs[tok * p.E + e] = l[j];
+      key[j] = e0 + j < p.E ? order_key(l[j]) : 0u;
+      if (p.groups > 1 && p.group_lanes == 0 && e0 + j < p.E) cs[tok * p.E + e0 + j] = l[j];
+    }
+    if (p.groups > 1 && p.group_lanes > 0) {
+      // a group is group_lanes whole lanes (a power of two): its two best scores by shuffles, then its rank
+      float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        b = fmaxf(b, fminf(a, l[j]));
+        a = fmaxf(a, l[j]);
+      }
+      for (int o = 1; o < p.group_lanes; o <<= 1) {
+        const float a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+        b = fmaxf(fminf(a, a2), fmaxf(b, b2));
+        a = fmaxf(a, a2);
+      }
+      const unsigned mine = order_key(p.sigmoid ? a + b : a);
+      const int g = li / p.group_lanes;
+      int above = 0;
+      for (int o = 0; o < p.groups; ++o) {
+        const unsigned other = __shfl_sync(0xffffffffu, mine, o * p.group_lanes, L);
+        above += (other > mine || (other == mine && o < g)) ? 1 : 0;
+      }
+      if (above >= p.top_groups)
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) key[j] = 0u;
     }
   }
-  if (p.groups > 1) {
+  if (p.groups > 1 && p.group_lanes == 0) {
     __syncwarp();
-    // lane g scans group g
-    for (int g = li; g < p.groups; g += L) {
+    for (int g = li; g < p.groups; g += L) {  // lane g scans group g
       const float* c = cs + tok * p.E + g * p.group_size;
       float a = -INFINITY, b = -INFINITY;
       for (int i = 0; i < p.group_size; ++i) {
@@ -155,67 +199,120 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_fwd_kernel(RouteParams
       if (!((kept >> (g & 31)) & 1u)) key[j] = 0u;
     }
   }
-  float chosen = 0.f;
+  // descending and stable: neighbours swap only when the later key is larger (EPL rounds of disjoint neighbours)
+  int id[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) id[j] = e0 + j;
+#pragma unroll
+  for (int round = 0; round < EPL; ++round)
+#pragma unroll
+    for (int j = round & 1; j + 1 < EPL; j += 2) {
+      const unsigned a = key[j], b = key[j + 1];
+      const bool swap = b > a;
+      const int ia = id[j], ib = id[j + 1];
+      key[j] = max(a, b);
+      key[j + 1] = min(a, b);
+      id[j] = swap ? ib : ia;
+      id[j + 1] = swap ? ia : ib;
+    }
   for (int r = 0; r < p.k; ++r) {
-    unsigned m = 0;
+    bool win = true;
+    if constexpr (L > 1) {
+      const unsigned gm = lanes_max<L>(key[0]);
+      unsigned who = __ballot_sync(0xffffffffu, key[0] == gm);
+      if constexpr (L < 32) who = (who >> (lane - li)) & ((1u << L) - 1u);
+      win = __ffs(who) - 1 == li;
+    }
+    if (win) {
+      si[tok * p.k + r] = id[0];
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) m = max(m, key[j]);
-    const unsigned gm = lanes_max<L>(m);
-    unsigned who = __ballot_sync(0xffffffffu, m == gm);
-    if constexpr (L < 32) who = (who >> (lane - li)) & ((1u << L) - 1u);
-    if (__ffs(who) - 1 == li) {
-      bool open = true;
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) {
-        if (open && key[j] == gm) {
-          open = false;
-          key[j] = 0u;
-          chosen += s[j];
-          sc[tok * p.k + r] = s[j];
-          si[tok * p.k + r] = e0 + j;
-        }
-      }
+      for (int j = 0; j + 1 < EPL; ++j) key[j] = key[j + 1], id[j] = id[j + 1];
+      key[EPL - 1] = 0u;
     }
   }
-  const float total = lanes_sum<L>(chosen);
   __syncwarp();
+  // the chosen experts' scores, L at a time; a token's lanes stay together in the sums (the loop count is the block's)
+  const T* row = reinterpret_cast<const T*>(p.logits) + (in ? n : 0) * p.ld;
+  if (!p.sigmoid && !whole) {
+    mx = to_f<T>(row[si[tok * p.k]]);  // the best of all (its group is the best group, and no bias moves the order)
+    if (mx == -INFINITY) mx = 0.f;
+  }
+  auto score = [&](int r) {
+    const float l = to_f<T>(row[si[tok * p.k + r]]);
+    return p.sigmoid ? sigmoid_of(l, expf(-fabsf(l))) : expf(l - mx);
+  };
+  float chosen = 0.f, mine = 0.f;
+  for (int r = li; r < p.k; r += L) {
+    mine = score(r);
+    chosen += mine;
+  }
+  chosen = lanes_sum<L>(chosen);
   if (!in) return;
   const bool ok = p.valid == nullptr || p.valid[n];
-  const float den = p.renorm ? total + 1e-20f * z : z;
+  const float den = p.renorm ? chosen + 1e-20f * z : z;
   for (int r = li; r < p.k; r += L) {
-    p.w[n * p.k + r] = ok ? sc[tok * p.k + r] / den * p.scale : 0.f;
+    const float s = p.k <= L ? mine : score(r);
+    p.w[n * p.k + r] = ok ? s / den * p.scale : 0.f;
     p.idx[n * p.k + r] = ok ? si[tok * p.k + r] : -1;
   }
 }
 
+// The chosen experts' values go into a zeroed row in shared memory, from which the lanes write the dense row.
 template <typename T, int L, int EPL>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_bwd_kernel(RouteParams p, const float* __restrict__ dw,
                                                                      T* __restrict__ dlogits) {
-  constexpr int TOKENS = ROUTE_WARPS * 32 / L;
-  const int li = lane_id() % L;
-  const long long n = (long long)blockIdx.x * TOKENS + threadIdx.x / L;
+  constexpr int TOKENS = ROUTE_WARPS * 32 / L, PITCH = L * EPL;
+  __shared__ __align__(16) float rows[TOKENS * PITCH];
+  const int li = lane_id() % L, tok = threadIdx.x / L;
+  const long long n = (long long)blockIdx.x * TOKENS + tok;
   const bool in = n < p.N;
   const int e0 = li * EPL;
-  const T* row = reinterpret_cast<const T*>(p.logits) + (in ? n : 0) * p.ld;
-  const float* w = p.w + (in ? n : 0) * p.k;
-  const float* g = dw + (in ? n : 0) * p.k;
-  const int* idx = p.idx + (in ? n : 0) * p.k;
-  float d[EPL];
-#pragma unroll
-  for (int j = 0; j < EPL; ++j) d[j] = 0.f;
+  const long long at = in ? n : 0;
+  const T* row = reinterpret_cast<const T*>(p.logits) + at * p.ld;
+  const float *w = p.w + at * p.k, *g = dw + at * p.k;
+  const int* idx = p.idx + at * p.k;
+  float* d = rows + tok * PITCH;
   const bool live = in && idx[0] >= 0;
-  float m = 0.f, total = 1e-20f;
-  if (live) {
-    for (int r = 0; r < p.k; ++r) {
-      m += w[r] * g[r];
-      if (p.sigmoid && p.renorm) {
-        const float l = to_f<T>(row[idx[r]]);
-        total += sigmoid_of(l, expf(-fabsf(l)));
-      }
+#pragma unroll
+  for (int j = 0; j < EPL; j += 4) *reinterpret_cast<float4*>(d + e0 + j) = make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncwarp();
+  // m = sum of r dw and S = sum of the chosen s; with k <= L each lane keeps what it read of its choice
+  int e = 0;
+  float we = 0.f, ge = 0.f, se = 0.f, de = 0.f;  // weight, its gradient, score s and s' of this lane's choice
+  auto choice = [&](int r) {
+    e = idx[r];
+    we = w[r];
+    ge = g[r];
+    if (p.sigmoid) {
+      const float l = to_f<T>(row[e]);
+      const float x = expf(-fabsf(l)), q = 1.f / (1.f + x);
+      se = (l >= 0.f ? 1.f : x) * q;
+      de = x * q * q;
     }
-    m /= p.scale;
+  };
+  float m = 0.f, total = 0.f;
+  if (live)
+    for (int r = li; r < p.k; r += L) {
+      choice(r);
+      m = fmaf(we, ge, m);
+      total += se;
+    }
+  m = lanes_sum<L>(m) / p.scale;
+  if (p.sigmoid && p.renorm) total = lanes_sum<L>(total) + 1e-20f;
+  if (live)
+    for (int r = li; r < p.k; r += L) {
+      if (p.k > L) choice(r);
+      const float up = p.renorm ? ge - m : ge;
+      d[e] = p.sigmoid ? p.scale * up * de / (p.renorm ? total : 1.f) : we * up;
+    }
+  __syncwarp();
+  float v[EPL];
+#pragma unroll
+  for (int j = 0; j < EPL; j += 4) {
+    const float4 t = *reinterpret_cast<const float4*>(d + e0 + j);
+    v[j] = t.x, v[j + 1] = t.y, v[j + 2] = t.z, v[j + 3] = t.w;
   }
-  if (!p.sigmoid && !p.renorm) {  // dense: every expert's probability is needed (warp-uniform branch)
+  if (!p.sigmoid && !p.renorm) {  // every expert's probability takes part
     float l[EPL];
     float mx = -INFINITY;
     if (live) load_logits<T, EPL>(p, n, e0, l);
@@ -234,44 +331,40 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_bwd_kernel(RouteParams
     }
     z = fmaxf(lanes_sum<L>(z), 1e-20f);
     if (live) {
+      const float f = p.scale * m / z;
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) d[j] = -p.scale * (l[j] / z) * m;
-    }
-  }
-  if (live) {
-    for (int r = 0; r < p.k; ++r) {
-      const int e = idx[r];
-      float v;
-      if (p.sigmoid) {
-        const float l = to_f<T>(row[e]);
-        const float x = expf(-fabsf(l)), q = 1.f + x;
-        const float ds = x / (q * q);
-        v = p.renorm ? p.scale * (g[r] - m) / total * ds : p.scale * g[r] * ds;
-      } else {
-        v = p.renorm ? w[r] * (g[r] - m) : w[r] * g[r];
-      }
-#pragma unroll
-      for (int j = 0; j < EPL; ++j)
-        if (e == e0 + j) d[j] += v;
+      for (int j = 0; j < EPL; ++j) v[j] = fmaf(-f, l[j], v[j]);
     }
   }
   if (!in) return;
   T* out = dlogits + n * p.E;
+  if (p.vec) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j)
-    if (e0 + j < p.E) out[e0 + j] = from_f<T>(d[j]);
+    for (int j = 0; j < EPL; j += 8)
+      if (e0 + j < p.E) store_vec<T, 8>(out + e0 + j, *reinterpret_cast<const float(*)[8]>(&v[j]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j)
+      if (e0 + j < p.E) out[e0 + j] = from_f<T>(v[j]);
+  }
 }
 
 namespace {
 
 template <typename T, int L, int EPL>
-cudaError_t route_run(const RouteParams& p, const float* dw, void* dlogits, cudaStream_t s) {
+cudaError_t route_run(RouteParams p, const float* dw, void* dlogits, cudaStream_t s) {
   constexpr int TOKENS = ROUTE_WARPS * 32 / L;
+  // whole 16-byte vectors of 8 logits, in rows and outputs; groups of a power of two of whole lanes
+  p.vec = p.E % 8 == 0 && p.ld % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.logits) | reinterpret_cast<uintptr_t>(p.bias) |
+                                             reinterpret_cast<uintptr_t>(dlogits)) & 15) == 0;
+  const int gl = p.group_size / EPL;
+  p.group_lanes = p.group_size % EPL == 0 && (gl & (gl - 1)) == 0 ? gl : 0;
   const unsigned grid = (unsigned)((p.N + TOKENS - 1) / TOKENS);
   if (dlogits != nullptr) {
     route_bwd_kernel<T, L, EPL><<<grid, ROUTE_WARPS * 32, 0, s>>>(p, dw, static_cast<T*>(dlogits));
   } else {
-    const size_t smem = (size_t)TOKENS * 4 * (2 * p.k + (p.groups > 1 ? p.E + kRouteMaxGroups : 0));
+    const bool scan = p.groups > 1 && p.group_lanes == 0;
+    const size_t smem = (size_t)TOKENS * 4 * (p.k + (scan ? p.E + kRouteMaxGroups : 0));
     route_fwd_kernel<T, L, EPL><<<grid, ROUTE_WARPS * 32, smem, s>>>(p);
   }
   return cudaGetLastError();
