@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "block_ops.h"
@@ -267,10 +268,10 @@ std::vector<at::Tensor> sandwich_fwd(at::Tensor x, at::Tensor y, OptT gate, OptT
   return {x_new, h, ry, rx};
 }
 
-// -> dx, dy, dgate, dshift, dscale; dpost_w and dw are accumulated (+=)
+// -> dx, dy, dgate, dshift, dscale; dpost_w and dw are added to (accumulate) or written
 std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Tensor y, OptT gate, OptT post_w, OptT w,
                                      OptT shift, OptT scale, OptT ry, OptT rx, OptT dpost_w, OptT dw, double res_scale,
-                                     double eps, at::Tensor err) {
+                                     double eps, at::Tensor err, bool add_post_w, bool add_w) {
   SandwichParams p = sandwich_params(x, y, gate, post_w, w, shift, scale, res_scale, eps);
   const c10::cuda::CUDAGuard guard(x.device());
   p.rstd_y = acc_f32(ry, p.M, x, "sandwich_bwd: ry");
@@ -303,7 +304,11 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
   }
   q.dpost_w = acc_f32(dpost_w, D, x, "sandwich_bwd: dpost_w");
   q.dw = acc_f32(dw, D, x, "sandwich_bwd: dw");
+  q.add_post_w = add_post_w;
+  q.add_w = add_w;
   if (p.M == 0) {
+    if (q.dpost_w != nullptr && !add_post_w) dpost_w->zero_();
+    if (q.dw != nullptr && !add_w) dw->zero_();
     if (dgate.defined()) dgate.zero_();
     if (dshift.defined()) dshift.zero_(), dscale.zero_();
     return {dx, dy, dgate, dshift, dscale};
@@ -374,10 +379,11 @@ std::tuple<at::Tensor, at::Tensor> rope_axes_fwd(at::Tensor q, at::Tensor k, at:
   return {qo, ko};
 }
 
-// -> dq_in, dk_in; dq_w and dk_w (both or neither) are accumulated (+=)
+// -> dq_in, dk_in; dq_w and dk_w (both or neither) are added to (accumulate) or written
 std::tuple<at::Tensor, at::Tensor> rope_axes_bwd(at::Tensor dq, at::Tensor dk, at::Tensor q, at::Tensor k,
                                                  at::Tensor pos, at::Tensor freq, at::Tensor axis, OptT q_w, OptT k_w,
-                                                 OptT dq_w, OptT dk_w, bool interleaved, double eps) {
+                                                 OptT dq_w, OptT dk_w, bool interleaved, double eps, bool add_q_w,
+                                                 bool add_k_w) {
   RopeAxesParams p = rope_params(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
   const c10::cuda::CUDAGuard guard(q.device());
   auto grad_ok = [&](const at::Tensor& g, const at::Tensor& t) {
@@ -390,29 +396,285 @@ std::tuple<at::Tensor, at::Tensor> rope_axes_bwd(at::Tensor dq, at::Tensor dk, a
   float* gk = acc_f32(dk_w, p.hd, q, "rope_axes_bwd: dk_w");
   TORCH_CHECK((gq == nullptr) == (gk == nullptr) && (gq == nullptr || p.q_w != nullptr),
               "rope_axes_bwd: dq_w and dk_w both or neither, with the norm weights");
-  if (p.M == 0) return {dqi, dki};
+  if (p.M == 0) {
+    if (gq != nullptr && !add_q_w) dq_w->zero_();
+    if (gk != nullptr && !add_k_w) dk_w->zero_();
+    return {dqi, dki};
+  }
   if (gq != nullptr)
     partial = at::empty({rope_axes_bwd_ctas(), 2, p.hd}, q.options().dtype(at::kFloat));
   BLOCK_LAUNCH(rope_axes_bwd_launch(p, dq.data_ptr(), dk.data_ptr(), dqi.data_ptr(), dki.data_ptr(),
-                                    gq != nullptr ? partial.data_ptr<float>() : nullptr, gq, gk,
+                                    gq != nullptr ? partial.data_ptr<float>() : nullptr, gq, gk, add_q_w, add_k_w,
                                     elem_of(q, "rope_axes_bwd"), at::cuda::getCurrentCUDAStream()),
                gq != nullptr ? 2 : 1);
   return {dqi, dki};
 }
 
+// ------------------------------------------------------------------------------------------------------ autograd
+// The differentiable forms are C++ autograd functions: a small training step is bound by the host, and a Python
+// autograd.Function costs more than the kernels it launches (forward + backward of 32768 x 8 routing: 79 us with it).
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+at::Tensor or_undefined(const OptT& t) { return given(t) ? *t : at::Tensor(); }
+OptT opt(const at::Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+
+// Python's grad-ready hooks (ops/fused.py): called with the parameter after its gradient was accumulated in place
+// (never freed: the callback must not outlive the interpreter that would have to release it)
+struct GradReady {
+  std::atomic<bool> on{false};
+  py::object notify;
+};
+GradReady& grad_ready() {
+  static GradReady* r = new GradReady;
+  return *r;
+}
+void set_grad_ready(bool on, py::object notify) {
+  grad_ready().notify = std::move(notify);
+  grad_ready().on = on;
+}
+
+// Where the backward puts the gradient of a small fp32 weight: in place into the leaf's .grad (no temporary, no
+// accumulation kernel), or a temporary that autograd takes.
+struct WeightGrad {
+  at::Tensor w, g;
+  bool direct = false, add = false;
+  explicit WeightGrad(const at::Tensor& weight) : w(weight) {
+    if (!w.defined() || !w.requires_grad()) return;
+    if (w.is_leaf() && w.scalar_type() == at::kFloat) {
+      at::Tensor& have = w.mutable_grad();
+      if (!have.defined()) {
+        have = at::empty_like(w);
+        direct = true;
+      } else if (have.scalar_type() == at::kFloat && have.is_contiguous() && have.device() == w.device()) {
+        direct = add = true;
+      }
+      if (direct) g = have.detach();
+    }
+    if (!direct) g = at::empty_like(w);
+  }
+  at::Tensor done() const {  // what autograd still has to add
+    if (!direct) return g;
+    if (grad_ready().on) {
+      py::gil_scoped_acquire gil;
+      grad_ready().notify(w);
+    }
+    return at::Tensor();
+  }
+};
+
+struct RouteFn : public torch::autograd::Function<RouteFn> {
+  static variable_list forward(AutogradContext* ctx, at::Tensor logits, OptT bias, OptT valid, int64_t k,
+                               bool sigmoid, int64_t groups, int64_t top_groups, bool renorm, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [w, idx] = route_fwd(logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale);
+    ctx->save_for_backward({logits, w, idx});
+    ctx->saved_data["sigmoid"] = sigmoid;
+    ctx->saved_data["renorm"] = renorm;
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({idx});
+    return {w, idx};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    at::Tensor d = route_bwd(saved[0], saved[1], saved[2], grads[0].contiguous(), ctx->saved_data["sigmoid"].toBool(),
+                             ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
+    variable_list out(9);
+    out[0] = d;
+    return out;
+  }
+};
+std::tuple<at::Tensor, at::Tensor> route_experts(at::Tensor logits, OptT bias, OptT valid, int64_t k, bool sigmoid,
+                                                 int64_t groups, int64_t top_groups, bool renorm, double scale) {
+  if (logits.dim() == 2 && logits.size(1) > 1 && logits.stride(1) != 1) logits = logits.contiguous();
+  if (!wants_grad({&logits})) return route_fwd(logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale);
+  auto out = RouteFn::apply(logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale);
+  return {out[0], out[1]};
+}
+
+struct DispatchFn : public torch::autograd::Function<DispatchFn> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor slot, at::Tensor offsets, at::Tensor counts,
+                            int64_t capacity, int64_t rows) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({slot, offsets, counts});
+    ctx->saved_data["capacity"] = capacity;
+    return expert_dispatch(x, slot, offsets, counts, capacity, rows);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    variable_list out(6);
+    out[0] = expert_combine(grads[0].contiguous(), OptT(), s[0], s[1], s[2], ctx->saved_data["capacity"].toInt());
+    return out;
+  }
+};
+at::Tensor dispatch_rows(at::Tensor x, at::Tensor slot, at::Tensor offsets, at::Tensor counts, int64_t capacity,
+                         int64_t rows) {
+  if (x.dim() == 2 && x.size(1) > 1 && x.stride(1) != 1) x = x.contiguous();
+  if (!wants_grad({&x})) return expert_dispatch(x, slot, offsets, counts, capacity, rows);
+  return DispatchFn::apply(x, slot, offsets, counts, capacity, rows);
+}
+
+struct CombineFn : public torch::autograd::Function<CombineFn> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor y, at::Tensor w, at::Tensor slot, at::Tensor offsets,
+                            at::Tensor counts, int64_t capacity) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({y, w, slot, offsets, counts});
+    ctx->saved_data["capacity"] = capacity;
+    return expert_combine(y, w, slot, offsets, counts, capacity);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    at::Tensor g = grads[0];
+    if (g.size(1) > 1 && g.stride(1) != 1) g = g.contiguous();
+    auto [dy, dw] = expert_combine_bwd(s[0], s[1], g, s[2], s[3], s[4], ctx->saved_data["capacity"].toInt());
+    variable_list out(6);
+    out[0] = dy;
+    out[1] = dw;
+    return out;
+  }
+};
+at::Tensor combine_rows(at::Tensor y, at::Tensor w, at::Tensor slot, at::Tensor offsets, at::Tensor counts,
+                        int64_t capacity) {
+  y = y.contiguous();
+  w = w.to(at::kFloat).contiguous();
+  if (!wants_grad({&y, &w})) return expert_combine(y, w, slot, offsets, counts, capacity);
+  return CombineFn::apply(y, w, slot, offsets, counts, capacity);
+}
+
+struct SandwichFn : public torch::autograd::Function<SandwichFn> {
+  static variable_list forward(AutogradContext* ctx, at::Tensor x, at::Tensor y, OptT gate, OptT post_w, OptT w,
+                               OptT shift, OptT scale, double res_scale, double eps, at::Tensor err) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto r = sandwich_fwd(x, y, gate, post_w, w, shift, scale, res_scale, eps, err);
+    ctx->save_for_backward({x, y, or_undefined(gate), or_undefined(post_w), or_undefined(w), or_undefined(shift),
+                            or_undefined(scale), r[2], r[3]});
+    ctx->saved_data["err"] = err;
+    ctx->saved_data["res_scale"] = res_scale;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    if (!r[1].defined()) return {r[0]};
+    return {r[0], r[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const at::Tensor dx_new = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
+    const at::Tensor dh = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
+    const WeightGrad gp(s[3]), gw(s[4]);
+    auto r = sandwich_bwd(opt(dx_new), opt(dh), s[0], s[1], opt(s[2]), opt(s[3]), opt(s[4]), opt(s[5]), opt(s[6]),
+                          opt(s[7]), opt(s[8]), opt(gp.g), opt(gw.g), ctx->saved_data["res_scale"].toDouble(),
+                          ctx->saved_data["eps"].toDouble(), ctx->saved_data["err"].toTensor(), gp.add, gw.add);
+    variable_list out(10);
+    out[0] = r[0];
+    out[1] = r[1];
+    out[2] = r[2];
+    out[3] = gp.done();
+    out[4] = gw.done();
+    out[5] = r[3];
+    out[6] = r[4];
+    return out;
+  }
+};
+std::tuple<at::Tensor, OptT> sandwich_norm(at::Tensor x, at::Tensor y, OptT gate, OptT post_w, OptT w, OptT shift,
+                                           OptT scale, double res_scale, double eps, at::Tensor err) {
+  x = x.contiguous();
+  y = y.contiguous();
+  if (given(shift) && given(scale) && shift->strides() != scale->strides()) {
+    shift = shift->contiguous();
+    scale = scale->contiguous();
+  }
+  const at::Tensor g = or_undefined(gate), p = or_undefined(post_w), ww = or_undefined(w), sh = or_undefined(shift),
+                   sc = or_undefined(scale);
+  if (!wants_grad({&x, &y, &g, &p, &ww, &sh, &sc})) {
+    auto r = sandwich_fwd(x, y, gate, post_w, w, shift, scale, res_scale, eps, err);
+    return {r[0], opt(r[1])};
+  }
+  auto out = SandwichFn::apply(x, y, gate, post_w, w, shift, scale, res_scale, eps, err);
+  return {out[0], out.size() > 1 ? OptT(out[1]) : OptT()};
+}
+
+// [B, T, H, d] -> [B T, H, d], in place when the tokens are evenly strided and a token's heads are contiguous
+at::Tensor token_rows(const at::Tensor& t) {
+  const int64_t B = t.size(0), T = t.size(1), H = t.size(2), d = t.size(3);
+  const bool even = (d <= 1 || t.stride(3) == 1) && (H <= 1 || t.stride(2) == d) &&
+                    (B <= 1 || T <= 1 || t.stride(0) == T * t.stride(1));
+  if (!even) return t.contiguous().view({B * T, H, d});
+  return t.as_strided({B * T, H, d}, {T > 1 || B <= 1 ? t.stride(1) : t.stride(0), d, 1});
+}
+struct RopeAxesFn : public torch::autograd::Function<RopeAxesFn> {
+  static variable_list forward(AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor pos, at::Tensor freq,
+                               at::Tensor axis, OptT q_w, OptT k_w, bool interleaved, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [qo, ko] = rope_axes_fwd(token_rows(q), token_rows(k), pos, freq, axis, q_w, k_w, interleaved, eps);
+    ctx->save_for_backward({q, k, pos, freq, axis, or_undefined(q_w), or_undefined(k_w)});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["eps"] = eps;
+    return {qo.view(q.sizes()), ko.view(k.sizes())};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const WeightGrad gq(s[5]), gk(s[6]);
+    // the two weights' sums come together: one that needs no gradient gets a scratch row
+    at::Tensor wq = gq.g, wk = gk.g;
+    if (wq.defined() != wk.defined()) (wq.defined() ? wk : wq) = at::empty_like(wq.defined() ? wq : wk);
+    auto [dq, dk] = rope_axes_bwd(grads[0].contiguous().flatten(0, 1), grads[1].contiguous().flatten(0, 1),
+                                  token_rows(s[0]), token_rows(s[1]), s[2], s[3], s[4], opt(s[5]), opt(s[6]), opt(wq),
+                                  opt(wk), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(),
+                                  gq.add, gk.add);
+    variable_list out(9);
+    out[0] = dq.view(s[0].sizes());
+    out[1] = dk.view(s[1].sizes());
+    out[5] = gq.done();
+    out[6] = gk.done();
+    return out;
+  }
+};
+std::tuple<at::Tensor, at::Tensor> rope_axes(at::Tensor q, at::Tensor k, at::Tensor pos, at::Tensor freq,
+                                             at::Tensor axis, OptT q_w, OptT k_w, bool interleaved, double eps) {
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && pos.dim() == 3 && pos.size(0) == q.size(0) && pos.size(1) == q.size(1) &&
+                  k.size(0) == q.size(0) && k.size(1) == q.size(1),
+              "rope_axes: q [B, T, Hq, d], k [B, T, Hkv, d], pos [B, T, axes]");
+  pos = pos.to(pos.is_floating_point() ? at::kFloat : at::kInt).contiguous().view({q.size(0) * q.size(1), pos.size(2)});
+  const at::Tensor wq = or_undefined(q_w), wk = or_undefined(k_w);
+  if (!wants_grad({&q, &k, &wq, &wk})) {
+    auto [qo, ko] = rope_axes_fwd(token_rows(q), token_rows(k), pos, freq, axis, q_w, k_w, interleaved, eps);
+    return {qo.view(q.sizes()), ko.view(k.sizes())};
+  }
+  auto out = RopeAxesFn::apply(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
+  return {out[0], out[1]};
+}
+
 }  // namespace
 
 void bind_block_ops(pybind11::module_& m) {
-  m.def("route_fwd", &route_fwd, "expert scores, group-limited top-k and weights of every token");
+  m.def("route_experts", &route_experts, "expert scores, group-limited top-k and weights of every token");
+  m.def("route_fwd", &route_fwd, "route_experts without autograd");
   m.def("route_bwd", &route_bwd, "gradient of the chosen experts' weights to the router's logits");
   m.def("expert_plan", &expert_plan, "stable row of every assignment in expert order, offsets and counts");
-  m.def("expert_dispatch", &expert_dispatch, "token rows into expert order");
-  m.def("expert_combine", &expert_combine, "weighted sum of a token's rows from expert order");
-  m.def("expert_combine_bwd", &expert_combine_bwd, "gradient of expert_combine to the rows and the weights");
-  m.def("sandwich_fwd", &sandwich_fwd, "x + r gate rmsnorm(y) post_w, then rmsnorm, w, scale and shift");
-  m.def("sandwich_bwd", &sandwich_bwd, "backward of sandwich_fwd");
-  m.def("rope_axes_fwd", &rope_axes_fwd, "q/k RMSNorm and rotary positions with several axes");
-  m.def("rope_axes_bwd", &rope_axes_bwd, "backward of rope_axes_fwd");
+  m.def("dispatch_rows", &dispatch_rows, "token rows into expert order");
+  m.def("expert_dispatch", &expert_dispatch, "dispatch_rows without autograd");
+  m.def("combine_rows", &combine_rows, "weighted sum of a token's rows from expert order");
+  m.def("expert_combine", &expert_combine, "combine_rows without autograd");
+  m.def("expert_combine_bwd", &expert_combine_bwd, "gradient of combine_rows to the rows and the weights");
+  m.def("sandwich_norm", &sandwich_norm, "x + r gate rmsnorm(y) post_w, then rmsnorm, w, scale and shift");
+  m.def("sandwich_fwd", &sandwich_fwd, "sandwich_norm without autograd, with its statistics");
+  m.def("sandwich_bwd", &sandwich_bwd, "backward of sandwich_fwd", py::arg("dx_new"), py::arg("dh"), py::arg("x"),
+        py::arg("y"), py::arg("gate"), py::arg("post_w"), py::arg("w"), py::arg("shift"), py::arg("scale"),
+        py::arg("ry"), py::arg("rx"), py::arg("dpost_w"), py::arg("dw"), py::arg("res_scale"), py::arg("eps"),
+        py::arg("err"), py::arg("add_post_w") = true, py::arg("add_w") = true);
+  m.def("rope_axes", &rope_axes, "q/k RMSNorm and rotary positions with several axes");
+  m.def("rope_axes_fwd", &rope_axes_fwd, "rope_axes of token rows without autograd");
+  m.def("rope_axes_bwd", &rope_axes_bwd, "backward of rope_axes_fwd", py::arg("dq"), py::arg("dk"), py::arg("q"),
+        py::arg("k"), py::arg("pos"), py::arg("freq"), py::arg("axis"), py::arg("q_w"), py::arg("k_w"),
+        py::arg("dq_w"), py::arg("dk_w"), py::arg("interleaved"), py::arg("eps"), py::arg("add_q_w") = true,
+        py::arg("add_k_w") = true);
+  m.def("set_grad_ready", &set_grad_ready, "callback for gradients that a backward accumulated in place");
 }
 
 }  // namespace tgo

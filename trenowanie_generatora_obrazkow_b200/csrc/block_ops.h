@@ -83,8 +83,9 @@ struct SandwichBwdParams {
   void* dgate;           // [B, D] contiguous, in x's type, or null
   void* dshift;
   void* dscale;
-  float* dpost_w;        // [D], accumulated
-  float* dw;             // [D], accumulated
+  float* dpost_w;        // [D], added to or written, or null
+  float* dw;
+  bool add_post_w, add_w;
   int ctas, rows_per_cta, groups;  // units of rows (see sandwich.cu), groups of samples of the reduction
 };
 // err: device error word of the kernels' bounded waits
@@ -110,10 +111,11 @@ struct RopeAxesParams {
   int M, axes, hq, hkv, hd, rot, interleaved;
 };
 cudaError_t rope_axes_fwd_launch(const RopeAxesParams& p, int elem, cudaStream_t s);
-// dq / dk [M, h, hd] contiguous -> dq_in / dk_in [M, h, hd] contiguous; dq_w / dk_w [hd] accumulated through partials
+// dq / dk [M, h, hd] contiguous -> dq_in / dk_in [M, h, hd] contiguous; dq_w / dk_w [hd] added to or written through partials
 // [rope_axes_bwd_ctas()][2][hd] (the most CTAs of any launch)
 int rope_axes_bwd_ctas();
 cudaError_t rope_axes_bwd_launch(const RopeAxesParams& p, const void* dq, const void* dk, void* dq_in, void* dk_in,
-                                 float* partial, float* dq_w, float* dk_w, int elem, cudaStream_t s);
+                                 float* partial, float* dq_w, float* dk_w, bool add_q_w, bool add_k_w, int elem,
+                                 cudaStream_t s);
 
 }  // namespace tgo

@@ -405,9 +405,9 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) rope_axes_bwd_any_kernel(Rope
   }
 }
 
-// dq_w / dk_w += the CTAs' partial sums, in a fixed order
+// dq_w / dk_w (+)= the CTAs' partial sums, in a fixed order
 __global__ void rope_weights_kernel(const float* __restrict__ partial, int ctas, int hd, float* __restrict__ dq_w,
-                                    float* __restrict__ dk_w) {
+                                    float* __restrict__ dk_w, bool add_q, bool add_k) {
   __shared__ float part[8][32];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
@@ -417,8 +417,8 @@ __global__ void rope_weights_kernel(const float* __restrict__ partial, int ctas,
   __syncthreads();
   if (threadIdx.y != 0 || c >= 2 * hd) return;
   for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
-  if (c < hd) dq_w[c] += s;
-  else dk_w[c - hd] += s;
+  float* dst = c < hd ? dq_w + c : dk_w + (c - hd);
+  *dst = (c < hd ? add_q : add_k) ? *dst + s : s;
 }
 
 namespace {
@@ -469,7 +469,8 @@ cudaError_t rope_fwd_run(const RopeAxesParams& p, int elem, cudaStream_t s) {
 
 template <typename T>
 cudaError_t rope_bwd_run(const RopeAxesParams& p, const void* dq, const void* dk, void* dq_in, void* dk_in,
-                         float* partial, float* dq_w, float* dk_w, int elem, cudaStream_t s) {
+                         float* partial, float* dq_w, float* dk_w, bool add_q_w, bool add_k_w, int elem,
+                                 cudaStream_t s) {
   const T *gq = static_cast<const T*>(dq), *gk = static_cast<const T*>(dk);
   T *iq = static_cast<T*>(dq_in), *ik = static_cast<T*>(dk_in);
   const bool vec = rope_vectors(p, elem, {dq, dk, dq_in, dk_in});
@@ -483,7 +484,7 @@ cudaError_t rope_bwd_run(const RopeAxesParams& p, const void* dq, const void* dk
   else rope_bwd_vec<T, 32>(p, gq, gk, iq, ik, partial, grid, s);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || partial == nullptr) return e;
-  rope_weights_kernel<<<(2 * p.hd + 31) / 32, dim3(32, 8), 0, s>>>(partial, grid, p.hd, dq_w, dk_w);
+  rope_weights_kernel<<<(2 * p.hd + 31) / 32, dim3(32, 8), 0, s>>>(partial, grid, p.hd, dq_w, dk_w, add_q_w, add_k_w);
   return cudaGetLastError();
 }
 
@@ -502,12 +503,13 @@ cudaError_t rope_axes_fwd_launch(const RopeAxesParams& p, int elem, cudaStream_t
 int rope_axes_bwd_ctas() { return num_sms() * 8; }
 
 cudaError_t rope_axes_bwd_launch(const RopeAxesParams& p, const void* dq, const void* dk, void* dq_in, void* dk_in,
-                                 float* partial, float* dq_w, float* dk_w, int elem, cudaStream_t s) {
+                                 float* partial, float* dq_w, float* dk_w, bool add_q_w, bool add_k_w, int elem,
+                                 cudaStream_t s) {
   if (p.M <= 0) return cudaSuccess;
   switch (elem) {
-    case ELEM_BF16: return rope_bwd_run<__nv_bfloat16>(p, dq, dk, dq_in, dk_in, partial, dq_w, dk_w, elem, s);
-    case ELEM_F16: return rope_bwd_run<__half>(p, dq, dk, dq_in, dk_in, partial, dq_w, dk_w, elem, s);
-    case ELEM_F32: return rope_bwd_run<float>(p, dq, dk, dq_in, dk_in, partial, dq_w, dk_w, elem, s);
+    case ELEM_BF16: return rope_bwd_run<__nv_bfloat16>(p, dq, dk, dq_in, dk_in, partial, dq_w, dk_w, add_q_w, add_k_w, elem, s);
+    case ELEM_F16: return rope_bwd_run<__half>(p, dq, dk, dq_in, dk_in, partial, dq_w, dk_w, add_q_w, add_k_w, elem, s);
+    case ELEM_F32: return rope_bwd_run<float>(p, dq, dk, dq_in, dk_in, partial, dq_w, dk_w, add_q_w, add_k_w, elem, s);
   }
   return cudaErrorInvalidValue;
 }

@@ -639,11 +639,11 @@ __global__ void __launch_bounds__(32 * RED_WARPS) sandwich_reduce_kernel(Sandwic
     for (int k = 0; k < RED_WARPS; ++k) t += part[k][warp][lane];
     float* dst = warp == 0 ? q.dw : q.dpost_w;
     if (gridDim.y > 1) q.wpart[((long long)blockIdx.y * 2 + warp) * p.D + c] = t;
-    else if (dst != nullptr) dst[c] += t;
+    else if (dst != nullptr) dst[c] = (warp == 0 ? q.add_w : q.add_post_w) ? dst[c] + t : t;
   }
 }
 
-// dw / dpost_w += the groups' sums (only with more than one group of samples)
+// dw / dpost_w from the groups' sums (only with more than one group of samples)
 __global__ void __launch_bounds__(256) sandwich_weights_kernel(SandwichParams p, SandwichBwdParams q) {
   __shared__ float part[8][32];
   const int lane = lane_id(), c = blockIdx.x * 32 + lane;
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(256) sandwich_weights_kernel(SandwichParams p,
   __syncthreads();
   if (warp_id() != 0 || c >= p.D || dst == nullptr) return;
   for (int i = 1; i < 8; ++i) s += part[i][lane];
-  dst[c] += s;
+  dst[c] = (blockIdx.y == 0 ? q.add_w : q.add_post_w) ? dst[c] + s : s;
 }
 
 namespace {

@@ -23,7 +23,7 @@ import math
 import torch
 
 from . import reference as R
-from ._ext import err_buf, ext
+from ._ext import _ERR, err_buf, ext
 from .gemm import gemm
 
 # ----------------------------------------------------------------------------------------------------------------
@@ -81,12 +81,26 @@ def set_bf16_weight(p, w):
 def add_grad_ready_hook(fn):
     """fn(param) is called right after a weight gradient was accumulated into ``param.grad`` by a fused op."""
     _GRAD_HOOKS.append(fn)
+    _hooks_to_ext()
     return fn
 
 
 def remove_grad_ready_hook(fn):
     if fn in _GRAD_HOOKS:
         _GRAD_HOOKS.remove(fn)
+        _hooks_to_ext()
+
+
+def _hooks_to_ext():
+    """The backward kernels with a C++ autograd node call the hooks themselves, while there are any."""
+    if torch.cuda.is_available():
+        ext().set_grad_ready(bool(_GRAD_HOOKS), _notify)
+
+
+def _err_word(t):
+    """The error word of t's device (ops/_ext.py)."""
+    buf = _ERR.get(t.get_device())
+    return buf if buf is not None else err_buf(t.device)
 
 
 def _grad_buffer(p):
@@ -339,29 +353,6 @@ def adanorm(x, y, gate, w, shift=None, scale=None, eps=R.EPS):
 # ----------------------------------------------------------------------------------------------------------------
 # norms before and after a branch
 # ----------------------------------------------------------------------------------------------------------------
-class _SandwichFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, y, gate, post_w, w, shift, scale, res_scale, eps):
-        x_new, h, ry, rx = ext().sandwich_fwd(x, y, gate, post_w, w, shift, scale, res_scale, eps, err_buf(x.device))
-        ctx.save_for_backward(x, y, gate, post_w, w, shift, scale, ry, rx)
-        ctx.how = (res_scale, eps)
-        ctx.params = (post_w, w)
-        ctx.set_materialize_grads(False)
-        return x_new, h
-
-    @staticmethod
-    def backward(ctx, dx_new, dh):
-        x, y, gate, post_w, w, shift, scale, ry, rx = ctx.saved_tensors
-        pp, wp = ctx.params
-        dpost, p_direct = _weight_grad_target(pp) if pp is not None and pp.requires_grad else (None, False)
-        dw, w_direct = _weight_grad_target(wp) if wp is not None and wp.requires_grad else (None, False)
-        dx, dy, dgate, dshift, dscale = ext().sandwich_bwd(
-            None if dx_new is None else dx_new.contiguous(), None if dh is None else dh.contiguous(), x, y, gate,
-            post_w, w, shift, scale, ry, rx, dpost, dw, *ctx.how, err_buf(x.device))
-        return (dx, dy, dgate, None if dpost is None else _weight_grad_done(pp, p_direct, dpost),
-                None if dw is None else _weight_grad_done(wp, w_direct, dw), dshift, dscale, None, None)
-
-
 def sandwich_norm(x, y, gate=None, post_w=None, w=None, shift=None, scale=None, res_scale=1.0, eps=R.EPS):
     """x_new = x + res_scale gate rmsnorm(y) post_w;  h = rmsnorm(x_new) w (1 + scale) + shift -> (x_new, h).
 
@@ -376,18 +367,17 @@ def sandwich_norm(x, y, gate=None, post_w=None, w=None, shift=None, scale=None, 
         raise ValueError("sandwich_norm: shift and scale come together, and with w")
     if not x.is_cuda:
         return R.sandwich_norm(x, y, gate, post_w, w, shift, scale, res_scale, eps)
-    x, y = x.contiguous(), y.contiguous()
-    if shift is not None and shift.stride(0) != scale.stride(0):
-        shift, scale = shift.contiguous(), scale.contiguous()
-    args = (x, y, gate, post_w, w, shift, scale, float(res_scale), float(eps))
-    if not torch.is_grad_enabled():
-        x_new, h = ext().sandwich_fwd(*args, err_buf(x.device))[:2]
-        return x_new, h
-    x_new, h = _SandwichFn.apply(*args)
+    args = (x, y, gate, post_w, w, shift, scale, res_scale, eps, _err_word(x))
+    x_new, h = ext().sandwich_norm(*args)
     if _SAC_ACTIVE[0] and h is not None:  # h is rebuilt from the tensors that the backward keeps anyway
         again = tuple(a.detach() if isinstance(a, torch.Tensor) else a for a in args)
-        _tag(h, _Recipe(lambda: (ext().sandwich_fwd(*again, err_buf(again[0].device))[1],)))
+        _tag(h, _Recipe(lambda: (_again(ext().sandwich_norm, again)[1],)))
     return x_new, h
+
+
+def _again(fn, args):
+    with torch.no_grad():
+        return fn(*args)
 
 
 # ----------------------------------------------------------------------------------------------------------------
@@ -409,32 +399,6 @@ def _axes_table(axes, theta, device):
     return ent
 
 
-class _RopeAxesFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, pos, freq, axis, q_w, k_w, interleaved, eps):
-        qo, ko = ext().rope_axes_fwd(q, k, pos, freq, axis, q_w, k_w, interleaved, eps)
-        if q_w is None:  # a rotation's gradient needs no input: q and k are kept for their shapes and types only
-            q, k = q.detach(), k.detach()
-        ctx.save_for_backward(q, k, pos, freq, axis, q_w, k_w)
-        ctx.how = (interleaved, eps)
-        ctx.params = (q_w, k_w)
-        return qo, ko
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        q, k, pos, freq, axis, q_w, k_w = ctx.saved_tensors
-        qp, kp = ctx.params
-        dqw = dkw = None
-        if q_w is not None and (qp.requires_grad or kp.requires_grad):
-            dqw, q_direct = _weight_grad_target(qp)
-            dkw, k_direct = _weight_grad_target(kp)
-        dq, dk = ext().rope_axes_bwd(dq.contiguous(), dk.contiguous(), q, k, pos, freq, axis, q_w, k_w, dqw, dkw,
-                                     *ctx.how)
-        if dqw is not None:
-            dqw, dkw = _weight_grad_done(qp, q_direct, dqw), _weight_grad_done(kp, k_direct, dkw)
-        return dq, dk, None, None, None, dqw, dkw, None, None
-
-
 def rope_axes(q, k, pos, axes, theta=10000.0, q_w=None, k_w=None, interleaved=True, eps=R.EPS):
     """Rotary positions with several axes, after a per-head RMSNorm when q_w / k_w [d] fp32 are given.
 
@@ -443,38 +407,31 @@ def rope_axes(q, k, pos, axes, theta=10000.0, q_w=None, k_w=None, interleaved=Tr
     of its share of the head by pos_a theta^(-2 m / axes[a]) (theta: one base or one per axis); channels past sum(axes)
     are only normalised. interleaved: pairs (2 i, 2 i + 1), else (i, i + sum(axes) / 2). axes=(d / 2, d / 2) with
     (row, column) positions is the image model's 2-D RoPE. Returns contiguous q, k."""
-    axes = tuple(int(a) for a in axes)
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1]:
-        raise ValueError("rope_axes: q [B, T, Hq, d] and k [B, T, Hkv, d] expected")
-    if not axes or any(a < 2 or a % 2 for a in axes) or sum(axes) > q.shape[-1] or len(axes) > 4:
-        raise ValueError(f"rope_axes: one to four axes of even widths of at most {q.shape[-1]} in all, got {axes}")
-    if tuple(pos.shape) != (*q.shape[:2], len(axes)):
-        raise ValueError(f"rope_axes: pos {(*q.shape[:2], len(axes))} expected, got {tuple(pos.shape)}")
-    if not isinstance(theta, (int, float)) and len(theta) != len(axes):
-        raise ValueError("rope_axes: one theta, or one per axis")
+    ent = _AXES_TABLES.get((tuple(axes), theta if isinstance(theta, (int, float)) else tuple(theta), q.device)) \
+        if q.is_cuda else None
+    if ent is None:
+        axes = tuple(int(a) for a in axes)
+        if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1]:
+            raise ValueError("rope_axes: q [B, T, Hq, d] and k [B, T, Hkv, d] expected")
+        if not axes or any(a < 2 or a % 2 for a in axes) or sum(axes) > q.shape[-1] or len(axes) > 4:
+            raise ValueError(f"rope_axes: one to four axes of even widths of at most {q.shape[-1]} in all, got {axes}")
+        if not isinstance(theta, (int, float)) and len(theta) != len(axes):
+            raise ValueError("rope_axes: one theta, or one per axis")
+        if tuple(pos.shape) != (*q.shape[:2], len(axes)):
+            raise ValueError(f"rope_axes: pos {(*q.shape[:2], len(axes))} expected, got {tuple(pos.shape)}")
+    elif pos.shape[-1] != len(axes):
+        raise ValueError(f"rope_axes: {len(axes)} positions per token expected, got {pos.shape[-1]}")
     if (q_w is None) != (k_w is None):
         raise ValueError("rope_axes: q_w and k_w come together")
     if not q.is_cuda:
         return R.rope_axes(q, k, pos, axes, theta, q_w, k_w, interleaved, eps)
-    B, T, Hq, d = q.shape
-    if not pos.is_floating_point():
-        pos = pos.to(torch.int32)
-    pos = (pos.float() if pos.is_floating_point() else pos).contiguous().view(B * T, len(axes))
-
-    def rows(t):  # [B T, H, d], in place when the tokens are evenly strided and a token's heads are contiguous
-        even = t.stride(3) == 1 and t.stride(2) == d and (B == 1 or t.stride(0) == T * t.stride(1))
-        return (t if even else t.contiguous()).flatten(0, 1)
-    q3, k3 = rows(q), rows(k)
-    args = (q3, k3, pos, *_axes_table(axes, theta, q.device), q_w, k_w, bool(interleaved), float(eps))
-    if not torch.is_grad_enabled():
-        qo, ko = ext().rope_axes_fwd(*args)
-        return qo.view(q.shape), ko.view(k.shape)
-    qo, ko = _RopeAxesFn.apply(*args)
-    qo, ko = qo.view(q.shape), ko.view(k.shape)
+    args = (q, k, pos, *(ent or _axes_table(axes, theta, q.device)), q_w, k_w, interleaved, eps)
+    qo, ko = ext().rope_axes(*args)
     if _SAC_ACTIVE[0]:
         again = tuple(a.detach() if isinstance(a, torch.Tensor) else a for a in args)
-        rec = _Recipe(lambda: tuple(ext().rope_axes_fwd(*again)))
-        qo._tgo_recipe, ko._tgo_recipe = (rec, 0, tuple(q.shape)), (rec, 1, tuple(k.shape))
+        rec = _Recipe(lambda: _again(ext().rope_axes, again))
+        _tag(qo, rec, 0)
+        _tag(ko, rec, 1)
     return qo, ko
 
 

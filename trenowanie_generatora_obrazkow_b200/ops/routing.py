@@ -30,21 +30,6 @@ class ExpertPlan(NamedTuple):
     rows: int
 
 
-class _RouteFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale):
-        w, idx = ext().route_fwd(logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale)
-        ctx.mark_non_differentiable(idx)
-        ctx.save_for_backward(logits, w, idx)
-        ctx.how = (sigmoid, renorm, scale)
-        return w, idx
-
-    @staticmethod
-    def backward(ctx, dw, _):
-        logits, w, idx = ctx.saved_tensors
-        return (ext().route_bwd(logits, w, idx, dw.contiguous(), *ctx.how),) + (None,) * 8
-
-
 def route_experts(logits, k, score="softmax", bias=None, groups=1, top_groups=1, renorm=True, scale=1.0, valid=None):
     """Choose k experts for every token: logits [N, E] (fp32, bf16 or fp16) -> (w fp32 [N, k], idx int32 [N, k]).
 
@@ -65,12 +50,7 @@ def route_experts(logits, k, score="softmax", bias=None, groups=1, top_groups=1,
                          f"{MAX_EXPERTS} experts in equal groups, k at most {MAX_CHOICES} and the kept groups' experts)")
     if not logits.is_cuda:
         return R.route_experts(logits, k, score, bias, groups, top_groups, renorm, scale, valid)
-    if logits.stride(1) != 1:
-        logits = logits.contiguous()
-    args = (logits, bias, valid, k, score == "sigmoid", groups, top_groups, renorm, float(scale))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _RouteFn.apply(*args)
-    return ext().route_fwd(*args)
+    return ext().route_experts(logits, bias, valid, k, score == "sigmoid", groups, top_groups, renorm, scale)
 
 
 def expert_plan(idx, experts, capacity=None):
@@ -81,24 +61,13 @@ def expert_plan(idx, experts, capacity=None):
     if capacity is not None and capacity < 1:
         raise ValueError("expert_plan: capacity of at least 1 row")
     cap = int(capacity or 0)
-    idx = idx.detach()
     if not idx.is_cuda:
         slot, offsets, counts = R.expert_plan(idx, experts, cap)
     else:
-        slot, offsets, counts = ext().expert_plan(idx.to(torch.int32).contiguous(), experts, cap)
+        if idx.dtype is not torch.int32 or not idx.is_contiguous():
+            idx = idx.to(torch.int32).contiguous()
+        slot, offsets, counts = ext().expert_plan(idx, experts, cap)
     return ExpertPlan(slot, offsets, counts, cap, experts * cap if cap else idx.numel())
-
-
-class _DispatchFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, plan):
-        ctx.save_for_backward(plan.slot, plan.offsets, plan.counts)
-        ctx.capacity = plan.capacity
-        return ext().expert_dispatch(x, plan.slot, plan.offsets, plan.counts, plan.capacity, plan.rows)
-
-    @staticmethod
-    def backward(ctx, dxs):
-        return ext().expert_combine(dxs.contiguous(), None, *ctx.saved_tensors, ctx.capacity), None
 
 
 def expert_dispatch(x, plan):
@@ -107,27 +76,7 @@ def expert_dispatch(x, plan):
         raise ValueError(f"expert_dispatch: x [{plan.slot.shape[0]}, D] expected, got {tuple(x.shape)}")
     if not x.is_cuda:
         return R.expert_dispatch(x, plan)
-    if x.stride(1) != 1:
-        x = x.contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _DispatchFn.apply(x, plan)
-    return ext().expert_dispatch(x, plan.slot, plan.offsets, plan.counts, plan.capacity, plan.rows)
-
-
-class _CombineFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, w, plan):
-        ctx.save_for_backward(y, w, plan.slot, plan.offsets, plan.counts)
-        ctx.capacity = plan.capacity
-        return ext().expert_combine(y, w, plan.slot, plan.offsets, plan.counts, plan.capacity)
-
-    @staticmethod
-    def backward(ctx, dout):
-        y, w, *rows = ctx.saved_tensors
-        if dout.stride(1) != 1:
-            dout = dout.contiguous()
-        dy, dw = ext().expert_combine_bwd(y, w, dout, *rows, ctx.capacity)
-        return dy, dw, None
+    return ext().dispatch_rows(x, *plan)
 
 
 def expert_combine(y, w, plan):
@@ -138,7 +87,4 @@ def expert_combine(y, w, plan):
                          f"{tuple(y.shape)} and {tuple(w.shape)}")
     if not y.is_cuda:
         return R.expert_combine(y, w, plan)
-    y, w = y.contiguous(), w.float().contiguous()
-    if torch.is_grad_enabled() and (y.requires_grad or w.requires_grad):
-        return _CombineFn.apply(y, w, plan)
-    return ext().expert_combine(y, w, plan.slot, plan.offsets, plan.counts, plan.capacity)
+    return ext().combine_rows(y, w, *plan[:4])
