@@ -5,8 +5,8 @@
 //     slot[a] = offsets[e] + rank                     packed: expert e owns rows [offsets[e], offsets[e + 1])
 //     slot[a] = e C + rank if rank < C, else -1       capacity C: static shapes, overflow dropped
 // idx < 0 (a padding token) takes no row. One launch: a cluster of CTAs splits the assignments into contiguous spans,
-// each warp counts its own span (lanes with the same expert find one another with match_any, the lowest adds), the
-// CTAs exchange their totals through distributed shared memory, and a second walk over the span hands out the rows.
+// each warp counts its own span, the CTAs exchange their totals through distributed shared memory, and a second walk over
+// the span hands out the rows (lanes with the same expert find one another by ballots).
 //
 // dispatch  xs[slot[n, j]] = x[n]                                backward  dx[n] = sum_j dxs[slot[n, j]]
 // combine   out[n] = sum_j w[n, j] y[slot[n, j]]                 backward  dy[slot[n, j]] = w[n, j] dout[n],
@@ -35,66 +35,92 @@ __device__ __forceinline__ int dsmem_load(const int* p, uint32_t cta) {
   return v;
 }
 
+// Lanes of the warp with this lane's expert (>= 0), from one ballot per bit of the expert's number: a constant
+// log2(E) + 1 ballots, where match_any takes a round per distinct value (8191 x 8 choices of 64: 18.4 us with it).
+__device__ __forceinline__ unsigned same_expert(int e, int bits) {
+  unsigned peers = __ballot_sync(0xffffffffu, e >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const bool set = (e >> b) & 1;
+    const unsigned m = __ballot_sync(0xffffffffu, set);
+    peers &= set ? m : ~m;
+  }
+  return peers;
+}
+
 }  // namespace
 
-// dynamic shared memory: cnt [warps][E], tot [E] (this CTA's assignments of every expert), pre [E], warp sums [32]
-__global__ void plan_kernel(PlanParams p) {
+// dynamic shared memory: cnt [E][33] (assignments of every expert and warp, one pad against bank conflicts), tot [E] (this
+// CTA's assignments of every expert), pre [E], warp sums [32]
+constexpr int PLAN_PITCH = 33;
+constexpr int PLAN_BATCH = 8;  // steps of 32 assignments whose loads a warp issues together
+
+__global__ void __launch_bounds__(1024) plan_kernel(PlanParams p) {
   extern __shared__ int plan_smem[];
   const int warps = blockDim.x >> 5, warp = warp_id(), lane = lane_id();
   int* cnt = plan_smem;
-  int* tot = cnt + warps * p.E;
+  int* tot = cnt + PLAN_PITCH * p.E;
   int* pre = tot + p.E;
   int* wsum = pre + p.E;
   const int ctas = gridDim.x, cta = blockIdx.x;
   // contiguous spans of whole 32-assignment steps
   const int steps = (p.A + 31) / 32, units = ctas * warps;
   const int per = (steps + units - 1) / units;
-  const long long a0 = (long long)(cta * warps + warp) * per * 32;
-  for (int i = threadIdx.x; i < warps * p.E; i += blockDim.x) cnt[i] = 0;
+  const long long a0 = (long long)(cta * warps + warp) * per * 32 + lane;
+  int e[PLAN_BATCH];
+  auto fetch = [&](int i0) {  // experts of the steps i0 .. i0 + PLAN_BATCH - 1, -1: none
+#pragma unroll
+    for (int i = 0; i < PLAN_BATCH; ++i) {
+      const long long a = a0 + (long long)(i0 + i) * 32;
+      e[i] = i0 + i < per && a < p.A ? p.idx[a] : -1;
+      if ((unsigned)e[i] >= (unsigned)p.E) e[i] = -1;
+    }
+  };
+  fetch(0);
+  for (int i = threadIdx.x; i < PLAN_PITCH * p.E; i += blockDim.x) cnt[i] = 0;
   __syncthreads();
-  int* mine = cnt + warp * p.E;
-  for (int i = 0; i < per; ++i) {
-    const long long a = a0 + i * 32 + lane;
-    int e = a < p.A ? p.idx[a] : -1;
-    if ((unsigned)e >= (unsigned)p.E) e = -1;
-    const unsigned peers = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && __ffs(peers) - 1 == lane) mine[e] += __popc(peers);
-    __syncwarp();
+  for (int i0 = 0; i0 < per; i0 += PLAN_BATCH) {
+    if (i0 > 0) fetch(i0);
+#pragma unroll
+    for (int i = 0; i < PLAN_BATCH; ++i)
+      if (e[i] >= 0) atomicAdd(&cnt[e[i] * PLAN_PITCH + warp], 1);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-    int run = 0;
-    for (int w = 0; w < warps; ++w) {
-      const int t = cnt[w * p.E + e];
-      cnt[w * p.E + e] = run;
-      run += t;
+  // a warp per expert: exclusive prefix of its counts over the CTA's warps
+  for (int x = warp; x < p.E; x += warps) {
+    const int v = lane < warps ? cnt[x * PLAN_PITCH + lane] : 0;
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
     }
-    tot[e] = run;
+    cnt[x * PLAN_PITCH + lane] = inc - v;
+    if (lane == 31) tot[x] = inc;
   }
   if (ctas > 1) cluster_sync();
   else __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-    int before = 0, all = 0;
-    if (ctas > 1) {
-      for (int c = 0; c < ctas; ++c) {
-        const int t = dsmem_load(tot + e, c);
-        before += c < cta ? t : 0;
-        all += t;
-      }
-    } else {
-      all = tot[e];
-    }
-    for (int w = 0; w < warps; ++w) cnt[w * p.E + e] += before;
-    pre[e] = all;
-    if (cta == 0) p.counts[e] = all;
-  }
-  __syncthreads();
-  // exclusive prefix of the totals (packed), in steps of the block
+  // totals over the CTAs (pre) and what the CTAs before this one hold (tot: read by the others, so kept apart)
   int carry = 0;
   for (int b = 0; b < p.E; b += blockDim.x) {
-    const int e = b + threadIdx.x;
-    const int v = e < p.E ? pre[e] : 0;
-    int inc = v;
+    const int x = b + threadIdx.x;
+    int before = 0, all = 0;
+    if (x < p.E) {
+      if (ctas > 1) {
+        int t[PLAN_CTAS];
+#pragma unroll
+        for (int c = 0; c < PLAN_CTAS; ++c) t[c] = dsmem_load(tot + x, c);
+#pragma unroll
+        for (int c = 0; c < PLAN_CTAS; ++c) {
+          before += c < cta ? t[c] : 0;
+          all += t[c];
+        }
+      } else {
+        all = tot[x];
+      }
+      if (cta == 0) p.counts[x] = all;
+    }
+    // exclusive prefix of the totals (packed), in steps of the block
+    int inc = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xffffffffu, inc, o);
@@ -102,31 +128,40 @@ __global__ void plan_kernel(PlanParams p) {
     }
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    int below = 0, sum = 0;
-    for (int w = 0; w < warps; ++w) {
-      below += w < warp ? wsum[w] : 0;
-      sum += wsum[w];
+    int w = lane < warps ? wsum[lane] : 0, run = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += t;
     }
-    if (e < p.E) pre[e] = p.capacity > 0 ? e * p.capacity : carry + below + inc - v;
+    const int below = __shfl_sync(0xffffffffu, run - w, warp), sum = __shfl_sync(0xffffffffu, run, 31);
+    if (x < p.E) {
+      const int start = p.capacity > 0 ? x * p.capacity : carry + below + inc - all;
+      pre[x] = start + before;  // row of this CTA's first assignment of x
+      if (cta == 0) p.offsets[x] = start;
+    }
     carry += sum;
     __syncthreads();
   }
-  if (cta == 0) {
-    for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.offsets[e] = pre[e];
-    if (threadIdx.x == 0) p.offsets[p.E] = p.capacity > 0 ? p.E * p.capacity : carry;
-  }
-  for (int i = 0; i < per; ++i) {
-    const long long a = a0 + i * 32 + lane;
-    int e = a < p.A ? p.idx[a] : -1;
-    if ((unsigned)e >= (unsigned)p.E) e = -1;
-    const unsigned peers = __match_any_sync(0xffffffffu, e);
-    const int ahead = __popc(peers & ((1u << lane) - 1u));
-    int rank = 0;
-    if (e >= 0) rank = mine[e] + ahead;
-    __syncwarp();
-    if (e >= 0 && ahead == 0) mine[e] += __popc(peers);
-    __syncwarp();
-    if (a < p.A) p.slot[a] = (e >= 0 && (p.capacity == 0 || rank < p.capacity)) ? pre[e] + rank : -1;
+  if (cta == 0 && threadIdx.x == 0) p.offsets[p.E] = p.capacity > 0 ? p.E * p.capacity : carry;
+  int* mine = cnt + warp;
+  const int bits = 32 - __clz(p.E - 1);
+  for (int i0 = 0; i0 < per; i0 += PLAN_BATCH) {
+    if (per > PLAN_BATCH) fetch(i0);
+#pragma unroll
+    for (int i = 0; i < PLAN_BATCH; ++i) {
+      if (i0 + i >= per) break;  // warp-uniform
+      const unsigned peers = same_expert(e[i], bits);
+      const int ahead = __popc(peers & ((1u << lane) - 1u));
+      int row = -1;
+      if (e[i] >= 0) row = pre[e[i]] + mine[e[i] * PLAN_PITCH] + ahead;
+      __syncwarp();
+      if (e[i] >= 0 && ahead == 0) mine[e[i] * PLAN_PITCH] += __popc(peers);
+      __syncwarp();
+      if (p.capacity > 0 && e[i] >= 0 && row >= (e[i] + 1) * p.capacity) row = -1;
+      const long long a = a0 + (long long)(i0 + i) * 32;
+      if (a < p.A) p.slot[a] = row;
+    }
   }
   if (ctas > 1) cluster_sync();  // no CTA leaves while another may still read its totals
 }
@@ -136,11 +171,11 @@ cudaError_t plan_launch(const PlanParams& p, cudaStream_t s) {
   // one CTA while it can keep up with one step of 32 per warp and a few rounds of it, else a cluster of 8
   const bool cluster = p.A > 8192;
   const int threads = cluster ? 1024 : std::min(1024, std::max(128, (p.A + 31) / 32 * 32));
-  const size_t smem = sizeof(int) * ((size_t)(threads / 32) * p.E + 2 * p.E + 32);
+  const size_t smem = sizeof(int) * ((PLAN_PITCH + 2) * p.E + 32);
   static bool set = false;
   if (!set) {
     cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(sizeof(int) * (34 * kRouteMaxExperts + 32)));
+                                         (int)(sizeof(int) * ((PLAN_PITCH + 2) * kRouteMaxExperts + 32)));
     if (e != cudaSuccess) return e;
     set = true;
   }
@@ -168,7 +203,20 @@ constexpr int FILL_ROWS = 8;   // rows that one warp looks over for clearing
 template <typename T, int V>
 struct RowCfg {  // vectors in flight per lane: 64 bytes of columns per lane and row
   static constexpr int U = V == 8 ? 4 / (sizeof(T) / 2) : 4;
-  static constexpr int COLS = U * 32 * V;  // columns of a part
+  static constexpr int COLS = U * 32 * V;  // the most columns of a part
+};
+
+// the slots (and weights) of a token's choices: lane j holds choice j (k <= 32), so no load stands between two rows
+struct Choices {
+  int slot;
+  float w;
+  __device__ __forceinline__ Choices(const ExpertRows& r, long long n, const float* weights) {
+    const bool on = lane_id() < r.k;
+    slot = on ? r.slot[n * r.k + lane_id()] : -1;
+    w = on && weights != nullptr ? weights[n * r.k + lane_id()] : 1.f;
+  }
+  __device__ __forceinline__ long long row(int j) const { return __shfl_sync(0xffffffffu, slot, j); }
+  __device__ __forceinline__ float weight(int j) const { return __shfl_sync(0xffffffffu, w, j); }
 };
 
 // rows [offsets[E], rows) (packed) or the unfilled tail of every expert (capacity)
@@ -191,101 +239,117 @@ __device__ void clear_rows(const ExpertRows& r, T* out, long long unit) {
 
 }  // namespace
 
+// a part: columns [c0, c1) of a row, at most RowCfg::COLS
 template <typename T, int V>
 __global__ void __launch_bounds__(ROW_WARPS * 32) dispatch_kernel(ExpertRows r, const T* __restrict__ x, long long ldx,
-                                                                  T* __restrict__ xs, int parts) {
+                                                                  T* __restrict__ xs, int parts, int cols) {
   using C = RowCfg<T, V>;
   const long long unit = (long long)blockIdx.x * ROW_WARPS + warp_id();
   if (unit >= (long long)r.N * parts) {
     clear_rows<T, V>(r, xs, unit - (long long)r.N * parts);
     return;
   }
-  const int n = (int)(unit / parts), c0 = (int)(unit % parts) * C::COLS + lane_id() * V;
+  const int n = (int)(unit / parts), part = (int)(unit % parts);
+  const int c0 = part * cols + lane_id() * V, c1 = min(r.D, (part + 1) * cols);
   Raw<T, V> v[C::U];
 #pragma unroll
   for (int u = 0; u < C::U; ++u)
-    if (c0 + u * 32 * V < r.D) v[u].load(x + (long long)n * ldx + c0 + u * 32 * V);
+    if (c0 + u * 32 * V < c1) v[u].load(x + (long long)n * ldx + c0 + u * 32 * V);
+  const Choices ch(r, n, nullptr);
   for (int j = 0; j < r.k; ++j) {
-    const long long slot = r.slot[(long long)n * r.k + j];
+    const long long slot = ch.row(j);
     if (slot < 0) continue;
     T* dst = xs + slot * r.D;
 #pragma unroll
     for (int u = 0; u < C::U; ++u)
-      if (c0 + u * 32 * V < r.D) v[u].store(dst + c0 + u * 32 * V);
+      if (c0 + u * 32 * V < c1) v[u].store(dst + c0 + u * 32 * V);
   }
 }
 
-template <typename T, int V>
+// J rows of U vectors per lane in flight, and U vectors of fp32 sums: few choices take wide parts, many take narrow parts
+// and more rows (8191 x 1280, 8 choices: U 4, J 2 50.9 us).
+template <typename T, int V, int U, int J>
 __global__ void __launch_bounds__(ROW_WARPS * 32) combine_kernel(ExpertRows r, const T* __restrict__ y,
                                                                  const float* __restrict__ w, T* __restrict__ out,
-                                                                 int parts) {
-  using C = RowCfg<T, V>;
+                                                                 int parts, int cols) {
   const long long unit = (long long)blockIdx.x * ROW_WARPS + warp_id();
   if (unit >= (long long)r.N * parts) return;
-  const int n = (int)(unit / parts), c0 = (int)(unit % parts) * C::COLS + lane_id() * V;
-  float acc[C::U][V];
+  const int n = (int)(unit / parts), part = (int)(unit % parts);
+  const int c0 = part * cols + lane_id() * V, c1 = min(r.D, (part + 1) * cols);
+  const Choices ch(r, n, w);
+  float acc[U][V];
 #pragma unroll
-  for (int u = 0; u < C::U; ++u)
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[u][i] = 0.f;
-  for (int j = 0; j < r.k; ++j) {
-    const long long slot = r.slot[(long long)n * r.k + j];
-    if (slot < 0) continue;
-    const float wj = w != nullptr ? w[(long long)n * r.k + j] : 1.f;
-    const T* src = y + slot * r.D;
-    Raw<T, V> v[C::U];
+  for (int j0 = 0; j0 < r.k; j0 += J) {
+    Raw<T, V> v[J][U];
+    float wj[J];
 #pragma unroll
-    for (int u = 0; u < C::U; ++u) {
-      if (c0 + u * 32 * V < r.D) v[u].load(src + c0 + u * 32 * V);
-      else v[u].zero();
+    for (int j = 0; j < J; ++j) {
+      // a dropped choice (and a missing one of the last pair) adds nothing: its rows are not read
+      const long long slot = ch.row((j0 + j) & 31);
+      const bool on = j0 + j < r.k && slot >= 0;
+      wj[j] = on ? ch.weight((j0 + j) & 31) : 0.f;  // `on` is the warp's
+      const T* src = y + slot * r.D;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (on && c0 + u * 32 * V < c1) v[j][u].load(src + c0 + u * 32 * V);
+        else v[j][u].zero();
+      }
     }
 #pragma unroll
-    for (int u = 0; u < C::U; ++u) {
-      float f[V];
-      v[u].get(f);
+    for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[u][i] = fmaf(wj, f[i], acc[u][i]);
-    }
+      for (int u = 0; u < U; ++u) {
+        float f[V];
+        v[j][u].get(f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[u][i] = fmaf(wj[j], f[i], acc[u][i]);
+      }
   }
 #pragma unroll
-  for (int u = 0; u < C::U; ++u)
-    if (c0 + u * 32 * V < r.D) store_vec<T, V>(out + (long long)n * r.D + c0 + u * 32 * V, acc[u]);
+  for (int u = 0; u < U; ++u)
+    if (c0 + u * 32 * V < c1) store_vec<T, V>(out + (long long)n * r.D + c0 + u * 32 * V, acc[u]);
 }
 
-// One warp per token: dout's columns are read once per part and used for the k rows; lane j keeps dw of choice j.
+// One warp per token: dout's columns are read once per part of U vectors per lane and used for the k rows; lane j keeps dw
+// of choice j. More warps beat more loads per warp here: 8191 x 1280, 8 choices, with two rows in flight and 99 registers
+// 90 us, with one row and 64 registers 74 us.
 template <typename T, int V>
-__global__ void __launch_bounds__(ROW_WARPS * 32) combine_bwd_kernel(ExpertRows r, const T* __restrict__ y,
+__global__ void __launch_bounds__(ROW_WARPS * 32, 4) combine_bwd_kernel(ExpertRows r, const T* __restrict__ y,
                                                                      const float* __restrict__ w,
                                                                      const T* __restrict__ dout, long long ldo,
                                                                      T* __restrict__ dy, float* __restrict__ dw) {
-  using C = RowCfg<T, V>;
+  constexpr int U = RowCfg<T, V>::U, COLS = RowCfg<T, V>::COLS;
   const long long n = (long long)blockIdx.x * ROW_WARPS + warp_id();
   if (n >= r.N) {
     clear_rows<T, V>(r, dy, n - r.N);
     return;
   }
   const int lane = lane_id();
+  const Choices ch(r, n, w);
   float mine = 0.f;
-  for (int c0 = lane * V; c0 - lane * V < r.D; c0 += C::COLS) {
-    Raw<T, V> g[C::U];
+  for (int c0 = lane * V; c0 - lane * V < r.D; c0 += COLS) {
+    Raw<T, V> g[U];
 #pragma unroll
-    for (int u = 0; u < C::U; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (c0 + u * 32 * V < r.D) g[u].load(dout + n * ldo + c0 + u * 32 * V);
       else g[u].zero();
     }
     for (int j = 0; j < r.k; ++j) {
-      const long long slot = r.slot[n * r.k + j];
+      const long long slot = ch.row(j);
       if (slot < 0) continue;
-      const float wj = w[n * r.k + j];
-      Raw<T, V> v[C::U];
+      const float wj = ch.weight(j);
+      Raw<T, V> v[U];
 #pragma unroll
-      for (int u = 0; u < C::U; ++u) {
+      for (int u = 0; u < U; ++u) {
         if (c0 + u * 32 * V < r.D) v[u].load(y + slot * r.D + c0 + u * 32 * V);
         else v[u].zero();
       }
       float dot = 0.f;
 #pragma unroll
-      for (int u = 0; u < C::U; ++u) {
+      for (int u = 0; u < U; ++u) {
         float a[V], b[V], o[V];
         g[u].get(a);
         v[u].get(b);
@@ -310,9 +374,11 @@ bool rows_aligned(const ExpertRows& r, const void* a, const void* b, long long l
   return r.D % 8 == 0 && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(a) & 15) == 0 &&
          (reinterpret_cast<uintptr_t>(b) & 15) == 0;
 }
-template <typename T, int V>
-int row_parts(const ExpertRows& r) {
-  return (r.D + RowCfg<T, V>::COLS - 1) / RowCfg<T, V>::COLS;
+// parts of a row of at most `most` columns, of equal numbers of whole vector columns
+int row_parts(const ExpertRows& r, int most, int step, int* cols) {
+  const int parts = (r.D + most - 1) / most;
+  *cols = ((r.D + parts - 1) / parts + step - 1) / step * step;
+  return parts;
 }
 bool row_grid(long long units, unsigned* grid) {
   const long long g = (units + ROW_WARPS - 1) / ROW_WARPS;
@@ -322,19 +388,26 @@ bool row_grid(long long units, unsigned* grid) {
 
 template <typename T, int V>
 cudaError_t dispatch_run(const ExpertRows& r, const T* x, long long ldx, T* xs, cudaStream_t s) {
-  const int parts = row_parts<T, V>(r);
+  int cols;
+  const int parts = row_parts(r, RowCfg<T, V>::COLS, 32 * V, &cols);
   unsigned grid;
   if (!row_grid((long long)r.N * parts + (r.rows + FILL_ROWS - 1) / FILL_ROWS, &grid)) return cudaErrorInvalidValue;
-  dispatch_kernel<T, V><<<grid, ROW_WARPS * 32, 0, s>>>(r, x, ldx, xs, parts);
+  dispatch_kernel<T, V><<<grid, ROW_WARPS * 32, 0, s>>>(r, x, ldx, xs, parts, cols);
+  return cudaGetLastError();
+}
+template <typename T, int V, int U, int J>
+cudaError_t combine_run_with(const ExpertRows& r, const T* y, const float* w, T* out, cudaStream_t s) {
+  int cols;
+  const int parts = row_parts(r, U * 32 * V, 32 * V, &cols);
+  unsigned grid;
+  if (!row_grid((long long)r.N * parts, &grid)) return cudaErrorInvalidValue;
+  combine_kernel<T, V, U, J><<<grid, ROW_WARPS * 32, 0, s>>>(r, y, w, out, parts, cols);
   return cudaGetLastError();
 }
 template <typename T, int V>
 cudaError_t combine_run(const ExpertRows& r, const T* y, const float* w, T* out, cudaStream_t s) {
-  const int parts = row_parts<T, V>(r);
-  unsigned grid;
-  if (!row_grid((long long)r.N * parts, &grid)) return cudaErrorInvalidValue;
-  combine_kernel<T, V><<<grid, ROW_WARPS * 32, 0, s>>>(r, y, w, out, parts);
-  return cudaGetLastError();
+  constexpr int U = RowCfg<T, V>::U;
+  return r.k <= 2 ? combine_run_with<T, V, U, 2>(r, y, w, out, s) : combine_run_with<T, V, U / 2, 4>(r, y, w, out, s);
 }
 template <typename T, int V>
 cudaError_t combine_bwd_run(const ExpertRows& r, const T* y, const float* w, const T* dout, long long ldo, T* dy,

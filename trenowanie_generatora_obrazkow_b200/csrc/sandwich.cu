@@ -16,6 +16,7 @@
 // sums per channel) per sample it meets. Entry unit + sample is unique (along the spans both only grow), so
 // units + samples entries hold them all; two small kernels add them in a fixed order.
 #include <algorithm>
+#include <vector>
 
 #include "block_ops.h"
 #include "common.cuh"
@@ -721,17 +722,43 @@ auto sw_bwd_pick(const SandwichParams& p, F f) {
   return sw_bwd_width<T, R>(p, f);
 }
 
-// Spans that fill every SM with the blocks that it holds; allows the kernel its shared memory.
+// Resident blocks per SM of a kernel with this block and shared memory; the two runtime calls are made once per thread,
+// kernel and shape (they cost as much host time as a launch).
+template <typename K>
+cudaError_t sw_resident(K kernel, int threads, int smem, int* blocks) {
+  struct Known {
+    const void* kernel;
+    int device, threads, smem, blocks;
+  };
+  thread_local std::vector<Known> known;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const void* id = reinterpret_cast<const void*>(kernel);
+  for (const Known& k : known)
+    if (k.kernel == id && k.device == dev && k.threads == threads && k.smem == smem) {
+      *blocks = k.blocks;
+      return cudaSuccess;
+    }
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(blocks, kernel, threads, smem);
+  if (e == cudaSuccess && *blocks < 1) e = cudaErrorInvalidValue;
+  if (e == cudaSuccess) {
+    if (known.size() >= 64) known.clear();
+    known.push_back({id, dev, threads, smem, *blocks});
+  }
+  return e;
+}
+
+// Spans that fill every SM with the blocks that it holds.
 template <typename K>
 cudaError_t sw_geom(K kernel, const SandwichParams& p, int R, int tensors, int es, SwGeom* g, int* smem) {
   const int threads = sw_threads(p, g);
   *smem = 128 + SW_STAGES * tensors * g->groups * R * p.D * es;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, *smem);
-  if (e != cudaSuccess) return e;
   int blocks = 0;
-  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, *smem);
+  cudaError_t e = sw_resident(kernel, threads, *smem, &blocks);
   if (e != cudaSuccess) return e;
-  const int units = num_sms() * std::max(1, blocks) * g->groups;
+  const int units = num_sms() * blocks * g->groups;
   g->span = ((p.M + units - 1) / units + R - 1) / R * R;
   g->steps = g->span / R;
   return cudaSuccess;
