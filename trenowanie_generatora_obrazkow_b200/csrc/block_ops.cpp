@@ -337,7 +337,8 @@ RopeAxesParams rope_params(const at::Tensor& q, const at::Tensor& k, const at::T
     return (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) == hd);
   };
   TORCH_CHECK(heads_ok(q) && heads_ok(k), "rope_axes: the heads of a token must be contiguous");
-  TORCH_CHECK(hd >= 2 && hd <= 1024 && M < (1ll << 31), "rope_axes: head dim 2 to 1024");
+  TORCH_CHECK(hd >= 2 && hd <= 1024 && M < (1ll << 31) && q.size(1) >= 1 && k.size(1) >= 1,
+              "rope_axes: head dim 2 to 1024, at least one head of each");
   TORCH_CHECK(pos.dim() == 2 && pos.size(0) == M && pos.is_contiguous() && pos.size(1) >= 1 &&
                   pos.size(1) <= kRopeMaxAxes && (pos.scalar_type() == at::kInt || pos.scalar_type() == at::kFloat),
               "rope_axes: pos int32 or fp32 [M, axes], at most ", kRopeMaxAxes, " axes");

@@ -34,21 +34,22 @@ __device__ __forceinline__ float position(const RopeAxesParams& p, long long tok
   return p.pos_f32 ? reinterpret_cast<const float*>(p.pos)[i] : (float)reinterpret_cast<const int*>(p.pos)[i];
 }
 
-// cos / sin of the pair of channel c for token tok
-__device__ __forceinline__ void turn_of(const RopeAxesParams& p, long long tok, int pair, float& cs, float& sn) {
-  const float pos = position(p, tok, p.axis[pair]);
-  const float hi = p.freq[pair], lo = p.freq[p.rot / 2 + pair];
+// cos / sin of an angle of pos (hi + lo) revolutions
+__device__ __forceinline__ void turn_at(float pos, float hi, float lo, float& cs, float& sn) {
   const float whole = pos * hi;
   float rev = whole - rintf(whole);
   rev += fmaf(pos, hi, -whole) + pos * lo;
   sincospif(2.f * rev, &sn, &cs);
+}
+__device__ __forceinline__ void turn_of(const RopeAxesParams& p, long long tok, int pair, float& cs, float& sn) {
+  turn_at(position(p, tok, p.axis[pair]), p.freq[pair], p.freq[p.rot / 2 + pair], cs, sn);
 }
 
 }  // namespace
 
 // ------------------------------------------------------------------------------------------------------------------
 // Vector form: head dims of whole 16-byte vectors up to 256 channels. LPH lanes of 8 channels per head (the next power of
-// two: a head dim of 96 leaves 4 of 16 lanes idle), 32 / LPH heads per pass, UNROLL passes' loads issued together.
+// two: a head dim of 96 leaves 4 of 16 lanes idle), 32 / LPH heads per pass, several passes' loads issued together.
 // A rotation is out[c] = x[c] A[c] + x[partner(c)] B[c] with A = w cos, B = -+ w sin of the channel's pair: 16 registers
 // that a token sets up once for its q heads and once for its k heads. The pairs' cos / sin are computed once per warp
 // (rot / 2 of them over 32 lanes) and shared through shared memory. The partner is the neighbour in the lane
@@ -56,7 +57,6 @@ __device__ __forceinline__ void turn_of(const RopeAxesParams& p, long long tok, 
 // ------------------------------------------------------------------------------------------------------------------
 namespace {
 
-constexpr int ROPE_UNROLL = 4;
 
 constexpr int ROPE_MAX_VEC_HD = 256;
 
@@ -67,18 +67,47 @@ __device__ __forceinline__ void identity_turns(const RopeAxesParams& p, float2 (
   for (int i = p.rot / 2 + lane_id(); i < SIZE; i += 32) sh[i] = make_float2(1.f, 0.f);
 }
 
+// A warp's share of the pairs (lane, lane + 32, ...): their table entries, kept over the whole kernel, and the next
+// token's positions, loaded a token ahead.
+template <int PAIRS>
+struct Pairs {
+  static constexpr int N = (PAIRS + 31) / 32;
+  float hi[N], lo[N], pos[N];
+  int axis[N];
+  __device__ __forceinline__ explicit Pairs(const RopeAxesParams& p) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = lane_id() + 32 * k;
+      const bool on = i < p.rot / 2;
+      axis[k] = on ? p.axis[i] : -1;
+      hi[k] = on ? p.freq[i] : 0.f;
+      lo[k] = on ? p.freq[p.rot / 2 + i] : 0.f;
+      pos[k] = 0.f;
+    }
+  }
+  __device__ __forceinline__ void fetch(const RopeAxesParams& p, long long tok) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (axis[k] >= 0 && tok < p.M) pos[k] = position(p, tok, axis[k]);
+  }
+  __device__ __forceinline__ void write(float2* sh) const {
+    __syncwarp();  // the last token's readers
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (axis[k] >= 0) {
+        float c, s;
+        turn_at(pos[k], hi[k], lo[k], c, s);
+        sh[lane_id() + 32 * k] = make_float2(c, s);
+      }
+    __syncwarp();
+  }
+};
+
 // this lane's cos and signed sin: out[c] = x[c] cs[c] + x[partner] sn[c]
 template <bool INTER>
-__device__ __forceinline__ void lane_turns(const RopeAxesParams& p, long long tok, float2* sh, int e0, float (&cs)[8],
+__device__ __forceinline__ void lane_turns(const RopeAxesParams& p, const float2* sh, int e0, float (&cs)[8],
                                            float (&sn)[8]) {
   const int half = p.rot / 2;
-  __syncwarp();
-  for (int i = lane_id(); i < half; i += 32) {
-    float c, s;
-    turn_of(p, tok, i, c, s);
-    sh[i] = make_float2(c, s);
-  }
-  __syncwarp();
   const int at = INTER ? e0 / 2 : (e0 < half ? e0 : e0 - half);
   const float4* t = reinterpret_cast<const float4*>(sh + at);
   if constexpr (INTER) {
@@ -127,77 +156,95 @@ __device__ __forceinline__ int partner_lane(const RopeAxesParams& p, int lane, i
 
 }  // namespace
 
+// Loads of the next batch of heads (of the same tensor, the other one, or the next token) are in flight while a batch is
+// worked on, and the next token's positions while this token's heads are: a token with few heads is otherwise a chain of
+// three memory latencies. 64 registers and 4 blocks per SM with 2 heads in flight per lane beat 3 blocks with 4 (32768
+// tokens x 32 heads of 128: 102 and 106 us; 65536 x 12 heads of 64: 82 and 100 us).
 template <typename T, int LPH, bool INTER>
-__global__ void __launch_bounds__(ROPE_WARPS * 32, 3) rope_axes_kernel(RopeAxesParams p) {
-  constexpr int HPP = 32 / LPH, U = ROPE_UNROLL;
+__global__ void __launch_bounds__(ROPE_WARPS * 32, sizeof(T) == 4 ? 3 : 4) rope_axes_kernel(RopeAxesParams p) {
+  constexpr int HPP = 32 / LPH, U = 2;
   __shared__ __align__(16) float2 turns[ROPE_WARPS][INTER ? LPH * 4 : LPH * 8];
   const int lane = lane_id(), sub = lane / LPH, e0 = (lane % LPH) * 8;
   const bool on = e0 < p.hd;
   const int src = INTER ? lane : partner_lane(p, lane, e0);
-  const int ep = (src % LPH) * 8;  // first partner channel (half-split)
+  const int ep = INTER ? e0 : (src % LPH) * 8;  // first partner channel
   const bool norm = p.q_w != nullptr;
   const float inv_hd = 1.f / p.hd;
+  float2* sh = turns[warp_id()];
   identity_turns(p, turns[warp_id()]);
-  for (long long tok = (long long)blockIdx.x * ROPE_WARPS + warp_id(); tok < p.M; tok += (long long)gridDim.x * ROPE_WARPS) {
-    float cs[8], sn[8];
-    lane_turns<INTER>(p, tok, turns[warp_id()], e0, cs, sn);
+  const long long stride = (long long)gridDim.x * ROPE_WARPS;
+  long long tok = (long long)blockIdx.x * ROPE_WARPS + warp_id();
+  Raw<T, 8> x[U];
+  auto fetch = [&](const T* in, int h0, int heads) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * HPP;
+      if (on && h < heads) x[u].load(in + h * p.hd + e0);
+      else x[u].zero();
+    }
+  };
+  if (tok < p.M) fetch(reinterpret_cast<const T*>(p.q) + tok * p.q_ts, sub, p.hq);
+  Pairs<LPH * 4> pairs(p);
+  pairs.fetch(p, tok);
+  for (; tok < p.M; tok += stride) {
+    pairs.write(sh);
+    pairs.fetch(p, tok + stride);
 #pragma unroll 1
     for (int which = 0; which < 2; ++which) {  // q heads, then k heads
       const int heads = which == 0 ? p.hq : p.hkv;
       const T* in = which == 0 ? reinterpret_cast<const T*>(p.q) + tok * p.q_ts
                                : reinterpret_cast<const T*>(p.k) + tok * p.k_ts;
-      T* out = (which == 0 ? reinterpret_cast<T*>(p.q_out) : reinterpret_cast<T*>(p.k_out)) + tok * heads * p.hd;
+      T* out = (which == 0 ? reinterpret_cast<T*>(p.q_out) : reinterpret_cast<T*>(p.k_out)) + tok * heads * p.hd + e0;
       const float* w = which == 0 ? p.q_w : p.k_w;
       float A[8], B[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) A[j] = cs[j], B[j] = sn[j];
+      lane_turns<INTER>(p, sh, e0, A, B);
       if (norm && on) {
         float a[8], b[8];
         load_vec<float, 8>(w + e0, a);
-        load_vec<float, 8>(w + (INTER ? e0 : ep), b);
+        load_vec<float, 8>(w + ep, b);
 #pragma unroll
         for (int j = 0; j < 8; ++j) A[j] *= a[j], B[j] *= b[INTER ? j ^ 1 : j];
       }
 #pragma unroll 1
       for (int h0 = sub; h0 - sub < heads; h0 += U * HPP) {
-        Raw<T, 8> x[U];
+        Raw<T, 8> cur[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * HPP;
-          if (on && h < heads) x[u].load(in + h * p.hd + e0);
-          else x[u].zero();
-        }
+        for (int u = 0; u < U; ++u) cur[u] = x[u];
+        if (h0 - sub + U * HPP < heads) fetch(in, h0 + U * HPP, heads);
+        else if (which == 0) fetch(reinterpret_cast<const T*>(p.k) + tok * p.k_ts, sub, p.hkv);
+        else if (tok + stride < p.M) fetch(reinterpret_cast<const T*>(p.q) + (tok + stride) * p.q_ts, sub, p.hq);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int h = h0 + u * HPP;
           if (h - sub >= heads) break;  // warp-uniform
           float f[8], g[8];
-          x[u].get(f);
-          partner_of<T, INTER>(x[u], src, g);
+          cur[u].get(f);
+          partner_of<T, INTER>(cur[u], src, g);
           float r = 1.f;
           if (norm) {
             float ss = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
-            r = rsqrtf(head_sum<LPH>(ss) * inv_hd + p.eps);
+            r = rsqrtf(fmaf(head_sum<LPH>(ss), inv_hd, p.eps));
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) f[j] = r * fmaf(f[j], A[j], g[j] * B[j]);
-          if (on && h < heads) store_vec<T, 8>(out + h * p.hd + e0, f);
+          if (on && h < heads) store_vec<T, 8>(out + h * p.hd, f);
         }
       }
     }
   }
 }
 
-// Backward, same layout. dw partials stay in registers over the whole grid-stride loop (a lane's channels are the same
-// for every head and token).
+// Backward, same layout (4 heads in flight per lane, no look-ahead over batches: with it 227 us, without 158 us at 32768 x 32
+// heads of 128). dw partials stay in registers over the whole grid-stride loop: a lane's channels are the same for every
+// head and token.
 template <typename T, int LPH, bool INTER>
 __global__ void __launch_bounds__(ROPE_WARPS * 32, 2) rope_axes_bwd_kernel(RopeAxesParams p, const T* __restrict__ dq,
                                                                         const T* __restrict__ dk,
                                                                         T* __restrict__ dq_in, T* __restrict__ dk_in,
                                                                         float* __restrict__ partial) {
-  constexpr int HPP = 32 / LPH, U = sizeof(T) == 4 ? 2 : ROPE_UNROLL;
+  constexpr int HPP = 32 / LPH, U = sizeof(T) == 4 ? 2 : 4;
   __shared__ __align__(16) float2 turns[ROPE_WARPS][INTER ? LPH * 4 : LPH * 8];
   __shared__ float dw[ROPE_WARPS][2][LPH * 8];
   const int lane = lane_id(), sub = lane / LPH, e0 = (lane % LPH) * 8;
@@ -208,17 +255,24 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 2) rope_axes_bwd_kernel(RopeA
   float acc[2][8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[0][j] = acc[1][j] = 0.f;
+  float2* sh = turns[warp_id()];
   identity_turns(p, turns[warp_id()]);
-  for (long long tok = (long long)blockIdx.x * ROPE_WARPS + warp_id(); tok < p.M; tok += (long long)gridDim.x * ROPE_WARPS) {
+  const long long stride = (long long)gridDim.x * ROPE_WARPS;
+  long long tok = (long long)blockIdx.x * ROPE_WARPS + warp_id();
+  Pairs<LPH * 4> pairs(p);
+  pairs.fetch(p, tok);
+  for (; tok < p.M; tok += stride) {
+    pairs.write(sh);
+    pairs.fetch(p, tok + stride);
     float cs[8], sn[8];
-    lane_turns<INTER>(p, tok, turns[warp_id()], e0, cs, sn);
+    lane_turns<INTER>(p, sh, e0, cs, sn);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       const int heads = which == 0 ? p.hq : p.hkv;
       const T* in = which == 0 ? reinterpret_cast<const T*>(p.q) + tok * p.q_ts
                                : reinterpret_cast<const T*>(p.k) + tok * p.k_ts;
       const T* grad = (which == 0 ? dq : dk) + tok * heads * p.hd;
-      T* out = (which == 0 ? dq_in : dk_in) + tok * heads * p.hd;
+      T* out = (which == 0 ? dq_in : dk_in) + tok * heads * p.hd + e0;
       float w[8] = {};
       if (norm && on) load_vec<float, 8>((which == 0 ? p.q_w : p.k_w) + e0, w);
 #pragma unroll 1
@@ -252,7 +306,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 2) rope_axes_bwd_kernel(RopeA
             }
             ss = head_sum<LPH>(ss);
             dot = head_sum<LPH>(dot);
-            const float r = rsqrtf(ss * inv_hd + p.eps);
+            const float r = rsqrtf(fmaf(ss, inv_hd, p.eps));
             const float m = dot * r * r * inv_hd;  // n mean(gn n) = x r (r dot / hd)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -260,7 +314,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 2) rope_axes_bwd_kernel(RopeA
               gf[j] = r * fmaf(gf[j], w[j], -xf[j] * m);
             }
           }
-          if (on && h < heads) store_vec<T, 8>(out + h * p.hd + e0, gf);
+          if (on && h < heads) store_vec<T, 8>(out + h * p.hd, gf);
         }
       }
     }
@@ -405,18 +459,22 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) rope_axes_bwd_any_kernel(Rope
   }
 }
 
-// dq_w / dk_w (+)= the CTAs' partial sums, in a fixed order
-__global__ void rope_weights_kernel(const float* __restrict__ partial, int ctas, int hd, float* __restrict__ dq_w,
-                                    float* __restrict__ dk_w, bool add_q, bool add_k) {
-  __shared__ float part[8][32];
-  const int c = blockIdx.x * 32 + threadIdx.x;
+// dq_w / dk_w (+)= the CTAs' partial sums, in a fixed order: lane = channel, the 32 warps share the CTAs
+__global__ void __launch_bounds__(1024) rope_weights_kernel(const float* __restrict__ partial, int ctas, int hd,
+                                                            float* __restrict__ dq_w, float* __restrict__ dk_w,
+                                                            bool add_q, bool add_k) {
+  __shared__ float part[32][32];
+  const int lane = lane_id(), warp = warp_id(), c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < 2 * hd)
-    for (int b = threadIdx.y; b < ctas; b += 8) s += partial[(long long)b * 2 * hd + c];
-  part[threadIdx.y][threadIdx.x] = s;
+  if (c < 2 * hd) {
+#pragma unroll 8
+    for (int b = warp; b < ctas; b += 32) s += partial[(long long)b * 2 * hd + c];
+  }
+  part[warp][lane] = s;
   __syncthreads();
-  if (threadIdx.y != 0 || c >= 2 * hd) return;
-  for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
+  if (warp != 0 || c >= 2 * hd) return;
+#pragma unroll
+  for (int i = 1; i < 32; ++i) s += part[i][lane];
   float* dst = c < hd ? dq_w + c : dk_w + (c - hd);
   *dst = (c < hd ? add_q : add_k) ? *dst + s : s;
 }
@@ -436,17 +494,20 @@ bool rope_vectors(const RopeAxesParams& p, int elem, std::initializer_list<const
   return (bits & 15) == 0;
 }
 
-// CTAs of the grid-stride kernels: a warp per token (vector form) or per token and head, at most 8 blocks per SM
-int rope_grid(const RopeAxesParams& p, bool vectors) {
+// CTAs of the grid-stride kernels: a warp per token (vector form) or per token and head. Backward: the blocks that the SMs
+// hold (more would add partial sums: 161 us with 2 per SM, 169 us with 8 at 32768 x 32 heads of 128); forward: a few times
+// that, so that the last tokens spread evenly (fp32: 194 us with 3, 179 us with 16).
+int rope_grid(const RopeAxesParams& p, bool vectors, int per_sm) {
   const long long units = vectors ? p.M : (long long)p.M * (p.hq + p.hkv);
-  return (int)std::min<long long>((units + ROPE_WARPS - 1) / ROPE_WARPS, (long long)num_sms() * 8);
+  return (int)std::min<long long>((units + ROPE_WARPS - 1) / ROPE_WARPS, (long long)num_sms() * per_sm);
 }
+constexpr int ROPE_FWD_BLOCKS = 16, ROPE_BWD_BLOCKS = 2, ROPE_ANY_BLOCKS = 4;
 
 template <typename T, int LPH>
 void rope_fwd_vec(const RopeAxesParams& p, cudaStream_t s) {
-  const long long grid = ((long long)p.M + ROPE_WARPS - 1) / ROPE_WARPS;
-  if (p.interleaved) rope_axes_kernel<T, LPH, true><<<(unsigned)grid, ROPE_WARPS * 32, 0, s>>>(p);
-  else rope_axes_kernel<T, LPH, false><<<(unsigned)grid, ROPE_WARPS * 32, 0, s>>>(p);
+  const int grid = rope_grid(p, true, ROPE_FWD_BLOCKS);
+  if (p.interleaved) rope_axes_kernel<T, LPH, true><<<grid, ROPE_WARPS * 32, 0, s>>>(p);
+  else rope_axes_kernel<T, LPH, false><<<grid, ROPE_WARPS * 32, 0, s>>>(p);
 }
 template <typename T, int LPH>
 void rope_bwd_vec(const RopeAxesParams& p, const T* dq, const T* dk, T* dqi, T* dki, float* partial, int grid,
@@ -459,7 +520,7 @@ void rope_bwd_vec(const RopeAxesParams& p, const T* dq, const T* dk, T* dqi, T* 
 
 template <typename T>
 cudaError_t rope_fwd_run(const RopeAxesParams& p, int elem, cudaStream_t s) {
-  if (!rope_vectors(p, elem)) rope_axes_any_kernel<T><<<rope_grid(p, false), ROPE_WARPS * 32, 0, s>>>(p);
+  if (!rope_vectors(p, elem)) rope_axes_any_kernel<T><<<rope_grid(p, false, ROPE_ANY_BLOCKS), ROPE_WARPS * 32, 0, s>>>(p);
   else if (p.hd <= 32) rope_fwd_vec<T, 4>(p, s);
   else if (p.hd <= 64) rope_fwd_vec<T, 8>(p, s);
   else if (p.hd <= 128) rope_fwd_vec<T, 16>(p, s);
@@ -474,7 +535,7 @@ cudaError_t rope_bwd_run(const RopeAxesParams& p, const void* dq, const void* dk
   const T *gq = static_cast<const T*>(dq), *gk = static_cast<const T*>(dk);
   T *iq = static_cast<T*>(dq_in), *ik = static_cast<T*>(dk_in);
   const bool vec = rope_vectors(p, elem, {dq, dk, dq_in, dk_in});
-  const int grid = rope_grid(p, vec);
+  const int grid = rope_grid(p, vec, vec ? ROPE_BWD_BLOCKS : ROPE_ANY_BLOCKS);
   if (!vec)
     rope_axes_bwd_any_kernel<T><<<grid, ROPE_WARPS * 32, sizeof(float) * ROPE_WARPS * 2 * p.hd, s>>>(p, gq, gk, iq, ik,
                                                                                                    partial);
@@ -484,7 +545,7 @@ cudaError_t rope_bwd_run(const RopeAxesParams& p, const void* dq, const void* dk
   else rope_bwd_vec<T, 32>(p, gq, gk, iq, ik, partial, grid, s);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || partial == nullptr) return e;
-  rope_weights_kernel<<<(2 * p.hd + 31) / 32, dim3(32, 8), 0, s>>>(partial, grid, p.hd, dq_w, dk_w, add_q_w, add_k_w);
+  rope_weights_kernel<<<(2 * p.hd + 31) / 32, 1024, 0, s>>>(partial, grid, p.hd, dq_w, dk_w, add_q_w, add_k_w);
   return cudaGetLastError();
 }
 
@@ -500,7 +561,7 @@ cudaError_t rope_axes_fwd_launch(const RopeAxesParams& p, int elem, cudaStream_t
   return cudaErrorInvalidValue;
 }
 
-int rope_axes_bwd_ctas() { return num_sms() * 8; }
+int rope_axes_bwd_ctas() { return num_sms() * std::max(ROPE_BWD_BLOCKS, ROPE_ANY_BLOCKS); }
 
 cudaError_t rope_axes_bwd_launch(const RopeAxesParams& p, const void* dq, const void* dk, void* dq_in, void* dk_in,
                                  float* partial, float* dq_w, float* dk_w, bool add_q_w, bool add_k_w, int elem,
