@@ -384,7 +384,7 @@ std::tuple<at::Tensor, at::Tensor> rope_axes_fwd(at::Tensor q, at::Tensor k, at:
 std::tuple<at::Tensor, at::Tensor> rope_axes_bwd(at::Tensor dq, at::Tensor dk, at::Tensor q, at::Tensor k,
                                                  at::Tensor pos, at::Tensor freq, at::Tensor axis, OptT q_w, OptT k_w,
                                                  OptT dq_w, OptT dk_w, bool interleaved, double eps, bool add_q_w,
-                                                 bool add_k_w) {
+                                                 bool add_k_w, OptT dq_out, OptT dk_out) {
   RopeAxesParams p = rope_params(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
   const c10::cuda::CUDAGuard guard(q.device());
   auto grad_ok = [&](const at::Tensor& g, const at::Tensor& t) {
@@ -392,7 +392,16 @@ std::tuple<at::Tensor, at::Tensor> rope_axes_bwd(at::Tensor dq, at::Tensor dk, a
            g.device() == t.device();
   };
   TORCH_CHECK(grad_ok(dq, q) && grad_ok(dk, k), "rope_axes_bwd: dq / dk contiguous, as q / k");
-  at::Tensor dqi = at::empty_like(dq), dki = at::empty_like(dk), partial;
+  auto out_ok = [&](const at::Tensor& o, const at::Tensor& t) {
+    return o.sizes() == t.sizes() && o.scalar_type() == t.scalar_type() && o.device() == t.device() &&
+           o.stride(2) == 1 && o.stride(1) == p.hd;
+  };
+  TORCH_CHECK((!given(dq_out) || out_ok(*dq_out, q)) && (!given(dk_out) || out_ok(*dk_out, k)),
+              "rope_axes_bwd: dq_out / dk_out as q / k, a token's heads contiguous");
+  at::Tensor dqi = given(dq_out) ? *dq_out : at::empty_like(dq), dki = given(dk_out) ? *dk_out : at::empty_like(dk);
+  at::Tensor partial;
+  p.dq_ts = dqi.stride(0);
+  p.dk_ts = dki.stride(0);
   float* gq = acc_f32(dq_w, p.hd, q, "rope_axes_bwd: dq_w");
   float* gk = acc_f32(dk_w, p.hd, q, "rope_axes_bwd: dk_w");
   TORCH_CHECK((gq == nullptr) == (gk == nullptr) && (gq == nullptr || p.q_w != nullptr),
@@ -443,12 +452,19 @@ void set_grad_ready(bool on, py::object notify) {
 }
 
 // Where the backward puts the gradient of a small fp32 weight: in place into the leaf's .grad (no temporary, no
-// accumulation kernel), or a temporary that autograd takes.
+// accumulation kernel), or a temporary that autograd takes. The parameter itself is kept beside the saved tensors: under
+// saved-tensor hooks a saved leaf comes back as another tensor, whose .grad nobody reads.
 struct WeightGrad {
   at::Tensor w, g;
   bool direct = false, add = false;
-  explicit WeightGrad(const at::Tensor& weight) : w(weight) {
-    if (!w.defined() || !w.requires_grad()) return;
+  static void keep(AutogradContext* ctx, const char* name, const OptT& weight) {
+    if (given(weight)) ctx->saved_data[name] = *weight;
+  }
+  WeightGrad(AutogradContext* ctx, const char* name) {
+    const auto it = ctx->saved_data.find(name);
+    if (it == ctx->saved_data.end()) return;
+    w = it->second.toTensor();
+    if (!w.requires_grad()) return;
     if (w.is_leaf() && w.scalar_type() == at::kFloat) {
       at::Tensor& have = w.mutable_grad();
       if (!have.defined()) {
@@ -556,6 +572,8 @@ struct SandwichFn : public torch::autograd::Function<SandwichFn> {
     auto r = sandwich_fwd(x, y, gate, post_w, w, shift, scale, res_scale, eps, err);
     ctx->save_for_backward({x, y, or_undefined(gate), or_undefined(post_w), or_undefined(w), or_undefined(shift),
                             or_undefined(scale), r[2], r[3]});
+    WeightGrad::keep(ctx, "post_w", post_w);
+    WeightGrad::keep(ctx, "w", w);
     ctx->saved_data["err"] = err;
     ctx->saved_data["res_scale"] = res_scale;
     ctx->saved_data["eps"] = eps;
@@ -567,7 +585,7 @@ struct SandwichFn : public torch::autograd::Function<SandwichFn> {
     const auto s = ctx->get_saved_variables();
     const at::Tensor dx_new = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
     const at::Tensor dh = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
-    const WeightGrad gp(s[3]), gw(s[4]);
+    const WeightGrad gp(ctx, "post_w"), gw(ctx, "w");
     auto r = sandwich_bwd(opt(dx_new), opt(dh), s[0], s[1], opt(s[2]), opt(s[3]), opt(s[4]), opt(s[5]), opt(s[6]),
                           opt(s[7]), opt(s[8]), opt(gp.g), opt(gw.g), ctx->saved_data["res_scale"].toDouble(),
                           ctx->saved_data["eps"].toDouble(), ctx->saved_data["err"].toTensor(), gp.add, gw.add);
@@ -614,20 +632,22 @@ struct RopeAxesFn : public torch::autograd::Function<RopeAxesFn> {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [qo, ko] = rope_axes_fwd(token_rows(q), token_rows(k), pos, freq, axis, q_w, k_w, interleaved, eps);
     ctx->save_for_backward({q, k, pos, freq, axis, or_undefined(q_w), or_undefined(k_w)});
+    WeightGrad::keep(ctx, "q_w", q_w);
+    WeightGrad::keep(ctx, "k_w", k_w);
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["eps"] = eps;
     return {qo.view(q.sizes()), ko.view(k.sizes())};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    const WeightGrad gq(s[5]), gk(s[6]);
+    const WeightGrad gq(ctx, "q_w"), gk(ctx, "k_w");
     // the two weights' sums come together: one that needs no gradient gets a scratch row
     at::Tensor wq = gq.g, wk = gk.g;
     if (wq.defined() != wk.defined()) (wq.defined() ? wk : wq) = at::empty_like(wq.defined() ? wq : wk);
     auto [dq, dk] = rope_axes_bwd(grads[0].contiguous().flatten(0, 1), grads[1].contiguous().flatten(0, 1),
                                   token_rows(s[0]), token_rows(s[1]), s[2], s[3], s[4], opt(s[5]), opt(s[6]), opt(wq),
                                   opt(wk), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(),
-                                  gq.add, gk.add);
+                                  gq.add, gk.add, OptT(), OptT());
     variable_list out(9);
     out[0] = dq.view(s[0].sizes());
     out[1] = dk.view(s[1].sizes());
@@ -674,7 +694,7 @@ void bind_block_ops(pybind11::module_& m) {
   m.def("rope_axes_bwd", &rope_axes_bwd, "backward of rope_axes_fwd", py::arg("dq"), py::arg("dk"), py::arg("q"),
         py::arg("k"), py::arg("pos"), py::arg("freq"), py::arg("axis"), py::arg("q_w"), py::arg("k_w"),
         py::arg("dq_w"), py::arg("dk_w"), py::arg("interleaved"), py::arg("eps"), py::arg("add_q_w") = true,
-        py::arg("add_k_w") = true);
+        py::arg("add_k_w") = true, py::arg("dq_out") = OptT(), py::arg("dk_out") = OptT());
   m.def("set_grad_ready", &set_grad_ready, "callback for gradients that a backward accumulated in place");
 }
 

@@ -109,9 +109,10 @@ struct RopeAxesParams {
   const float* k_w;
   float eps;
   int M, axes, hq, hkv, hd, rot, interleaved;
+  long long dq_ts, dk_ts;  // backward: token strides of dq_in / dk_in
 };
 cudaError_t rope_axes_fwd_launch(const RopeAxesParams& p, int elem, cudaStream_t s);
-// dq / dk [M, h, hd] contiguous -> dq_in / dk_in [M, h, hd] contiguous; dq_w / dk_w [hd] added to or written through partials
+// dq / dk [M, h, hd] contiguous -> dq_in / dk_in [M, h, hd], a token's heads contiguous; dq_w / dk_w [hd] added to or written through partials
 // [rope_axes_bwd_ctas()][2][hd] (the most CTAs of any launch)
 int rope_axes_bwd_ctas();
 cudaError_t rope_axes_bwd_launch(const RopeAxesParams& p, const void* dq, const void* dk, void* dq_in, void* dk_in,

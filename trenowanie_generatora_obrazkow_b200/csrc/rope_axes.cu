@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 2) rope_axes_bwd_kernel(RopeA
       const T* in = which == 0 ? reinterpret_cast<const T*>(p.q) + tok * p.q_ts
                                : reinterpret_cast<const T*>(p.k) + tok * p.k_ts;
       const T* grad = (which == 0 ? dq : dk) + tok * heads * p.hd;
-      T* out = (which == 0 ? dq_in : dk_in) + tok * heads * p.hd + e0;
+      T* out = (which == 0 ? dq_in + tok * p.dq_ts : dk_in + tok * p.dk_ts) + e0;
       float w[8] = {};
       if (norm && on) load_vec<float, 8>((which == 0 ? p.q_w : p.k_w) + e0, w);
 #pragma unroll 1
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) rope_axes_bwd_any_kernel(Rope
     const T* src = reinterpret_cast<const T*>(is_q ? p.q : p.k) + tok * (is_q ? p.q_ts : p.k_ts) + (long long)h * p.hd;
     const long long o = (tok * (is_q ? p.hq : p.hkv) + h) * p.hd;
     const T* g = (is_q ? dq : dk) + o;
-    T* dst = (is_q ? dq_in : dk_in) + o;
+    T* dst = (is_q ? dq_in + tok * p.dq_ts : dk_in + tok * p.dk_ts) + (long long)h * p.hd;
     const float* w = is_q ? p.q_w : p.k_w;
     auto pair_grad = [&](int i, int& ca, int& cb, float& ga, float& gb) {
       ca = p.interleaved ? 2 * i : i, cb = p.interleaved ? 2 * i + 1 : i + half;
@@ -485,7 +485,9 @@ namespace {
 // element of another lane.
 bool rope_vectors(const RopeAxesParams& p, int elem, std::initializer_list<const void*> more = {}) {
   const int per = elem == ELEM_F32 ? 4 : 8;  // elements of a 16-byte word
-  if (p.hd % 8 != 0 || p.hd > ROPE_MAX_VEC_HD || p.q_ts % per != 0 || p.k_ts % per != 0) return false;
+  if (p.hd % 8 != 0 || p.hd > ROPE_MAX_VEC_HD || p.q_ts % per != 0 || p.k_ts % per != 0 || p.dq_ts % per != 0 ||
+      p.dk_ts % per != 0)
+    return false;
   if (!p.interleaved && p.rot % 16 != 0) return false;
   uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) |
                    reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_out) |

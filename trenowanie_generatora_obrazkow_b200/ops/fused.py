@@ -15,6 +15,7 @@ autograd. Each CUDA op is a ``torch.autograd.Function`` whose backward is a hand
 * ``swiglu``        silu(a) * b.
 * ``sandwich_norm`` norms before and after a branch with its gate and residual scale (x + r gate norm(y), then the next
                     branch's norm and modulation).
+* ``axes_attention_core``  ``self_attention_core`` with such positions.
 * ``rope_axes``     q/k RMSNorm and rotary positions with several axes (time, height, width) from integer positions.
 * ``varlen_attention`` packed variable-length (causal) attention for the frozen caption LM (inference only).
 """
@@ -512,6 +513,71 @@ def self_attention_core(qkv, heads, kv_heads, head_dim, q_w=None, k_w=None, cos=
         return R.attention(q, k, v, kv_len, scale).reshape(B, T, heads * head_dim)
     return _SelfAttnFn.apply(qkv.contiguous(), q_w, k_w, _rope_arg(cos), _rope_arg(sin), kv_len, heads, kv_heads,
                              head_dim, float(scale), eps)
+
+
+class _AxesAttnFn(torch.autograd.Function):
+    """_SelfAttnFn with positions instead of tables: q / k norm and multi-axis rotary, flash attention, and a backward
+    that writes dq, dk and dv straight into the rows of dqkv."""
+
+    @staticmethod
+    def forward(ctx, qkv, pos, freq, axis, q_w, k_w, kv_len, hq, hkv, hd, scale, interleaved, eps):
+        B, T, _ = qkv.shape
+        rows = qkv.view(B * T, hq + 2 * hkv, hd)
+        qi, ki = rows[:, :hq], rows[:, hq:hq + hkv]
+        q, k = ext().rope_axes_fwd(qi, ki, pos, freq, axis, q_w, k_w, interleaved, eps)
+        v4 = rows[:, hq + hkv:].view(B, T, hkv, hd)
+        o, lse = ext().attention_fwd(q.view(B, T, hq, hd), k.view(B, T, hkv, hd), v4, kv_len, scale, None,
+                                     err_buf(qkv.device))
+        if _SAC_ACTIVE[0]:
+            rd = rows.detach()
+            rec = _Recipe(lambda: tuple(ext().rope_axes_fwd(rd[:, :hq], rd[:, hq:hq + hkv], pos, freq, axis, q_w, k_w,
+                                                            interleaved, eps)))
+            _tag(q, rec, 0)
+            _tag(k, rec, 1)
+        ctx.save_for_backward(qkv, q, k, o, lse, pos, freq, axis, q_w, k_w, kv_len)
+        ctx.dims = (hq, hkv, hd, scale, interleaved, eps)
+        ctx.q_param, ctx.k_param = q_w, k_w
+        return o.view(B, T, hq * hd)
+
+    @staticmethod
+    def backward(ctx, do):
+        qkv, q, k, o, lse, pos, freq, axis, q_w, k_w, kv_len = ctx.saved_tensors
+        hq, hkv, hd, scale, interleaved, eps = ctx.dims
+        B, T, _ = qkv.shape
+        dqkv = torch.empty_like(qkv)
+        rows, drows = qkv.view(B * T, hq + 2 * hkv, hd), dqkv.view(B * T, hq + 2 * hkv, hd)
+        v4, dv4 = (r[:, hq + hkv:].view(B, T, hkv, hd) for r in (rows, drows))
+        dq, dk = torch.empty_like(q), torch.empty_like(k)
+        ext().attention_bwd(q.view(B, T, hq, hd), k.view(B, T, hkv, hd), v4, o, lse,
+                            do.contiguous().view(B, T, hq, hd), kv_len, scale, dq.view(B, T, hq, hd),
+                            dk.view(B, T, hkv, hd), dv4, err_buf(q.device))
+        dwq = dwk = None
+        if q_w is not None and (ctx.q_param.requires_grad or ctx.k_param.requires_grad):
+            dwq, q_direct = _weight_grad_target(ctx.q_param)
+            dwk, k_direct = _weight_grad_target(ctx.k_param)
+        ext().rope_axes_bwd(dq, dk, rows[:, :hq], rows[:, hq:hq + hkv], pos, freq, axis, q_w, k_w, dwq, dwk,
+                            interleaved, eps, dq_out=drows[:, :hq], dk_out=drows[:, hq:hq + hkv])
+        if dwq is not None:
+            dwq = _weight_grad_done(ctx.q_param, q_direct, dwq)
+            dwk = _weight_grad_done(ctx.k_param, k_direct, dwk)
+        return dqkv, None, None, None, dwq, dwk, None, None, None, None, None, None, None
+
+
+def axes_attention_core(qkv, pos, axes, heads, kv_heads, head_dim, theta=10000.0, q_w=None, k_w=None, kv_len=None,
+                        scale=None, interleaved=True, eps=R.EPS):
+    """Self-attention with multi-axis rotary positions: qkv [B, T, (heads + 2 kv_heads) head_dim], pos [B, T, axes] (see
+    ``rope_axes``) -> [B, T, heads head_dim]; keys at positions >= kv_len[b] are masked. Head dims 64 and 128 on CUDA."""
+    scale = head_dim ** -0.5 if scale is None else scale
+    B, T, _ = qkv.shape
+    if not qkv.is_cuda:
+        q, k, v = qkv.view(B, T, heads + 2 * kv_heads, head_dim).split([heads, kv_heads, kv_heads], dim=2)
+        q, k = rope_axes(q, k, pos, axes, theta, q_w, k_w, interleaved, eps)
+        return R.attention(q, k, v, kv_len, scale).reshape(B, T, heads * head_dim)
+    if tuple(pos.shape) != (B, T, len(axes)) or sum(axes) > head_dim:
+        raise ValueError(f"axes_attention_core: pos {(B, T, len(axes))} and axes of at most {head_dim} channels")
+    pos = (pos.float() if pos.is_floating_point() else pos.to(torch.int32)).contiguous().view(B * T, len(axes))
+    return _AxesAttnFn.apply(qkv.contiguous(), pos, *_axes_table(axes, theta, qkv.device), q_w, k_w, kv_len, heads,
+                             kv_heads, head_dim, float(scale), bool(interleaved), float(eps))
 
 
 class _CrossAttnFn(torch.autograd.Function):
