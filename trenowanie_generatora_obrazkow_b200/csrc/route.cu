@@ -11,19 +11,22 @@
 // s' = s (1 - s), S = sum of the chosen s. The selection and the bias take no gradient.
 //
 // L lanes hold one token, EPL consecutive experts each, so a row is read once with wide loads and every later step works on
-// registers. c is mapped to an unsigned key of the same order (NaN lowest, -0 as +0). Each lane sorts its keys (stable, so
-// equal keys keep their index order), then each of the k steps takes the largest head of the L lists; the lowest lane
-// that holds it wins (its experts have the lowest indices) and drops its head. What the weights need beyond the choice
+// registers. c is mapped to an unsigned key of the same order (NaN lowest, -0 as +0). Each lane keeps its best
+// keys at the front (equal keys in index order), then each of the k steps takes the largest head of the L lanes; the
+// lowest lane that holds it wins (its experts have the lowest indices) and drops its head. What the weights need beyond the choice
 // is computed for the k chosen alone, from logits read again (they are in the cache).
+#include <algorithm>
+
 #include "block_ops.h"
 #include "common.cuh"
+#include "kernels.h"
 #include "vec.cuh"
 
 namespace tgo {
 
 namespace {
 
-constexpr int ROUTE_WARPS = 4;
+constexpr int ROUTE_WARPS = 4, ROUTE_BWD_BLOCKS = 8;
 
 __device__ __forceinline__ unsigned order_key(float c) {
   c += 0.f;  // -0 -> +0
@@ -199,14 +202,15 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_fwd_kernel(RouteParams
       if (!((kept >> (g & 31)) & 1u)) key[j] = 0u;
     }
   }
-  // descending and stable: neighbours swap only when the later key is larger (EPL rounds of disjoint neighbours)
+  // The lane's two best go to the front by two passes over neighbours, which swap only when the later key is larger (stable).
+  // A lane that has given both is rare; then every lane of the warp makes one more pass. (Sorting all eight: 78 us.)
   int id[EPL];
 #pragma unroll
   for (int j = 0; j < EPL; ++j) id[j] = e0 + j;
+  auto best_to = [&](int front) {
 #pragma unroll
-  for (int round = 0; round < EPL; ++round)
-#pragma unroll
-    for (int j = round & 1; j + 1 < EPL; j += 2) {
+    for (int j = EPL - 2; j >= 0; --j) {
+      if (j < front) continue;
       const unsigned a = key[j], b = key[j + 1];
       const bool swap = b > a;
       const int ia = id[j], ib = id[j + 1];
@@ -215,19 +219,27 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_fwd_kernel(RouteParams
       id[j] = swap ? ib : ia;
       id[j + 1] = swap ? ia : ib;
     }
+  };
+  best_to(0);
+  best_to(1);
+  int ready = 2;  // heads in order
+  const unsigned lower = ((1u << li) - 1u) << (lane - li);  // the token's lanes below this one
   for (int r = 0; r < p.k; ++r) {
+    if (__any_sync(0xffffffffu, ready == 0)) {
+      best_to(0);
+      ready = max(ready, 1);
+    }
     bool win = true;
     if constexpr (L > 1) {
       const unsigned gm = lanes_max<L>(key[0]);
-      unsigned who = __ballot_sync(0xffffffffu, key[0] == gm);
-      if constexpr (L < 32) who = (who >> (lane - li)) & ((1u << L) - 1u);
-      win = __ffs(who) - 1 == li;
+      const unsigned who = __ballot_sync(0xffffffffu, key[0] == gm);
+      win = key[0] == gm && (who & lower) == 0u;
     }
-    if (win) {
+    if (win) {  // the second moves up and leaves a hole, which the next pass carries to the back
       si[tok * p.k + r] = id[0];
-#pragma unroll
-      for (int j = 0; j + 1 < EPL; ++j) key[j] = key[j + 1], id[j] = id[j + 1];
-      key[EPL - 1] = 0u;
+      key[0] = key[1], id[0] = id[1];
+      key[1] = 0u;
+      --ready;
     }
   }
   __syncwarp();
@@ -257,95 +269,135 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_fwd_kernel(RouteParams
   }
 }
 
-// The chosen experts' values go into a zeroed row in shared memory, from which the lanes write the dense row.
+// The chosen experts' values go into a zeroed row in shared memory, from which the lanes write the dense row. A warp walks
+// its tokens with a grid stride and, while each lane holds one choice (k <= L), loads two tokens ahead: the choices of the
+// token after next, and the next token's logits at its choices (an address that depends on them). Without that, a token
+// is a chain of two memory latencies (65536 x 256: 33 us with one token per warp).
 template <typename T, int L, int EPL>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_bwd_kernel(RouteParams p, const float* __restrict__ dw,
                                                                      T* __restrict__ dlogits) {
   constexpr int TOKENS = ROUTE_WARPS * 32 / L, PITCH = L * EPL;
   __shared__ __align__(16) float rows[TOKENS * PITCH];
   const int li = lane_id() % L, tok = threadIdx.x / L;
-  const long long n = (long long)blockIdx.x * TOKENS + tok;
-  const bool in = n < p.N;
   const int e0 = li * EPL;
-  const long long at = in ? n : 0;
-  const T* row = reinterpret_cast<const T*>(p.logits) + at * p.ld;
-  const float *w = p.w + at * p.k, *g = dw + at * p.k;
-  const int* idx = p.idx + at * p.k;
   float* d = rows + tok * PITCH;
-  const bool live = in && idx[0] >= 0;
-#pragma unroll
-  for (int j = 0; j < EPL; j += 4) *reinterpret_cast<float4*>(d + e0 + j) = make_float4(0.f, 0.f, 0.f, 0.f);
-  __syncwarp();
-  // m = sum of r dw and S = sum of the chosen s; with k <= L each lane keeps what it read of its choice
-  int e = 0;
-  float we = 0.f, ge = 0.f, se = 0.f, de = 0.f;  // weight, its gradient, score s and s' of this lane's choice
-  auto choice = [&](int r) {
-    e = idx[r];
-    we = w[r];
-    ge = g[r];
-    if (p.sigmoid) {
-      const float l = to_f<T>(row[e]);
-      const float x = expf(-fabsf(l)), q = 1.f / (1.f + x);
-      se = (l >= 0.f ? 1.f : x) * q;
-      de = x * q * q;
-    }
+  const bool one = p.k <= L;
+  struct Choice {
+    int e = -1;  // -1: none (a token past the end, or without experts, or a lane past k)
+    float w = 0.f, g = 0.f;
   };
-  float m = 0.f, total = 0.f;
-  if (live)
-    for (int r = li; r < p.k; r += L) {
-      choice(r);
-      m = fmaf(we, ge, m);
-      total += se;
+  auto choice = [&](long long n, int r) {
+    Choice c;
+    if (n < p.N && r < p.k) {
+      c.e = p.idx[n * p.k + r];
+      c.w = p.w[n * p.k + r];
+      c.g = dw[n * p.k + r];
     }
-  m = lanes_sum<L>(m) / p.scale;
-  if (p.sigmoid && p.renorm) total = lanes_sum<L>(total) + 1e-20f;
-  if (live)
-    for (int r = li; r < p.k; r += L) {
-      if (p.k > L) choice(r);
-      const float up = p.renorm ? ge - m : ge;
-      d[e] = p.sigmoid ? p.scale * up * de / (p.renorm ? total : 1.f) : we * up;
-    }
-  __syncwarp();
-  float v[EPL];
-#pragma unroll
-  for (int j = 0; j < EPL; j += 4) {
-    const float4 t = *reinterpret_cast<const float4*>(d + e0 + j);
-    v[j] = t.x, v[j + 1] = t.y, v[j + 2] = t.z, v[j + 3] = t.w;
+    return c;
+  };
+  auto logit = [&](long long n, const Choice& c) {
+    return p.sigmoid && c.e >= 0 ? to_f<T>(reinterpret_cast<const T*>(p.logits)[n * p.ld + c.e]) : 0.f;
+  };
+  auto scores = [&](float l, float& s, float& ds) {  // s and s' = s (1 - s)
+    const float x = expf(-fabsf(l)), q = 1.f / (1.f + x);
+    s = (l >= 0.f ? 1.f : x) * q;
+    ds = x * q * q;
+  };
+  const long long stride = (long long)gridDim.x * TOKENS;
+  long long n = (long long)blockIdx.x * TOKENS + tok;
+  const long long rounds = (p.N - (long long)blockIdx.x * TOKENS + stride - 1) / stride;  // the block's, for the barriers
+  Choice cur, nxt;
+  float lc = 0.f;
+  if (one) {
+    cur = choice(n, li);
+    nxt = choice(n + stride, li);
+    lc = logit(n, cur);
   }
-  if (!p.sigmoid && !p.renorm) {  // every expert's probability takes part
-    float l[EPL];
-    float mx = -INFINITY;
-    if (live) load_logits<T, EPL>(p, n, e0, l);
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      if (!live) l[j] = 0.f;
-      mx = fmaxf(mx, l[j]);
+  for (long long it = 0; it < rounds; ++it, n += stride) {
+    Choice far;
+    float ln = 0.f;
+    if (one) {
+      far = choice(n + 2 * stride, li);
+      ln = logit(n + stride, nxt);
     }
-    mx = lanes_max<L>(mx);
-    if (mx == -INFINITY) mx = 0.f;
-    float z = 0.f;
+    const bool in = n < p.N;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      l[j] = e0 + j < p.E ? expf(l[j] - mx) : 0.f;
-      z += l[j];
+    for (int j = 0; j < EPL; j += 4) *reinterpret_cast<float4*>(d + e0 + j) = make_float4(0.f, 0.f, 0.f, 0.f);
+    // m = sum of r dw and S = sum of the chosen s
+    float m = 0.f, total = 0.f, se = 0.f, de = 0.f;
+    if (one) {
+      if (p.sigmoid && cur.e >= 0) scores(lc, se, de);
+      m = cur.w * cur.g;
+      total = se;
+    } else {
+      for (int r = li; r < p.k; r += L) {
+        const Choice c = choice(n, r);
+        if (p.sigmoid && c.e >= 0) scores(logit(n, c), se, de);
+        m = fmaf(c.w, c.g, m);
+        total += c.e >= 0 ? se : 0.f;
+      }
     }
-    z = fmaxf(lanes_sum<L>(z), 1e-20f);
-    if (live) {
+    m = lanes_sum<L>(m) / p.scale;
+    if (p.sigmoid && p.renorm) total = lanes_sum<L>(total) + 1e-20f;
+    __syncwarp();
+    auto put = [&](const Choice& c, float ds) {
+      const float up = p.renorm ? c.g - m : c.g;
+      if (c.e >= 0) d[c.e] = p.sigmoid ? p.scale * up * ds / (p.renorm ? total : 1.f) : c.w * up;
+    };
+    if (one) {
+      put(cur, de);
+    } else {
+      for (int r = li; r < p.k; r += L) {
+        const Choice c = choice(n, r);
+        if (p.sigmoid && c.e >= 0) scores(logit(n, c), se, de);
+        put(c, de);
+      }
+    }
+    __syncwarp();
+    float v[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; j += 4) {
+      const float4 t = *reinterpret_cast<const float4*>(d + e0 + j);
+      v[j] = t.x, v[j + 1] = t.y, v[j + 2] = t.z, v[j + 3] = t.w;
+    }
+    if (!p.sigmoid && !p.renorm) {  // every expert's probability takes part (m is 0 for a token without experts)
+      float l[EPL];
+      float mx = -INFINITY;
+      if (in) load_logits<T, EPL>(p, n, e0, l);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        if (!in) l[j] = 0.f;
+        mx = fmaxf(mx, l[j]);
+      }
+      mx = lanes_max<L>(mx);
+      if (mx == -INFINITY) mx = 0.f;
+      float z = 0.f;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        l[j] = e0 + j < p.E ? expf(l[j] - mx) : 0.f;
+        z += l[j];
+      }
+      z = fmaxf(lanes_sum<L>(z), 1e-20f);
       const float f = p.scale * m / z;
+      if (m != 0.f)
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) v[j] = fmaf(-f, l[j], v[j]);
+        for (int j = 0; j < EPL; ++j) v[j] = fmaf(-f, l[j], v[j]);
     }
-  }
-  if (!in) return;
-  T* out = dlogits + n * p.E;
-  if (p.vec) {
+    if (in) {
+      T* out = dlogits + n * p.E;
+      if (p.vec) {
 #pragma unroll
-    for (int j = 0; j < EPL; j += 8)
-      if (e0 + j < p.E) store_vec<T, 8>(out + e0 + j, *reinterpret_cast<const float(*)[8]>(&v[j]));
-  } else {
+        for (int j = 0; j < EPL; j += 8)
+          if (e0 + j < p.E) store_vec<T, 8>(out + e0 + j, *reinterpret_cast<const float(*)[8]>(&v[j]));
+      } else {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j)
-      if (e0 + j < p.E) out[e0 + j] = from_f<T>(v[j]);
+        for (int j = 0; j < EPL; ++j)
+          if (e0 + j < p.E) out[e0 + j] = from_f<T>(v[j]);
+      }
+    }
+    cur = nxt;
+    nxt = far;
+    lc = ln;
   }
 }
 
@@ -361,7 +413,9 @@ cudaError_t route_run(RouteParams p, const float* dw, void* dlogits, cudaStream_
   p.group_lanes = p.group_size % EPL == 0 && (gl & (gl - 1)) == 0 ? gl : 0;
   const unsigned grid = (unsigned)((p.N + TOKENS - 1) / TOKENS);
   if (dlogits != nullptr) {
-    route_bwd_kernel<T, L, EPL><<<grid, ROUTE_WARPS * 32, 0, s>>>(p, dw, static_cast<T*>(dlogits));
+    // blocks that the SMs hold, walking the tokens
+    route_bwd_kernel<T, L, EPL><<<std::min<unsigned>(grid, num_sms() * ROUTE_BWD_BLOCKS), ROUTE_WARPS * 32, 0, s>>>(
+        p, dw, static_cast<T*>(dlogits));
   } else {
     const bool scan = p.groups > 1 && p.group_lanes == 0;
     const size_t smem = (size_t)TOKENS * 4 * (p.k + (scan ? p.E + kRouteMaxGroups : 0));
