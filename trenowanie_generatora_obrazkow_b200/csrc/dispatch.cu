@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) dispatch_kernel(ExpertRows r, 
 // J rows of U vectors per lane in flight, and U vectors of fp32 sums: few choices take wide parts, many take narrow parts
 // and more rows (8191 x 1280, 8 choices: U 4, J 2 50.9 us).
 template <typename T, int V, int U, int J>
-__global__ void __launch_bounds__(ROW_WARPS * 32) combine_kernel(ExpertRows r, const T* __restrict__ y,
+__global__ void __launch_bounds__(ROW_WARPS * 32, 4) combine_kernel(ExpertRows r, const T* __restrict__ y,
                                                                  const float* __restrict__ w, T* __restrict__ out,
                                                                  int parts, int cols) {
   const long long unit = (long long)blockIdx.x * ROW_WARPS + warp_id();

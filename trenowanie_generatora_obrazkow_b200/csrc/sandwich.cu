@@ -597,9 +597,8 @@ __global__ void __launch_bounds__(32 * RED_WARPS) sandwich_reduce_kernel(Sandwic
     const bool live = b < b1 && ok;
     float s[3] = {0.f, 0.f, 0.f};
     if (live) {
-      const int first = (int)((long long)b * T_rows / q.rows_per_cta);
-      const int last = (int)(((long long)(b + 1) * T_rows - 1) / q.rows_per_cta);
-#pragma unroll 4
+      const int first = b * T_rows / q.rows_per_cta, last = ((b + 1) * T_rows - 1) / q.rows_per_cta;  // rows fit an int
+#pragma unroll 8
       for (int k = first + share; k <= last; k += wps) {
         const float* src = q.partial + (long long)(k + b) * 3 * p.D + c;
 #pragma unroll
