@@ -12,6 +12,9 @@
 //     mean(a g yn) = mean(a yn (dx' + rx dh cw)) - rx m mean(a yn n),    m = mean(dh cw n).
 // Statistics and sums are fp32; x' is rounded only when it is stored, so h comes from the unrounded sum.
 //
+// Bound by memory (4 rows forward, 6 backward): 32 x 1024 x 2048 bf16 takes 96 / 167 us, 0.85 / 0.74 of a plain copy's rate;
+// below it the row reductions' barriers and, backward, 128 registers (16 warps per SM) are what is left.
+//
 // Column sums: a unit (a CTA, or a group of its threads) owns a contiguous span of rows and writes one partial row (three
 // sums per channel) per sample it meets. Entry unit + sample is unique (along the spans both only grow), so
 // units + samples entries hold them all; two small kernels add them in a fixed order.
