@@ -152,6 +152,36 @@ def test_route_gradient_by_differences():
                 assert (num - x.grad[:, e].double()).abs().max() < 2e-6  # h^2 third derivative + fp32 gradient
 
 
+@pytest.mark.parametrize("score,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True)])
+def test_route_padding_rows_stop_gradients(score, renorm):
+    """NaN that reaches a padding row's weights does not reach its logits; an error reaches second derivatives."""
+    g = gen(14)
+    logits = rnd(g, 6, 40).requires_grad_()
+    valid = torch.tensor([True, False, True, True, False, True], device="cuda")
+    w, _ = Rt.route_experts(logits, 3, score=score, renorm=renorm, valid=valid)
+    dw = rnd(g, 6, 3)
+    dw[~valid] = math.nan
+    w.backward(dw)
+    assert torch.isfinite(logits.grad).all() and (logits.grad[~valid] == 0).all() and (logits.grad[0] != 0).any()
+    w, _ = Rt.route_experts(logits, 3)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(w.sum(), logits, create_graph=True)
+
+
+def test_broadcast_rows_share_their_gradient():
+    """One modulation row expanded over the samples (stride 0): its gradient is the sum over them."""
+    g = gen(15)
+    ins = sandwich_inputs(g, 3, 20, 256, True, True, True, True, F32)
+    one = {n: ins[n][:1].clone().requires_grad_() for n in ("gate", "shift", "scale")}
+    each = {n: one[n].detach().expand(3, -1).contiguous().requires_grad_() for n in one}
+    for rows in ({n: t.expand(3, -1) for n, t in one.items()}, each):
+        a, b = Fz.sandwich_norm(**{**ins, **rows})
+        (a.square().sum() + b.square().sum()).backward()
+    for n in one:
+        want = each[n].grad.sum(0, keepdim=True)
+        assert torch.allclose(one[n].grad, want, rtol=1e-5, atol=1e-5 * want.abs().max().item())
+
+
 def test_route_strided_rows_and_empty():
     g = gen(4)
     wide = rnd(g, 50, 40)

@@ -427,6 +427,11 @@ using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
 using torch::autograd::variable_list;
 
+// The backward kernels record nothing: a second derivative would silently miss their part.
+void first_order_only() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "routed block operators are differentiable once (create_graph=True is not "
+              "supported)");
+}
 bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : ts)
@@ -500,6 +505,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
     return {w, idx};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only();
     const auto saved = ctx->get_saved_variables();
     at::Tensor d = route_bwd(saved[0], saved[1], saved[2], grads[0].contiguous(), ctx->saved_data["sigmoid"].toBool(),
                              ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
@@ -525,6 +531,7 @@ struct DispatchFn : public torch::autograd::Function<DispatchFn> {
     return expert_dispatch(x, slot, offsets, counts, capacity, rows);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only();
     const auto s = ctx->get_saved_variables();
     variable_list out(6);
     out[0] = expert_combine(grads[0].contiguous(), OptT(), s[0], s[1], s[2], ctx->saved_data["capacity"].toInt());
@@ -547,6 +554,7 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
     return expert_combine(y, w, slot, offsets, counts, capacity);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only();
     const auto s = ctx->get_saved_variables();
     at::Tensor g = grads[0];
     if (g.size(1) > 1 && g.stride(1) != 1) g = g.contiguous();
@@ -582,6 +590,7 @@ struct SandwichFn : public torch::autograd::Function<SandwichFn> {
     return {r[0], r[1]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only();
     const auto s = ctx->get_saved_variables();
     const at::Tensor dx_new = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
     const at::Tensor dh = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
@@ -639,6 +648,7 @@ struct RopeAxesFn : public torch::autograd::Function<RopeAxesFn> {
     return {qo.view(q.sizes()), ko.view(k.sizes())};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only();
     const auto s = ctx->get_saved_variables();
     const WeightGrad gq(ctx, "q_w"), gk(ctx, "k_w");
     // the two weights' sums come together: one that needs no gradient gets a scratch row

@@ -173,12 +173,9 @@ cudaError_t plan_launch(const PlanParams& p, cudaStream_t s) {
   const bool cluster = p.A > 8192;
   const int threads = cluster ? 1024 : std::min(1024, std::max(128, (p.A + 31) / 32 * 32));
   const size_t smem = sizeof(int) * ((PLAN_PITCH + 2) * p.E + 32);
-  static bool set = false;
-  if (!set) {
-    cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(sizeof(int) * ((PLAN_PITCH + 2) * kRouteMaxExperts + 32)));
+  if (smem > 48 * 1024) {  // over about 340 experts
+    cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    set = true;
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(cluster ? PLAN_CTAS : 1);

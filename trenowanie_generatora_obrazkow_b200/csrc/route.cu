@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_bwd_kernel(RouteParams
     if (n < p.N && r < p.k) {
       c.e = p.idx[n * p.k + r];
       c.w = p.w[n * p.k + r];
-      c.g = dw[n * p.k + r];
+      c.g = c.e >= 0 ? dw[n * p.k + r] : 0.f;  // whatever reaches a padding row ends here
     }
     return c;
   };
