@@ -445,6 +445,46 @@ def test_rope_axes_is_the_2d_rope():
     check(frac, want, 2 * q.double().abs().amax(), "fractions")
 
 
+def test_gradients_by_differences():
+    """Directional derivatives of the fp32 kernels' own forwards (central differences, h = 2^-6) against <gradient,
+    direction>. The difference of the sum of n = 2 * 3 * 24 * 64 outputs of size 1 carries n^1/2 2^-24 / h = 4e-4 of
+    rounding and h^2 / 6 = 4e-5 of the third derivative per unit, both far below 1e-2 of a derivative's size."""
+    g = gen(16)
+    ins = sandwich_inputs(g, 2, 24, 192, True, True, True, True, F32)
+    up = [rnd(g, 2, 24, 192) for _ in range(2)]
+    q, k = rnd(g, 2, 24, 3, 64), rnd(g, 2, 24, 1, 64)
+    pos = torch.randint(0, 50, (2, 24, 2), device="cuda", generator=g)
+    plan = Rt.expert_plan(choices(g, 48, 6, 2), 6, capacity=20)
+
+    def sandwich(x, y, gate, post_w, w, shift, scale):
+        return Fz.sandwich_norm(x, y, gate, post_w, w, shift, scale, res_scale=0.7)
+
+    def rope(q, k, qw, kw):
+        return Fz.rope_axes(q, k, pos, (32, 24), q_w=qw, k_w=kw)
+
+    def rows(x, y, w):
+        return Rt.expert_dispatch(x, plan), Rt.expert_combine(y, w, plan)
+    cases = [(sandwich, [t.contiguous() for t in ins.values()], up),
+             (rope, [q, k, rnd(g, 64, std=0.1, mean=1.0), rnd(g, 64, std=0.1, mean=1.0)],
+              [rnd(g, 2, 24, 3, 64), rnd(g, 2, 24, 1, 64)]),
+             (rows, [rnd(g, 48, 96), rnd(g, plan.rows, 96), torch.rand(48, 2, device="cuda", generator=g)],
+              [rnd(g, plan.rows, 96), rnd(g, 48, 96)])]
+    h = 2.0 ** -6
+    for fn, xs, ups in cases:
+        def f(args):
+            with torch.no_grad():
+                return sum((o.double() * u.double()).sum() for o, u in zip(fn(*args), ups)).item()
+        leaves = [x.clone().requires_grad_() for x in xs]
+        torch.autograd.backward(list(fn(*leaves)), ups)
+        for i, leaf in enumerate(leaves):
+            d = rnd(g, *leaf.shape)
+            shifted = lambda s: [x + s * h * d if j == i else x for j, x in enumerate(xs)]
+            num = (f(shifted(1)) - f(shifted(-1))) / (2 * h)
+            want = (leaf.grad.double() * d.double()).sum().item()
+            size = (leaf.grad.double().norm() * d.double().norm() / d.numel() ** 0.5).item()
+            assert abs(num - want) < 1e-2 * max(size, 1.0), (fn.__name__, i, num, want, size)
+
+
 def test_ops_on_a_side_stream():
     """Inputs made on one stream, used on another after it waited: results as on the default stream."""
     g = gen(13)
