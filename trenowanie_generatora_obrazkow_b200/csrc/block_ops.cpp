@@ -1,6 +1,7 @@
 // Torch-facing wrappers of the routed block's kernels (block_ops.h): argument checks, outputs, launches on the current
 // stream. Registered in the extension module by ops.cpp.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -34,6 +35,12 @@ int elem_of(const at::Tensor& t, const char* what) {
   }
   return -1;
 }
+// An uninitialised contiguous tensor on as's device, past the dispatcher (half the host time of at::empty; a small step
+// makes a dozen of them).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& as) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, as.device(), c10::nullopt));
+}
+at::Tensor fresh_like(const at::Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t); }
 bool given(const OptT& t) { return t.has_value() && t->defined(); }
 void same_device(const at::Tensor& t, const at::Tensor& as, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.device() == as.device(), what, ": a tensor on ", as.device(), " expected");
@@ -94,8 +101,8 @@ std::tuple<at::Tensor, at::Tensor> route_fwd(at::Tensor logits, OptT bias, OptT 
                 "route: valid bool [N]");
     p.valid = valid->data_ptr<bool>();
   }
-  at::Tensor w = at::empty({p.N, k}, logits.options().dtype(at::kFloat));
-  at::Tensor idx = at::empty({p.N, k}, logits.options().dtype(at::kInt));
+  at::Tensor w = fresh({p.N, k}, at::kFloat, logits);
+  at::Tensor idx = fresh({p.N, k}, at::kInt, logits);
   p.w = w.data_ptr<float>();
   p.idx = idx.data_ptr<int>();
   BLOCK_LAUNCH(route_fwd_launch(p, elem_of(logits, "route"), at::cuda::getCurrentCUDAStream()), p.N > 0);
@@ -112,7 +119,7 @@ at::Tensor route_bwd(at::Tensor logits, at::Tensor w, at::Tensor idx, at::Tensor
   p.w = const_cast<float*>(vec_f32(w, w.numel(), logits, "route_bwd: w"));
   p.idx = idx.data_ptr<int>();
   const float* g = vec_f32(dw, w.numel(), logits, "route_bwd: dw");
-  at::Tensor d = at::empty({p.N, p.E}, logits.options());
+  at::Tensor d = fresh({p.N, p.E}, logits.scalar_type(), logits);
   BLOCK_LAUNCH(route_bwd_launch(p, g, d.data_ptr(), elem_of(logits, "route_bwd"), at::cuda::getCurrentCUDAStream()),
                p.N > 0);
   return d;
@@ -131,9 +138,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> expert_plan(at::Tensor idx, int64
   p.A = (int)idx.numel();
   p.E = (int)experts;
   p.capacity = (int)capacity;
-  at::Tensor slot = at::empty_like(idx);
-  at::Tensor offsets = at::empty({experts + 1}, idx.options());
-  at::Tensor counts = at::empty({experts}, idx.options());
+  at::Tensor slot = fresh_like(idx);
+  at::Tensor offsets = fresh({experts + 1}, at::kInt, idx);
+  at::Tensor counts = fresh({experts}, at::kInt, idx);
   p.slot = slot.data_ptr<int>();
   p.offsets = offsets.data_ptr<int>();
   p.counts = counts.data_ptr<int>();
@@ -171,7 +178,7 @@ at::Tensor expert_dispatch(at::Tensor x, at::Tensor slot, at::Tensor offsets, at
               "expert_dispatch: x [N, D] with contiguous rows, one per planned token");
   const c10::cuda::CUDAGuard guard(x.device());
   const ExpertRows r = expert_rows(slot, offsets, counts, capacity, rows, x.size(1), x);
-  at::Tensor xs = at::empty({rows, x.size(1)}, x.options());
+  at::Tensor xs = fresh({rows, x.size(1)}, x.scalar_type(), x);
   BLOCK_LAUNCH(dispatch_launch(r, x.data_ptr(), x.stride(0), xs.data_ptr(), elem_of(x, "expert_dispatch"),
                                at::cuda::getCurrentCUDAStream()), 1);
   return xs;
@@ -183,7 +190,7 @@ at::Tensor expert_combine(at::Tensor y, OptT w, at::Tensor slot, at::Tensor offs
   const c10::cuda::CUDAGuard guard(y.device());
   const ExpertRows r = expert_rows(slot, offsets, counts, capacity, y.size(0), y.size(1), y);
   const float* wp = vec_f32(w, slot.numel(), y, "expert_combine: w");
-  at::Tensor out = at::empty({r.N, y.size(1)}, y.options());
+  at::Tensor out = fresh({r.N, y.size(1)}, y.scalar_type(), y);
   BLOCK_LAUNCH(combine_launch(r, y.data_ptr(), wp, out.data_ptr(), elem_of(y, "expert_combine"),
                               at::cuda::getCurrentCUDAStream()), 1);
   return out;
@@ -199,7 +206,7 @@ std::tuple<at::Tensor, at::Tensor> expert_combine_bwd(at::Tensor y, at::Tensor w
   const c10::cuda::CUDAGuard guard(y.device());
   const ExpertRows r = expert_rows(slot, offsets, counts, capacity, y.size(0), y.size(1), y);
   const float* wp = vec_f32(w, slot.numel(), y, "expert_combine_bwd: w");
-  at::Tensor dy = at::empty_like(y), dw = at::empty({r.N, r.k}, y.options().dtype(at::kFloat));
+  at::Tensor dy = fresh_like(y), dw = fresh({r.N, r.k}, at::kFloat, y);
   BLOCK_LAUNCH(combine_bwd_launch(r, y.data_ptr(), wp, dout.data_ptr(), dout.stride(0), dy.data_ptr(),
                                   dw.data_ptr<float>(), elem_of(y, "expert_combine_bwd"),
                                   at::cuda::getCurrentCUDAStream()), 1);
@@ -250,16 +257,15 @@ std::vector<at::Tensor> sandwich_fwd(at::Tensor x, at::Tensor y, OptT gate, OptT
                                      double res_scale, double eps, at::Tensor err) {
   SandwichParams p = sandwich_params(x, y, gate, post_w, w, shift, scale, res_scale, eps);
   const c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor x_new = at::empty_like(x), h, ry, rx;
+  at::Tensor x_new = fresh_like(x), h, ry, rx;
   p.x_new = x_new.data_ptr();
-  auto f32 = x.options().dtype(at::kFloat);
   if (p.post_w != nullptr) {
-    ry = at::empty({p.M}, f32);
+    ry = fresh({p.M}, at::kFloat, x);
     p.rstd_y = ry.data_ptr<float>();
   }
   if (p.w != nullptr) {
-    h = at::empty_like(x);
-    rx = at::empty({p.M}, f32);
+    h = fresh_like(x);
+    rx = fresh({p.M}, at::kFloat, x);
     p.h = h.data_ptr();
     p.rstd_x = rx.data_ptr<float>();
   }
@@ -287,18 +293,17 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
   };
   q.dx_new = grad_in(dx_new, "sandwich_bwd: dx_new");
   q.dh = grad_in(dh, "sandwich_bwd: dh");
-  at::Tensor dx = at::empty_like(x), dy = at::empty_like(x), dgate, dshift, dscale;
+  at::Tensor dx = fresh_like(x), dy = fresh_like(x), dgate, dshift, dscale;
   q.dx = dx.data_ptr();
   q.dy = dy.data_ptr();
   const int64_t B = x.size(0), D = x.size(2);
   if (p.gate != nullptr) {
-    dgate = at::empty({B, D}, x.options());
+    dgate = fresh({B, D}, x.scalar_type(), x);
     q.dgate = dgate.data_ptr();
   }
   if (p.scale != nullptr) {
-    at::Tensor both = at::empty({2, B, D}, x.options());
-    dshift = both[0];
-    dscale = both[1];
+    dshift = fresh({B, D}, x.scalar_type(), x);
+    dscale = fresh({B, D}, x.scalar_type(), x);
     q.dshift = dshift.data_ptr();
     q.dscale = dscale.data_ptr();
   }
@@ -316,7 +321,7 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
   const int elem = elem_of(x, "sandwich_bwd");
   BLOCK_LAUNCH(sandwich_bwd_plan(p, elem, &q), 0);
   const int64_t entries = q.ctas + B, floats = entries * 3 * D + (int64_t)q.groups * 2 * D;
-  at::Tensor scratch = at::empty({floats}, x.options().dtype(at::kFloat));
+  at::Tensor scratch = fresh({floats}, at::kFloat, x);
   q.partial = scratch.data_ptr<float>();
   q.wpart = q.partial + entries * 3 * D;
   BLOCK_LAUNCH(sandwich_bwd_launch(p, q, elem, err_word(err, x), at::cuda::getCurrentCUDAStream()), 3);
@@ -324,23 +329,38 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
 }
 
 // -------------------------------------------------------------------------------------------------- multi-axis rotary
+// [M, H, d] rows or [B, T, H, d] with evenly strided tokens, the heads of a token contiguous: the token stride; else -1
+int64_t token_stride(const at::Tensor& t) {
+  const int64_t n = t.dim(), d = t.size(n - 1), H = t.size(n - 2), T = t.size(n - 3), B = n == 4 ? t.size(0) : 1;
+  if ((d > 1 && t.stride(n - 1) != 1) || (H > 1 && t.stride(n - 2) != d)) return -1;
+  if (B > 1 && T > 1 && t.stride(0) != T * t.stride(1)) return -1;
+  return T > 1 || B <= 1 ? t.stride(n - 3) : t.stride(0);
+}
+at::Tensor even_tokens(const at::Tensor& t) {
+  return (t.dim() == 3 || t.dim() == 4) && token_stride(t) < 0 ? t.contiguous() : t;
+}
+
 RopeAxesParams rope_params(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& freq,
                            const at::Tensor& axis, const OptT& q_w, const OptT& k_w, bool interleaved, double eps) {
-  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3, "rope_axes: q [M, Hq, d], k [M, Hkv, d]");
+  const int64_t n = q.dim();
+  TORCH_CHECK(q.is_cuda() && (n == 3 || n == 4) && k.dim() == n && pos.dim() == n - 1,
+              "rope_axes: q [B, T, Hq, d], k [B, T, Hkv, d], pos [B, T, axes] (or all without B)");
   same_device(k, q, "rope_axes: k");
   same_device(pos, q, "rope_axes: pos");
   same_device(freq, q, "rope_axes: freq");
   same_device(axis, q, "rope_axes: axis");
-  const int64_t M = q.size(0), hd = q.size(2);
-  TORCH_CHECK(k.size(0) == M && k.size(2) == hd && k.scalar_type() == q.scalar_type(), "rope_axes: k as q");
-  auto heads_ok = [&](const at::Tensor& t) {
-    return (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) == hd);
-  };
-  TORCH_CHECK(heads_ok(q) && heads_ok(k), "rope_axes: the heads of a token must be contiguous");
-  TORCH_CHECK(hd >= 2 && hd <= 1024 && M < (1ll << 31) && q.size(1) >= 1 && k.size(1) >= 1,
+  int64_t M = 1;
+  for (int64_t i = 0; i + 2 < n; ++i) {
+    M *= q.size(i);
+    TORCH_CHECK(k.size(i) == q.size(i) && pos.size(i) == q.size(i), "rope_axes: k and pos for q's tokens");
+  }
+  const int64_t hd = q.size(n - 1), axes = pos.size(n - 2), hq = q.size(n - 2), hkv = k.size(n - 2);
+  TORCH_CHECK(k.size(n - 1) == hd && k.scalar_type() == q.scalar_type(), "rope_axes: k as q");
+  const int64_t q_ts = token_stride(q), k_ts = token_stride(k);
+  TORCH_CHECK(q_ts >= 0 && k_ts >= 0, "rope_axes: the heads of a token must be contiguous, its tokens evenly strided");
+  TORCH_CHECK(hd >= 2 && hd <= 1024 && M < (1ll << 31) && hq >= 1 && hkv >= 1,
               "rope_axes: head dim 2 to 1024, at least one head of each");
-  TORCH_CHECK(pos.dim() == 2 && pos.size(0) == M && pos.is_contiguous() && pos.size(1) >= 1 &&
-                  pos.size(1) <= kRopeMaxAxes && (pos.scalar_type() == at::kInt || pos.scalar_type() == at::kFloat),
+  TORCH_CHECK(pos.is_contiguous() && axes >= 1 && axes <= kRopeMaxAxes && (pos.scalar_type() == at::kInt || pos.scalar_type() == at::kFloat),
               "rope_axes: pos int32 or fp32 [M, axes], at most ", kRopeMaxAxes, " axes");
   TORCH_CHECK(freq.scalar_type() == at::kFloat && freq.is_contiguous() && freq.dim() == 2 && freq.size(0) == 2 &&
                   axis.scalar_type() == at::kInt && axis.is_contiguous() && axis.numel() == freq.size(1) &&
@@ -349,8 +369,8 @@ RopeAxesParams rope_params(const at::Tensor& q, const at::Tensor& k, const at::T
   RopeAxesParams p{};
   p.q = q.data_ptr();
   p.k = k.data_ptr();
-  p.q_ts = q.stride(0);
-  p.k_ts = k.stride(0);
+  p.q_ts = q_ts;
+  p.k_ts = k_ts;
   p.pos = pos.data_ptr();
   p.pos_f32 = pos.scalar_type() == at::kFloat;
   p.freq = freq.data_ptr<float>();
@@ -360,9 +380,9 @@ RopeAxesParams rope_params(const at::Tensor& q, const at::Tensor& k, const at::T
   TORCH_CHECK((p.q_w == nullptr) == (p.k_w == nullptr), "rope_axes: q and k norm weights both or neither");
   p.eps = (float)eps;
   p.M = (int)M;
-  p.axes = (int)pos.size(1);
-  p.hq = (int)q.size(1);
-  p.hkv = (int)k.size(1);
+  p.axes = (int)axes;
+  p.hq = (int)hq;
+  p.hkv = (int)hkv;
   p.hd = (int)hd;
   p.rot = (int)(2 * freq.size(1));
   p.interleaved = interleaved;
@@ -373,7 +393,7 @@ std::tuple<at::Tensor, at::Tensor> rope_axes_fwd(at::Tensor q, at::Tensor k, at:
                                                  at::Tensor axis, OptT q_w, OptT k_w, bool interleaved, double eps) {
   RopeAxesParams p = rope_params(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
   const c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  at::Tensor qo = fresh_like(q), ko = fresh_like(k);
   p.q_out = qo.data_ptr();
   p.k_out = ko.data_ptr();
   BLOCK_LAUNCH(rope_axes_fwd_launch(p, elem_of(q, "rope_axes"), at::cuda::getCurrentCUDAStream()), p.M > 0);
@@ -394,14 +414,14 @@ std::tuple<at::Tensor, at::Tensor> rope_axes_bwd(at::Tensor dq, at::Tensor dk, a
   TORCH_CHECK(grad_ok(dq, q) && grad_ok(dk, k), "rope_axes_bwd: dq / dk contiguous, as q / k");
   auto out_ok = [&](const at::Tensor& o, const at::Tensor& t) {
     return o.sizes() == t.sizes() && o.scalar_type() == t.scalar_type() && o.device() == t.device() &&
-           o.stride(2) == 1 && o.stride(1) == p.hd;
+           token_stride(o) >= 0;
   };
   TORCH_CHECK((!given(dq_out) || out_ok(*dq_out, q)) && (!given(dk_out) || out_ok(*dk_out, k)),
               "rope_axes_bwd: dq_out / dk_out as q / k, a token's heads contiguous");
-  at::Tensor dqi = given(dq_out) ? *dq_out : at::empty_like(dq), dki = given(dk_out) ? *dk_out : at::empty_like(dk);
+  at::Tensor dqi = given(dq_out) ? *dq_out : fresh_like(dq), dki = given(dk_out) ? *dk_out : fresh_like(dk);
   at::Tensor partial;
-  p.dq_ts = dqi.stride(0);
-  p.dk_ts = dki.stride(0);
+  p.dq_ts = token_stride(dqi);
+  p.dk_ts = token_stride(dki);
   float* gq = acc_f32(dq_w, p.hd, q, "rope_axes_bwd: dq_w");
   float* gk = acc_f32(dk_w, p.hd, q, "rope_axes_bwd: dk_w");
   TORCH_CHECK((gq == nullptr) == (gk == nullptr) && (gq == nullptr || p.q_w != nullptr),
@@ -412,7 +432,7 @@ std::tuple<at::Tensor, at::Tensor> rope_axes_bwd(at::Tensor dq, at::Tensor dk, a
     return {dqi, dki};
   }
   if (gq != nullptr)
-    partial = at::empty({rope_axes_bwd_ctas(), 2, p.hd}, q.options().dtype(at::kFloat));
+    partial = fresh({rope_axes_bwd_ctas(), 2, p.hd}, at::kFloat, q);
   BLOCK_LAUNCH(rope_axes_bwd_launch(p, dq.data_ptr(), dk.data_ptr(), dqi.data_ptr(), dki.data_ptr(),
                                     gq != nullptr ? partial.data_ptr<float>() : nullptr, gq, gk, add_q_w, add_k_w,
                                     elem_of(q, "rope_axes_bwd"), at::cuda::getCurrentCUDAStream()),
@@ -473,14 +493,14 @@ struct WeightGrad {
     if (w.is_leaf() && w.scalar_type() == at::kFloat) {
       at::Tensor& have = w.mutable_grad();
       if (!have.defined()) {
-        have = at::empty_like(w);
+        have = fresh_like(w);
         direct = true;
       } else if (have.scalar_type() == at::kFloat && have.is_contiguous() && have.device() == w.device()) {
         direct = add = true;
       }
       if (direct) g = have.detach();
     }
-    if (!direct) g = at::empty_like(w);
+    if (!direct) g = fresh_like(w);
   }
   at::Tensor done() const {  // what autograd still has to add
     if (!direct) return g;
@@ -627,25 +647,17 @@ std::tuple<at::Tensor, OptT> sandwich_norm(at::Tensor x, at::Tensor y, OptT gate
   return {out[0], out.size() > 1 ? OptT(out[1]) : OptT()};
 }
 
-// [B, T, H, d] -> [B T, H, d], in place when the tokens are evenly strided and a token's heads are contiguous
-at::Tensor token_rows(const at::Tensor& t) {
-  const int64_t B = t.size(0), T = t.size(1), H = t.size(2), d = t.size(3);
-  const bool even = (d <= 1 || t.stride(3) == 1) && (H <= 1 || t.stride(2) == d) &&
-                    (B <= 1 || T <= 1 || t.stride(0) == T * t.stride(1));
-  if (!even) return t.contiguous().view({B * T, H, d});
-  return t.as_strided({B * T, H, d}, {T > 1 || B <= 1 ? t.stride(1) : t.stride(0), d, 1});
-}
 struct RopeAxesFn : public torch::autograd::Function<RopeAxesFn> {
   static variable_list forward(AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor pos, at::Tensor freq,
                                at::Tensor axis, OptT q_w, OptT k_w, bool interleaved, double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [qo, ko] = rope_axes_fwd(token_rows(q), token_rows(k), pos, freq, axis, q_w, k_w, interleaved, eps);
+    auto [qo, ko] = rope_axes_fwd(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
     ctx->save_for_backward({q, k, pos, freq, axis, or_undefined(q_w), or_undefined(k_w)});
     WeightGrad::keep(ctx, "q_w", q_w);
     WeightGrad::keep(ctx, "k_w", k_w);
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["eps"] = eps;
-    return {qo.view(q.sizes()), ko.view(k.sizes())};
+    return {qo, ko};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order_only();
@@ -653,14 +665,13 @@ struct RopeAxesFn : public torch::autograd::Function<RopeAxesFn> {
     const WeightGrad gq(ctx, "q_w"), gk(ctx, "k_w");
     // the two weights' sums come together: one that needs no gradient gets a scratch row
     at::Tensor wq = gq.g, wk = gk.g;
-    if (wq.defined() != wk.defined()) (wq.defined() ? wk : wq) = at::empty_like(wq.defined() ? wq : wk);
-    auto [dq, dk] = rope_axes_bwd(grads[0].contiguous().flatten(0, 1), grads[1].contiguous().flatten(0, 1),
-                                  token_rows(s[0]), token_rows(s[1]), s[2], s[3], s[4], opt(s[5]), opt(s[6]), opt(wq),
-                                  opt(wk), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(),
+    if (wq.defined() != wk.defined()) (wq.defined() ? wk : wq) = fresh_like(wq.defined() ? wq : wk);
+    auto [dq, dk] = rope_axes_bwd(grads[0].contiguous(), grads[1].contiguous(), s[0], s[1], s[2], s[3], s[4],
+                                  opt(s[5]), opt(s[6]), opt(wq), opt(wk), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(),
                                   gq.add, gk.add, OptT(), OptT());
     variable_list out(9);
-    out[0] = dq.view(s[0].sizes());
-    out[1] = dk.view(s[1].sizes());
+    out[0] = dq;
+    out[1] = dk;
     out[5] = gq.done();
     out[6] = gk.done();
     return out;
@@ -668,15 +679,11 @@ struct RopeAxesFn : public torch::autograd::Function<RopeAxesFn> {
 };
 std::tuple<at::Tensor, at::Tensor> rope_axes(at::Tensor q, at::Tensor k, at::Tensor pos, at::Tensor freq,
                                              at::Tensor axis, OptT q_w, OptT k_w, bool interleaved, double eps) {
-  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && pos.dim() == 3 && pos.size(0) == q.size(0) && pos.size(1) == q.size(1) &&
-                  k.size(0) == q.size(0) && k.size(1) == q.size(1),
-              "rope_axes: q [B, T, Hq, d], k [B, T, Hkv, d], pos [B, T, axes]");
-  pos = pos.to(pos.is_floating_point() ? at::kFloat : at::kInt).contiguous().view({q.size(0) * q.size(1), pos.size(2)});
+  q = even_tokens(q);
+  k = even_tokens(k);
+  pos = pos.to(pos.is_floating_point() ? at::kFloat : at::kInt).contiguous();
   const at::Tensor wq = or_undefined(q_w), wk = or_undefined(k_w);
-  if (!wants_grad({&q, &k, &wq, &wk})) {
-    auto [qo, ko] = rope_axes_fwd(token_rows(q), token_rows(k), pos, freq, axis, q_w, k_w, interleaved, eps);
-    return {qo.view(q.sizes()), ko.view(k.sizes())};
-  }
+  if (!wants_grad({&q, &k, &wq, &wk})) return rope_axes_fwd(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
   auto out = RopeAxesFn::apply(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
   return {out[0], out[1]};
 }
