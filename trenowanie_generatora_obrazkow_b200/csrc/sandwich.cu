@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(SW_THREADS) sandwich_bwd_any_kernel(SandwichPa
 // ------------------------------------------------------------------------------------------------------------------
 namespace {
 
-constexpr int SW_STAGES = 2;
+constexpr int SW_STAGES = 2;  // 3 and 4: the backward at 32 x 1024 x 2048 takes 178 and 207 us instead of 170
 constexpr int SW_MAX_VEC_D = 4096;
 constexpr int SW_MAX_GROUPS = 8;  // 256 threads of 32 each
 
