@@ -119,3 +119,9 @@ def test_refusals():
               lambda: Fz.rope_axes(q, q, pos, (8, 8)), lambda: Fz.rope_axes(q, q, pos, (3,))):
         with pytest.raises(ValueError):
             f()
+
+
+def test_axes_table_is_no_inference_tensor():
+    with torch.inference_mode():
+        freq, axis = Fz._axes_table((10, 6), 555.0, torch.device("cpu"))
+    assert not freq.is_inference() and not axis.is_inference()

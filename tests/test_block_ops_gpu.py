@@ -499,6 +499,40 @@ def test_ops_on_a_side_stream():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_rope_tables_made_while_sampling_serve_training():
+    """The first call for a set of axes may come under inference_mode; a training step after it saves the same tables."""
+    g = gen(31)
+    q, k = rnd(g, 1, 5, 2, 32), rnd(g, 1, 5, 1, 32)
+    pos = torch.arange(5, device="cuda", dtype=torch.int32).view(1, 5, 1)
+    with torch.inference_mode():
+        first = Fz.rope_axes(q, k, pos, (26,), theta=777.0)
+    q.requires_grad_()
+    again = Fz.rope_axes(q, k, pos, (26,), theta=777.0)
+    again[0].sum().backward()
+    assert torch.equal(first[0], again[0]) and q.grad is not None
+
+
+def test_one_expert_column_of_a_wider_table():
+    logits = torch.zeros(3, 8, device="cuda")[:, ::2][:, :1]
+    w, idx = Rt.route_experts(logits, 1)
+    assert (w == 1).all() and (idx == 0).all()
+
+
+def test_sandwich_scratch_without_modulation():
+    """Without gate or modulation all rows are one sample: the backward's scratch does not grow with B."""
+    g = gen(32)
+    x, y = (rnd(g, 20000, 1, 256, dtype=BF16).requires_grad_() for _ in range(2))
+    w = torch.ones(256, device="cuda", requires_grad=True)
+    x_new, h = Fz.sandwich_norm(x, y, w=w)
+    d = torch.ones_like(h)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    torch.autograd.backward([h], [d])
+    size = x.numel() * x.element_size()
+    assert torch.cuda.max_memory_allocated() - base <= 2 * size + (16 << 20)
+
+
 def test_refusals():
     """Bad arguments end in an exception before any launch."""
     x = torch.zeros(2, 4, 16, device="cuda", dtype=BF16)
@@ -514,6 +548,8 @@ def test_refusals():
            lambda: Rt.route_experts(torch.zeros(4, 8, device="cuda"), 2, scale=0.0),
            lambda: Rt.expert_plan(torch.zeros(4, device="cuda", dtype=torch.int32), 4),
            lambda: Rt.expert_plan(torch.zeros(4, 2, device="cuda", dtype=torch.int32), 4, capacity=0),
+           lambda: Rt.expert_plan(torch.zeros(4, 2, device="cuda", dtype=torch.int32), 4, capacity=2 ** 29 - 16384),
+           lambda: Rt.expert_plan(torch.zeros(4, 2, device="cuda", dtype=torch.int32), 4, capacity=2 ** 62),
            lambda: Fz.sandwich_norm(x, x[:1]), lambda: Fz.sandwich_norm(x, x, shift=x[:, 0], w=w),
            lambda: Fz.sandwich_norm(x, x, shift=x[:, 0], scale=x[:, 0]),
            lambda: Fz.sandwich_norm(x, x, gate=x[:1, 0], w=w), lambda: Fz.sandwich_norm(x, x.float(), w=w),
@@ -524,6 +560,8 @@ def test_refusals():
             lambda: Fz.rope_axes(q, q, pos, (8, 8)), lambda: Fz.rope_axes(q, q[..., :8], pos, (8,)),
             lambda: Fz.rope_axes(q, q, pos, (8,), q_w=w), lambda: Fz.rope_axes(q, q.float(), pos, (8,)),
             lambda: Fz.rope_axes(q, q, pos, (8,), theta=(1.0, 2.0))]
+    Fz.rope_axes(q, q, pos, (16,))
+    bad += [lambda: Fz.rope_axes(q[0], q[0], pos[0], (16,)), lambda: Fz.rope_axes(q, q, pos[..., :0], (16,))]
     plan = Rt.expert_plan(torch.zeros(4, 2, device="cuda", dtype=torch.int32), 4)
     bad += [lambda: Rt.expert_dispatch(torch.zeros(5, 16, device="cuda"), plan),
             lambda: Rt.expert_combine(torch.zeros(7, 16, device="cuda"), torch.zeros(4, 2, device="cuda"), plan),

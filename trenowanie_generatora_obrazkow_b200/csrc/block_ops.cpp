@@ -65,7 +65,8 @@ int* err_word(const at::Tensor& err, const at::Tensor& as) {
 // ---------------------------------------------------------------------------------------------------------- routing
 RouteParams route_params(const at::Tensor& logits, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups,
                          bool renorm, double scale) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, "route: logits [N, E] with contiguous rows");
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
+              "route: logits [N, E] with contiguous rows");
   const int64_t N = logits.size(0), E = logits.size(1);
   TORCH_CHECK(N < (1ll << 31) && E >= 1 && E <= kRouteMaxExperts, "route: 1 to ", kRouteMaxExperts, " experts");
   TORCH_CHECK(groups >= 1 && groups <= kRouteMaxGroups && E % groups == 0, "route: groups must divide the experts (at most ",
@@ -130,7 +131,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> expert_plan(at::Tensor idx, int64
   TORCH_CHECK(idx.is_cuda() && idx.dim() == 2 && idx.scalar_type() == at::kInt && idx.is_contiguous(),
               "expert_plan: idx int32 [N, k], contiguous");
   TORCH_CHECK(experts >= 1 && experts <= kRouteMaxExperts, "expert_plan: 1 to ", kRouteMaxExperts, " experts");
-  TORCH_CHECK(capacity >= 0 && capacity * experts < (1ll << 31) && idx.numel() < (1ll << 31) - 65536,
+  // a row number is an int, also before the capacity cuts it off
+  TORCH_CHECK(capacity >= 0 && capacity < (1ll << 31) && capacity * experts + idx.numel() < (1ll << 31) - 65536,
               "expert_plan: too many rows");
   const c10::cuda::CUDAGuard guard(idx.device());
   PlanParams p{};
@@ -320,7 +322,8 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
   }
   const int elem = elem_of(x, "sandwich_bwd");
   BLOCK_LAUNCH(sandwich_bwd_plan(p, elem, &q), 0);
-  const int64_t entries = q.ctas + B, floats = entries * 3 * D + (int64_t)q.groups * 2 * D;
+  // one entry per span and per sample that begins in it; without modulation all rows are one sample's
+  const int64_t entries = q.ctas + (p.gate != nullptr || p.scale != nullptr ? B : 1), floats = entries * 3 * D + (int64_t)q.groups * 2 * D;
   at::Tensor scratch = fresh({floats}, at::kFloat, x);
   q.partial = scratch.data_ptr<float>();
   q.wpart = q.partial + entries * 3 * D;

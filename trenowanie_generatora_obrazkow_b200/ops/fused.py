@@ -392,10 +392,11 @@ def _axes_table(axes, theta, device):
     key = (tuple(axes), theta if isinstance(theta, (int, float)) else tuple(theta), device)
     ent = _AXES_TABLES.get(key)
     if ent is None:
-        freq, axis = R.axes_frequencies(axes, theta)
-        rev = freq / (2 * math.pi)
-        hi = rev.float()
-        ent = (torch.stack([hi, (rev - hi.double()).float()]).to(device), axis.to(device))
+        with torch.inference_mode(False):  # a table made while sampling is saved by a later training step's backward
+            freq, axis = R.axes_frequencies(axes, theta)
+            rev = freq / (2 * math.pi)
+            hi = rev.float()
+            ent = (torch.stack([hi, (rev - hi.double()).float()]).to(device), axis.to(device))
         _AXES_TABLES[key] = ent
     return ent
 
@@ -420,8 +421,9 @@ def rope_axes(q, k, pos, axes, theta=10000.0, q_w=None, k_w=None, interleaved=Tr
             raise ValueError("rope_axes: one theta, or one per axis")
         if tuple(pos.shape) != (*q.shape[:2], len(axes)):
             raise ValueError(f"rope_axes: pos {(*q.shape[:2], len(axes))} expected, got {tuple(pos.shape)}")
-    elif pos.shape[-1] != len(axes):
-        raise ValueError(f"rope_axes: {len(axes)} positions per token expected, got {pos.shape[-1]}")
+    elif q.dim() != 4 or pos.shape[-1] != len(axes):  # the extension checks the rest
+        raise ValueError(f"rope_axes: q [B, T, Hq, d] and {len(axes)} positions per token expected, got "
+                         f"{tuple(q.shape)} and {tuple(pos.shape)}")
     if (q_w is None) != (k_w is None):
         raise ValueError("rope_axes: q_w and k_w come together")
     if not q.is_cuda:
@@ -540,6 +542,7 @@ class _AxesAttnFn(torch.autograd.Function):
         return o.view(B, T, hq * hd)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         qkv, q, k, o, lse, pos, freq, axis, q_w, k_w, kv_len = ctx.saved_tensors
         hq, hkv, hd, scale, interleaved, eps = ctx.dims
