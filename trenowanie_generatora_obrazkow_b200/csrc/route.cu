@@ -15,9 +15,10 @@
 // keys at the front (equal keys in index order), then each of the k steps takes the largest head of the L lanes; the
 // lowest lane that holds it wins (its experts have the lowest indices) and drops its head. What the weights need beyond the choice
 // is computed for the k chosen alone, from logits read again (they are in the cache).
-// 65536 x 256 fp32, 8 of 8 groups: forward 70 us (bound by instruction issue, 87 %: the exact scores of 256 experts cost
-// more than reading them), backward 29 us; 32768 x 8, 2 chosen: at the launch's own time.
+// 65536 x 256 fp32, k 8, 4 of 8 groups: forward 63 us (bound by instruction issue, about 740 per token: the exact sigmoids
+// and the group ranks 10 us each, the lists 20 us; 43 us for softmax without groups), backward 29 us; 32768 x 8, 2 chosen: at the launch's own time.
 #include <algorithm>
+#include <cfloat>
 
 #include "block_ops.h"
 #include "common.cuh"
@@ -29,13 +30,16 @@ namespace tgo {
 namespace {
 
 constexpr int ROUTE_WARPS = 4, ROUTE_BWD_BLOCKS = 8;
+// blocks per SM: 64 registers hold 8 experts per lane (9 blocks spill, 7 take 2 us more), 16 experts want 80
+constexpr int route_fwd_blocks(int epl) { return epl > 8 ? 6 : 8; }
 
-__device__ __forceinline__ unsigned order_key(float c) {
-  c += 0.f;  // -0 -> +0
+// c is no NaN and not -0
+__device__ __forceinline__ unsigned number_key(float c) {
   const unsigned u = __float_as_uint(c);
-  const unsigned key = (u >> 31) ? ~u : (u | 0x80000000u);
-  return c != c ? 1u : key;  // 0 is kept for "not a candidate"
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
+// NaN comes last; 0 is kept for "not a candidate"
+__device__ __forceinline__ unsigned order_key(float c) { return c != c ? 1u : number_key(c); }
 
 template <int L>
 __device__ __forceinline__ float lanes_max(float v) {
@@ -66,6 +70,13 @@ __device__ __forceinline__ unsigned lanes_or(unsigned v) {
   return v;
 }
 
+// shared memory of a forward warp, in bytes (a multiple of 8)
+__host__ __device__ __forceinline__ int route_warp_smem(const RouteParams& p, int tokens, int steps) {
+  const bool scan = p.groups > 1 && p.group_lanes == 0;
+  const int words = steps * tokens * (2 + p.k) + (scan ? tokens * (p.E + kRouteMaxGroups) : 0);
+  return (words + 1) / 2 * 8;
+}
+
 // EPL logits from expert e0 on; vec: E, the row stride and the base allow 16-byte loads of 8 logits
 template <typename T, int EPL>
 __device__ __forceinline__ void load_logits(const RouteParams& p, long long n, int e0, float (&l)[EPL]) {
@@ -86,68 +97,82 @@ __device__ __forceinline__ void load_logits(const RouteParams& p, long long n, i
   }
 }
 
-// sigmoid from e = exp(-|l|) <= 1: no overflow, small scores keep their relative precision
-__device__ __forceinline__ float sigmoid_of(float l, float e) { return (l >= 0.f ? 1.f : e) / (1.f + e); }
+// 1 + exp(-l) is rounded once relative to itself, so small scores keep their relative precision; below l = -88 they are 0
+__device__ __forceinline__ float sigmoid_of(float l) { return __frcp_rn(1.f + expf(-l)); }
 
 }  // namespace
 
+// A warp takes a batch of `steps` x 32 / L tokens: each step chooses for its tokens while the next step's logits are in
+// flight, and the end computes the weights of the whole batch's choices together, `slots` = the power of two from k on
+// lanes per token. One token per warp instead (its end in 8 of 32 lanes): 70 us against 63 us at 65536 x 256, k 8. A grid
+// of resident warps that walk the batches: 68 us, as the last round is not full.
 template <typename T, int L, int EPL>
-__global__ void __launch_bounds__(ROUTE_WARPS * 32) route_fwd_kernel(RouteParams p) {
-  constexpr int TOKENS = ROUTE_WARPS * 32 / L;  // per block
-  extern __shared__ uint8_t route_smem[];
-  // chosen experts [TOKENS][k]; for groups that do not fall on whole lanes also selection and group scores
-  int* si = reinterpret_cast<int*>(route_smem);
-  float* cs = reinterpret_cast<float*>(si + TOKENS * p.k);
+__global__ void __launch_bounds__(ROUTE_WARPS * 32, route_fwd_blocks(EPL)) route_fwd_kernel(RouteParams p, int steps,
+                                                                                       int slots) {
+  constexpr int TOKENS = 32 / L;  // of a step
+  extern __shared__ __align__(16) uint8_t route_smem[];
+  const int batch = steps * TOKENS;
+  // the warp's: (max, sum) of the whole rows [batch], chosen experts [batch][k]; for groups that do not fall on whole
+  // lanes also the step's selection and group scores
+  float2* mxz = reinterpret_cast<float2*>(route_smem + warp_id() * route_warp_smem(p, TOKENS, steps));
+  int* chosen = reinterpret_cast<int*>(mxz + batch);
+  float* cs = reinterpret_cast<float*>(chosen + batch * p.k);
   float* gsc = cs + TOKENS * p.E;
-  const int lane = lane_id(), li = lane % L, tok = threadIdx.x / L;
-  const long long n = (long long)blockIdx.x * TOKENS + tok;
-  const bool in = n < p.N;
+  const int lane = lane_id(), li = lane % L, tok = lane / L;
   const int e0 = li * EPL;
+  const unsigned lower = ((1u << li) - 1u) << (lane - li);  // the token's lanes below this one
+  const int group_shift = __ffs(p.group_lanes) - 1;
   const bool whole = !p.sigmoid && (p.bias != nullptr || !p.renorm);  // softmax: the sum over all experts matters
-  unsigned key[EPL];
-  float z = 1.f, mx = 0.f;
-  {
-    float l[EPL];
-    if (in) {
-      load_logits<T, EPL>(p, n, e0, l);
+  float bias[EPL];  // 0 without one; adding 0 also turns -0 into +0
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) bias[j] = p.bias != nullptr && e0 + j < p.E ? p.bias[e0 + j] + 0.f : 0.f;
+  float next[EPL];
+  auto fetch = [&](long long n) {
+    if (n < p.N) {
+      load_logits<T, EPL>(p, n, e0, next);
     } else {
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) l[j] = 0.f;
+      for (int j = 0; j < EPL; ++j) next[j] = 0.f;
     }
+  };
+  const long long base = ((long long)blockIdx.x * ROUTE_WARPS + warp_id()) * batch;
+  if (base >= p.N) return;
+  fetch(base + tok);
+  for (int step = 0; step < steps; ++step) {
+    if (base + step * TOKENS >= p.N) break;
+    const int at = step * TOKENS + tok;  // in the batch
+    float l[EPL];
+    unsigned key[EPL];
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) l[j] = next[j];
+    if (step + 1 < steps) fetch(base + at + TOKENS);
     if (whole) {
-      mx = -INFINITY;
+      float mx = -INFINITY, z = 0.f;
 #pragma unroll
       for (int j = 0; j < EPL; ++j) mx = fmaxf(mx, l[j]);
       mx = lanes_max<L>(mx);
       if (mx == -INFINITY) mx = 0.f;  // every expert at -inf: all s are 0, and so are the weights
-      z = 0.f;
 #pragma unroll
       for (int j = 0; j < EPL; ++j) z += e0 + j < p.E ? expf(l[j] - mx) : 0.f;
       z = fmaxf(lanes_sum<L>(z), 1e-20f);
+      if (li == 0) mxz[at] = make_float2(mx, z);
     }
     if (p.sigmoid) {
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) l[j] = sigmoid_of(l[j], expf(-fabsf(l[j])));
+      for (int j = 0; j < EPL; ++j) l[j] = sigmoid_of(l[j]);
     }
-    if (p.bias != nullptr) {
-      if (p.vec) {
 #pragma unroll
-        for (int v = 0; v < EPL; v += 8) {
-          float f[8] = {};
-          if (e0 + v < p.E) load_vec<float, 8>(p.bias + e0 + v, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) l[v + j] += f[j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < EPL; ++j)
-          if (e0 + j < p.E) l[j] += p.bias[e0 + j];
-      }
-    }
+    for (int j = 0; j < EPL; ++j) l[j] += bias[j];
+    // one test finds a lane that may hold NaN (also +inf with -inf) and one a lane past the last expert
+    float all = l[0];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      key[j] = e0 + j < p.E ? order_key(l[j]) : 0u;
-      if (p.groups > 1 && p.group_lanes == 0 && e0 + j < p.E) cs[tok * p.E + e0 + j] = l[j];
+      key[j] = number_key(l[j]);
+      if (j > 0) all += l[j];
+    }
+    if (!(fabsf(all) <= FLT_MAX) || e0 + EPL > p.E) {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) key[j] = e0 + j < p.E ? order_key(l[j]) : 0u;
     }
     if (p.groups > 1 && p.group_lanes > 0) {
       // a group is group_lanes whole lanes (a power of two): its two best scores by shuffles, then its rank
@@ -163,111 +188,126 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_fwd_kernel(RouteParams
         a = fmaxf(a, a2);
       }
       const unsigned mine = order_key(p.sigmoid ? a + b : a);
-      const int g = li / p.group_lanes;
-      int above = 0;
-      for (int o = 0; o < p.groups; ++o) {
-        const unsigned other = __shfl_sync(0xffffffffu, mine, o * p.group_lanes, L);
-        above += (other > mine || (other == mine && o < g)) ? 1 : 0;
+      const int g = li >> group_shift;
+      int above = 0;  // groups that come before this one; its lanes share the comparisons
+      for (int o0 = 0; o0 < p.groups; o0 += p.group_lanes) {
+        const int o = o0 + (li & (p.group_lanes - 1));
+        const unsigned other = __shfl_sync(0xffffffffu, mine, o << group_shift, L);
+        above += o < p.groups && (other > mine || (other == mine && o < g)) ? 1 : 0;
       }
+      for (int o = 1; o < p.group_lanes; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
       if (above >= p.top_groups)
 #pragma unroll
         for (int j = 0; j < EPL; ++j) key[j] = 0u;
-    }
-  }
-  if (p.groups > 1 && p.group_lanes == 0) {
-    __syncwarp();
-    for (int g = li; g < p.groups; g += L) {  // lane g scans group g
-      const float* c = cs + tok * p.E + g * p.group_size;
-      float a = -INFINITY, b = -INFINITY;
-      for (int i = 0; i < p.group_size; ++i) {
-        const float v = c[i];
-        b = fmaxf(b, fminf(a, v));
-        a = fmaxf(a, v);
+    } else if (p.groups > 1) {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < EPL; ++j)
+        if (e0 + j < p.E) cs[tok * p.E + e0 + j] = l[j];
+      __syncwarp();
+      for (int g = li; g < p.groups; g += L) {  // lane g scans group g
+        const float* c = cs + tok * p.E + g * p.group_size;
+        float a = -INFINITY, b = -INFINITY;
+        for (int i = 0; i < p.group_size; ++i) {
+          const float v = c[i];
+          b = fmaxf(b, fminf(a, v));
+          a = fmaxf(a, v);
+        }
+        gsc[tok * kRouteMaxGroups + g] = (p.sigmoid && p.group_size > 1) ? a + b : a;
       }
-      gsc[tok * kRouteMaxGroups + g] = (p.sigmoid && p.group_size > 1) ? a + b : a;
-    }
-    __syncwarp();
-    unsigned kept = 0;
-    for (int g = li; g < p.groups; g += L) {
-      const unsigned mine = order_key(gsc[tok * kRouteMaxGroups + g]);
-      int above = 0;
-      for (int o = 0; o < p.groups; ++o) {
-        const unsigned other = order_key(gsc[tok * kRouteMaxGroups + o]);
-        above += (other > mine || (other == mine && o < g)) ? 1 : 0;
+      __syncwarp();
+      unsigned kept = 0;
+      for (int g = li; g < p.groups; g += L) {
+        const unsigned mine = order_key(gsc[tok * kRouteMaxGroups + g]);
+        int above = 0;
+        for (int o = 0; o < p.groups; ++o) {
+          const unsigned other = order_key(gsc[tok * kRouteMaxGroups + o]);
+          above += (other > mine || (other == mine && o < g)) ? 1 : 0;
+        }
+        if (above < p.top_groups) kept |= 1u << g;
       }
-      if (above < p.top_groups) kept |= 1u << g;
-    }
-    kept = lanes_or<L>(kept);
+      kept = lanes_or<L>(kept);
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const unsigned g = ((unsigned)(e0 + j) * p.group_magic) >> 22;
-      if (!((kept >> (g & 31)) & 1u)) key[j] = 0u;
+      for (int j = 0; j < EPL; ++j) {
+        const unsigned g = ((unsigned)(e0 + j) * p.group_magic) >> 22;
+        if (!((kept >> (g & 31)) & 1u)) key[j] = 0u;
+      }
     }
-  }
-  // The lane's two best go to the front by two passes over neighbours, which swap only when the later key is larger (stable).
-  // A lane that has given both is rare; then every lane of the warp makes one more pass. (Sorting all eight: 78 us.)
-  int id[EPL];
+    // The lane's two best go to the front by two passes over neighbours, which swap only when the later key is larger
+    // (stable). A lane that has given both is rare; then every lane of the warp makes one more pass. (Sorting all
+    // eight: 78 us.)
+    int id[EPL];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) id[j] = e0 + j;
-  auto best_to = [&](int front) {
+    for (int j = 0; j < EPL; ++j) id[j] = e0 + j;
+    auto best_to = [&](int front) {
 #pragma unroll
-    for (int j = EPL - 2; j >= 0; --j) {
-      if (j < front) continue;
-      const unsigned a = key[j], b = key[j + 1];
-      const bool swap = b > a;
-      const int ia = id[j], ib = id[j + 1];
-      key[j] = max(a, b);
-      key[j + 1] = min(a, b);
-      id[j] = swap ? ib : ia;
-      id[j + 1] = swap ? ia : ib;
-    }
-  };
-  best_to(0);
-  best_to(1);
-  int ready = 2;  // heads in order
-  const unsigned lower = ((1u << li) - 1u) << (lane - li);  // the token's lanes below this one
-  for (int r = 0; r < p.k; ++r) {
-    if (__any_sync(0xffffffffu, ready == 0)) {
-      best_to(0);
-      ready = max(ready, 1);
-    }
-    bool win = true;
-    if constexpr (L > 1) {
-      const unsigned gm = lanes_max<L>(key[0]);
-      const unsigned who = __ballot_sync(0xffffffffu, key[0] == gm);
-      win = key[0] == gm && (who & lower) == 0u;
-    }
-    if (win) {  // the second moves up and leaves a hole, which the next pass carries to the back
-      si[tok * p.k + r] = id[0];
-      key[0] = key[1], id[0] = id[1];
-      key[1] = 0u;
-      --ready;
+      for (int j = EPL - 2; j >= 0; --j) {
+        if (j < front) continue;
+        const unsigned a = key[j], b = key[j + 1];
+        const bool swap = b > a;
+        const int ia = id[j], ib = id[j + 1];
+        key[j] = max(a, b);
+        key[j + 1] = min(a, b);
+        id[j] = swap ? ib : ia;
+        id[j + 1] = swap ? ia : ib;
+      }
+    };
+    best_to(0);
+    best_to(1);
+    unsigned won = 0u, spent = 0u;  // lanes that have given one; lanes that have none in front
+    for (int r = 0; r < p.k; ++r) {
+      if (spent != 0u) best_to(0);
+      bool win = true;
+      unsigned winners = 0xffffffffu;
+      if constexpr (L > 1) {
+        const unsigned gm = lanes_max<L>(key[0]);
+        const bool top = key[0] == gm;
+        const unsigned who = __ballot_sync(0xffffffffu, top);
+        if constexpr (L == 32) {
+          winners = who & (0u - who);
+          win = (winners >> lane) & 1u;
+        } else {
+          win = top && (who & lower) == 0u;
+          winners = __ballot_sync(0xffffffffu, win);
+        }
+      }
+      spent = won & winners;
+      won |= winners;
+      if (win) {  // the second moves up and leaves a hole, which the next pass carries to the back
+        chosen[at * p.k + r] = id[0];
+        key[0] = key[1], id[0] = id[1];
+        key[1] = 0u;
+      }
     }
   }
   __syncwarp();
-  // the chosen experts' scores, L at a time; a token's lanes stay together in the sums (the loop count is the block's)
-  const T* row = reinterpret_cast<const T*>(p.logits) + (in ? n : 0) * p.ld;
-  if (!p.sigmoid && !whole) {
-    mx = to_f<T>(row[si[tok * p.k]]);  // the best of all (its group is the best group, and no bias moves the order)
-    if (mx == -INFINITY) mx = 0.f;
-  }
-  auto score = [&](int r) {
-    const float l = to_f<T>(row[si[tok * p.k + r]]);
-    return p.sigmoid ? sigmoid_of(l, expf(-fabsf(l))) : expf(l - mx);
-  };
-  float chosen = 0.f, mine = 0.f;
-  for (int r = li; r < p.k; r += L) {
-    mine = score(r);
-    chosen += mine;
-  }
-  chosen = lanes_sum<L>(chosen);
-  if (!in) return;
-  const bool ok = p.valid == nullptr || p.valid[n];
-  const float den = p.renorm ? chosen + 1e-20f * z : z;
-  for (int r = li; r < p.k; r += L) {
-    const float s = p.k <= L ? mine : score(r);
-    p.w[n * p.k + r] = ok ? s / den * p.scale : 0.f;
-    p.idx[n * p.k + r] = ok ? si[tok * p.k + r] : -1;
+  const int shift = __ffs(slots) - 1;
+  // scores and weights of the batch's choices, `slots` lanes per token (a token's first choice in its first lane)
+  for (int i = lane; i - lane < batch * slots; i += 32) {
+    const int at = i >> shift, r = i & (slots - 1);
+    const long long n = base + at;
+    const bool on = at < batch && n < p.N && r < p.k;
+    const int e = on ? chosen[at * p.k + r] : 0;
+    const float l = on ? to_f<T>(reinterpret_cast<const T*>(p.logits)[n * p.ld + e]) : 0.f;
+    float s, z = 1.f;
+    if (p.sigmoid) {
+      s = sigmoid_of(l);
+    } else {
+      // without the whole row's: the best of all (its group is the best group, and no bias moves the order)
+      float mx = __shfl_sync(0xffffffffu, l, lane & ~(slots - 1));
+      if (whole && on) {
+        const float2 t = mxz[at];
+        mx = t.x, z = t.y;
+      }
+      s = expf(l - (mx == -INFINITY ? 0.f : mx));
+    }
+    float sum = on ? s : 0.f;
+    for (int o = slots / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (on) {
+      const bool ok = p.valid == nullptr || p.valid[n];
+      p.w[n * p.k + r] = ok ? s / (p.renorm ? sum + 1e-20f * z : z) * p.scale : 0.f;
+      p.idx[n * p.k + r] = ok ? e : -1;
+    }
   }
 }
 
@@ -419,9 +459,15 @@ cudaError_t route_run(RouteParams p, const float* dw, void* dlogits, cudaStream_
     route_bwd_kernel<T, L, EPL><<<std::min<unsigned>(grid, num_sms() * ROUTE_BWD_BLOCKS), ROUTE_WARPS * 32, 0, s>>>(
         p, dw, static_cast<T*>(dlogits));
   } else {
-    const bool scan = p.groups > 1 && p.group_lanes == 0;
-    const size_t smem = (size_t)TOKENS * 4 * (p.k + (scan ? p.E + kRouteMaxGroups : 0));
-    route_fwd_kernel<T, L, EPL><<<grid, ROUTE_WARPS * 32, smem, s>>>(p);
+    // as many steps per batch as fill the lanes of its end, while every warp that the SMs hold still gets a batch
+    int slots = 1;
+    while (slots < p.k) slots *= 2;
+    const long long warps = (long long)num_sms() * route_fwd_blocks(EPL) * ROUTE_WARPS, per = 32 / L;
+    const int steps = (int)std::max(1ll, std::min<long long>(L / slots, p.N / (warps * per)));
+    const long long batches = (p.N + steps * per - 1) / (steps * per);
+    const unsigned blocks = (unsigned)((batches + ROUTE_WARPS - 1) / ROUTE_WARPS);
+    const size_t smem = (size_t)ROUTE_WARPS * route_warp_smem(p, (int)per, steps);
+    route_fwd_kernel<T, L, EPL><<<blocks, ROUTE_WARPS * 32, smem, s>>>(p, steps, slots);
   }
   return cudaGetLastError();
 }
