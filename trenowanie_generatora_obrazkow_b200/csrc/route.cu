@@ -13,10 +13,11 @@
 // L lanes hold one token, EPL consecutive experts each, so a row is read once with wide loads and every later step works on
 // registers. c is mapped to an unsigned key of the same order (NaN lowest, -0 as +0). Each lane keeps its best
 // keys at the front (equal keys in index order), then each of the k steps takes the largest head of the L lanes; the
-// lowest lane that holds it wins (its experts have the lowest indices) and drops its head. What the weights need beyond the choice
-// is computed for the k chosen alone, from logits read again (they are in the cache).
-// 65536 x 256 fp32, k 8, 4 of 8 groups: forward 63 us (bound by instruction issue, about 740 per token: the exact sigmoids
-// and the group ranks 10 us each, the lists 20 us; 43 us for softmax without groups), backward 29 us; 32768 x 8, 2 chosen: at the launch's own time.
+// lowest lane that holds it wins (its experts have the lowest indices) and drops its head. What the weights need beyond
+// the choice is computed for the k chosen alone, from logits read again (they are in the cache).
+// 65536 x 256 fp32, k 8, 4 of 8 groups: forward 63 us, bound by instruction issue (80 %, about 780 per token: the exact
+// sigmoids and the group ranks 10 us each, the lists 20 us; without either 43 us), backward 29 us; 32768 x 8, 2 chosen: at
+// the launch's own time.
 #include <algorithm>
 #include <cfloat>
 
