@@ -152,6 +152,27 @@ def test_route_gradient_by_differences():
                 assert (num - x.grad[:, e].double()).abs().max() < 2e-6  # h^2 third derivative + fp32 gradient
 
 
+@pytest.mark.parametrize("N,E,k,score,bias,groups,top,renorm,dtype", [
+    (30011, 256, 3, "sigmoid", True, 8, 4, True, F32), (40003, 256, 1, "softmax", True, 1, 1, False, BF16),
+    (30001, 240, 6, "sigmoid", True, 10, 3, True, F32), (30007, 500, 2, "softmax", False, 1, 1, True, F16),
+    (60005, 100, 2, "softmax", True, 5, 2, True, F32), (90001, 61, 1, "sigmoid", False, 1, 1, False, BF16),
+    (300007, 8, 1, "softmax", False, 2, 1, True, F32)])
+def test_route_many_tokens_as_few(N, E, k, score, bias, groups, top, renorm, dtype):
+    """A warp takes several tokens one after the other when there are many: each token's result is that of a short call."""
+    g = gen(33)
+    logits = rnd(g, N, E, std=2.0, dtype=dtype)
+    logits[::97, ::3] = -math.inf
+    logits[5::1013] = math.nan
+    valid = torch.rand(N, device="cuda", generator=g) > 0.1
+    kw = dict(score=score, bias=rnd(g, E, std=0.1) if bias else None, groups=groups, top_groups=top, renorm=renorm)
+    w, idx = Rt.route_experts(logits, k, valid=valid, **kw)
+    for a in range(0, N, 2048):
+        rows = slice(a, min(N, a + 2048))
+        w1, idx1 = Rt.route_experts(logits[rows], k, valid=valid[rows], **kw)
+        assert torch.equal(idx[rows], idx1), a
+        assert torch.equal(w[rows].nan_to_num(nan=-7.0), w1.nan_to_num(nan=-7.0)), a
+
+
 @pytest.mark.parametrize("score,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True)])
 def test_route_padding_rows_stop_gradients(score, renorm):
     """NaN that reaches a padding row's weights does not reach its logits; an error reaches second derivatives."""
