@@ -173,7 +173,10 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_fwd_blocks(EPL)) route
     }
     if (!(fabsf(all) <= FLT_MAX) || e0 + EPL > p.E) {
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) key[j] = e0 + j < p.E ? order_key(l[j]) : 0u;
+      for (int j = 0; j < EPL; ++j) {
+        key[j] = e0 + j < p.E ? order_key(l[j]) : 0u;
+        l[j] = fmaxf(l[j], -INFINITY);  // NaN adds nothing to its group's worth (fminf and fmaxf would pass it over)
+      }
     }
     if (p.groups > 1 && p.group_lanes > 0) {
       // a group is group_lanes whole lanes (a power of two): its two best scores by shuffles, then its rank
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_fwd_blocks(EPL)) route
         b = fmaxf(fminf(a, a2), fmaxf(b, b2));
         a = fmaxf(a, a2);
       }
-      const unsigned mine = order_key(p.sigmoid ? a + b : a);
+      const unsigned mine = number_key(fmaxf(p.sigmoid ? a + b : a, -INFINITY));  // +inf with -inf counts as -inf
       const int g = li >> group_shift;
       int above = 0;  // groups that come before this one; its lanes share the comparisons
       for (int o0 = 0; o0 < p.groups; o0 += p.group_lanes) {
@@ -214,15 +217,15 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_fwd_blocks(EPL)) route
           b = fmaxf(b, fminf(a, v));
           a = fmaxf(a, v);
         }
-        gsc[tok * kRouteMaxGroups + g] = (p.sigmoid && p.group_size > 1) ? a + b : a;
+        gsc[tok * kRouteMaxGroups + g] = fmaxf((p.sigmoid && p.group_size > 1) ? a + b : a, -INFINITY);
       }
       __syncwarp();
       unsigned kept = 0;
       for (int g = li; g < p.groups; g += L) {
-        const unsigned mine = order_key(gsc[tok * kRouteMaxGroups + g]);
+        const unsigned mine = number_key(gsc[tok * kRouteMaxGroups + g]);
         int above = 0;
         for (int o = 0; o < p.groups; ++o) {
-          const unsigned other = order_key(gsc[tok * kRouteMaxGroups + o]);
+          const unsigned other = number_key(gsc[tok * kRouteMaxGroups + o]);
           above += (other > mine || (other == mine && o < g)) ? 1 : 0;
         }
         if (above < p.top_groups) kept |= 1u << g;
