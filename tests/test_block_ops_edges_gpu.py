@@ -54,3 +54,32 @@ def test_nan_adds_nothing_to_its_group(score, E, groups, k):
     _, idx = Rt.route_experts(logits, k, score=score, bias=bias, groups=groups, top_groups=top)
     _, want = R.route_experts(logits, k, score, bias, groups, top)
     assert torch.equal(idx, want)
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# gradients of the norm weights
+# ----------------------------------------------------------------------------------------------------------------
+def test_a_refused_backward_leaves_no_grad_behind():
+    """A backward that ends in an exception (here: the allocator's limit) gives a weight no .grad of unwritten memory."""
+    x, y = (torch.zeros(4, 2048, 4096, device="cuda", dtype=BF16, requires_grad=True) for _ in range(2))
+    q, k = (torch.zeros(4, 2048, 32, 128, device="cuda", dtype=BF16, requires_grad=True) for _ in range(2))
+    pos = torch.zeros(4, 2048, 1, device="cuda", dtype=torch.int32)
+    post_w, w = (torch.ones(4096, device="cuda", requires_grad=True) for _ in range(2))
+    q_w, k_w = (torch.ones(128, device="cuda", requires_grad=True) for _ in range(2))
+    outs = (Fz.sandwich_norm(x, y, post_w=post_w, w=w), Fz.rope_axes(q, k, pos, (128,), q_w=q_w, k_w=k_w))
+    ups = torch.ones_like(outs[0][0]), torch.ones_like(outs[1][0])
+    total = torch.cuda.mem_get_info()[1]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    try:
+        torch.cuda.set_per_process_memory_fraction(torch.cuda.memory_reserved() / total)  # 64 MB gradients do not fit
+        for o, up in zip(outs, ups):
+            with pytest.raises(torch.OutOfMemoryError):
+                torch.autograd.backward(o, [up, up], retain_graph=True)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert all(t.grad is None for t in (post_w, w, q_w, k_w))
+    for o, up in zip(outs, ups):
+        torch.autograd.backward(o, [up, up])
+    # rows of zeros: the norm of the sum is 0, and with it every gradient of a weight
+    assert all((t.grad == 0).all() for t in (post_w, w, q_w, k_w))

@@ -480,8 +480,9 @@ void set_grad_ready(bool on, py::object notify) {
 }
 
 // Where the backward puts the gradient of a small fp32 weight: in place into the leaf's .grad (no temporary, no
-// accumulation kernel), or a temporary that autograd takes. The parameter itself is kept beside the saved tensors: under
-// saved-tensor hooks a saved leaf comes back as another tensor, whose .grad nobody reads.
+// accumulation kernel), or a temporary that autograd takes. A leaf without a .grad gets the buffer that the kernel writes,
+// once it is launched (a refusal before that leaves no .grad behind). The parameter itself is kept beside the saved tensors:
+// under saved-tensor hooks a saved leaf comes back as another tensor, whose .grad nobody reads.
 struct WeightGrad {
   at::Tensor w, g;
   bool direct = false, add = false;
@@ -494,19 +495,19 @@ struct WeightGrad {
     w = it->second.toTensor();
     if (!w.requires_grad()) return;
     if (w.is_leaf() && w.scalar_type() == at::kFloat) {
-      at::Tensor& have = w.mutable_grad();
+      const at::Tensor& have = w.grad();
       if (!have.defined()) {
-        have = fresh_like(w);
         direct = true;
       } else if (have.scalar_type() == at::kFloat && have.is_contiguous() && have.device() == w.device()) {
         direct = add = true;
+        g = have.detach();
       }
-      if (direct) g = have.detach();
     }
-    if (!direct) g = fresh_like(w);
+    if (!add) g = fresh_like(w);
   }
-  at::Tensor done() const {  // what autograd still has to add
+  at::Tensor done() const {  // after the launch: what autograd still has to add
     if (!direct) return g;
+    if (!add) w.mutable_grad() = g;
     if (grad_ready().on) {
       py::gil_scoped_acquire gil;
       grad_ready().notify(w);
