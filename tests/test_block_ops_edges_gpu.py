@@ -83,3 +83,68 @@ def test_a_refused_backward_leaves_no_grad_behind():
         torch.autograd.backward(o, [up, up])
     # rows of zeros: the norm of the sum is 0, and with it every gradient of a weight
     assert all((t.grad == 0).all() for t in (post_w, w, q_w, k_w))
+
+
+@pytest.mark.parametrize("op", ["sandwich", "sandwich of 700 samples", "rope", "rope, any head dim", "attention"])
+@pytest.mark.parametrize("given", ["none", "leaf", "twice"])
+def test_one_leaf_in_both_weight_places(op, given):
+    """A weight that serves as post_w and w, or as q_w and k_w: its gradient is the sum of both, also when .grad holds
+    something already, and the ready hooks hear of it once. Tolerance: the sums of n fp32 products differ from the 64-bit
+    ones by less than 1e-5 of their root sum of squares; bf16 attention in front of the weights' sums allows 2 %."""
+    g = gen(41)
+    tol = 2e-2 if op == "attention" else 1e-5
+    d = {"sandwich": 256, "sandwich of 700 samples": 264, "rope": 64, "rope, any head dim": 50, "attention": 64}[op]
+    weight = rnd(g, d, std=0.1, mean=1.0)
+    if op.startswith("sandwich"):
+        B, T = (3, 40) if op == "sandwich" else (700, 3)
+        x, y, up = rnd(g, B, T, d), rnd(g, B, T, d), [rnd(g, B, T, d), rnd(g, B, T, d)]
+        gate, shift, scale = (rnd(g, B, d, std=0.3) for _ in range(3))
+        run = lambda w, p, c=lambda t: t: (p.sandwich_norm(c(x), c(y), c(gate), w, w, c(shift), c(scale)), [c(u) for u in up])
+    elif op == "attention":
+        qkv, up = rnd(g, 2, 70, 6 * d, dtype=BF16), [rnd(g, 2, 70, 4 * d, dtype=BF16)]
+        pos = torch.randint(0, 50, (2, 70, 1), device="cuda", generator=g).int()
+
+        def run(w, p, c=lambda t: t):
+            if p is Fz:
+                return [Fz.axes_attention_core(qkv.clone().requires_grad_(), pos, (d,), 4, 1, d, q_w=w, k_w=w)], up
+            q, k, v = c(qkv).view(2, 70, 6, d).split([4, 1, 1], dim=2)
+            q, k = R.rope_axes(q, k, pos, (d,), q_w=w, k_w=w)
+            return [R.attention(q, k, v, None, d ** -0.5).reshape(2, 70, 4 * d)], [c(u) for u in up]
+    else:
+        q, k, up = rnd(g, 2, 33, 3, d), rnd(g, 2, 33, 1, d), [rnd(g, 2, 33, 3, d), rnd(g, 2, 33, 1, d)]
+        pos = torch.randint(0, 50, (2, 33, 1), device="cuda", generator=g).int()
+        run = lambda w, p, c=lambda t: t: (p.rope_axes(c(q), c(k), pos, (d // 2 // 2 * 2,), q_w=w, k_w=w), [c(u) for u in up])
+    w64 = weight.double().requires_grad_()
+    outs, ups = run(w64, R, lambda t: t.double())
+    torch.autograd.backward(list(outs), ups)
+    want = w64.grad
+    start = torch.zeros(d, device="cuda")
+    w = weight.clone().requires_grad_()
+    if given != "none":
+        w.grad = rnd(g, d)
+        start = w.grad.clone()
+    heard = []
+    hook = Fz.add_grad_ready_hook(lambda p: heard.append(p))
+    try:
+        for _ in range(2 if given == "twice" else 1):
+            outs, ups = run(w, Fz)
+            torch.autograd.backward(list(outs), ups)
+    finally:
+        Fz.remove_grad_ready_hook(hook)
+    want = want * (2 if given == "twice" else 1)
+    size = want.norm()
+    assert (w.grad.double() - start.double() - want).norm() <= tol * size, ((w.grad.double() - start - want).norm() / size)
+    assert len(heard) == (2 if given == "twice" else 1) and all(p is w for p in heard)
+
+
+def test_two_leaves_with_one_grad():
+    """Two weights whose .grad is the same memory: both sums arrive there."""
+    g = gen(42)
+    x, y, up = rnd(g, 2, 30, 128), rnd(g, 2, 30, 128), rnd(g, 2, 30, 128)
+    a, b = (rnd(g, 128, std=0.1, mean=1.0).requires_grad_() for _ in range(2))
+    Fz.sandwich_norm(x, y, post_w=a, w=b)[1].backward(up)
+    want = a.grad + b.grad
+    both = torch.zeros(128, device="cuda")
+    a.grad, b.grad = both, both.view(128)
+    Fz.sandwich_norm(x, y, post_w=a, w=b)[1].backward(up)
+    assert torch.allclose(both, want, rtol=1e-5, atol=1e-5 * want.abs().max().item())

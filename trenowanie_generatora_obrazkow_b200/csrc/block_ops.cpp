@@ -479,16 +479,15 @@ void set_grad_ready(bool on, py::object notify) {
   grad_ready().on = on;
 }
 
-// Where the backward puts the gradient of a small fp32 weight: in place into the leaf's .grad (no temporary, no
-// accumulation kernel), or a temporary that autograd takes. A leaf without a .grad gets the buffer that the kernel writes,
-// once it is launched (a refusal before that leaves no .grad behind). The parameter itself is kept beside the saved tensors:
-// under saved-tensor hooks a saved leaf comes back as another tensor, whose .grad nobody reads.
+// Where a backward with two norm weights puts their gradients: in place into a leaf's .grad (no temporary, no accumulation
+// kernel), or a temporary that autograd takes. A leaf without a .grad gets the buffer that the kernel writes, once it is
+// launched (a refusal before that leaves no .grad behind). The parameter itself is kept beside the saved tensors: under
+// saved-tensor hooks a saved leaf comes back as another tensor, whose .grad nobody reads.
+// The kernels write the two gradients without regard to each other, so they never share memory: one leaf in both places
+// (tied weights), or two with one .grad, has its second gradient written to a temporary and added after the launch.
 struct WeightGrad {
   at::Tensor w, g;
   bool direct = false, add = false;
-  static void keep(AutogradContext* ctx, const char* name, const OptT& weight) {
-    if (given(weight)) ctx->saved_data[name] = *weight;
-  }
   WeightGrad(AutogradContext* ctx, const char* name) {
     const auto it = ctx->saved_data.find(name);
     if (it == ctx->saved_data.end()) return;
@@ -505,14 +504,36 @@ struct WeightGrad {
     }
     if (!add) g = fresh_like(w);
   }
-  at::Tensor done() const {  // after the launch: what autograd still has to add
+  // after the launch: what autograd still has to add
+  at::Tensor put() const {
     if (!direct) return g;
-    if (!add) w.mutable_grad() = g;
-    if (grad_ready().on) {
-      py::gil_scoped_acquire gil;
-      grad_ready().notify(w);
-    }
+    at::Tensor& have = w.mutable_grad();
+    if (!have.defined()) have = g;
+    else if (!add) have.add_(g);
     return at::Tensor();
+  }
+};
+struct WeightGrads {
+  WeightGrad a, b;
+  static void keep(AutogradContext* ctx, const char* name, const OptT& weight) {
+    if (given(weight)) ctx->saved_data[name] = *weight;
+  }
+  WeightGrads(AutogradContext* ctx, const char* first, const char* second) : a(ctx, first), b(ctx, second) {
+    if (a.add && b.add) {
+      const float *p = a.g.data_ptr<float>(), *q = b.g.data_ptr<float>();
+      if (p < q + b.g.numel() && q < p + a.g.numel()) {
+        b.g = fresh_like(b.w);
+        b.add = false;
+      }
+    }
+  }
+  void done(at::Tensor& first, at::Tensor& second) const {
+    first = a.put();
+    second = b.put();
+    if (!grad_ready().on) return;
+    py::gil_scoped_acquire gil;  // each parameter once, when all of its gradient is there
+    if (a.direct) grad_ready().notify(a.w);
+    if (b.direct && !(a.direct && b.w.is_same(a.w))) grad_ready().notify(b.w);
   }
 };
 
@@ -604,8 +625,8 @@ struct SandwichFn : public torch::autograd::Function<SandwichFn> {
     auto r = sandwich_fwd(x, y, gate, post_w, w, shift, scale, res_scale, eps, err);
     ctx->save_for_backward({x, y, or_undefined(gate), or_undefined(post_w), or_undefined(w), or_undefined(shift),
                             or_undefined(scale), r[2], r[3]});
-    WeightGrad::keep(ctx, "post_w", post_w);
-    WeightGrad::keep(ctx, "w", w);
+    WeightGrads::keep(ctx, "post_w", post_w);
+    WeightGrads::keep(ctx, "w", w);
     ctx->saved_data["err"] = err;
     ctx->saved_data["res_scale"] = res_scale;
     ctx->saved_data["eps"] = eps;
@@ -618,16 +639,15 @@ struct SandwichFn : public torch::autograd::Function<SandwichFn> {
     const auto s = ctx->get_saved_variables();
     const at::Tensor dx_new = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
     const at::Tensor dh = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
-    const WeightGrad gp(ctx, "post_w"), gw(ctx, "w");
+    const WeightGrads gw(ctx, "post_w", "w");
     auto r = sandwich_bwd(opt(dx_new), opt(dh), s[0], s[1], opt(s[2]), opt(s[3]), opt(s[4]), opt(s[5]), opt(s[6]),
-                          opt(s[7]), opt(s[8]), opt(gp.g), opt(gw.g), ctx->saved_data["res_scale"].toDouble(),
-                          ctx->saved_data["eps"].toDouble(), ctx->saved_data["err"].toTensor(), gp.add, gw.add);
+                          opt(s[7]), opt(s[8]), opt(gw.a.g), opt(gw.b.g), ctx->saved_data["res_scale"].toDouble(),
+                          ctx->saved_data["eps"].toDouble(), ctx->saved_data["err"].toTensor(), gw.a.add, gw.b.add);
     variable_list out(10);
     out[0] = r[0];
     out[1] = r[1];
     out[2] = r[2];
-    out[3] = gp.done();
-    out[4] = gw.done();
+    gw.done(out[3], out[4]);
     out[5] = r[3];
     out[6] = r[4];
     return out;
@@ -657,8 +677,8 @@ struct RopeAxesFn : public torch::autograd::Function<RopeAxesFn> {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [qo, ko] = rope_axes_fwd(q, k, pos, freq, axis, q_w, k_w, interleaved, eps);
     ctx->save_for_backward({q, k, pos, freq, axis, or_undefined(q_w), or_undefined(k_w)});
-    WeightGrad::keep(ctx, "q_w", q_w);
-    WeightGrad::keep(ctx, "k_w", k_w);
+    WeightGrads::keep(ctx, "q_w", q_w);
+    WeightGrads::keep(ctx, "k_w", k_w);
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["eps"] = eps;
     return {qo, ko};
@@ -666,18 +686,17 @@ struct RopeAxesFn : public torch::autograd::Function<RopeAxesFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order_only();
     const auto s = ctx->get_saved_variables();
-    const WeightGrad gq(ctx, "q_w"), gk(ctx, "k_w");
+    const WeightGrads gw(ctx, "q_w", "k_w");
     // the two weights' sums come together: one that needs no gradient gets a scratch row
-    at::Tensor wq = gq.g, wk = gk.g;
+    at::Tensor wq = gw.a.g, wk = gw.b.g;
     if (wq.defined() != wk.defined()) (wq.defined() ? wk : wq) = fresh_like(wq.defined() ? wq : wk);
-    auto [dq, dk] = rope_axes_bwd(grads[0].contiguous(), grads[1].contiguous(), s[0], s[1], s[2], s[3], s[4],
-                                  opt(s[5]), opt(s[6]), opt(wq), opt(wk), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(),
-                                  gq.add, gk.add, OptT(), OptT());
+    auto [dq, dk] = rope_axes_bwd(grads[0].contiguous(), grads[1].contiguous(), s[0], s[1], s[2], s[3], s[4], opt(s[5]),
+                                  opt(s[6]), opt(wq), opt(wk), ctx->saved_data["interleaved"].toBool(),
+                                  ctx->saved_data["eps"].toDouble(), gw.a.add, gw.b.add, OptT(), OptT());
     variable_list out(9);
     out[0] = dq;
     out[1] = dk;
-    out[5] = gq.done();
-    out[6] = gk.done();
+    gw.done(out[5], out[6]);
     return out;
   }
 };

@@ -554,15 +554,22 @@ class _AxesAttnFn(torch.autograd.Function):
         ext().attention_bwd(q.view(B, T, hq, hd), k.view(B, T, hkv, hd), v4, o, lse,
                             do.contiguous().view(B, T, hq, hd), kv_len, scale, dq.view(B, T, hq, hd),
                             dk.view(B, T, hkv, hd), dv4, err_buf(q.device))
-        dwq = dwk = None
+        dwq = dwk = tied = None
         if q_w is not None and (ctx.q_param.requires_grad or ctx.k_param.requires_grad):
             dwq, q_direct = _weight_grad_target(ctx.q_param)
             dwk, k_direct = _weight_grad_target(ctx.k_param)
+            if dwq.data_ptr() == dwk.data_ptr():  # one weight for q and k: the kernel wants the two sums apart
+                tied, dwk = dwk, torch.zeros_like(dwk)
         ext().rope_axes_bwd(dq, dk, rows[:, :hq], rows[:, hq:hq + hkv], pos, freq, axis, q_w, k_w, dwq, dwk,
                             interleaved, eps, dq_out=drows[:, :hq], dk_out=drows[:, hq:hq + hkv])
+        if tied is not None:
+            tied += dwk
         if dwq is not None:
             dwq = _weight_grad_done(ctx.q_param, q_direct, dwq)
-            dwk = _weight_grad_done(ctx.k_param, k_direct, dwk)
+            if ctx.k_param is not ctx.q_param or not k_direct:  # a tied weight's gradient is ready once
+                dwk = _weight_grad_done(ctx.k_param, k_direct, dwk)
+            else:
+                dwk = None
         return dqkv, None, None, None, dwq, dwk, None, None, None, None, None, None, None
 
 
