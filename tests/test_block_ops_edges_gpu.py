@@ -57,6 +57,31 @@ def test_nan_adds_nothing_to_its_group(score, E, groups, k):
 
 
 # ----------------------------------------------------------------------------------------------------------------
+# rotary positions
+# ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("d,axes,norm,interleaved,dtype", [(776, (768,), True, True, F32), (1024, (512, 256), True, False, BF16),
+                                                           (1024, (1024,), False, True, F32), (1023, (10,), True, True, F32)])
+def test_rope_axes_of_the_widest_heads(d, axes, norm, interleaved, dtype):
+    """Head dims up to 1024, forward and backward. Each output is rounded once (half a unit of its type, doubled) and
+    carries at most 64 fp32 roundings of its largest terms: a pair's two products and the norm's mean over d channels."""
+    g = gen(43)
+    unit = {BF16: 2.0 ** -8, F32: 2.0 ** -23}[dtype]
+    q, k, dq, dk = (rnd(g, 2, 9, h, d, dtype=dtype) for h in (3, 1, 3, 1))
+    pos = torch.randint(0, 64, (2, 9, len(axes)), device="cuda", generator=g).int()
+    ws = [rnd(g, d, std=0.1, mean=1.0) for _ in range(2)] if norm else [None, None]
+    leaf = [t.clone().requires_grad_() if t is not None else None for t in (q, k, *ws)]
+    wide = [t.double().requires_grad_() if t is not None else None for t in (q, k, *ws)]
+    out = Fz.rope_axes(*leaf[:2], pos, axes, q_w=leaf[2], k_w=leaf[3], interleaved=interleaved)
+    want = R.rope_axes(*wide[:2], pos, axes, q_w=wide[2], k_w=wide[3], interleaved=interleaved)
+    torch.autograd.backward(list(out), [dq, dk])
+    torch.autograd.backward(list(want), [dq.double(), dk.double()])
+    for a, b in list(zip(out, want)) + [(a.grad, b.grad) for a, b in zip(leaf[:2], wide[:2])]:
+        assert (a.double() - b).abs().max() <= (unit + 64 * 2.0 ** -24) * 2 * b.abs().max()
+    for a, b in zip(leaf[2:], wide[2:]):  # sums over 18 or 54 rows
+        assert a is None or (a.grad.double() - b.grad).norm() <= 64 * 2.0 ** -24 * 54 ** 0.5 * b.grad.norm()
+
+
+# ----------------------------------------------------------------------------------------------------------------
 # gradients of the norm weights
 # ----------------------------------------------------------------------------------------------------------------
 def test_a_refused_backward_leaves_no_grad_behind():

@@ -389,8 +389,9 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) rope_axes_bwd_any_kernel(Rope
                                                                             float* __restrict__ partial) {
   extern __shared__ float rope_smem[];
   const int heads = p.hq + p.hkv, half = p.rot / 2;
-  float* acc = rope_smem + warp_id() * 2 * p.hd;
-  for (int c = lane_id(); c < 2 * p.hd; c += 32) acc[c] = 0.f;
+  float* acc = rope_smem + warp_id() * 2 * p.hd;  // only with norm weights
+  if (p.q_w != nullptr)
+    for (int c = lane_id(); c < 2 * p.hd; c += 32) acc[c] = 0.f;
   __syncwarp();
   const long long units = (long long)p.M * heads;
   for (long long u = (long long)blockIdx.x * ROPE_WARPS + warp_id(); u < units; u += (long long)gridDim.x * ROPE_WARPS) {
@@ -541,10 +542,15 @@ cudaError_t rope_bwd_run(const RopeAxesParams& p, const void* dq, const void* dk
   T *iq = static_cast<T*>(dq_in), *ik = static_cast<T*>(dk_in);
   const bool vec = rope_vectors(p, elem, {dq, dk, dq_in, dk_in});
   const int grid = rope_grid(p, vec, vec ? ROPE_BWD_BLOCKS : ROPE_ANY_BLOCKS);
-  if (!vec)
-    rope_axes_bwd_any_kernel<T><<<grid, ROPE_WARPS * 32, sizeof(float) * ROPE_WARPS * 2 * p.hd, s>>>(p, gq, gk, iq, ik,
-                                                                                                   partial);
-  else if (p.hd <= 32) rope_bwd_vec<T, 4>(p, gq, gk, iq, ik, partial, grid, s);
+  if (!vec) {
+    // the weights' sums of every warp: none without weights, more than the default 48 KB above 768 channels
+    const int smem = p.q_w != nullptr ? (int)sizeof(float) * ROPE_WARPS * 2 * p.hd : 0;
+    if (smem > 48 * 1024) {
+      cudaError_t e = cudaFuncSetAttribute(rope_axes_bwd_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return e;
+    }
+    rope_axes_bwd_any_kernel<T><<<grid, ROPE_WARPS * 32, smem, s>>>(p, gq, gk, iq, ik, partial);
+  } else if (p.hd <= 32) rope_bwd_vec<T, 4>(p, gq, gk, iq, ik, partial, grid, s);
   else if (p.hd <= 64) rope_bwd_vec<T, 8>(p, gq, gk, iq, ik, partial, grid, s);
   else if (p.hd <= 128) rope_bwd_vec<T, 16>(p, gq, gk, iq, ik, partial, grid, s);
   else rope_bwd_vec<T, 32>(p, gq, gk, iq, ik, partial, grid, s);
