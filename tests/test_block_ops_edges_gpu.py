@@ -82,6 +82,22 @@ def test_rope_axes_of_the_widest_heads(d, axes, norm, interleaved, dtype):
 
 
 # ----------------------------------------------------------------------------------------------------------------
+# sandwich norm
+# ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(1, 2 ** 31 - 1000, 1), (2 ** 20, 2 ** 11 - 1, 8), (2 ** 16, 2 ** 16, 8), (1, 4, 16385)])
+def test_sandwich_norm_refuses_more_rows_than_it_counts(shape):
+    """Rows are counted in 32 bits: sizes at that limit are refused before a copy or a launch (the inputs are expanded,
+    so they take no memory)."""
+    x = torch.zeros(1, 1, 1, device="cuda", dtype=BF16).expand(shape)
+    w = torch.ones(1, device="cuda").expand(shape[2])
+    Fz.err_buf("cuda")  # the device's error word is made once
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(RuntimeError, match="rows"):
+        Fz.sandwich_norm(x, x, w=w)
+    assert torch.cuda.memory_allocated() == before
+
+
+# ----------------------------------------------------------------------------------------------------------------
 # gradients of the norm weights
 # ----------------------------------------------------------------------------------------------------------------
 def test_a_refused_backward_leaves_no_grad_behind():

@@ -227,14 +227,20 @@ const void* sample_rows(const OptT& t, int64_t B, int64_t D, const at::Tensor& x
   return t->data_ptr();
 }
 
+// The row loops count in 32 bits and step past the last row by at most a grid or a span.
+void sandwich_limits(const at::Tensor& x) {
+  TORCH_CHECK(x.dim() == 3 && x.size(2) >= 1 && x.size(2) <= 16384 && x.size(0) * x.size(1) < (1ll << 31) - (1 << 20),
+              "sandwich_norm: x [B, T, D] of at most 16384 channels and 2^31 - 2^20 rows");
+}
+
 SandwichParams sandwich_params(const at::Tensor& x, const at::Tensor& y, const OptT& gate, const OptT& post_w,
                                const OptT& w, const OptT& shift, const OptT& scale, double res_scale, double eps) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 3 && x.is_contiguous(), "sandwich_norm: x [B, T, D], contiguous");
   TORCH_CHECK(y.is_contiguous() && y.sizes() == x.sizes() && y.scalar_type() == x.scalar_type(),
               "sandwich_norm: y as x");
   same_device(y, x, "sandwich_norm: y");
+  sandwich_limits(x);
   const int64_t B = x.size(0), T = x.size(1), D = x.size(2);
-  TORCH_CHECK(D >= 1 && D <= 16384 && B * T < (1ll << 31), "sandwich_norm: at most 16384 channels");
   TORCH_CHECK(given(shift) == given(scale), "sandwich_norm: shift and scale together");
   TORCH_CHECK(given(w) || !given(scale), "sandwich_norm: shift and scale need w (the norm they modulate)");
   SandwichParams p{};
@@ -655,6 +661,7 @@ struct SandwichFn : public torch::autograd::Function<SandwichFn> {
 };
 std::tuple<at::Tensor, OptT> sandwich_norm(at::Tensor x, at::Tensor y, OptT gate, OptT post_w, OptT w, OptT shift,
                                            OptT scale, double res_scale, double eps, at::Tensor err) {
+  sandwich_limits(x);  // before anything is copied
   x = x.contiguous();
   y = y.contiguous();
   if (given(shift) && given(scale) && shift->strides() != scale->strides()) {

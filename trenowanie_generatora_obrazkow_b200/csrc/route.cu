@@ -457,7 +457,7 @@ cudaError_t route_run(RouteParams p, const float* dw, void* dlogits, cudaStream_
                                              reinterpret_cast<uintptr_t>(dlogits)) & 15) == 0;
   const int gl = p.group_size / EPL;
   p.group_lanes = p.group_size % EPL == 0 && (gl & (gl - 1)) == 0 ? gl : 0;
-  const unsigned grid = (unsigned)((p.N + TOKENS - 1) / TOKENS);
+  const unsigned grid = (unsigned)(((long long)p.N + TOKENS - 1) / TOKENS);
   if (dlogits != nullptr) {
     // blocks that the SMs hold, walking the tokens
     route_bwd_kernel<T, L, EPL><<<std::min<unsigned>(grid, num_sms() * ROUTE_BWD_BLOCKS), ROUTE_WARPS * 32, 0, s>>>(
