@@ -56,6 +56,31 @@ def test_nan_adds_nothing_to_its_group(score, E, groups, k):
     assert torch.equal(idx, want)
 
 
+@pytest.mark.parametrize("E,k", [(8, 2), (40, 3), (256, 8), (500, 32)])
+def test_gradient_of_nearly_impossible_choices(E, k):
+    """softmax, renormalised, and a bias that moves the choice to experts of a probability near 1e-20: the + 1e-20 of the
+    divisor takes part, and the gradient reaches the experts that hold the probability. Tolerance: 64 fp32 roundings of
+    the terms w |dw - m| and scale m, relative to the largest term of the row."""
+    g = gen(44)
+    N = 60
+    logits = rnd(g, N, E)
+    logits[:, : E // 4] += torch.linspace(0, 90, N, device="cuda")[:, None]  # chosen sums from all of it to 1e-39
+    logits[::7, -1] = -math.inf
+    bias = torch.zeros(E, device="cuda")
+    bias[: E // 4] = -1000.0
+    dw = rnd(g, N, k)
+    x, y = logits.clone().requires_grad_(), logits.double().requires_grad_()
+    w, idx = Rt.route_experts(x, k, bias=bias, scale=2.5)
+    w64, want = R.route_experts(y, k, "softmax", bias.double(), scale=2.5)
+    assert torch.equal(idx, want) and (idx >= E // 4).all()
+    w.backward(dw)
+    w64.backward(dw.double())
+    assert (y.grad[:, : E // 4].abs().amax(1) > 1e-3).any()  # rows where it matters are among them
+    terms = 2.5 * dw.double().abs().amax(1, keepdim=True) * (w64.detach().sum(1, keepdim=True) / 2.5)
+    assert ((w.double() - w64).abs() <= 64 * 2.0 ** -24 * w64 + 1e-30).all()
+    assert ((x.grad.double() - y.grad).abs() <= 64 * 2.0 ** -24 * terms + 1e-30).all()
+
+
 # ----------------------------------------------------------------------------------------------------------------
 # rotary positions
 # ----------------------------------------------------------------------------------------------------------------

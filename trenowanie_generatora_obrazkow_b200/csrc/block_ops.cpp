@@ -110,9 +110,10 @@ std::tuple<at::Tensor, at::Tensor> route_fwd(at::Tensor logits, OptT bias, OptT 
   return {w, idx};
 }
 
-at::Tensor route_bwd(at::Tensor logits, at::Tensor w, at::Tensor idx, at::Tensor dw, bool sigmoid, bool renorm,
-                     double scale) {
+at::Tensor route_bwd(at::Tensor logits, at::Tensor w, at::Tensor idx, at::Tensor dw, bool biased, bool sigmoid,
+                     bool renorm, double scale) {
   RouteParams p = route_params(logits, w.size(1), sigmoid, 1, 1, renorm, scale);
+  p.biased = biased;
   const c10::cuda::CUDAGuard guard(logits.device());
   same_device(idx, logits, "route_bwd: idx");
   TORCH_CHECK(idx.scalar_type() == at::kInt && idx.is_contiguous() && idx.sizes() == w.sizes() && w.size(0) == p.N,
@@ -549,6 +550,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [w, idx] = route_fwd(logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale);
     ctx->save_for_backward({logits, w, idx});
+    ctx->saved_data["biased"] = given(bias);
     ctx->saved_data["sigmoid"] = sigmoid;
     ctx->saved_data["renorm"] = renorm;
     ctx->saved_data["scale"] = scale;
@@ -558,8 +560,9 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order_only();
     const auto saved = ctx->get_saved_variables();
-    at::Tensor d = route_bwd(saved[0], saved[1], saved[2], grads[0].contiguous(), ctx->saved_data["sigmoid"].toBool(),
-                             ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
+    at::Tensor d = route_bwd(saved[0], saved[1], saved[2], grads[0].contiguous(), ctx->saved_data["biased"].toBool(),
+                             ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["renorm"].toBool(),
+                             ctx->saved_data["scale"].toDouble());
     variable_list out(9);
     out[0] = d;
     return out;

@@ -23,6 +23,7 @@ struct RouteParams {
   int groups, top_groups, group_size;
   unsigned group_magic;    // ceil(2^22 / group_size): e / group_size == (e * magic) >> 22 for e < 512
   int sigmoid, renorm;
+  int biased;              // backward: the choice was made with a bias
   float scale;
   int vec, group_lanes;    // set by the launchers (route.cu)
 };

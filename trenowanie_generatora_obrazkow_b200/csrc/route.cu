@@ -6,9 +6,12 @@
 // best groups stay. The k experts of largest c are chosen, ties to the lowest index; their weights are
 //     w_j = scale s_j / (sum of the chosen s + 1e-20)      (renorm)      or      scale s_j.
 // Gradient to the logits, with r_j = w_j / scale and m = sum_j r_j dw_j over the chosen:
-//     softmax, renorm   dl_j = w_j (dw_j - m)                         sigmoid, renorm   dl_j = scale (dw_j - m) s_j' / S
-//     softmax           dl_i = [i chosen] w_i dw_i - scale p_i m      sigmoid           dl_j = scale dw_j s_j'
-// s' = s (1 - s), S = sum of the chosen s. The selection and the bias take no gradient.
+//     softmax, renorm   dl_i = [i chosen] w_i (dw_i - m) - scale p_i m 1e-20 / S
+//     softmax           dl_i = [i chosen] w_i dw_i - scale p_i m
+//     sigmoid, renorm   dl_j = scale (dw_j - m) s_j' / S              sigmoid           dl_j = scale dw_j s_j'
+// s' = s (1 - s), S = sum of the chosen s (+ 1e-20). The selection and the bias take no gradient. 1e-20 / S, which is
+// 1 - sum of r, matters only where a bias moved the choice to experts of next to no probability: without a bias, and
+// where it is below the rounding of the sum, the other experts' logits are not read.
 //
 // L lanes hold one token, EPL consecutive experts each, so a row is read once with wide loads and every later step works on
 // registers. c is mapped to an unsigned key of the same order (NaN lowest, -0 as +0). Each lane keeps its best
@@ -31,6 +34,8 @@ namespace tgo {
 namespace {
 
 constexpr int ROUTE_WARPS = 4, ROUTE_BWD_BLOCKS = 8;
+// Above the rounding of a sum of up to 32 weights divided by their own sum (about 8 units of 2^-24).
+constexpr float ROUTE_LOST = 0x1p-20f;
 // blocks per SM: 64 registers hold 8 experts per lane (9 blocks spill, 7 take 2 us more), 16 experts want 80
 constexpr int route_fwd_blocks(int epl) { return epl > 8 ? 6 : 8; }
 
@@ -307,9 +312,25 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_fwd_blocks(EPL)) route
     }
     float sum = on ? s : 0.f;
     for (int o = slots / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    float div = p.renorm ? sum + 1e-20f * z : z;
+    if (whole && p.renorm && __any_sync(0xffffffffu, on && sum < 1e-13f)) {
+      // A bias can move the choice far below the row's best. From about 30 on, the rounding of l - mx shows in the scores
+      // and they end up subnormal beside 1e-20: such a token's are taken relative to its best choice, 1e-20 z exp(gap)
+      // in two factors with the gap's own rounding given back.
+      float best = on ? l : -INFINITY;
+      for (int o = slots / 2; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+      const float top = on ? mxz[at].x : 0.f;
+      if (best == -INFINITY) best = top;  // nothing but switched-off experts: weights of 0
+      const float e = on ? expf(l - best) : 0.f;
+      float all = e;
+      for (int o = slots / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+      const float gap = top - best, back = top - gap, lost = (top - (gap + back)) + (back - best);
+      const float half_gap = expf(0.5f * gap);
+      if (sum < 1e-13f) s = e, div = all + 1e-20f * z * half_gap * half_gap * (1.f + lost);
+    }
     if (on) {
       const bool ok = p.valid == nullptr || p.valid[n];
-      p.w[n * p.k + r] = ok ? s / (p.renorm ? sum + 1e-20f * z : z) * p.scale : 0.f;
+      p.w[n * p.k + r] = ok ? s / div * p.scale : 0.f;
       p.idx[n * p.k + r] = ok ? e : -1;
     }
   }
@@ -369,22 +390,31 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_bwd_kernel(RouteParams
     const bool in = n < p.N;
 #pragma unroll
     for (int j = 0; j < EPL; j += 4) *reinterpret_cast<float4*>(d + e0 + j) = make_float4(0.f, 0.f, 0.f, 0.f);
-    // m = sum of r dw and S = sum of the chosen s
+    // m = sum of r dw; total = S = sum of the chosen s (sigmoid) or sum of w (softmax)
     float m = 0.f, total = 0.f, se = 0.f, de = 0.f;
     if (one) {
       if (p.sigmoid && cur.e >= 0) scores(lc, se, de);
       m = cur.w * cur.g;
-      total = se;
+      total = p.sigmoid ? se : cur.w;
     } else {
       for (int r = li; r < p.k; r += L) {
         const Choice c = choice(n, r);
         if (p.sigmoid && c.e >= 0) scores(logit(n, c), se, de);
         m = fmaf(c.w, c.g, m);
-        total += c.e >= 0 ? se : 0.f;
+        total += p.sigmoid ? (c.e >= 0 ? se : 0.f) : c.w;
       }
     }
     m = lanes_sum<L>(m) / p.scale;
-    if (p.sigmoid && p.renorm) total = lanes_sum<L>(total) + 1e-20f;
+    float others = 1.f;  // share of m that every expert's probability takes part in
+    if (p.renorm) {
+      others = 0.f;
+      if (p.sigmoid) {
+        total = lanes_sum<L>(total) + 1e-20f;
+      } else if (p.biased) {
+        others = 1.f - lanes_sum<L>(total) / p.scale;  // 1e-20 / S
+        if (others < ROUTE_LOST) others = 0.f;
+      }
+    }
     __syncwarp();
     auto put = [&](const Choice& c, float ds) {
       const float up = p.renorm ? c.g - m : c.g;
@@ -406,7 +436,8 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_bwd_kernel(RouteParams
       const float4 t = *reinterpret_cast<const float4*>(d + e0 + j);
       v[j] = t.x, v[j + 1] = t.y, v[j + 2] = t.z, v[j + 3] = t.w;
     }
-    if (!p.sigmoid && !p.renorm) {  // every expert's probability takes part (m is 0 for a token without experts)
+    // a token without experts has m 0; the lanes of a warp go together
+    if (!p.sigmoid && (!p.renorm || (p.biased && __any_sync(0xffffffffu, others * m != 0.f)))) {
       float l[EPL];
       float mx = -INFINITY;
       if (in) load_logits<T, EPL>(p, n, e0, l);
@@ -424,8 +455,8 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_bwd_kernel(RouteParams
         z += l[j];
       }
       z = fmaxf(lanes_sum<L>(z), 1e-20f);
-      const float f = p.scale * m / z;
-      if (m != 0.f)
+      const float f = p.scale * m * others / z;
+      if (others * m != 0.f)
 #pragma unroll
         for (int j = 0; j < EPL; ++j) v[j] = fmaf(-f, l[j], v[j]);
     }
