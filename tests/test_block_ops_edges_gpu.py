@@ -214,3 +214,30 @@ def test_two_leaves_with_one_grad():
     a.grad, b.grad = both, both.view(128)
     Fz.sandwich_norm(x, y, post_w=a, w=b)[1].backward(up)
     assert torch.allclose(both, want, rtol=1e-5, atol=1e-5 * want.abs().max().item())
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Dual tensors: an error instead of results without their tangents, with and without requires_grad."""
+    from torch.autograd import forward_ad
+    g = gen(45)
+    logits, x, w = rnd(g, 6, 8), rnd(g, 6, 16), torch.rand(6, 2, device="cuda", generator=g)
+    plan = Rt.expert_plan(Rt.route_experts(logits, 2)[1], 8)
+    y, q = rnd(g, plan.rows, 16), rnd(g, 2, 3, 2, 16)
+    pos = torch.zeros(2, 3, 1, device="cuda", dtype=torch.int32)
+    gate, weight = rnd(g, 2, 16), rnd(g, 16)
+    x3 = x.view(2, 3, 16)
+    calls = [(lambda t: Rt.route_experts(t, 2), logits), (lambda t: Rt.expert_dispatch(t, plan), x),
+             (lambda t: Rt.expert_combine(t, w, plan), y), (lambda t: Rt.expert_combine(y, t, plan), w),
+             (lambda t: Fz.sandwich_norm(t, x3, w=weight), x3), (lambda t: Fz.sandwich_norm(x3, x3, t, w=weight), gate),
+             (lambda t: Fz.sandwich_norm(x3, x3, w=t), weight), (lambda t: Fz.rope_axes(t, q, pos, (16,)), q),
+             (lambda t: Fz.rope_axes(q, q, pos, (16,), q_w=t, k_w=weight), weight)]
+    for leaf in (False, True):
+        with forward_ad.dual_level():
+            for f, t in calls:
+                dual = forward_ad.make_dual(t.clone().requires_grad_(leaf), torch.ones_like(t))
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    f(dual)
+                with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
+                    f(dual)
+    for f, t in calls:
+        f(t)

@@ -2,6 +2,7 @@
 // stream. Registered in the extension module by ops.cpp.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -462,7 +463,11 @@ void first_order_only() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "routed block operators are differentiable once (create_graph=True is not "
               "supported)");
 }
+// Nor have they a forward-mode form: a dual tensor would lose its tangent on the way.
 bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    for (const at::Tensor* t : ts)
+      TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "routed block operators have no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
