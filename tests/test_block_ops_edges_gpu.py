@@ -56,6 +56,26 @@ def test_nan_adds_nothing_to_its_group(score, E, groups, k):
     assert torch.equal(idx, want)
 
 
+@pytest.mark.parametrize("E", [8, 12, 64, 256, 500])
+def test_sigmoid_tells_far_negative_logits_apart(E):
+    """Logits from -86 to -101 (scores down to 2^-146): the choice goes by the logits, not by the index. Scores below 2^-126
+    are whole multiples of 2^-149."""
+    logits = torch.full((40, E), -math.inf, device="cuda")
+    rows = torch.arange(40, device="cuda")
+    for i in range(8):
+        logits[rows, (rows * 5 + i * 3) % 8] = -101.0 + 2 * i + rows / 80
+    k = 4
+    w, idx = Rt.route_experts(logits, k, score="sigmoid", renorm=False)
+    want = logits.double().topk(k).indices
+    assert torch.equal(idx.long(), want)
+    p = torch.sigmoid(logits.double()).gather(1, want)
+    assert ((w.double() - p).abs() <= p * 2.0 ** -20 + 2.0 ** -149).all()
+    assert torch.equal(R.route_experts(logits, k, "sigmoid")[1], idx)
+    assert torch.equal(R.route_experts(logits.cpu(), k, "sigmoid")[1], idx.cpu())
+    low = torch.tensor([[-103.0, -102.0, -101.5, -101.0, -104.0, -200.0, -math.inf, -103.5]], device="cuda")
+    assert Rt.route_experts(low, 3, score="sigmoid")[1].tolist() == [[3, 2, 1]]
+
+
 @pytest.mark.parametrize("E,k", [(8, 2), (40, 3), (256, 8), (500, 32)])
 def test_gradient_of_nearly_impossible_choices(E, k):
     """softmax, renormalised, and a bias that moves the choice to experts of a probability near 1e-20: the + 1e-20 of the

@@ -103,8 +103,12 @@ __device__ __forceinline__ void load_logits(const RouteParams& p, long long n, i
   }
 }
 
-// 1 + exp(-l) is rounded once relative to itself, so small scores keep their relative precision; below l = -88 they are 0
+// 1 + exp(-l) is rounded once relative to itself, so small scores keep their relative precision, until exp(-l) comes near
+// the largest float: below l = -88.7 this is 0. There the score is exp(l) (they differ by exp(l) of it), subnormal
+// down to l = -104, and logits are still told apart. Few tokens hold such a logit, and switched-off experts (-inf) are none.
 __device__ __forceinline__ float sigmoid_of(float l) { return __frcp_rn(1.f + expf(-l)); }
+constexpr float FAR_DOWN = 9.f;
+__device__ __forceinline__ bool far_down(float l) { return fabsf(l + 96.f) < FAR_DOWN; }
 
 }  // namespace
 
@@ -164,8 +168,21 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_fwd_blocks(EPL)) route
       if (li == 0) mxz[at] = make_float2(mx, z);
     }
     if (p.sigmoid) {
+      float far = FAR_DOWN, sc[EPL];
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) l[j] = sigmoid_of(l[j]);
+      for (int j = 0; j < EPL; j += 2) {
+        const float2 t = x2_split(x2_add(x2(l[j], l[j + 1]), x2(96.f)));
+        far = fminf(far, fminf(fabsf(t.x), fabsf(t.y)));
+      }
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) sc[j] = sigmoid_of(l[j]);
+      if (__builtin_expect(far < FAR_DOWN, 0)) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j)
+          if (far_down(l[j])) sc[j] = expf(l[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) l[j] = sc[j];
     }
 #pragma unroll
     for (int j = 0; j < EPL; ++j) l[j] += bias[j];
@@ -300,7 +317,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_fwd_blocks(EPL)) route
     const float l = on ? to_f<T>(reinterpret_cast<const T*>(p.logits)[n * p.ld + e]) : 0.f;
     float s, z = 1.f;
     if (p.sigmoid) {
-      s = sigmoid_of(l);
+      s = far_down(l) ? expf(l) : sigmoid_of(l);
     } else {
       // without the whole row's: the best of all (its group is the best group, and no bias moves the order)
       float mx = __shfl_sync(0xffffffffu, l, lane & ~(slots - 1));

@@ -150,7 +150,8 @@ def route_experts(logits, k, score="softmax", bias=None, groups=1, top_groups=1,
         p = torch.where((l == -math.inf), torch.zeros_like(p), p)
         key = l.detach()
     else:
-        p = torch.sigmoid(l)
+        ex = torch.exp(torch.where(l >= 0, -l, l))  # torch's own sigmoid is 0 below -88 in 32 bits: ties of what differs
+        p = torch.where(l >= 0, torch.ones_like(ex), ex) / (1 + ex)
         key = p.detach()
     if bias is not None:
         key = key + bias
