@@ -7,6 +7,7 @@ import torch
 
 _C = None
 _ERR = {}
+_ON_LOAD = []  # called once the compiled module is there, with the first ext()
 
 
 def ext():
@@ -20,6 +21,8 @@ def ext():
             raise ImportError("trenowanie_generatora_obrazkow_b200._C is not built; run "
                               "`python setup.py build_ext --inplace` in the repository root") from e
         _C = mod
+        for fn in _ON_LOAD:
+            fn()
     return _C
 
 

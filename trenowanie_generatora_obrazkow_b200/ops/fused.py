@@ -23,6 +23,7 @@ import math
 
 import torch
 
+from . import _ext
 from . import reference as R
 from ._ext import _ERR, err_buf, ext
 from .gemm import gemm
@@ -93,9 +94,13 @@ def remove_grad_ready_hook(fn):
 
 
 def _hooks_to_ext():
-    """The backward kernels with a C++ autograd node call the hooks themselves, while there are any."""
-    if torch.cuda.is_available():
-        ext().set_grad_ready(bool(_GRAD_HOOKS), _notify)
+    """The backward kernels with a C++ autograd node call the hooks themselves, while there are any. A process that has
+    not loaded the extension (training on the CPU) does not load it for this: it hears of the hooks when it is loaded."""
+    if _ext._C is not None:
+        _ext._C.set_grad_ready(bool(_GRAD_HOOKS), _notify)
+
+
+_ext._ON_LOAD.append(_hooks_to_ext)
 
 
 def _err_word(t):
