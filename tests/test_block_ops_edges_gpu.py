@@ -261,3 +261,45 @@ def test_forward_mode_derivatives_are_refused():
                     f(dual)
     for f, t in calls:
         f(t)
+
+
+def test_launch_counts_are_those_of_the_kernels():
+    """The extension's launch counter against the kernels that torch's profiler sees."""
+    from trenowanie_generatora_obrazkow_b200.ops._ext import ext
+    g = gen(46)
+    leaf = lambda *s: rnd(g, *s).requires_grad_()
+    w, logits, pos = leaf(64), leaf(9, 8), torch.zeros(2, 3, 1, device="cuda", dtype=torch.int32)
+    Fz.err_buf("cuda")
+
+    def sandwich(B, T, weights, gate):
+        x, y, m = leaf(B, T, 64), leaf(B, T, 64), leaf(B, 64)
+        post_w, w = (leaf(64) if weights else torch.ones(64, device="cuda") for _ in range(2))
+        a, h = Fz.sandwich_norm(x, y, m if gate else None, post_w=post_w, w=w)
+        return lambda: torch.autograd.backward([a, h], [x.detach(), y.detach()])
+
+    def rope(norm):
+        q, k = leaf(2, 3, 4, 64), leaf(2, 3, 2, 64)
+        a, b = Fz.rope_axes(q, k, pos, (64,), q_w=leaf(64) if norm else None, k_w=leaf(64) if norm else None)
+        return lambda: torch.autograd.backward([a, b], [q.detach(), k.detach()])
+
+    def rows(n, d, cap):
+        plan = Rt.expert_plan(torch.zeros(n, 2, device="cuda", dtype=torch.int32), 4, capacity=cap)
+        x, y, u = leaf(n, d), leaf(plan.rows, d), torch.ones(n, 2, device="cuda")
+
+        def f():
+            a, b = Rt.expert_dispatch(x, plan), Rt.expert_combine(y, u, plan)
+            torch.autograd.backward([a, b], [y.detach(), x.detach()])
+        return f
+    cases = [sandwich(2, 8, True, True), sandwich(2, 8, False, True), sandwich(300, 2, True, True),
+             sandwich(300, 2, False, True), sandwich(300, 2, True, False), rope(True), rope(False), rows(5, 16, None),
+             rows(5, 16, 3), rows(0, 16, 3), rows(0, 16, None), rows(5, 0, None), lambda: Rt.route_experts(logits, 2),
+             lambda: Rt.route_experts(logits[:0], 2), lambda: Fz.sandwich_norm(torch.zeros(0, 3, 64, device="cuda"),
+                                                                               torch.zeros(0, 3, 64, device="cuda"), w=w)]
+    for i, f in enumerate(cases):
+        torch.cuda.synchronize()
+        n0 = ext().launch_count()
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+            f()
+            torch.cuda.synchronize()
+        seen = sum(e.count for e in prof.key_averages() if "tgo::" in e.key)
+        assert ext().launch_count() - n0 == seen, (i, ext().launch_count() - n0, seen)

@@ -184,7 +184,7 @@ at::Tensor expert_dispatch(at::Tensor x, at::Tensor slot, at::Tensor offsets, at
   const ExpertRows r = expert_rows(slot, offsets, counts, capacity, rows, x.size(1), x);
   at::Tensor xs = fresh({rows, x.size(1)}, x.scalar_type(), x);
   BLOCK_LAUNCH(dispatch_launch(r, x.data_ptr(), x.stride(0), xs.data_ptr(), elem_of(x, "expert_dispatch"),
-                               at::cuda::getCurrentCUDAStream()), 1);
+                               at::cuda::getCurrentCUDAStream()), xs.numel() > 0);
   return xs;
 }
 
@@ -196,7 +196,7 @@ at::Tensor expert_combine(at::Tensor y, OptT w, at::Tensor slot, at::Tensor offs
   const float* wp = vec_f32(w, slot.numel(), y, "expert_combine: w");
   at::Tensor out = fresh({r.N, y.size(1)}, y.scalar_type(), y);
   BLOCK_LAUNCH(combine_launch(r, y.data_ptr(), wp, out.data_ptr(), elem_of(y, "expert_combine"),
-                              at::cuda::getCurrentCUDAStream()), 1);
+                              at::cuda::getCurrentCUDAStream()), out.numel() > 0);
   return out;
 }
 
@@ -213,7 +213,7 @@ std::tuple<at::Tensor, at::Tensor> expert_combine_bwd(at::Tensor y, at::Tensor w
   at::Tensor dy = fresh_like(y), dw = fresh({r.N, r.k}, at::kFloat, y);
   BLOCK_LAUNCH(combine_bwd_launch(r, y.data_ptr(), wp, dout.data_ptr(), dout.stride(0), dy.data_ptr(),
                                   dw.data_ptr<float>(), elem_of(y, "expert_combine_bwd"),
-                                  at::cuda::getCurrentCUDAStream()), 1);
+                                  at::cuda::getCurrentCUDAStream()), r.N > 0 || r.rows > 0);
   return {dy, dw};
 }
 
@@ -335,7 +335,8 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
   at::Tensor scratch = fresh({floats}, at::kFloat, x);
   q.partial = scratch.data_ptr<float>();
   q.wpart = q.partial + entries * 3 * D;
-  BLOCK_LAUNCH(sandwich_bwd_launch(p, q, elem, err_word(err, x), at::cuda::getCurrentCUDAStream()), 3);
+  const bool two_steps = q.groups > 1 && (q.dw != nullptr || q.dpost_w != nullptr);  // of the weights' sums
+  BLOCK_LAUNCH(sandwich_bwd_launch(p, q, elem, err_word(err, x), at::cuda::getCurrentCUDAStream()), 2 + two_steps);
   return {dx, dy, dgate, dshift, dscale};
 }
 

@@ -427,7 +427,7 @@ cudaError_t combine_bwd_run(const ExpertRows& r, const T* y, const float* w, con
   return cudaErrorInvalidValue
 
 cudaError_t dispatch_launch(const ExpertRows& r, const void* x, long long ldx, void* xs, int elem, cudaStream_t s) {
-  if (r.D <= 0 || (r.N <= 0 && r.rows <= 0)) return cudaSuccess;
+  if (r.D <= 0 || r.rows <= 0) return cudaSuccess;
 #define TGO_CALL(T)                                                                                        \
   return rows_aligned<T>(r, x, xs, ldx)                                                                    \
              ? dispatch_run<T, 8>(r, static_cast<const T*>(x), ldx, static_cast<T*>(xs), s)                \

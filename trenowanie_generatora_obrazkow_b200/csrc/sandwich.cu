@@ -17,7 +17,8 @@
 //
 // Column sums: a unit (a CTA, or a group of its threads) owns a contiguous span of rows and writes one partial row (three
 // sums per channel) per sample it meets. Entry unit + sample is unique (along the spans both only grow), so
-// units + samples entries hold them all; two small kernels add them in a fixed order.
+// units + samples entries hold them all. A second launch adds them in a fixed order, and from 257 samples on a third the
+// weights' sums of its groups of samples.
 #include <algorithm>
 #include <vector>
 
