@@ -101,6 +101,18 @@ def test_gradient_of_nearly_impossible_choices(E, k):
     assert ((x.grad.double() - y.grad).abs() <= 64 * 2.0 ** -24 * terms + 1e-30).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16])
+def test_plan_of_numbers_that_are_no_expert(dtype):
+    """Whatever lies outside 0 .. experts - 1 takes no row, in wide types too."""
+    info = torch.iinfo(dtype)
+    idx = torch.tensor([[0, 3], [4, -1], [info.max, info.min], [1, min(info.max, 2 ** 32 + 1)], [min(info.max, 2 ** 32), 2]],
+                       dtype=dtype)
+    plan = Rt.expert_plan(idx.cuda(), 4)
+    slot, offsets, counts = R.expert_plan(idx, 4)
+    assert torch.equal(plan.slot.cpu(), slot) and torch.equal(plan.counts.cpu(), counts)
+    assert plan.counts.tolist() == [1, 1, 1, 1] and torch.equal(plan.offsets.cpu(), offsets)
+
+
 # ----------------------------------------------------------------------------------------------------------------
 # rotary positions
 # ----------------------------------------------------------------------------------------------------------------

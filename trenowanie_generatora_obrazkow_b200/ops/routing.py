@@ -54,8 +54,9 @@ def route_experts(logits, k, score="softmax", bias=None, groups=1, top_groups=1,
 
 
 def expert_plan(idx, experts, capacity=None):
-    """Rows of the assignments idx int [N, k] (< 0: none) in expert order, token order within an expert. capacity: every
-    expert owns that many rows and later assignments are dropped (their slot is -1); None: packed without gaps."""
+    """Rows of the assignments idx int [N, k] (outside 0 .. experts - 1: none) in expert order, token order within an
+    expert. capacity: every expert owns that many rows and later assignments are dropped (their slot is -1); None: packed
+    without gaps."""
     if idx.dim() != 2 or not 1 <= experts <= MAX_EXPERTS:
         raise ValueError(f"expert_plan: idx [N, k] and 1 to {MAX_EXPERTS} experts")
     if capacity is not None and capacity < 1:
@@ -65,6 +66,8 @@ def expert_plan(idx, experts, capacity=None):
         slot, offsets, counts = R.expert_plan(idx, experts, cap)
     else:
         if idx.dtype is not torch.int32 or not idx.is_contiguous():
+            if idx.dtype is torch.int64:  # what does not fit 32 bits is no expert
+                idx = idx.clamp(-1, experts)
             idx = idx.to(torch.int32).contiguous()
         slot, offsets, counts = ext().expert_plan(idx, experts, cap)
     return ExpertPlan(slot, offsets, counts, cap, experts * cap if cap else idx.numel())
