@@ -48,3 +48,13 @@ def test_grad_ready_hooks_do_not_load_the_extension(monkeypatch):
     finally:
         Fz.remove_grad_ready_hook(hook)
     assert told[-1][0] is False
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("scale", [0.0, 1e-50, -1e-39, 1e39, math.inf, math.nan])
+def test_scale_that_fp32_does_not_hold_is_refused(device, scale):
+    """The weights' gradient is divided by the scale in 32 bits."""
+    logits = torch.randn(2, 8, device=device)
+    with pytest.raises(ValueError, match="scale"):
+        Rt.route_experts(logits, 2, scale=scale)
+    assert Rt.route_experts(logits, 2, scale=-2.0 ** -126)[0].shape == (2, 2)

@@ -75,7 +75,8 @@ RouteParams route_params(const at::Tensor& logits, int64_t k, bool sigmoid, int6
   TORCH_CHECK(top_groups >= 1 && top_groups <= groups, "route: 1 <= top_groups <= groups");
   TORCH_CHECK(k >= 1 && k <= kRouteMaxK && k <= top_groups * (E / groups), "route: k between 1 and ", kRouteMaxK,
               " and at most the experts of the kept groups");
-  TORCH_CHECK(std::isfinite(scale) && scale != 0.0, "route: scale must be finite and not zero");
+  // the backward divides by it
+  TORCH_CHECK(std::isnormal((float)scale), "route: scale must be a normal fp32 number and not zero");
   RouteParams p{};
   p.logits = logits.data_ptr();
   p.ld = logits.stride(0);

@@ -37,7 +37,7 @@ def route_experts(logits, k, score="softmax", bias=None, groups=1, top_groups=1,
     ``bias`` [E] fp32 (for balance: it moves the choice, not the weights), in descending order, ties to the lowest
     index. groups > 1: only the ``top_groups`` best of the ``groups`` equal runs of experts take part, a group's worth
     being its best expert (softmax) or the sum of its two best (sigmoid). renorm divides the weights by their sum
-    (+ 1e-20); ``scale`` (not zero) multiplies them. valid [N] bool: False rows get w 0 and idx -1. NaN logits are chosen
+    (+ 1e-20); ``scale`` (a normal fp32 number) multiplies them. valid [N] bool: False rows get w 0 and idx -1. NaN logits are chosen
     last; the weights of their row are unspecified. The gradient reaches the logits through the weights (once)."""
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"route_experts: score is 'softmax' or 'sigmoid', not {score!r}")
@@ -48,6 +48,8 @@ def route_experts(logits, k, score="softmax", bias=None, groups=1, top_groups=1,
             and 1 <= k <= min(MAX_CHOICES, top_groups * (E // groups))):
         raise ValueError(f"route_experts: {E} experts, groups={groups}, top_groups={top_groups}, k={k} (at most "
                          f"{MAX_EXPERTS} experts in equal groups, k at most {MAX_CHOICES} and the kept groups' experts)")
+    if not 2.0 ** -126 <= abs(scale) < 2.0 ** 128:
+        raise ValueError(f"route_experts: scale is a normal fp32 number and not zero, not {scale}")
     if not logits.is_cuda:
         return R.route_experts(logits, k, score, bias, groups, top_groups, renorm, scale, valid)
     return ext().route_experts(logits, bias, valid, k, score == "sigmoid", groups, top_groups, renorm, scale)
