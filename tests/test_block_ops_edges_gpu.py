@@ -138,6 +138,20 @@ def test_rope_axes_of_the_widest_heads(d, axes, norm, interleaved, dtype):
         assert a is None or (a.grad.double() - b.grad).norm() <= 64 * 2.0 ** -24 * 54 ** 0.5 * b.grad.norm()
 
 
+@pytest.mark.parametrize("d", [64, 50])
+def test_rope_axes_at_the_last_positions(d):
+    """Integer positions up to 2^24 and fractional ones, fastest pairs included: angles to 2^-22 of a revolution (the
+    two-part frequency's rest, 2^-48 relative to the first part, times 2^24 turns, and fp32 roundings of a fraction)."""
+    g = gen(47)
+    q = torch.ones(1, 4000, 1, d, device="cuda")
+    pos = torch.randint(0, 2 ** 24, (1, 4000, 1), device="cuda", generator=g).int()
+    pos[0, :4, 0] = torch.tensor([0, 1, 2 ** 24 - 1, -2 ** 24 + 1])
+    for p in (pos, torch.rand(1, 4000, 1, device="cuda", generator=g) * 1000, pos.float()):
+        got, _ = Fz.rope_axes(q, q, p, (d,), theta=1e4)
+        want, _ = R.rope_axes(q.double(), q.double(), p, (d,), theta=1e4)
+        assert (got.double() - want).abs().max() <= 2 ** 0.5 * 2 * math.pi * 2.0 ** -22 + 2.0 ** -22
+
+
 # ----------------------------------------------------------------------------------------------------------------
 # sandwich norm
 # ----------------------------------------------------------------------------------------------------------------

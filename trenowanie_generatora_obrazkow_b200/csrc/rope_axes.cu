@@ -37,9 +37,10 @@ __device__ __forceinline__ float position(const RopeAxesParams& p, long long tok
   return p.pos_f32 ? reinterpret_cast<const float*>(p.pos)[i] : (float)reinterpret_cast<const int*>(p.pos)[i];
 }
 
-// cos / sin of an angle of pos (hi + lo) revolutions
+// cos / sin of an angle of pos (hi + lo) revolutions. The product has to be the rounded one where its whole turns are taken
+// off: fused into that subtraction it would bring its rounding error in twice.
 __device__ __forceinline__ void turn_at(float pos, float hi, float lo, float& cs, float& sn) {
-  const float whole = pos * hi;
+  const float whole = __fmul_rn(pos, hi);
   float rev = whole - rintf(whole);
   rev += fmaf(pos, hi, -whole) + pos * lo;
   sincospif(2.f * rev, &sn, &cs);
