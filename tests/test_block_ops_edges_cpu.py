@@ -1,13 +1,19 @@
 """Edges of the routed block's operators that need no GPU: the CPU definitions at special values, and what the modules do on a
 machine without the compiled extension."""
 import math
+import os
+import socket
 import sys
+import tempfile
 import types
 
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 import trenowanie_generatora_obrazkow_b200 as package
+from trenowanie_generatora_obrazkow_b200.models.routed import RoutedConfig, RoutedDenoiser, RoutedMLP
 from trenowanie_generatora_obrazkow_b200.ops import _ext
 from trenowanie_generatora_obrazkow_b200.ops import fused as Fz
 from trenowanie_generatora_obrazkow_b200.ops import routing as Rt
@@ -58,3 +64,48 @@ def test_scale_that_fp32_does_not_hold_is_refused(device, scale):
     with pytest.raises(ValueError, match="scale"):
         Rt.route_experts(logits, 2, scale=scale)
     assert Rt.route_experts(logits, 2, scale=-2.0 ** -126)[0].shape == (2, 2)
+
+
+def _balance_model():
+    torch.manual_seed(3)
+    cfg = RoutedConfig(latent_channels=4, dim=32, depth=2, heads=2, kv_heads=2, axes=(4, 6, 6), text_dim=8, experts=8,
+                       top_k=2, expert_hidden=16, groups=1, top_groups=1)
+    return RoutedDenoiser(cfg), RoutedMLP(16, 8, experts=8, top_k=1)
+
+
+def _balance_inputs():
+    g = torch.Generator().manual_seed(4)
+    rnd = lambda *s: torch.randn(*s, generator=g)
+    return rnd(4, 4, 2, 3, 5), torch.rand(4, generator=g), rnd(4, 3, 8), rnd(4, 50, 16) + 0.5
+
+
+def _balance_steps(rows):
+    model, mlp = _balance_model()
+    z, t, text, h = (x[rows] for x in _balance_inputs())
+    with torch.no_grad():
+        for _ in range(5):
+            model(z, t, text)
+            mlp(h)
+            model.update_balance(0.05)
+            mlp.update_balance(0.05)
+    return torch.stack([*(b.mlp.balance for b in model.blocks), mlp.balance])
+
+
+def _balance_worker(rank, world, port, out):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    n = 4 // world
+    torch.save(_balance_steps(slice(rank * n, rank * n + n)), os.path.join(out, f"{rank}.pt"))
+    dist.destroy_process_group()
+
+
+def test_balance_is_that_of_all_ranks():
+    """Two ranks with half of the samples each move the balance bias as one process with all of them."""
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    with tempfile.TemporaryDirectory() as out:
+        mp.spawn(_balance_worker, args=(2, port, out), nprocs=2, join=True)
+        a, b = (torch.load(os.path.join(out, f"{r}.pt")) for r in range(2))
+    want = _balance_steps(slice(None))
+    assert want.abs().sum() > 0 and torch.equal(a, b) and torch.allclose(a, want, atol=1e-6)

@@ -19,6 +19,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+import torch.distributed as dist
 import torch.nn as nn
 
 from ..ops import fused as Fz
@@ -49,6 +50,12 @@ class RoutedConfig:
     route_scale: float = 1.0
     capacity_factor: float = 1.25
     res_scale: float = 1.0
+
+
+def _total_load(load, group):
+    if dist.is_available() and dist.is_initialized() and dist.get_world_size(group) > 1:
+        dist.all_reduce(load, group=group)
+    return load
 
 
 class RoutedMLP(nn.Module):
@@ -93,11 +100,14 @@ class RoutedMLP(nn.Module):
         return Rt.expert_combine(y.to(h.dtype), w, plan).view(h.shape)
 
     @torch.no_grad()
-    def update_balance(self, rate=1e-3):
-        """Move the balance bias of overloaded experts down and of underloaded ones up (once per step)."""
+    def update_balance(self, rate=1e-3, group=None):
+        """Move the balance bias of overloaded experts down and of underloaded ones up (once per step). The load is that of
+        all ranks of the process group (None: the default one, where there is one), so replicas keep one bias."""
         if self.counts is not None:
-            load = self.counts.float()
-            self.balance += rate * (load.mean() - load).sign()
+            self._move_balance(_total_load(self.counts.float(), group), rate)
+
+    def _move_balance(self, load, rate):
+        self.balance += rate * (load.mean() - load).sign()
 
 
 class RoutedBlock(nn.Module):
@@ -174,6 +184,10 @@ class RoutedDenoiser(nn.Module):
         _, hn = Fz.sandwich_norm(x, *pending, self.norm.weight, res_scale=self.config.res_scale)
         return Fz.linear(hn, self.patch_out).transpose(1, 2).reshape(b, c, f, h, w)
 
-    def update_balance(self, rate=1e-3):
-        for blk in self.blocks:
-            blk.mlp.update_balance(rate)
+    @torch.no_grad()
+    def update_balance(self, rate=1e-3, group=None):
+        """RoutedMLP.update_balance of every block, with one sum over the ranks."""
+        mlps = [blk.mlp for blk in self.blocks if blk.mlp.counts is not None]
+        if mlps:
+            for mlp, load in zip(mlps, _total_load(torch.stack([m.counts.float() for m in mlps]), group)):
+                mlp._move_balance(load, rate)
