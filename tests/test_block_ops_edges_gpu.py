@@ -4,6 +4,7 @@ places, lengths and sizes at the limits), each against the definition in 64 bits
 import math
 
 import pytest
+import test_block_ops_gpu as plain
 import torch
 
 from trenowanie_generatora_obrazkow_b200.ops import fused as Fz
@@ -166,6 +167,15 @@ def test_sandwich_norm_refuses_more_rows_than_it_counts(shape):
     with pytest.raises(RuntimeError, match="rows"):
         Fz.sandwich_norm(x, x, w=w)
     assert torch.cuda.memory_allocated() == before
+
+
+@pytest.mark.parametrize("B,T,D,post,gate,mod,pre,res,dtype", [
+    (2, 10, 2560, True, True, True, True, 0.5, BF16), (3, 7, 2304, True, True, True, True, 1.0, F16),
+    (2, 400, 2064, True, False, False, True, 1.0, BF16), (4, 90, 2560, True, True, True, True, 1.0, F32),
+    (2, 31, 2056, False, True, True, True, 1.0, BF16), (2, 12, 2568, True, True, True, True, 1.0, F16)])
+def test_sandwich_norm_of_2056_to_2560_channels(B, T, D, post, gate, mod, pre, res, dtype):
+    """The widths whose backward takes one row per step, and one past them, against 64 bits."""
+    plain.test_sandwich_norm(B, T, D, post, gate, mod, pre, res, dtype)
 
 
 # ----------------------------------------------------------------------------------------------------------------

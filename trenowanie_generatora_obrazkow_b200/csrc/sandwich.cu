@@ -693,21 +693,28 @@ int sw_blocks(const SandwichParams& p, const SwGeom& g) {
 }
 
 // Calls f(kernel, R, tensors, element size) with the variant for p: R rows per step, as many as divide a sample's rows;
-// threads up to 256 (8 slots of the group sums), 320 and 512 (16 slots).
+// threads up to 256 (8 slots of the group sums) or 512 (16 slots). The backward of 257 to 320 threads (2056 to 2560
+// channels) has a variant of its own, two blocks per SM in 96 registers with one row per step; us at 32 x 1024 x 2560 bf16 / fp32:
+// that 201 / 341, in 512 threads with two rows 221 (fp32: one row 355), in 320 threads with two rows 356 (spills). 7 x 333 x
+// 2560: 24.3, 25.4, 38.4. The forward needs none: 116 / 240 with 320 threads, 116 / 221 with 512.
 template <typename T, int R, typename F>
 auto sw_fwd_width(const SandwichParams& p, F f) {
   SwGeom g;
-  const int threads = sw_threads(p, &g);
-  if (threads <= 256) return f(sandwich_fwd_kernel<T, R, 8, 256, 2>, R, 2, (int)sizeof(T));
-  if (threads <= 320) return f(sandwich_fwd_kernel<T, R, 16, 320, 2>, R, 2, (int)sizeof(T));
+  if (sw_threads(p, &g) <= 256) return f(sandwich_fwd_kernel<T, R, 8, 256, 2>, R, 2, (int)sizeof(T));
   return f(sandwich_fwd_kernel<T, R, 16, 512, 1>, R, 2, (int)sizeof(T));
+}
+bool sw_bwd_narrow(const SandwichParams& p) {
+  SwGeom g;
+  const int threads = sw_threads(p, &g);
+  return threads > 256 && threads <= 320;
 }
 template <typename T, int R, typename F>
 auto sw_bwd_width(const SandwichParams& p, F f) {
   SwGeom g;
-  const int threads = sw_threads(p, &g);
-  if (threads <= 256) return f(sandwich_bwd_kernel<T, R, 8, 256, 2>, R, 4, (int)sizeof(T));
-  if (threads <= 320) return f(sandwich_bwd_kernel<T, R, 16, 320, 2>, R, 4, (int)sizeof(T));
+  if (sw_threads(p, &g) <= 256) return f(sandwich_bwd_kernel<T, R, 8, 256, 2>, R, 4, (int)sizeof(T));
+  if constexpr (R == 1) {
+    if (sw_bwd_narrow(p)) return f(sandwich_bwd_kernel<T, R, 16, 320, 2>, R, 4, (int)sizeof(T));
+  }
   return f(sandwich_bwd_kernel<T, R, 16, 512, 1>, R, 4, (int)sizeof(T));
 }
 template <typename T, int R, typename F>
@@ -720,7 +727,7 @@ auto sw_fwd_pick(const SandwichParams& p, F f) {
 template <typename T, int R, typename F>
 auto sw_bwd_pick(const SandwichParams& p, F f) {
   if constexpr (R > 1) {
-    if (samples_of(p) > 1 && p.T % R != 0) return sw_bwd_pick<T, R / 2>(p, f);
+    if ((samples_of(p) > 1 && p.T % R != 0) || sw_bwd_narrow(p)) return sw_bwd_pick<T, R / 2>(p, f);
   }
   return sw_bwd_width<T, R>(p, f);
 }
