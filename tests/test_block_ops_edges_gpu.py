@@ -114,6 +114,17 @@ def test_plan_of_numbers_that_are_no_expert(dtype):
     assert plan.counts.tolist() == [1, 1, 1, 1] and torch.equal(plan.offsets.cpu(), offsets)
 
 
+@pytest.mark.parametrize("N,E,k,cap", [(1023, 64, 2, None), (1024, 64, 2, None), (1025, 64, 2, 30), (2049, 8, 1, None),
+                                       (683, 512, 3, 4), (2000, 256, 2, None), (4096, 7, 2, 1100)])
+def test_plan_on_both_sides_of_the_cluster(N, E, k, cap):
+    """One CTA up to 2048 assignments, a cluster above: the same stable order."""
+    idx = plain.choices(gen(48), N, E, k, 0.1)
+    plan = Rt.expert_plan(idx, E, capacity=cap)
+    slot, offsets, counts = R.expert_plan(idx.cpu(), E, cap or 0)
+    assert torch.equal(plan.slot.cpu(), slot) and torch.equal(plan.offsets.cpu(), offsets)
+    assert torch.equal(plan.counts.cpu(), counts)
+
+
 # ----------------------------------------------------------------------------------------------------------------
 # rotary positions
 # ----------------------------------------------------------------------------------------------------------------
