@@ -732,20 +732,10 @@ std::tuple<at::Tensor, at::Tensor> rope_axes(at::Tensor q, at::Tensor k, at::Ten
 
 void bind_block_ops(pybind11::module_& m) {
   m.def("route_experts", &route_experts, "expert scores, group-limited top-k and weights of every token");
-  m.def("route_fwd", &route_fwd, "route_experts without autograd");
-  m.def("route_bwd", &route_bwd, "gradient of the chosen experts' weights to the router's logits");
   m.def("expert_plan", &expert_plan, "stable row of every assignment in expert order, offsets and counts");
   m.def("dispatch_rows", &dispatch_rows, "token rows into expert order");
-  m.def("expert_dispatch", &expert_dispatch, "dispatch_rows without autograd");
   m.def("combine_rows", &combine_rows, "weighted sum of a token's rows from expert order");
-  m.def("expert_combine", &expert_combine, "combine_rows without autograd");
-  m.def("expert_combine_bwd", &expert_combine_bwd, "gradient of combine_rows to the rows and the weights");
   m.def("sandwich_norm", &sandwich_norm, "x + r gate rmsnorm(y) post_w, then rmsnorm, w, scale and shift");
-  m.def("sandwich_fwd", &sandwich_fwd, "sandwich_norm without autograd, with its statistics");
-  m.def("sandwich_bwd", &sandwich_bwd, "backward of sandwich_fwd", py::arg("dx_new"), py::arg("dh"), py::arg("x"),
-        py::arg("y"), py::arg("gate"), py::arg("post_w"), py::arg("w"), py::arg("shift"), py::arg("scale"),
-        py::arg("ry"), py::arg("rx"), py::arg("dpost_w"), py::arg("dw"), py::arg("res_scale"), py::arg("eps"),
-        py::arg("err"), py::arg("add_post_w") = true, py::arg("add_w") = true);
   m.def("rope_axes", &rope_axes, "q/k RMSNorm and rotary positions with several axes");
   m.def("rope_axes_fwd", &rope_axes_fwd, "rope_axes of token rows without autograd");
   m.def("rope_axes_bwd", &rope_axes_bwd, "backward of rope_axes_fwd", py::arg("dq"), py::arg("dk"), py::arg("q"),
