@@ -164,6 +164,47 @@ def test_rope_axes_at_the_last_positions(d):
         assert (got.double() - want).abs().max() <= 2 ** 0.5 * 2 * math.pi * 2.0 ** -22 + 2.0 ** -22
 
 
+# (B, T, Hq, Hkv, d, axes, interleaved, norm, kv_len, positions): one token, masked tails, a sample without keys, shared
+# heads, partial rotation
+@pytest.mark.parametrize("B,T,hq,hkv,d,axes,inter,norm,lens,frac", [
+    (2, 77, 4, 2, 64, (16, 24, 24), True, True, (77, 30), False), (1, 130, 2, 2, 128, (64, 64), False, True, None, True),
+    (3, 64, 6, 2, 128, (32, 32), False, False, (64, 1, 0), False), (2, 1, 4, 1, 64, (64,), False, True, None, False),
+    (2, 33, 3, 3, 64, (20,), True, False, (33, 0), True), (1, 257, 8, 8, 128, (16, 56, 56), False, True, (200,), False)])
+def test_axes_attention_core(B, T, hq, hkv, d, axes, inter, norm, lens, frac):
+    """Forward and gradients against the 64-bit definition. q and k after the rotation, the probabilities and the output are
+    rounded to bf16, in the backward dS and the gradients too: 2 % and 4 % of the norm, as for self_attention_core."""
+    g = gen(50)
+    qkv, up = rnd(g, B, T, (hq + 2 * hkv) * d, dtype=BF16), rnd(g, B, T, hq * d, dtype=BF16)
+    ws = [rnd(g, d, std=0.1, mean=1.0) for _ in range(2)] if norm else [None, None]
+    pos = torch.randint(0, 60, (B, T, len(axes)), device="cuda", generator=g)
+    pos = pos.float() * 0.5 - 3.25 if frac else pos
+    kv_len = None if lens is None else torch.tensor(lens, device="cuda", dtype=torch.int32)
+    leaf = [t.clone().requires_grad_() if t is not None else None for t in (qkv, *ws)]
+    out = Fz.axes_attention_core(leaf[0], pos, axes, hq, hkv, d, q_w=leaf[1], k_w=leaf[2], kv_len=kv_len, interleaved=inter)
+    out.backward(up)
+    wide = [t.double().requires_grad_() if t is not None else None for t in (qkv, *ws)]
+    q, k, v = wide[0].view(B, T, hq + 2 * hkv, d).split([hq, hkv, hkv], dim=2)
+    q, k = R.rope_axes(q, k, pos, axes, q_w=wide[1], k_w=wide[2], interleaved=inter)
+    live = [b for b in range(B) if lens is None or lens[b] > 0]
+    want = R.attention(q[live], k[live], v[live], None if lens is None else kv_len[live], d ** -0.5)
+    want.backward(up[live].double().view(len(live), T, hq, d))
+    want = want.detach().reshape(len(live), T, hq * d)
+    rel = lambda a, b: ((a.double() - b).norm() / b.norm()).item()
+    assert rel(out[live], want) < 2e-2 and rel(leaf[0].grad[live], wide[0].grad[live]) < 4e-2
+    parts = zip(leaf[0].grad.view(B, T, -1, d).split([hq, hkv, hkv], 2), wide[0].grad.view(B, T, -1, d).split([hq, hkv, hkv], 2))
+    for a, b in parts:  # dq, dk, dv (below: keys past kv_len get exactly nothing)
+        assert b.norm() == 0 and a.norm() == 0 or rel(a, b) < 4e-2 or b.norm() < 1e-6 * wide[0].grad.norm()
+    for b in live if lens is not None else []:
+        assert (leaf[0].grad.view(B, T, -1, d)[b, lens[b]:, hq:] == 0).all()
+    dead = [b for b in range(B) if b not in live]
+    assert (out[dead] == 0).all() and (leaf[0].grad[dead] == 0).all()
+    for a, b in zip(leaf[1:], wide[1:]):
+        assert a is None or rel(a.grad, b.grad) < 4e-2 or b.grad.norm() < 1e-6 * wide[0].grad.norm()
+    with torch.no_grad():
+        again = Fz.axes_attention_core(qkv, pos, axes, hq, hkv, d, q_w=ws[0], k_w=ws[1], kv_len=kv_len, interleaved=inter)
+    assert torch.equal(again, out)
+
+
 # ----------------------------------------------------------------------------------------------------------------
 # sandwich norm
 # ----------------------------------------------------------------------------------------------------------------
@@ -187,6 +228,38 @@ def test_sandwich_norm_refuses_more_rows_than_it_counts(shape):
 def test_sandwich_norm_of_2056_to_2560_channels(B, T, D, post, gate, mod, pre, res, dtype):
     """The widths whose backward takes one row per step, and one past them, against 64 bits."""
     plain.test_sandwich_norm(B, T, D, post, gate, mod, pre, res, dtype)
+
+
+@pytest.mark.parametrize("B,T,D,post,gate,mod,pre,res,dtype", [
+    (256, 2, 128, True, True, True, True, 1.0, BF16), (257, 1, 128, True, True, True, True, 1.0, BF16),
+    (700, 3, 264, True, True, False, True, 0.5, F32), (513, 2, 577, True, False, True, True, 1.0, F16),
+    (16500, 1, 64, True, True, True, True, 1.0, F32), (300, 2, 96, False, True, False, False, 1.0, F32)])
+def test_sandwich_norm_of_many_samples(B, T, D, post, gate, mod, pre, res, dtype):
+    """More than 256 gated or modulated samples: the weights' gradients are summed in groups of samples first."""
+    plain.test_sandwich_norm(B, T, D, post, gate, mod, pre, res, dtype)
+
+
+@pytest.mark.parametrize("B", [200, 700])
+def test_sandwich_norm_of_many_samples_into_a_grad(B):
+    """The same sums added to what .grad holds, with either weight left out. fp32; 1e-5 of the gradient's norm: sums of B 3
+    products, 2^-24 of each and of the partial sums."""
+    g = gen(49)
+    ins = plain.sandwich_inputs(g, B, 3, 128, True, True, True, True, F32)
+    up = [rnd(g, B, 3, 128) for _ in range(2)]
+    d = {n: t.double().requires_grad_() for n, t in ins.items()}
+    torch.autograd.backward(list(R.sandwich_norm(**d)), [u.double() for u in up])
+    for only in ("both", "w", "post_w"):
+        leaf = {n: t.clone().requires_grad_(n not in ("w", "post_w") or only in ("both", n)) for n, t in ins.items()}
+        start = {n: rnd(g, 128) for n in ("w", "post_w") if leaf[n].requires_grad}
+        for n, s in start.items():
+            leaf[n].grad = s.clone()
+        torch.autograd.backward(list(Fz.sandwich_norm(**leaf)), up)
+        for n in ("w", "post_w"):
+            if n in start:
+                diff = leaf[n].grad.double() - start[n].double() - d[n].grad
+                assert diff.norm() <= 1e-5 * (d[n].grad.norm() + start[n].norm())
+            else:
+                assert leaf[n].grad is None
 
 
 # ----------------------------------------------------------------------------------------------------------------
