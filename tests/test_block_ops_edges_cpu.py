@@ -109,3 +109,19 @@ def test_balance_is_that_of_all_ranks():
         a, b = (torch.load(os.path.join(out, f"{r}.pt")) for r in range(2))
     want = _balance_steps(slice(None))
     assert want.abs().sum() > 0 and torch.equal(a, b) and torch.allclose(a, want, atol=1e-6)
+
+
+both_devices = pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+
+
+@both_devices
+def test_empty_rows_of_any_stride(device):
+    """Empty tensors that are expanded or transposed are taken like contiguous ones."""
+    plan = Rt.expert_plan(torch.zeros(0, 2, device=device, dtype=torch.int32), 8, capacity=4)
+    empty = torch.zeros(1, 1, device=device).expand(0, 64)
+    pos = torch.zeros(2, 0, 1, device=device, dtype=torch.int32)
+    for x in (empty, torch.zeros(64, 0, device=device).t()):
+        assert Rt.route_experts(x, 2)[0].shape == (0, 2) and Rt.expert_dispatch(x, plan).shape == (32, 64)
+        h = Fz.sandwich_norm(x.view(0, 3, 64), x.view(0, 3, 64), gate=x, w=torch.ones(64, device=device))[1]
+        q = x.view(2, 0, 64).unflatten(-1, (4, 16)).transpose(0, 1).transpose(0, 1)
+        assert h.shape == (0, 3, 64) and Fz.rope_axes(q, q, pos, (16,))[0].shape == (2, 0, 4, 16)

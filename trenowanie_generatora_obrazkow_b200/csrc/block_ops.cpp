@@ -57,6 +57,9 @@ float* acc_f32(const OptT& t, int64_t n, const at::Tensor& as, const char* what)
   return const_cast<float*>(vec_f32(t, n, as, what));
 }
 
+// [N, D] with a row's elements side by side (an empty tensor's strides say nothing: a sum's gradient expands to 0)
+bool whole_rows(const at::Tensor& t) { return t.numel() == 0 || t.size(1) == 1 || t.stride(1) == 1; }
+
 int* err_word(const at::Tensor& err, const at::Tensor& as) {
   same_device(err, as, "err");
   TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() >= 1, "err: int32 error word");
@@ -66,7 +69,7 @@ int* err_word(const at::Tensor& err, const at::Tensor& as) {
 // ---------------------------------------------------------------------------------------------------------- routing
 RouteParams route_params(const at::Tensor& logits, int64_t k, bool sigmoid, int64_t groups, int64_t top_groups,
                          bool renorm, double scale) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && whole_rows(logits),
               "route: logits [N, E] with contiguous rows");
   const int64_t N = logits.size(0), E = logits.size(1);
   TORCH_CHECK(N < (1ll << 31) && E >= 1 && E <= kRouteMaxExperts, "route: 1 to ", kRouteMaxExperts, " experts");
@@ -179,7 +182,7 @@ ExpertRows expert_rows(const at::Tensor& slot, const at::Tensor& offsets, const 
 
 at::Tensor expert_dispatch(at::Tensor x, at::Tensor slot, at::Tensor offsets, at::Tensor counts, int64_t capacity,
                            int64_t rows) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(0) == slot.size(0) && (x.size(1) <= 1 || x.stride(1) == 1),
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(0) == slot.size(0) && whole_rows(x),
               "expert_dispatch: x [N, D] with contiguous rows, one per planned token");
   const c10::cuda::CUDAGuard guard(x.device());
   const ExpertRows r = expert_rows(slot, offsets, counts, capacity, rows, x.size(1), x);
@@ -205,7 +208,7 @@ std::tuple<at::Tensor, at::Tensor> expert_combine_bwd(at::Tensor y, at::Tensor w
                                                       at::Tensor offsets, at::Tensor counts, int64_t capacity) {
   TORCH_CHECK(y.is_cuda() && y.dim() == 2 && y.is_contiguous(), "expert_combine_bwd: y [rows, D], contiguous");
   TORCH_CHECK(dout.dim() == 2 && dout.size(0) == slot.size(0) && dout.size(1) == y.size(1) &&
-                  dout.scalar_type() == y.scalar_type() && (dout.size(1) <= 1 || dout.stride(1) == 1),
+                  dout.scalar_type() == y.scalar_type() && whole_rows(dout),
               "expert_combine_bwd: dout [N, D] with contiguous rows, in y's type");
   same_device(dout, y, "expert_combine_bwd: dout");
   const c10::cuda::CUDAGuard guard(y.device());
@@ -224,7 +227,7 @@ const void* sample_rows(const OptT& t, int64_t B, int64_t D, const at::Tensor& x
   if (!given(t)) return nullptr;
   same_device(*t, x, what);
   TORCH_CHECK(t->dim() == 2 && t->size(0) == B && t->size(1) == D && t->scalar_type() == x.scalar_type() &&
-                  (D <= 1 || t->stride(1) == 1),
+                  whole_rows(*t),
               what, ": [", B, ", ", D, "] rows in x's type with contiguous channels expected");
   *stride = B > 1 ? t->stride(0) : 0;
   return t->data_ptr();
@@ -344,6 +347,7 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
 // -------------------------------------------------------------------------------------------------- multi-axis rotary
 // [M, H, d] rows or [B, T, H, d] with evenly strided tokens, the heads of a token contiguous: the token stride; else -1
 int64_t token_stride(const at::Tensor& t) {
+  if (t.numel() == 0) return 0;
   const int64_t n = t.dim(), d = t.size(n - 1), H = t.size(n - 2), T = t.size(n - 3), B = n == 4 ? t.size(0) : 1;
   if ((d > 1 && t.stride(n - 1) != 1) || (H > 1 && t.stride(n - 2) != d)) return -1;
   if (B > 1 && T > 1 && t.stride(0) != T * t.stride(1)) return -1;
@@ -577,7 +581,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
 };
 std::tuple<at::Tensor, at::Tensor> route_experts(at::Tensor logits, OptT bias, OptT valid, int64_t k, bool sigmoid,
                                                  int64_t groups, int64_t top_groups, bool renorm, double scale) {
-  if (logits.dim() == 2 && logits.size(1) > 1 && logits.stride(1) != 1) logits = logits.contiguous();
+  if (logits.dim() == 2 && !whole_rows(logits)) logits = logits.contiguous();
   if (!wants_grad({&logits})) return route_fwd(logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale);
   auto out = RouteFn::apply(logits, bias, valid, k, sigmoid, groups, top_groups, renorm, scale);
   return {out[0], out[1]};
@@ -601,7 +605,7 @@ struct DispatchFn : public torch::autograd::Function<DispatchFn> {
 };
 at::Tensor dispatch_rows(at::Tensor x, at::Tensor slot, at::Tensor offsets, at::Tensor counts, int64_t capacity,
                          int64_t rows) {
-  if (x.dim() == 2 && x.size(1) > 1 && x.stride(1) != 1) x = x.contiguous();
+  if (x.dim() == 2 && !whole_rows(x)) x = x.contiguous();
   if (!wants_grad({&x})) return expert_dispatch(x, slot, offsets, counts, capacity, rows);
   return DispatchFn::apply(x, slot, offsets, counts, capacity, rows);
 }
@@ -618,7 +622,7 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
     first_order_only();
     const auto s = ctx->get_saved_variables();
     at::Tensor g = grads[0];
-    if (g.size(1) > 1 && g.stride(1) != 1) g = g.contiguous();
+    if (!whole_rows(g)) g = g.contiguous();
     auto [dy, dw] = expert_combine_bwd(s[0], s[1], g, s[2], s[3], s[4], ctx->saved_data["capacity"].toInt());
     variable_list out(6);
     out[0] = dy;
