@@ -125,3 +125,17 @@ def test_empty_rows_of_any_stride(device):
         h = Fz.sandwich_norm(x.view(0, 3, 64), x.view(0, 3, 64), gate=x, w=torch.ones(64, device=device))[1]
         q = x.view(2, 0, 64).unflatten(-1, (4, 16)).transpose(0, 1).transpose(0, 1)
         assert h.shape == (0, 3, 64) and Fz.rope_axes(q, q, pos, (16,))[0].shape == (2, 0, 4, 16)
+
+
+@both_devices
+def test_experts_of_no_tokens(device):
+    """Empty results and gradients, unfilled rows of 0."""
+    idx = torch.zeros(0, 2, device=device, dtype=torch.int32)
+    x, w = torch.zeros(0, 64, device=device, requires_grad=True), torch.zeros(0, 2, device=device, requires_grad=True)
+    for cap, rows in ((4, 32), (None, 0)):
+        plan = Rt.expert_plan(idx, 8, capacity=cap)
+        xs = Rt.expert_dispatch(x, plan)
+        out = Rt.expert_combine(xs, w, plan)
+        assert xs.shape == (rows, 64) and (xs == 0).all() and (plan.counts == 0).all() and out.shape == (0, 64)
+        out.sum().backward()
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape

@@ -210,8 +210,8 @@ def expert_combine(y, w, plan):
     rows = torch.cat([y, y.new_zeros(1, y.shape[1])])[torch.where(slot >= 0, slot, torch.full_like(slot, plan.rows))]
     keep = (slot >= 0).view(n, k, 1)
     wide = torch.promote_types(y.dtype, torch.float32)
-    return torch.where(keep, rows.view(n, k, -1).to(wide) * w[..., None].to(wide), torch.zeros((), dtype=wide)).sum(
-        1).to(y.dtype)
+    rows = rows.view(n, k, y.shape[1]).to(wide) * w[..., None].to(wide)
+    return torch.where(keep, rows, torch.zeros((), dtype=wide)).sum(1).to(y.dtype)
 
 
 def sandwich_norm(x, y, gate=None, post_w=None, w=None, shift=None, scale=None, res_scale=1.0, eps=EPS):
