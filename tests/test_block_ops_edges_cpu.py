@@ -139,3 +139,12 @@ def test_experts_of_no_tokens(device):
         assert xs.shape == (rows, 64) and (xs == 0).all() and (plan.counts == 0).all() and out.shape == (0, 64)
         out.sum().backward()
     assert x.grad.shape == x.shape and w.grad.shape == w.shape
+
+
+@both_devices
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_routing_of_no_tokens(device, score):
+    logits = torch.zeros(0, 8, device=device, requires_grad=True)
+    w, idx = Rt.route_experts(logits, 2, score=score)
+    w.sum().backward()
+    assert w.shape == idx.shape == (0, 2) and logits.grad.shape == (0, 8)

@@ -554,7 +554,7 @@ cudaError_t route_fwd_launch(const RouteParams& p, int elem, cudaStream_t s) {
   return route_launch(p, nullptr, nullptr, elem, s);
 }
 cudaError_t route_bwd_launch(const RouteParams& p, const float* dw, void* dlogits, int elem, cudaStream_t s) {
-  return dlogits == nullptr ? cudaErrorInvalidValue : route_launch(p, dw, dlogits, elem, s);
+  return p.N > 0 && dlogits == nullptr ? cudaErrorInvalidValue : route_launch(p, dw, dlogits, elem, s);
 }
 
 }  // namespace tgo
