@@ -148,3 +148,25 @@ def test_routing_of_no_tokens(device, score):
     w, idx = Rt.route_experts(logits, 2, score=score)
     w.sum().backward()
     assert w.shape == idx.shape == (0, 2) and logits.grad.shape == (0, 8)
+
+
+no_tokens = pytest.mark.parametrize("B,T", [(2, 0), (0, 5)])
+
+
+@both_devices
+@no_tokens
+@pytest.mark.parametrize("parts", ["all", "no modulation", "no h"])
+def test_sandwich_norm_of_no_tokens(device, B, T, parts):
+    """Empty results, gradients of 0 for the rows of a sample and for the weights."""
+    x, y = (torch.zeros(B, T, 64, device=device, requires_grad=True) for _ in range(2))
+    post_w, w = (torch.ones(64, device=device, requires_grad=True) for _ in range(2))
+    mods = [torch.ones(B, 64, device=device, requires_grad=True) for _ in range(3)]
+    if parts == "all":
+        outs = Fz.sandwich_norm(x, y, mods[0], post_w, w, *mods[1:])
+    elif parts == "no modulation":
+        outs = Fz.sandwich_norm(x, y, None, post_w, w)
+    else:
+        outs = Fz.sandwich_norm(x, y, mods[0], post_w)[:1]
+    torch.autograd.backward(outs, [torch.ones_like(o) for o in outs])
+    assert all(o.shape == (B, T, 64) for o in outs) and x.grad.shape == y.grad.shape == x.shape
+    assert all(t.grad is None or (t.grad == 0).all() for t in (post_w, w, *mods))

@@ -296,7 +296,7 @@ std::vector<at::Tensor> sandwich_bwd(OptT dx_new, OptT dh, at::Tensor x, at::Ten
   const c10::cuda::CUDAGuard guard(x.device());
   p.rstd_y = acc_f32(ry, p.M, x, "sandwich_bwd: ry");
   p.rstd_x = acc_f32(rx, p.M, x, "sandwich_bwd: rx");
-  TORCH_CHECK((p.rstd_y != nullptr || p.post_w == nullptr) && (p.rstd_x != nullptr || p.w == nullptr),
+  TORCH_CHECK(p.M == 0 || ((p.rstd_y != nullptr || p.post_w == nullptr) && (p.rstd_x != nullptr || p.w == nullptr)),
               "sandwich_bwd: the forward's statistics");
   SandwichBwdParams q{};
   auto grad_in = [&](const OptT& t, const char* what) -> const void* {
