@@ -170,3 +170,25 @@ def test_sandwich_norm_of_no_tokens(device, B, T, parts):
     torch.autograd.backward(outs, [torch.ones_like(o) for o in outs])
     assert all(o.shape == (B, T, 64) for o in outs) and x.grad.shape == y.grad.shape == x.shape
     assert all(t.grad is None or (t.grad == 0).all() for t in (post_w, w, *mods))
+
+
+@both_devices
+@no_tokens
+def test_rope_axes_of_no_tokens(device, B, T):
+    q, k = (torch.zeros(B, T, h, 64, device=device, requires_grad=True) for h in (4, 1))
+    w = torch.ones(64, device=device, requires_grad=True)
+    outs = Fz.rope_axes(q, k, torch.zeros(B, T, 1, device=device, dtype=torch.int32), (64,), q_w=w, k_w=w)
+    torch.autograd.backward(outs, [torch.ones_like(o) for o in outs])
+    assert outs[0].shape == q.grad.shape == q.shape and (w.grad == 0).all()
+
+
+@both_devices
+@no_tokens
+def test_axes_attention_of_no_tokens(device, B, T):
+    qkv = torch.zeros(B, T, 6 * 64, device=device, dtype=torch.bfloat16 if device == "cuda" else torch.float32,
+                      requires_grad=True)
+    pos = torch.zeros(B, T, 1, device=device, dtype=torch.int32)
+    w = torch.ones(64, device=device, requires_grad=True)
+    o = Fz.axes_attention_core(qkv, pos, (64,), 4, 1, 64, q_w=w, k_w=w)
+    o.backward(torch.ones_like(o))
+    assert o.shape == (B, T, 256) and qkv.grad.shape == qkv.shape and (w.grad is None or (w.grad == 0).all())

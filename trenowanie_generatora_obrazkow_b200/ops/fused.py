@@ -590,6 +590,8 @@ def axes_attention_core(qkv, pos, axes, heads, kv_heads, head_dim, theta=10000.0
         return R.attention(q, k, v, kv_len, scale).reshape(B, T, heads * head_dim)
     if tuple(pos.shape) != (B, T, len(axes)) or sum(axes) > head_dim:
         raise ValueError(f"axes_attention_core: pos {(B, T, len(axes))} and axes of at most {head_dim} channels")
+    if B * T == 0:  # the attention kernels take no empty tensors
+        return qkv[..., :heads * head_dim].contiguous()
     pos = (pos.float() if pos.is_floating_point() else pos.to(torch.int32)).contiguous().view(B * T, len(axes))
     return _AxesAttnFn.apply(qkv.contiguous(), pos, *_axes_table(axes, theta, qkv.device), q_w, k_w, kv_len, heads,
                              kv_heads, head_dim, float(scale), bool(interleaved), float(eps))
