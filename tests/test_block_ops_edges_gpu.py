@@ -423,3 +423,35 @@ def test_launch_counts_are_those_of_the_kernels():
             torch.cuda.synchronize()
         seen = sum(e.count for e in prof.key_averages() if "tgo::" in e.key)
         assert ext().launch_count() - n0 == seen, (i, ext().launch_count() - n0, seen)
+
+
+def test_operators_in_a_graph():
+    """Captured in a CUDA graph and replayed with other inputs in place: the results of plain calls."""
+    g = gen(51)
+    N, E, D = 300, 64, 256
+    make = lambda: dict(logits=rnd(g, N, E), x=rnd(g, N, D, dtype=BF16), a=rnd(g, 2, 150, D, dtype=BF16),
+                        b=rnd(g, 2, 150, D, dtype=BF16), gate=rnd(g, 2, D, dtype=BF16),
+                        pos=torch.randint(0, 90, (2, 150, 2), device="cuda", generator=g).int())
+    w, ones = rnd(g, D, std=0.1, mean=1.0), torch.ones(64, device="cuda")
+
+    def run(i):
+        r, idx = Rt.route_experts(i["logits"], 4, score="sigmoid", groups=8, top_groups=4)
+        plan = Rt.expert_plan(idx, E)
+        out = Rt.expert_combine(Rt.expert_dispatch(i["x"], plan), r, plan)
+        x, h = Fz.sandwich_norm(i["a"], i["b"], i["gate"], w, w)
+        q, k = Fz.rope_axes(h.unflatten(-1, (4, 64)), x.unflatten(-1, (4, 64)), i["pos"], (32, 32), q_w=ones, k_w=ones)
+        return r, idx, plan.slot, plan.offsets, out, x, h, q, k
+    state, other = make(), make()
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(state)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run(state)
+        for name, t in other.items():
+            state[name].copy_(t)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, run(other)))
