@@ -192,3 +192,17 @@ def test_axes_attention_of_no_tokens(device, B, T):
     o = Fz.axes_attention_core(qkv, pos, (64,), 4, 1, 64, q_w=w, k_w=w)
     o.backward(torch.ones_like(o))
     assert o.shape == (B, T, 256) and qkv.grad.shape == qkv.shape and (w.grad is None or (w.grad == 0).all())
+
+
+@pytest.mark.parametrize("name", ["w_in", "w_out", "router.weight"])
+def test_routed_mlp_trains_each_weight_alone(name):
+    """With every other weight frozen and an input without gradients, the one that is left gets the same gradient."""
+    torch.manual_seed(5)
+    mlp, h, up = RoutedMLP(16, 8, experts=4, top_k=2, capacity_factor=4.0), torch.randn(10, 16), torch.randn(10, 16)
+    mlp(h).backward(up)
+    want = dict(mlp.named_parameters())[name].grad
+    mlp.zero_grad(set_to_none=True)
+    for n, p in mlp.named_parameters():
+        p.requires_grad_(n == name)
+    mlp(h).backward(up)
+    assert want.norm() > 0 and torch.allclose(dict(mlp.named_parameters())[name].grad, want, atol=1e-6)

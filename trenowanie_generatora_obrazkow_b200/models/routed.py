@@ -87,7 +87,7 @@ class RoutedMLP(nn.Module):
         """h [..., dim]; valid (bool, h's shape without dim): padding tokens take no expert and get zeros."""
         x2 = h.reshape(-1, self.dim)
         w, idx = self.route(x2, None if valid is None else valid.reshape(-1))
-        training = torch.is_grad_enabled() and (x2.requires_grad or self.w_in.requires_grad)
+        training = torch.is_grad_enabled() and any(t.requires_grad for t in (x2, self.w_in, self.w_out))
         plan = Rt.expert_plan(idx, self.E, self.capacity(x2.shape[0]) if training else None)
         self.counts = plan.counts
         xs = Rt.expert_dispatch(x2, plan)
