@@ -12,8 +12,9 @@
 // combine   out[n] = sum_j w[n, j] y[slot[n, j]]                 backward  dy[slot[n, j]] = w[n, j] dout[n],
 //                                                                          dw[n, j] = <dout[n], y[slot[n, j]]>
 // All are bound by memory: the kernels walk tokens, not rows, so a token's row is read once for its k copies and a sum
-// over its k rows stays in registers (fp32, fixed order: no atomics). 32768 x 2048 bf16, 2 choices: dispatch 84 us, combine
-// 72 us, its backward 125 us (0.85, 0.86, 0.90 of a plain copy's rate); 8191 x 1280, 8 choices: 37, 45, 72 us.
+// over its k rows stays in registers (fp32, fixed order: no atomics). 32768 x 2048 bf16, 2 choices, with their launches:
+// dispatch 84 us, combine 72 us, its backward 125 us (0.85, 0.86, 0.90 of a plain copy's rate); 8191 x 1280, 8 choices: 37,
+// 45, 72 us. The plan: 9 us for 65536 assignments to 8 experts, 11 us to 64.
 #include <algorithm>
 
 #include "block_ops.h"

@@ -7,10 +7,9 @@
 // fraction of a revolution is kept, so positions of a long clip lose nothing that small ones have (|pos| < 2^24).
 // Backward: the transposed rotation, then the norm's gradient with x and its rstd recomputed from q / k:
 //     n = x r, gn = w g:   dx = r (gn - n mean(gn n)),   dw = sum over tokens and heads of g n.
-// Bound by memory with many heads per token (32768 tokens x 32 heads of 128 bf16: 101 / 161 us, 0.81 / 0.77 of a plain
-// copy's rate), by instruction issue with few (65536 x 12 heads of 64: 82 / 116 us): a token's angles are shared by its
+// Bound by memory with many heads per token (32768 tokens x 32 heads of 128 bf16: 99 / 157 us, 0.83 / 0.78 of a plain
+// copy's rate), by instruction issue with few (65536 x 12 heads of 64: 79 / 110 us): a token's angles are shared by its
 // heads alone.
-//
 #include <algorithm>
 #include <initializer_list>
 

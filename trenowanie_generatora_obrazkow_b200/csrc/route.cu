@@ -18,9 +18,9 @@
 // keys at the front (equal keys in index order), then each of the k steps takes the largest head of the L lanes; the
 // lowest lane that holds it wins (its experts have the lowest indices) and drops its head. What the weights need beyond
 // the choice is computed for the k chosen alone, from logits read again (they are in the cache).
-// 65536 x 256 fp32, k 8, 4 of 8 groups: forward 63 us, bound by instruction issue (80 %, about 780 per token: the exact
-// sigmoids and the group ranks 10 us each, the lists 20 us; without either 43 us), backward 29 us; 32768 x 8, 2 chosen: at
-// the launch's own time.
+// 65536 x 256 fp32, k 8, 4 of 8 groups: forward 60 us, bound by instruction issue (80 %, about 800 per token: the exact
+// sigmoids and the group ranks 10 us each, the lists 20 us; softmax without groups 43 us), 69 us with 2 % of the experts at
+// -inf (an overflowed exponential sends its reciprocal down the slow path); backward 26 us; 32768 x 8, 2 chosen: 3.6 / 3.2 us.
 #include <algorithm>
 #include <cfloat>
 
@@ -114,8 +114,8 @@ __device__ __forceinline__ bool far_down(float l) { return fabsf(l + 96.f) < FAR
 
 // A warp takes a batch of `steps` x 32 / L tokens: each step chooses for its tokens while the next step's logits are in
 // flight, and the end computes the weights of the whole batch's choices together, `slots` = the power of two from k on
-// lanes per token. One token per warp instead (its end in 8 of 32 lanes): 70 us against 63 us at 65536 x 256, k 8. A grid
-// of resident warps that walk the batches: 68 us, as the last round is not full.
+// lanes per token. At 65536 x 256, k 8, where this took 63 us with its launch, one token per warp (its end in 8 of 32 lanes)
+// took 70 us, and a grid of resident warps that walk the batches 68 us, as the last round is not full.
 template <typename T, int L, int EPL>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_fwd_blocks(EPL)) route_fwd_kernel(RouteParams p, int steps,
                                                                                        int slots) {

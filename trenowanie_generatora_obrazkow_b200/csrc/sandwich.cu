@@ -12,8 +12,8 @@
 //     mean(a g yn) = mean(a yn (dx' + rx dh cw)) - rx m mean(a yn n),    m = mean(dh cw n).
 // Statistics and sums are fp32; x' is rounded only when it is stored, so h comes from the unrounded sum.
 //
-// Bound by memory (4 rows forward, 6 backward): 32 x 1024 x 2048 bf16 takes 96 / 167 us, 0.85 / 0.74 of a plain copy's rate;
-// below it the row reductions' barriers and, backward, 128 registers (16 warps per SM) are what is left.
+// Bound by memory (4 rows forward, 6 backward): the kernels of 32 x 1024 x 2048 bf16 take 92 / 161 us, 0.89 / 0.76 of a plain
+// copy's rate; below it the row reductions' barriers and, backward, 128 registers (16 warps per SM) are what is left.
 //
 // Column sums: a unit (a CTA, or a group of its threads) owns a contiguous span of rows and writes one partial row (three
 // sums per channel) per sample it meets. Entry unit + sample is unique (along the spans both only grow), so
@@ -664,8 +664,9 @@ __global__ void __launch_bounds__(256) sandwich_weights_kernel(SandwichParams p,
 
 namespace {
 
-// Rows per step and group (16-bit and fp32 rows). 32 x 1024 x 2048 bf16: forward 1 / 2 / 4 rows 139 / 96 / 100 us, backward
-// 1 / 2 rows 181 / 175 us; fp32 32 x 1024 x 1024 backward 2 rows spill (165 us against 155 us).
+// Rows per step and group (16-bit and fp32 rows). 32 samples of 2048 bf16 channels, 1023 rows (one per step, as two do not
+// divide them) / 1024 rows (two per step): forward 96 / 92 us, backward 159 / 153 us; fp32 32 x 1024 x 1024 backward 2 rows
+// spill (165 us against 155 us with one).
 template <typename T>
 struct SwRows {
   static constexpr int FWD = 2, BWD = sizeof(T) == 2 ? 2 : 1;

@@ -366,7 +366,8 @@ def sandwich_norm(x, y, gate=None, post_w=None, w=None, shift=None, scale=None, 
     views are read in place); post_w, w [D] fp32. Every part but x and y may be left out: post_w None adds the branch
     without a norm, gate None without a gate, w None returns h = None, shift / scale come together and need w. Statistics
     and sums are fp32, each output is rounded once. The norm weights' gradients are accumulated in place into their
-    ``.grad`` like ``adanorm``'s."""
+    ``.grad`` like ``adanorm``'s (``torch.autograd.grad`` does not return them, tensor hooks on them do not run). On CUDA: at
+    most 16384 channels; x and y of any layout are copied to rows, gate, shift and scale need contiguous channels."""
     if x.dim() != 3 or y.shape != x.shape:
         raise ValueError(f"sandwich_norm: x and y [B, T, D], got {tuple(x.shape)} and {tuple(y.shape)}")
     if (shift is None) != (scale is None) or (scale is not None and w is None):
@@ -413,7 +414,9 @@ def rope_axes(q, k, pos, axes, theta=10000.0, q_w=None, k_w=None, interleaved=Tr
     [B, T, len(axes)] int32 or fp32 (fractions for interpolated grids; |pos| < 2^24). Axis a turns the axes[a] / 2 pairs
     of its share of the head by pos_a theta^(-2 m / axes[a]) (theta: one base or one per axis); channels past sum(axes)
     are only normalised. interleaved: pairs (2 i, 2 i + 1), else (i, i + sum(axes) / 2). axes=(d / 2, d / 2) with
-    (row, column) positions is the image model's 2-D RoPE. Returns contiguous q, k."""
+    (row, column) positions is the image model's 2-D RoPE. Returns contiguous q, k. Head dims up to 1024 on CUDA, where the
+    gradients of q_w and k_w are accumulated in place into their ``.grad`` (``torch.autograd.grad`` does not return them,
+    tensor hooks on them do not run)."""
     ent = _AXES_TABLES.get((tuple(axes), theta if isinstance(theta, (int, float)) else tuple(theta), q.device)) \
         if q.is_cuda else None
     if ent is None:
@@ -581,7 +584,8 @@ class _AxesAttnFn(torch.autograd.Function):
 def axes_attention_core(qkv, pos, axes, heads, kv_heads, head_dim, theta=10000.0, q_w=None, k_w=None, kv_len=None,
                         scale=None, interleaved=True, eps=R.EPS):
     """Self-attention with multi-axis rotary positions: qkv [B, T, (heads + 2 kv_heads) head_dim], pos [B, T, axes] (see
-    ``rope_axes``) -> [B, T, heads head_dim]; keys at positions >= kv_len[b] are masked. Head dims 64 and 128 on CUDA."""
+    ``rope_axes``) -> [B, T, heads head_dim]; keys at positions >= kv_len[b] are masked. Head dims 64 and 128 on CUDA, where
+    the gradients of q_w and k_w go to their ``.grad`` like ``rope_axes``'."""
     scale = head_dim ** -0.5 if scale is None else scale
     B, T, _ = qkv.shape
     if not qkv.is_cuda:

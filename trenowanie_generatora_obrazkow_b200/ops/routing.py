@@ -37,8 +37,9 @@ def route_experts(logits, k, score="softmax", bias=None, groups=1, top_groups=1,
     ``bias`` [E] fp32 (for balance: it moves the choice, not the weights), in descending order, ties to the lowest
     index. groups > 1: only the ``top_groups`` best of the ``groups`` equal runs of experts take part, a group's worth
     being its best expert (softmax) or the sum of its two best (sigmoid). renorm divides the weights by their sum
-    (+ 1e-20); ``scale`` (a normal fp32 number) multiplies them. valid [N] bool: False rows get w 0 and idx -1. NaN logits are chosen
-    last; the weights of their row are unspecified. The gradient reaches the logits through the weights (once)."""
+    (+ 1e-20); ``scale`` (a normal fp32 number) multiplies them. valid [N] bool: False rows get w 0 and idx -1. NaN logits
+    are chosen last and count as -inf for their group; the weights of their row are unspecified. The gradient reaches the
+    logits through the weights (once; forward-mode derivatives are refused)."""
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"route_experts: score is 'softmax' or 'sigmoid', not {score!r}")
     if logits.dim() != 2:
