@@ -47,8 +47,8 @@ def listed():
         dict(name="linear 2047x1000->777", op="linear", m=2047, k=1000, n=777, bias=False, dtype="bfloat16"),
         # the SwiGLU MLP of the 2048-wide model over one micro-batch, bf16 weights
         dict(name="mlp 32768x2048x5504", op="mlp", m=32768, k=2048, h=5504, dtype="bfloat16"),
-        # the MLP of the 576-wide test model over an odd number of tokens
-        dict(name="mlp 333x576x1536", op="mlp", m=333, k=576, h=1536, dtype="bfloat16"),
+        # the MLP of the 512-wide text encoder over an odd number of tokens
+        dict(name="mlp 333x512x1408", op="mlp", m=333, k=512, h=1408, dtype="bfloat16"),
         # the activation alone, its input kept in 8 bits
         dict(name="swiglu 32768x5504", op="swiglu", m=32768, h=5504, dtype="bfloat16"),
         # the text refiner's activation over one caption
