@@ -13,7 +13,7 @@ along the rows of x, Q'(x) with blocks along its columns. Five operators:
 * mlp     [a | b] = Q(x) Q(W1)^T rounded to x's type;  g = silu(a) b;  y = Q(g) Q(W2)^T;  the backward reads x, g, [a | b]
           in 8 bits: dg = Q(dy) Q'(W2) rounded;  [da | db] = dsilu of Q([a | b]);  dx = Q(dab) Q'(W1);
           dW1 = Q'(dab)^T Q'(x);  dW2 = Q'(dy)^T Q'(g)
-* swiglu  g = silu(a) b;  [da | db] from dg and Q([a | b])
+* swiglu  g = silu(a) b;  [da | db] from dg and Q(a), Q(b), whose blocks start at their own first columns
 """
 import math
 
@@ -193,7 +193,7 @@ def _plain(s):
         dg = (_q(dy) @ _qt(w2)).to(dt)
         dab = _silu_mul_grad(_q(ab), dg)
         return [y, (_q(dab) @ _qt(w1)).to(dt), (_qt(dab).t() @ _qt(x)).to(dt), (_qt(dy).t() @ _qt(g)).to(dt)]
-    return [_silu_mul(x).to(dt), _silu_mul_grad(_q(x), dy).to(dt)]
+    return [_silu_mul(x).to(dt), _silu_mul_grad(torch.cat([_q(v) for v in x.chunk(2, dim=1)], dim=1), dy).to(dt)]
 
 
 def _silu_mul(ab):
@@ -313,7 +313,8 @@ def exact(case, seed):
         return [y, _grid(dab, 1) @ _grid(w1, 0), _grid(dab, 0).t() @ _grid(x, 0), _grid(dy, 0).t() @ _grid(g, 0)]
     h = c["h"]
     x64 = x.double()
-    return [x64[:, :h] * torch.sigmoid(x64[:, :h]) * x64[:, h:], _dswiglu64(_grid(x, 1), dy.double())]
+    kept = torch.cat([_grid(x[:, :h], 1), _grid(x[:, h:], 1)], dim=1)
+    return [x64[:, :h] * torch.sigmoid(x64[:, :h]) * x64[:, h:], _dswiglu64(kept, dy.double())]
 
 
 def _dswiglu64(ab, dg):
