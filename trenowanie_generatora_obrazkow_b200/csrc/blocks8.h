@@ -1,0 +1,93 @@
+// Launch interfaces of the 8-bit block operators: packing into e4m3 with a power-of-two scale for each block of 128,
+// products of such operands, SwiGLU with its input kept in 8 bits. Plain CUDA types only; the torch-facing checks are in
+// blocks8_ops.cpp.
+//
+// The 8-bit form of X [R, K] (blocks along K): codes [R, Kp] e4m3, Kp = K rounded up to 128, zeros past K, and one byte
+// e + 127 per block (its scale is 2^e) in atoms of 512 bytes [ceil(R / 128)][ceil(Kp / 512)][32][4][4]: row 128 i + 32 c + r,
+// block 4 j + b stands at [i][j][r][c][b]. This is the order in which the tensor core takes scale factors (32 lanes of
+// four columns of four bytes), so an atom goes to tensor memory with one copy. Bytes of rows past R and blocks past Kp
+// are 0.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace tgo {
+
+struct Pack8Params {
+  const void* x;        // [M, K] of the element type, rows ld elements apart
+  long long ld;
+  int M, K;
+  uint8_t* codes;       // [M, Kp] blocks along K, or null
+  uint8_t* scales;
+  uint8_t* codes_t;     // [K, Mp] blocks along M (of x^T), or null
+  uint8_t* scales_t;
+  float* sums;          // [ceil(M / 128)][K] sums over the rows of each tile, or null (with codes_t)
+};
+cudaError_t pack8_launch(const Pack8Params& p, int elem, cudaStream_t s);
+// out[k] (+)= sum of tiles' rows of sums [T][K], in order
+cudaError_t colsum_launch(const float* sums, int T, int K, float* out, bool add, cudaStream_t s);
+// codes [R, Kp] -> out [R, K] rows ldo apart
+cudaError_t unpack8_launch(const uint8_t* codes, const uint8_t* scales, int R, int K, void* out, long long ldo, int elem,
+                           cudaStream_t s);
+
+enum Gemm8Out : int { OUT_BF16 = 0, OUT_F16 = 1, OUT_F32 = 2 };  // as ElemType
+struct Gemm8Params {
+  int M, N, kb;             // kb: blocks of 128 along the contraction
+  const uint8_t* sfa;       // scale bytes of A and B
+  const uint8_t* sfb;
+  void* C;                  // [M, N], rows ldc elements apart
+  long long ldc;
+  const float* bias;        // [N] or null
+  int add;                  // C += (fp32 C only)
+  int chunk_kb;             // contraction blocks per accumulator (a multiple of 4); further ones join in fp32 in order
+  int c_tma;                // C goes through its tensor map
+  int* err;
+};
+constexpr int kGemm8Tile = 128;  // rows of A's box
+// ta / tb: uint8 maps {Kp, rows, 1} with boxes {128, 128 or bn, 1}, 128-byte swizzle; tc: {N, M, 1}, box {32, 32, 1}
+cudaError_t gemm8_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Gemm8Params& p, int bn,
+                         int out, cudaStream_t s);
+
+// y [M, N] = Q(x) W^T + bias for few rows, x packed on the way (one launch)
+constexpr int kFewRows = 16;
+struct FewRowsParams {
+  const void* x;            // [M, K], rows ldx apart
+  long long ldx;
+  const uint8_t* codes;     // W [N, Kp]
+  const uint8_t* scales;
+  const float* bias;        // [N] or null
+  void* y;                  // [M, N] contiguous, in x's type
+  int M, N, K;
+};
+cudaError_t few_rows_launch(const FewRowsParams& p, int elem, cudaStream_t s);
+
+// SwiGLU over ab [M, 2 H] (rows ld apart), H a multiple of 128 unless only g and the checkpoint are wanted
+struct Swiglu8Params {
+  const void* ab;
+  long long ld;
+  int M, H;
+  void* g;                  // [M, H] in ab's type, or null
+  uint8_t* ck;              // ab in 8 bits, [M, 2 Hp]: a's and b's blocks each from their own first column, or null
+  uint8_t* ck_scales;       // of [M, 2 Hp]
+  uint8_t* g8;              // g in 8 bits [M, Hp], or null
+  uint8_t* g8_scales;
+  uint8_t* g8t;             // [H, Mp] blocks along M, or null
+  uint8_t* g8t_scales;
+};
+cudaError_t swiglu8_fwd_launch(const Swiglu8Params& p, int elem, cudaStream_t s);
+struct Swiglu8BwdParams {
+  const void* dg;           // [M, H], rows ld apart
+  long long ld;
+  const uint8_t* ck;        // as the forward wrote it
+  const uint8_t* ck_scales;
+  int M, H;
+  void* dab;                // [M, 2 H] in dg's type, or null
+  uint8_t* d8;              // dab in 8 bits [M, 2 H] (H a multiple of 128), or null
+  uint8_t* d8_scales;
+  uint8_t* d8t;             // [2 H, Mp]
+  uint8_t* d8t_scales;
+};
+cudaError_t swiglu8_bwd_launch(const Swiglu8BwdParams& p, int elem, cudaStream_t s);
+
+}  // namespace tgo

@@ -1,0 +1,546 @@
+// Torch-facing wrappers of the 8-bit block operators (blocks8.h): argument checks, outputs, tensor maps, launches on the
+// current stream, autograd nodes. Registered in the extension module by ops.cpp.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cudaTypedefs.h>
+#include <torch/extension.h>
+
+#include "blocks8.h"
+#include "torch_util.h"
+
+namespace tgo {
+
+PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder();  // ops.cpp
+int num_sms();                                     // gemm.cu
+
+namespace {
+
+const char* const kWhat = "8-bit block operators";
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
+
+// A packed matrix: codes [rows, 128 ceil(cols / 128)] e4m3, scale bytes (blocks8.h)
+struct Packed {
+  at::Tensor codes, scales;
+  int64_t rows = 0, cols = 0;
+  int64_t blocks() const { return up(cols, 128); }
+  bool there() const { return codes.defined(); }
+  uint8_t* c() const { return codes.defined() ? static_cast<uint8_t*>(codes.data_ptr()) : nullptr; }
+  uint8_t* s() const { return scales.defined() ? scales.data_ptr<uint8_t>() : nullptr; }
+};
+
+Packed fresh_packed(int64_t rows, int64_t cols, const at::Tensor& as) {
+  Packed p;
+  p.rows = rows;
+  p.cols = cols;
+  p.codes = fresh({rows, p.blocks() * 128}, at::kFloat8_e4m3fn, as);
+  p.scales = fresh({up(rows, 128), up(p.blocks(), 4), 32, 4, 4}, at::kByte, as);
+  return p;
+}
+Packed given_packed(const at::Tensor& codes, const at::Tensor& scales, int64_t cols, const char* what) {
+  Packed p;
+  p.codes = codes;
+  p.scales = scales;
+  p.cols = cols;
+  TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kFloat8_e4m3fn && codes.dim() == 2 && codes.is_contiguous() &&
+                  cols >= 0 && cols < (1ll << 31) - 128 && codes.size(1) == p.blocks() * 128,
+              what, ": codes e4m3 [rows, 128 ceil(", cols, " / 128)], contiguous, expected");
+  p.rows = codes.size(0);
+  same_device(scales, codes, what);
+  TORCH_CHECK(scales.scalar_type() == at::kByte && scales.is_contiguous() && p.rows < (1ll << 31) - 128 &&
+                  scales.sizes() == at::IntArrayRef({up(p.rows, 128), up(p.blocks(), 4), 32, 4, 4}),
+              what, ": scales uint8 [", up(p.rows, 128), ", ", up(p.blocks(), 4), ", 32, 4, 4], contiguous, expected");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0, what, ": 16-byte aligned codes and scales");
+  return p;
+}
+
+// [M, K] with a row's elements side by side and rows that do not overlap; other layouts are copied
+at::Tensor rows_of(const at::Tensor& t) {
+  return whole_rows(t) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) ? t : t.contiguous();
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+void check_matrix(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2, what, ": a CUDA matrix expected");
+  TORCH_CHECK(t.size(1) >= 1 && t.size(1) < (1ll << 31) - 128 && t.size(0) < (1ll << 31) - 128, what,
+              ": at least one column and fewer than 2^31 - 128 rows and columns");
+}
+
+// packs x [M, K] (rows_of): blocks along the rows (r), along the columns as the rows of x^T (c), column sums (sums [K] fp32)
+void pack(const at::Tensor& x, Packed* r, Packed* c, float* sums, bool add, const char* what) {
+  check_matrix(x, what);
+  const int64_t M = x.size(0), K = x.size(1);
+  const int elem = elem_of(x, what);
+  if (r != nullptr) *r = fresh_packed(M, K, x);
+  if (c != nullptr) *c = fresh_packed(K, M, x);
+  const cudaStream_t s = at::cuda::getCurrentCUDAStream();
+  if (M == 0) {
+    if (sums != nullptr && !add) TORCH_CHECK(cudaMemsetAsync(sums, 0, K * sizeof(float), s) == cudaSuccess, what);
+    return;
+  }
+  Pack8Params p{};
+  p.x = x.data_ptr();
+  p.ld = row_stride(x);
+  p.M = (int)M;
+  p.K = (int)K;
+  if (r != nullptr) p.codes = r->c(), p.scales = r->s();
+  if (c != nullptr) p.codes_t = c->c(), p.scales_t = c->s();
+  at::Tensor part;
+  if (sums != nullptr) {
+    part = fresh({up(M, 128), K}, at::kFloat, x);
+    p.sums = part.data_ptr<float>();
+  }
+  BLOCK_LAUNCH(pack8_launch(p, elem, s), 1);
+  if (sums != nullptr) BLOCK_LAUNCH(colsum_launch(p.sums, (int)up(M, 128), (int)K, sums, add, s), 1);
+}
+
+CUtensorMap codes_map(const Packed& a, uint32_t box_rows) {
+  CUtensorMap m;
+  const uint64_t width = a.blocks() * 128;
+  cuuint64_t dims[3] = {width, (cuuint64_t)a.rows, 1};
+  cuuint64_t strides[2] = {width, width * (cuuint64_t)a.rows};
+  cuuint32_t box[3] = {128, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = tmap_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.c(), dims, strides, box, estr,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "tensor map of 8-bit codes: code ", (int)r);
+  return m;
+}
+// C [M, N] with rows ldc apart; false where a map cannot address it (the kernel then stores rows itself): base and rows off
+// 16 bytes, or rows that end inside 16 bytes, which a store fills up past the row's end
+bool out_map(CUtensorMap* m, const at::Tensor& C, int64_t ldc) {
+  const uint64_t es = C.element_size();
+  if (reinterpret_cast<uintptr_t>(C.data_ptr()) % 16 != 0 || (ldc * es) % 16 != 0 ||
+      (C.size(1) * es) % 16 != 0) return false;
+  const bool f32 = C.scalar_type() == at::kFloat;
+  cuuint64_t dims[3] = {(cuuint64_t)C.size(1), (cuuint64_t)C.size(0), 1};
+  cuuint64_t strides[2] = {ldc * es, ldc * es * (cuuint64_t)C.size(0)};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const auto type = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : C.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return tmap_encoder()(m, type, 3, C.data_ptr(), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// C [M, N] (+)= a b^T (+ bias)
+void product(const Packed& a, const Packed& b, const at::Tensor& C, const float* bias, bool add, int* err) {
+  TORCH_CHECK(a.cols == b.cols, "gemm_blocks: sums over ", a.cols, " and ", b.cols);
+  if (a.rows == 0 || b.rows == 0) return;
+  if (a.cols == 0) {  // a sum of nothing
+    if (!add) C.zero_();
+    TORCH_CHECK(bias == nullptr, "gemm_blocks: a bias of a sum of nothing");
+    return;
+  }
+  Gemm8Params p{};
+  p.M = (int)a.rows;
+  p.N = (int)b.rows;
+  p.kb = (int)a.blocks();
+  p.sfa = a.s();
+  p.sfb = b.s();
+  p.C = C.data_ptr();
+  p.ldc = row_stride(C);
+  p.bias = bias;
+  p.add = add;
+  p.err = err;
+  const int out = elem_of(C, "gemm_blocks");
+  // The tensor core's fp32 sums drop what does not fit their 24 bits instead of rounding: a sum of one sign over 32768
+  // lost 3.6e-5 of itself, 1.3e-6 over 4096. Sums that are returned in fp32 are joined from parts of 4096.
+  p.chunk_kb = out == OUT_F32 ? 32 : (int)up(p.kb, 4) * 4;
+  CUtensorMap tc;
+  p.c_tma = out_map(&tc, C, p.ldc);
+  // 128 x 256 tiles where they fill the GPU, else twice as many of 128 x 128
+  const int bn = up(p.M, 128) * up(p.N, 256) >= num_sms() ? 256 : 128;
+  const CUtensorMap ta = codes_map(a, kGemm8Tile), tb = codes_map(b, bn);
+  if (!p.c_tma) tc = ta;
+  BLOCK_LAUNCH(gemm8_launch(ta, tb, tc, p, bn, out, at::cuda::getCurrentCUDAStream()), 1);
+}
+
+void small_vector(const OptT& bias, int64_t n, const at::Tensor& as, const char* what) {
+  if (!given(bias)) return;
+  same_device(*bias, as, what);
+  TORCH_CHECK(bias->is_floating_point() && bias->dim() == 1 && bias->size(0) == n, what, ": bias [", n, "] expected");
+}
+// the bias in fp32 (a copy where it is not)
+at::Tensor bias_f32(const OptT& bias) { return given(bias) ? bias->detach().to(at::kFloat).contiguous() : at::Tensor(); }
+const float* ptr_f32(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+// ------------------------------------------------------------------------------------------------ packing, products
+std::vector<at::Tensor> pack8(at::Tensor x, bool rows, bool cols) {
+  TORCH_CHECK(rows || cols, "quantize_blocks: a side");
+  check_matrix(x, "quantize_blocks");
+  const c10::cuda::CUDAGuard guard(x.device());
+  x = rows_of(x.detach());
+  Packed r, c;
+  pack(x, rows ? &r : nullptr, cols ? &c : nullptr, nullptr, false, "quantize_blocks");
+  std::vector<at::Tensor> out;
+  if (rows) out.insert(out.end(), {r.codes, r.scales});
+  if (cols) out.insert(out.end(), {c.codes, c.scales});
+  return out;
+}
+
+at::Tensor unpack8(at::Tensor codes, at::Tensor scales, int64_t cols, at::ScalarType type) {
+  const Packed p = given_packed(codes, scales, cols, "dequantize_blocks");
+  const c10::cuda::CUDAGuard guard(codes.device());
+  at::Tensor out = fresh({p.rows, cols}, type, codes);
+  const int elem = elem_of(out, "dequantize_blocks");
+  if (out.numel() > 0)
+    BLOCK_LAUNCH(unpack8_launch(p.c(), p.s(), (int)p.rows, (int)cols, out.data_ptr(), cols, elem,
+                                at::cuda::getCurrentCUDAStream()), 1);
+  return out;
+}
+
+at::Tensor gemm8(at::Tensor a, at::Tensor as, at::Tensor b, at::Tensor bs, int64_t cols, at::ScalarType type, OptT out,
+                 OptT bias, bool add, at::Tensor err) {
+  const Packed p = given_packed(a, as, cols, "gemm_blocks: a"), q = given_packed(b, bs, cols, "gemm_blocks: b");
+  same_device(b, a, "gemm_blocks: b");
+  const c10::cuda::CUDAGuard guard(a.device());
+  small_vector(bias, q.rows, a, "gemm_blocks");
+  at::Tensor C = given(out) ? *out : fresh({p.rows, q.rows}, type, a);
+  same_device(C, a, "gemm_blocks: out");
+  TORCH_CHECK(C.dim() == 2 && C.size(0) == p.rows && C.size(1) == q.rows && whole_rows(C) &&
+                  (C.size(0) <= 1 || C.stride(0) >= C.size(1)), "gemm_blocks: out [", p.rows, ", ", q.rows,
+              "] with contiguous rows expected");
+  TORCH_CHECK(!(C.requires_grad() && at::GradMode::is_enabled()), "gemm_blocks: out must not require a gradient");
+  TORCH_CHECK(!add || (given(out) && C.scalar_type() == at::kFloat && !given(bias)),
+              "gemm_blocks: adding takes an fp32 out and no bias");
+  const at::Tensor b32 = bias_f32(bias);
+  product(p, q, C, ptr_f32(b32), add, err_word(err, a));
+  return C;
+}
+
+// ----------------------------------------------------------------------------------------------------------- linear
+// Q(x) W^T + bias with W held in 8 bits; no gradient
+at::Tensor linear8_frozen(at::Tensor x, at::Tensor codes, at::Tensor scales, int64_t cols, OptT bias, at::Tensor err) {
+  const Packed w = given_packed(codes, scales, cols, "linear_blocks: weight");
+  same_device(codes, x, "linear_blocks: weight");
+  check_matrix(x, "linear_blocks");
+  TORCH_CHECK(x.size(1) == cols, "linear_blocks: x [..., ", cols, "] expected, got ", x.size(1), " columns");
+  const bool graph = wants_grad({&x}, kWhat) || (given(bias) && wants_grad({&*bias}, kWhat));
+  TORCH_CHECK(!graph, "linear_blocks: a weight held in 8 bits passes no gradient on (use torch.no_grad() or detach x)");
+  const c10::cuda::CUDAGuard guard(x.device());
+  small_vector(bias, w.rows, x, "linear_blocks");
+  x = rows_of(x);
+  const at::Tensor b32 = bias_f32(bias);
+  at::Tensor y = fresh({x.size(0), w.rows}, x.scalar_type(), x);
+  if (y.numel() == 0) return y;
+  if (x.size(0) <= kFewRows) {
+    FewRowsParams p{};
+    p.x = x.data_ptr();
+    p.ldx = row_stride(x);
+    p.codes = w.c();
+    p.scales = w.s();
+    p.bias = ptr_f32(b32);
+    p.y = y.data_ptr();
+    p.M = (int)x.size(0);
+    p.N = (int)w.rows;
+    p.K = (int)cols;
+    BLOCK_LAUNCH(few_rows_launch(p, elem_of(x, "linear_blocks"), at::cuda::getCurrentCUDAStream()), 1);
+    return y;
+  }
+  Packed q;
+  pack(x, &q, nullptr, nullptr, false, "linear_blocks");
+  product(q, w, y, ptr_f32(b32), false, err_word(err, x));
+  return y;
+}
+
+// The operands of a backward product are packed along the axis that it sums over: x^T and W^T are written while the
+// forward packs x and W. x itself is not kept: its checkpoint is the operand of the weight's gradient.
+void keep(variable_list* saved, const Packed& p) {
+  saved->push_back(p.codes);
+  saved->push_back(p.scales);
+}
+Packed kept(const variable_list& saved, size_t at, int64_t cols) {
+  Packed p;
+  p.codes = saved[at];
+  p.scales = saved[at + 1];
+  p.rows = p.codes.defined() ? p.codes.size(0) : 0;
+  p.cols = cols;
+  return p;
+}
+// a product that sums over no rows at all
+bool zero_sum(const WeightGrad& g, int64_t rows) {
+  if (rows > 0) return false;
+  if (!g.add) g.g.zero_();
+  return true;
+}
+// the weight's gradient where autograd or the leaf wants it
+at::Tensor weight_grad(const WeightGrad& g, const Packed& dy, const Packed& x, int64_t rows, int* err) {
+  if (!g.g.defined()) return at::Tensor();
+  if (!zero_sum(g, rows)) product(dy, x, g.g, nullptr, g.add, err);
+  return g.put();
+}
+void notify(std::initializer_list<const WeightGrad*> gs) {
+  if (!grad_ready().on) return;
+  py::gil_scoped_acquire gil;
+  for (const WeightGrad* g : gs)
+    if (g->direct) grad_ready().notify(g->w);
+}
+
+struct Linear8Fn : public torch::autograd::Function<Linear8Fn> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor w, OptT bias, at::Tensor err) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const bool dx = x.requires_grad(), dw = w.requires_grad();
+    Packed xr, xt, wr, wt;
+    pack(x, &xr, dw ? &xt : nullptr, nullptr, false, "linear_blocks");
+    pack(w, &wr, dx ? &wt : nullptr, nullptr, false, "linear_blocks: weight");
+    at::Tensor y = fresh({x.size(0), w.size(0)}, x.scalar_type(), x);
+    const at::Tensor b32 = bias_f32(bias);
+    product(xr, wr, y, ptr_f32(b32), false, err_word(err, x));
+    variable_list saved;
+    keep(&saved, xt);
+    keep(&saved, wt);
+    ctx->save_for_backward(saved);
+    ctx->saved_data["w"] = w;
+    if (given(bias)) ctx->saved_data["bias"] = *bias;
+    ctx->saved_data["err"] = err;
+    ctx->saved_data["dx"] = dx;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only(kWhat);
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor dy = rows_of(grads[0]);
+    const c10::cuda::CUDAGuard guard(dy.device());
+    const int64_t M = dy.size(0), N = dy.size(1);
+    const bool dx = ctx->saved_data["dx"].toBool();
+    const at::Tensor err = ctx->saved_data["err"].toTensor();
+    int* const e = err_word(err, dy);
+    const Packed xt = kept(saved, 0, M), wt = kept(saved, 2, N);
+    const WeightGrad gw(ctx, "w"), gb(ctx, "bias");
+    Packed r, c;
+    // the bias' sums are fp32 wherever they go
+    at::Tensor sums = gb.g.defined() ? (gb.g.scalar_type() == at::kFloat ? gb.g : fresh({N}, at::kFloat, dy)) : at::Tensor();
+    const bool cols = gw.g.defined() || sums.defined();
+    if (dx || cols)
+      pack(dy, dx ? &r : nullptr, cols ? &c : nullptr, sums.defined() ? sums.data_ptr<float>() : nullptr, gb.add,
+           "linear_blocks: gradient");
+    variable_list out(4);
+    if (dx) {
+      out[0] = fresh({M, wt.rows}, dy.scalar_type(), dy);
+      product(r, wt, out[0], nullptr, false, e);
+    }
+    out[1] = weight_grad(gw, c, xt, M, e);
+    if (sums.defined()) {
+      if (gb.g.scalar_type() != at::kFloat) gb.g.copy_(sums);
+      out[2] = gb.put();
+    }
+    notify({&gw, &gb});
+    return out;
+  }
+};
+
+at::Tensor linear8(at::Tensor x, at::Tensor w, OptT bias, at::Tensor err) {
+  check_matrix(x, "linear_blocks");
+  check_matrix(w, "linear_blocks: weight");
+  same_device(w, x, "linear_blocks: weight");
+  TORCH_CHECK(x.size(1) == w.size(1) && w.size(0) >= 1, "linear_blocks: x [..., K] and weight [N, K] expected, got ",
+              x.sizes(), " and ", w.sizes());
+  elem_of(x, "linear_blocks");
+  elem_of(w, "linear_blocks: weight");
+  const c10::cuda::CUDAGuard guard(x.device());
+  small_vector(bias, w.size(0), x, "linear_blocks");
+  x = rows_of(x);
+  const at::Tensor b = or_undefined(bias);
+  if (wants_grad({&x, &w, &b}, kWhat)) {
+    if (!whole_rows(w)) w = w.contiguous();
+    return Linear8Fn::apply(x, w, bias, err);
+  }
+  w = rows_of(w);
+  Packed xr, wr;
+  pack(x, &xr, nullptr, nullptr, false, "linear_blocks");
+  pack(w, &wr, nullptr, nullptr, false, "linear_blocks: weight");
+  at::Tensor y = fresh({x.size(0), w.size(0)}, x.scalar_type(), x);
+  const at::Tensor b32 = bias_f32(bias);
+  product(xr, wr, y, ptr_f32(b32), false, err_word(err, x));
+  return y;
+}
+
+// ----------------------------------------------------------------------------------------------------------- SwiGLU
+void swiglu_forward(const at::Tensor& ab, at::Tensor* g, Packed* ck, Packed* g8, Packed* g8t) {
+  const int64_t M = ab.size(0), H = ab.size(1) / 2, Hp = up(H, 128) * 128;
+  if (g != nullptr) *g = fresh({M, H}, ab.scalar_type(), ab);
+  if (ck != nullptr) *ck = fresh_packed(M, 2 * Hp, ab);
+  if (g8 != nullptr) *g8 = fresh_packed(M, H, ab);
+  if (g8t != nullptr) *g8t = fresh_packed(H, M, ab);
+  if (M == 0) return;
+  Swiglu8Params p{};
+  p.ab = ab.data_ptr();
+  p.ld = row_stride(ab);
+  p.M = (int)M;
+  p.H = (int)H;
+  if (g != nullptr) p.g = g->data_ptr();
+  if (ck != nullptr) p.ck = ck->c(), p.ck_scales = ck->s();
+  if (g8 != nullptr) p.g8 = g8->c(), p.g8_scales = g8->s();
+  if (g8t != nullptr) p.g8t = g8t->c(), p.g8t_scales = g8t->s();
+  BLOCK_LAUNCH(swiglu8_fwd_launch(p, elem_of(ab, "swiglu_blocks"), at::cuda::getCurrentCUDAStream()), 1);
+}
+void swiglu_backward(const at::Tensor& dg, const Packed& ck, int64_t H, at::Tensor* dab, Packed* d8, Packed* d8t) {
+  const int64_t M = dg.size(0);
+  if (dab != nullptr) *dab = fresh({M, 2 * H}, dg.scalar_type(), dg);
+  if (d8 != nullptr) *d8 = fresh_packed(M, 2 * H, dg);
+  if (d8t != nullptr) *d8t = fresh_packed(2 * H, M, dg);
+  if (M == 0) return;
+  Swiglu8BwdParams p{};
+  p.dg = dg.data_ptr();
+  p.ld = row_stride(dg);
+  p.ck = ck.c();
+  p.ck_scales = ck.s();
+  p.M = (int)M;
+  p.H = (int)H;
+  if (dab != nullptr) p.dab = dab->data_ptr();
+  if (d8 != nullptr) p.d8 = d8->c(), p.d8_scales = d8->s();
+  if (d8t != nullptr) p.d8t = d8t->c(), p.d8t_scales = d8t->s();
+  BLOCK_LAUNCH(swiglu8_bwd_launch(p, elem_of(dg, "swiglu_blocks"), at::cuda::getCurrentCUDAStream()), 1);
+}
+
+struct Swiglu8Fn : public torch::autograd::Function<Swiglu8Fn> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor ab) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    at::Tensor g;
+    Packed ck;
+    swiglu_forward(ab, &g, &ck, nullptr, nullptr);
+    ctx->save_for_backward({ck.codes, ck.scales});
+    return g;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only(kWhat);
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor dg = rows_of(grads[0]);
+    const c10::cuda::CUDAGuard guard(dg.device());
+    at::Tensor dab;
+    swiglu_backward(dg, kept(saved, 0, saved[0].size(1)), dg.size(1), &dab, nullptr, nullptr);
+    return {dab};
+  }
+};
+at::Tensor swiglu8(at::Tensor ab) {
+  check_matrix(ab, "swiglu_blocks");
+  TORCH_CHECK(ab.size(1) % 2 == 0 && ab.size(1) < (1ll << 31) - 512, "swiglu_blocks: an even number of columns");
+  elem_of(ab, "swiglu_blocks");
+  const c10::cuda::CUDAGuard guard(ab.device());
+  ab = rows_of(ab);
+  if (wants_grad({&ab}, kWhat)) return Swiglu8Fn::apply(ab);
+  at::Tensor g;
+  swiglu_forward(ab, &g, nullptr, nullptr, nullptr);
+  return g;
+}
+
+// -------------------------------------------------------------------------------------------------------------- MLP
+struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor w1, at::Tensor w2, at::Tensor err) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const bool dx = x.requires_grad(), dw1 = w1.requires_grad(), dw2 = w2.requires_grad(), up_too = dx || dw1;
+    Packed xr, xt, w1r, w1t, w2r, w2t, ck, g8, g8t;
+    pack(x, &xr, dw1 ? &xt : nullptr, nullptr, false, "mlp_blocks");
+    pack(w1, &w1r, dx ? &w1t : nullptr, nullptr, false, "mlp_blocks: in_proj");
+    pack(w2, &w2r, up_too ? &w2t : nullptr, nullptr, false, "mlp_blocks: out_proj");
+    int* const e = err_word(err, x);
+    {
+      at::Tensor ab = fresh({x.size(0), w1.size(0)}, x.scalar_type(), x);
+      product(xr, w1r, ab, nullptr, false, e);
+      swiglu_forward(ab, nullptr, up_too ? &ck : nullptr, &g8, dw2 ? &g8t : nullptr);
+    }
+    at::Tensor y = fresh({x.size(0), w2.size(0)}, x.scalar_type(), x);
+    product(g8, w2r, y, nullptr, false, e);
+    variable_list saved;
+    keep(&saved, xt);
+    keep(&saved, w1t);
+    keep(&saved, w2t);
+    keep(&saved, ck);
+    keep(&saved, g8t);
+    ctx->save_for_backward(saved);
+    ctx->saved_data["w1"] = w1;
+    ctx->saved_data["w2"] = w2;
+    ctx->saved_data["err"] = err;
+    ctx->saved_data["dx"] = dx;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only(kWhat);
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor dy = rows_of(grads[0]);
+    const c10::cuda::CUDAGuard guard(dy.device());
+    const int64_t M = dy.size(0), N = dy.size(1);
+    const bool dx = ctx->saved_data["dx"].toBool();
+    const at::Tensor err = ctx->saved_data["err"].toTensor();
+    int* const e = err_word(err, dy);
+    const WeightGrad g1(ctx, "w1"), g2(ctx, "w2");
+    const bool up_too = dx || g1.g.defined();
+    const Packed w2t = kept(saved, 4, N);
+    const int64_t H = ctx->saved_data["w2"].toTensor().size(1);
+    variable_list out(4);
+    Packed dyr, dyt;
+    if (up_too || g2.g.defined())
+      pack(dy, up_too ? &dyr : nullptr, g2.g.defined() ? &dyt : nullptr, nullptr, false, "mlp_blocks: gradient");
+    out[2] = weight_grad(g2, dyt, kept(saved, 8, M), M, e);
+    if (up_too) {
+      Packed d8, d8t;
+      {
+        at::Tensor dg = fresh({M, H}, dy.scalar_type(), dy);
+        product(dyr, w2t, dg, nullptr, false, e);
+        swiglu_backward(dg, kept(saved, 6, 2 * H), H, nullptr, &d8, &d8t);
+      }
+      if (dx) {
+        const Packed w1t = kept(saved, 2, 2 * H);
+        out[0] = fresh({M, w1t.rows}, dy.scalar_type(), dy);
+        product(d8, w1t, out[0], nullptr, false, e);
+      }
+      out[1] = weight_grad(g1, d8t, kept(saved, 0, M), M, e);
+    }
+    notify({&g2, &g1});
+    return out;
+  }
+};
+at::Tensor mlp8(at::Tensor x, at::Tensor w1, at::Tensor w2, at::Tensor err) {
+  check_matrix(x, "mlp_blocks");
+  check_matrix(w1, "mlp_blocks: in_proj");
+  check_matrix(w2, "mlp_blocks: out_proj");
+  same_device(w1, x, "mlp_blocks: in_proj");
+  same_device(w2, x, "mlp_blocks: out_proj");
+  TORCH_CHECK(x.size(1) == w1.size(1) && w1.size(0) == 2 * w2.size(1) && w2.size(0) >= 1 && w2.size(1) % 128 == 0,
+              "mlp_blocks: x [..., K], in_proj [2 H, K] and out_proj [N, H] with H a multiple of 128 expected, got ",
+              x.sizes(), ", ", w1.sizes(), " and ", w2.sizes());
+  elem_of(x, "mlp_blocks");
+  elem_of(w1, "mlp_blocks: in_proj");
+  elem_of(w2, "mlp_blocks: out_proj");
+  const c10::cuda::CUDAGuard guard(x.device());
+  x = rows_of(x);
+  if (wants_grad({&x, &w1, &w2}, kWhat)) {
+    if (!whole_rows(w1)) w1 = w1.contiguous();
+    if (!whole_rows(w2)) w2 = w2.contiguous();
+    return Mlp8Fn::apply(x, w1, w2, err);
+  }
+  w1 = rows_of(w1);
+  w2 = rows_of(w2);
+  Packed xr, w1r, w2r, g8;
+  pack(x, &xr, nullptr, nullptr, false, "mlp_blocks");
+  pack(w1, &w1r, nullptr, nullptr, false, "mlp_blocks: in_proj");
+  pack(w2, &w2r, nullptr, nullptr, false, "mlp_blocks: out_proj");
+  int* const e = err_word(err, x);
+  at::Tensor ab = fresh({x.size(0), w1.size(0)}, x.scalar_type(), x), y = fresh({x.size(0), w2.size(0)}, x.scalar_type(), x);
+  product(xr, w1r, ab, nullptr, false, e);
+  swiglu_forward(ab, nullptr, nullptr, &g8, nullptr);
+  product(g8, w2r, y, nullptr, false, e);
+  return y;
+}
+
+}  // namespace
+
+void bind_blocks8(pybind11::module_& m) {
+  m.def("pack8", &pack8, "rows and / or columns of a matrix in 8-bit blocks -> codes, scales of each");
+  m.def("unpack8", [](at::Tensor codes, at::Tensor scales, int64_t cols, py::object dtype) {
+    return unpack8(codes, scales, cols, torch::python::detail::py_object_to_dtype(dtype));
+  }, "the values that 8-bit blocks stand for");
+  m.def("gemm8", [](at::Tensor a, at::Tensor as, at::Tensor b, at::Tensor bs, int64_t cols, py::object dtype, OptT out,
+                    OptT bias, bool add, at::Tensor err) {
+    return gemm8(a, as, b, bs, cols, torch::python::detail::py_object_to_dtype(dtype), out, bias, add, err);
+  }, "C (+)= a b^T (+ bias) of packed matrices");
+  m.def("linear8_frozen", &linear8_frozen, "x times a weight held in 8 bits");
+  m.def("linear8", &linear8, "linear layer on 8-bit products, forward and backward");
+  m.def("swiglu8", &swiglu8, "silu(a) b with its input kept in 8 bits for the backward");
+  m.def("mlp8", &mlp8, "SwiGLU MLP on 8-bit products, forward and backward");
+}
+
+}  // namespace tgo

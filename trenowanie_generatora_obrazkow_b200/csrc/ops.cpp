@@ -16,6 +16,7 @@ static std::atomic<long long> g_launches{0};
 long long launch_count() { return g_launches.load(); }
 void count_launches(int n) { g_launches += n; }     // block_ops.cpp
 void bind_block_ops(pybind11::module_& m);          // block_ops.cpp
+void bind_blocks8(pybind11::module_& m);            // blocks8_ops.cpp
 
 #define TGO_CHECK_LAUNCH_N(expr, n)                                                        \
   do {                                                                                     \
@@ -38,7 +39,7 @@ static void bind_context() {
   }
 }
 
-static PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {
+PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {  // also blocks8_ops.cpp
   bind_context();
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   if (fn == nullptr) {
@@ -1276,6 +1277,7 @@ void peer_copy(int64_t dst, at::Tensor src, int64_t dst_version, int64_t counter
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   tgo::bind_block_ops(m);
+  tgo::bind_blocks8(m);
   m.doc() = "sm_100a kernels: tcgen05 GEMM, fused norms, attention, optimizer and comm kernels";
   m.def("gemm", &tgo::gemm, "tcgen05 bf16 GEMM: C = alpha * op(A) op(B)^T (+ beta D)", py::arg("A"), py::arg("B"),
         py::arg("C"), py::arg("a_mn"), py::arg("b_mn"), py::arg("D") = c10::nullopt, py::arg("alpha") = 1.0,

@@ -261,3 +261,98 @@ def rope_axes(q, k, pos, axes, theta=10000.0, q_w=None, k_w=None, interleaved=Tr
             rot = torch.cat((a * cos - b * sin, b * cos + a * sin), dim=-1)
         return torch.cat((rot, rest), dim=-1)
     return turn(q, q_w).to(q.dtype), turn(k, k_w).to(k.dtype)
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# 8-bit blocks: e4m3 with a power-of-two scale for each 128 values of a row
+# ----------------------------------------------------------------------------------------------------------------
+def quantize_blocks(x):
+    """x [M, K] -> (codes e4m3 [M, Kp], scales uint8 [ceil(M / 128), ceil(Kp / 512), 32, 4, 4]): see ops/blocks8.py."""
+    M, K = x.shape
+    nb, rt = -(-K // 128), -(-M // 128)
+    f = torch.nn.functional.pad(x.detach().float(), (0, nb * 128 - K)).view(M, nb, 128)
+    finite = f.isfinite()
+    top = torch.where(finite, f.abs(), 0.0).amax(-1)
+    m, e = torch.frexp(top)  # top = m 2^e, 1/2 <= m < 1; 448 = 7/8 2^9
+    e = torch.where(top > 0, torch.where(m <= 0.875, e - 9, e - 8).clamp_min(-127), -127)
+    q = torch.where(finite, torch.ldexp(f, -e[..., None]), math.nan).to(torch.float8_e4m3fn)
+    scales = torch.zeros(rt * 128, -(-nb // 4) * 4, dtype=torch.uint8, device=x.device)
+    scales[:M, :nb] = (e + 127).to(torch.uint8)
+    return q.view(M, nb * 128), scales.view(rt, 4, 32, -1, 4).permute(0, 3, 2, 1, 4).contiguous()
+
+
+def dequantize_blocks(codes, scales, cols):
+    """The values of quantize_blocks' output, fp32 [M, cols]."""
+    M, width = codes.shape
+    rt, quads = scales.shape[:2]
+    e = scales.permute(0, 3, 2, 1, 4).reshape(rt * 128, quads * 4)[:M, :width // 128].int() - 127
+    return torch.ldexp(codes.float().view(M, -1, 128), e[..., None]).view(M, width)[:, :cols]
+
+
+def in_blocks(x):
+    """The values that 8 bits hold of x [M, K], blocks along the rows (fp32)."""
+    return dequantize_blocks(*quantize_blocks(x), x.shape[1])
+
+
+class LinearBlocks(torch.autograd.Function):
+    """y = Q(x) Q(W)^T + b; dx = Q(dy) Q'(W); dW = Q'(dy)^T Q'(x) (Q: blocks along the rows, Q': along the columns)."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias):
+        ctx.xt, ctx.wt = in_blocks(x.t()), in_blocks(w.t())
+        ctx.types = w.dtype, None if bias is None else bias.dtype
+        y = in_blocks(x) @ in_blocks(w).t()
+        return (y if bias is None else y + bias.float()).to(x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        dx = (in_blocks(dy) @ ctx.wt.t()).to(dy.dtype)
+        dw = (in_blocks(dy.t()) @ ctx.xt.t()).to(ctx.types[0])
+        return dx, dw, None if ctx.types[1] is None else dy.float().sum(0).to(ctx.types[1])
+
+
+def swiglu_f32(ab):
+    a, b = ab.float().chunk(2, dim=-1)
+    return torch.nn.functional.silu(a) * b
+
+
+def swiglu_grad_f32(ab, dg):
+    a, b = ab.float().chunk(2, dim=-1)
+    dg, s = dg.float(), torch.sigmoid(a)
+    return torch.cat([dg * b * s * (1 + a * (1 - s)), dg * a * s], dim=-1)
+
+
+class SwigluBlocks(torch.autograd.Function):
+    """silu(a) b; the backward reads a and b in 8-bit blocks (each from its own first column)."""
+
+    @staticmethod
+    def forward(ctx, ab):
+        ctx.ab = torch.cat([in_blocks(v) for v in ab.chunk(2, dim=-1)], dim=-1)
+        return swiglu_f32(ab).to(ab.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dg):
+        return swiglu_grad_f32(ctx.ab, dg).to(dg.dtype)
+
+
+class MlpBlocks(torch.autograd.Function):
+    """[a | b] = Q(x) Q(W1)^T in x's type, g = silu(a) b, y = Q(g) Q(W2)^T; the backward reads x, g, a and b in 8 bits."""
+
+    @staticmethod
+    def forward(ctx, x, w1, w2):
+        ab = (in_blocks(x) @ in_blocks(w1).t()).to(x.dtype)
+        g = swiglu_f32(ab)
+        ctx.xt, ctx.w1t, ctx.w2t, ctx.gt = (in_blocks(v.t()) for v in (x, w1, w2, g))
+        ctx.ab = in_blocks(ab)
+        ctx.types = w1.dtype, w2.dtype
+        return (in_blocks(g) @ in_blocks(w2).t()).to(x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        dg = (in_blocks(dy) @ ctx.w2t.t()).to(dy.dtype)
+        dab = swiglu_grad_f32(ctx.ab, dg)
+        return ((in_blocks(dab) @ ctx.w1t.t()).to(dy.dtype), (in_blocks(dab.t()) @ ctx.xt.t()).to(ctx.types[0]),
+                (in_blocks(dy.t()) @ ctx.gt.t()).to(ctx.types[1]))
