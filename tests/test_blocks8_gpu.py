@@ -488,3 +488,20 @@ def test_launch_counts():
         before = ext().launch_count()
         call()
         assert ext().launch_count() - before == n
+
+
+@pytest.mark.parametrize("tile", [0, 1, 2])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (130, 300, 700), (520, 513, 1500), (300, 61, 4500), (2100, 2600, 640)])
+def test_every_tile(M, N, K, tile):
+    a, b = rnd(M, K, seed=3, dtype=torch.float32), rnd(N, K, seed=4, dtype=torch.float32)
+    A, Bb, qa, qb = B8.quantize_blocks(a), B8.quantize_blocks(b), held(a), held(b)
+    want = qa @ qb.t()
+    ext().set_gemm8_tile(tile)
+    try:
+        for dtype in TYPES:
+            assert_within(B8.gemm_blocks(A, Bb, dtype=dtype), want, product_tol(qa, qb, dtype, want))
+        out = torch.ones(M, N, device=DEV)
+        B8.gemm_blocks(A, Bb, out=out, accumulate=True)
+        assert_within(out, want + 1, product_tol(qa, qb, torch.float32, want) + (want + 1).abs() * 2.0 ** -23 + 2.0 ** -23)
+    finally:
+        ext().set_gemm8_tile(-1)

@@ -12,6 +12,8 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "block_ops.h"
 #include "blocks8.h"
@@ -26,10 +28,8 @@ constexpr int TILE = 128, PACK_THREADS = 256;
 constexpr int ATOM = 512;
 
 // ---------------------------------------------------------------------------------------------------------- scales
-__device__ __forceinline__ int scale_byte(float amax) {
-  const uint32_t u = __float_as_uint(amax);
-  return max(0, (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0));
-}
+// With u the bits of A: the carry out of the mantissa's top bits is the step from m <= 1.75 to m > 1.75.
+__device__ __forceinline__ int scale_byte(float amax) { return max(0, (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8); }
 __device__ __forceinline__ float scale_inv(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }  // 2^-e
 __device__ __forceinline__ float scale_of(int byte) {                                                          // 2^e
   return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u);
@@ -38,73 +38,127 @@ __device__ __forceinline__ float scale_of(int byte) {                           
 __device__ __forceinline__ long long scale_at(int r, int b, int quads) {
   return ((long long)(r >> 7) * quads + (b >> 2)) * ATOM + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
 }
-__device__ __forceinline__ uint32_t codes2(float a, float b) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
 }
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) { return codes2(a, b) | (codes2(c, d) << 16); }
-__device__ __forceinline__ uint2 codes8(const float (&f)[8], float k) {
-  return make_uint2(codes4(f[0] * k, f[1] * k, f[2] * k, f[3] * k), codes4(f[4] * k, f[5] * k, f[6] * k, f[7] * k));
+__device__ __forceinline__ uint32_t codes2(float a, float b) {  // a in the low byte
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(a), "f"(b));
+  return r;
 }
+__device__ __forceinline__ uint32_t codes4(float2 a, float2 b) { return codes2(a.x, a.y) | (codes2(b.x, b.y) << 16); }
 __device__ __forceinline__ float2 values2(uint32_t codes) {  // low two bytes
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-__device__ __forceinline__ void values8(uint2 c, float k, float (&f)[8]) {
+__device__ __forceinline__ void values8(uint2 c, float k, float2 (&f)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 t = values2((i < 2 ? c.x : c.y) >> ((i & 1) * 16));
-    f[2 * i] = t.x * k;
-    f[2 * i + 1] = t.y * k;
-  }
+  for (int i = 0; i < 4; ++i) f[i] = mul2(values2((i < 2 ? c.x : c.y) >> ((i & 1) * 16)), make_float2(k, k));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {  // passes over NaN
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // ------------------------------------------------------------------------------------------------------------ loads
-// n (0 to 8) elements of a row; 16-byte loads where vec (the row's start is aligned and n is 0 or 8)
+// Eight values of a row: fp32 as four pairs; 16-bit types as they are stored, unpacked where they are used (half the
+// registers, and maxima of two values at a time).
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&f)[8]) {
-  Raw<T, 8> r;
-  r.zero();
-  if (vec) {
-    if (n > 0) r.load(p);
-    r.get(f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = j < n ? to_f(p[j]) : 0.f;
+struct Eight {
+  static constexpr bool WIDE = sizeof(T) == 4;
+  using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  uint32_t u[WIDE ? 8 : 4];
+  __device__ __forceinline__ float2 pair(int w) const {
+    if constexpr (WIDE) return make_float2(__uint_as_float(u[2 * w]), __uint_as_float(u[2 * w + 1]));
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      return make_float2(__uint_as_float(u[w] << 16), __uint_as_float(u[w] & 0xffff0000u));
+    else return __half22float2(*reinterpret_cast<const __half2*>(&u[w]));
   }
-}
+  __device__ __forceinline__ void set(int w, float2 v) {
+    if constexpr (WIDE) {
+      u[2 * w] = __float_as_uint(v.x), u[2 * w + 1] = __float_as_uint(v.y);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 t = __floats2bfloat162_rn(v.x, v.y);
+      u[w] = *reinterpret_cast<const uint32_t*>(&t);
+    } else {
+      const __half2 t = __floats2half2_rn(v.x, v.y);
+      u[w] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+  }
+  // n (0 to 8) elements of a row; 16-byte loads where vec (the address is aligned and n is 0 or 8)
+  __device__ __forceinline__ void load(const T* p, int n, bool vec) {
+#pragma unroll
+    for (int i = 0; i < (WIDE ? 8 : 4); ++i) u[i] = 0u;
+    if (vec) {
+      if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < (WIDE ? 2 : 1); ++i) {
+          const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + i);
+          u[4 * i] = q.x, u[4 * i + 1] = q.y, u[4 * i + 2] = q.z, u[4 * i + 3] = q.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) set(w, make_float2(2 * w < n ? to_f(p[2 * w]) : 0.f, 2 * w + 1 < n ? to_f(p[2 * w + 1]) : 0.f));
+    }
+  }
+  __device__ __forceinline__ void fetch(const T* p) {  // aligned shared memory
+#pragma unroll
+    for (int i = 0; i < (WIDE ? 2 : 1); ++i) {
+      const uint4 q = reinterpret_cast<const uint4*>(p)[i];
+      u[4 * i] = q.x, u[4 * i + 1] = q.y, u[4 * i + 2] = q.z, u[4 * i + 3] = q.w;
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int n, bool vec) const {
+    if (vec) {
+      if (n <= 0) return;
+#pragma unroll
+      for (int i = 0; i < (WIDE ? 2 : 1); ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) p[j] = from_f<T>((j & 1) ? pair(j >> 1).y : pair(j >> 1).x);
+    }
+  }
+  // magnitudes: NaN passes over, an infinity shows
+  static __device__ __forceinline__ uint32_t top2(uint32_t a, uint32_t b) {
+    const Two r = __hmax2(__habs2(*reinterpret_cast<const Two*>(&a)), __habs2(*reinterpret_cast<const Two*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ float2 widen(uint32_t v) {
+    Eight e;
+    e.u[0] = v;
+    return e.pair(0);
+  }
+  __device__ __forceinline__ float top() const {
+    if constexpr (WIDE) {
+      const float2 a = pair(0), b = pair(1), c = pair(2), d = pair(3);
+      return fmaxf(max3(max3(fabsf(a.x), fabsf(a.y), fabsf(b.x)), fabsf(b.y), fabsf(c.x)), max3(fabsf(c.y), fabsf(d.x), fabsf(d.y)));
+    } else {
+      const float2 m = widen(top2(top2(u[0], u[1]), top2(u[2], u[3])));
+      return fmaxf(m.x, m.y);
+    }
+  }
+  __device__ __forceinline__ void drop_infinities() {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float2 v = pair(w);
+      if (fabsf(v.x) == INFINITY) v.x = NAN;
+      if (fabsf(v.y) == INFINITY) v.y = NAN;
+      set(w, v);
+    }
+  }
+};
+
 template <typename T>
-__device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&f)[8]) {
-  if (vec) {
-    if (n <= 0) return;
-    Raw<T, 8> r;
-    r.put(f);
-    r.store(p);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = from_f<T>(f[j]);
-  }
-}
-__device__ __forceinline__ float top8(const float (&f)[8]) {
-  float a = fmaxf(fabsf(f[0]), fabsf(f[1])), b = fmaxf(fabsf(f[2]), fabsf(f[3]));
-  float c = fmaxf(fabsf(f[4]), fabsf(f[5])), d = fmaxf(fabsf(f[6]), fabsf(f[7]));
-  return fmaxf(fmaxf(a, b), fmaxf(c, d));
-}
-// fmaxf passes over NaN, an infinity shows: it becomes NaN and the largest finite magnitude is taken again
-__device__ __forceinline__ float finite_top8(float (&f)[8]) {
-  float m = top8(f);
-  if (m == INFINITY) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (fabsf(f[j]) == INFINITY) f[j] = NAN;
-    m = top8(f);
-  }
-  return m;
-}
-__device__ __forceinline__ float max16(float m) {  // over the 16 lanes of a row
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
+__device__ __forceinline__ uint2 codes8(const Eight<T>& v, float inv) {
+  const float2 k = make_float2(inv, inv);
+  return make_uint2(codes4(mul2(v.pair(0), k), mul2(v.pair(1), k)), codes4(mul2(v.pair(2), k), mul2(v.pair(3), k)));
 }
 
 // ------------------------------------------------------------------------------------------------------- tile output
@@ -116,101 +170,162 @@ struct Side {             // one 8-bit output
 };
 struct TileShared {
   float part[8][TILE];
+  float inv[TILE];
   uint4 t[TILE * TILE / 16];  // transposed codes: column c's eight bytes of rows 8 i .. at c * 16 + (i ^ (c / 8 % 16))
 };
 
-// rows of the tile: row0 + 8 rg + i, blocks along the columns (block kb of nb)
-__device__ __forceinline__ void emit_rows(const Side& o, float (&v)[8][8], int row0, int kb, int nb, int rg, int l16) {
+// The maxima m of the R rows from r0 on over this thread's columns -> 2^-e of each row over the 16 lanes that share it; the
+// scale bytes are written (also of rows past `rows` in their atom). Each exchange halves the rows that a lane still carries:
+// 8 shuffles for 8 rows instead of 32.
+template <int R>
+__device__ __forceinline__ void row_scales(const float (&m)[R], uint8_t* scales, int r0, int kb, int nb, int quads, int rows,
+                                           float (&inv)[R]) {
+  const int lane = threadIdx.x & 31;
+  float a[R / 2], b[R == 8 ? 2 : 1], c;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = row0 + 8 * rg + i;
-    const int byte = scale_byte(max16(finite_top8(v[i])));
-    if (r < o.rows) *reinterpret_cast<uint2*>(o.codes + (long long)r * o.width + kb * TILE + 8 * l16) = codes8(v[i], scale_inv(byte));
-    if (l16 == 0) {
-      uint8_t* s = o.scales + scale_at(r, kb, o.quads);
+  for (int k = 0; k < R / 2; ++k) {
+    const float keep = (lane & 8) ? m[R / 2 + k] : m[k], send = (lane & 8) ? m[k] : m[R / 2 + k];
+    a[k] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, 8));
+  }
+#pragma unroll
+  for (int k = 0; k < R / 4; ++k) {
+    const float keep = (lane & 4) ? a[R / 4 + k] : a[k], send = (lane & 4) ? a[k] : a[R / 4 + k];
+    b[k] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, 4));
+  }
+  if constexpr (R == 8) c = fmaxf((lane & 2) ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, (lane & 2) ? b[0] : b[1], 2));
+  else c = fmaxf(b[0], __shfl_xor_sync(0xffffffffu, b[0], 2));
+  c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, 1));
+  const int byte = scale_byte(c);
+  const float mine = scale_inv(byte);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    inv[i] = __shfl_sync(0xffffffffu, mine, (lane & 16) | (R == 8 ? ((i & 4) << 1) | ((i & 2) << 1) | ((i & 1) << 1) : i << 2));
+  if ((lane & (R == 8 ? 1 : 3)) == 0) {
+    const int r = r0 + ((lane & 15) >> (R == 8 ? 1 : 2));
+    if (r < ((rows + TILE - 1) & ~(TILE - 1))) {
+      uint8_t* s = scales + scale_at(r, kb, quads);
       s[0] = (uint8_t)byte;
       if (kb == nb - 1)
-        for (int b = 1; b < 4 - (kb & 3); ++b) s[b] = 0;
+        for (int k = 1; k < 4 - (kb & 3); ++k) s[k] = 0;
     }
   }
 }
-// columns col0 + 8 l16 + j as rows of the transposed form, blocks along the tile's rows (block mb of nb)
-__device__ __forceinline__ void emit_cols(const Side& o, float (&v)[8][8], int col0, int mb, int nb, int rg, int l16,
-                                          TileShared& sh) {
+
+// Packs the tile whose rows row0 + 8 rg + i and columns col0 + 8 l16 + j the thread holds in v[i]: blocks along the rows
+// (block kb of nkb) and / or along the columns as rows of the transposed form (block mb of nmb).
+template <bool ROWS, bool COLS, typename T>
+__device__ __forceinline__ void emit(Eight<T> (&v)[8], const Side& r, const Side& c, int row0, int col0, int kb, int nkb, int mb,
+                                     int nmb, TileShared& sh) {
+  const int l16 = threadIdx.x & 15, rg = threadIdx.x >> 4;
   float m[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m[j] = 0.f;
+  for (int i = 0; i < 8; ++i) m[i] = v[i].top();
+  if (fmaxf(max3(max3(m[0], m[1], m[2]), m[3], m[4]), max3(m[5], m[6], m[7])) == INFINITY) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    finite_top8(v[i]);
+      for (int k = 0; k < 8; ++k)
+        if (k == i) v[k].drop_infinities();
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = fmaxf(m[j], fabsf(v[i][j]));
+    for (int i = 0; i < 8; ++i) m[i] = v[i].top();
   }
+  if constexpr (COLS) {
+    float2 t[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
-  __syncthreads();  // the tile before has been read
-  if ((rg & 1) == 0) {
-    *reinterpret_cast<float4*>(&sh.part[rg >> 1][8 * l16]) = make_float4(m[0], m[1], m[2], m[3]);
-    *reinterpret_cast<float4*>(&sh.part[rg >> 1][8 * l16 + 4]) = make_float4(m[4], m[5], m[6], m[7]);
-  }
-  __syncthreads();
+    for (int w = 0; w < 4; ++w) {
+      if constexpr (Eight<T>::WIDE) {
+        t[w] = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float4 a = *reinterpret_cast<const float4*>(&sh.part[w][8 * l16]);
-    const float4 b = *reinterpret_cast<const float4*>(&sh.part[w][8 * l16 + 4]);
-    m[0] = fmaxf(m[0], a.x), m[1] = fmaxf(m[1], a.y), m[2] = fmaxf(m[2], a.z), m[3] = fmaxf(m[3], a.w);
-    m[4] = fmaxf(m[4], b.x), m[5] = fmaxf(m[5], b.y), m[6] = fmaxf(m[6], b.z), m[7] = fmaxf(m[7], b.w);
-  }
-  uint2* t = reinterpret_cast<uint2*>(sh.t);
+        for (int i = 0; i < 8; i += 2) {
+          const float2 p = v[i].pair(w), q = v[i + 1].pair(w);
+          t[w] = make_float2(max3(t[w].x, fabsf(p.x), fabsf(q.x)), max3(t[w].y, fabsf(p.y), fabsf(q.y)));
+        }
+      } else {
+        uint32_t a = Eight<T>::top2(v[0].u[w], v[1].u[w]);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int byte = scale_byte(m[j]);
-    float f[8];
+        for (int i = 2; i < 8; ++i) a = Eight<T>::top2(a, v[i].u[w]);
+        t[w] = Eight<T>::widen(a);
+      }
+      t[w].x = fmaxf(t[w].x, __shfl_xor_sync(0xffffffffu, t[w].x, 16));
+      t[w].y = fmaxf(t[w].y, __shfl_xor_sync(0xffffffffu, t[w].y, 16));
+    }
+    if ((rg & 1) == 0) {
+      *reinterpret_cast<float4*>(&sh.part[rg >> 1][8 * l16]) = make_float4(t[0].x, t[0].y, t[1].x, t[1].y);
+      *reinterpret_cast<float4*>(&sh.part[rg >> 1][8 * l16 + 4]) = make_float4(t[2].x, t[2].y, t[3].x, t[3].y);
+    }
+    __syncthreads();
+    if (threadIdx.x < TILE) {
+      float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = v[i][j];
-    t[(8 * l16 + j) * 16 + (rg ^ l16)] = codes8(f, scale_inv(byte));
-    if (rg == 0) {
-      uint8_t* s = o.scales + scale_at(col0 + 8 * l16 + j, mb, o.quads);
+      for (int w = 0; w < 8; ++w) top = fmaxf(top, sh.part[w][threadIdx.x]);
+      const int byte = scale_byte(top);
+      sh.inv[threadIdx.x] = scale_inv(byte);
+      uint8_t* s = c.scales + scale_at(col0 + threadIdx.x, mb, c.quads);
       s[0] = (uint8_t)byte;
-      if (mb == nb - 1)
-        for (int b = 1; b < 4 - (mb & 3); ++b) s[b] = 0;
+      if (mb == nmb - 1)
+        for (int k = 1; k < 4 - (mb & 3); ++k) s[k] = 0;
     }
   }
-  __syncthreads();
+  if constexpr (ROWS) {
+    float inv[8];
+    row_scales(m, r.scales, row0 + 8 * rg, kb, nkb, r.quads, r.rows, inv);
+    uint8_t* d = r.codes + (long long)(row0 + 8 * rg) * r.width + kb * TILE + 8 * l16;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int at = threadIdx.x + k * PACK_THREADS, c = at >> 3, pair = at & 7, key = (c >> 3) & 15;
-    uint4 u = sh.t[c * 8 + (pair ^ (key >> 1))];
-    if (key & 1) u = make_uint4(u.z, u.w, u.x, u.y);
-    if (col0 + c < o.rows) *reinterpret_cast<uint4*>(o.codes + (long long)(col0 + c) * o.width + mb * TILE + pair * 16) = u;
+    for (int i = 0; i < 8; ++i) {
+      const uint2 q = codes8(v[i], inv[i]);
+      if (row0 + 8 * rg + i < r.rows) *reinterpret_cast<uint2*>(d) = q;
+      d += r.width;
+    }
+  }
+  if constexpr (COLS) {
+    __syncthreads();
+    uint2* t = reinterpret_cast<uint2*>(sh.t);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float2 k = *reinterpret_cast<const float2*>(&sh.inv[8 * l16 + 2 * w]);
+      float2 f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = mul2(v[i].pair(w), k);
+      t[(8 * l16 + 2 * w) * 16 + (rg ^ l16)] =
+          make_uint2(codes2(f[0].x, f[1].x) | codes2(f[2].x, f[3].x) << 16, codes2(f[4].x, f[5].x) | codes2(f[6].x, f[7].x) << 16);
+      t[(8 * l16 + 2 * w + 1) * 16 + (rg ^ l16)] =
+          make_uint2(codes2(f[0].y, f[1].y) | codes2(f[2].y, f[3].y) << 16, codes2(f[4].y, f[5].y) | codes2(f[6].y, f[7].y) << 16);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = threadIdx.x + k * PACK_THREADS, col = at >> 3, pair = at & 7, key = (col >> 3) & 15;
+      uint4 u = sh.t[col * 8 + (pair ^ (key >> 1))];
+      if (key & 1) u = make_uint4(u.z, u.w, u.x, u.y);
+      if (col0 + col < c.rows) *reinterpret_cast<uint4*>(c.codes + (long long)(col0 + col) * c.width + mb * TILE + pair * 16) = u;
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------- pack
 template <typename T, bool ROWS, bool COLS, bool SUMS>
-__global__ void __launch_bounds__(PACK_THREADS) pack8_kernel(const T* __restrict__ x, long long ld, int M, int K, bool vec,
-                                                            Side rows, Side cols, float* __restrict__ sums) {
+__global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 4 ? 2 : 3)
+    pack8_kernel(const T* __restrict__ x, long long ld, int M, int K, bool vec, Side rows, Side cols, float* __restrict__ sums) {
   __shared__ __align__(16) TileShared sh;
   const int nkb = (K + TILE - 1) / TILE, nmb = (M + TILE - 1) / TILE;
   const int kb = blockIdx.x % nkb, mb = blockIdx.x / nkb;
   const int l16 = threadIdx.x & 15, rg = threadIdx.x >> 4;
   const int row0 = mb * TILE, c = kb * TILE + 8 * l16, n = max(0, min(8, K - c));
-  float v[8][8];
+  Eight<T> v[8];
+  const T* p = x + (long long)(row0 + 8 * rg) * ld + c;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = row0 + 8 * rg + i;
-    load8<T>(x + (long long)r * ld + c, r < M ? n : 0, vec, v[i]);
-  }
+  for (int i = 0; i < 8; ++i, p += ld) v[i].load(p, row0 + 8 * rg + i < M ? n : 0, vec);
   if constexpr (SUMS) {  // before anything becomes NaN
-    float m[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      m[j] = ((v[0][j] + v[1][j]) + (v[2][j] + v[3][j])) + ((v[4][j] + v[5][j]) + (v[6][j] + v[7][j]));
-      m[j] += __shfl_xor_sync(0xffffffffu, m[j], 16);
+    for (int w = 0; w < 4; ++w) {
+      float2 a = v[0].pair(w);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) a.x += v[i].pair(w).x, a.y += v[i].pair(w).y;
+      a.x += __shfl_xor_sync(0xffffffffu, a.x, 16);
+      a.y += __shfl_xor_sync(0xffffffffu, a.y, 16);
+      if ((rg & 1) == 0) *reinterpret_cast<float2*>(&sh.part[rg >> 1][8 * l16 + 2 * w]) = a;
     }
-    if ((rg & 1) == 0)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sh.part[rg >> 1][8 * l16 + j] = m[j];
     __syncthreads();
     if (threadIdx.x < TILE && kb * TILE + threadIdx.x < K) {
       float a = 0.f;
@@ -218,9 +333,9 @@ __global__ void __launch_bounds__(PACK_THREADS) pack8_kernel(const T* __restrict
       for (int w = 0; w < 8; ++w) a += sh.part[w][threadIdx.x];
       sums[(long long)mb * K + kb * TILE + threadIdx.x] = a;
     }
+    __syncthreads();
   }
-  if constexpr (ROWS) emit_rows(rows, v, row0, kb, nkb, rg, l16);
-  if constexpr (COLS) emit_cols(cols, v, kb * TILE, mb, nmb, rg, l16, sh);
+  emit<ROWS, COLS, T>(v, rows, cols, row0, kb * TILE, kb, nkb, mb, nmb, sh);
 }
 
 bool aligned16(const void* p, long long stride_bytes) {
@@ -275,163 +390,476 @@ __global__ void __launch_bounds__(256) colsum_kernel(const float* __restrict__ s
 }
 
 // ----------------------------------------------------------------------------------------------------------- unpack
+// a thread: 16 codes of a row
 template <typename T>
 __global__ void __launch_bounds__(256) unpack8_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                      int R, int K, long long width, int quads, T* __restrict__ out,
+                                                      int R, int K, int width, int quads, T* __restrict__ out,
                                                       long long ldo, bool vec) {
-  const int per = (int)(width / 8);  // groups of eight codes of a row
-  const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (at >= (long long)R * per) return;
-  const int r = (int)(at / per), c = (int)(at % per) * 8;
-  if (c >= K) return;
-  float f[8];
-  values8(*reinterpret_cast<const uint2*>(codes + (long long)r * width + c), scale_of(scales[scale_at(r, c >> 7, quads)]), f);
-  store8<T>(out + (long long)r * ldo + c, min(8, K - c), vec, f);
+  const int per = width / 16;
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int r = (int)(at / per), c = (int)(at - (long long)r * per) * 16;
+  if (at >= (long long)R * per || c >= K) return;
+  const uint4 q = __ldg(reinterpret_cast<const uint4*>(codes + (long long)r * width + c));
+  const float k = scale_of(__ldg(scales + scale_at(r, c >> 7, quads)));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float2 f[4];
+    values8(h == 0 ? make_uint2(q.x, q.y) : make_uint2(q.z, q.w), k, f);
+    Eight<T> e;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) e.set(w, f[w]);
+    e.store(out + (long long)r * ldo + c + 8 * h, max(0, min(8, K - c - 8 * h)), vec);
+  }
 }
 
 template <typename T>
 cudaError_t unpack_typed(const uint8_t* codes, const uint8_t* scales, int R, int K, void* out, long long ldo, cudaStream_t s) {
   const int nb = (K + TILE - 1) / TILE;
-  const long long groups = (long long)R * nb * (TILE / 8), blocks = (groups + 255) / 256;
+  const long long groups = (long long)R * nb * (TILE / 16), blocks = (groups + 255) / 256;
   if (blocks >= (1ll << 31)) return cudaErrorInvalidValue;
   const bool vec = K % 8 == 0 && aligned16(out, ldo * (long long)sizeof(T));
-  unpack8_kernel<T><<<(int)blocks, 256, 0, s>>>(codes, scales, R, K, (long long)nb * TILE, (nb + 3) / 4,
-                                               static_cast<T*>(out), ldo, vec);
+  unpack8_kernel<T><<<(int)blocks, 256, 0, s>>>(codes, scales, R, K, nb * TILE, (nb + 3) / 4, static_cast<T*>(out), ldo, vec);
   return cudaGetLastError();
 }
 
 // ----------------------------------------------------------------------------------------------------------- SwiGLU
-// g = silu(a) b = a b / (1 + exp(-a)): __expf is within 2 ulp + 2^-21 |a| of exp, which rounding to 16 bits hides; for
-// fp32 results expf is used
+// s = 1 / (1 + exp(-a)). For 16-bit types exp2 and the reciprocal are the hardware's approximations (an argument rounded to
+// 2^-24 of itself and two units in the last place), which the result's rounding hides; fp32 results take the library's.
 template <bool FINE>
 __device__ __forceinline__ float sigmoid(float a) {
-  const float e = FINE ? expf(-a) : __expf(-a);
-  return FINE ? 1.f / (1.f + e) : __fdividef(1.f, 1.f + e);
-}
-
-// G: g in ab's type; Q: g in 8 bits (Side g8, and g8t where its codes are given). The checkpoint's blocks are those of a
-// [M, 2 Hp] matrix: a's first, then b's.
-template <typename T, bool G, bool Q>
-__global__ void __launch_bounds__(PACK_THREADS) swiglu8_fwd_kernel(const T* __restrict__ ab, long long ld, int M, int H,
-                                                                  bool vec, bool vec_g, T* __restrict__ g, Side ck, Side g8,
-                                                                  Side g8t) {
-  __shared__ __align__(16) TileShared sh;
-  const int nhb = (H + TILE - 1) / TILE, nmb = (M + TILE - 1) / TILE;
-  const int hb = blockIdx.x % nhb, mb = blockIdx.x / nhb;
-  const int l16 = threadIdx.x & 15, rg = threadIdx.x >> 4;
-  const int row0 = mb * TILE, c = hb * TILE + 8 * l16, n = max(0, min(8, H - c));
-  float v[8][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = row0 + 8 * rg + i, nr = r < M ? n : 0;
-    float a[8], b[8];
-    const T* p = ab + (long long)r * ld + c;
-    load8<T>(p, nr, vec, a);
-    load8<T>(p + H, nr, vec, b);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = a[j] * sigmoid<sizeof(T) == 4>(a[j]) * b[j];
-    if constexpr (G) store8<T>(g + (long long)r * H + c, nr, vec_g, v[i]);
-    if (ck.codes != nullptr) {
-      const int ba = scale_byte(max16(finite_top8(a))), bb = scale_byte(max16(finite_top8(b)));
-      if (r < M) {
-        uint8_t* d = ck.codes + (long long)r * ck.width + c;
-        *reinterpret_cast<uint2*>(d) = codes8(a, scale_inv(ba));
-        *reinterpret_cast<uint2*>(d + (long long)nhb * TILE) = codes8(b, scale_inv(bb));
-      }
-      if (l16 == 0) {
-        ck.scales[scale_at(r, hb, ck.quads)] = (uint8_t)ba;
-        uint8_t* s = ck.scales + scale_at(r, nhb + hb, ck.quads);
-        s[0] = (uint8_t)bb;
-        if (hb == nhb - 1)
-          for (int k = 1; k < 4 - ((nhb + hb) & 3); ++k) s[k] = 0;
-      }
-    }
-  }
-  if constexpr (Q) {
-    emit_rows(g8, v, row0, hb, nhb, rg, l16);
-    if (g8t.codes != nullptr) emit_cols(g8t, v, hb * TILE, mb, nmb, rg, l16, sh);
+  if constexpr (FINE) {
+    return 1.f / (1.f + expf(-a));
+  } else {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
   }
 }
 
-// dg, Q(a), Q(b) -> da = dg b s (1 + a (1 - s)), db = dg a s with s = sigmoid(a). D: in dg's type; Q: in 8 bits, both
-// ways. One half after the other, so that a thread holds one tile's values.
-template <typename T, bool D, bool Q>
-__global__ void __launch_bounds__(PACK_THREADS) swiglu8_bwd_kernel(const T* __restrict__ dg, long long ld, int M, int H,
-                                                                  bool vec, bool vec_d, T* __restrict__ dab, Side ck,
-                                                                  Side d8, Side d8t) {
-  __shared__ __align__(16) TileShared sh;
-  const int nhb = (H + TILE - 1) / TILE, nmb = (M + TILE - 1) / TILE;
-  const int hb = blockIdx.x % nhb, mb = blockIdx.x / nhb;
-  const int l16 = threadIdx.x & 15, rg = threadIdx.x >> 4;
-  const int row0 = mb * TILE, c = hb * TILE + 8 * l16, n = max(0, min(8, H - c));
-  uint2 ca[8], cb[8];
-  float dgv[8][8];
+// scale of row r's block b for the eight rows from r0 = 8 k on: 16 bytes apart
+__device__ __forceinline__ const uint8_t* scales_from(const Side& s, int r0, int b) { return s.scales + scale_at(r0, b, s.quads); }
+
+// g in ab's type, the checkpoint of ab in 8 bits. Rows alone: a thread holds 8 columns of RPT rows. The checkpoint's blocks
+// are those of a [M, 2 Hp] matrix: a's first, then b's.
+template <typename T, bool CK>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) swiglu8_fwd_kernel(const T* __restrict__ ab, long long ld, int M, int H, bool vec,
+                                                          bool vec_g, T* __restrict__ g, Side ck) {
+  constexpr int RPT = 4;
+  const int nhb = (H + TILE - 1) / TILE;
+  const int hb = blockIdx.x % nhb, l16 = threadIdx.x & 15;
+  const int r0 = (blockIdx.x / nhb) * 16 * RPT + (threadIdx.x >> 4) * RPT;
+  const int c = hb * TILE + 8 * l16, n = max(0, min(8, H - c));
+  Eight<T> a[RPT], b[RPT];
+  const T* p = ab + (long long)r0 * ld + c;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = row0 + 8 * rg + i;
-    load8<T>(dg + (long long)r * ld + c, r < M ? n : 0, vec, dgv[i]);
-    ca[i] = cb[i] = make_uint2(0u, 0u);
-    if (r < M) {
-      const uint8_t* s = ck.codes + (long long)r * ck.width + c;
-      ca[i] = *reinterpret_cast<const uint2*>(s);
-      cb[i] = *reinterpret_cast<const uint2*>(s + (long long)nhb * TILE);
-    }
+  for (int i = 0; i < RPT; ++i, p += ld) {
+    a[i].load(p, r0 + i < M ? n : 0, vec);
+    b[i].load(p + H, r0 + i < M ? n : 0, vec);
   }
-  float v[8][8];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int i = 0; i < RPT; ++i) {
+    Eight<T> o;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = row0 + 8 * rg + i;
-      float a[8], b[8];
-      values8(ca[i], scale_of(ck.scales[scale_at(r, hb, ck.quads)]), a);
-      if (half == 0) values8(cb[i], scale_of(ck.scales[scale_at(r, nhb + hb, ck.quads)]), b);
+    for (int w = 0; w < 4; ++w) {
+      const float2 x = a[i].pair(w), y = b[i].pair(w);
+      o.set(w, make_float2(x.x * sigmoid<sizeof(T) == 4>(x.x) * y.x, x.y * sigmoid<sizeof(T) == 4>(x.y) * y.y));
+    }
+    o.store(g + (long long)(r0 + i) * H + c, r0 + i < M ? n : 0, vec_g);
+  }
+  if constexpr (CK) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float s = sigmoid<sizeof(T) == 4>(a[j]);
-        v[i][j] = half == 0 ? dgv[i][j] * b[j] * s * (1.f + a[j] * (1.f - s)) : dgv[i][j] * a[j] * s;
+    for (int h = 0; h < 2; ++h) {
+      Eight<T>(&v)[RPT] = h == 0 ? a : b;
+      float m[RPT], inv[RPT];
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        m[i] = v[i].top();
+        if (m[i] == INFINITY) {
+          v[i].drop_infinities();
+          m[i] = v[i].top();
+        }
       }
-      if constexpr (D) store8<T>(dab + (long long)r * 2 * H + half * H + c, r < M ? n : 0, vec_d, v[i]);
-    }
-    if constexpr (Q) {
-      emit_rows(d8, v, row0, half * nhb + hb, 2 * nhb, rg, l16);
-      emit_cols(d8t, v, half * H + hb * TILE, mb, nmb, rg, l16, sh);
+      row_scales(m, ck.scales, r0, h * nhb + hb, 2 * nhb, ck.quads, ck.rows, inv);
+      uint8_t* d = ck.codes + (long long)r0 * ck.width + (long long)h * nhb * TILE + c;
+#pragma unroll
+      for (int i = 0; i < RPT; ++i, d += ck.width)
+        if (r0 + i < M) *reinterpret_cast<uint2*>(d) = codes8(v[i], inv[i]);
     }
   }
+}
+
+// dg, Q(a), Q(b) -> [da | db] in dg's type: da = dg b s (1 + a (1 - s)), db = dg a s with s = sigmoid(a)
+template <bool FINE>
+__device__ __forceinline__ void swiglu_grad(float2 a, float2 b, float2 dg, float2& da, float2& db) {
+  const float2 s = make_float2(sigmoid<FINE>(a.x), sigmoid<FINE>(a.y));
+  const float2 t = mul2(dg, s);
+  const float2 u = make_float2(fmaf(a.x, 1.f - s.x, 1.f), fmaf(a.y, 1.f - s.y, 1.f));
+  da = mul2(mul2(t, b), u);
+  db = mul2(t, a);
+}
+template <typename T>
+__global__ void __launch_bounds__(256) swiglu8_bwd_kernel(const T* __restrict__ dg, long long ld, int M, int H, bool vec,
+                                                          bool vec_d, T* __restrict__ dab, Side ck) {
+  constexpr int RPT = 4;
+  const int nhb = (H + TILE - 1) / TILE;
+  const int hb = blockIdx.x % nhb, l16 = threadIdx.x & 15;
+  const int r0 = (blockIdx.x / nhb) * 16 * RPT + (threadIdx.x >> 4) * RPT;
+  const int c = hb * TILE + 8 * l16, n = max(0, min(8, H - c));
+  Eight<T> dv[RPT];
+  uint2 ca[RPT], cb[RPT];
+  float ka[RPT], kb[RPT];
+  const T* p = dg + (long long)r0 * ld + c;
+  const uint8_t* q = ck.codes + (long long)r0 * ck.width + c;
+  const uint8_t *sa = scales_from(ck, r0, hb), *sb = scales_from(ck, r0, nhb + hb);
+#pragma unroll
+  for (int i = 0; i < RPT; ++i, p += ld, q += ck.width) {
+    const bool in = r0 + i < M;
+    dv[i].load(p, in ? n : 0, vec);
+    ca[i] = in ? __ldg(reinterpret_cast<const uint2*>(q)) : make_uint2(0u, 0u);
+    cb[i] = in ? __ldg(reinterpret_cast<const uint2*>(q + (long long)nhb * TILE)) : make_uint2(0u, 0u);
+    ka[i] = in ? scale_of(__ldg(sa + 16 * i)) : 0.f;
+    kb[i] = in ? scale_of(__ldg(sb + 16 * i)) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    float2 a[4], b[4];
+    values8(ca[i], ka[i], a);
+    values8(cb[i], kb[i], b);
+    Eight<T> oa, ob;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float2 da, db;
+      swiglu_grad<sizeof(T) == 4>(a[w], b[w], dv[i].pair(w), da, db);
+      oa.set(w, da);
+      ob.set(w, db);
+    }
+    T* o = dab + (long long)(r0 + i) * 2 * H + c;
+    oa.store(o, r0 + i < M ? n : 0, vec_d);
+    ob.store(o + H, r0 + i < M ? n : 0, vec_d);
+  }
+}
+
+// ---- the forms of the MLP: everything that is written is in 8 bits, both ways where a weight's gradient wants it. One CTA of
+// 512 threads per SM walks over tiles of 128 x 128; the tiles come by TMA, two ahead of the arithmetic (fp32: one), so no
+// registers and no address arithmetic go into loads. A thread holds 8 columns of 4 rows; the backward holds da and db at once
+// and takes each exponential once. What bounds them is the arithmetic: some 25 and 30 instructions an element.
+constexpr int QT_THREADS = 512, QT_R = 4;
+template <typename T>
+struct QtStages {
+  static constexpr int N = sizeof(T) == 4 ? 1 : 2;
+};
+struct QtOut {  // transposed side of one tile: maxima of the 16 warps, 2^-e, codes
+  float part[16][TILE];
+  float inv[TILE];
+  uint4 t[TILE * TILE / 16];  // column c's four bytes of rows 4 i .. at word c * 32 + (i ^ 2 (c / 8 % 16))
+};
+
+template <typename T>
+__device__ __forceinline__ float finite_top(Eight<T>& v) {
+  float m = v.top();
+  if (m == INFINITY) {
+    v.drop_infinities();
+    m = v.top();
+  }
+  return m;
+}
+// rows of the tile into d: blocks along the columns
+template <typename T>
+__device__ __forceinline__ void qt_rows(Eight<T> (&v)[QT_R], const Side& o, int r0, int kb, int nkb, int l16) {
+  float m[QT_R], inv[QT_R];
+#pragma unroll
+  for (int i = 0; i < QT_R; ++i) m[i] = finite_top(v[i]);
+  row_scales(m, o.scales, r0, kb, nkb, o.quads, o.rows, inv);
+  uint8_t* d = o.codes + (long long)r0 * o.width + kb * TILE + 8 * l16;
+#pragma unroll
+  for (int i = 0; i < QT_R; ++i, d += o.width)
+    if (r0 + i < o.rows) *reinterpret_cast<uint2*>(d) = codes8(v[i], inv[i]);
+}
+__device__ __forceinline__ void qt_cols_part(Eight<float> (&v)[QT_R], QtOut& sh, int l16) {
+  float2 t[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float2 a = v[0].pair(w), b = v[1].pair(w), c = v[2].pair(w), d = v[3].pair(w);
+    t[w] = make_float2(fmaxf(max3(fabsf(a.x), fabsf(b.x), fabsf(c.x)), fabsf(d.x)),
+                       fmaxf(max3(fabsf(a.y), fabsf(b.y), fabsf(c.y)), fabsf(d.y)));
+    t[w].x = fmaxf(t[w].x, __shfl_xor_sync(0xffffffffu, t[w].x, 16));
+    t[w].y = fmaxf(t[w].y, __shfl_xor_sync(0xffffffffu, t[w].y, 16));
+  }
+  if ((threadIdx.x & 16) == 0) {
+    float* p = sh.part[threadIdx.x >> 5] + 8 * l16;
+    *reinterpret_cast<float4*>(p) = make_float4(t[0].x, t[0].y, t[1].x, t[1].y);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(t[2].x, t[2].y, t[3].x, t[3].y);
+  }
+}
+__device__ __forceinline__ void qt_cols_scale(QtOut& sh, int c, const Side& o, int col0, int mb, int nmb) {
+  float top = 0.f;
+#pragma unroll
+  for (int w = 0; w < 16; w += 2) top = max3(top, sh.part[w][c], sh.part[w + 1][c]);
+  const int byte = scale_byte(top);
+  sh.inv[c] = scale_inv(byte);
+  uint8_t* s = o.scales + scale_at(col0 + c, mb, o.quads);
+  s[0] = (uint8_t)byte;
+  if (mb == nmb - 1)
+    for (int k = 1; k < 4 - (mb & 3); ++k) s[k] = 0;
+}
+__device__ __forceinline__ void qt_cols_codes(Eight<float> (&v)[QT_R], QtOut& sh, int l16) {
+  uint32_t* t = reinterpret_cast<uint32_t*>(sh.t) + (8 * l16) * 32 + ((threadIdx.x >> 4) ^ (2 * l16));
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float2 k = *reinterpret_cast<const float2*>(&sh.inv[8 * l16 + 2 * w]);
+    const float2 a = mul2(v[0].pair(w), k), b = mul2(v[1].pair(w), k), c = mul2(v[2].pair(w), k), d = mul2(v[3].pair(w), k);
+    t[(2 * w) * 32] = codes2(a.x, b.x) | codes2(c.x, d.x) << 16;
+    t[(2 * w + 1) * 32] = codes2(a.y, b.y) | codes2(c.y, d.y) << 16;
+  }
+}
+__device__ __forceinline__ void qt_cols_store(const QtOut& sh, const Side& o, int col0, int mb) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int at = threadIdx.x + k * QT_THREADS, col = at >> 3, quad = at & 7, key = (col >> 3) & 15;
+    uint4 u = sh.t[col * 8 + (quad ^ (key >> 1))];
+    if (key & 1) u = make_uint4(u.z, u.w, u.x, u.y);
+    *reinterpret_cast<uint4*>(o.codes + (long long)(col0 + col) * o.width + mb * TILE + quad * 16) = u;
+  }
+}
+
+// after a wait that ran out: the loads on their way land (or are given up on) before the CTA ends
+template <int N>
+__device__ __forceinline__ void drain(uint64_t* full, int it, int tile, int tiles, int* err) {
+  for (int k = 0; k < N && tile + k * (int)gridDim.x < tiles; ++k)
+    mbar_wait(&full[(it + k) % N], ((it + k) / N) & 1, err, ERR_MBAR_TIMEOUT_EPILOGUE);
+}
+
+template <typename T>
+struct SwigluFwdShared {
+  struct Stage {
+    T a[TILE * TILE], b[TILE * TILE];
+  } stage[QtStages<T>::N];
+  QtOut out;
+  uint64_t full[QtStages<T>::N];
+};
+template <typename T, bool QT, bool CK>
+__global__ void __launch_bounds__(QT_THREADS, 1)
+    swiglu8_fwd_q_kernel(const __grid_constant__ CUtensorMap tm, int M, int H, Side ck, Side g8, Side g8t, int* err) {
+  constexpr int N = QtStages<T>::N;
+  extern __shared__ __align__(128) uint8_t raw[];
+  SwigluFwdShared<T>& sh = *reinterpret_cast<SwigluFwdShared<T>*>(raw);
+  const int nhb = H / TILE, nmb = (M + TILE - 1) / TILE, tiles = nhb * nmb;
+  const int l16 = threadIdx.x & 15, rg = threadIdx.x >> 4;
+  auto fetch = [&](int tile, int s) {
+    const int hb = tile % nhb, mb = tile / nhb;
+    mbar_expect_tx(&sh.full[s], sizeof(sh.stage[s]));
+    tma_load_3d(sh.stage[s].a, &tm, &sh.full[s], hb * TILE, mb * TILE, 0);
+    tma_load_3d(sh.stage[s].b, &tm, &sh.full[s], H + hb * TILE, mb * TILE, 0);
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < N; ++s) mbar_init(&sh.full[s], 1);
+    fence_barrier_init();
+    for (int s = 0; s < N; ++s)
+      if ((int)(blockIdx.x + s * gridDim.x) < tiles) fetch(blockIdx.x + s * gridDim.x, s);
+  }
+  __syncthreads();
+  int it = 0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++it) {
+    const int s = it % N, hb = tile % nhb, mb = tile / nhb, r0 = mb * TILE + QT_R * rg;
+    const bool got = mbar_wait(&sh.full[s], (it / N) & 1, err, ERR_MBAR_TIMEOUT_EPILOGUE);
+    Eight<T> a[QT_R], b[QT_R];
+#pragma unroll
+    for (int i = 0; i < QT_R; ++i) {
+      a[i].fetch(&sh.stage[s].a[(QT_R * rg + i) * TILE + 8 * l16]);
+      b[i].fetch(&sh.stage[s].b[(QT_R * rg + i) * TILE + 8 * l16]);
+    }
+    if (!__syncthreads_and(got)) {  // else the stage has been read
+      if (threadIdx.x == 0) drain<N>(sh.full, it, tile, tiles, err);
+      break;
+    }
+    if (threadIdx.x == 0 && tile + N * (int)gridDim.x < tiles) fetch(tile + N * gridDim.x, s);
+    Eight<float> v[QT_R];
+#pragma unroll
+    for (int i = 0; i < QT_R; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float2 x = a[i].pair(w);
+        v[i].set(w, mul2(mul2(x, make_float2(sigmoid<sizeof(T) == 4>(x.x), sigmoid<sizeof(T) == 4>(x.y))), b[i].pair(w)));
+      }
+    if constexpr (CK) {
+      qt_rows(a, ck, r0, hb, 2 * nhb, l16);
+      qt_rows(b, ck, r0, nhb + hb, 2 * nhb, l16);
+    }
+    qt_rows(v, g8, r0, hb, nhb, l16);
+    if constexpr (QT) {
+      qt_cols_part(v, sh.out, l16);
+      __syncthreads();
+      if (threadIdx.x < TILE) qt_cols_scale(sh.out, threadIdx.x, g8t, hb * TILE, mb, nmb);
+      __syncthreads();
+      qt_cols_codes(v, sh.out, l16);
+      __syncthreads();
+      qt_cols_store(sh.out, g8t, hb * TILE, mb);
+    }
+  }
+}
+
+template <typename T>
+struct SwigluBwdShared {
+  struct Stage {
+    T dg[TILE * TILE];
+    uint8_t a[TILE * TILE], b[TILE * TILE];
+    uint8_t sa[ATOM], sb[ATOM];
+  } stage[QtStages<T>::N];
+  QtOut out[2];
+  uint64_t full[QtStages<T>::N];
+};
+template <typename T>
+__global__ void __launch_bounds__(QT_THREADS, 1)
+    swiglu8_bwd_q_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tmck, int M, int H, Side ck,
+                         Side d8, Side d8t, int* err) {
+  constexpr int N = QtStages<T>::N;
+  extern __shared__ __align__(128) uint8_t raw[];
+  SwigluBwdShared<T>& sh = *reinterpret_cast<SwigluBwdShared<T>*>(raw);
+  const int nhb = H / TILE, nmb = (M + TILE - 1) / TILE, tiles = nhb * nmb;
+  const int l16 = threadIdx.x & 15, rg = threadIdx.x >> 4;
+  auto fetch = [&](int tile, int s) {
+    const int hb = tile % nhb, mb = tile / nhb;
+    auto& st = sh.stage[s];
+    mbar_expect_tx(&sh.full[s], sizeof(st));
+    tma_load_3d(st.dg, &tm, &sh.full[s], hb * TILE, mb * TILE, 0);
+    tma_load_3d(st.a, &tmck, &sh.full[s], hb * TILE, mb * TILE, 0);
+    tma_load_3d(st.b, &tmck, &sh.full[s], H + hb * TILE, mb * TILE, 0);
+    bulk_load(st.sa, ck.scales + ((long long)mb * ck.quads + (hb >> 2)) * ATOM, ATOM, &sh.full[s]);
+    bulk_load(st.sb, ck.scales + ((long long)mb * ck.quads + ((nhb + hb) >> 2)) * ATOM, ATOM, &sh.full[s]);
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < N; ++s) mbar_init(&sh.full[s], 1);
+    fence_barrier_init();
+    for (int s = 0; s < N; ++s)
+      if ((int)(blockIdx.x + s * gridDim.x) < tiles) fetch(blockIdx.x + s * gridDim.x, s);
+  }
+  __syncthreads();
+  int it = 0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++it) {
+    const int s = it % N, hb = tile % nhb, mb = tile / nhb, r0 = mb * TILE + QT_R * rg;
+    const auto& st = sh.stage[s];
+    const bool got = mbar_wait(&sh.full[s], (it / N) & 1, err, ERR_MBAR_TIMEOUT_EPILOGUE);
+    Eight<T> dv[QT_R];
+    uint2 ca[QT_R], cb[QT_R];
+    uint8_t ba[QT_R], bb[QT_R];
+    const int sc = (QT_R * rg & 31) * 16 + (QT_R * rg >> 5) * 4;
+#pragma unroll
+    for (int i = 0; i < QT_R; ++i) {
+      const int at = (QT_R * rg + i) * TILE + 8 * l16;
+      dv[i].fetch(&st.dg[at]);
+      ca[i] = *reinterpret_cast<const uint2*>(&st.a[at]);
+      cb[i] = *reinterpret_cast<const uint2*>(&st.b[at]);
+      ba[i] = st.sa[sc + 16 * i + (hb & 3)];
+      bb[i] = st.sb[sc + 16 * i + ((nhb + hb) & 3)];
+    }
+    if (!__syncthreads_and(got)) {  // else the stage has been read
+      if (threadIdx.x == 0) drain<N>(sh.full, it, tile, tiles, err);
+      break;
+    }
+    if (threadIdx.x == 0 && tile + N * (int)gridDim.x < tiles) fetch(tile + N * gridDim.x, s);
+    Eight<float> va[QT_R], vb[QT_R];
+#pragma unroll
+    for (int i = 0; i < QT_R; ++i) {
+      float2 a[4], b[4];
+      values8(ca[i], scale_of(ba[i]), a);
+      values8(cb[i], scale_of(bb[i]), b);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float2 da, db;
+        swiglu_grad<sizeof(T) == 4>(a[w], b[w], dv[i].pair(w), da, db);
+        va[i].set(w, da);
+        vb[i].set(w, db);
+      }
+    }
+    qt_rows(va, d8, r0, hb, 2 * nhb, l16);
+    qt_rows(vb, d8, r0, nhb + hb, 2 * nhb, l16);
+    qt_cols_part(va, sh.out[0], l16);
+    qt_cols_part(vb, sh.out[1], l16);
+    __syncthreads();
+    if (threadIdx.x < TILE) qt_cols_scale(sh.out[0], threadIdx.x, d8t, hb * TILE, mb, nmb);
+    else if (threadIdx.x < 2 * TILE) qt_cols_scale(sh.out[1], threadIdx.x - TILE, d8t, H + hb * TILE, mb, nmb);
+    __syncthreads();
+    qt_cols_codes(va, sh.out[0], l16);
+    qt_cols_codes(vb, sh.out[1], l16);
+    __syncthreads();
+    qt_cols_store(sh.out[0], d8t, hb * TILE, mb);
+    qt_cols_store(sh.out[1], d8t, H + hb * TILE, mb);
+  }
+}
+
+template <typename K>
+cudaError_t qt_launch(K kern, size_t shared, std::atomic<uint64_t>& set, int* grid, long long tiles) {
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess && (dev > 63 || !((set.load(std::memory_order_relaxed) >> dev) & 1))) {  // once per device
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+    if (e == cudaSuccess && dev <= 63) set.fetch_or(1ull << dev);
+  }
+  *grid = (int)std::min<long long>(tiles, sms);
+  return e;
+}
+template <typename T, bool QT, bool CK>
+cudaError_t swiglu_fwd_q(const CUtensorMap& tm, const Swiglu8Params& p, long long tiles, Side ck, Side g8, Side g8t,
+                         cudaStream_t s) {
+  static std::atomic<uint64_t> set{0};
+  auto kern = swiglu8_fwd_q_kernel<T, QT, CK>;
+  static_assert(sizeof(SwigluFwdShared<T>) <= 232448, "shared memory");
+  int grid = 0;
+  const cudaError_t e = qt_launch(kern, sizeof(SwigluFwdShared<T>), set, &grid, tiles);
+  if (e != cudaSuccess) return e;
+  kern<<<grid, QT_THREADS, sizeof(SwigluFwdShared<T>), s>>>(tm, p.M, p.H, ck, g8, g8t, p.err);
+  return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t swiglu_fwd_typed(const Swiglu8Params& p, cudaStream_t s) {
   const int nhb = (p.H + TILE - 1) / TILE;
-  const long long tiles = (long long)nhb * ((p.M + TILE - 1) / TILE);
-  if (tiles >= (1ll << 31)) return cudaErrorInvalidValue;
-  const bool vec = p.H % 8 == 0 && aligned16(p.ab, p.ld * (long long)sizeof(T));
-  const bool vec_g = p.H % 8 == 0 && aligned16(p.g, 0);
   const Side ck = side(p.ck, p.ck_scales, p.M, 2 * nhb * TILE), g8 = side(p.g8, p.g8_scales, p.M, p.H),
              g8t = side(p.g8t, p.g8t_scales, p.H, p.M);
+  if (p.g8 != nullptr) {
+    const long long tiles = (long long)nhb * ((p.M + TILE - 1) / TILE);
+    if (tiles >= (1ll << 30) || p.map == nullptr) return cudaErrorInvalidValue;
+    if (p.g8t != nullptr)
+      return p.ck != nullptr ? swiglu_fwd_q<T, true, true>(*p.map, p, tiles, ck, g8, g8t, s)
+                             : swiglu_fwd_q<T, true, false>(*p.map, p, tiles, ck, g8, g8t, s);
+    return p.ck != nullptr ? swiglu_fwd_q<T, false, true>(*p.map, p, tiles, ck, g8, g8t, s)
+                           : swiglu_fwd_q<T, false, false>(*p.map, p, tiles, ck, g8, g8t, s);
+  }
+  const long long blocks = (long long)nhb * ((p.M + 63) / 64);
+  if (blocks >= (1ll << 31)) return cudaErrorInvalidValue;
+  const bool vec = p.H % 8 == 0 && aligned16(p.ab, p.ld * (long long)sizeof(T));
+  const bool vec_g = p.H % 8 == 0 && aligned16(p.g, 0);
   const T* ab = static_cast<const T*>(p.ab);
   T* g = static_cast<T*>(p.g);
-  if (p.g8 != nullptr)
-    swiglu8_fwd_kernel<T, false, true><<<(int)tiles, PACK_THREADS, 0, s>>>(ab, p.ld, p.M, p.H, vec, vec_g, g, ck, g8, g8t);
-  else
-    swiglu8_fwd_kernel<T, true, false><<<(int)tiles, PACK_THREADS, 0, s>>>(ab, p.ld, p.M, p.H, vec, vec_g, g, ck, g8, g8t);
+  if (p.ck != nullptr) swiglu8_fwd_kernel<T, true><<<(int)blocks, 256, 0, s>>>(ab, p.ld, p.M, p.H, vec, vec_g, g, ck);
+  else swiglu8_fwd_kernel<T, false><<<(int)blocks, 256, 0, s>>>(ab, p.ld, p.M, p.H, vec, vec_g, g, ck);
   return cudaGetLastError();
 }
 template <typename T>
 cudaError_t swiglu_bwd_typed(const Swiglu8BwdParams& p, cudaStream_t s) {
   const int nhb = (p.H + TILE - 1) / TILE;
-  const long long tiles = (long long)nhb * ((p.M + TILE - 1) / TILE);
-  if (tiles >= (1ll << 31)) return cudaErrorInvalidValue;
-  const bool vec = p.H % 8 == 0 && aligned16(p.dg, p.ld * (long long)sizeof(T));
-  const bool vec_d = p.H % 8 == 0 && aligned16(p.dab, 0);
   const Side ck = side(const_cast<uint8_t*>(p.ck), const_cast<uint8_t*>(p.ck_scales), p.M, 2 * nhb * TILE),
              d8 = side(p.d8, p.d8_scales, p.M, 2 * p.H), d8t = side(p.d8t, p.d8t_scales, 2 * p.H, p.M);
-  const T* dg = static_cast<const T*>(p.dg);
-  T* dab = static_cast<T*>(p.dab);
-  if (p.d8 != nullptr)
-    swiglu8_bwd_kernel<T, false, true><<<(int)tiles, PACK_THREADS, 0, s>>>(dg, p.ld, p.M, p.H, vec, vec_d, dab, ck, d8, d8t);
-  else
-    swiglu8_bwd_kernel<T, true, false><<<(int)tiles, PACK_THREADS, 0, s>>>(dg, p.ld, p.M, p.H, vec, vec_d, dab, ck, d8, d8t);
+  if (p.d8 != nullptr) {
+    const long long tiles = (long long)nhb * ((p.M + TILE - 1) / TILE);
+    if (tiles >= (1ll << 30) || p.map == nullptr || p.ck_map == nullptr) return cudaErrorInvalidValue;
+    static std::atomic<uint64_t> set{0};
+    auto kern = swiglu8_bwd_q_kernel<T>;
+    static_assert(sizeof(SwigluBwdShared<T>) <= 232448, "shared memory");
+    int grid = 0;
+    const cudaError_t e = qt_launch(kern, sizeof(SwigluBwdShared<T>), set, &grid, tiles);
+    if (e != cudaSuccess) return e;
+    kern<<<grid, QT_THREADS, sizeof(SwigluBwdShared<T>), s>>>(*p.map, *p.ck_map, p.M, p.H, ck, d8, d8t, p.err);
+    return cudaGetLastError();
+  }
+  const long long blocks = (long long)nhb * ((p.M + 63) / 64);
+  if (blocks >= (1ll << 31)) return cudaErrorInvalidValue;
+  const bool vec = p.H % 8 == 0 && aligned16(p.dg, p.ld * (long long)sizeof(T));
+  const bool vec_d = p.H % 8 == 0 && aligned16(p.dab, 0);
+  swiglu8_bwd_kernel<T><<<(int)blocks, 256, 0, s>>>(static_cast<const T*>(p.dg), p.ld, p.M, p.H, vec, vec_d,
+                                                    static_cast<T*>(p.dab), ck);
   return cudaGetLastError();
 }
 
@@ -480,13 +908,18 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const FewRowsParams p, bo
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int m = 8 * i + g;
-      float f[4][8];  // columns 16 t .. + 15 and 64 + 16 t .. + 15 of the block
+      Eight<T> f[4];  // columns 16 t .. + 15 and 64 + 16 t .. + 15 of the block
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const int c = kb * TILE + (h >> 1) * 64 + 16 * t + (h & 1) * 8;
-        load8<T>(x + m * p.ldx + c, m < p.M ? max(0, min(8, p.K - c)) : 0, vec, f[h]);
+        f[h].load(x + m * p.ldx + c, m < p.M ? max(0, min(8, p.K - c)) : 0, vec);
       }
-      float top = fmaxf(fmaxf(finite_top8(f[0]), finite_top8(f[1])), fmaxf(finite_top8(f[2]), finite_top8(f[3])));
+      float top = fmaxf(fmaxf(f[0].top(), f[1].top()), fmaxf(f[2].top(), f[3].top()));
+      if (top == INFINITY) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) f[h].drop_infinities();
+        top = fmaxf(fmaxf(f[0].top(), f[1].top()), fmaxf(f[2].top(), f[3].top()));
+      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int byte = scale_byte(top);

@@ -44,10 +44,14 @@ struct Gemm8Params {
   int c_tma;                // C goes through its tensor map
   int* err;
 };
-constexpr int kGemm8Tile = 128;  // rows of A's box
-// ta / tb: uint8 maps {Kp, rows, 1} with boxes {128, 128 or bn, 1}, 128-byte swizzle; tc: {N, M, 1}, box {32, 32, 1}
-cudaError_t gemm8_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Gemm8Params& p, int bn,
-                         int out, cudaStream_t s);
+enum Gemm8Tile : int { TILE_128x128 = 0, TILE_PAIR_192 = 1, TILE_PAIR_256 = 2 };  // pairs of CTAs: 256 x 192, 256 x 256
+// a, b: uint8 maps {Kp, rows, 1} with boxes {128, 128, 1} (b of TILE_PAIR_192: {128, 96, 1}), 128-byte swizzle; c: {N, M, 1},
+// box {32, 32, 1}; sa, sb (pairs alone): the scale atoms as 32-bit words {128, ceil(kb / 4), row tiles}, boxes {128, 1, 1}
+// and {128, 1, 2}
+struct Gemm8Maps {
+  CUtensorMap a, b, c, sa, sb;
+};
+cudaError_t gemm8_launch(const Gemm8Maps& t, const Gemm8Params& p, Gemm8Tile tile, int out, cudaStream_t s);
 
 // y [M, N] = Q(x) W^T + bias for few rows, x packed on the way (one launch)
 constexpr int kFewRows = 16;
@@ -62,7 +66,7 @@ struct FewRowsParams {
 };
 cudaError_t few_rows_launch(const FewRowsParams& p, int elem, cudaStream_t s);
 
-// SwiGLU over ab [M, 2 H] (rows ld apart), H a multiple of 128 unless only g and the checkpoint are wanted
+// SwiGLU over ab [M, 2 H] (rows ld apart). With g8: H a multiple of 128 and map: ab {2 H, M, 1} in its type, box {128, 128, 1}
 struct Swiglu8Params {
   const void* ab;
   long long ld;
@@ -74,6 +78,8 @@ struct Swiglu8Params {
   uint8_t* g8_scales;
   uint8_t* g8t;             // [H, Mp] blocks along M, or null
   uint8_t* g8t_scales;
+  const CUtensorMap* map;
+  int* err;
 };
 cudaError_t swiglu8_fwd_launch(const Swiglu8Params& p, int elem, cudaStream_t s);
 struct Swiglu8BwdParams {
@@ -87,6 +93,9 @@ struct Swiglu8BwdParams {
   uint8_t* d8_scales;
   uint8_t* d8t;             // [2 H, Mp]
   uint8_t* d8t_scales;
+  const CUtensorMap* map;     // with d8: dg {H, M, 1} in its type and ck {2 H, M, 1} as bytes, boxes {128, 128, 1}
+  const CUtensorMap* ck_map;
+  int* err;
 };
 cudaError_t swiglu8_bwd_launch(const Swiglu8BwdParams& p, int elem, cudaStream_t s);
 

@@ -5,6 +5,8 @@
 #include <cudaTypedefs.h>
 #include <torch/extension.h>
 
+#include <atomic>
+
 #include "blocks8.h"
 #include "torch_util.h"
 
@@ -125,6 +127,36 @@ bool out_map(CUtensorMap* m, const at::Tensor& C, int64_t ldc) {
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+CUtensorMap scales_map(const Packed& a, uint32_t box_tiles) {
+  CUtensorMap m;
+  const uint64_t quads = up(a.blocks(), 4);
+  cuuint64_t dims[3] = {128, quads, (cuuint64_t)up(a.rows, 128)};
+  cuuint64_t strides[2] = {512, quads * 512};
+  cuuint32_t box[3] = {128, 1, box_tiles};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = tmap_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, a.s(), dims, strides, box, estr,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "tensor map of 8-bit scales: code ", (int)r);
+  return m;
+}
+
+// The tile whose waves over the GPU take the fewest cycles: a block of 128 costs 480 (128 x 128, bound by its loads; 380 where
+// they do not fill the GPU), 430 (256 x 192, loads) or 512 (256 x 256, the products), a sum's beginning and end 300, 800 or
+// 2600 (its accumulators share columns).
+// Measured at 32768 x 6144 x 2048: 436, 287 and 305 us; x 2048 x 6144: 418, 281 and 264 us; 2047 x 777 x 1000: 17, 21 and 26 us.
+std::atomic<int> g_tile{-1};  // for comparisons of the variants: -1 chooses
+Gemm8Tile tile_of(const Gemm8Params& p) {
+  if (g_tile >= 0) return (Gemm8Tile)g_tile.load();
+  const int64_t sms = num_sms(), sums = up(p.kb, p.chunk_kb);
+  const int64_t tiles = up(p.M, 128) * up(p.N, 128);
+  const int64_t one = up(tiles, sms) * (p.kb * (tiles > sms ? 480 : 380) + sums * 300);
+  const int64_t p192 = up(up(p.M, 256) * up(p.N, 192), sms / 2) * (p.kb * 430 + sums * 800);
+  const int64_t p256 = up(up(p.M, 256) * up(p.N, 256), sms / 2) * (p.kb * 512 + sums * 2600);
+  if (one <= p192 && one <= p256) return TILE_128x128;
+  return p192 <= p256 ? TILE_PAIR_192 : TILE_PAIR_256;
+}
+
 // C [M, N] (+)= a b^T (+ bias)
 void product(const Packed& a, const Packed& b, const at::Tensor& C, const float* bias, bool add, int* err) {
   TORCH_CHECK(a.cols == b.cols, "gemm_blocks: sums over ", a.cols, " and ", b.cols);
@@ -149,13 +181,16 @@ void product(const Packed& a, const Packed& b, const at::Tensor& C, const float*
   // The tensor core's fp32 sums drop what does not fit their 24 bits instead of rounding: a sum of one sign over 32768
   // lost 3.6e-5 of itself, 1.3e-6 over 4096. Sums that are returned in fp32 are joined from parts of 4096.
   p.chunk_kb = out == OUT_F32 ? 32 : (int)up(p.kb, 4) * 4;
-  CUtensorMap tc;
-  p.c_tma = out_map(&tc, C, p.ldc);
-  // 128 x 256 tiles where they fill the GPU, else twice as many of 128 x 128
-  const int bn = up(p.M, 128) * up(p.N, 256) >= num_sms() ? 256 : 128;
-  const CUtensorMap ta = codes_map(a, kGemm8Tile), tb = codes_map(b, bn);
-  if (!p.c_tma) tc = ta;
-  BLOCK_LAUNCH(gemm8_launch(ta, tb, tc, p, bn, out, at::cuda::getCurrentCUDAStream()), 1);
+  Gemm8Maps t;
+  p.c_tma = out_map(&t.c, C, p.ldc);
+  const Gemm8Tile tile = tile_of(p);
+  t.a = codes_map(a, 128);
+  t.b = codes_map(b, tile == TILE_PAIR_192 ? 96 : 128);
+  if (tile != TILE_128x128) {
+    t.sa = scales_map(a, 1);
+    t.sb = scales_map(b, 2);
+  }
+  BLOCK_LAUNCH(gemm8_launch(t, p, tile, out, at::cuda::getCurrentCUDAStream()), 1);
 }
 
 void small_vector(const OptT& bias, int64_t n, const at::Tensor& as, const char* what) {
@@ -359,7 +394,25 @@ at::Tensor linear8(at::Tensor x, at::Tensor w, OptT bias, at::Tensor err) {
 }
 
 // ----------------------------------------------------------------------------------------------------------- SwiGLU
-void swiglu_forward(const at::Tensor& ab, at::Tensor* g, Packed* ck, Packed* g8, Packed* g8t) {
+// plain {cols, rows, 1} map with a {128, 128, 1} box
+CUtensorMap tile_map(const void* base, CUtensorMapDataType type, uint64_t size, uint64_t cols, uint64_t rows, uint64_t ld) {
+  CUtensorMap m;
+  cuuint64_t dims[3] = {cols, rows, 1};
+  cuuint64_t strides[2] = {ld * size, ld * size * rows};
+  cuuint32_t box[3] = {128, 128, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = tmap_encoder()(&m, type, 3, const_cast<void*>(base), dims, strides, box, estr,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "tensor map of activations: code ", (int)r);
+  return m;
+}
+CUtensorMap tile_map(const at::Tensor& t) {
+  const auto type = t.scalar_type() == at::kFloat  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                    : t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return tile_map(t.data_ptr(), type, t.element_size(), t.size(1), t.size(0), t.size(1));
+}
+void swiglu_forward(const at::Tensor& ab, at::Tensor* g, Packed* ck, Packed* g8, Packed* g8t, int* err) {
   const int64_t M = ab.size(0), H = ab.size(1) / 2, Hp = up(H, 128) * 128;
   if (g != nullptr) *g = fresh({M, H}, ab.scalar_type(), ab);
   if (ck != nullptr) *ck = fresh_packed(M, 2 * Hp, ab);
@@ -375,9 +428,15 @@ void swiglu_forward(const at::Tensor& ab, at::Tensor* g, Packed* ck, Packed* g8,
   if (ck != nullptr) p.ck = ck->c(), p.ck_scales = ck->s();
   if (g8 != nullptr) p.g8 = g8->c(), p.g8_scales = g8->s();
   if (g8t != nullptr) p.g8t = g8t->c(), p.g8t_scales = g8t->s();
+  CUtensorMap map;
+  if (g8 != nullptr) {  // ab is the contiguous output of a product
+    map = tile_map(ab);
+    p.map = &map;
+    p.err = err;
+  }
   BLOCK_LAUNCH(swiglu8_fwd_launch(p, elem_of(ab, "swiglu_blocks"), at::cuda::getCurrentCUDAStream()), 1);
 }
-void swiglu_backward(const at::Tensor& dg, const Packed& ck, int64_t H, at::Tensor* dab, Packed* d8, Packed* d8t) {
+void swiglu_backward(const at::Tensor& dg, const Packed& ck, int64_t H, at::Tensor* dab, Packed* d8, Packed* d8t, int* err) {
   const int64_t M = dg.size(0);
   if (dab != nullptr) *dab = fresh({M, 2 * H}, dg.scalar_type(), dg);
   if (d8 != nullptr) *d8 = fresh_packed(M, 2 * H, dg);
@@ -393,6 +452,14 @@ void swiglu_backward(const at::Tensor& dg, const Packed& ck, int64_t H, at::Tens
   if (dab != nullptr) p.dab = dab->data_ptr();
   if (d8 != nullptr) p.d8 = d8->c(), p.d8_scales = d8->s();
   if (d8t != nullptr) p.d8t = d8t->c(), p.d8t_scales = d8t->s();
+  CUtensorMap map, ck_map;
+  if (d8 != nullptr) {  // dg is the contiguous output of a product
+    map = tile_map(dg);
+    ck_map = tile_map(p.ck, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 2 * H, M, 2 * H);
+    p.map = &map;
+    p.ck_map = &ck_map;
+    p.err = err;
+  }
   BLOCK_LAUNCH(swiglu8_bwd_launch(p, elem_of(dg, "swiglu_blocks"), at::cuda::getCurrentCUDAStream()), 1);
 }
 
@@ -401,7 +468,7 @@ struct Swiglu8Fn : public torch::autograd::Function<Swiglu8Fn> {
     at::AutoDispatchBelowADInplaceOrView below;
     at::Tensor g;
     Packed ck;
-    swiglu_forward(ab, &g, &ck, nullptr, nullptr);
+    swiglu_forward(ab, &g, &ck, nullptr, nullptr, nullptr);
     ctx->save_for_backward({ck.codes, ck.scales});
     return g;
   }
@@ -411,7 +478,7 @@ struct Swiglu8Fn : public torch::autograd::Function<Swiglu8Fn> {
     const at::Tensor dg = rows_of(grads[0]);
     const c10::cuda::CUDAGuard guard(dg.device());
     at::Tensor dab;
-    swiglu_backward(dg, kept(saved, 0, saved[0].size(1)), dg.size(1), &dab, nullptr, nullptr);
+    swiglu_backward(dg, kept(saved, 0, saved[0].size(1)), dg.size(1), &dab, nullptr, nullptr, nullptr);
     return {dab};
   }
 };
@@ -423,7 +490,7 @@ at::Tensor swiglu8(at::Tensor ab) {
   ab = rows_of(ab);
   if (wants_grad({&ab}, kWhat)) return Swiglu8Fn::apply(ab);
   at::Tensor g;
-  swiglu_forward(ab, &g, nullptr, nullptr, nullptr);
+  swiglu_forward(ab, &g, nullptr, nullptr, nullptr, nullptr);
   return g;
 }
 
@@ -440,7 +507,7 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
     {
       at::Tensor ab = fresh({x.size(0), w1.size(0)}, x.scalar_type(), x);
       product(xr, w1r, ab, nullptr, false, e);
-      swiglu_forward(ab, nullptr, up_too ? &ck : nullptr, &g8, dw2 ? &g8t : nullptr);
+      swiglu_forward(ab, nullptr, up_too ? &ck : nullptr, &g8, dw2 ? &g8t : nullptr, e);
     }
     at::Tensor y = fresh({x.size(0), w2.size(0)}, x.scalar_type(), x);
     product(g8, w2r, y, nullptr, false, e);
@@ -480,7 +547,7 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
       {
         at::Tensor dg = fresh({M, H}, dy.scalar_type(), dy);
         product(dyr, w2t, dg, nullptr, false, e);
-        swiglu_backward(dg, kept(saved, 6, 2 * H), H, nullptr, &d8, &d8t);
+        swiglu_backward(dg, kept(saved, 6, 2 * H), H, nullptr, &d8, &d8t, e);
       }
       if (dx) {
         const Packed w1t = kept(saved, 2, 2 * H);
@@ -521,7 +588,7 @@ at::Tensor mlp8(at::Tensor x, at::Tensor w1, at::Tensor w2, at::Tensor err) {
   int* const e = err_word(err, x);
   at::Tensor ab = fresh({x.size(0), w1.size(0)}, x.scalar_type(), x), y = fresh({x.size(0), w2.size(0)}, x.scalar_type(), x);
   product(xr, w1r, ab, nullptr, false, e);
-  swiglu_forward(ab, nullptr, nullptr, &g8, nullptr);
+  swiglu_forward(ab, nullptr, nullptr, &g8, nullptr, e);
   product(g8, w2r, y, nullptr, false, e);
   return y;
 }
@@ -537,6 +604,10 @@ void bind_blocks8(pybind11::module_& m) {
                     OptT bias, bool add, at::Tensor err) {
     return gemm8(a, as, b, bs, cols, torch::python::detail::py_object_to_dtype(dtype), out, bias, add, err);
   }, "C (+)= a b^T (+ bias) of packed matrices");
+  m.def("set_gemm8_tile", [](int64_t t) {
+    TORCH_CHECK(t >= -1 && t <= 2, "set_gemm8_tile: -1 (chosen by size), 0 (128 x 128), 1 (256 x 192), 2 (256 x 256)");
+    g_tile = (int)t;
+  }, "tile of the 8-bit products (A/B runs)");
   m.def("linear8_frozen", &linear8_frozen, "x times a weight held in 8 bits");
   m.def("linear8", &linear8, "linear layer on 8-bit products, forward and backward");
   m.def("swiglu8", &swiglu8, "silu(a) b with its input kept in 8 bits for the backward");

@@ -10,6 +10,7 @@
 // the whole sum is there. A scale atom (128 rows x 4 blocks, 512 bytes) goes from shared to tensor memory with one copy
 // every fourth block.
 #include <algorithm>
+#include <atomic>
 
 #include "blocks8.h"
 #include "common.cuh"
@@ -23,16 +24,20 @@ namespace {
 constexpr int BM = 128, BK = 128, THREADS = 192;
 constexpr int ATOM = 512;
 
-template <int BN>
+// Two CTAs of a cluster share a tile of 256 x BN (PAIR, cta_group::2): each loads 128 rows of A and half of B's, so a block
+// of k moves 32 KB (BN 256) or 28 KB (BN 192) into an SM in the 512 or 384 cycles that its products take. An SM takes in some
+// 64 bytes a cycle while all do: one CTA with 128 x 256 (48 KB) ran at 2.4 PFLOP/s where the pairs reach 2.9 to 3.1.
+template <int BN, bool PAIR>
 struct Cfg {
-  static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
+  static constexpr int A_BYTES = BM * BK, B_ROWS = PAIR ? BN / 2 : BN, B_BYTES = B_ROWS * BK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 4 : 6;
-  static constexpr int SF_BYTES = (1 + BN / 128) * ATOM;  // of a stage: A's atom, B's atoms
+  static constexpr int STAGES = STAGE_BYTES == 32768 ? 6 : 7;
+  static constexpr int B_ATOMS = (BN + 127) / 128;         // a tile of 192 begins at the start or the middle of an atom
+  static constexpr int SF_BYTES = (1 + B_ATOMS) * ATOM;    // of a stage: A's atom, B's atoms
   static constexpr int C_STAGE = 4096;                    // epilogue staging of one warp
-  static constexpr int SMEM = 1024 + STAGES * (STAGE_BYTES + SF_BYTES) + 4 * C_STAGE;
+  static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + ((STAGES * SF_BYTES + 1023) & ~1023) + 4 * C_STAGE;
   // Tensor memory (512 columns): two accumulators and the scale factors. Two of 256 columns leave no room, so they share
-  // 16 columns, which the epilogue reads first.
+  // 16 columns, which the epilogue reads first: the next sum waits for that, some 2600 cycles a tile.
   static constexpr int ACC1 = BN == 256 ? 240 : BN;
   static constexpr int SFA = 496, SFB = 500;
 };
@@ -41,18 +46,31 @@ struct Cfg {
 __device__ __forceinline__ constexpr uint32_t idesc_mx(int M, int N, uint32_t sf) {
   return (sf << 4) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27) | (sf << 29);
 }
+template <bool PAIR>
 __device__ __forceinline__ void umma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
+#define UMMA_MX(CTAS)                                                                                                     \
+  asm volatile(                                                                                                           \
+      "{\n\t.reg .pred p;\n\t"                                                                                           \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                                         \
+      "tcgen05.mma.cta_group::" CTAS ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d), \
+      "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                                    \
+      : "memory")
+  if constexpr (PAIR) UMMA_MX("2");
+  else UMMA_MX("1");
+#undef UMMA_MX
 }
 // one atom, 32 rows of 16 bytes: four columns, the same in every quarter of the lanes
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {  // a pair: in both CTAs, each from its own
+  if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// arrives once on the barrier (a pair: on both CTAs') when what this thread has issued is done
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (PAIR) umma_commit_pair_mc(bar, 0x3);
+  else umma_commit(bar);
 }
 // shared-memory descriptor without swizzle: groups of 8 rows of 16 bytes, 128 bytes apart
 __device__ __forceinline__ uint64_t sdesc_plain(uint32_t saddr) {
@@ -94,26 +112,28 @@ __device__ __forceinline__ void store_one(void* C, long long at, float v, bool a
   }
 }
 
-template <int BN, int OUT>
+template <int BN, int OUT, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 const __grid_constant__ CUtensorMap tmC, const Gemm8Params p) {
-  using F = Cfg<BN>;
-  constexpr int STAGES = F::STAGES;
+                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmSA,
+                 const __grid_constant__ CUtensorMap tmSB, const Gemm8Params p) {
+  using F = Cfg<BN, PAIR>;
+  constexpr int STAGES = F::STAGES, TM = PAIR ? 2 * BM : BM, EPI_WARPS = PAIR ? 8 : 4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const smem_sf = smem + STAGES * F::STAGE_BYTES;
-  uint8_t* const smem_c = smem_sf + STAGES * F::SF_BYTES;
+  uint8_t* const smem_c = smem + STAGES * F::STAGE_BYTES + ((STAGES * F::SF_BYTES + 1023) & ~1023);
   __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], tfull_bar[2], tempty_bar[2], done_bar;
   __shared__ uint32_t tmem_base_sh;
   __shared__ volatile int abort_sh;
 
   const int warp = warp_id(), lane = lane_id();
-  const int num_m = (p.M + BM - 1) / BM, num_n = (p.N + BN - 1) / BN;
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const bool leader = rank == 0;  // issues the pair's products; its barriers count both CTAs' loads and epilogues
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int num_m = (p.M + TM - 1) / TM, num_n = (p.N + BN - 1) / BN;
   const int num_tiles = num_m * num_n;
   const int chunks = (p.kb + p.chunk_kb - 1) / p.chunk_kb;
-  const int kq = (p.kb + 3) / 4;       // scale atoms of a row tile
-  const int nbt = (p.N + 127) / 128;   // row tiles of B's scales
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -122,7 +142,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], 4);
+      mbar_init(&tempty_bar[a], EPI_WARPS);
     }
     mbar_init(&done_bar, 1);
     abort_sh = 0;
@@ -131,103 +151,146 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
+    if constexpr (PAIR) prefetch_tmap(&tmSA), prefetch_tmap(&tmSB);
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_base_sh, 512);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(&tmem_base_sh, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&tmem_base_sh, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the peer's barriers are there before anything arrives on them
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_sh;
 
+  // The two warps that feed the tensor core run as whole warps and elect a lane where an instruction wants one thread: the
+  // operands then stay in uniform registers. With one lane in the loop each product cost its thread some 70 cycles of moving
+  // operands, and the thread, not the tensor core, was the bound (690 cycles for a block of 4 x 128).
   if (warp == 0) {
-    if (lane == 0) {
-      // ---------------- loads ----------------
-      int stage = 0, filled = 0;
-      uint32_t phase = 0;
-      for (int tile = blockIdx.x; tile < num_tiles && !abort_sh; tile += gridDim.x) {
-        const int mt = tile / num_n, nt = tile % num_n;
-        for (int kb = 0; kb < p.kb; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, p.err, ERR_MBAR_TIMEOUT_PRODUCER)) {
-            abort_sh = 1;
-            break;
-          }
+    // ---------------- loads ----------------
+    const int kq = (p.kb + 3) / 4;      // scale atoms of a row tile
+    const int nbt = (p.N + 127) / 128;  // row tiles of B's scales
+    int stage = 0, filled = 0;
+    uint32_t phase = 0;
+    bool free = true, ok = true;  // free: the stage is known to be free
+    for (int tile = first; tile < num_tiles && ok; tile += step) {
+      const int mt = tile / num_n, nt = tile % num_n;
+      const int m0 = mt * TM + rank * BM, n0 = nt * BN + rank * F::B_ROWS;
+      for (int kb = 0; kb < p.kb; ++kb) {
+        if (!free) {
+          ok = __all_sync(0xffffffffu, mbar_wait_poll(&empty_bar[stage], phase ^ 1, p.err, ERR_MBAR_TIMEOUT_PRODUCER) &&
+                                           !abort_sh);
+          if (!ok) break;
+        }
+        const int next = stage + 1 == STAGES ? 0 : stage + 1;
+        const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
+        free = __all_sync(0xffffffffu, mbar_test_wait(&empty_bar[next], next_phase ^ 1));
+        if (elect_one()) {
           uint8_t* sa = smem + stage * F::STAGE_BYTES;
           uint8_t* sf = smem_sf + stage * F::SF_BYTES;
           const bool scales = (kb & 3) == 0;
-          const int nb = min(BN / 128, nbt - nt * (BN / 128));
-          mbar_expect_tx(&full_bar[stage], F::STAGE_BYTES + (scales ? (1 + nb) * ATOM : 0));
-          tma_load_3d(sa, &tmA, &full_bar[stage], kb * BK, mt * BM, 0);
-          tma_load_3d(sa + F::A_BYTES, &tmB, &full_bar[stage], kb * BK, nt * BN, 0);
-          if (scales) {
-            bulk_load(sf, p.sfa + ((long long)mt * kq + (kb >> 2)) * ATOM, ATOM, &full_bar[stage]);
-            for (int i = 0; i < nb; ++i)
-              bulk_load(sf + (1 + i) * ATOM, p.sfb + ((long long)(nt * (BN / 128) + i) * kq + (kb >> 2)) * ATOM, ATOM,
-                        &full_bar[stage]);
-          }
-          filled = min(filled + 1, STAGES);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
+          if constexpr (PAIR) {
+            if (leader) mbar_expect_tx(&full_bar[stage], 2 * (F::STAGE_BYTES + (scales ? F::SF_BYTES : 0)));
+            const uint32_t bar = mapa_shared(smem_u32(&full_bar[stage]), 0);
+            tma_load_3d_pair(sa, &tmA, bar, kb * BK, m0, 0);
+            tma_load_3d_pair(sa + F::A_BYTES, &tmB, bar, kb * BK, n0, 0);
+            if (scales) {
+              tma_load_3d_pair(sf, &tmSA, bar, 0, kb >> 2, mt * 2 + rank);
+              tma_load_3d_pair(sf + ATOM, &tmSB, bar, 0, kb >> 2, nt * BN / 128);
+            }
+          } else {
+            const int nb = min(F::B_ATOMS, nbt - nt * (BN / 128));
+            mbar_expect_tx(&full_bar[stage], F::STAGE_BYTES + (scales ? (1 + nb) * ATOM : 0));
+            tma_load_3d(sa, &tmA, &full_bar[stage], kb * BK, m0, 0);
+            tma_load_3d(sa + F::A_BYTES, &tmB, &full_bar[stage], kb * BK, n0, 0);
+            if (scales) {
+              bulk_load(sf, p.sfa + ((long long)mt * kq + (kb >> 2)) * ATOM, ATOM, &full_bar[stage]);
+              for (int i = 0; i < nb; ++i)
+                bulk_load(sf + (1 + i) * ATOM, p.sfb + ((long long)(nt * (BN / 128) + i) * kq + (kb >> 2)) * ATOM, ATOM,
+                          &full_bar[stage]);
+            }
           }
         }
-      }
-      // the last loads have landed before the block ends, also after a wait that ran out
-      for (int i = 0; i < filled; ++i) {
-        stage = stage == 0 ? STAGES - 1 : stage - 1;
-        if (stage == STAGES - 1) phase ^= 1;
-        if (!mbar_wait(&full_bar[stage], phase, p.err, ERR_MBAR_TIMEOUT_PRODUCER)) break;
+        __syncwarp();
+        filled = min(filled + 1, STAGES);
+        stage = next;
+        phase = next_phase;
       }
     }
+    if (!ok) abort_sh = 1;
+    // the last loads have landed before the block (the pair) ends, also after a wait that ran out
+    for (int i = 0; i < filled && leader; ++i) {
+      stage = stage == 0 ? STAGES - 1 : stage - 1;
+      if (stage == STAGES - 1) phase ^= 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, p.err, ERR_MBAR_TIMEOUT_PRODUCER))) break;
+    }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (leader) {
       // ---------------- products ----------------
       const uint64_t a0 = sdesc_sw128(smem_u32(smem), 16, 1024), b0 = sdesc_sw128(smem_u32(smem) + F::A_BYTES, 16, 1024);
       const uint64_t s0 = sdesc_plain(smem_u32(smem_sf));
       const uint32_t sfa = tmem_base + F::SFA, sfb = tmem_base + F::SFB;
+      // a look at the next block's barrier comes before this block's products
       int stage = 0, unit = 0;
       uint32_t phase = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      bool ok = true, ready = false;
+      for (int tile = first; tile < num_tiles && ok; tile += step) {
         for (int c = 0; c < chunks && ok; ++c, ++unit) {
           // accumulators that share columns: the unit before has given up its shared ones; else: the one before that
           // has been read
           constexpr int back = BN == 256 ? 1 : 2;
           if (unit >= back) {
             const int u = unit - back;
-            ok = !abort_sh && mbar_wait(&tempty_bar[u & 1], (u >> 1) & 1, p.err, ERR_MBAR_TIMEOUT_MMA);
+            ok = __all_sync(0xffffffffu, mbar_wait_poll(&tempty_bar[u & 1], (u >> 1) & 1, p.err, ERR_MBAR_TIMEOUT_MMA) &&
+                                             !abort_sh);
             if (!ok) break;
           }
           tc_fence_after();
           const uint32_t d = tmem_base + ((unit & 1) ? F::ACC1 : 0);
+          const uint32_t sfb_n = sfb + (BN % 128 != 0 && (tile % num_n & 1) ? 2 : 0);  // 64 columns into the first atom
           const int k0 = c * p.chunk_kb, k1 = min(p.kb, k0 + p.chunk_kb);
           for (int kb = k0; kb < k1; ++kb) {
-            ok = !abort_sh && mbar_wait(&full_bar[stage], phase, p.err, ERR_MBAR_TIMEOUT_MMA);
-            if (!ok) break;
+            if (!ready) {
+              ok = __all_sync(0xffffffffu, mbar_wait_poll(&full_bar[stage], phase, p.err, ERR_MBAR_TIMEOUT_MMA) && !abort_sh);
+              if (!ok) break;
+            }
+            const int next = stage + 1 == STAGES ? 0 : stage + 1;
+            const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
+            ready = __all_sync(0xffffffffu, mbar_test_wait(&full_bar[next], next_phase));
             tc_fence_after();
-            if ((kb & 3) == 0) {
-              const uint64_t s = sdesc_add(s0, stage * F::SF_BYTES);
+            if (elect_one()) {
+              if ((kb & 3) == 0) {
+                const uint64_t s = sdesc_add(s0, stage * F::SF_BYTES);
 #pragma unroll
-              for (int i = 0; i <= BN / 128; ++i) copy_scales(i == 0 ? sfa : sfb + (i - 1) * 4, sdesc_add(s, i * ATOM));
-            }
-            const uint64_t a = sdesc_add(a0, stage * F::STAGE_BYTES), b = sdesc_add(b0, stage * F::STAGE_BYTES);
-            const uint32_t id = idesc_mx(BM, BN, kb & 3);
+                for (int i = 0; i <= F::B_ATOMS; ++i)
+                  copy_scales<PAIR>(i == 0 ? sfa : sfb + (i - 1) * 4, sdesc_add(s, i * ATOM));
+              }
+              const uint64_t a = sdesc_add(a0, stage * F::STAGE_BYTES), b = sdesc_add(b0, stage * F::STAGE_BYTES);
+              const uint32_t id = idesc_mx(TM, BN, kb & 3);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) umma_mx(d, a + 2 * k, b + 2 * k, id, sfa, sfb, (kb != k0 || k != 0) ? 1u : 0u);
-            umma_commit(&empty_bar[stage]);
-            if (++stage == STAGES) {
-              stage = 0;
-              phase ^= 1;
+              for (int k = 0; k < 4; ++k)
+                umma_mx<PAIR>(d, a + 2 * k, b + 2 * k, id, sfa, sfb_n, (kb != k0 || k != 0) ? 1u : 0u);
+              commit<PAIR>(&empty_bar[stage]);
+              if (kb == k1 - 1) commit<PAIR>(&tfull_bar[unit & 1]);
             }
+            __syncwarp();
+            stage = next;
+            phase = next_phase;
           }
-          if (ok) umma_commit(&tfull_bar[unit & 1]);
         }
       }
       if (!ok) {  // what was issued is over before tensor memory is given back
         abort_sh = 1;
-        umma_commit(&done_bar);
-        mbar_wait(&done_bar, 0, p.err, ERR_MBAR_TIMEOUT_MMA);
+        if (elect_one()) {
+          commit<PAIR>(&done_bar);
+          mbar_wait(&done_bar, 0, p.err, ERR_MBAR_TIMEOUT_MMA);
+        }
+        __syncwarp();
       }
     }
   } else {
@@ -237,11 +300,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr int BUFS = OUT == OUT_F32 ? 1 : 2;
     int turn = 0, unit = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-      const int m0 = (tile / num_n) * BM + q * 32, n0 = (tile % num_n) * BN;
+    for (int tile = first; tile < num_tiles && ok; tile += step) {
+      const int m0 = (tile / num_n) * TM + rank * BM + q * 32, n0 = (tile % num_n) * BN;
       for (int c = 0; c < chunks; ++c, ++unit) {
         int got = 0;
-        if (lane == 0) got = mbar_wait(&tfull_bar[unit & 1], (unit >> 1) & 1, p.err, ERR_MBAR_TIMEOUT_EPILOGUE) ? 1 : 0;
+        if (lane == 0) got = mbar_wait_poll(&tfull_bar[unit & 1], (unit >> 1) & 1, p.err, ERR_MBAR_TIMEOUT_EPILOGUE) ? 1 : 0;
         ok = __shfl_sync(0xffffffffu, got, 0) != 0;
         if (!ok) {
           abort_sh = 1;
@@ -262,7 +325,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (i == (BN == 256 ? 0 : BN / 32 - 1)) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty_bar[unit & 1]);
+            if (lane == 0) {
+              if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[unit & 1]), 0));
+              else mbar_arrive(&tempty_bar[unit & 1]);
+            }
           }
           if (m0 >= p.M || n0 + col >= p.N) continue;
           float v[32];
@@ -305,41 +371,64 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the pair still has products or arrivals in flight
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
   }
 }
 
-template <int BN, int OUT>
-cudaError_t launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Gemm8Params& p,
-                   cudaStream_t s) {
-  auto kern = gemm8_kernel<BN, OUT>;
-  static_assert(Cfg<BN>::SMEM + 1024 <= 232448, "dynamic + static shared memory");
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BN>::SMEM);
+template <int BN, int OUT, bool PAIR>
+cudaError_t launch(const Gemm8Maps& t, const Gemm8Params& p, cudaStream_t s) {
+  using F = Cfg<BN, PAIR>;
+  auto kern = gemm8_kernel<BN, OUT, PAIR>;
+  static_assert(F::SMEM + 1024 <= 232448, "dynamic + static shared memory");
+  static std::atomic<uint64_t> set{0};  // bit d: done on device d
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  const long long tiles = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-  if (tiles >= (1ll << 31)) return cudaErrorInvalidValue;
-  kern<<<(int)std::min<long long>(tiles, num_sms()), THREADS, Cfg<BN>::SMEM, s>>>(ta, tb, tc, p);
-  return cudaGetLastError();
+  if (dev > 63 || !((set.load(std::memory_order_relaxed) >> dev) & 1)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+    if (e != cudaSuccess) return e;
+    if (dev <= 63) set.fetch_or(1ull << dev);
+  }
+  constexpr int TM = PAIR ? 2 * BM : BM;
+  const long long tiles = (long long)((p.M + TM - 1) / TM) * ((p.N + BN - 1) / BN);
+  if (tiles >= (1ll << 30)) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(PAIR ? 2 * (int)std::min<long long>(tiles, num_sms() / 2) : (int)std::min<long long>(tiles, num_sms()));
+  c.blockDim = dim3(THREADS);
+  c.dynamicSmemBytes = F::SMEM;
+  c.stream = s;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = 2;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  c.attrs = &cluster;
+  c.numAttrs = PAIR ? 1 : 0;
+  e = cudaLaunchKernelEx(&c, kern, t.a, t.b, t.c, t.sa, t.sb, p);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+template <int BN, bool PAIR>
+cudaError_t launch_out(const Gemm8Maps& t, const Gemm8Params& p, int out, cudaStream_t s) {
+  if (out == OUT_BF16) return launch<BN, OUT_BF16, PAIR>(t, p, s);
+  if (out == OUT_F16) return launch<BN, OUT_F16, PAIR>(t, p, s);
+  return launch<BN, OUT_F32, PAIR>(t, p, s);
 }
 
 }  // namespace
 
-cudaError_t gemm8_launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Gemm8Params& p, int bn,
-                         int out, cudaStream_t s) {
+cudaError_t gemm8_launch(const Gemm8Maps& t, const Gemm8Params& p, Gemm8Tile tile, int out, cudaStream_t s) {
   if (p.M <= 0 || p.N <= 0 || p.kb <= 0 || p.chunk_kb <= 0 || p.chunk_kb % 4 != 0) return cudaErrorInvalidValue;
   if (out != OUT_F32 && (p.add || p.chunk_kb < p.kb)) return cudaErrorInvalidValue;
   if (p.add && p.bias != nullptr) return cudaErrorInvalidValue;
-  if (bn == 256) {
-    if (out == OUT_BF16) return launch<256, OUT_BF16>(ta, tb, tc, p, s);
-    if (out == OUT_F16) return launch<256, OUT_F16>(ta, tb, tc, p, s);
-    return launch<256, OUT_F32>(ta, tb, tc, p, s);
+  switch (tile) {
+    case TILE_PAIR_256: return launch_out<256, true>(t, p, out, s);
+    case TILE_PAIR_192: return launch_out<192, true>(t, p, out, s);
+    case TILE_128x128: return launch_out<128, false>(t, p, out, s);
   }
-  if (bn != 128) return cudaErrorInvalidValue;
-  if (out == OUT_BF16) return launch<128, OUT_BF16>(ta, tb, tc, p, s);
-  if (out == OUT_F16) return launch<128, OUT_F16>(ta, tb, tc, p, s);
-  return launch<128, OUT_F32>(ta, tb, tc, p, s);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace tgo
