@@ -305,11 +305,10 @@ __device__ __forceinline__ void emit(Eight<T> (&v)[8], const Side& r, const Side
 
 // ------------------------------------------------------------------------------------------------------------- pack
 template <typename T, bool ROWS, bool COLS, bool SUMS>
-__global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 4 ? 2 : 3)
-    pack8_kernel(const T* __restrict__ x, long long ld, int M, int K, bool vec, Side rows, Side cols, float* __restrict__ sums) {
-  __shared__ __align__(16) TileShared sh;
+__device__ __forceinline__ void pack_tile(const T* __restrict__ x, long long ld, int M, int K, bool vec, const Side& rows,
+                                          const Side& cols, float* __restrict__ sums, int tile, TileShared& sh) {
   const int nkb = (K + TILE - 1) / TILE, nmb = (M + TILE - 1) / TILE;
-  const int kb = blockIdx.x % nkb, mb = blockIdx.x / nkb;
+  const int kb = tile % nkb, mb = tile / nkb;
   const int l16 = threadIdx.x & 15, rg = threadIdx.x >> 4;
   const int row0 = mb * TILE, c = kb * TILE + 8 * l16, n = max(0, min(8, K - c));
   Eight<T> v[8];
@@ -336,6 +335,39 @@ __global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 4 ? 2 : 3)
     __syncthreads();
   }
   emit<ROWS, COLS, T>(v, rows, cols, row0, kb * TILE, kb, nkb, mb, nmb, sh);
+}
+template <typename T, bool ROWS, bool COLS, bool SUMS>
+__global__ void __launch_bounds__(PACK_THREADS, sizeof(T) == 4 ? 2 : 3)
+    pack8_kernel(const T* __restrict__ x, long long ld, int M, int K, bool vec, Side rows, Side cols, float* __restrict__ sums) {
+  __shared__ __align__(16) TileShared sh;
+  pack_tile<T, ROWS, COLS, SUMS>(x, ld, M, K, vec, rows, cols, sums, blockIdx.x, sh);
+}
+// tiles of several tensors, of any types
+struct PackJobs {
+  struct {
+    const void* x;
+    long long ld;
+    int M, K, elem, first;  // first: the tensor's first tile
+    bool vec;
+    Side rows, cols;
+  } job[3];
+  int n;
+};
+__global__ void __launch_bounds__(PACK_THREADS, 2) pack8_jobs_kernel(const __grid_constant__ PackJobs p) {
+  __shared__ __align__(16) TileShared sh;
+  int k = 0;
+  while (k + 1 < p.n && (int)blockIdx.x >= p.job[k + 1].first) ++k;
+  const auto& j = p.job[k];
+  const int tile = blockIdx.x - j.first;
+  auto run = [&](auto t) {
+    using T = decltype(t);
+    const T* x = static_cast<const T*>(j.x);
+    if (j.cols.codes != nullptr) pack_tile<T, true, true, false>(x, j.ld, j.M, j.K, j.vec, j.rows, j.cols, nullptr, tile, sh);
+    else pack_tile<T, true, false, false>(x, j.ld, j.M, j.K, j.vec, j.rows, j.cols, nullptr, tile, sh);
+  };
+  if (j.elem == ELEM_BF16) run(__nv_bfloat16());
+  else if (j.elem == ELEM_F16) run(__half());
+  else run(float());
 }
 
 bool aligned16(const void* p, long long stride_bytes) {
@@ -981,10 +1013,34 @@ cudaError_t by_type(int elem, F&& f) {
 
 }  // namespace
 
-cudaError_t pack8_launch(const Pack8Params& p, int elem, cudaStream_t s) {
+cudaError_t pack8_launch(const Pack8Params& p, cudaStream_t s) {
   if (p.M <= 0 || p.K <= 0 || (p.codes == nullptr && p.codes_t == nullptr) || (p.sums != nullptr && p.codes_t == nullptr))
     return cudaErrorInvalidValue;
-  return by_type(elem, [&](auto t) { return pack_typed<decltype(t)>(p, s); });
+  return by_type(p.elem, [&](auto t) { return pack_typed<decltype(t)>(p, s); });
+}
+cudaError_t pack8_jobs_launch(const Pack8Jobs& p, cudaStream_t s) {
+  if (p.n < 1 || p.n > 3) return cudaErrorInvalidValue;
+  PackJobs q{};
+  q.n = p.n;
+  long long tiles = 0;
+  for (int i = 0; i < p.n; ++i) {
+    const Pack8Params& j = p.job[i];
+    if (j.M <= 0 || j.K <= 0 || j.codes == nullptr || j.sums != nullptr || j.elem < ELEM_BF16 || j.elem > ELEM_F32)
+      return cudaErrorInvalidValue;
+    q.job[i].x = j.x;
+    q.job[i].ld = j.ld;
+    q.job[i].M = j.M;
+    q.job[i].K = j.K;
+    q.job[i].elem = j.elem;
+    q.job[i].first = (int)tiles;
+    q.job[i].vec = j.K % 8 == 0 && aligned16(j.x, j.ld * (j.elem == ELEM_F32 ? 4 : 2));
+    q.job[i].rows = side(j.codes, j.scales, j.M, j.K);
+    q.job[i].cols = side(j.codes_t, j.scales_t, j.K, j.M);
+    tiles += (long long)((j.K + TILE - 1) / TILE) * ((j.M + TILE - 1) / TILE);
+    if (tiles >= (1ll << 31)) return cudaErrorInvalidValue;
+  }
+  pack8_jobs_kernel<<<(int)tiles, PACK_THREADS, 0, s>>>(q);
+  return cudaGetLastError();
 }
 cudaError_t colsum_launch(const float* sums, int T, int K, float* out, bool add, cudaStream_t s) {
   if (T <= 0 || K <= 0) return cudaErrorInvalidValue;

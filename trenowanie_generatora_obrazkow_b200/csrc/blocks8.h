@@ -17,14 +17,20 @@ namespace tgo {
 struct Pack8Params {
   const void* x;        // [M, K] of the element type, rows ld elements apart
   long long ld;
-  int M, K;
+  int M, K, elem;       // elem: ElemType
   uint8_t* codes;       // [M, Kp] blocks along K, or null
   uint8_t* scales;
   uint8_t* codes_t;     // [K, Mp] blocks along M (of x^T), or null
   uint8_t* scales_t;
   float* sums;          // [ceil(M / 128)][K] sums over the rows of each tile, or null (with codes_t)
 };
-cudaError_t pack8_launch(const Pack8Params& p, int elem, cudaStream_t s);
+cudaError_t pack8_launch(const Pack8Params& p, cudaStream_t s);
+// up to three tensors in one launch, each with codes and no sums
+struct Pack8Jobs {
+  Pack8Params job[3];
+  int n;
+};
+cudaError_t pack8_jobs_launch(const Pack8Jobs& p, cudaStream_t s);
 // out[k] (+)= sum of tiles' rows of sums [T][K], in order
 cudaError_t colsum_launch(const float* sums, int T, int K, float* out, bool add, cudaStream_t s);
 // codes [R, Kp] -> out [R, K] rows ldo apart

@@ -21,28 +21,60 @@ const char* const kWhat = "8-bit block operators";
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
-// A packed matrix: codes [rows, 128 ceil(cols / 128)] e4m3, scale bytes (blocks8.h)
+// A packed matrix: codes [rows, 128 ceil(cols / 128)] e4m3, scale bytes (blocks8.h); the memory belongs to someone else
 struct Packed {
-  at::Tensor codes, scales;
+  uint8_t* codes = nullptr;
+  uint8_t* scales = nullptr;
   int64_t rows = 0, cols = 0;
   int64_t blocks() const { return up(cols, 128); }
-  bool there() const { return codes.defined(); }
-  uint8_t* c() const { return codes.defined() ? static_cast<uint8_t*>(codes.data_ptr()) : nullptr; }
-  uint8_t* s() const { return scales.defined() ? scales.data_ptr<uint8_t>() : nullptr; }
+  int64_t code_bytes() const { return rows * blocks() * 128; }
+  int64_t scale_bytes() const { return up(rows, 128) * up(blocks(), 4) * 512; }
 };
-
-Packed fresh_packed(int64_t rows, int64_t cols, const at::Tensor& as) {
+// Packed matrices in one allocation (a small step makes a dozen of them). The plan of a forward's checkpoint is made again
+// by its backward, on the same memory.
+struct Arena {
+  Packed* parts[8];
+  int n = 0;
+  void add(Packed* p, int64_t rows, int64_t cols) {
+    p->rows = rows;
+    p->cols = cols;
+    parts[n++] = p;
+  }
+  int64_t bytes() const {
+    int64_t b = 0;
+    for (int i = 0; i < n; ++i) b += up(parts[i]->code_bytes(), 512) * 512 + parts[i]->scale_bytes();
+    return b;
+  }
+  at::Tensor on(const at::Tensor& as) {
+    at::Tensor mem = fresh({bytes()}, at::kByte, as);
+    at(mem);
+    return mem;
+  }
+  void at(const at::Tensor& mem) {
+    TORCH_CHECK(mem.is_cuda() && mem.scalar_type() == at::kByte && mem.is_contiguous() && mem.numel() == bytes() &&
+                    reinterpret_cast<uintptr_t>(mem.data_ptr()) % 16 == 0, kWhat, ": the saved checkpoint has changed");
+    uint8_t* p = mem.data_ptr<uint8_t>();
+    for (int i = 0; i < n; ++i) {
+      parts[i]->codes = p;
+      p += up(parts[i]->code_bytes(), 512) * 512;
+      parts[i]->scales = p;
+      p += parts[i]->scale_bytes();
+    }
+  }
+};
+// as tensors of their own (what quantize_blocks returns)
+Packed fresh_packed(int64_t rows, int64_t cols, const at::Tensor& as, std::vector<at::Tensor>* out) {
   Packed p;
   p.rows = rows;
   p.cols = cols;
-  p.codes = fresh({rows, p.blocks() * 128}, at::kFloat8_e4m3fn, as);
-  p.scales = fresh({up(rows, 128), up(p.blocks(), 4), 32, 4, 4}, at::kByte, as);
+  out->push_back(fresh({rows, p.blocks() * 128}, at::kFloat8_e4m3fn, as));
+  p.codes = static_cast<uint8_t*>(out->back().data_ptr());
+  out->push_back(fresh({up(rows, 128), up(p.blocks(), 4), 32, 4, 4}, at::kByte, as));
+  p.scales = out->back().data_ptr<uint8_t>();
   return p;
 }
 Packed given_packed(const at::Tensor& codes, const at::Tensor& scales, int64_t cols, const char* what) {
   Packed p;
-  p.codes = codes;
-  p.scales = scales;
   p.cols = cols;
   TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kFloat8_e4m3fn && codes.dim() == 2 && codes.is_contiguous() &&
                   cols >= 0 && cols < (1ll << 31) - 128 && codes.size(1) == p.blocks() * 128,
@@ -52,8 +84,10 @@ Packed given_packed(const at::Tensor& codes, const at::Tensor& scales, int64_t c
   TORCH_CHECK(scales.scalar_type() == at::kByte && scales.is_contiguous() && p.rows < (1ll << 31) - 128 &&
                   scales.sizes() == at::IntArrayRef({up(p.rows, 128), up(p.blocks(), 4), 32, 4, 4}),
               what, ": scales uint8 [", up(p.rows, 128), ", ", up(p.blocks(), 4), ", 32, 4, 4], contiguous, expected");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
-                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0, what, ": 16-byte aligned codes and scales");
+  p.codes = static_cast<uint8_t*>(codes.data_ptr());
+  p.scales = scales.data_ptr<uint8_t>();
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(p.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(p.scales) % 16 == 0, what,
+              ": 16-byte aligned codes and scales");
   return p;
 }
 
@@ -68,32 +102,53 @@ void check_matrix(const at::Tensor& t, const char* what) {
               ": at least one column and fewer than 2^31 - 128 rows and columns");
 }
 
-// packs x [M, K] (rows_of): blocks along the rows (r), along the columns as the rows of x^T (c), column sums (sums [K] fp32)
-void pack(const at::Tensor& x, Packed* r, Packed* c, float* sums, bool add, const char* what) {
-  check_matrix(x, what);
-  const int64_t M = x.size(0), K = x.size(1);
-  const int elem = elem_of(x, what);
-  if (r != nullptr) *r = fresh_packed(M, K, x);
-  if (c != nullptr) *c = fresh_packed(K, M, x);
+// Packs x [M, K] (rows_of) into r (blocks along the rows) and / or c (along the columns, as the rows of x^T); sums [K] fp32:
+// the column sums (with c).
+struct PackJob {
+  const at::Tensor& x;
+  const Packed* r;
+  const Packed* c;
+};
+Pack8Params pack_params(const PackJob& j) {
+  Pack8Params p{};
+  p.x = j.x.data_ptr();
+  p.ld = row_stride(j.x);
+  p.M = (int)j.x.size(0);
+  p.K = (int)j.x.size(1);
+  p.elem = elem_of(j.x, kWhat);
+  if (j.r != nullptr) p.codes = j.r->codes, p.scales = j.r->scales;
+  if (j.c != nullptr) p.codes_t = j.c->codes, p.scales_t = j.c->scales;
+  return p;
+}
+void pack(const PackJob& j, float* sums = nullptr, bool add = false) {
+  const int64_t M = j.x.size(0), K = j.x.size(1);
   const cudaStream_t s = at::cuda::getCurrentCUDAStream();
   if (M == 0) {
-    if (sums != nullptr && !add) TORCH_CHECK(cudaMemsetAsync(sums, 0, K * sizeof(float), s) == cudaSuccess, what);
+    if (sums != nullptr && !add) TORCH_CHECK(cudaMemsetAsync(sums, 0, K * sizeof(float), s) == cudaSuccess, kWhat);
     return;
   }
-  Pack8Params p{};
-  p.x = x.data_ptr();
-  p.ld = row_stride(x);
-  p.M = (int)M;
-  p.K = (int)K;
-  if (r != nullptr) p.codes = r->c(), p.scales = r->s();
-  if (c != nullptr) p.codes_t = c->c(), p.scales_t = c->s();
+  Pack8Params p = pack_params(j);
   at::Tensor part;
   if (sums != nullptr) {
-    part = fresh({up(M, 128), K}, at::kFloat, x);
+    part = fresh({up(M, 128), K}, at::kFloat, j.x);
     p.sums = part.data_ptr<float>();
   }
-  BLOCK_LAUNCH(pack8_launch(p, elem, s), 1);
+  BLOCK_LAUNCH(pack8_launch(p, s), 1);
   if (sums != nullptr) BLOCK_LAUNCH(colsum_launch(p.sums, (int)up(M, 128), (int)K, sums, add, s), 1);
+}
+// Several tensors (rows always wanted): one launch where they are small. Two launches cost the host some 4 us more than one,
+// and their kernels' tails; past a few tiles per SM the kernels made for one type are faster.
+void pack_all(std::initializer_list<PackJob> jobs) {
+  Pack8Jobs all{};
+  int64_t tiles = 0;
+  for (const PackJob& j : jobs) tiles += up(j.x.size(0), 128) * up(j.x.size(1), 128);
+  if (tiles > 4 * num_sms()) {
+    for (const PackJob& j : jobs) pack(j);
+    return;
+  }
+  for (const PackJob& j : jobs)
+    if (j.x.size(0) > 0) all.job[all.n++] = pack_params(j);
+  if (all.n > 0) BLOCK_LAUNCH(pack8_jobs_launch(all, at::cuda::getCurrentCUDAStream()), 1);
 }
 
 CUtensorMap codes_map(const Packed& a, uint32_t box_rows) {
@@ -103,7 +158,7 @@ CUtensorMap codes_map(const Packed& a, uint32_t box_rows) {
   cuuint64_t strides[2] = {width, width * (cuuint64_t)a.rows};
   cuuint32_t box[3] = {128, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = tmap_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.c(), dims, strides, box, estr,
+  const CUresult r = tmap_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.codes, dims, strides, box, estr,
                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "tensor map of 8-bit codes: code ", (int)r);
@@ -134,7 +189,7 @@ CUtensorMap scales_map(const Packed& a, uint32_t box_tiles) {
   cuuint64_t strides[2] = {512, quads * 512};
   cuuint32_t box[3] = {128, 1, box_tiles};
   cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = tmap_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, a.s(), dims, strides, box, estr,
+  const CUresult r = tmap_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, a.scales, dims, strides, box, estr,
                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "tensor map of 8-bit scales: code ", (int)r);
@@ -170,8 +225,8 @@ void product(const Packed& a, const Packed& b, const at::Tensor& C, const float*
   p.M = (int)a.rows;
   p.N = (int)b.rows;
   p.kb = (int)a.blocks();
-  p.sfa = a.s();
-  p.sfb = b.s();
+  p.sfa = a.scales;
+  p.sfb = b.scales;
   p.C = C.data_ptr();
   p.ldc = row_stride(C);
   p.bias = bias;
@@ -199,7 +254,11 @@ void small_vector(const OptT& bias, int64_t n, const at::Tensor& as, const char*
   TORCH_CHECK(bias->is_floating_point() && bias->dim() == 1 && bias->size(0) == n, what, ": bias [", n, "] expected");
 }
 // the bias in fp32 (a copy where it is not)
-at::Tensor bias_f32(const OptT& bias) { return given(bias) ? bias->detach().to(at::kFloat).contiguous() : at::Tensor(); }
+at::Tensor bias_f32(const OptT& bias) {
+  if (!given(bias)) return at::Tensor();
+  if (bias->scalar_type() == at::kFloat && bias->is_contiguous()) return *bias;
+  return bias->detach().to(at::kFloat).contiguous();
+}
 const float* ptr_f32(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 
 // ------------------------------------------------------------------------------------------------ packing, products
@@ -208,11 +267,12 @@ std::vector<at::Tensor> pack8(at::Tensor x, bool rows, bool cols) {
   check_matrix(x, "quantize_blocks");
   const c10::cuda::CUDAGuard guard(x.device());
   x = rows_of(x.detach());
-  Packed r, c;
-  pack(x, rows ? &r : nullptr, cols ? &c : nullptr, nullptr, false, "quantize_blocks");
+  elem_of(x, "quantize_blocks");
   std::vector<at::Tensor> out;
-  if (rows) out.insert(out.end(), {r.codes, r.scales});
-  if (cols) out.insert(out.end(), {c.codes, c.scales});
+  Packed r, c;
+  if (rows) r = fresh_packed(x.size(0), x.size(1), x, &out);
+  if (cols) c = fresh_packed(x.size(1), x.size(0), x, &out);
+  pack({x, rows ? &r : nullptr, cols ? &c : nullptr});
   return out;
 }
 
@@ -222,7 +282,7 @@ at::Tensor unpack8(at::Tensor codes, at::Tensor scales, int64_t cols, at::Scalar
   at::Tensor out = fresh({p.rows, cols}, type, codes);
   const int elem = elem_of(out, "dequantize_blocks");
   if (out.numel() > 0)
-    BLOCK_LAUNCH(unpack8_launch(p.c(), p.s(), (int)p.rows, (int)cols, out.data_ptr(), cols, elem,
+    BLOCK_LAUNCH(unpack8_launch(p.codes, p.scales, (int)p.rows, (int)cols, out.data_ptr(), cols, elem,
                                 at::cuda::getCurrentCUDAStream()), 1);
   return out;
 }
@@ -260,13 +320,14 @@ at::Tensor linear8_frozen(at::Tensor x, at::Tensor codes, at::Tensor scales, int
   x = rows_of(x);
   const at::Tensor b32 = bias_f32(bias);
   at::Tensor y = fresh({x.size(0), w.rows}, x.scalar_type(), x);
+  elem_of(x, "linear_blocks");
   if (y.numel() == 0) return y;
   if (x.size(0) <= kFewRows) {
     FewRowsParams p{};
     p.x = x.data_ptr();
     p.ldx = row_stride(x);
-    p.codes = w.c();
-    p.scales = w.s();
+    p.codes = w.codes;
+    p.scales = w.scales;
     p.bias = ptr_f32(b32);
     p.y = y.data_ptr();
     p.M = (int)x.size(0);
@@ -276,25 +337,16 @@ at::Tensor linear8_frozen(at::Tensor x, at::Tensor codes, at::Tensor scales, int
     return y;
   }
   Packed q;
-  pack(x, &q, nullptr, nullptr, false, "linear_blocks");
+  Arena arena;
+  arena.add(&q, x.size(0), x.size(1));
+  const at::Tensor mem = arena.on(x);
+  pack({x, &q, nullptr});
   product(q, w, y, ptr_f32(b32), false, err_word(err, x));
   return y;
 }
 
 // The operands of a backward product are packed along the axis that it sums over: x^T and W^T are written while the
 // forward packs x and W. x itself is not kept: its checkpoint is the operand of the weight's gradient.
-void keep(variable_list* saved, const Packed& p) {
-  saved->push_back(p.codes);
-  saved->push_back(p.scales);
-}
-Packed kept(const variable_list& saved, size_t at, int64_t cols) {
-  Packed p;
-  p.codes = saved[at];
-  p.scales = saved[at + 1];
-  p.rows = p.codes.defined() ? p.codes.size(0) : 0;
-  p.cols = cols;
-  return p;
-}
 // a product that sums over no rows at all
 bool zero_sum(const WeightGrad& g, int64_t rows) {
   if (rows > 0) return false;
@@ -318,20 +370,23 @@ struct Linear8Fn : public torch::autograd::Function<Linear8Fn> {
   static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor w, OptT bias, at::Tensor err) {
     at::AutoDispatchBelowADInplaceOrView below;
     const bool dx = x.requires_grad(), dw = w.requires_grad();
+    const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
     Packed xr, xt, wr, wt;
-    pack(x, &xr, dw ? &xt : nullptr, nullptr, false, "linear_blocks");
-    pack(w, &wr, dx ? &wt : nullptr, nullptr, false, "linear_blocks: weight");
-    at::Tensor y = fresh({x.size(0), w.size(0)}, x.scalar_type(), x);
+    Arena now, later;
+    now.add(&xr, M, K);
+    now.add(&wr, N, K);
+    if (dw) later.add(&xt, K, M);
+    if (dx) later.add(&wt, K, N);
+    const at::Tensor mem = now.on(x), checkpoint = later.on(x);
+    pack_all({{x, &xr, dw ? &xt : nullptr}, {w, &wr, dx ? &wt : nullptr}});
+    at::Tensor y = fresh({M, N}, x.scalar_type(), x);
     const at::Tensor b32 = bias_f32(bias);
     product(xr, wr, y, ptr_f32(b32), false, err_word(err, x));
-    variable_list saved;
-    keep(&saved, xt);
-    keep(&saved, wt);
-    ctx->save_for_backward(saved);
+    ctx->save_for_backward({checkpoint});
     ctx->saved_data["w"] = w;
     if (given(bias)) ctx->saved_data["bias"] = *bias;
     ctx->saved_data["err"] = err;
-    ctx->saved_data["dx"] = dx;
+    ctx->saved_data["of"] = (dx ? 1 : 0) + (dw ? 2 : 0);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -339,22 +394,27 @@ struct Linear8Fn : public torch::autograd::Function<Linear8Fn> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor dy = rows_of(grads[0]);
     const c10::cuda::CUDAGuard guard(dy.device());
-    const int64_t M = dy.size(0), N = dy.size(1);
-    const bool dx = ctx->saved_data["dx"].toBool();
+    const int64_t M = dy.size(0), N = dy.size(1), of = ctx->saved_data["of"].toInt();
+    const bool dx = of & 1;
     const at::Tensor err = ctx->saved_data["err"].toTensor();
     int* const e = err_word(err, dy);
-    const Packed xt = kept(saved, 0, M), wt = kept(saved, 2, N);
     const WeightGrad gw(ctx, "w"), gb(ctx, "bias");
-    Packed r, c;
+    const int64_t K = ctx->saved_data["w"].toTensor().size(1);
+    Packed xt, wt, r, c;
+    Arena before, now;
+    if (of & 2) before.add(&xt, K, M);
+    if (of & 1) before.add(&wt, K, N);
+    before.at(saved[0]);
     // the bias' sums are fp32 wherever they go
     at::Tensor sums = gb.g.defined() ? (gb.g.scalar_type() == at::kFloat ? gb.g : fresh({N}, at::kFloat, dy)) : at::Tensor();
-    const bool cols = gw.g.defined() || sums.defined();
-    if (dx || cols)
-      pack(dy, dx ? &r : nullptr, cols ? &c : nullptr, sums.defined() ? sums.data_ptr<float>() : nullptr, gb.add,
-           "linear_blocks: gradient");
+    const bool dw = gw.g.defined(), cols = dw || sums.defined();
+    if (dx) now.add(&r, M, N);
+    if (cols) now.add(&c, N, M);
+    const at::Tensor mem = now.on(dy);
+    if (dx || cols) pack({dy, dx ? &r : nullptr, cols ? &c : nullptr}, sums.defined() ? sums.data_ptr<float>() : nullptr, gb.add);
     variable_list out(4);
     if (dx) {
-      out[0] = fresh({M, wt.rows}, dy.scalar_type(), dy);
+      out[0] = fresh({M, K}, dy.scalar_type(), dy);
       product(r, wt, out[0], nullptr, false, e);
     }
     out[1] = weight_grad(gw, c, xt, M, e);
@@ -385,8 +445,11 @@ at::Tensor linear8(at::Tensor x, at::Tensor w, OptT bias, at::Tensor err) {
   }
   w = rows_of(w);
   Packed xr, wr;
-  pack(x, &xr, nullptr, nullptr, false, "linear_blocks");
-  pack(w, &wr, nullptr, nullptr, false, "linear_blocks: weight");
+  Arena now;
+  now.add(&xr, x.size(0), x.size(1));
+  now.add(&wr, w.size(0), w.size(1));
+  const at::Tensor mem = now.on(x);
+  pack_all({{x, &xr, nullptr}, {w, &wr, nullptr}});
   at::Tensor y = fresh({x.size(0), w.size(0)}, x.scalar_type(), x);
   const at::Tensor b32 = bias_f32(bias);
   product(xr, wr, y, ptr_f32(b32), false, err_word(err, x));
@@ -412,12 +475,9 @@ CUtensorMap tile_map(const at::Tensor& t) {
                     : t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   return tile_map(t.data_ptr(), type, t.element_size(), t.size(1), t.size(0), t.size(1));
 }
-void swiglu_forward(const at::Tensor& ab, at::Tensor* g, Packed* ck, Packed* g8, Packed* g8t, int* err) {
-  const int64_t M = ab.size(0), H = ab.size(1) / 2, Hp = up(H, 128) * 128;
+void swiglu_forward(const at::Tensor& ab, at::Tensor* g, const Packed* ck, const Packed* g8, const Packed* g8t, int* err) {
+  const int64_t M = ab.size(0), H = ab.size(1) / 2;
   if (g != nullptr) *g = fresh({M, H}, ab.scalar_type(), ab);
-  if (ck != nullptr) *ck = fresh_packed(M, 2 * Hp, ab);
-  if (g8 != nullptr) *g8 = fresh_packed(M, H, ab);
-  if (g8t != nullptr) *g8t = fresh_packed(H, M, ab);
   if (M == 0) return;
   Swiglu8Params p{};
   p.ab = ab.data_ptr();
@@ -425,9 +485,9 @@ void swiglu_forward(const at::Tensor& ab, at::Tensor* g, Packed* ck, Packed* g8,
   p.M = (int)M;
   p.H = (int)H;
   if (g != nullptr) p.g = g->data_ptr();
-  if (ck != nullptr) p.ck = ck->c(), p.ck_scales = ck->s();
-  if (g8 != nullptr) p.g8 = g8->c(), p.g8_scales = g8->s();
-  if (g8t != nullptr) p.g8t = g8t->c(), p.g8t_scales = g8t->s();
+  if (ck != nullptr) p.ck = ck->codes, p.ck_scales = ck->scales;
+  if (g8 != nullptr) p.g8 = g8->codes, p.g8_scales = g8->scales;
+  if (g8t != nullptr) p.g8t = g8t->codes, p.g8t_scales = g8t->scales;
   CUtensorMap map;
   if (g8 != nullptr) {  // ab is the contiguous output of a product
     map = tile_map(ab);
@@ -436,22 +496,21 @@ void swiglu_forward(const at::Tensor& ab, at::Tensor* g, Packed* ck, Packed* g8,
   }
   BLOCK_LAUNCH(swiglu8_fwd_launch(p, elem_of(ab, "swiglu_blocks"), at::cuda::getCurrentCUDAStream()), 1);
 }
-void swiglu_backward(const at::Tensor& dg, const Packed& ck, int64_t H, at::Tensor* dab, Packed* d8, Packed* d8t, int* err) {
+void swiglu_backward(const at::Tensor& dg, const Packed& ck, int64_t H, at::Tensor* dab, const Packed* d8, const Packed* d8t,
+                     int* err) {
   const int64_t M = dg.size(0);
   if (dab != nullptr) *dab = fresh({M, 2 * H}, dg.scalar_type(), dg);
-  if (d8 != nullptr) *d8 = fresh_packed(M, 2 * H, dg);
-  if (d8t != nullptr) *d8t = fresh_packed(2 * H, M, dg);
   if (M == 0) return;
   Swiglu8BwdParams p{};
   p.dg = dg.data_ptr();
   p.ld = row_stride(dg);
-  p.ck = ck.c();
-  p.ck_scales = ck.s();
+  p.ck = ck.codes;
+  p.ck_scales = ck.scales;
   p.M = (int)M;
   p.H = (int)H;
   if (dab != nullptr) p.dab = dab->data_ptr();
-  if (d8 != nullptr) p.d8 = d8->c(), p.d8_scales = d8->s();
-  if (d8t != nullptr) p.d8t = d8t->c(), p.d8t_scales = d8t->s();
+  if (d8 != nullptr) p.d8 = d8->codes, p.d8_scales = d8->scales;
+  if (d8t != nullptr) p.d8t = d8t->codes, p.d8t_scales = d8t->scales;
   CUtensorMap map, ck_map;
   if (d8 != nullptr) {  // dg is the contiguous output of a product
     map = tile_map(dg);
@@ -468,8 +527,10 @@ struct Swiglu8Fn : public torch::autograd::Function<Swiglu8Fn> {
     at::AutoDispatchBelowADInplaceOrView below;
     at::Tensor g;
     Packed ck;
+    Arena later;
+    later.add(&ck, ab.size(0), 2 * up(ab.size(1) / 2, 128) * 128);
+    ctx->save_for_backward({later.on(ab)});
     swiglu_forward(ab, &g, &ck, nullptr, nullptr, nullptr);
-    ctx->save_for_backward({ck.codes, ck.scales});
     return g;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -478,7 +539,11 @@ struct Swiglu8Fn : public torch::autograd::Function<Swiglu8Fn> {
     const at::Tensor dg = rows_of(grads[0]);
     const c10::cuda::CUDAGuard guard(dg.device());
     at::Tensor dab;
-    swiglu_backward(dg, kept(saved, 0, saved[0].size(1)), dg.size(1), &dab, nullptr, nullptr, nullptr);
+    Packed ck;
+    Arena before;
+    before.add(&ck, dg.size(0), 2 * up(dg.size(1), 128) * 128);
+    before.at(saved[0]);
+    swiglu_backward(dg, ck, dg.size(1), &dab, nullptr, nullptr, nullptr);
     return {dab};
   }
 };
@@ -495,33 +560,47 @@ at::Tensor swiglu8(at::Tensor ab) {
 }
 
 // -------------------------------------------------------------------------------------------------------------- MLP
+// what the backward reads: x^T (of bit 2: in_proj's gradient), W1^T (bit 1: x's gradient), W2^T and [a | b] (either), g^T (bit 4:
+// out_proj's gradient)
+struct MlpCheckpoint {
+  Packed xt, w1t, w2t, ck, gt;
+  Arena arena;
+  MlpCheckpoint(int64_t M, int64_t K, int64_t H, int64_t N, int64_t of) {
+    if (of & 2) arena.add(&xt, K, M);
+    if (of & 1) arena.add(&w1t, K, 2 * H);
+    if (of & 3) arena.add(&w2t, H, N);
+    if (of & 3) arena.add(&ck, M, 2 * H);
+    if (of & 4) arena.add(&gt, H, M);
+  }
+};
 struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
   static at::Tensor forward(AutogradContext* ctx, at::Tensor x, at::Tensor w1, at::Tensor w2, at::Tensor err) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const bool dx = x.requires_grad(), dw1 = w1.requires_grad(), dw2 = w2.requires_grad(), up_too = dx || dw1;
-    Packed xr, xt, w1r, w1t, w2r, w2t, ck, g8, g8t;
-    pack(x, &xr, dw1 ? &xt : nullptr, nullptr, false, "mlp_blocks");
-    pack(w1, &w1r, dx ? &w1t : nullptr, nullptr, false, "mlp_blocks: in_proj");
-    pack(w2, &w2r, up_too ? &w2t : nullptr, nullptr, false, "mlp_blocks: out_proj");
+    const int64_t M = x.size(0), K = x.size(1), H = w2.size(1), N = w2.size(0);
+    const int64_t of = (x.requires_grad() ? 1 : 0) + (w1.requires_grad() ? 2 : 0) + (w2.requires_grad() ? 4 : 0);
+    MlpCheckpoint c(M, K, H, N, of);
+    const at::Tensor checkpoint = c.arena.on(x);
+    Packed xr, w1r, w2r, g8;
+    Arena now;
+    now.add(&xr, M, K);
+    now.add(&w1r, 2 * H, K);
+    now.add(&w2r, N, H);
+    now.add(&g8, M, H);
+    const at::Tensor mem = now.on(x);
+    pack_all({{x, &xr, of & 2 ? &c.xt : nullptr}, {w1, &w1r, of & 1 ? &c.w1t : nullptr}, {w2, &w2r, of & 3 ? &c.w2t : nullptr}});
     int* const e = err_word(err, x);
     {
-      at::Tensor ab = fresh({x.size(0), w1.size(0)}, x.scalar_type(), x);
+      at::Tensor ab = fresh({M, 2 * H}, x.scalar_type(), x);
       product(xr, w1r, ab, nullptr, false, e);
-      swiglu_forward(ab, nullptr, up_too ? &ck : nullptr, &g8, dw2 ? &g8t : nullptr, e);
+      swiglu_forward(ab, nullptr, of & 3 ? &c.ck : nullptr, &g8, of & 4 ? &c.gt : nullptr, e);
     }
-    at::Tensor y = fresh({x.size(0), w2.size(0)}, x.scalar_type(), x);
+    at::Tensor y = fresh({M, N}, x.scalar_type(), x);
     product(g8, w2r, y, nullptr, false, e);
-    variable_list saved;
-    keep(&saved, xt);
-    keep(&saved, w1t);
-    keep(&saved, w2t);
-    keep(&saved, ck);
-    keep(&saved, g8t);
-    ctx->save_for_backward(saved);
+    ctx->save_for_backward({checkpoint});
     ctx->saved_data["w1"] = w1;
     ctx->saved_data["w2"] = w2;
     ctx->saved_data["err"] = err;
-    ctx->saved_data["dx"] = dx;
+    ctx->saved_data["of"] = of;
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -529,32 +608,36 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor dy = rows_of(grads[0]);
     const c10::cuda::CUDAGuard guard(dy.device());
-    const int64_t M = dy.size(0), N = dy.size(1);
-    const bool dx = ctx->saved_data["dx"].toBool();
+    const int64_t of = ctx->saved_data["of"].toInt();
+    const int64_t M = dy.size(0), N = dy.size(1), H = ctx->saved_data["w2"].toTensor().size(1),
+                  K = ctx->saved_data["w1"].toTensor().size(1);
     const at::Tensor err = ctx->saved_data["err"].toTensor();
     int* const e = err_word(err, dy);
     const WeightGrad g1(ctx, "w1"), g2(ctx, "w2");
-    const bool up_too = dx || g1.g.defined();
-    const Packed w2t = kept(saved, 4, N);
-    const int64_t H = ctx->saved_data["w2"].toTensor().size(1);
+    const bool dx = of & 1, dw1 = g1.g.defined(), dw2 = g2.g.defined(), up_too = dx || dw1;
+    MlpCheckpoint c(M, K, H, N, of);
+    c.arena.at(saved[0]);
+    Packed dyr, dyt, d8, d8t;
+    Arena now;
+    if (up_too) now.add(&dyr, M, N);
+    if (dw2) now.add(&dyt, N, M);
+    if (up_too) now.add(&d8, M, 2 * H);
+    if (up_too) now.add(&d8t, 2 * H, M);
+    const at::Tensor mem = now.on(dy);
+    if (up_too || dw2) pack({dy, up_too ? &dyr : nullptr, dw2 ? &dyt : nullptr});
     variable_list out(4);
-    Packed dyr, dyt;
-    if (up_too || g2.g.defined())
-      pack(dy, up_too ? &dyr : nullptr, g2.g.defined() ? &dyt : nullptr, nullptr, false, "mlp_blocks: gradient");
-    out[2] = weight_grad(g2, dyt, kept(saved, 8, M), M, e);
+    out[2] = weight_grad(g2, dyt, c.gt, M, e);
     if (up_too) {
-      Packed d8, d8t;
       {
         at::Tensor dg = fresh({M, H}, dy.scalar_type(), dy);
-        product(dyr, w2t, dg, nullptr, false, e);
-        swiglu_backward(dg, kept(saved, 6, 2 * H), H, nullptr, &d8, &d8t, e);
+        product(dyr, c.w2t, dg, nullptr, false, e);
+        swiglu_backward(dg, c.ck, H, nullptr, &d8, &d8t, e);
       }
       if (dx) {
-        const Packed w1t = kept(saved, 2, 2 * H);
-        out[0] = fresh({M, w1t.rows}, dy.scalar_type(), dy);
-        product(d8, w1t, out[0], nullptr, false, e);
+        out[0] = fresh({M, K}, dy.scalar_type(), dy);
+        product(d8, c.w1t, out[0], nullptr, false, e);
       }
-      out[1] = weight_grad(g1, d8t, kept(saved, 0, M), M, e);
+      out[1] = weight_grad(g1, d8t, c.xt, M, e);
     }
     notify({&g2, &g1});
     return out;
@@ -582,9 +665,13 @@ at::Tensor mlp8(at::Tensor x, at::Tensor w1, at::Tensor w2, at::Tensor err) {
   w1 = rows_of(w1);
   w2 = rows_of(w2);
   Packed xr, w1r, w2r, g8;
-  pack(x, &xr, nullptr, nullptr, false, "mlp_blocks");
-  pack(w1, &w1r, nullptr, nullptr, false, "mlp_blocks: in_proj");
-  pack(w2, &w2r, nullptr, nullptr, false, "mlp_blocks: out_proj");
+  Arena now;
+  now.add(&xr, x.size(0), x.size(1));
+  now.add(&w1r, w1.size(0), w1.size(1));
+  now.add(&w2r, w2.size(0), w2.size(1));
+  now.add(&g8, x.size(0), w2.size(1));
+  const at::Tensor mem = now.on(x);
+  pack_all({{x, &xr, nullptr}, {w1, &w1r, nullptr}, {w2, &w2r, nullptr}});
   int* const e = err_word(err, x);
   at::Tensor ab = fresh({x.size(0), w1.size(0)}, x.scalar_type(), x), y = fresh({x.size(0), w2.size(0)}, x.scalar_type(), x);
   product(xr, w1r, ab, nullptr, false, e);
