@@ -82,6 +82,7 @@ def main():
     p.add_argument("--attn-scale", type=float, default=1.0)
     p.add_argument("--t-shift", type=float, default=1.0)
     p.add_argument("--batch", type=int, default=64)
+    p.add_argument("--fp8", action="store_true", help="denoiser on 8-bit products (e4m3, a scale for each 128 values)")
     p.add_argument("--export", action="store_true")
     a = p.parse_args()
     device = torch.device("cuda") if torch.cuda.is_available() else torch.device("cpu")
@@ -90,6 +91,9 @@ def main():
     te_cfg, den_cfg = te.config, den.config
     print(f"{a.ckpt}: step {info['step']}, {info['weights']} weights")
     te.to(device).eval(), den.to(device).eval()
+    if a.fp8:
+        from trenowanie_generatora_obrazkow_b200.models.quant import use_fp8
+        use_fp8(den)
     for m in den.modules():
         if hasattr(m, "logit_mult"):
             m.logit_mult = a.attn_scale

@@ -1,0 +1,130 @@
+"""Models and commands on 8-bit products and with 8-bit activation checkpoints (CPU definitions)."""
+import os
+import socket
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from trenowanie_generatora_obrazkow_b200.models import DenoiserConfig, build_models
+from trenowanie_generatora_obrazkow_b200.models.config import TE_SIZES
+from trenowanie_generatora_obrazkow_b200.models.quant import BlockLinear, quantize, use_fp8
+from trenowanie_generatora_obrazkow_b200.ops import blocks8 as B8
+from trenowanie_generatora_obrazkow_b200.ops import fused as Fz
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _model():
+    torch.manual_seed(0)
+    te, den = build_models(DenoiserConfig(dim=128, depth=2, heads=2, mlp_hidden=384, text_dim=128, latent_size=4),
+                           TE_SIZES["states-nano"], device="cpu")
+    te.init_weights(), den.init_weights()
+    with torch.no_grad():
+        for p in list(te.parameters()) + list(den.parameters()):
+            p.add_(0.05 * torch.randn_like(p))
+    return te, den
+
+
+def _step(te, den):
+    g = torch.Generator().manual_seed(1)
+    x, t, st = torch.randn(2, 128, 4, 4, generator=g), torch.rand(2, generator=g), torch.randn(2, 16, 64, generator=g)
+    params = list(te.parameters()) + list(den.parameters())
+    for p in params:
+        p.grad = None
+    text, valid = te(lm_states=st)
+    out = den(x, t, text, valid)
+    out.square().mean().backward()
+    return out.detach(), [None if p.grad is None else p.grad.clone() for p in params]
+
+
+def test_marked_blocks_run_on_8_bit_products():
+    te, den = _model()
+    plain, grads = _step(te, den)
+    names = [n for n, _ in den.named_parameters()]
+    use_fp8(te), use_fp8(den)
+    assert den.blocks[0].mlp.in_proj.fp8 and "fp8" not in den.patch_in.__dict__
+    assert [n for n, _ in den.named_parameters()] == names
+    out, g8 = _step(te, den)
+    # a value's error is at most 2^-4 of it; products of many add up like noise
+    assert 0 < ((out - plain).norm() / plain.norm()).item() < 0.1
+    assert [g is None for g in grads] == [g is None for g in g8]
+    whole = torch.cat([g.flatten() for g in grads if g is not None]), torch.cat([g.flatten() for g in g8 if g is not None])
+    assert ((whole[1] - whole[0]).norm() / whole[0].norm()).item() < 0.1
+    with torch.no_grad():  # weights held in 8 bits: the same products
+        text, valid = te(lm_states=torch.randn(2, 16, 64, generator=torch.Generator().manual_seed(2)))
+        x = torch.randn(2, 128, 4, 4)
+        first = den(x, torch.rand(2), text, valid)
+        kept = den.blocks[0].attn.qkv.weight._tgo_fp8
+        den(x, torch.rand(2), text, valid)
+        assert den.blocks[0].attn.qkv.weight._tgo_fp8 is kept and torch.isfinite(first).all()
+        den.blocks[0].attn.qkv.weight.mul_(2)
+        den(x, torch.rand(2), text, valid)
+        assert den.blocks[0].attn.qkv.weight._tgo_fp8 is not kept
+    use_fp8(te, False), use_fp8(den, False)
+    assert torch.equal(_step(*_model())[0], plain)
+
+
+def test_held_weights_give_the_training_forward():
+    lin = torch.nn.Linear(130, 48)
+    lin.fp8 = True
+    x = torch.randn(5, 130)
+    y = Fz.linear(x, lin)
+    with torch.no_grad():
+        assert torch.equal(Fz.linear(x, lin), y)
+    a, b = torch.nn.Linear(64, 256, bias=False), torch.nn.Linear(128, 32, bias=False)
+    a.fp8 = b.fp8 = True
+    x = torch.randn(5, 64)
+    y = Fz.mlp_fp8(x, a, b)
+    with torch.no_grad():
+        assert torch.equal(Fz.mlp_fp8(x, a, b), y)
+
+
+def test_checkpoint_mode_keeps_the_swiglu_in_8_bits():
+    te, den = _model()
+    plain, grads = _step(te, den)
+    te.checkpoint_blocks = den.checkpoint_blocks = "fp8"
+    out, g8 = _step(te, den)
+    assert torch.equal(out, plain)  # the forward is the same
+    for n, (a, b) in zip([n for n, _ in te.named_parameters()] + [n for n, _ in den.named_parameters()], zip(grads, g8)):
+        if a is not None:
+            assert ((a - b).norm() / a.norm().clamp_min(1e-12)).item() < 0.1, n
+    assert Fz._PACK8_ACTIVE[0] == 0 and Fz._SAC_ACTIVE[0] == 0
+
+
+def test_block_linear():
+    m = torch.nn.Sequential(torch.nn.Linear(130, 64), torch.nn.GELU(), torch.nn.Linear(64, 8, bias=False))
+    x = torch.randn(3, 7, 130)
+    want = m(x)
+    w = m[0].weight
+    quantize(m, "fp8_block")
+    assert isinstance(m[0], BlockLinear) and m[0].w.dtype == torch.float8_e4m3fn
+    assert torch.equal(m[0](x), B8.linear_blocks(x, B8.quantize_blocks(w), m[0].bias.detach()))
+    assert ((m(x) - want).norm() / want.norm()).item() < 0.1
+    state = {k: v.clone() for k, v in m.state_dict().items()}
+    m.load_state_dict(state)
+
+
+@pytest.mark.parametrize("flags", [["--fp8"], ["--act-checkpoint", "fp8"], ["--fp8", "--act-checkpoint", "fp8"]])
+def test_train_command(tmp_path, flags):
+    r = subprocess.run([sys.executable, "train.py", "--synthetic", "16", "--out", str(tmp_path / "run"), "--size", "nano",
+                        "--te-size", "13m", "--batch", "2", "--micro-batch", "2", "--steps", "1", "--eval-every", "0",
+                        "--no-wandb", "--ckpt-every", "0"] + flags, cwd=ROOT, capture_output=True, text=True, timeout=600,
+                       env=dict(os.environ, CUDA_VISIBLE_DEVICES=""))
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("opd", [False, True])
+def test_pipeline_command(tmp_path, opd):
+    with socket.socket() as sock:
+        sock.bind(("127.0.0.1", 0))
+        port = sock.getsockname()[1]
+    mode = ["--dance-opd", "--teacher-size", "nano", "--batch", "2", "--micro-batch", "1", "--opd-rollout-steps", "2"] if opd \
+        else ["--pp", "2", "--microbatches", "2", "--micro-batch", "1", "--act-checkpoint", "fp8"]
+    r = subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes", "1", "--nproc-per-node", "1" if opd else "2",
+                        "--master-addr", "127.0.0.1", "--master-port", str(port), "train_pp.py", "--out", str(tmp_path),
+                        "--size", "nano", "--te-size", "states-nano", "--res", "128", "--steps", "1", "--log-every", "1",
+                        "--fp8"] + mode, cwd=ROOT, capture_output=True, text=True, timeout=600,
+                       env=dict(os.environ, CUDA_VISIBLE_DEVICES="", DIST_BACKEND="gloo"))
+    assert r.returncode == 0 and "step 1/1" in r.stdout, r.stdout[-2000:] + r.stderr[-3000:]

@@ -1,0 +1,161 @@
+"""The DiT on 8-bit products and with 8-bit activation checkpoints on the GPU, and the operators in a run together."""
+import pytest
+import torch
+
+from trenowanie_generatora_obrazkow_b200.ops import blocks8 as B8
+from trenowanie_generatora_obrazkow_b200.ops import fused as Fz
+from trenowanie_generatora_obrazkow_b200.ops._ext import check_errors
+
+pytestmark = pytest.mark.gpu
+
+
+def _model():
+    from trenowanie_generatora_obrazkow_b200.models import DenoiserConfig, LMEncoderConfig, build_models
+    den_cfg = DenoiserConfig(dim=512, depth=2, heads=4, mlp_hidden=1408, text_dim=512, latent_size=16)
+    te_cfg = LMEncoderConfig(repo="", tok_suffix="", lm_dim=256, skip_last=0, dim=512, depth=1, heads=8, kv_heads=2,
+                             head_dim=64, mlp_hidden=1408, max_tokens=32, backend="states")
+    torch.manual_seed(0)
+    te, den = build_models(den_cfg, te_cfg, device="cuda")
+    te.init_weights(), den.init_weights()
+    with torch.no_grad():
+        for p in list(te.parameters()) + list(den.parameters()):
+            p.add_(0.02 * torch.randn_like(p))
+    return te, den
+
+
+def _step(te, den, mode=False):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(4, 128, 16, 16, device="cuda", generator=g)
+    t = torch.rand(4, device="cuda", generator=g)
+    st = torch.randn(4, 32, 256, device="cuda", generator=g).bfloat16()
+    te.checkpoint_blocks = den.checkpoint_blocks = mode
+    params = list(te.parameters()) + list(den.parameters())
+    for p in params:
+        p.grad = None
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    text, valid = te(lm_states=st)
+    out = den(x, t, text, valid)
+    held = torch.cuda.memory_allocated() - base
+    out.float().square().mean().backward()
+    torch.cuda.synchronize()
+    check_errors("cuda")
+    return out.detach().float(), [None if p.grad is None else p.grad.clone() for p in params], held
+
+
+def _apart(a, b):
+    a, b = (torch.cat([g.flatten() for g in x if g is not None]) for x in (a, b))
+    return ((a - b).norm() / b.norm()).item()
+
+
+def test_dit_on_8_bit_products():
+    from trenowanie_generatora_obrazkow_b200.models.quant import use_fp8
+    te, den = _model()
+    plain, grads, _ = _step(te, den)
+    use_fp8(te), use_fp8(den)
+    out, g8, _ = _step(te, den)
+    # each value is off by at most 2^-4 of itself; sums of many add up like noise
+    assert 0 < ((out - plain).norm() / plain.norm()).item() < 0.1
+    assert [g is None for g in grads] == [g is None for g in g8]
+    assert _apart(g8, grads) < 0.1
+    again, g9, _ = _step(te, den)
+    assert torch.equal(again, out)
+    with torch.no_grad():
+        g = torch.Generator(device="cuda").manual_seed(3)
+        x = torch.randn(4, 128, 16, 16, device="cuda", generator=g)
+        t = torch.rand(4, device="cuda", generator=g)
+        st = torch.randn(4, 32, 256, device="cuda", generator=g).bfloat16()
+        text, valid = te(lm_states=st)
+        held = den(x, t, text, valid).float()
+    assert ((held - out).norm() / out.norm()).item() < 0.02  # held weights: the same products without a graph
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_checkpoint_mode_fp8(fp8):
+    from trenowanie_generatora_obrazkow_b200.models.quant import use_fp8
+    te, den = _model()
+    if fp8:
+        use_fp8(te), use_fp8(den)
+    plain, grads, held = _step(te, den)
+    sel, _, held_sel = _step(te, den, "selective")
+    out, g8, held8 = _step(te, den, "fp8")
+    assert ((out - plain).norm() / plain.norm()).item() < 0.01  # the SwiGLU kernels differ by a rounding
+    assert _apart(g8, grads) < 0.05
+    if not fp8:
+        assert held8 < held_sel < held, (held8, held_sel, held)
+
+
+def test_trainer_step_and_optimizer_on_8_bit_products():
+    from trenowanie_generatora_obrazkow_b200.models import DenoiserConfig, LMEncoderConfig
+    from trenowanie_generatora_obrazkow_b200.train.trainer import TrainConfig, Trainer
+    den = DenoiserConfig(dim=512, depth=2, heads=4, mlp_hidden=1408, text_dim=512, latent_size=16)
+    te = LMEncoderConfig(repo="", tok_suffix="", lm_dim=256, skip_last=0, dim=512, depth=1, heads=8, kv_heads=2,
+                         head_dim=64, mlp_hidden=1408, max_tokens=32, backend="states")
+    device = torch.device("cuda", 0)
+    tr = Trainer(den, te, TrainConfig(global_batch=4, micro_batch=2, steps=10, fp8=True), device)
+    before = tr.den.blocks[0].mlp.in_proj.weight.detach().clone()
+    batch = {"x0": torch.randn(4, 128, 16, 16, device=device),
+             "lm_states": torch.randn(4, 32, 256, device=device, dtype=torch.bfloat16)}
+    losses = [tr.step(batch) for _ in range(2)]
+    torch.cuda.synchronize()
+    check_errors(device)
+    assert all(torch.isfinite(v).item() for v in losses)
+    assert tr.den.blocks[0].mlp.in_proj.weight.grad.dtype == torch.float32
+    assert not torch.equal(before, tr.den.blocks[0].mlp.in_proj.weight)
+
+
+def test_operators_in_a_run():
+    """Packing, a layer, the MLP, a layer on held weights and the checkpointed activation, one after another."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    r = lambda *s, std=1.0: torch.randn(*s, device="cuda", generator=g) * std  # noqa: E731
+    x = r(3, 111, 256).bfloat16().requires_grad_()
+    w0, w1, w2, w3 = r(320, 256, std=1 / 16), r(768, 320, std=1 / 18), r(320, 384, std=1 / 20), r(256, 320, std=1 / 18)
+    ws = [w.requires_grad_() for w in (w0, w1, w2)]
+    h = B8.linear_blocks(x, w0)
+    y = h + B8.mlp_blocks(h, w1, w2)
+    g0 = B8.swiglu_blocks(y)
+    g0.backward(torch.ones_like(g0))
+    # the same in fp32 torch operations without packing: noise of 8 bits apart
+    xr = x.detach().float().requires_grad_()
+    wr = [w.detach().clone().requires_grad_() for w in ws]
+    hr = xr @ wr[0].t()
+    a, b = (hr @ wr[1].t()).chunk(2, dim=-1)
+    yr = hr + (torch.nn.functional.silu(a) * b) @ wr[2].t()
+    p, q = yr.chunk(2, dim=-1)
+    gr = torch.nn.functional.silu(p) * q
+    gr.backward(torch.ones_like(gr))
+    for got, want in [(g0, gr), (x.grad, xr.grad)] + [(w.grad, v.grad) for w, v in zip(ws, wr)]:
+        assert ((got.float() - want).norm() / want.norm()).item() < 0.12
+    with torch.no_grad():
+        last = B8.linear_blocks(y, B8.quantize_blocks(w3))
+        few = B8.linear_blocks(y[:1, :9], B8.quantize_blocks(w3))
+        assert last.shape == (3, 111, 256)
+        assert torch.allclose(few.float(), last[:1, :9].float(), rtol=2 ** -7, atol=1e-2)
+    check_errors("cuda")
+
+
+@pytest.mark.parametrize("M", [0, 1, 7, 16, 17, 200])
+def test_mlp_on_held_weights(M):
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = torch.randn(M, 200, device="cuda", generator=g)
+    w1, w2 = torch.randn(512, 200, device="cuda", generator=g) / 14, torch.randn(72, 256, device="cuda", generator=g) / 16
+    y = B8.mlp_blocks(x, B8.quantize_blocks(w1), B8.quantize_blocks(w2))
+    want = B8.mlp_blocks(x, w1, w2)
+    # few rows sum in another order: a value of g at a border may be packed to its neighbour, 2^-3 of it
+    assert y.shape == want.shape and (M == 0 or ((y - want).norm() / want.norm()).item() < 0.01)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        B8.mlp_blocks(x.clone().requires_grad_(), B8.quantize_blocks(w1), B8.quantize_blocks(w2))
+    with pytest.raises(TypeError):
+        B8.mlp_blocks(x, w1, B8.quantize_blocks(w2))
+
+
+def test_block_linear_and_marked_layers():
+    from trenowanie_generatora_obrazkow_b200.models.quant import quantize
+    lin = torch.nn.Linear(300, 136, device="cuda")
+    lin.fp8 = True
+    x = torch.randn(2, 9, 300, device="cuda").bfloat16()
+    with torch.no_grad():
+        marked = Fz.linear(x, lin)
+    m = torch.nn.Sequential(lin)
+    assert torch.equal(quantize(m, "fp8_block")(x), marked)

@@ -119,9 +119,12 @@ def build_parser():
     a("--offload", action="store_true")
     a("--outer-comm", choices=["bf16", "fp32"], default="bf16")
     a("--muon-momentum-dtype", choices=["fp32", "bf16"], default="fp32")
-    a("--act-checkpoint", nargs="?", const="full", default=None, choices=["full", "selective"],
-      help="activation checkpointing per block: full recompute, or selective (keep GEMM / attention outputs, "
-           "recompute the norms, q/k-norm + RoPE and SwiGLU in the backward)")
+    a("--act-checkpoint", nargs="?", const="full", default=None, choices=["full", "selective", "fp8"],
+      help="activation checkpointing per block: full recompute, selective (keep GEMM / attention outputs, "
+           "recompute the norms, q/k-norm + RoPE and SwiGLU in the backward), or fp8 (selective with the SwiGLU's "
+           "input and output kept in 8 bits)")
+    a("--fp8", action="store_true", help="8-bit products (e4m3, a scale for each 128 values) in the blocks' linear layers, "
+      "forward and backward; weights, gradients and optimizer stay as they are")
     a("--workers", type=int, default=4)
     a("--seed", type=int, default=0)
     a("--log-every", type=int, default=None)
@@ -274,7 +277,7 @@ def main():
                      repa_until=args.repa_until, repa_every=args.repa_every, repa_target=args.repa_target,
                      irepa=args.irepa, text_bucket=args.text_bucket, length_sort=args.length_sort,
                      outer_lr=args.outer_lr, outer_momentum=args.outer_momentum, outer_comm=args.outer_comm,
-                     offload=args.offload, seed=args.seed, act_checkpoint=args.act_checkpoint,
+                     offload=args.offload, seed=args.seed, act_checkpoint=args.act_checkpoint, fp8=args.fp8,
                      random_lm=args.random_lm)
     tr = Trainer(den_cfg, te_cfg, tc, device)
     te, den = tr.te, tr.den

@@ -49,9 +49,12 @@ def build_parser():
     a("--microbatches", type=int, default=None, help="micro-batches per step and replica (default 4 x pp)")
     a("--micro-batch", type=int, default=4)
     a("--te-cost", type=float, default=1.0, help="text encoder + stem cost in blocks (stage balancing)")
-    a("--act-checkpoint", nargs="?", const="full", default=None, choices=["full", "selective"],
-      help="activation checkpointing per block: full recompute, or selective (keep GEMM / attention outputs, "
-           "recompute the norms, q/k-norm + RoPE and SwiGLU in the backward)")
+    a("--act-checkpoint", nargs="?", const="full", default=None, choices=["full", "selective", "fp8"],
+      help="activation checkpointing per block: full recompute, selective (keep GEMM / attention outputs, "
+           "recompute the norms, q/k-norm + RoPE and SwiGLU in the backward), or fp8 (selective with the SwiGLU's "
+           "input and output kept in 8 bits)")
+    a("--fp8", action="store_true", help="8-bit products (e4m3, a scale for each 128 values) in the blocks' linear layers, "
+      "forward and backward; weights, gradients and optimizer stay as they are")
     a("--te-checkpoint", action="store_true", help="recompute the text encoder in the backward (with --act-checkpoint "
       "the whole first stage is recomputed already)")
     a("--steps", type=int, default=100)
@@ -417,7 +420,10 @@ def run_fm(args, den_cfg, te_cfg, lay, device, ctl, text_group):
                       muon_gamma=args.muon_gamma, clip=args.clip, ema=args.ema, cfg_drop=args.cfg_drop,
                       seed=args.seed, t_shift=args.t_shift, grad_comm=grad_comm)
     tr = PPTrainer(den_cfg, te_cfg, cfg, device, args.pp, M, args.te_cost, world=world, groups=groups)
-    tr.model.act_checkpoint = args.act_checkpoint or False  # per block: "full" or "selective"
+    tr.model.act_checkpoint = args.act_checkpoint or False  # per block: "full", "selective" or "fp8"
+    if args.fp8:
+        from trenowanie_generatora_obrazkow_b200.models.quant import use_fp8
+        use_fp8(tr.model)
     if tr.first and args.te_checkpoint:
         tr.model.te_checkpoint = True
     step, samples = pp_checkpoint.resume(tr, args.out, args.resume_opt_mismatch, group=learner_group)
@@ -610,6 +616,9 @@ def run_opd(args, den_cfg, te_cfg, lay, device, ctl, text_group):
         return
     torch.manual_seed(args.seed)
     te, den = build_models(den_cfg, te_cfg, device=device)
+    if args.fp8:
+        from trenowanie_generatora_obrazkow_b200.models.quant import use_fp8
+        use_fp8(te), use_fp8(den)
     params = list(te.parameters()) + list(den.parameters())
     if role == "actor":
         jobs = RolloutActor(te, den, params, device, ctl, kw).serve()

@@ -307,41 +307,48 @@ at::Tensor gemm8(at::Tensor a, at::Tensor as, at::Tensor b, at::Tensor bs, int64
 }
 
 // ----------------------------------------------------------------------------------------------------------- linear
-// Q(x) W^T + bias with W held in 8 bits; no gradient
-at::Tensor linear8_frozen(at::Tensor x, at::Tensor codes, at::Tensor scales, int64_t cols, OptT bias, at::Tensor err) {
-  const Packed w = given_packed(codes, scales, cols, "linear_blocks: weight");
-  same_device(codes, x, "linear_blocks: weight");
-  check_matrix(x, "linear_blocks");
-  TORCH_CHECK(x.size(1) == cols, "linear_blocks: x [..., ", cols, "] expected, got ", x.size(1), " columns");
-  const bool graph = wants_grad({&x}, kWhat) || (given(bias) && wants_grad({&*bias}, kWhat));
-  TORCH_CHECK(!graph, "linear_blocks: a weight held in 8 bits passes no gradient on (use torch.no_grad() or detach x)");
-  const c10::cuda::CUDAGuard guard(x.device());
-  small_vector(bias, w.rows, x, "linear_blocks");
-  x = rows_of(x);
-  const at::Tensor b32 = bias_f32(bias);
-  at::Tensor y = fresh({x.size(0), w.rows}, x.scalar_type(), x);
-  elem_of(x, "linear_blocks");
-  if (y.numel() == 0) return y;
+// y = Q(x) w^T + bias; few rows of x in one launch, packed on the way
+void times_held(const at::Tensor& x, const Packed& w, const at::Tensor& y, const float* bias, int* err) {
+  if (y.numel() == 0) return;
   if (x.size(0) <= kFewRows) {
     FewRowsParams p{};
     p.x = x.data_ptr();
     p.ldx = row_stride(x);
     p.codes = w.codes;
     p.scales = w.scales;
-    p.bias = ptr_f32(b32);
+    p.bias = bias;
     p.y = y.data_ptr();
     p.M = (int)x.size(0);
     p.N = (int)w.rows;
-    p.K = (int)cols;
-    BLOCK_LAUNCH(few_rows_launch(p, elem_of(x, "linear_blocks"), at::cuda::getCurrentCUDAStream()), 1);
-    return y;
+    p.K = (int)w.cols;
+    BLOCK_LAUNCH(few_rows_launch(p, elem_of(x, kWhat), at::cuda::getCurrentCUDAStream()), 1);
+    return;
   }
   Packed q;
   Arena arena;
   arena.add(&q, x.size(0), x.size(1));
   const at::Tensor mem = arena.on(x);
   pack({x, &q, nullptr});
-  product(q, w, y, ptr_f32(b32), false, err_word(err, x));
+  product(q, w, y, bias, false, err);
+}
+void no_graph(std::initializer_list<const at::Tensor*> ts, const char* what) {
+  TORCH_CHECK(!wants_grad(ts, kWhat), what, ": a weight held in 8 bits passes no gradient on (use torch.no_grad() or detach x)");
+}
+// Q(x) W^T + bias with W held in 8 bits; no gradient
+at::Tensor linear8_frozen(at::Tensor x, at::Tensor codes, at::Tensor scales, int64_t cols, OptT bias, at::Tensor err) {
+  const Packed w = given_packed(codes, scales, cols, "linear_blocks: weight");
+  same_device(codes, x, "linear_blocks: weight");
+  check_matrix(x, "linear_blocks");
+  elem_of(x, "linear_blocks");
+  TORCH_CHECK(x.size(1) == cols && w.rows >= 1, "linear_blocks: x [..., ", cols, "] expected, got ", x.size(1), " columns");
+  const at::Tensor b = or_undefined(bias);
+  no_graph({&x, &b}, "linear_blocks");
+  const c10::cuda::CUDAGuard guard(x.device());
+  small_vector(bias, w.rows, x, "linear_blocks");
+  x = rows_of(x);
+  const at::Tensor b32 = bias_f32(bias);
+  at::Tensor y = fresh({x.size(0), w.rows}, x.scalar_type(), x);
+  times_held(x, w, y, ptr_f32(b32), err_word(err, x));
   return y;
 }
 
@@ -680,6 +687,32 @@ at::Tensor mlp8(at::Tensor x, at::Tensor w1, at::Tensor w2, at::Tensor err) {
   return y;
 }
 
+// with both weights held in 8 bits; no gradient
+at::Tensor mlp8_frozen(at::Tensor x, at::Tensor c1, at::Tensor s1, at::Tensor c2, at::Tensor s2, int64_t K, int64_t H,
+                       at::Tensor err) {
+  const Packed w1 = given_packed(c1, s1, K, "mlp_blocks: in_proj"), w2 = given_packed(c2, s2, H, "mlp_blocks: out_proj");
+  same_device(c1, x, "mlp_blocks: in_proj");
+  same_device(c2, x, "mlp_blocks: out_proj");
+  check_matrix(x, "mlp_blocks");
+  elem_of(x, "mlp_blocks");
+  TORCH_CHECK(x.size(1) == K && w1.rows == 2 * H && H >= 1 && w2.rows >= 1 && H % 128 == 0,
+              "mlp_blocks: x [..., K], in_proj [2 H, K] and out_proj [N, H] with H a multiple of 128 expected");
+  no_graph({&x}, "mlp_blocks");
+  const c10::cuda::CUDAGuard guard(x.device());
+  x = rows_of(x);
+  int* const e = err_word(err, x);
+  const int64_t M = x.size(0);
+  at::Tensor ab = fresh({M, 2 * H}, x.scalar_type(), x), y = fresh({M, w2.rows}, x.scalar_type(), x);
+  times_held(x, w1, ab, nullptr, e);
+  Packed g8;
+  Arena now;
+  now.add(&g8, M, H);
+  const at::Tensor mem = now.on(x);
+  swiglu_forward(ab, nullptr, nullptr, &g8, nullptr, e);
+  product(g8, w2, y, nullptr, false, e);
+  return y;
+}
+
 }  // namespace
 
 void bind_blocks8(pybind11::module_& m) {
@@ -698,6 +731,7 @@ void bind_blocks8(pybind11::module_& m) {
   m.def("linear8_frozen", &linear8_frozen, "x times a weight held in 8 bits");
   m.def("linear8", &linear8, "linear layer on 8-bit products, forward and backward");
   m.def("swiglu8", &swiglu8, "silu(a) b with its input kept in 8 bits for the backward");
+  m.def("mlp8_frozen", &mlp8_frozen, "SwiGLU MLP with weights held in 8 bits");
   m.def("mlp8", &mlp8, "SwiGLU MLP on 8-bit products, forward and backward");
 }
 

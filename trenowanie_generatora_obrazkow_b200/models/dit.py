@@ -36,6 +36,8 @@ class SwiGLU(nn.Module):
         self.out_proj = nn.Linear(hidden, dim, bias=False)
 
     def forward(self, h):
+        if Fz.marked_fp8(self.in_proj, self.out_proj):
+            return Fz.mlp_fp8(h, self.in_proj, self.out_proj)
         return Fz.linear(Fz.up_swiglu(h, self.in_proj), self.out_proj)
 
 
@@ -122,7 +124,7 @@ class Denoiser(nn.Module):
         self.norm = RMSNorm(dim)
         self.patch_out = nn.Linear(dim, cfg.latent_channels, bias=False)
         self._rope_cache = {}
-        self.checkpoint_blocks = False  # activation checkpointing: False, "full" / True or "selective"
+        self.checkpoint_blocks = False  # activation checkpointing: False, "full" / True, "selective" or "fp8"
 
     # ---------------------------------------------------------------------------------------------- RoPE tables
     def rope(self, h, w, device):
@@ -176,7 +178,7 @@ class Denoiser(nn.Module):
         hidden = None
         hi = len(self.blocks) if hi is None else hi
         for i in range(lo, hi):
-            # activation checkpointing: False, "full" (True) or "selective" (ops/fused.py run_block)
+            # activation checkpointing: False, "full" (True), "selective" or "fp8" (ops/fused.py run_block)
             x, pending = Fz.run_block(self.blocks[i], (x, pending, t6, text, text_len, cos, sin),
                                       self.checkpoint_blocks)
             if i + 1 == hidden_at:

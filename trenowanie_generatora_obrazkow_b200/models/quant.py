@@ -1,4 +1,5 @@
-"""Frozen quantized projections for teacher models (reference aurora/klein.py:45-107).
+"""Frozen quantized projections for teacher models (reference aurora/klein.py:45-107), and 8-bit products for this
+framework's own blocks.
 
 * ``QLinear``: 8-bit weights with one scale per group of ``group`` consecutive inputs of an output row, symmetric
   int8 (max |w| / 127) or fp8 e4m3 (max |w| / 448, e4m3's largest normal value); dequantised to the activation dtype
@@ -7,13 +8,19 @@
 * ``W8A8Linear``: per-output-channel int8 weights, dynamic per-token int8 activations, int32 accumulation. On CUDA
   the activations are quantised by one kernel and multiplied by the tcgen05 ``kind::i8`` GEMM with both scales
   applied in its epilogue (``ext().quantize_rows_i8``, ``ext().gemm_i8``); elsewhere ``torch._int_mm``. Used for
-  frozen teachers only; the training path never quantises.
-* ``quantize(module, kind)``: replaces every ``nn.Linear`` below ``module`` in place (kind "int8", "fp8" or
+  frozen teachers only.
+* ``BlockLinear``: e4m3 weights with a power-of-two scale for each 128 inputs, activations packed the same way in the call
+  (``ops.blocks8``): one launch for up to 16 rows, the block-scaled tcgen05 product above. No gradient.
+* ``quantize(module, kind)``: replaces every ``nn.Linear`` below ``module`` in place (kind "int8", "fp8", "fp8_block" or
   "w8a8"; w8a8 only where both feature counts are multiples of 8, as the int8 GEMM requires).
+* ``use_fp8(module)``: the linear layers of every DiT and text block below ``module`` run on 8-bit products, in training
+  forward and backward (fp32 master weights and gradients, ``ops.blocks8.linear_blocks`` / ``mlp_blocks``), without
+  gradients with weights packed once per version. Parameters and checkpoints keep their names and types.
 """
 import torch
 import torch.nn as nn
 
+from ..ops import blocks8 as B8
 from ..ops import fused as Fz
 
 
@@ -79,10 +86,37 @@ class W8A8Linear(nn.Module):
         return out.to(x.dtype).reshape(*x.shape[:-1], -1)
 
 
+class BlockLinear(nn.Module):
+    def __init__(self, lin: nn.Linear):
+        super().__init__()
+        w = B8.quantize_blocks(lin.weight.detach())
+        self.register_buffer("w", w.codes)
+        self.register_buffer("s", w.scales)
+        self.bias = lin.bias
+        self.in_features, self.out_features = lin.in_features, lin.out_features
+
+    @torch.no_grad()
+    def forward(self, x):
+        return B8.linear_blocks(x, B8.Blocks8(self.w, self.s, self.in_features), self.bias)
+
+
+def use_fp8(module: nn.Module, on: bool = True) -> nn.Module:
+    from .dit import DenoiserBlock
+    from .text import TextBlock
+    for block in module.modules():
+        if isinstance(block, (DenoiserBlock, TextBlock)):
+            for lin in block.modules():
+                if isinstance(lin, nn.Linear):
+                    lin.fp8 = on
+    return module
+
+
 def quantize(module: nn.Module, kind: str) -> nn.Module:
     for name, child in list(module.named_children()):
         if isinstance(child, nn.Linear):
-            if kind == "w8a8":
+            if kind == "fp8_block":
+                setattr(module, name, BlockLinear(child))
+            elif kind == "w8a8":
                 if child.in_features % 8 == 0 and child.out_features % 8 == 0:
                     setattr(module, name, W8A8Linear(child))
             else:

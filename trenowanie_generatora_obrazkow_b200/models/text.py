@@ -48,6 +48,8 @@ class SwiGLU(nn.Module):
         self.out_proj = nn.Linear(hidden, dim, bias=False)
 
     def forward(self, h):
+        if Fz.marked_fp8(self.in_proj, self.out_proj):
+            return Fz.mlp_fp8(h, self.in_proj, self.out_proj)
         return Fz.linear(Fz.swiglu(Fz.linear(h, self.in_proj)), self.out_proj)
 
 
@@ -70,7 +72,7 @@ class TextBlock(nn.Module):
 
 def _run_blocks(blocks, x, lens, cos, sin, final_norm, checkpoint=False):
     pending = None
-    for blk in blocks:  # checkpoint: False, "full" (True) or "selective" (ops/fused.py run_block)
+    for blk in blocks:  # checkpoint: False, "full" (True), "selective" or "fp8" (ops/fused.py run_block)
         x, pending = Fz.run_block(blk, (x, pending, lens, cos, sin), checkpoint)
     _, h = Fz.adanorm(x, pending, None, final_norm.weight)
     return h

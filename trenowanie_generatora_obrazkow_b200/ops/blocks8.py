@@ -94,6 +94,11 @@ def _weight_of(layer, what):
     raise TypeError(f"{what}: an nn.Linear, a weight tensor or a Blocks8 expected, got {type(layer).__name__}")
 
 
+def _no_graph(*ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError("a weight held in 8 bits passes no gradient on (use torch.no_grad() or detach x)")
+
+
 def linear_blocks(x, layer_or_weight, bias=None):
     """y = Q(x) Q(W)^T + b: x [..., K] (bf16, fp16 or fp32) -> [..., N] in x's type. W: an ``nn.Linear``, a weight tensor
     [N, K] (packed in the call) or a Blocks8 (held in 8 bits; passes no gradient on). bias [N] fp32 or a 16-bit type. Rows of
@@ -109,9 +114,7 @@ def linear_blocks(x, layer_or_weight, bias=None):
     x2 = x if x.dim() == 2 else x.reshape(-1, K)
     if not x.is_cuda:
         if isinstance(w, Blocks8):
-            if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-                raise RuntimeError("linear_blocks: a weight held in 8 bits passes no gradient on (use torch.no_grad() or "
-                                   "detach x)")
+            _no_graph(x, bias)
             y = R.in_blocks(x2) @ R.dequantize_blocks(*w).t()
             y = (y if bias is None else y + bias.float()).to(x.dtype)
         else:
@@ -135,20 +138,32 @@ def swiglu_blocks(ab):
 
 def mlp_blocks(x, in_proj, out_proj):
     """SwiGLU MLP on 8-bit products: [a | b] = Q(x) Q(W1)^T rounded to x's type, g = silu(a) b, y = Q(g) Q(W2)^T; x [..., K],
-    in_proj [2 H, K], out_proj [N, H] (``nn.Linear`` without bias, or weight tensors) -> [..., N]. With H a multiple of 128 the
-    activation kernels write and read g, [a | b] and their gradient in 8 bits only; other widths run ``linear_blocks``,
-    ``swiglu_blocks`` and ``linear_blocks`` (g is then rounded to x's type before it is packed)."""
+    in_proj [2 H, K], out_proj [N, H] (``nn.Linear`` without bias, weight tensors, or both Blocks8: held in 8 bits, no gradient)
+    -> [..., N]. With H a multiple of 128 the activation kernels write and read g, [a | b] and their gradient in 8 bits only;
+    other widths run ``linear_blocks``, ``swiglu_blocks`` and ``linear_blocks`` (g is then rounded to x's type before it is
+    packed)."""
     w1, b1 = _weight_of(in_proj, "mlp_blocks")
     w2, b2 = _weight_of(out_proj, "mlp_blocks")
     if b1 is not None or b2 is not None:
         raise ValueError("mlp_blocks: projections without bias expected")
-    if isinstance(w1, Blocks8) or isinstance(w2, Blocks8):
-        raise TypeError("mlp_blocks: weights held in 8 bits go through linear_blocks")
-    if w1.dim() != 2 or w2.dim() != 2 or w1.shape[0] != 2 * w2.shape[1] or x.dim() < 1 or x.shape[-1] != w1.shape[1]:
+    held = isinstance(w1, Blocks8)
+    if held != isinstance(w2, Blocks8):
+        raise TypeError("mlp_blocks: both weights held in 8 bits, or neither")
+    if len(w1.shape) != 2 or len(w2.shape) != 2 or w1.shape[0] != 2 * w2.shape[1] or x.dim() < 1 or x.shape[-1] != w1.shape[1]:
         raise ValueError(f"mlp_blocks: x [..., K], in_proj [2 H, K] and out_proj [N, H] expected, got {tuple(x.shape)}, "
                          f"{tuple(w1.shape)} and {tuple(w2.shape)}")
     if w2.shape[1] % 128:
         return linear_blocks(swiglu_blocks(linear_blocks(x, w1)), w2)
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    y = ext().mlp8(x2, w1, w2, _err_word(x)) if x.is_cuda else R.MlpBlocks.apply(x2, w1, w2)
+    if x.is_cuda:
+        if held:
+            y = ext().mlp8_frozen(x2, w1.codes, w1.scales, w2.codes, w2.scales, w1.cols, w2.cols, _err_word(x))
+        else:
+            y = ext().mlp8(x2, w1, w2, _err_word(x))
+    elif held:
+        _no_graph(x2)
+        g = R.swiglu_f32((R.in_blocks(x2) @ R.dequantize_blocks(*w1).t()).to(x.dtype))
+        y = (R.in_blocks(g) @ R.dequantize_blocks(*w2).t()).to(x.dtype)
+    else:
+        y = R.MlpBlocks.apply(x2, w1, w2)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], w2.shape[0])

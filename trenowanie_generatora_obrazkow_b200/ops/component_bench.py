@@ -3,7 +3,7 @@
   python -m trenowanie_generatora_obrazkow_b200.ops.component_bench ckpt --size 2b --blocks 4 --mb 16 --inflight 8
   python -m trenowanie_generatora_obrazkow_b200.ops.component_bench te --layers 4 8 12 --batch 32 --tokens 96
 
-ckpt  speed and peak memory of activation checkpointing (none / full / selective) for one pipeline stage's worth of
+ckpt  speed and peak memory of activation checkpointing (none / full / selective / fp8) for one pipeline stage's worth of
       denoiser blocks in a 1F1B-like pattern: ``inflight`` micro-batches are run forward and kept, then run backward
       in order (the activations a stage holds at once). Reported per mode: device ms per micro-batch forward +
       backward and the peak memory above the weights.
@@ -131,7 +131,7 @@ def main(argv=None):
     c.add_argument("--inflight", type=int, default=8)
     c.add_argument("--res", type=int, default=256)
     c.add_argument("--text-len", type=int, default=96)
-    c.add_argument("--modes", nargs="+", default=["none", "full", "selective"], choices=["none", "full", "selective"])
+    c.add_argument("--modes", nargs="+", default=["none", "full", "selective"], choices=["none", "full", "selective", "fp8"])
     c.add_argument("--iters", type=int, default=3)
     c.add_argument("--warmup", type=int, default=1)
     t = sub.add_parser("te")

@@ -17,6 +17,8 @@ autograd. Each CUDA op is a ``torch.autograd.Function`` whose backward is a hand
                     branch's norm and modulation).
 * ``axes_attention_core``  ``self_attention_core`` with such positions.
 * ``rope_axes``     q/k RMSNorm and rotary positions with several axes (time, height, width) from integer positions.
+* layers marked by ``models.quant.use_fp8`` run on the 8-bit products of ``blocks8.py`` (``linear``,
+                    ``mlp_fp8``).
 * ``varlen_attention`` packed variable-length (causal) attention for the frozen caption LM (inference only).
 """
 import math
@@ -24,6 +26,7 @@ import math
 import torch
 
 from . import _ext
+from . import blocks8 as B8
 from . import reference as R
 from ._ext import _ERR, err_buf, ext
 from .gemm import gemm
@@ -62,12 +65,39 @@ def swiglu_weight(p):
     return ent[1]
 
 
+def fp8_weight(p):
+    """8-bit copy (``blocks8.Blocks8``) of a weight for calls without gradients, cached like bf16_weight."""
+    ent = getattr(p, "_tgo_fp8", None)
+    ver = p._version
+    if ent is None or ent[0] != ver or ent[1].codes.device != p.device or ent[1].shape != p.shape:
+        p._tgo_fp8 = ent = (ver, B8.quantize_blocks(p.detach()))
+    return ent[1]
+
+
+def _trains(x, *ps):
+    return torch.is_grad_enabled() and (x.requires_grad or any(p is not None and p.requires_grad for p in ps))
+
+
+def marked_fp8(*layers):
+    """Whether all of these nn.Linear are marked for 8-bit products (``models.quant.use_fp8``)."""
+    return all(layer.__dict__.get("fp8") for layer in layers)
+
+
+def mlp_fp8(x, in_proj, out_proj):
+    """SwiGLU MLP of two marked layers (2 H gate | up rows, H inputs, no bias) on 8-bit products: packs the weights in the
+    call while gradients are recorded, else once per version of them."""
+    if x.is_cuda and x.dtype != torch.bfloat16:
+        x = x.to(torch.bfloat16)
+    w1, w2 = in_proj.weight, out_proj.weight
+    return B8.mlp_blocks(x, w1, w2) if _trains(x, w1, w2) else B8.mlp_blocks(x, fp8_weight(w1), fp8_weight(w2))
+
+
 def up_swiglu(x, layer):
     """silu(x Wg^T) * (x Wu^T) for an nn.Linear of (2H, D) gate | up rows. On CUDA without autograd (sampling) and
     H % 128 == 0: one GEMM whose epilogue applies the SwiGLU (the (M, 2H) product never reaches memory)."""
     w = layer.weight
     H = w.shape[0] // 2
-    if x.is_cuda and not (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)) and H % 128 == 0:
+    if x.is_cuda and not marked_fp8(layer) and not (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)) and H % 128 == 0:
         x2 = x.reshape(-1, x.shape[-1]).to(torch.bfloat16).contiguous()
         out = torch.empty(x2.shape[0], H, device=x.device, dtype=torch.bfloat16)
         ext().gemm_swiglu(x2, swiglu_weight(w), out, err_buf(x.device))
@@ -150,6 +180,7 @@ def _weight_grad_done(w, direct, g):
 # from tensors that are saved anyway (the residual stream, q/k/v, the up projection's output); everything else is
 # saved as usual, so no GEMM or attention is recomputed.
 _SAC_ACTIVE = [0]
+_PACK8_ACTIVE = [0]
 
 
 class _Recipe:
@@ -183,14 +214,29 @@ def _tag_view(view, base):
     r = getattr(base, "_tgo_recipe", None)
     if r is not None and view is not base and view.data_ptr() == base.data_ptr():
         view._tgo_recipe = (r[0], r[1], tuple(view.shape))
+    if getattr(base, "_tgo_pack8", False):
+        view._tgo_pack8 = True
+
+
+class _Held:
+    """A saved tensor in 8-bit blocks along its last axis."""
+    __slots__ = ("blocks", "shape", "dtype")
+
+    def __init__(self, t):
+        self.blocks = B8.quantize_blocks(t.detach().reshape(-1, t.shape[-1]))
+        self.shape, self.dtype = t.shape, t.dtype
 
 
 def _pack(t):
+    if getattr(t, "_tgo_pack8", False):
+        return _Held(t)
     r = getattr(t, "_tgo_recipe", None)
     return t if r is None else _Rebuild(*r)
 
 
 def _unpack(x):
+    if isinstance(x, _Held):
+        return B8.dequantize_blocks(x.blocks, x.dtype).view(x.shape)
     if not isinstance(x, _Rebuild):
         return x
     out = x.recipe.get(x.index)
@@ -211,11 +257,28 @@ class selective_recompute:
         return self._hooks.__exit__(*exc)
 
 
+class packed_checkpoint(selective_recompute):
+    """selective_recompute with the SwiGLU's input and output kept in 8-bit blocks (3 H bytes a token instead of the input's
+    4 H): the SwiGLU backward reads its input from 8 bits, the down projection's weight gradient the output."""
+
+    def __enter__(self):
+        _PACK8_ACTIVE[0] += 1
+        return super().__enter__()
+
+    def __exit__(self, *exc):
+        _PACK8_ACTIVE[0] -= 1
+        return super().__exit__(*exc)
+
+
 def run_block(block, args, mode):
     """block(*args) with activation checkpointing: mode None / False (none), "full" / True (recompute the whole
-    block in the backward) or "selective" (recompute only its elementwise results)."""
+    block in the backward), "selective" (recompute only its elementwise results) or "fp8" (selective, the SwiGLU's input and
+    output in 8 bits)."""
     if not mode or not torch.is_grad_enabled():
         return block(*args)
+    if mode == "fp8":
+        with packed_checkpoint():
+            return block(*args)
     if mode == "selective":
         with selective_recompute():
             return block(*args)
@@ -266,6 +329,10 @@ def linear(x, layer_or_weight, bias=None):
     """y = x @ W^T (+ b). Accepts an ``nn.Linear`` (its weight and bias) or a weight tensor."""
     if isinstance(layer_or_weight, torch.nn.Linear):
         weight, bias = layer_or_weight.weight, layer_or_weight.bias
+        if marked_fp8(layer_or_weight):
+            if x.is_cuda and x.dtype != torch.bfloat16:
+                x = x.to(torch.bfloat16)
+            return B8.linear_blocks(x, weight if _trains(x, weight, bias) else fp8_weight(weight), bias)
     else:
         weight = layer_or_weight
     if not x.is_cuda:
@@ -687,6 +754,10 @@ def fm_inputs(x0, eps, t):
 
 
 def swiglu(ab):
+    if _PACK8_ACTIVE[0]:
+        g = B8.swiglu_blocks(ab)
+        g._tgo_pack8 = True
+        return g
     if not ab.is_cuda:
         return R.swiglu(ab)
     ab = ab.contiguous()

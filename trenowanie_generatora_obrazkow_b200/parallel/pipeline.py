@@ -158,7 +158,7 @@ class StageModel(nn.Module):
         from ..ops import fused as Fz
         cos, sin = self.rope(side, side, x.device)
         pending = None
-        for blk in self.blocks:  # act_checkpoint: False, "full" or "selective" (ops/fused.py run_block)
+        for blk in self.blocks:  # act_checkpoint: False, "full", "selective" or "fp8" (ops/fused.py run_block)
             x, pending = Fz.run_block(blk, (x, pending, t6, text, text_len, cos, sin), self.act_checkpoint)
         if self.last:
             from ..ops import fused as Fz

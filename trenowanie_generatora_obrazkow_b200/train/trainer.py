@@ -90,7 +90,8 @@ class TrainConfig:
     outer_comm: str = "bf16"
     offload: bool = False
     seed: int = 0
-    act_checkpoint: object = False  # False, "full" (or True) or "selective"
+    act_checkpoint: object = False  # False, "full" (or True), "selective" or "fp8" (SwiGLU tensors kept in 8 bits)
+    fp8: bool = False               # 8-bit products in the blocks' linear layers (models/quant.py use_fp8)
     random_lm: bool = False
     moe_experts: int = 0          # > 0: every moe_every-th block's MLP becomes an MoE layer
     moe_top_k: int = 2
@@ -131,7 +132,7 @@ class Trainer:
             from ..models.moe import MoEMLP, moe_denoiser
             ep_group = dist.group.WORLD if (cfg.expert_parallel and self.distributed and self.world > 1) else None
             # fully recomputed blocks would replay the peer exchange (its epochs): those use NCCL
-            transport = cfg.moe_transport if cfg.act_checkpoint in (False, None, "", "selective") else "nccl"
+            transport = cfg.moe_transport if cfg.act_checkpoint in (False, None, "", "selective", "fp8") else "nccl"
             moe_denoiser(den, cfg.moe_experts, cfg.moe_top_k, cfg.moe_hidden, cfg.moe_every, cfg.moe_capacity, ep_group,
                          transport)
             torch.manual_seed(cfg.seed * 7919 + (self.rank if ep_group is not None else 0))
@@ -144,6 +145,9 @@ class Trainer:
                     if ep_group is not None:
                         self.expert_params += [m.w_in, m.w_out]
         self.den.checkpoint_blocks = cfg.act_checkpoint
+        if cfg.fp8:
+            from ..models.quant import use_fp8
+            use_fp8(self.den), use_fp8(self.te)
         self.lm_te = isinstance(te, LMTextEncoder)
         if self.lm_te:
             te.checkpoint_blocks = cfg.act_checkpoint
