@@ -22,6 +22,8 @@
 
 namespace tgo {
 
+int num_sms();  // gemm.cu
+
 namespace {
 
 constexpr int TILE = 128, PACK_THREADS = 256;
@@ -161,6 +163,21 @@ __device__ __forceinline__ uint2 codes8(const Eight<T>& v, float inv) {
   return make_uint2(codes4(mul2(v.pair(0), k), mul2(v.pair(1), k)), codes4(mul2(v.pair(2), k), mul2(v.pair(3), k)));
 }
 
+// the largest finite magnitude of each row; infinities become NaN (one test for all rows)
+template <typename T, int R>
+__device__ __forceinline__ void finite_tops(Eight<T> (&v)[R], float (&m)[R]) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < R; ++i) top = fmaxf(top, m[i] = v[i].top());
+  if (top == INFINITY) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      v[i].drop_infinities();
+      m[i] = v[i].top();
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------- tile output
 struct Side {             // one 8-bit output
   uint8_t* codes;
@@ -180,28 +197,30 @@ struct TileShared {
 template <int R>
 __device__ __forceinline__ void row_scales(const float (&m)[R], uint8_t* scales, int r0, int kb, int nb, int quads, int rows,
                                            float (&inv)[R]) {
+  static_assert(R == 2 || R == 4 || R == 8, "rows of a thread");
+  constexpr int KEPT = R == 8 ? 1 : R == 4 ? 2 : 3;  // lane bits below those that choose the row
   const int lane = threadIdx.x & 31;
-  float a[R / 2], b[R == 8 ? 2 : 1], c;
+  float a[R];
 #pragma unroll
-  for (int k = 0; k < R / 2; ++k) {
-    const float keep = (lane & 8) ? m[R / 2 + k] : m[k], send = (lane & 8) ? m[k] : m[R / 2 + k];
-    a[k] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, 8));
-  }
+  for (int i = 0; i < R; ++i) a[i] = m[i];
 #pragma unroll
-  for (int k = 0; k < R / 4; ++k) {
-    const float keep = (lane & 4) ? a[R / 4 + k] : a[k], send = (lane & 4) ? a[k] : a[R / 4 + k];
-    b[k] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, 4));
+  for (int n = R / 2, bit = 8; bit > 0; n /= 2, bit /= 2) {
+    if (n > 0) {
+#pragma unroll
+      for (int k = 0; k < n; ++k) {
+        const float keep = (lane & bit) ? a[n + k] : a[k], send = (lane & bit) ? a[k] : a[n + k];
+        a[k] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, bit));
+      }
+    } else {
+      a[0] = fmaxf(a[0], __shfl_xor_sync(0xffffffffu, a[0], bit));
+    }
   }
-  if constexpr (R == 8) c = fmaxf((lane & 2) ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, (lane & 2) ? b[0] : b[1], 2));
-  else c = fmaxf(b[0], __shfl_xor_sync(0xffffffffu, b[0], 2));
-  c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, 1));
-  const int byte = scale_byte(c);
+  const int byte = scale_byte(a[0]);
   const float mine = scale_inv(byte);
 #pragma unroll
-  for (int i = 0; i < R; ++i)
-    inv[i] = __shfl_sync(0xffffffffu, mine, (lane & 16) | (R == 8 ? ((i & 4) << 1) | ((i & 2) << 1) | ((i & 1) << 1) : i << 2));
-  if ((lane & (R == 8 ? 1 : 3)) == 0) {
-    const int r = r0 + ((lane & 15) >> (R == 8 ? 1 : 2));
+  for (int i = 0; i < R; ++i) inv[i] = __shfl_sync(0xffffffffu, mine, (lane & 16) | (i << KEPT));
+  if ((lane & ((1 << KEPT) - 1)) == 0) {
+    const int r = r0 + ((lane & 15) >> KEPT);
     if (r < ((rows + TILE - 1) & ~(TILE - 1))) {
       uint8_t* s = scales + scale_at(r, kb, quads);
       s[0] = (uint8_t)byte;
@@ -218,18 +237,7 @@ __device__ __forceinline__ void emit(Eight<T> (&v)[8], const Side& r, const Side
                                      int nmb, TileShared& sh) {
   const int l16 = threadIdx.x & 15, rg = threadIdx.x >> 4;
   float m[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m[i] = v[i].top();
-  if (fmaxf(max3(max3(m[0], m[1], m[2]), m[3], m[4]), max3(m[5], m[6], m[7])) == INFINITY) {
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k == i) v[k].drop_infinities();
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = v[i].top();
-  }
+  finite_tops(v, m);
   if constexpr (COLS) {
     float2 t[4];
 #pragma unroll
@@ -469,53 +477,45 @@ __device__ __forceinline__ float sigmoid(float a) {
   }
 }
 
-// scale of row r's block b for the eight rows from r0 = 8 k on: 16 bytes apart
-__device__ __forceinline__ const uint8_t* scales_from(const Side& s, int r0, int b) { return s.scales + scale_at(r0, b, s.quads); }
-
-// g in ab's type, the checkpoint of ab in 8 bits. Rows alone: a thread holds 8 columns of RPT rows. The checkpoint's blocks
-// are those of a [M, 2 Hp] matrix: a's first, then b's.
-template <typename T, bool CK>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) swiglu8_fwd_kernel(const T* __restrict__ ab, long long ld, int M, int H, bool vec,
-                                                          bool vec_g, T* __restrict__ g, Side ck) {
-  constexpr int RPT = 4;
+// g in ab's type, the checkpoint of ab in 8 bits. Rows alone: a thread holds 8 columns of ROW_R rows (two: enough warps to keep
+// the memory busy; at 32768 x 5504 the
+// backward took 265 us with four, 212 with two). The checkpoint's
+// blocks are those of a [M, 2 Hp] matrix: a's first, then b's. Rows past the last are read as the last one and not written.
+constexpr int ROW_R = 2;
+template <typename T, bool VEC, bool CK>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) swiglu8_fwd_kernel(const T* __restrict__ ab, long long ld, int M, int H, bool vec_g,
+                                                          T* __restrict__ g, Side ck) {
   const int nhb = (H + TILE - 1) / TILE;
   const int hb = blockIdx.x % nhb, l16 = threadIdx.x & 15;
-  const int r0 = (blockIdx.x / nhb) * 16 * RPT + (threadIdx.x >> 4) * RPT;
+  const int r0 = (blockIdx.x / nhb) * 16 * ROW_R + (threadIdx.x >> 4) * ROW_R;
   const int c = hb * TILE + 8 * l16, n = max(0, min(8, H - c));
-  Eight<T> a[RPT], b[RPT];
-  const T* p = ab + (long long)r0 * ld + c;
+  Eight<T> a[ROW_R], b[ROW_R];
 #pragma unroll
-  for (int i = 0; i < RPT; ++i, p += ld) {
-    a[i].load(p, r0 + i < M ? n : 0, vec);
-    b[i].load(p + H, r0 + i < M ? n : 0, vec);
+  for (int i = 0; i < ROW_R; ++i) {
+    const T* p = ab + (long long)min(r0 + i, M - 1) * ld + c;
+    a[i].load(p, n, VEC);
+    b[i].load(p + H, n, VEC);
   }
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
+  for (int i = 0; i < ROW_R; ++i) {
     Eight<T> o;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float2 x = a[i].pair(w), y = b[i].pair(w);
       o.set(w, make_float2(x.x * sigmoid<sizeof(T) == 4>(x.x) * y.x, x.y * sigmoid<sizeof(T) == 4>(x.y) * y.y));
     }
-    o.store(g + (long long)(r0 + i) * H + c, r0 + i < M ? n : 0, vec_g);
+    if (r0 + i < M) o.store(g + (long long)(r0 + i) * H + c, n, vec_g);
   }
   if constexpr (CK) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      Eight<T>(&v)[RPT] = h == 0 ? a : b;
-      float m[RPT], inv[RPT];
-#pragma unroll
-      for (int i = 0; i < RPT; ++i) {
-        m[i] = v[i].top();
-        if (m[i] == INFINITY) {
-          v[i].drop_infinities();
-          m[i] = v[i].top();
-        }
-      }
+      Eight<T>(&v)[ROW_R] = h == 0 ? a : b;
+      float m[ROW_R], inv[ROW_R];
+      finite_tops(v, m);
       row_scales(m, ck.scales, r0, h * nhb + hb, 2 * nhb, ck.quads, ck.rows, inv);
       uint8_t* d = ck.codes + (long long)r0 * ck.width + (long long)h * nhb * TILE + c;
 #pragma unroll
-      for (int i = 0; i < RPT; ++i, d += ck.width)
+      for (int i = 0; i < ROW_R; ++i, d += ck.width)
         if (r0 + i < M) *reinterpret_cast<uint2*>(d) = codes8(v[i], inv[i]);
     }
   }
@@ -530,31 +530,28 @@ __device__ __forceinline__ void swiglu_grad(float2 a, float2 b, float2 dg, float
   da = mul2(mul2(t, b), u);
   db = mul2(t, a);
 }
-template <typename T>
-__global__ void __launch_bounds__(256) swiglu8_bwd_kernel(const T* __restrict__ dg, long long ld, int M, int H, bool vec,
-                                                          bool vec_d, T* __restrict__ dab, Side ck) {
-  constexpr int RPT = 4;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) swiglu8_bwd_kernel(const T* __restrict__ dg, long long ld, int M, int H, bool vec_d,
+                                                          T* __restrict__ dab, Side ck) {
   const int nhb = (H + TILE - 1) / TILE;
   const int hb = blockIdx.x % nhb, l16 = threadIdx.x & 15;
-  const int r0 = (blockIdx.x / nhb) * 16 * RPT + (threadIdx.x >> 4) * RPT;
+  const int r0 = (blockIdx.x / nhb) * 16 * ROW_R + (threadIdx.x >> 4) * ROW_R;
   const int c = hb * TILE + 8 * l16, n = max(0, min(8, H - c));
-  Eight<T> dv[RPT];
-  uint2 ca[RPT], cb[RPT];
-  float ka[RPT], kb[RPT];
-  const T* p = dg + (long long)r0 * ld + c;
-  const uint8_t* q = ck.codes + (long long)r0 * ck.width + c;
-  const uint8_t *sa = scales_from(ck, r0, hb), *sb = scales_from(ck, r0, nhb + hb);
+  Eight<T> dv[ROW_R];
+  uint2 ca[ROW_R], cb[ROW_R];
+  float ka[ROW_R], kb[ROW_R];
 #pragma unroll
-  for (int i = 0; i < RPT; ++i, p += ld, q += ck.width) {
-    const bool in = r0 + i < M;
-    dv[i].load(p, in ? n : 0, vec);
-    ca[i] = in ? __ldg(reinterpret_cast<const uint2*>(q)) : make_uint2(0u, 0u);
-    cb[i] = in ? __ldg(reinterpret_cast<const uint2*>(q + (long long)nhb * TILE)) : make_uint2(0u, 0u);
-    ka[i] = in ? scale_of(__ldg(sa + 16 * i)) : 0.f;
-    kb[i] = in ? scale_of(__ldg(sb + 16 * i)) : 0.f;
+  for (int i = 0; i < ROW_R; ++i) {
+    const int r = min(r0 + i, M - 1);
+    dv[i].load(dg + (long long)r * ld + c, n, VEC);
+    const uint8_t* q = ck.codes + (long long)r * ck.width + c;
+    ca[i] = __ldg(reinterpret_cast<const uint2*>(q));
+    cb[i] = __ldg(reinterpret_cast<const uint2*>(q + (long long)nhb * TILE));
+    ka[i] = scale_of(__ldg(ck.scales + scale_at(r, hb, ck.quads)));
+    kb[i] = scale_of(__ldg(ck.scales + scale_at(r, nhb + hb, ck.quads)));
   }
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
+  for (int i = 0; i < ROW_R; ++i) {
     float2 a[4], b[4];
     values8(ca[i], ka[i], a);
     values8(cb[i], kb[i], b);
@@ -566,9 +563,11 @@ __global__ void __launch_bounds__(256) swiglu8_bwd_kernel(const T* __restrict__ 
       oa.set(w, da);
       ob.set(w, db);
     }
-    T* o = dab + (long long)(r0 + i) * 2 * H + c;
-    oa.store(o, r0 + i < M ? n : 0, vec_d);
-    ob.store(o + H, r0 + i < M ? n : 0, vec_d);
+    if (r0 + i < M) {
+      T* o = dab + (long long)(r0 + i) * 2 * H + c;
+      oa.store(o, n, vec_d);
+      ob.store(o + H, n, vec_d);
+    }
   }
 }
 
@@ -587,21 +586,11 @@ struct QtOut {  // transposed side of one tile: maxima of the 16 warps, 2^-e, co
   uint4 t[TILE * TILE / 16];  // column c's four bytes of rows 4 i .. at word c * 32 + (i ^ 2 (c / 8 % 16))
 };
 
-template <typename T>
-__device__ __forceinline__ float finite_top(Eight<T>& v) {
-  float m = v.top();
-  if (m == INFINITY) {
-    v.drop_infinities();
-    m = v.top();
-  }
-  return m;
-}
 // rows of the tile into d: blocks along the columns
 template <typename T>
 __device__ __forceinline__ void qt_rows(Eight<T> (&v)[QT_R], const Side& o, int r0, int kb, int nkb, int l16) {
   float m[QT_R], inv[QT_R];
-#pragma unroll
-  for (int i = 0; i < QT_R; ++i) m[i] = finite_top(v[i]);
+  finite_tops(v, m);
   row_scales(m, o.scales, r0, kb, nkb, o.quads, o.rows, inv);
   uint8_t* d = o.codes + (long long)r0 * o.width + kb * TILE + 8 * l16;
 #pragma unroll
@@ -822,14 +811,13 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
 
 template <typename K>
 cudaError_t qt_launch(K kern, size_t shared, std::atomic<uint64_t>& set, int* grid, long long tiles) {
-  int dev = 0, sms = 0;
+  int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess && (dev > 63 || !((set.load(std::memory_order_relaxed) >> dev) & 1))) {  // once per device
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
     if (e == cudaSuccess && dev <= 63) set.fetch_or(1ull << dev);
   }
-  *grid = (int)std::min<long long>(tiles, sms);
+  *grid = (int)std::min<long long>(tiles, num_sms());
   return e;
 }
 template <typename T, bool QT, bool CK>
@@ -859,14 +847,21 @@ cudaError_t swiglu_fwd_typed(const Swiglu8Params& p, cudaStream_t s) {
     return p.ck != nullptr ? swiglu_fwd_q<T, false, true>(*p.map, p, tiles, ck, g8, g8t, s)
                            : swiglu_fwd_q<T, false, false>(*p.map, p, tiles, ck, g8, g8t, s);
   }
-  const long long blocks = (long long)nhb * ((p.M + 63) / 64);
+  const long long blocks = (long long)nhb * ((p.M + 16 * ROW_R - 1) / (16 * ROW_R));
   if (blocks >= (1ll << 31)) return cudaErrorInvalidValue;
   const bool vec = p.H % 8 == 0 && aligned16(p.ab, p.ld * (long long)sizeof(T));
   const bool vec_g = p.H % 8 == 0 && aligned16(p.g, 0);
   const T* ab = static_cast<const T*>(p.ab);
   T* g = static_cast<T*>(p.g);
-  if (p.ck != nullptr) swiglu8_fwd_kernel<T, true><<<(int)blocks, 256, 0, s>>>(ab, p.ld, p.M, p.H, vec, vec_g, g, ck);
-  else swiglu8_fwd_kernel<T, false><<<(int)blocks, 256, 0, s>>>(ab, p.ld, p.M, p.H, vec, vec_g, g, ck);
+#define FWD(VEC, CK) swiglu8_fwd_kernel<T, VEC, CK><<<(int)blocks, 256, 0, s>>>(ab, p.ld, p.M, p.H, vec_g, g, ck)
+  if (p.ck != nullptr) {
+    if (vec) FWD(true, true);
+    else FWD(false, true);
+  } else {
+    if (vec) FWD(true, false);
+    else FWD(false, false);
+  }
+#undef FWD
   return cudaGetLastError();
 }
 template <typename T>
@@ -886,56 +881,64 @@ cudaError_t swiglu_bwd_typed(const Swiglu8BwdParams& p, cudaStream_t s) {
     kern<<<grid, QT_THREADS, sizeof(SwigluBwdShared<T>), s>>>(*p.map, *p.ck_map, p.M, p.H, ck, d8, d8t, p.err);
     return cudaGetLastError();
   }
-  const long long blocks = (long long)nhb * ((p.M + 63) / 64);
+  const long long blocks = (long long)nhb * ((p.M + 16 * ROW_R - 1) / (16 * ROW_R));
   if (blocks >= (1ll << 31)) return cudaErrorInvalidValue;
   const bool vec = p.H % 8 == 0 && aligned16(p.dg, p.ld * (long long)sizeof(T));
   const bool vec_d = p.H % 8 == 0 && aligned16(p.dab, 0);
-  swiglu8_bwd_kernel<T><<<(int)blocks, 256, 0, s>>>(static_cast<const T*>(p.dg), p.ld, p.M, p.H, vec, vec_d,
-                                                    static_cast<T*>(p.dab), ck);
+  const T* dg = static_cast<const T*>(p.dg);
+  T* dab = static_cast<T*>(p.dab);
+  if (vec) swiglu8_bwd_kernel<T, true><<<(int)blocks, 256, 0, s>>>(dg, p.ld, p.M, p.H, vec_d, dab, ck);
+  else swiglu8_bwd_kernel<T, false><<<(int)blocks, 256, 0, s>>>(dg, p.ld, p.M, p.H, vec_d, dab, ck);
   return cudaGetLastError();
 }
 
 // --------------------------------------------------------------------------------------------------------- few rows
-// y [M, N] = Q(x) W^T + bias for at most 16 rows of x (tokens of a serving step). Reading W bounds it (N Kp bytes): one
-// launch, x is packed where it is used. A CTA owns 16 rows of W, its warps every eighth block of 128; all of a warp's
-// loads of a block are 16 bytes per lane and independent. The products run on mma.m16n8k32 (W rows x tokens); the order
-// of k inside a block is free, so a lane's 16 consecutive bytes serve as its operand words of two instructions, for W
-// and for x alike. A block's sum is scaled in fp32, the warps' sums are added in order.
-__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
+// y [M, N] = Q(x) W^T + bias for at most 16 rows of x (tokens of a serving step), in one launch: x is packed where it is used.
+// Reading W bounds it (N Kp bytes). A CTA owns 16 RT rows of W, each of up to 8 warps every eighth block of 128; a warp's loads
+// of a block are 16 bytes per lane and independent. e4m3 values are fp16 values, so the products run on mma.m16n8k16 (W rows
+// x tokens) with fp32 sums, after one conversion of two codes each; the order of k inside a block is free, so a lane's 16
+// consecutive bytes serve as its operands of four instructions, for W and for x alike. A block's sum is scaled in fp32, the
+// warps' sums are added in order.
+// One token 2048 -> 6144 (12.6 MB, 1.9 us at the copy rate): 5.3 us, of which a launch takes about 2; 6.0 with 4 warps, 6.6 with
+// 16 (two waves), 5.7 with the 8-bit form of the instruction.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// four codes as two fp16 pairs
+__device__ __forceinline__ void halves(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi) : "r"(codes));
+}
 
-template <typename T, int NT>  // NT: groups of eight rows of x
-__global__ void __launch_bounds__(256) few_rows_kernel(const FewRowsParams p, bool vec) {
-  __shared__ float part[8][16][8 * NT + 1];
+constexpr int FEW_WARPS = 8;
+template <typename T, int NT, int RT>  // NT: groups of eight rows of x
+__global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_kernel(const FewRowsParams p, bool vec) {
+  __shared__ float part[FEW_WARPS][16 * RT][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int warps = blockDim.x >> 5;
   const int nb = (p.K + TILE - 1) / TILE, quads = (nb + 3) / 4;
   const long long width = (long long)nb * TILE;
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * 16 * RT;
   const T* x = static_cast<const T*>(p.x);
-  float acc[NT][4];
+  float acc[RT][NT][4];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[r][i][0] = acc[r][i][1] = acc[r][i][2] = acc[r][i][3] = 0.f;
   for (int kb = warp; kb < nb; kb += warps) {
-    uint4 w[2][2];  // [row g, g + 8][half of the block]
-    float ws[2];
+    uint4 w[2 * RT][2];  // [row g + 8 r][half of the block]
+    float ws[2 * RT];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int n = n0 + g + 8 * r;
-      w[r][0] = w[r][1] = make_uint4(0u, 0u, 0u, 0u);
-      ws[r] = 0.f;
-      if (n < p.N) {
-        const uint8_t* src = p.codes + n * width + kb * TILE + 16 * t;
-        w[r][0] = __ldg(reinterpret_cast<const uint4*>(src));
-        w[r][1] = __ldg(reinterpret_cast<const uint4*>(src + 64));
-        ws[r] = scale_of(__ldg(p.scales + scale_at(n, kb, quads)));
-      }
+    for (int r = 0; r < 2 * RT; ++r) {
+      const int n = min(n0 + g + 8 * r, p.N - 1);  // rows past the last: not written
+      const uint8_t* src = p.codes + n * width + kb * TILE + 16 * t;
+      w[r][0] = __ldg(reinterpret_cast<const uint4*>(src));
+      w[r][1] = __ldg(reinterpret_cast<const uint4*>(src + 64));
+      ws[r] = scale_of(__ldg(p.scales + scale_at(n, kb, quads)));
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -946,58 +949,78 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const FewRowsParams p, bo
         const int c = kb * TILE + (h >> 1) * 64 + 16 * t + (h & 1) * 8;
         f[h].load(x + m * p.ldx + c, m < p.M ? max(0, min(8, p.K - c)) : 0, vec);
       }
-      float top = fmaxf(fmaxf(f[0].top(), f[1].top()), fmaxf(f[2].top(), f[3].top()));
-      if (top == INFINITY) {
-#pragma unroll
-        for (int h = 0; h < 4; ++h) f[h].drop_infinities();
-        top = fmaxf(fmaxf(f[0].top(), f[1].top()), fmaxf(f[2].top(), f[3].top()));
-      }
+      float tops[4];
+      finite_tops(f, tops);
+      float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int byte = scale_byte(top);
       const float inv = scale_inv(byte);
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
+      float d[RT][4] = {};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint2 lo = codes8(f[2 * h], inv), hi = codes8(f[2 * h + 1], inv);
-        mma_e4m3(d, w[0][h].x, w[1][h].x, w[0][h].y, w[1][h].y, lo.x, lo.y);
-        mma_e4m3(d, w[0][h].z, w[1][h].z, w[0][h].w, w[1][h].w, hi.x, hi.y);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t b0, b1;
+          halves(q == 0 ? lo.x : q == 1 ? lo.y : q == 2 ? hi.x : hi.y, b0, b1);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const uint4 &u = w[2 * r][h], &v = w[2 * r + 1][h];
+            uint32_t a0, a1, a2, a3;
+            halves(q == 0 ? u.x : q == 1 ? u.y : q == 2 ? u.z : u.w, a0, a2);
+            halves(q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w, a1, a3);
+            mma_f16(d[r], a0, a1, a2, a3, b0, b1);
+          }
+        }
       }
       // d: rows g, g + 8 of W, tokens 2 t, 2 t + 1, whose scales their own lanes hold
       const float s = scale_of(byte);
       const float s0 = __shfl_sync(0xffffffffu, s, 8 * t), s1 = __shfl_sync(0xffffffffu, s, 8 * t + 4);
-      acc[i][0] += d[0] * s0 * ws[0];
-      acc[i][1] += d[1] * s1 * ws[0];
-      acc[i][2] += d[2] * s0 * ws[1];
-      acc[i][3] += d[3] * s1 * ws[1];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        acc[r][i][0] += d[r][0] * s0 * ws[2 * r];
+        acc[r][i][1] += d[r][1] * s1 * ws[2 * r];
+        acc[r][i][2] += d[r][2] * s0 * ws[2 * r + 1];
+        acc[r][i][3] += d[r][3] * s1 * ws[2 * r + 1];
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    part[warp][g][8 * i + 2 * t] = acc[i][0];
-    part[warp][g][8 * i + 2 * t + 1] = acc[i][1];
-    part[warp][g + 8][8 * i + 2 * t] = acc[i][2];
-    part[warp][g + 8][8 * i + 2 * t + 1] = acc[i][3];
-  }
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      part[warp][16 * r + g][8 * i + 2 * t] = acc[r][i][0];
+      part[warp][16 * r + g][8 * i + 2 * t + 1] = acc[r][i][1];
+      part[warp][16 * r + g + 8][8 * i + 2 * t] = acc[r][i][2];
+      part[warp][16 * r + g + 8][8 * i + 2 * t + 1] = acc[r][i][3];
+    }
   __syncthreads();
   T* y = static_cast<T*>(p.y);
-  for (int at = threadIdx.x; at < 16 * 8 * NT; at += blockDim.x) {
-    const int m = at >> 4, r = at & 15, n = n0 + r;
-    if (m >= p.M || n >= p.N) continue;
+  for (int at = threadIdx.x; at < 16 * RT * p.M; at += blockDim.x) {
+    const int m = at / (16 * RT), r = at % (16 * RT), n = n0 + r;
+    if (n >= p.N) continue;
     float v = 0.f;
-    for (int w = 0; w < warps; ++w) v += part[w][r][m];
+    for (int k = 0; k < warps; ++k) v += part[k][r][m];
     if (p.bias != nullptr) v += p.bias[n];
     y[(long long)m * p.N + n] = from_f<T>(v);
   }
 }
 
 template <typename T>
-cudaError_t few_rows_typed(const FewRowsParams& p, cudaStream_t s) {
-  const int nb = (p.K + TILE - 1) / TILE, warps = std::min(8, nb);
+cudaError_t few_rows_typed(const FewRowsParams& p, int sms, cudaStream_t s) {
+  const int nb = (p.K + TILE - 1) / TILE, threads = std::min(FEW_WARPS, nb) * 32;
   const bool vec = p.K % 8 == 0 && aligned16(p.x, p.ldx * (long long)sizeof(T));
-  const int grid = (p.N + 15) / 16;
-  if (p.M <= 8) few_rows_kernel<T, 1><<<grid, warps * 32, 0, s>>>(p, vec);
-  else few_rows_kernel<T, 2><<<grid, warps * 32, 0, s>>>(p, vec);
+  // 32 rows of W share a packed x where they still fill the GPU
+  if ((p.N + 31) / 32 >= sms) {
+    const int grid = (p.N + 31) / 32;
+    if (p.M <= 8) few_rows_kernel<T, 1, 2><<<grid, threads, 0, s>>>(p, vec);
+    else few_rows_kernel<T, 2, 2><<<grid, threads, 0, s>>>(p, vec);
+  } else {
+    const int grid = (p.N + 15) / 16;
+    if (p.M <= 8) few_rows_kernel<T, 1, 1><<<grid, threads, 0, s>>>(p, vec);
+    else few_rows_kernel<T, 2, 1><<<grid, threads, 0, s>>>(p, vec);
+  }
   return cudaGetLastError();
 }
 
@@ -1054,7 +1077,7 @@ cudaError_t unpack8_launch(const uint8_t* codes, const uint8_t* scales, int R, i
 }
 cudaError_t few_rows_launch(const FewRowsParams& p, int elem, cudaStream_t s) {
   if (p.M <= 0 || p.M > kFewRows || p.N <= 0 || p.K <= 0) return cudaErrorInvalidValue;
-  return by_type(elem, [&](auto t) { return few_rows_typed<decltype(t)>(p, s); });
+  return by_type(elem, [&](auto t) { return few_rows_typed<decltype(t)>(p, num_sms(), s); });
 }
 cudaError_t swiglu8_fwd_launch(const Swiglu8Params& p, int elem, cudaStream_t s) {
   if (p.M <= 0 || p.H <= 0 || (p.g == nullptr) == (p.g8 == nullptr) || (p.g8t != nullptr && p.g8 == nullptr))

@@ -54,13 +54,13 @@ def quantize_blocks(x, side="rows"):
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"quantize_blocks: a matrix of at least one column expected, got {tuple(x.shape)}")
     M, K = x.shape
-    if not x.is_cuda:
-        got = ([R.quantize_blocks(x)] if side != "cols" else []) + ([R.quantize_blocks(x.t())] if side != "rows" else [])
-    else:
+    if x.is_cuda:
         t = ext().pack8(x, side != "cols", side != "rows")
-        got = [t[:2], t[2:]] if side == "both" else [t]
-    out = [Blocks8(*g, n) for g, n in zip(got, {"rows": (K,), "cols": (M,), "both": (K, M)}[side])]
-    return out[0] if len(out) == 1 else tuple(out)
+    else:
+        t = (R.quantize_blocks(x) if side != "cols" else ()) + (R.quantize_blocks(x.t()) if side != "rows" else ())
+    if side == "both":
+        return Blocks8(t[0], t[1], K), Blocks8(t[2], t[3], M)
+    return Blocks8(t[0], t[1], K if side == "rows" else M)
 
 
 def dequantize_blocks(b, dtype=torch.bfloat16):
@@ -103,6 +103,8 @@ def linear_blocks(x, layer_or_weight, bias=None):
     """y = Q(x) Q(W)^T + b: x [..., K] (bf16, fp16 or fp32) -> [..., N] in x's type. W: an ``nn.Linear``, a weight tensor
     [N, K] (packed in the call) or a Blocks8 (held in 8 bits; passes no gradient on). bias [N] fp32 or a 16-bit type. Rows of
     any stride are read in place, other layouts copied."""
+    if type(layer_or_weight) is Blocks8 and x.is_cuda and x.dim() == 2 and x.shape[1] == layer_or_weight[2]:
+        return ext().linear8_frozen(x, *layer_or_weight, bias, _err_word(x))  # a single token's cost is the host's
     w, own_bias = _weight_of(layer_or_weight, "linear_blocks")
     if own_bias is not None:
         if bias is not None:
