@@ -95,6 +95,8 @@ def test_trainer_step_and_optimizer_on_8_bit_products():
     device = torch.device("cuda", 0)
     tr = Trainer(den, te, TrainConfig(global_batch=4, micro_batch=2, steps=10, fp8=True), device)
     before = tr.den.blocks[0].mlp.in_proj.weight.detach().clone()
+    layers = [tr.den.blocks[1].attn.qkv, tr.den.blocks[0].mlp.out_proj, tr.te.blocks[0].mlp.in_proj]
+    held = [Fz.fp8_weight(m.weight) for m in layers]  # as an evaluation between steps leaves them
     batch = {"x0": torch.randn(4, 128, 16, 16, device=device),
              "lm_states": torch.randn(4, 32, 256, device=device, dtype=torch.bfloat16)}
     losses = [tr.step(batch) for _ in range(2)]
@@ -103,6 +105,9 @@ def test_trainer_step_and_optimizer_on_8_bit_products():
     assert all(torch.isfinite(v).item() for v in losses)
     assert tr.den.blocks[0].mlp.in_proj.weight.grad.dtype == torch.float32
     assert not torch.equal(before, tr.den.blocks[0].mlp.in_proj.weight)
+    for m, old in zip(layers, held):  # the optimizer's kernels write the weights past autograd's version counter
+        now = Fz.fp8_weight(m.weight)
+        assert now is not old and torch.equal(now.codes.view(torch.uint8), B8.quantize_blocks(m.weight).codes.view(torch.uint8))
 
 
 def test_operators_in_a_run():
@@ -159,3 +164,11 @@ def test_block_linear_and_marked_layers():
         marked = Fz.linear(x, lin)
     m = torch.nn.Sequential(lin)
     assert torch.equal(quantize(m, "fp8_block")(x), marked)
+
+
+@pytest.mark.parametrize("M", [3, 40])
+def test_far_scales(M):
+    """Large activations against small weights: the product is in range, and so is the result."""
+    x, w = torch.full((M, 128), 2.0 ** 118, device="cuda"), torch.full((16, 128), 2.0 ** -60, device="cuda")
+    got = B8.linear_blocks(x, B8.quantize_blocks(w))
+    assert torch.equal(got, torch.full((M, 16), 2.0 ** 65, device="cuda"))

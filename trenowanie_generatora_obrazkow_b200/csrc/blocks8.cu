@@ -979,10 +979,11 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_kernel(const FewRowsP
       const float s0 = __shfl_sync(0xffffffffu, s, 8 * t), s1 = __shfl_sync(0xffffffffu, s, 8 * t + 4);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        acc[r][i][0] += d[r][0] * s0 * ws[2 * r];
-        acc[r][i][1] += d[r][1] * s1 * ws[2 * r];
-        acc[r][i][2] += d[r][2] * s0 * ws[2 * r + 1];
-        acc[r][i][3] += d[r][3] * s1 * ws[2 * r + 1];
+        // powers of two: their product is exact, and out of range only where the result is
+        acc[r][i][0] += d[r][0] * (s0 * ws[2 * r]);
+        acc[r][i][1] += d[r][1] * (s1 * ws[2 * r]);
+        acc[r][i][2] += d[r][2] * (s0 * ws[2 * r + 1]);
+        acc[r][i][3] += d[r][3] * (s1 * ws[2 * r + 1]);
       }
     }
   }

@@ -39,10 +39,11 @@ def shadow_ptr(p):
 
 def after_raw_update(params):
     """Parameters were changed by raw-pointer kernels that also refreshed their bf16 shadows: drop the other
-    derived copies (the interleaved SwiGLU weight) so they are rebuilt from the new values."""
+    derived copies (the interleaved SwiGLU weight, the 8-bit weight) so they are rebuilt from the new values."""
     for p in params:
-        if getattr(p, "_tgo_swiglu", None) is not None:
-            p._tgo_swiglu = None
+        for copy in ("_tgo_swiglu", "_tgo_fp8"):
+            if getattr(p, copy, None) is not None:
+                setattr(p, copy, None)
 
 
 class GradNorm:
