@@ -205,7 +205,7 @@ def train_linear(x, w, b, dy, fn=B8.linear_blocks):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N,K,bias", [(1, 16, 128, True), (77, 96, 128, False), (130, 777, 100, True), (513, 128, 1000, True),
-                                        (5000, 64, 72, True)])
+                                        (5000, 64, 72, True), (4000, 2600, 1500, False), (12000, 700, 2048, True)])
 def test_linear_gradients(M, N, K, bias, dtype):
     x, w, dy = rnd(M, K, seed=1, dtype=dtype), rnd(N, K, seed=2, std=K ** -0.5, dtype=torch.float32), rnd(M, N, seed=3, std=0.1, dtype=dtype)
     b = rnd(N, seed=4, dtype=torch.float32) if bias else None
@@ -505,3 +505,34 @@ def test_every_tile(M, N, K, tile):
         assert_within(out, want + 1, product_tol(qa, qb, torch.float32, want) + (want + 1).abs() * 2.0 ** -23 + 2.0 ** -23)
     finally:
         ext().set_gemm8_tile(-1)
+
+
+@pytest.mark.parametrize("tile", [0, 1, 2])
+@pytest.mark.parametrize("M,N,K", [(700, 96, 300), (9000, 640, 520), (2300, 3000, 1800), (300, 4096, 8192)])
+def test_gradients_of_a_layer_in_one_launch(M, N, K, tile):
+    """The input's and the weight's gradient share a launch, whichever has the longer sums and however the tiles fill it."""
+    x, w, dy = rnd(M, K, seed=1), rnd(N, K, seed=2, std=K ** -0.5, dtype=torch.float32), rnd(M, N, seed=3, std=0.1)
+    ext().set_gemm8_tile(tile)
+    try:
+        got = train_linear(x, w, None, dy)
+        alone = B8.gemm_blocks(B8.quantize_blocks(dy), B8.quantize_blocks(w, "cols")), \
+            B8.gemm_blocks(B8.quantize_blocks(dy, "cols"), B8.quantize_blocks(x, "cols"), dtype=torch.float32)
+    finally:
+        ext().set_gemm8_tile(-1)
+    assert torch.equal(got[1], alone[0]) and torch.equal(got[2], alone[1])
+    dw = held_t(dy).t() @ held_t(x)
+    assert_within(got[2], dw, product_tol(held_t(dy).t(), held_t(x).t(), torch.float32, dw))
+
+
+def test_backward_called_from_another_stream():
+    x, lin, dy = rnd(4096, 512, seed=1), torch.nn.Linear(512, 2048, device=DEV), rnd(4096, 2048, seed=3)
+    want = train_linear(x, lin.weight, lin.bias, dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    leaf = x.clone().requires_grad_()
+    with torch.cuda.stream(side):
+        y = B8.linear_blocks(leaf, lin)
+    torch.cuda.current_stream().wait_stream(side)
+    y.backward(dy)  # runs where the forward ran; what it wrote is there for this stream
+    got = [leaf.grad.clone(), lin.weight.grad.clone(), lin.bias.grad.clone()]
+    assert all(torch.equal(a, b) for a, b in zip(got, want[1:]))

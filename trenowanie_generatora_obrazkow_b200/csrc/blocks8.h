@@ -37,27 +37,36 @@ cudaError_t colsum_launch(const float* sums, int T, int K, float* out, bool add,
 cudaError_t unpack8_launch(const uint8_t* codes, const uint8_t* scales, int R, int K, void* out, long long ldo, int elem,
                            cudaStream_t s);
 
-enum Gemm8Out : int { OUT_BF16 = 0, OUT_F16 = 1, OUT_F32 = 2 };  // as ElemType
-struct Gemm8Params {
+struct Gemm8Problem {
   int M, N, kb;             // kb: blocks of 128 along the contraction
   const uint8_t* sfa;       // scale bytes of A and B
   const uint8_t* sfb;
   void* C;                  // [M, N], rows ldc elements apart
   long long ldc;
   const float* bias;        // [N] or null
+  int elem;                 // of C
   int add;                  // C += (fp32 C only)
   int chunk_kb;             // contraction blocks per accumulator (a multiple of 4); further ones join in fp32 in order
   int c_tma;                // C goes through its tensor map
-  int* err;
+  int tiles;                // set by the launcher
 };
 enum Gemm8Tile : int { TILE_128x128 = 0, TILE_PAIR_192 = 1, TILE_PAIR_256 = 2 };  // pairs of CTAs: 256 x 192, 256 x 256
-// a, b: uint8 maps {Kp, rows, 1} with boxes {128, 128, 1} (b of TILE_PAIR_192: {128, 96, 1}), 128-byte swizzle; c: {N, M, 1},
-// box {32, 32, 1}; sa, sb (pairs alone): the scale atoms as 32-bit words {128, ceil(kb / 4), row tiles}, boxes {128, 1, 1}
-// and {128, 1, 2}
+// One or two independent products in a launch. a, b: uint8 maps {Kp, rows, 1} with boxes {128, 128, 1} (b of TILE_PAIR_192:
+// {128, 96, 1}), 128-byte swizzle; c: {N, M, 1}, box {32, 32, 1}; sa, sb (pairs alone): the scale atoms as 32-bit words
+// {128, ceil(kb / 4), row tiles}, boxes {128, 1, 1} and {128, 1, 2}
 struct Gemm8Maps {
-  CUtensorMap a, b, c, sa, sb;
+  CUtensorMap a[2], b[2], c[2], sa[2], sb[2];
 };
-cudaError_t gemm8_launch(const Gemm8Maps& t, const Gemm8Params& p, Gemm8Tile tile, int out, cudaStream_t s);
+struct Gemm8Params {
+  Gemm8Problem q[2];
+  int n;
+  int late;                 // set by the launcher, as `spare`: see gemm8.cu
+  int spare;
+  int* err;
+};
+// cycles of one output tile (its products, and its sums' beginnings and ends)
+long long gemm8_tile_cycles(const Gemm8Problem& q, Gemm8Tile tile, bool fills);
+cudaError_t gemm8_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8Tile tile, cudaStream_t s);
 
 // y [M, N] = Q(x) W^T + bias for few rows, x packed on the way (one launch)
 constexpr int kFewRows = 16;

@@ -5,6 +5,7 @@
 #include <cudaTypedefs.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "blocks8.h"
@@ -196,56 +197,86 @@ CUtensorMap scales_map(const Packed& a, uint32_t box_tiles) {
   return m;
 }
 
-// The tile whose waves over the GPU take the fewest cycles: a block of 128 costs 480 (128 x 128, bound by its loads; 380 where
-// they do not fill the GPU), 430 (256 x 192, loads) or 512 (256 x 256, the products), a sum's beginning and end 300, 800 or
-// 2600 (its accumulators share columns).
-// Measured at 32768 x 6144 x 2048: 436, 287 and 305 us; x 2048 x 6144: 418, 281 and 264 us; 2047 x 777 x 1000: 17, 21 and 26 us.
+// a product C [M, N] (+)= a b^T (+ bias)
+struct Product {
+  const Packed &a, &b;
+  const at::Tensor& C;
+  const float* bias;
+  bool add;
+};
 std::atomic<int> g_tile{-1};  // for comparisons of the variants: -1 chooses
+// The tile whose products end first on the whole GPU, by the cycles of a tile (gemm8.cu). Measured at 32768 x 6144 x 2048: 436
+// us for 128 x 128, 287 for 256 x 192, 305 for 256 x 256; x 2048 x 6144: 418, 281 and 264; 2047 x 777 x 1000: 17, 21 and 26.
 Gemm8Tile tile_of(const Gemm8Params& p) {
   if (g_tile >= 0) return (Gemm8Tile)g_tile.load();
-  const int64_t sms = num_sms(), sums = up(p.kb, p.chunk_kb);
-  const int64_t tiles = up(p.M, 128) * up(p.N, 128);
-  const int64_t one = up(tiles, sms) * (p.kb * (tiles > sms ? 480 : 380) + sums * 300);
-  const int64_t p192 = up(up(p.M, 256) * up(p.N, 192), sms / 2) * (p.kb * 430 + sums * 800);
-  const int64_t p256 = up(up(p.M, 256) * up(p.N, 256), sms / 2) * (p.kb * 512 + sums * 2600);
-  if (one <= p192 && one <= p256) return TILE_128x128;
-  return p192 <= p256 ? TILE_PAIR_192 : TILE_PAIR_256;
+  const int rows[3] = {128, 256, 256}, cols[3] = {128, 192, 256};
+  Gemm8Tile best = TILE_128x128;
+  int64_t least = 0;
+  for (int k = 0; k < 3; ++k) {
+    const int64_t units = k == 0 ? num_sms() : num_sms() / 2;
+    int64_t tiles[2] = {0, 0}, cost[2] = {0, 0}, all = 0, work = 0;
+    for (int i = 0; i < p.n; ++i) all += tiles[i] = up(p.q[i].M, rows[k]) * up(p.q[i].N, cols[k]);
+    for (int i = 0; i < p.n; ++i) work += tiles[i] * (cost[i] = gemm8_tile_cycles(p.q[i], (Gemm8Tile)k, all > units));
+    // one product: whole waves; two: the first one's waves, or all work and half of a second one's tile
+    const int64_t ends = std::max(up(tiles[0], units) * cost[0], p.n == 1 ? 0 : work / units + cost[1] / 2);
+    if (k == 0 || ends < least) {
+      least = ends;
+      best = (Gemm8Tile)k;
+    }
+  }
+  return best;
 }
 
-// C [M, N] (+)= a b^T (+ bias)
-void product(const Packed& a, const Packed& b, const at::Tensor& C, const float* bias, bool add, int* err) {
-  TORCH_CHECK(a.cols == b.cols, "gemm_blocks: sums over ", a.cols, " and ", b.cols);
-  if (a.rows == 0 || b.rows == 0) return;
-  if (a.cols == 0) {  // a sum of nothing
-    if (!add) C.zero_();
-    TORCH_CHECK(bias == nullptr, "gemm_blocks: a bias of a sum of nothing");
-    return;
-  }
+// One or two products in a launch
+void products(std::initializer_list<Product> list, int* err) {
   Gemm8Params p{};
-  p.M = (int)a.rows;
-  p.N = (int)b.rows;
-  p.kb = (int)a.blocks();
-  p.sfa = a.scales;
-  p.sfb = b.scales;
-  p.C = C.data_ptr();
-  p.ldc = row_stride(C);
-  p.bias = bias;
-  p.add = add;
-  p.err = err;
-  const int out = elem_of(C, "gemm_blocks");
-  // The tensor core's fp32 sums drop what does not fit their 24 bits instead of rounding: a sum of one sign over 32768
-  // lost 3.6e-5 of itself, 1.3e-6 over 4096. Sums that are returned in fp32 are joined from parts of 4096.
-  p.chunk_kb = out == OUT_F32 ? 32 : (int)up(p.kb, 4) * 4;
   Gemm8Maps t;
-  p.c_tma = out_map(&t.c, C, p.ldc);
-  const Gemm8Tile tile = tile_of(p);
-  t.a = codes_map(a, 128);
-  t.b = codes_map(b, tile == TILE_PAIR_192 ? 96 : 128);
-  if (tile != TILE_128x128) {
-    t.sa = scales_map(a, 1);
-    t.sb = scales_map(b, 2);
+  const Product* of[2] = {nullptr, nullptr};
+  for (const Product& w : list) {
+    TORCH_CHECK(w.a.cols == w.b.cols, "gemm_blocks: sums over ", w.a.cols, " and ", w.b.cols);
+    if (w.a.rows == 0 || w.b.rows == 0) continue;
+    if (w.a.cols == 0) {  // a sum of nothing
+      TORCH_CHECK(w.bias == nullptr, "gemm_blocks: a bias of a sum of nothing");
+      if (!w.add) w.C.zero_();
+      continue;
+    }
+    of[p.n++] = &w;
   }
-  BLOCK_LAUNCH(gemm8_launch(t, p, tile, out, at::cuda::getCurrentCUDAStream()), 1);
+  if (p.n == 2 && of[0]->a.cols < of[1]->a.cols) std::swap(of[0], of[1]);  // the longer sums first
+  for (int i = 0; i < p.n; ++i) {
+    const Product& w = *of[i];
+    Gemm8Problem& q = p.q[i];
+    q.M = (int)w.a.rows;
+    q.N = (int)w.b.rows;
+    q.kb = (int)w.a.blocks();
+    q.sfa = w.a.scales;
+    q.sfb = w.b.scales;
+    q.C = w.C.data_ptr();
+    q.ldc = row_stride(w.C);
+    q.bias = w.bias;
+    q.add = w.add;
+    q.elem = elem_of(w.C, "gemm_blocks");
+    // The tensor core's fp32 sums drop what does not fit their 24 bits instead of rounding: a sum of one sign over 32768
+    // lost 3.6e-5 of itself, 1.3e-6 over 4096. Sums that are returned in fp32 are joined from parts of 4096.
+    q.chunk_kb = q.elem == ELEM_F32 ? 32 : (int)up(q.kb, 4) * 4;
+    q.c_tma = out_map(&t.c[i], w.C, q.ldc);
+  }
+  if (p.n == 0) return;
+  p.err = err;
+  const Gemm8Tile tile = tile_of(p);
+  for (int i = 0; i < p.n; ++i) {
+    t.a[i] = codes_map(of[i]->a, 128);
+    t.b[i] = codes_map(of[i]->b, tile == TILE_PAIR_192 ? 96 : 128);
+    if (tile != TILE_128x128) {
+      t.sa[i] = scales_map(of[i]->a, 1);
+      t.sb[i] = scales_map(of[i]->b, 2);
+    }
+    if (!p.q[i].c_tma) t.c[i] = t.a[i];
+  }
+  BLOCK_LAUNCH(gemm8_launch(t, p, tile, at::cuda::getCurrentCUDAStream()), 1);
+}
+void product(const Packed& a, const Packed& b, const at::Tensor& C, const float* bias, bool add, int* err) {
+  products({{a, b, C, bias, add}}, err);
 }
 
 void small_vector(const OptT& bias, int64_t n, const at::Tensor& as, const char* what) {
@@ -354,17 +385,13 @@ at::Tensor linear8_frozen(at::Tensor x, at::Tensor codes, at::Tensor scales, int
 
 // The operands of a backward product are packed along the axis that it sums over: x^T and W^T are written while the
 // forward packs x and W. x itself is not kept: its checkpoint is the operand of the weight's gradient.
-// a product that sums over no rows at all
-bool zero_sum(const WeightGrad& g, int64_t rows) {
-  if (rows > 0) return false;
-  if (!g.add) g.g.zero_();
-  return true;
-}
-// the weight's gradient where autograd or the leaf wants it
-at::Tensor weight_grad(const WeightGrad& g, const Packed& dy, const Packed& x, int64_t rows, int* err) {
-  if (!g.g.defined()) return at::Tensor();
-  if (!zero_sum(g, rows)) product(dy, x, g.g, nullptr, g.add, err);
-  return g.put();
+// In one launch: a layer's input gradient dx = r wt^T (null: not wanted) and its weight's gradient dw = c xt^T where autograd
+// or the leaf wants it
+void gradients(const at::Tensor* dx, const Packed& r, const Packed& wt, const WeightGrad& dw, const Packed& c, const Packed& xt,
+               int* err) {
+  if (dx != nullptr && dw.g.defined()) products({{r, wt, *dx, nullptr, false}, {c, xt, dw.g, nullptr, dw.add}}, err);
+  else if (dx != nullptr) product(r, wt, *dx, nullptr, false, err);
+  else if (dw.g.defined()) product(c, xt, dw.g, nullptr, dw.add, err);
 }
 void notify(std::initializer_list<const WeightGrad*> gs) {
   if (!grad_ready().on) return;
@@ -420,11 +447,9 @@ struct Linear8Fn : public torch::autograd::Function<Linear8Fn> {
     const at::Tensor mem = now.on(dy);
     if (dx || cols) pack({dy, dx ? &r : nullptr, cols ? &c : nullptr}, sums.defined() ? sums.data_ptr<float>() : nullptr, gb.add);
     variable_list out(4);
-    if (dx) {
-      out[0] = fresh({M, K}, dy.scalar_type(), dy);
-      product(r, wt, out[0], nullptr, false, e);
-    }
-    out[1] = weight_grad(gw, c, xt, M, e);
+    if (dx) out[0] = fresh({M, K}, dy.scalar_type(), dy);
+    gradients(dx ? &out[0] : nullptr, r, wt, gw, c, xt, e);
+    out[1] = gw.put();
     if (sums.defined()) {
       if (gb.g.scalar_type() != at::kFloat) gb.g.copy_(sums);
       out[2] = gb.put();
@@ -633,18 +658,16 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
     const at::Tensor mem = now.on(dy);
     if (up_too || dw2) pack({dy, up_too ? &dyr : nullptr, dw2 ? &dyt : nullptr});
     variable_list out(4);
-    out[2] = weight_grad(g2, dyt, c.gt, M, e);
+    at::Tensor dg;
+    if (up_too) dg = fresh({M, H}, dy.scalar_type(), dy);
+    gradients(up_too ? &dg : nullptr, dyr, c.w2t, g2, dyt, c.gt, e);
+    out[2] = g2.put();
     if (up_too) {
-      {
-        at::Tensor dg = fresh({M, H}, dy.scalar_type(), dy);
-        product(dyr, c.w2t, dg, nullptr, false, e);
-        swiglu_backward(dg, c.ck, H, nullptr, &d8, &d8t, e);
-      }
-      if (dx) {
-        out[0] = fresh({M, K}, dy.scalar_type(), dy);
-        product(d8, c.w1t, out[0], nullptr, false, e);
-      }
-      out[1] = weight_grad(g1, d8t, c.xt, M, e);
+      swiglu_backward(dg, c.ck, H, nullptr, &d8, &d8t, e);
+      dg = at::Tensor();
+      if (dx) out[0] = fresh({M, K}, dy.scalar_type(), dy);
+      gradients(dx ? &out[0] : nullptr, d8, c.w1t, g1, d8t, c.xt, e);
+      out[1] = g1.put();
     }
     notify({&g2, &g1});
     return out;

@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "block_ops.h"
 #include "blocks8.h"
 #include "common.cuh"
 
@@ -79,7 +80,7 @@ __device__ __forceinline__ uint64_t sdesc_plain(uint32_t saddr) {
 
 template <int OUT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (OUT == OUT_BF16) return pack_bf16x2(a, b);
+  if constexpr (OUT == ELEM_BF16) return pack_bf16x2(a, b);
   __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
 }
@@ -87,7 +88,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // 32 values of a row to the staging tile, in the swizzled order of C's map (16-bit: rows of 64 bytes; fp32: of 128)
 template <int OUT>
 __device__ __forceinline__ void stage_row(uint8_t* buf, int lane, const float (&v)[32]) {
-  if constexpr (OUT == OUT_F32) {
+  if constexpr (OUT == ELEM_F32) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
@@ -100,23 +101,42 @@ __device__ __forceinline__ void stage_row(uint8_t* buf, int lane, const float (&
                      pack2<OUT>(v[8 * j + 4], v[8 * j + 5]), pack2<OUT>(v[8 * j + 6], v[8 * j + 7]));
   }
 }
-template <int OUT>
-__device__ __forceinline__ void store_one(void* C, long long at, float v, bool add) {
-  if constexpr (OUT == OUT_F32) {
+__device__ __forceinline__ void store_one(int elem, void* C, long long at, float v, bool add) {
+  if (elem == ELEM_F32) {
     float* c = reinterpret_cast<float*>(C) + at;
     *c = add ? *c + v : v;
-  } else if constexpr (OUT == OUT_BF16) {
+  } else if (elem == ELEM_BF16) {
     reinterpret_cast<__nv_bfloat16*>(C)[at] = __float2bfloat16_rn(v);
   } else {
     reinterpret_cast<__half*>(C)[at] = __float2half_rn(v);
   }
 }
 
-template <int BN, int OUT, bool PAIR>
+// The tiles of a unit (a CTA, a pair), one after another. The tiles of the first product (the longer ones) are dealt out in
+// turn; where that leaves `late` units with one more than the others, these others take `spare` rounds of the second product's
+// tiles before all take part: two products end together that apart would each leave units idle in their last wave.
+struct Schedule {
+  int unit, units, mine, late, spare;
+  __device__ Schedule(const Gemm8Params& p, int unit_, int units_)
+      : unit(unit_), units(units_), late(p.late), spare(p.spare) {
+    mine = p.q[0].tiles > unit ? (p.q[0].tiles - unit + units - 1) / units : 0;
+  }
+  __device__ __forceinline__ bool at(const Gemm8Params& p, int step, int& product, int& tile) const {
+    product = 0;
+    tile = step * units + unit;
+    if (step < mine) return true;
+    if (p.n < 2) return false;
+    const int t = step - mine, early = units - late;
+    product = 1;
+    if (unit >= late && t < spare) tile = t * early + unit - late;
+    else tile = spare * early + (unit >= late ? t - spare : t) * units + unit;
+    return tile < p.q[1].tiles;
+  }
+};
+
+template <int BN, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
-    gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmSA,
-                 const __grid_constant__ CUtensorMap tmSB, const Gemm8Params p) {
+    gemm8_kernel(const __grid_constant__ Gemm8Maps maps, const __grid_constant__ Gemm8Params p) {
   using F = Cfg<BN, PAIR>;
   constexpr int STAGES = F::STAGES, TM = PAIR ? 2 * BM : BM, EPI_WARPS = PAIR ? 8 : 4;
   extern __shared__ uint8_t smem_raw[];
@@ -130,10 +150,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = warp_id(), lane = lane_id();
   const int rank = PAIR ? (int)cluster_ctarank() : 0;
   const bool leader = rank == 0;  // issues the pair's products; its barriers count both CTAs' loads and epilogues
-  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
-  const int num_m = (p.M + TM - 1) / TM, num_n = (p.N + BN - 1) / BN;
-  const int num_tiles = num_m * num_n;
-  const int chunks = (p.kb + p.chunk_kb - 1) / p.chunk_kb;
+  const Schedule sched(p, PAIR ? blockIdx.x >> 1 : blockIdx.x, PAIR ? gridDim.x >> 1 : gridDim.x);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -148,10 +165,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     abort_sh = 0;
     fence_barrier_init();
   }
-  if (warp == 0 && lane == 0) {
-    prefetch_tmap(&tmA);
-    prefetch_tmap(&tmB);
-    if constexpr (PAIR) prefetch_tmap(&tmSA), prefetch_tmap(&tmSB);
+  if (warp == 0 && lane < p.n) {
+    prefetch_tmap(&maps.a[lane]);
+    prefetch_tmap(&maps.b[lane]);
+    if constexpr (PAIR) prefetch_tmap(&maps.sa[lane]), prefetch_tmap(&maps.sb[lane]);
   }
   if (warp == 1) {
     if constexpr (PAIR) {
@@ -173,15 +190,19 @@ __global__ void __launch_bounds__(THREADS, 1)
   // operands, and the thread, not the tensor core, was the bound (690 cycles for a block of 4 x 128).
   if (warp == 0) {
     // ---------------- loads ----------------
-    const int kq = (p.kb + 3) / 4;      // scale atoms of a row tile
-    const int nbt = (p.N + 127) / 128;  // row tiles of B's scales
     int stage = 0, filled = 0;
     uint32_t phase = 0;
     bool free = true, ok = true;  // free: the stage is known to be free
-    for (int tile = first; tile < num_tiles && ok; tile += step) {
+    int which, tile;
+    for (int step = 0; ok && sched.at(p, step, which, tile); ++step) {
+      const Gemm8Problem& q = p.q[which];
+      const CUtensorMap *tmA = &maps.a[which], *tmB = &maps.b[which], *tmSA = &maps.sa[which], *tmSB = &maps.sb[which];
+      const int num_n = (q.N + BN - 1) / BN;
+      const int kq = (q.kb + 3) / 4;      // scale atoms of a row tile
+      const int nbt = (q.N + 127) / 128;  // row tiles of B's scales
       const int mt = tile / num_n, nt = tile % num_n;
       const int m0 = mt * TM + rank * BM, n0 = nt * BN + rank * F::B_ROWS;
-      for (int kb = 0; kb < p.kb; ++kb) {
+      for (int kb = 0; kb < q.kb; ++kb) {
         if (!free) {
           ok = __all_sync(0xffffffffu, mbar_wait_poll(&empty_bar[stage], phase ^ 1, p.err, ERR_MBAR_TIMEOUT_PRODUCER) &&
                                            !abort_sh);
@@ -197,21 +218,21 @@ __global__ void __launch_bounds__(THREADS, 1)
           if constexpr (PAIR) {
             if (leader) mbar_expect_tx(&full_bar[stage], 2 * (F::STAGE_BYTES + (scales ? F::SF_BYTES : 0)));
             const uint32_t bar = mapa_shared(smem_u32(&full_bar[stage]), 0);
-            tma_load_3d_pair(sa, &tmA, bar, kb * BK, m0, 0);
-            tma_load_3d_pair(sa + F::A_BYTES, &tmB, bar, kb * BK, n0, 0);
+            tma_load_3d_pair(sa, tmA, bar, kb * BK, m0, 0);
+            tma_load_3d_pair(sa + F::A_BYTES, tmB, bar, kb * BK, n0, 0);
             if (scales) {
-              tma_load_3d_pair(sf, &tmSA, bar, 0, kb >> 2, mt * 2 + rank);
-              tma_load_3d_pair(sf + ATOM, &tmSB, bar, 0, kb >> 2, nt * BN / 128);
+              tma_load_3d_pair(sf, tmSA, bar, 0, kb >> 2, mt * 2 + rank);
+              tma_load_3d_pair(sf + ATOM, tmSB, bar, 0, kb >> 2, nt * BN / 128);
             }
           } else {
             const int nb = min(F::B_ATOMS, nbt - nt * (BN / 128));
             mbar_expect_tx(&full_bar[stage], F::STAGE_BYTES + (scales ? (1 + nb) * ATOM : 0));
-            tma_load_3d(sa, &tmA, &full_bar[stage], kb * BK, m0, 0);
-            tma_load_3d(sa + F::A_BYTES, &tmB, &full_bar[stage], kb * BK, n0, 0);
+            tma_load_3d(sa, tmA, &full_bar[stage], kb * BK, m0, 0);
+            tma_load_3d(sa + F::A_BYTES, tmB, &full_bar[stage], kb * BK, n0, 0);
             if (scales) {
-              bulk_load(sf, p.sfa + ((long long)mt * kq + (kb >> 2)) * ATOM, ATOM, &full_bar[stage]);
+              bulk_load(sf, q.sfa + ((long long)mt * kq + (kb >> 2)) * ATOM, ATOM, &full_bar[stage]);
               for (int i = 0; i < nb; ++i)
-                bulk_load(sf + (1 + i) * ATOM, p.sfb + ((long long)(nt * (BN / 128) + i) * kq + (kb >> 2)) * ATOM, ATOM,
+                bulk_load(sf + (1 + i) * ATOM, q.sfb + ((long long)(nt * (BN / 128) + i) * kq + (kb >> 2)) * ATOM, ATOM,
                           &full_bar[stage]);
             }
           }
@@ -239,8 +260,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       int stage = 0, unit = 0;
       uint32_t phase = 0;
       bool ok = true, ready = false;
-      for (int tile = first; tile < num_tiles && ok; tile += step) {
-        for (int c = 0; c < chunks && ok; ++c, ++unit) {
+      int which, tile;
+      for (int step = 0; ok && sched.at(p, step, which, tile); ++step) {
+        const int kbs = p.q[which].kb, chunk_kb = p.q[which].chunk_kb;
+        const uint32_t sfb_n = sfb + (BN % 128 != 0 && (tile % ((p.q[which].N + BN - 1) / BN) & 1) ? 2 : 0);  // 64 columns in
+        for (int c = 0; c * chunk_kb < kbs && ok; ++c, ++unit) {
           // accumulators that share columns: the unit before has given up its shared ones; else: the one before that
           // has been read
           constexpr int back = BN == 256 ? 1 : 2;
@@ -252,8 +276,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           tc_fence_after();
           const uint32_t d = tmem_base + ((unit & 1) ? F::ACC1 : 0);
-          const uint32_t sfb_n = sfb + (BN % 128 != 0 && (tile % num_n & 1) ? 2 : 0);  // 64 columns into the first atom
-          const int k0 = c * p.chunk_kb, k1 = min(p.kb, k0 + p.chunk_kb);
+          const int k0 = c * chunk_kb, k1 = min(kbs, k0 + chunk_kb);
           for (int kb = k0; kb < k1; ++kb) {
             if (!ready) {
               ok = __all_sync(0xffffffffu, mbar_wait_poll(&full_bar[stage], phase, p.err, ERR_MBAR_TIMEOUT_MMA) && !abort_sh);
@@ -295,14 +318,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // ---------------- epilogue: warp q owns rows 32 q .. 32 q + 31 of the tile ----------------
-    const int q = warp & 3;
-    uint8_t* const cbuf = smem_c + q * F::C_STAGE;
-    constexpr int BUFS = OUT == OUT_F32 ? 1 : 2;
-    int turn = 0, unit = 0;
-    bool ok = true;
-    for (int tile = first; tile < num_tiles && ok; tile += step) {
-      const int m0 = (tile / num_n) * TM + rank * BM + q * 32, n0 = (tile % num_n) * BN;
-      for (int c = 0; c < chunks; ++c, ++unit) {
+    const int quarter = warp & 3;
+    uint8_t* const cbuf = smem_c + quarter * F::C_STAGE;
+    int turn = 0, unit = 0, which, tile;
+    bool ok = true, any_tma = false;
+    for (int step = 0; ok && sched.at(p, step, which, tile); ++step) {
+      const Gemm8Problem& q = p.q[which];
+      const CUtensorMap* tmC = &maps.c[which];
+      const int num_n = (q.N + BN - 1) / BN;
+      const int m0 = (tile / num_n) * TM + rank * BM + quarter * 32, n0 = (tile % num_n) * BN;
+      const bool f32 = q.elem == ELEM_F32;
+      for (int c = 0; c * q.chunk_kb < q.kb; ++c, ++unit) {
         int got = 0;
         if (lane == 0) got = mbar_wait_poll(&tfull_bar[unit & 1], (unit >> 1) & 1, p.err, ERR_MBAR_TIMEOUT_EPILOGUE) ? 1 : 0;
         ok = __shfl_sync(0xffffffffu, got, 0) != 0;
@@ -311,10 +337,14 @@ __global__ void __launch_bounds__(THREADS, 1)
           break;
         }
         tc_fence_after();
-        const bool add = OUT == OUT_F32 && (c > 0 || p.add);
-        // chunks of one sum join in order: what the lane has sent has been written
-        if (c > 0 && p.c_tma && lane == 0) bulk_wait_group_all();
-        const uint32_t t = tmem_base + ((unit & 1) ? F::ACC1 : 0) + ((uint32_t)(q * 32) << 16);
+        const bool add = f32 && (c > 0 || q.add);
+        if (lane == 0) {
+          // chunks of one sum join in order: what the lane has sent has been written; else: the staging tile is free, whatever
+          // the last product's type was
+          if (c > 0 && q.c_tma) bulk_wait_group_all();
+          else if (any_tma) bulk_wait_group_read<0>();
+        }
+        const uint32_t t = tmem_base + ((unit & 1) ? F::ACC1 : 0) + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
         for (int i = 0; i < BN / 32; ++i) {
           // the columns that the accumulators share come first: the last of the even one, the first of the odd one
@@ -330,25 +360,33 @@ __global__ void __launch_bounds__(THREADS, 1)
               else mbar_arrive(&tempty_bar[unit & 1]);
             }
           }
-          if (m0 >= p.M || n0 + col >= p.N) continue;
+          if (m0 >= q.M || n0 + col >= q.N) continue;
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-          if (p.bias != nullptr && c == 0) {
+          if (q.bias != nullptr && c == 0) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += n0 + col + j < p.N ? __ldg(p.bias + n0 + col + j) : 0.f;
+            for (int j = 0; j < 32; ++j) v[j] += n0 + col + j < q.N ? __ldg(q.bias + n0 + col + j) : 0.f;
           }
-          if (p.c_tma) {
-            uint8_t* buf = cbuf + (turn % BUFS) * (F::C_STAGE / BUFS);
-            ++turn;
-            if (lane == 0) bulk_wait_group_read<BUFS - 1>();
-            __syncwarp();
-            stage_row<OUT>(buf, lane, v);
+          if (q.c_tma) {
+            any_tma = true;
+            uint8_t* buf = cbuf;
+            if (f32) {
+              if (lane == 0) bulk_wait_group_read<0>();
+              __syncwarp();
+              stage_row<ELEM_F32>(buf, lane, v);
+            } else {  // two tiles in turn
+              buf += (turn++ & 1) * (F::C_STAGE / 2);
+              if (lane == 0) bulk_wait_group_read<1>();
+              __syncwarp();
+              if (q.elem == ELEM_BF16) stage_row<ELEM_BF16>(buf, lane, v);
+              else stage_row<ELEM_F16>(buf, lane, v);
+            }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (add) tma_reduce_add_3d(&tmC, buf, n0 + col, m0, 0);
-              else tma_store_3d(&tmC, buf, n0 + col, m0, 0);
+              if (add) tma_reduce_add_3d(tmC, buf, n0 + col, m0, 0);
+              else tma_store_3d(tmC, buf, n0 + col, m0, 0);
               bulk_commit_group();
             }
           } else {  // rows that a tensor map cannot address: through the staging tile, a row of 32 values at a time
@@ -357,17 +395,17 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) s[lane * 32 + (j ^ lane)] = v[j];
             __syncwarp();
-            if (n0 + col + lane < p.N) {
-              const int rows = min(32, p.M - m0);
+            if (n0 + col + lane < q.N) {
+              const int rows = min(32, q.M - m0);
 #pragma unroll 4
               for (int j = 0; j < rows; ++j)
-                store_one<OUT>(p.C, (long long)(m0 + j) * p.ldc + n0 + col + lane, s[j * 32 + (lane ^ j)], add);
+                store_one(q.elem, q.C, (long long)(m0 + j) * q.ldc + n0 + col + lane, s[j * 32 + (lane ^ j)], add);
             }
           }
         }
       }
     }
-    if (p.c_tma && lane == 0) bulk_wait_group_all();
+    if (any_tma && lane == 0) bulk_wait_group_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -379,10 +417,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <int BN, int OUT, bool PAIR>
-cudaError_t launch(const Gemm8Maps& t, const Gemm8Params& p, cudaStream_t s) {
+template <int BN, bool PAIR>
+cudaError_t launch(const Gemm8Maps& t, Gemm8Params& p, Gemm8Tile tile, cudaStream_t s) {
   using F = Cfg<BN, PAIR>;
-  auto kern = gemm8_kernel<BN, OUT, PAIR>;
+  auto kern = gemm8_kernel<BN, PAIR>;
   static_assert(F::SMEM + 1024 <= 232448, "dynamic + static shared memory");
   static std::atomic<uint64_t> set{0};  // bit d: done on device d
   int dev = 0;
@@ -394,10 +432,22 @@ cudaError_t launch(const Gemm8Maps& t, const Gemm8Params& p, cudaStream_t s) {
     if (dev <= 63) set.fetch_or(1ull << dev);
   }
   constexpr int TM = PAIR ? 2 * BM : BM;
-  const long long tiles = (long long)((p.M + TM - 1) / TM) * ((p.N + BN - 1) / BN);
-  if (tiles >= (1ll << 30)) return cudaErrorInvalidValue;
+  long long all = 0;
+  for (int i = 0; i < p.n; ++i) {
+    const long long tiles = (long long)((p.q[i].M + TM - 1) / TM) * ((p.q[i].N + BN - 1) / BN);
+    if (tiles >= (1ll << 29)) return cudaErrorInvalidValue;
+    p.q[i].tiles = (int)tiles;
+    all += tiles;
+  }
+  const int units = (int)std::min<long long>(all, PAIR ? num_sms() / 2 : num_sms());
+  p.late = p.spare = 0;
+  if (p.n == 2 && p.q[0].tiles % units != 0) {
+    p.late = p.q[0].tiles % units;
+    const long long a = gemm8_tile_cycles(p.q[0], tile, true), b = gemm8_tile_cycles(p.q[1], tile, true);
+    p.spare = (int)std::min<long long>((a + b / 2) / b, 1 << 20);
+  }
   cudaLaunchConfig_t c{};
-  c.gridDim = dim3(PAIR ? 2 * (int)std::min<long long>(tiles, num_sms() / 2) : (int)std::min<long long>(tiles, num_sms()));
+  c.gridDim = dim3(PAIR ? 2 * units : units);
   c.blockDim = dim3(THREADS);
   c.dynamicSmemBytes = F::SMEM;
   c.stream = s;
@@ -407,26 +457,32 @@ cudaError_t launch(const Gemm8Maps& t, const Gemm8Params& p, cudaStream_t s) {
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   c.attrs = &cluster;
   c.numAttrs = PAIR ? 1 : 0;
-  e = cudaLaunchKernelEx(&c, kern, t.a, t.b, t.c, t.sa, t.sb, p);
+  e = cudaLaunchKernelEx(&c, kern, t, p);
   return e != cudaSuccess ? e : cudaGetLastError();
-}
-template <int BN, bool PAIR>
-cudaError_t launch_out(const Gemm8Maps& t, const Gemm8Params& p, int out, cudaStream_t s) {
-  if (out == OUT_BF16) return launch<BN, OUT_BF16, PAIR>(t, p, s);
-  if (out == OUT_F16) return launch<BN, OUT_F16, PAIR>(t, p, s);
-  return launch<BN, OUT_F32, PAIR>(t, p, s);
 }
 
 }  // namespace
 
-cudaError_t gemm8_launch(const Gemm8Maps& t, const Gemm8Params& p, Gemm8Tile tile, int out, cudaStream_t s) {
-  if (p.M <= 0 || p.N <= 0 || p.kb <= 0 || p.chunk_kb <= 0 || p.chunk_kb % 4 != 0) return cudaErrorInvalidValue;
-  if (out != OUT_F32 && (p.add || p.chunk_kb < p.kb)) return cudaErrorInvalidValue;
-  if (p.add && p.bias != nullptr) return cudaErrorInvalidValue;
+// A block of 128 costs 480 (128 x 128, bound by its loads; 380 where they do not fill the GPU), 430 (256 x 192, loads) or 512
+// (256 x 256, the products), a sum's beginning and end 300, 800 or 2600 (its accumulators share columns).
+long long gemm8_tile_cycles(const Gemm8Problem& q, Gemm8Tile tile, bool fills) {
+  const long long sums = (q.kb + q.chunk_kb - 1) / q.chunk_kb;
+  if (tile == TILE_128x128) return (long long)q.kb * (fills ? 480 : 380) + sums * 300;
+  return tile == TILE_PAIR_192 ? (long long)q.kb * 430 + sums * 800 : (long long)q.kb * 512 + sums * 2600;
+}
+
+cudaError_t gemm8_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8Tile tile, cudaStream_t s) {
+  if (p.n < 1 || p.n > 2) return cudaErrorInvalidValue;
+  for (int i = 0; i < p.n; ++i) {
+    const Gemm8Problem& q = p.q[i];
+    if (q.M <= 0 || q.N <= 0 || q.kb <= 0 || q.chunk_kb <= 0 || q.chunk_kb % 4 != 0) return cudaErrorInvalidValue;
+    if (q.elem != ELEM_F32 && (q.add || q.chunk_kb < q.kb)) return cudaErrorInvalidValue;
+    if (q.elem < ELEM_BF16 || q.elem > ELEM_F32 || (q.add && q.bias != nullptr)) return cudaErrorInvalidValue;
+  }
   switch (tile) {
-    case TILE_PAIR_256: return launch_out<256, true>(t, p, out, s);
-    case TILE_PAIR_192: return launch_out<192, true>(t, p, out, s);
-    case TILE_128x128: return launch_out<128, false>(t, p, out, s);
+    case TILE_PAIR_256: return launch<256, true>(t, p, tile, s);
+    case TILE_PAIR_192: return launch<192, true>(t, p, tile, s);
+    case TILE_128x128: return launch<128, false>(t, p, tile, s);
   }
   return cudaErrorInvalidValue;
 }
