@@ -15,6 +15,7 @@
 #include "block_ops.h"
 #include "blocks8.h"
 #include "common.cuh"
+#include "vec.cuh"
 
 namespace tgo {
 
@@ -101,14 +102,25 @@ __device__ __forceinline__ void stage_row(uint8_t* buf, int lane, const float (&
                      pack2<OUT>(v[8 * j + 4], v[8 * j + 5]), pack2<OUT>(v[8 * j + 6], v[8 * j + 7]));
   }
 }
-__device__ __forceinline__ void store_one(int elem, void* C, long long at, float v, bool add) {
-  if (elem == ELEM_F32) {
-    float* c = reinterpret_cast<float*>(C) + at;
-    *c = add ? *c + v : v;
-  } else if (elem == ELEM_BF16) {
-    reinterpret_cast<__nv_bfloat16*>(C)[at] = __float2bfloat16_rn(v);
-  } else {
-    reinterpret_cast<__half*>(C)[at] = __float2half_rn(v);
+// a lane's column of a staged 32 x 32 tile to C; eight rows at a time, so that the reads do not wait for the stores
+template <typename T>
+__device__ __forceinline__ void store_rows(const Gemm8Problem& q, long long at, const float* s, int rows, bool add, int lane) {
+  T* c = reinterpret_cast<T*>(q.C) + at;
+#pragma unroll
+  for (int j = 0; j < 32; j += 8) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = s[(j + k) * 32 + (lane ^ (j + k))];
+    if constexpr (sizeof(T) == 4) {
+      if (add) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (j + k < rows) v[k] += c[(j + k) * q.ldc];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (j + k < rows) c[(j + k) * q.ldc] = from_f<T>(v[k]);
   }
 }
 
@@ -397,9 +409,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             __syncwarp();
             if (n0 + col + lane < q.N) {
               const int rows = min(32, q.M - m0);
-#pragma unroll 4
-              for (int j = 0; j < rows; ++j)
-                store_one(q.elem, q.C, (long long)(m0 + j) * q.ldc + n0 + col + lane, s[j * 32 + (lane ^ j)], add);
+              const long long at = (long long)m0 * q.ldc + n0 + col + lane;
+              if (f32) store_rows<float>(q, at, s, rows, add, lane);
+              else if (q.elem == ELEM_BF16) store_rows<__nv_bfloat16>(q, at, s, rows, add, lane);
+              else store_rows<__half>(q, at, s, rows, add, lane);
             }
           }
         }
