@@ -90,6 +90,41 @@ def gemm_case(M, N, K, a_mn=False, b_mn=False, accumulate=False):
     return ours, lib, 2.0 * M * N * K, 2 * (M * K + N * K) + out.element_size() * M * N * (2 if accumulate else 1)
 
 
+def gemm8_case(M, N, K, out=torch.bfloat16):
+    """8-bit product of packed operands against cuBLAS in bf16."""
+    from . import blocks8 as B8
+    a, b = _bf16(M, K), _bf16(N, K, scale=K ** -0.5)
+    a8, b8 = B8.quantize_blocks(a), B8.quantize_blocks(b)
+    c, bt = torch.empty(M, N, device="cuda", dtype=out), b.t()
+    return lambda: B8.gemm_blocks(a8, b8, out=c), lambda: torch.matmul(a, bt), 2 * M * N * K, 0
+
+
+def linear8_case(M, N, K):
+    """Forward and both gradients of a layer on 8-bit products (packing included) against bf16 through cuBLAS."""
+    from . import blocks8 as B8
+    x, dy = _bf16(M, K).requires_grad_(), _bf16(M, N)
+    w = torch.randn(N, K, device="cuda").mul_(K ** -0.5).requires_grad_()
+    w16 = w.detach().bfloat16().requires_grad_()
+
+    def ours():
+        x.grad = w.grad = None
+        B8.linear_blocks(x, w).backward(dy)
+
+    def lib():
+        x.grad = w16.grad = None
+        F.linear(x, w16).backward(dy)
+
+    return ours, lib, 6 * M * N * K, 0
+
+
+def pack8_case(M, K):
+    """Packing along rows and columns in one pass against a copy of the same bytes (2 B read, 2 B written)."""
+    from . import blocks8 as B8
+    x = _bf16(M, K)
+    out = torch.empty_like(x)
+    return lambda: B8.quantize_blocks(x, "both"), lambda: out.copy_(x), 0, 4 * M * K
+
+
 def gemm_i8_case(M, N, K):
     """W8A8: our kind::i8 GEMM with the scales in its epilogue vs torch._int_mm + the scaling (the reference's
     teacher path); counted as 2 M N K integer operations."""
@@ -314,6 +349,12 @@ def cases(small):
         "euler_cfg": lambda: euler_case(8, 64, 128),
         "gemm_swiglu": lambda: swiglu_gemm_case(M, D, MLP),
         "gemm_grouped": lambda: grouped_gemm_case(M, 8192, D, 8),  # MoE experts: up projection of hidden 4096
+        # 8-bit blocks: products, a training layer, packing
+        "gemm8_qkv": lambda: gemm8_case(M, 3 * D, D),
+        "gemm8_mlp_down": lambda: gemm8_case(M, D, MLP),
+        "gemm8_wgrad_qkv": lambda: gemm8_case(3 * D, D, M, out=torch.float32),
+        "linear8_qkv": lambda: linear8_case(M, 3 * D, D),
+        "pack8": lambda: pack8_case(M, D),
         # Newton-Schulz buckets of the 1.24B model on one GPU: 2048 x 2048 (q, k, v, out, cross q / out of 24
         # blocks) and 2048 x 5504 (SwiGLU gate / up / down)
         "ns_2048": lambda: ns_case(24 if small else 144, D, D),
