@@ -383,6 +383,39 @@ def test_mlp_of_other_widths_and_no_rows():
     assert y.shape == (0, 64) and all((t.grad == 0).all() for t in leaves[1:]) and leaves[0].grad.shape == (0, 64)
 
 
+@pytest.mark.parametrize("wants", [(1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 0, 0)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,K,H", [(1, 64, 128), (17, 0, 128), (129, 100, 384), (384, 1540, 256), (2500, 512, 1408)])
+def test_mlp_in_fewer_launches(M, K, H, dtype, wants):
+    """The first product and the activation give the same bits in one launch as in two, also of infinities, NaN and overflow."""
+    x, w1, w2 = rnd(M, K, seed=1, dtype=dtype), rnd(2 * H, K, seed=2, std=max(K, 1) ** -0.5, dtype=torch.float32), \
+        rnd(96, H, seed=3, std=H ** -0.5, dtype=torch.float32)
+    dy = rnd(M, 96, seed=4, std=0.1, dtype=dtype)
+    if K and M > 16:
+        x[3] *= 2000.0  # g overflows fp16, not the products' sums
+        x[7, 5] = float("inf")
+        w1[H + 9, 11] = float("nan")
+    if K == 0:
+        with pytest.raises(RuntimeError, match="at least one column"):
+            B8.mlp_blocks(x, w1, w2)
+        return
+    held_w = B8.quantize_blocks(w1), B8.quantize_blocks(w2)
+    results = []
+    for fused in (True, False):
+        ext().set_mlp8_fused(fused)
+        try:
+            leaves = [t.clone().requires_grad_(bool(w)) for t, w in zip((x, w1, w2), wants)]
+            y = B8.mlp_blocks(*leaves)
+            if any(wants):
+                y.backward(dy)
+            results.append([y.detach(), B8.mlp_blocks(x, *held_w)] + [t.grad for t in leaves if t.grad is not None])
+        finally:
+            ext().set_mlp8_fused(True)
+    assert len(results[0]) == 2 + sum(wants)
+    for a, b in zip(*results):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
 # ----------------------------------------------------------------------------------------------------- streams, graphs
 def test_captured_and_replayed():
     lin = torch.nn.Linear(256, 384, device=DEV)

@@ -9,13 +9,12 @@
 // 128 in registers, a thread 8 rows x 8 columns: the row maxima need 16 lanes of a warp, the column maxima the tile's 8
 // warps (through shared memory), and eight codes of a column are eight bytes, so the transposed tile is staged in 16 KB
 // of shared memory without bank conflicts and leaves as whole lines.
-#include <cuda_fp8.h>
-
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
 
 #include "block_ops.h"
+#include "blocks8.cuh"
 #include "blocks8.h"
 #include "common.cuh"
 #include "vec.cuh"
@@ -26,45 +25,7 @@ int num_sms();  // gemm.cu
 
 namespace {
 
-constexpr int TILE = 128, PACK_THREADS = 256;
-constexpr int ATOM = 512;
-
-// ---------------------------------------------------------------------------------------------------------- scales
-// With u the bits of A: the carry out of the mantissa's top bits is the step from m <= 1.75 to m > 1.75.
-__device__ __forceinline__ int scale_byte(float amax) { return max(0, (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8); }
-__device__ __forceinline__ float scale_inv(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }  // 2^-e
-__device__ __forceinline__ float scale_of(int byte) {                                                          // 2^e
-  return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u);
-}
-// offset of the scale byte of row r and block b; quads: atoms of a row tile, ceil(blocks / 4)
-__device__ __forceinline__ long long scale_at(int r, int b, int quads) {
-  return ((long long)(r >> 7) * quads + (b >> 2)) * ATOM + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\t"
-      "mov.b64 {%0, %1}, x;\n}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ uint32_t codes2(float a, float b) {  // a in the low byte
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t codes4(float2 a, float2 b) { return codes2(a.x, a.y) | (codes2(b.x, b.y) << 16); }
-__device__ __forceinline__ float2 values2(uint32_t codes) {  // low two bytes
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-__device__ __forceinline__ void values8(uint2 c, float k, float2 (&f)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = mul2(values2((i < 2 ? c.x : c.y) >> ((i & 1) * 16)), make_float2(k, k));
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {  // passes over NaN
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
+constexpr int PACK_THREADS = 256;
 
 // ------------------------------------------------------------------------------------------------------------ loads
 // Eight values of a row: fp32 as four pairs; 16-bit types as they are stored, unpacked where they are used (half the
@@ -179,12 +140,6 @@ __device__ __forceinline__ void finite_tops(Eight<T> (&v)[R], float (&m)[R]) {
 }
 
 // ------------------------------------------------------------------------------------------------------- tile output
-struct Side {             // one 8-bit output
-  uint8_t* codes;
-  uint8_t* scales;
-  int rows, quads;        // of the codes; atoms of a row tile
-  long long width;        // bytes of a row: the blocked axis rounded up to 128
-};
 struct TileShared {
   float part[8][TILE];
   float inv[TILE];
@@ -381,11 +336,6 @@ __global__ void __launch_bounds__(PACK_THREADS, 2) pack8_jobs_kernel(const __gri
 bool aligned16(const void* p, long long stride_bytes) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride_bytes & 15) == 0;
 }
-Side side(uint8_t* codes, uint8_t* scales, int rows, int along) {
-  const int nb = (along + TILE - 1) / TILE;
-  return Side{codes, scales, rows, (nb + 3) / 4, (long long)nb * TILE};
-}
-
 template <typename T>
 cudaError_t pack_typed(const Pack8Params& p, cudaStream_t s) {
   const long long tiles = (long long)((p.K + TILE - 1) / TILE) * ((p.M + TILE - 1) / TILE);
@@ -463,20 +413,6 @@ cudaError_t unpack_typed(const uint8_t* codes, const uint8_t* scales, int R, int
 }
 
 // ----------------------------------------------------------------------------------------------------------- SwiGLU
-// s = 1 / (1 + exp(-a)). For 16-bit types exp2 and the reciprocal are the hardware's approximations (an argument rounded to
-// 2^-24 of itself and two units in the last place), which the result's rounding hides; fp32 results take the library's.
-template <bool FINE>
-__device__ __forceinline__ float sigmoid(float a) {
-  if constexpr (FINE) {
-    return 1.f / (1.f + expf(-a));
-  } else {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return r;
-  }
-}
-
 // g in ab's type, the checkpoint of ab in 8 bits. Rows alone: a thread holds 8 columns of ROW_R rows (two: enough warps to keep
 // the memory busy; at 32768 x 5504 the
 // backward took 265 us with four, 212 with two). The checkpoint's

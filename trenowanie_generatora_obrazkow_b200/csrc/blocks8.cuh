@@ -1,0 +1,75 @@
+// Device helpers of the 8-bit block kernels (blocks8.cu, gemm8.cu): scales, conversions, the sigmoid, an output's place.
+#pragma once
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+namespace tgo {
+namespace {
+
+constexpr int TILE = 128;
+constexpr int ATOM = 512;
+
+// ---------------------------------------------------------------------------------------------------------- scales
+// With u the bits of A: the carry out of the mantissa's top bits is the step from m <= 1.75 to m > 1.75.
+__device__ __forceinline__ int scale_byte(float amax) { return max(0, (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8); }
+__device__ __forceinline__ float scale_inv(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }  // 2^-e
+__device__ __forceinline__ float scale_of(int byte) {                                                          // 2^e
+  return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u);
+}
+// offset of the scale byte of row r and block b; quads: atoms of a row tile, ceil(blocks / 4)
+__device__ __forceinline__ long long scale_at(int r, int b, int quads) {
+  return ((long long)(r >> 7) * quads + (b >> 2)) * ATOM + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\t"
+      "mov.b64 {%0, %1}, x;\n}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ uint32_t codes2(float a, float b) {  // a in the low byte
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t codes4(float2 a, float2 b) { return codes2(a.x, a.y) | (codes2(b.x, b.y) << 16); }
+__device__ __forceinline__ float2 values2(uint32_t codes) {  // low two bytes
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ void values8(uint2 c, float k, float2 (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = mul2(values2((i < 2 ? c.x : c.y) >> ((i & 1) * 16)), make_float2(k, k));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {  // passes over NaN
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// s = 1 / (1 + exp(-a)). For 16-bit types exp2 and the reciprocal are the hardware's approximations (an argument rounded to
+// 2^-24 of itself and two units in the last place), which the result's rounding hides; fp32 results take the library's.
+template <bool FINE>
+__device__ __forceinline__ float sigmoid(float a) {
+  if constexpr (FINE) {
+    return 1.f / (1.f + expf(-a));
+  } else {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
+  }
+}
+
+struct Side {             // one 8-bit output
+  uint8_t* codes;
+  uint8_t* scales;
+  int rows, quads;        // of the codes; atoms of a row tile
+  long long width;        // bytes of a row: the blocked axis rounded up to 128
+};
+inline Side side(uint8_t* codes, uint8_t* scales, int rows, int along) {
+  const int nb = (along + TILE - 1) / TILE;
+  return Side{codes, scales, rows, (nb + 3) / 4, (long long)nb * TILE};
+}
+
+}  // namespace
+}  // namespace tgo

@@ -554,6 +554,65 @@ void swiglu_backward(const at::Tensor& dg, const Packed& ck, int64_t H, at::Tens
   BLOCK_LAUNCH(swiglu8_bwd_launch(p, elem_of(dg, "swiglu_blocks"), at::cuda::getCurrentCUDAStream()), 1);
 }
 
+// a map of 8-bit outputs {inner, rows, 1}
+CUtensorMap bytes_map(const uint8_t* base, uint64_t inner, uint64_t rows, uint32_t box_inner, uint32_t box_rows, bool swizzle) {
+  CUtensorMap m;
+  cuuint64_t dims[3] = {inner, rows, 1};
+  cuuint64_t strides[2] = {inner, inner * rows};
+  cuuint32_t box[3] = {box_inner, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = tmap_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(base), dims, strides, box, estr,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                    swizzle ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "tensor map of 8-bit outputs: code ", (int)r);
+  return m;
+}
+std::atomic<bool> g_fused{true};  // for comparisons: the MLP's first product and its activation in one launch
+// [a | b] = x w^T rounded to `like`'s type, g = silu(a) b: the checkpoint (ck, or null), g along its rows and (g8t, or null) its
+// columns. 16-bit types: one launch, the activations stay on the chip; fp32 (whose values do not fit the registers): two.
+void product_swiglu(const Packed& x, const Packed& w, const at::Tensor& like, const Packed* ck, const Packed& g8,
+                    const Packed* g8t, int* err) {
+  const int64_t M = x.rows, H = w.rows / 2;
+  if (M == 0) return;
+  const int elem = elem_of(like, kWhat);
+  if (elem == ELEM_F32 || !g_fused) {
+    at::Tensor ab = fresh({M, 2 * H}, like.scalar_type(), like);
+    product(x, w, ab, nullptr, false, err);
+    swiglu_forward(ab, nullptr, ck, &g8, g8t, err);
+    return;
+  }
+  Gemm8Params p{};
+  Gemm8Problem& q = p.q[0];
+  p.n = 1;
+  p.err = err;
+  q.M = (int)M;
+  q.N = (int)(2 * H);
+  q.kb = (int)x.blocks();
+  q.sfa = x.scales;
+  q.sfb = w.scales;
+  q.elem = elem;
+  q.chunk_kb = (int)up(q.kb, 4) * 4;
+  Gemm8Maps t;
+  t.a[0] = codes_map(x, 128);
+  t.b[0] = codes_map(w, 128);
+  t.sa[0] = scales_map(x, 1);
+  t.sb[0] = scales_map(w, 1);
+  t.c[0] = t.a[0];
+  const CUtensorMap g8_map = bytes_map(g8.codes, H, M, 32, 32, true);
+  const CUtensorMap ck_map = ck != nullptr ? bytes_map(ck->codes, 2 * H, M, 32, 32, true) : g8_map;
+  const CUtensorMap g8t_map = g8t != nullptr ? bytes_map(g8t->codes, g8t->blocks() * 128, H, 32, 32, false) : g8_map;
+  Gemm8SwigluOut o{};
+  if (ck != nullptr) o.ck = ck->codes, o.ck_scales = ck->scales;
+  o.g8 = g8.codes;
+  o.g8_scales = g8.scales;
+  if (g8t != nullptr) o.g8t = g8t->codes, o.g8t_scales = g8t->scales;
+  o.ck_map = &ck_map;
+  o.g8_map = &g8_map;
+  o.g8t_map = &g8t_map;
+  BLOCK_LAUNCH(gemm8_swiglu_launch(t, p, o, at::cuda::getCurrentCUDAStream()), 1);
+}
+
 struct Swiglu8Fn : public torch::autograd::Function<Swiglu8Fn> {
   static at::Tensor forward(AutogradContext* ctx, at::Tensor ab) {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -621,11 +680,7 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
     const at::Tensor mem = now.on(x);
     pack_all({{x, &xr, of & 2 ? &c.xt : nullptr}, {w1, &w1r, of & 1 ? &c.w1t : nullptr}, {w2, &w2r, of & 3 ? &c.w2t : nullptr}});
     int* const e = err_word(err, x);
-    {
-      at::Tensor ab = fresh({M, 2 * H}, x.scalar_type(), x);
-      product(xr, w1r, ab, nullptr, false, e);
-      swiglu_forward(ab, nullptr, of & 3 ? &c.ck : nullptr, &g8, of & 4 ? &c.gt : nullptr, e);
-    }
+    product_swiglu(xr, w1r, x, of & 3 ? &c.ck : nullptr, g8, of & 4 ? &c.gt : nullptr, e);
     at::Tensor y = fresh({M, N}, x.scalar_type(), x);
     product(g8, w2r, y, nullptr, false, e);
     ctx->save_for_backward({checkpoint});
@@ -703,9 +758,8 @@ at::Tensor mlp8(at::Tensor x, at::Tensor w1, at::Tensor w2, at::Tensor err) {
   const at::Tensor mem = now.on(x);
   pack_all({{x, &xr, nullptr}, {w1, &w1r, nullptr}, {w2, &w2r, nullptr}});
   int* const e = err_word(err, x);
-  at::Tensor ab = fresh({x.size(0), w1.size(0)}, x.scalar_type(), x), y = fresh({x.size(0), w2.size(0)}, x.scalar_type(), x);
-  product(xr, w1r, ab, nullptr, false, e);
-  swiglu_forward(ab, nullptr, nullptr, &g8, nullptr, e);
+  at::Tensor y = fresh({x.size(0), w2.size(0)}, x.scalar_type(), x);
+  product_swiglu(xr, w1r, x, nullptr, g8, nullptr, e);
   product(g8, w2r, y, nullptr, false, e);
   return y;
 }
@@ -725,13 +779,20 @@ at::Tensor mlp8_frozen(at::Tensor x, at::Tensor c1, at::Tensor s1, at::Tensor c2
   x = rows_of(x);
   int* const e = err_word(err, x);
   const int64_t M = x.size(0);
-  at::Tensor ab = fresh({M, 2 * H}, x.scalar_type(), x), y = fresh({M, w2.rows}, x.scalar_type(), x);
-  times_held(x, w1, ab, nullptr, e);
-  Packed g8;
+  at::Tensor y = fresh({M, w2.rows}, x.scalar_type(), x);
+  Packed xr, g8;
   Arena now;
+  if (M > kFewRows) now.add(&xr, M, K);
   now.add(&g8, M, H);
   const at::Tensor mem = now.on(x);
-  swiglu_forward(ab, nullptr, nullptr, &g8, nullptr, e);
+  if (M > kFewRows) {
+    pack({x, &xr, nullptr});
+    product_swiglu(xr, w1, x, nullptr, g8, nullptr, e);
+  } else {
+    at::Tensor ab = fresh({M, 2 * H}, x.scalar_type(), x);
+    times_held(x, w1, ab, nullptr, e);
+    swiglu_forward(ab, nullptr, nullptr, &g8, nullptr, e);
+  }
   product(g8, w2, y, nullptr, false, e);
   return y;
 }
@@ -751,6 +812,7 @@ void bind_blocks8(pybind11::module_& m) {
     TORCH_CHECK(t >= -1 && t <= 2, "set_gemm8_tile: -1 (chosen by size), 0 (128 x 128), 1 (256 x 192), 2 (256 x 256)");
     g_tile = (int)t;
   }, "tile of the 8-bit products (A/B runs)");
+  m.def("set_mlp8_fused", [](bool on) { g_fused = on; }, "MLP's first 8-bit product with its activation in one launch (A/B runs)");
   m.def("linear8_frozen", &linear8_frozen, "x times a weight held in 8 bits");
   m.def("linear8", &linear8, "linear layer on 8-bit products, forward and backward");
   m.def("swiglu8", &swiglu8, "silu(a) b with its input kept in 8 bits for the backward");

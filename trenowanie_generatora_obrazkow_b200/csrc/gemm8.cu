@@ -11,8 +11,10 @@
 // every fourth block.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "block_ops.h"
+#include "blocks8.cuh"
 #include "blocks8.h"
 #include "common.cuh"
 #include "vec.cuh"
@@ -23,21 +25,24 @@ int num_sms();  // gemm.cu
 
 namespace {
 
-constexpr int BM = 128, BK = 128, THREADS = 192;
-constexpr int ATOM = 512;
+constexpr int BM = 128, BK = 128;
 
 // Two CTAs of a cluster share a tile of 256 x BN (PAIR, cta_group::2): each loads 128 rows of A and half of B's, so a block
 // of k moves 32 KB (BN 256) or 28 KB (BN 192) into an SM in the 512 or 384 cycles that its products take. An SM takes in some
 // 64 bytes a cycle while all do: one CTA with 128 x 256 (48 KB) ran at 2.4 PFLOP/s where the pairs reach 2.9 to 3.1.
-template <int BN, bool PAIR>
+// S: void, or the 16-bit type of a SwiGLU epilogue's [a | b], whose results leave in 8 bits alone (see there)
+template <int BN, bool PAIR, typename S>
 struct Cfg {
+  static constexpr bool SWIGLU = !std::is_void<S>::value;
+  static constexpr int EPI_WARPS = SWIGLU ? 16 : 4, THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int A_BYTES = BM * BK, B_ROWS = PAIR ? BN / 2 : BN, B_BYTES = B_ROWS * BK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = STAGE_BYTES == 32768 ? 6 : 7;
+  static constexpr int STAGES = SWIGLU ? 5 : STAGE_BYTES == 32768 ? 6 : 7;
   static constexpr int B_ATOMS = (BN + 127) / 128;         // a tile of 192 begins at the start or the middle of an atom
   static constexpr int SF_BYTES = (1 + B_ATOMS) * ATOM;    // of a stage: A's atom, B's atoms
-  static constexpr int C_STAGE = 4096;                    // epilogue staging of one warp
-  static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + ((STAGES * SF_BYTES + 1023) & ~1023) + 4 * C_STAGE;
+  static constexpr int C_STAGE = SWIGLU ? 3072 : 4096;    // epilogue staging of one warp
+  static constexpr int MAXIMA = SWIGLU ? (4 * 3 + 4 + 1) * BM * 4 : 0;
+  static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + ((STAGES * SF_BYTES + 1023) & ~1023) + EPI_WARPS * C_STAGE + MAXIMA;
   // Tensor memory (512 columns): two accumulators and the scale factors. Two of 256 columns leave no room, so they share
   // 16 columns, which the epilogue reads first: the next sum waits for that, some 2600 cycles a tile.
   static constexpr int ACC1 = BN == 256 ? 240 : BN;
@@ -124,6 +129,15 @@ __device__ __forceinline__ void store_rows(const Gemm8Problem& q, long long at, 
   }
 }
 
+struct Gemm8Swiglu {
+  CUtensorMap ck_map, g8_map, g8t_map;
+  Side ck, g8, g8t;
+};
+
+struct NoSwiglu {};
+template <typename S>
+using SwigluOf = std::conditional_t<std::is_void<S>::value, NoSwiglu, Gemm8Swiglu>;
+
 // The tiles of a unit (a CTA, a pair), one after another. The tiles of the first product (the longer ones) are dealt out in
 // turn; where that leaves `late` units with one more than the others, these others take `spare` rounds of the second product's
 // tiles before all take part: two products end together that apart would each leave units idle in their last wave.
@@ -146,11 +160,72 @@ struct Schedule {
   }
 };
 
-template <int BN, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1)
-    gemm8_kernel(const __grid_constant__ Gemm8Maps maps, const __grid_constant__ Gemm8Params p) {
-  using F = Cfg<BN, PAIR>;
-  constexpr int STAGES = F::STAGES, TM = PAIR ? 2 * BM : BM, EPI_WARPS = PAIR ? 8 : 4;
+// ------------------------------------------------------------------------------------------------- SwiGLU epilogue
+// One CTA's half of a tile of 256 rows x (128 columns a | the same 128 columns b): a and b, rounded to S, stay in registers, g =
+// silu(a) b in fp32; they leave as 8-bit blocks alone: the checkpoint of a and b, g along its rows, g along its columns. A
+// tile is a block of both axes, so no other CTA is asked for a maximum. Sixteen warps: quarter (32 rows, a thread each) x strip
+// (32 columns), what two blocks' values and a third in fp32 leave room for in registers. The strips of a row meet in shared
+// memory, as do the quarters of a column, whose maximum over a warp's rows is one integer reduction.
+struct SwigluShared {
+  float rows[4][3][BM];  // [strip][a, b, g][row]
+  float cols[4][BM];     // [quarter][column]: of g
+  float inv[BM];         // 2^-e of g's columns
+};
+__device__ __forceinline__ bool all_of_512(bool ok) {  // barrier of the epilogue's warps, with their verdict
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 512, p;\n\tselp.u32 %0, 1, 0, q;\n}"
+               : "=r"(r) : "r"((uint32_t)ok) : "memory");
+  return r != 0;
+}
+template <typename S>
+struct PairOf;
+template <>
+struct PairOf<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+  static __device__ __forceinline__ float2 get(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+};
+template <>
+struct PairOf<__half> {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 get(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+};
+__device__ __forceinline__ float finite_or_nan(float v) { return fabsf(v) == INFINITY ? NAN : v; }
+// 16 pairs of a row: the largest finite magnitude; infinities become NaN
+template <typename S>
+__device__ __forceinline__ float finite_top16(uint32_t (&u)[16]) {
+  auto top = [&] {
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 v = PairOf<S>::get(u[j]);
+      m = max3(m, fabsf(v.x), fabsf(v.y));
+    }
+    return m;
+  };
+  float m = top();
+  if (m == INFINITY) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 v = PairOf<S>::get(u[j]);
+      u[j] = PairOf<S>::pack(finite_or_nan(v.x), finite_or_nan(v.y));
+    }
+    m = top();
+  }
+  return m;
+}
+
+template <int BN, bool PAIR, typename S>
+__global__ void __launch_bounds__((Cfg<BN, PAIR, S>::THREADS), 1)
+    gemm8_kernel(const __grid_constant__ Gemm8Maps maps, const __grid_constant__ Gemm8Params p,
+                 const __grid_constant__ SwigluOf<S> sw) {
+  using F = Cfg<BN, PAIR, S>;
+  constexpr bool SWIGLU = F::SWIGLU;
+  constexpr int STAGES = F::STAGES, TM = PAIR ? 2 * BM : BM, EPI_WARPS = (PAIR ? 2 : 1) * F::EPI_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const smem_sf = smem + STAGES * F::STAGE_BYTES;
@@ -196,7 +271,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_sh;
-
   // The two warps that feed the tensor core run as whole warps and elect a lane where an instruction wants one thread: the
   // operands then stay in uniform registers. With one lane in the loop each product cost its thread some 70 cycles of moving
   // operands, and the thread, not the tensor core, was the bound (690 cycles for a block of 4 x 128).
@@ -209,11 +283,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int step = 0; ok && sched.at(p, step, which, tile); ++step) {
       const Gemm8Problem& q = p.q[which];
       const CUtensorMap *tmA = &maps.a[which], *tmB = &maps.b[which], *tmSA = &maps.sa[which], *tmSB = &maps.sb[which];
-      const int num_n = (q.N + BN - 1) / BN;
+      const int num_n = (q.N + BN - 1) / BN;  // SwiGLU: N is a multiple of 256
       const int kq = (q.kb + 3) / 4;      // scale atoms of a row tile
       const int nbt = (q.N + 127) / 128;  // row tiles of B's scales
       const int mt = tile / num_n, nt = tile % num_n;
-      const int m0 = mt * TM + rank * BM, n0 = nt * BN + rank * F::B_ROWS;
+      // SwiGLU: one CTA brings the rows of a, the other those of b
+      const int m0 = mt * TM + rank * BM, n0 = SWIGLU ? nt * 128 + rank * (q.N / 2) : nt * BN + rank * F::B_ROWS;
       for (int kb = 0; kb < q.kb; ++kb) {
         if (!free) {
           ok = __all_sync(0xffffffffu, mbar_wait_poll(&empty_bar[stage], phase ^ 1, p.err, ERR_MBAR_TIMEOUT_PRODUCER) &&
@@ -234,7 +309,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             tma_load_3d_pair(sa + F::A_BYTES, tmB, bar, kb * BK, n0, 0);
             if (scales) {
               tma_load_3d_pair(sf, tmSA, bar, 0, kb >> 2, mt * 2 + rank);
-              tma_load_3d_pair(sf + ATOM, tmSB, bar, 0, kb >> 2, nt * BN / 128);
+              if constexpr (SWIGLU) {
+                tma_load_3d_pair(sf + ATOM, tmSB, bar, 0, kb >> 2, nt);
+                tma_load_3d_pair(sf + 2 * ATOM, tmSB, bar, 0, kb >> 2, q.N / 256 + nt);
+              } else {
+                tma_load_3d_pair(sf + ATOM, tmSB, bar, 0, kb >> 2, nt * BN / 128);
+              }
             }
           } else {
             const int nb = min(F::B_ATOMS, nbt - nt * (BN / 128));
@@ -328,8 +408,162 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
       }
     }
+  } else if constexpr (SWIGLU) {
+    // ---------------- SwiGLU epilogue ----------------
+    const int quarter = warp & 3, strip = (warp - 2) >> 2, r = quarter * 32 + lane;
+    uint8_t* const buf = smem_c + (warp - 2) * F::C_STAGE;  // 32 rows (of a, then of g; of b) and 32 columns of 32 bytes
+    SwigluShared& sh = *reinterpret_cast<SwigluShared*>(smem_c + F::EPI_WARPS * F::C_STAGE);
+    const Gemm8Problem& q = p.q[0];
+    const int nhb = q.N / 256, nmb = (q.M + 127) / 128;
+    int unit = 0, which, tile;
+    for (int step = 0; sched.at(p, step, which, tile); ++step, ++unit) {
+      const int hb = tile % nhb, mb = (tile / nhb) * 2 + rank;
+      int got = 0;
+      if (lane == 0) got = mbar_wait_poll(&tfull_bar[unit & 1], (unit >> 1) & 1, p.err, ERR_MBAR_TIMEOUT_EPILOGUE) ? 1 : 0;
+      const bool ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+      tc_fence_after();
+      const uint32_t t = tmem_base + ((unit & 1) ? F::ACC1 : 0) + ((uint32_t)(quarter * 32) << 16) + 32 * strip;
+      uint32_t pa[16], pb[16];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t ra[16], rb[16];
+        tmem_ld_32x32b_x16(t + 16 * c, ra);
+        tmem_ld_32x32b_x16(t + 128 + 16 * c, rb);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          pa[8 * c + j] = PairOf<S>::pack(__uint_as_float(ra[2 * j]), __uint_as_float(ra[2 * j + 1]));
+          pb[8 * c + j] = PairOf<S>::pack(__uint_as_float(rb[2 * j]), __uint_as_float(rb[2 * j + 1]));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[unit & 1]), 0));
+      if (sw.ck.codes != nullptr) {
+        sh.rows[strip][0][r] = finite_top16<S>(pa);
+        sh.rows[strip][1][r] = finite_top16<S>(pb);
+      }
+      if (!all_of_512(ok)) {  // every warp's wait ends by itself, so all are here
+        abort_sh = 1;
+        break;
+      }
+      // strip k writes the scales of a, b, g and of g's columns
+      auto row_scale = [&](int k, const Side& o, int b, int blocks) {
+        const int byte = scale_byte(fmaxf(fmaxf(sh.rows[0][k][r], sh.rows[1][k][r]), fmaxf(sh.rows[2][k][r], sh.rows[3][k][r])));
+        if (strip == k && mb < nmb) {
+          uint8_t* s = o.scales + scale_at(mb * BM + r, b, o.quads);
+          s[0] = (uint8_t)byte;
+          if (b == blocks - 1)
+            for (int i = 1; i < 4 - (b & 3); ++i) s[i] = 0;
+        }
+        return scale_inv(byte);
+      };
+      const int m0 = mb * BM + quarter * 32, h0 = hb * 128 + 32 * strip;
+      const bool rows_there = m0 < q.M;
+      auto send = [&](const CUtensorMap* map, uint8_t* from, int x, int y) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(map, from, x, y, 0);
+          bulk_commit_group();
+        }
+      };
+      // half i of a row's 32 bytes, in the 32-byte swizzle of the maps
+      auto half = [&](uint8_t* to, int i) { return reinterpret_cast<uint4*>(to + lane * 32 + ((i ^ ((lane >> 2) & 1)) << 4)); };
+      auto put_pairs = [&](uint8_t* to, const uint32_t(&u)[16], float inv) {
+        const float2 s = make_float2(inv, inv);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t w[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            w[n] = codes4(mul2(PairOf<S>::get(u[8 * i + 2 * n]), s), mul2(PairOf<S>::get(u[8 * i + 2 * n + 1]), s));
+          *half(to, i) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      };
+      if (lane == 0) bulk_wait_group_read<0>();
+      __syncwarp();
+      if (sw.ck.codes != nullptr) {
+        const float inv_a = row_scale(0, sw.ck, hb, 2 * nhb), inv_b = row_scale(1, sw.ck, nhb + hb, 2 * nhb);
+        if (rows_there) {
+          put_pairs(buf, pa, inv_a);
+          send(&sw.ck_map, buf, h0, m0);
+          put_pairs(buf + 1024, pb, inv_b);
+          send(&sw.ck_map, buf + 1024, q.N / 2 + h0, m0);
+        }
+      }
+      float g[32];
+      float mg = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 a = PairOf<S>::get(pa[j]);
+        const float2 v = mul2(mul2(a, make_float2(sigmoid<false>(a.x), sigmoid<false>(a.y))), PairOf<S>::get(pb[j]));
+        g[2 * j] = v.x;
+        g[2 * j + 1] = v.y;
+        mg = max3(mg, fabsf(v.x), fabsf(v.y));
+      }
+      if (mg == INFINITY) {
+        mg = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) mg = fmaxf(mg, fabsf(g[j] = finite_or_nan(g[j])));
+      }
+      sh.rows[strip][2][r] = mg;
+      if (sw.g8t.codes != nullptr) {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(g[j]), 0.f)));  // passes over NaN
+          if (lane == j) mine = top;
+        }
+        sh.cols[quarter][32 * strip + lane] = __uint_as_float(mine);
+      }
+      asm volatile("bar.sync 1, 512;" ::: "memory");  // g's maxima are there, those of a and b read
+      const float inv_g = row_scale(2, sw.g8, hb, nhb);
+      if (sw.g8t.codes != nullptr && strip == 3) {
+        const int byte = scale_byte(fmaxf(fmaxf(sh.cols[0][r], sh.cols[1][r]), fmaxf(sh.cols[2][r], sh.cols[3][r])));
+        sh.inv[r] = scale_inv(byte);
+        if (mb < nmb) {
+          uint8_t* s = sw.g8t.scales + scale_at(hb * 128 + r, mb, sw.g8t.quads);
+          s[0] = (uint8_t)byte;
+          if (mb == nmb - 1)
+            for (int i = 1; i < 4 - (mb & 3); ++i) s[i] = 0;
+        }
+      }
+      asm volatile("bar.sync 1, 512;" ::: "memory");  // the scales of g's columns are there
+      if (sw.g8t.codes != nullptr && m0 < nmb * BM) {
+        uint8_t* to = buf + 2048 + lane;
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 k = *reinterpret_cast<const float2*>(&sh.inv[32 * strip + j]);
+          const uint32_t w = codes2(g[j] * k.x, g[j + 1] * k.y);
+          to[j * 32] = (uint8_t)w;
+          to[(j + 1) * 32] = (uint8_t)(w >> 8);
+        }
+        send(&sw.g8t_map, buf + 2048, m0, h0);
+      }
+      if (rows_there) {
+        if (lane == 0) {  // a's codes are out of the buffer; those of b and of g's columns may not be
+          if (sw.g8t.codes != nullptr) bulk_wait_group_read<2>();
+          else bulk_wait_group_read<1>();
+        }
+        __syncwarp();
+        const float2 s = make_float2(inv_g, inv_g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t w[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float* v = &g[16 * i + 4 * n];
+            w[n] = codes4(mul2(make_float2(v[0], v[1]), s), mul2(make_float2(v[2], v[3]), s));
+          }
+          *half(buf, i) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        send(&sw.g8_map, buf, h0, m0);
+      }
+    }
+    if (lane == 0) bulk_wait_group_all();
   } else {
-    // ---------------- epilogue: warp q owns rows 32 q .. 32 q + 31 of the tile ----------------
+    // ---------------- epilogue: a warp owns 32 rows of the tile ----------------
     const int quarter = warp & 3;
     uint8_t* const cbuf = smem_c + quarter * F::C_STAGE;
     int turn = 0, unit = 0, which, tile;
@@ -430,10 +664,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <int BN, bool PAIR>
-cudaError_t launch(const Gemm8Maps& t, Gemm8Params& p, Gemm8Tile tile, cudaStream_t s) {
-  using F = Cfg<BN, PAIR>;
-  auto kern = gemm8_kernel<BN, PAIR>;
+template <int BN, bool PAIR, typename S = void>
+cudaError_t launch(const Gemm8Maps& t, Gemm8Params& p, const SwigluOf<S>& sw, Gemm8Tile tile, cudaStream_t s) {
+  using F = Cfg<BN, PAIR, S>;
+  auto kern = gemm8_kernel<BN, PAIR, S>;
   static_assert(F::SMEM + 1024 <= 232448, "dynamic + static shared memory");
   static std::atomic<uint64_t> set{0};  // bit d: done on device d
   int dev = 0;
@@ -461,7 +695,7 @@ cudaError_t launch(const Gemm8Maps& t, Gemm8Params& p, Gemm8Tile tile, cudaStrea
   }
   cudaLaunchConfig_t c{};
   c.gridDim = dim3(PAIR ? 2 * units : units);
-  c.blockDim = dim3(THREADS);
+  c.blockDim = dim3(F::THREADS);
   c.dynamicSmemBytes = F::SMEM;
   c.stream = s;
   cudaLaunchAttribute cluster{};
@@ -470,7 +704,7 @@ cudaError_t launch(const Gemm8Maps& t, Gemm8Params& p, Gemm8Tile tile, cudaStrea
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   c.attrs = &cluster;
   c.numAttrs = PAIR ? 1 : 0;
-  e = cudaLaunchKernelEx(&c, kern, t, p);
+  e = cudaLaunchKernelEx(&c, kern, t, p, sw);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -484,19 +718,39 @@ long long gemm8_tile_cycles(const Gemm8Problem& q, Gemm8Tile tile, bool fills) {
   return tile == TILE_PAIR_192 ? (long long)q.kb * 430 + sums * 800 : (long long)q.kb * 512 + sums * 2600;
 }
 
-cudaError_t gemm8_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8Tile tile, cudaStream_t s) {
-  if (p.n < 1 || p.n > 2) return cudaErrorInvalidValue;
+static bool valid(const Gemm8Params& p) {
+  if (p.n < 1 || p.n > 2) return false;
   for (int i = 0; i < p.n; ++i) {
     const Gemm8Problem& q = p.q[i];
-    if (q.M <= 0 || q.N <= 0 || q.kb <= 0 || q.chunk_kb <= 0 || q.chunk_kb % 4 != 0) return cudaErrorInvalidValue;
-    if (q.elem != ELEM_F32 && (q.add || q.chunk_kb < q.kb)) return cudaErrorInvalidValue;
-    if (q.elem < ELEM_BF16 || q.elem > ELEM_F32 || (q.add && q.bias != nullptr)) return cudaErrorInvalidValue;
+    if (q.M <= 0 || q.N <= 0 || q.kb <= 0 || q.chunk_kb <= 0 || q.chunk_kb % 4 != 0) return false;
+    if (q.elem != ELEM_F32 && (q.add || q.chunk_kb < q.kb)) return false;
+    if (q.elem < ELEM_BF16 || q.elem > ELEM_F32 || (q.add && q.bias != nullptr)) return false;
   }
+  return true;
+}
+cudaError_t gemm8_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8Tile tile, cudaStream_t s) {
+  if (!valid(p)) return cudaErrorInvalidValue;
+  const NoSwiglu none{};
   switch (tile) {
-    case TILE_PAIR_256: return launch<256, true>(t, p, tile, s);
-    case TILE_PAIR_192: return launch<192, true>(t, p, tile, s);
-    case TILE_128x128: return launch<128, false>(t, p, tile, s);
+    case TILE_PAIR_256: return launch<256, true>(t, p, none, tile, s);
+    case TILE_PAIR_192: return launch<192, true>(t, p, none, tile, s);
+    case TILE_128x128: return launch<128, false>(t, p, none, tile, s);
   }
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t gemm8_swiglu_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8SwigluOut o, cudaStream_t s) {
+  if (!valid(p) || p.n != 1 || p.q[0].N % 256 != 0 || p.q[0].bias != nullptr || o.g8 == nullptr) return cudaErrorInvalidValue;
+  const int H = p.q[0].N / 2, M = p.q[0].M;
+  Gemm8Swiglu sw{};
+  sw.ck = side(o.ck, o.ck_scales, M, 2 * H);
+  sw.g8 = side(o.g8, o.g8_scales, M, H);
+  sw.g8t = side(o.g8t, o.g8t_scales, H, M);
+  sw.ck_map = *o.ck_map;
+  sw.g8_map = *o.g8_map;
+  sw.g8t_map = *o.g8t_map;
+  if (p.q[0].elem == ELEM_BF16) return launch<256, true, __nv_bfloat16>(t, p, sw, TILE_PAIR_256, s);
+  if (p.q[0].elem == ELEM_F16) return launch<256, true, __half>(t, p, sw, TILE_PAIR_256, s);
   return cudaErrorInvalidValue;
 }
 
