@@ -424,21 +424,24 @@ __global__ void __launch_bounds__((Cfg<BN, PAIR, S>::THREADS), 1)
       tc_fence_after();
       const uint32_t t = tmem_base + ((unit & 1) ? F::ACC1 : 0) + ((uint32_t)(quarter * 32) << 16) + 32 * strip;
       uint32_t pa[16], pb[16];
+      // the accumulators' shared columns first: the last 16 of the even one's b, the first 16 of the odd one's a
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t ra[16], rb[16];
         tmem_ld_32x32b_x16(t + 16 * c, ra);
-        tmem_ld_32x32b_x16(t + 128 + 16 * c, rb);
+        tmem_ld_32x32b_x16(t + 128 + 16 * (c ^ 1), rb);
         tmem_ld_wait();
+        if (c == 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[unit & 1]), 0));
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           pa[8 * c + j] = PairOf<S>::pack(__uint_as_float(ra[2 * j]), __uint_as_float(ra[2 * j + 1]));
-          pb[8 * c + j] = PairOf<S>::pack(__uint_as_float(rb[2 * j]), __uint_as_float(rb[2 * j + 1]));
+          pb[8 * (c ^ 1) + j] = PairOf<S>::pack(__uint_as_float(rb[2 * j]), __uint_as_float(rb[2 * j + 1]));
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty_bar[unit & 1]), 0));
       if (sw.ck.codes != nullptr) {
         sh.rows[strip][0][r] = finite_top16<S>(pa);
         sh.rows[strip][1][r] = finite_top16<S>(pb);
