@@ -414,13 +414,12 @@ cudaError_t unpack_typed(const uint8_t* codes, const uint8_t* scales, int R, int
 
 // ----------------------------------------------------------------------------------------------------------- SwiGLU
 // g in ab's type, the checkpoint of ab in 8 bits. Rows alone: a thread holds 8 columns of ROW_R rows (two: enough warps to keep
-// the memory busy; at 32768 x 5504 the
-// backward took 265 us with four, 212 with two). The checkpoint's
-// blocks are those of a [M, 2 Hp] matrix: a's first, then b's. Rows past the last are read as the last one and not written.
+// the memory busy; at 32768 x 5504 the backward took 265 us with four, 212 with two). The checkpoint's blocks are those of a
+// [M, 2 Hp] matrix: a's first, then b's. Rows past the last are read as the last one and not written.
 constexpr int ROW_R = 2;
 template <typename T, bool VEC, bool CK>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) swiglu8_fwd_kernel(const T* __restrict__ ab, long long ld, int M, int H, bool vec_g,
-                                                          T* __restrict__ g, Side ck) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4)
+    swiglu8_fwd_kernel(const T* __restrict__ ab, long long ld, int M, int H, bool vec_g, T* __restrict__ g, Side ck) {
   const int nhb = (H + TILE - 1) / TILE;
   const int hb = blockIdx.x % nhb, l16 = threadIdx.x & 15;
   const int r0 = (blockIdx.x / nhb) * 16 * ROW_R + (threadIdx.x >> 4) * ROW_R;
@@ -507,7 +506,8 @@ __global__ void __launch_bounds__(256) swiglu8_bwd_kernel(const T* __restrict__ 
   }
 }
 
-// ---- the forms of the MLP: everything that is written is in 8 bits, both ways where a weight's gradient wants it. One CTA of
+// ---- the forms of the MLP: everything that is written is in 8 bits, both ways where a weight's gradient wants it (the forward
+// of 16-bit types has them in its product's epilogue but for few rows, which want g along the rows alone). One CTA of
 // 512 threads per SM walks over tiles of 128 x 128; the tiles come by TMA, two ahead of the arithmetic (fp32: one), so no
 // registers and no address arithmetic go into loads. A thread holds 8 columns of 4 rows; the backward holds da and db at once
 // and takes each exponential once. What bounds them is the arithmetic: some 25 and 30 instructions an element.
@@ -777,11 +777,15 @@ cudaError_t swiglu_fwd_typed(const Swiglu8Params& p, cudaStream_t s) {
   if (p.g8 != nullptr) {
     const long long tiles = (long long)nhb * ((p.M + TILE - 1) / TILE);
     if (tiles >= (1ll << 30) || p.map == nullptr) return cudaErrorInvalidValue;
-    if (p.g8t != nullptr)
-      return p.ck != nullptr ? swiglu_fwd_q<T, true, true>(*p.map, p, tiles, ck, g8, g8t, s)
-                             : swiglu_fwd_q<T, true, false>(*p.map, p, tiles, ck, g8, g8t, s);
-    return p.ck != nullptr ? swiglu_fwd_q<T, false, true>(*p.map, p, tiles, ck, g8, g8t, s)
-                           : swiglu_fwd_q<T, false, false>(*p.map, p, tiles, ck, g8, g8t, s);
+    if constexpr (sizeof(T) == 4) {
+      if (p.g8t != nullptr)
+        return p.ck != nullptr ? swiglu_fwd_q<T, true, true>(*p.map, p, tiles, ck, g8, g8t, s)
+                               : swiglu_fwd_q<T, true, false>(*p.map, p, tiles, ck, g8, g8t, s);
+      if (p.ck != nullptr) return swiglu_fwd_q<T, false, true>(*p.map, p, tiles, ck, g8, g8t, s);
+    } else if (p.g8t != nullptr || p.ck != nullptr) {
+      return cudaErrorInvalidValue;
+    }
+    return swiglu_fwd_q<T, false, false>(*p.map, p, tiles, ck, g8, g8t, s);
   }
   const long long blocks = (long long)nhb * ((p.M + 16 * ROW_R - 1) / (16 * ROW_R));
   if (blocks >= (1ll << 31)) return cudaErrorInvalidValue;

@@ -568,7 +568,6 @@ CUtensorMap bytes_map(const uint8_t* base, uint64_t inner, uint64_t rows, uint32
   TORCH_CHECK(r == CUDA_SUCCESS, "tensor map of 8-bit outputs: code ", (int)r);
   return m;
 }
-std::atomic<bool> g_fused{true};  // for comparisons: the MLP's first product and its activation in one launch
 // [a | b] = x w^T rounded to `like`'s type, g = silu(a) b: the checkpoint (ck, or null), g along its rows and (g8t, or null) its
 // columns. 16-bit types: one launch, the activations stay on the chip; fp32 (whose values do not fit the registers): two.
 void product_swiglu(const Packed& x, const Packed& w, const at::Tensor& like, const Packed* ck, const Packed& g8,
@@ -576,7 +575,7 @@ void product_swiglu(const Packed& x, const Packed& w, const at::Tensor& like, co
   const int64_t M = x.rows, H = w.rows / 2;
   if (M == 0) return;
   const int elem = elem_of(like, kWhat);
-  if (elem == ELEM_F32 || !g_fused) {
+  if (elem == ELEM_F32) {
     at::Tensor ab = fresh({M, 2 * H}, like.scalar_type(), like);
     product(x, w, ab, nullptr, false, err);
     swiglu_forward(ab, nullptr, ck, &g8, g8t, err);
@@ -812,7 +811,6 @@ void bind_blocks8(pybind11::module_& m) {
     TORCH_CHECK(t >= -1 && t <= 2, "set_gemm8_tile: -1 (chosen by size), 0 (128 x 128), 1 (256 x 192), 2 (256 x 256)");
     g_tile = (int)t;
   }, "tile of the 8-bit products (A/B runs)");
-  m.def("set_mlp8_fused", [](bool on) { g_fused = on; }, "MLP's first 8-bit product with its activation in one launch (A/B runs)");
   m.def("linear8_frozen", &linear8_frozen, "x times a weight held in 8 bits");
   m.def("linear8", &linear8, "linear layer on 8-bit products, forward and backward");
   m.def("swiglu8", &swiglu8, "silu(a) b with its input kept in 8 bits for the backward");
