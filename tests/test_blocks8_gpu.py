@@ -426,6 +426,23 @@ def test_mlp_gives_the_same_whatever_it_keeps(M, K, H, dtype):
         assert torch.equal(every[0], B8.mlp_blocks(x, B8.quantize_blocks(w1), B8.quantize_blocks(w2)))
 
 
+@pytest.mark.parametrize("before", [False, True])
+def test_mlp_of_one_weight_twice(before):
+    """in_proj and out_proj the same parameter: its gradient is the sum of both, added to what was there."""
+    H = 128
+    x, w, dy = rnd(70, H, seed=1), rnd(2 * H, H, seed=2, std=H ** -0.5, dtype=torch.float32), rnd(70, 2 * H, seed=3)
+    two = [w.clone().requires_grad_(), w.clone().requires_grad_()]
+    B8.mlp_blocks(x, *two).backward(dy)
+    one = w.clone().requires_grad_()
+    if before:
+        one.grad = torch.ones_like(w)
+    B8.mlp_blocks(x, one, one).backward(dy)
+    want = two[0].grad.double() + two[1].grad.double() + float(before)
+    # two fp32 additions, each off by half a step of its result
+    tol = 2.0 ** -24 * (want.abs() + (1 + two[1].grad.double()).abs() + (1 + two[0].grad.double()).abs())
+    assert ((one.grad.double() - want).abs() <= tol * 1.001).all()
+
+
 # ----------------------------------------------------------------------------------------------------- streams, graphs
 def test_captured_and_replayed():
     lin = torch.nn.Linear(256, 384, device=DEV)

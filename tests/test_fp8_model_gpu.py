@@ -1,4 +1,6 @@
 """The DiT on 8-bit products and with 8-bit activation checkpoints on the GPU, and the operators in a run together."""
+import io
+
 import pytest
 import torch
 
@@ -172,3 +174,54 @@ def test_far_scales(M):
     x, w = torch.full((M, 128), 2.0 ** 118, device="cuda"), torch.full((16, 128), 2.0 ** -60, device="cuda")
     got = B8.linear_blocks(x, B8.quantize_blocks(w))
     assert torch.equal(got, torch.full((M, 16), 2.0 ** 65, device="cuda"))
+
+
+def test_captured_layer_packs_for_itself():
+    """A graph of marked layers without gradients reads the weights as they are at each replay, and leaves nothing behind that
+    an eager call would take for packed."""
+    from trenowanie_generatora_obrazkow_b200.models.quant import use_fp8
+    te, den = _model()
+    use_fp8(den)
+    mlp, qkv = den.blocks[0].mlp, den.blocks[0].attn.qkv
+    x = torch.randn(300, 512, device="cuda", dtype=torch.bfloat16)
+
+    def run():
+        return Fz.mlp_fp8(x, mlp.in_proj, mlp.out_proj), Fz.linear(x, qkv)
+    with torch.no_grad():
+        other = torch.cuda.Stream()
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            B8.mlp_blocks(x, mlp.in_proj, mlp.out_proj)
+        torch.cuda.current_stream().wait_stream(other)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run()
+        first = run()  # before any replay
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+        for lin in (mlp.in_proj, mlp.out_proj, qkv):
+            lin.weight.mul_(1.25)
+        graph.replay()
+        want = run()
+        assert all(torch.equal(a, b) and not torch.equal(a, c) for a, b, c in zip(got, want, first))
+
+
+def test_packed_weight_on_another_stream():
+    lin = torch.nn.Linear(2048, 8192, device="cuda", bias=False)
+    lin.fp8 = True
+    x = torch.randn(64, 2048, device="cuda", dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+    with torch.no_grad():
+        want = B8.linear_blocks(x, B8.quantize_blocks(lin.weight))
+        torch.cuda.synchronize()
+        for _ in range(20):
+            lin.weight._tgo_fp8 = None
+            first = Fz.linear(x, lin)  # packs here
+            with torch.cuda.stream(side):
+                second = Fz.linear(x, lin)
+            torch.cuda.synchronize()
+            assert torch.equal(first, want) and torch.equal(second, want)
+        file = io.BytesIO()
+        torch.save(lin, file)  # the copy and its stream stay behind
+        again = torch.load(io.BytesIO(file.getvalue()), weights_only=False)
+        assert again.weight._tgo_fp8 is None and torch.equal(Fz.linear(x, again), want)

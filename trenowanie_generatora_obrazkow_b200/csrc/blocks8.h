@@ -92,7 +92,8 @@ struct FewRowsParams {
 };
 cudaError_t few_rows_launch(const FewRowsParams& p, int elem, cudaStream_t s);
 
-// SwiGLU over ab [M, 2 H] (rows ld apart). With g8: H a multiple of 128, of 16-bit types neither ck nor g8t, and map: ab {2 H, M, 1} in its type, box {128, 128, 1}
+// SwiGLU over ab [M, 2 H] (rows ld apart). With g8: H a multiple of 128, of 16-bit types neither ck nor g8t (those are
+// gemm8_swiglu_launch's), and map: ab {2 H, M, 1} in its type, box {128, 128, 1}
 struct Swiglu8Params {
   const void* ab;
   long long ld;

@@ -168,7 +168,8 @@ struct Schedule {
 // memory, as do the quarters of a column, whose maximum over a warp's rows is one integer reduction. The codes leave by TMA
 // through 3 KB of staging a warp, which costs one of the loads' six stages. At 32768 x 2048 -> 2 x 5504 the launch takes 713 us,
 // 14.3 k cycles a tile, of which the epilogue fills 12.7 k (two exponential-unit operations and four conversions an element)
-// beside the next tile's products; product and activation apart took 555 + 331 us, and 2.2 GB went through memory.
+// beside the next tile's products; product and activation apart took 555 + 331 us, and a and b crossed memory
+// twice (1.4 GB).
 struct SwigluShared {
   float rows[4][3][BM];  // [strip][a, b, g][row]
   float cols[4][BM];     // [quarter][column]: of g

@@ -141,9 +141,9 @@ def swiglu_blocks(ab):
 def mlp_blocks(x, in_proj, out_proj):
     """SwiGLU MLP on 8-bit products: [a | b] = Q(x) Q(W1)^T rounded to x's type, g = silu(a) b, y = Q(g) Q(W2)^T; x [..., K],
     in_proj [2 H, K], out_proj [N, H] (``nn.Linear`` without bias, weight tensors, or both Blocks8: held in 8 bits, no gradient)
-    -> [..., N]. With H a multiple of 128, g, [a | b] and their gradient are
-    written in 8 bits only (of 16-bit types by the first product itself; [a | b] where the backward wants it); other widths run
-    ``linear_blocks``, ``swiglu_blocks`` and ``linear_blocks`` (g is then rounded to x's type before it is packed)."""
+    -> [..., N]. With H a multiple of 128, g, [a | b] and their gradient are written in 8 bits only (of 16-bit types by the first
+    product itself; [a | b] where the backward wants it); other widths run ``linear_blocks``, ``swiglu_blocks`` and
+    ``linear_blocks`` (g is then rounded to x's type before it is packed)."""
     w1, b1 = _weight_of(in_proj, "mlp_blocks")
     w2, b2 = _weight_of(out_proj, "mlp_blocks")
     if b1 is not None or b2 is not None:

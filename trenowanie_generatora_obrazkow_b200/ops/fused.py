@@ -65,12 +65,27 @@ def swiglu_weight(p):
     return ent[1]
 
 
+class _WeightCopy(tuple):
+    """What fp8_weight keeps on a parameter; a parameter that is pickled takes none along."""
+    __slots__ = ()
+
+    def __reduce_ex__(self, protocol):
+        return type(None), ()
+
+
 def fp8_weight(p):
-    """8-bit copy (``blocks8.Blocks8``) of a weight for calls without gradients, cached like bf16_weight."""
+    """8-bit copy (``blocks8.Blocks8``) of a weight for calls without gradients, cached like bf16_weight; another stream than
+    the one that packed it waits for that. A CUDA graph packs for itself: its replays read the weight's values of the time."""
+    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+        return B8.quantize_blocks(p.detach())
     ent = getattr(p, "_tgo_fp8", None)
     ver = p._version
+    stream = torch.cuda.current_stream(p.device) if p.is_cuda else None
     if ent is None or ent[0] != ver or ent[1].codes.device != p.device or ent[1].shape != p.shape:
-        p._tgo_fp8 = ent = (ver, B8.quantize_blocks(p.detach()))
+        p._tgo_fp8 = ent = _WeightCopy((ver, B8.quantize_blocks(p.detach()), stream, stream and stream.record_event()))
+    elif ent[2] != stream:
+        stream.wait_event(ent[3])
+        ent[1].codes.record_stream(stream), ent[1].scales.record_stream(stream)
     return ent[1]
 
 
