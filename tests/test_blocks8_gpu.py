@@ -426,6 +426,20 @@ def test_mlp_gives_the_same_whatever_it_keeps(M, K, H, dtype):
         assert torch.equal(every[0], B8.mlp_blocks(x, B8.quantize_blocks(w1), B8.quantize_blocks(w2)))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,H", [(300, 640, 384), (1000, 256, 1408)])
+def test_mlp_rows_are_those_of_its_parts(M, K, H, dtype):
+    x, w1, w2 = rnd(M, K, seed=1, dtype=dtype), rnd(2 * H, K, seed=2, std=K ** -0.5, dtype=torch.float32), \
+        rnd(96, H, seed=3, std=H ** -0.5, dtype=torch.float32)
+    a, b = B8.linear_blocks(x, w1).float().chunk(2, 1)
+    g = a * torch.sigmoid(a) * b
+    y = B8.gemm_blocks(B8.quantize_blocks(g), B8.quantize_blocks(w2), dtype=dtype)
+    # g may be off by a few 2^-24 of itself, 2^-21 at most; e4m3's borders are at least 2^-4 of a value apart, so one value in
+    # 2^-4 / 2^-20 = 2^16 falls on another side, and of the rows of H values at most one in 2^16 / H (2 %) is touched
+    same = (y == B8.mlp_blocks(x, w1, w2)).all(1).double().mean().item()
+    assert same > 0.9
+
+
 @pytest.mark.parametrize("before", [False, True])
 def test_mlp_of_one_weight_twice(before):
     """in_proj and out_proj the same parameter: its gradient is the sum of both, added to what was there."""

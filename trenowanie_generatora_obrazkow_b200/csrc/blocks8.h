@@ -69,13 +69,13 @@ long long gemm8_tile_cycles(const Gemm8Problem& q, Gemm8Tile tile, bool fills);
 cudaError_t gemm8_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8Tile tile, cudaStream_t s);
 
 // The first product of a SwiGLU MLP, [a | b] = A B^T (B [2 H, K], H a multiple of 128, 16-bit q.elem), and its activation: what
-// the backward and the second product read, in 8 bits. Maps: as TILE_PAIR_256, sb's box {128, 1, 1}; ck {2 H, M, 1} and g8 {H, M,
-// 1} as bytes, boxes {32, 32, 1}, 32-byte swizzle; g8t {Mp, H, 1}, the same box, none.
+// the backward and the second product read, in 8 bits. Maps: as TILE_PAIR_256, sb's box {128, 1, 1}; g8t as bytes {Mp, H, 1}, box
+// {32, 32, 1}, no swizzle.
 struct Gemm8SwigluOut {
   uint8_t *ck, *ck_scales;    // [M, 2 H], or null
   uint8_t *g8, *g8_scales;    // [M, H]
   uint8_t *g8t, *g8t_scales;  // [H, Mp], or null
-  const CUtensorMap *ck_map, *g8_map, *g8t_map;  // any map in place of one that is not wanted
+  const CUtensorMap* g8t_map;
 };
 cudaError_t gemm8_swiglu_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8SwigluOut o, cudaStream_t s);
 

@@ -489,12 +489,13 @@ at::Tensor linear8(at::Tensor x, at::Tensor w, OptT bias, at::Tensor err) {
 }
 
 // ----------------------------------------------------------------------------------------------------------- SwiGLU
-// plain {cols, rows, 1} map with a {128, 128, 1} box
-CUtensorMap tile_map(const void* base, CUtensorMapDataType type, uint64_t size, uint64_t cols, uint64_t rows, uint64_t ld) {
+// plain {cols, rows, 1} map with a {side, side, 1} box
+CUtensorMap tile_map(const void* base, CUtensorMapDataType type, uint64_t size, uint64_t cols, uint64_t rows, uint64_t ld,
+                     uint32_t side = 128) {
   CUtensorMap m;
   cuuint64_t dims[3] = {cols, rows, 1};
   cuuint64_t strides[2] = {ld * size, ld * size * rows};
-  cuuint32_t box[3] = {128, 128, 1};
+  cuuint32_t box[3] = {side, side, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = tmap_encoder()(&m, type, 3, const_cast<void*>(base), dims, strides, box, estr,
                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
@@ -554,20 +555,6 @@ void swiglu_backward(const at::Tensor& dg, const Packed& ck, int64_t H, at::Tens
   BLOCK_LAUNCH(swiglu8_bwd_launch(p, elem_of(dg, "swiglu_blocks"), at::cuda::getCurrentCUDAStream()), 1);
 }
 
-// a map of 8-bit outputs {inner, rows, 1}
-CUtensorMap bytes_map(const uint8_t* base, uint64_t inner, uint64_t rows, uint32_t box_inner, uint32_t box_rows, bool swizzle) {
-  CUtensorMap m;
-  cuuint64_t dims[3] = {inner, rows, 1};
-  cuuint64_t strides[2] = {inner, inner * rows};
-  cuuint32_t box[3] = {box_inner, box_rows, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = tmap_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(base), dims, strides, box, estr,
-                                    CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                    swizzle ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "tensor map of 8-bit outputs: code ", (int)r);
-  return m;
-}
 // [a | b] = x w^T rounded to `like`'s type, g = silu(a) b: the checkpoint (ck, or null), g along its rows and (g8t, or null) its
 // columns. 16-bit types: one launch, the activations stay on the chip; fp32 (whose values do not fit the registers): two.
 void product_swiglu(const Packed& x, const Packed& w, const at::Tensor& like, const Packed* ck, const Packed& g8,
@@ -598,17 +585,17 @@ void product_swiglu(const Packed& x, const Packed& w, const at::Tensor& like, co
   t.sa[0] = scales_map(x, 1);
   t.sb[0] = scales_map(w, 1);
   t.c[0] = t.a[0];
-  const CUtensorMap g8_map = bytes_map(g8.codes, H, M, 32, 32, true);
-  const CUtensorMap ck_map = ck != nullptr ? bytes_map(ck->codes, 2 * H, M, 32, 32, true) : g8_map;
-  const CUtensorMap g8t_map = g8t != nullptr ? bytes_map(g8t->codes, g8t->blocks() * 128, H, 32, 32, false) : g8_map;
   Gemm8SwigluOut o{};
   if (ck != nullptr) o.ck = ck->codes, o.ck_scales = ck->scales;
   o.g8 = g8.codes;
   o.g8_scales = g8.scales;
-  if (g8t != nullptr) o.g8t = g8t->codes, o.g8t_scales = g8t->scales;
-  o.ck_map = &ck_map;
-  o.g8_map = &g8_map;
-  o.g8t_map = &g8t_map;
+  CUtensorMap g8t_map;
+  if (g8t != nullptr) {
+    g8t_map = tile_map(g8t->codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g8t->blocks() * 128, H, g8t->blocks() * 128, 32);
+    o.g8t = g8t->codes;
+    o.g8t_scales = g8t->scales;
+    o.g8t_map = &g8t_map;
+  }
   BLOCK_LAUNCH(gemm8_swiglu_launch(t, p, o, at::cuda::getCurrentCUDAStream()), 1);
 }
 

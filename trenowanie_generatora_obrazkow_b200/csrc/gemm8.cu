@@ -37,10 +37,10 @@ struct Cfg {
   static constexpr int EPI_WARPS = SWIGLU ? 16 : 4, THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int A_BYTES = BM * BK, B_ROWS = PAIR ? BN / 2 : BN, B_BYTES = B_ROWS * BK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = SWIGLU ? 5 : STAGE_BYTES == 32768 ? 6 : 7;
+  static constexpr int STAGES = STAGE_BYTES == 32768 ? 6 : 7;
   static constexpr int B_ATOMS = (BN + 127) / 128;         // a tile of 192 begins at the start or the middle of an atom
   static constexpr int SF_BYTES = (1 + B_ATOMS) * ATOM;    // of a stage: A's atom, B's atoms
-  static constexpr int C_STAGE = SWIGLU ? 3072 : 4096;    // epilogue staging of one warp
+  static constexpr int C_STAGE = SWIGLU ? 1024 : 4096;    // epilogue staging of one warp
   static constexpr int MAXIMA = SWIGLU ? (4 * 3 + 4 + 1) * BM * 4 : 0;
   static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + ((STAGES * SF_BYTES + 1023) & ~1023) + EPI_WARPS * C_STAGE + MAXIMA;
   // Tensor memory (512 columns): two accumulators and the scale factors. Two of 256 columns leave no room, so they share
@@ -130,7 +130,7 @@ __device__ __forceinline__ void store_rows(const Gemm8Problem& q, long long at, 
 }
 
 struct Gemm8Swiglu {
-  CUtensorMap ck_map, g8_map, g8t_map;
+  CUtensorMap g8t_map;
   Side ck, g8, g8t;
 };
 
@@ -165,10 +165,11 @@ struct Schedule {
 // silu(a) b in fp32; they leave as 8-bit blocks alone: the checkpoint of a and b, g along its rows, g along its columns. A
 // tile is a block of both axes, so no other CTA is asked for a maximum. Sixteen warps: quarter (32 rows, a thread each) x strip
 // (32 columns), what two blocks' values and a third in fp32 leave room for in registers. The strips of a row meet in shared
-// memory, as do the quarters of a column, whose maximum over a warp's rows is one integer reduction. The codes leave by TMA
-// through 3 KB of staging a warp, which costs one of the loads' six stages. At 32768 x 2048 -> 2 x 5504 the launch takes 713 us,
-// 14.3 k cycles a tile, of which the epilogue fills 12.7 k (two exponential-unit operations and four conversions an element)
-// beside the next tile's products; product and activation apart took 555 + 331 us, and a and b crossed memory
+// memory, as do the quarters of a column, whose maximum over a warp's rows is one integer reduction. Codes of rows
+// leave from the registers, 32 bytes a store; those of columns through 1 KB of staging a warp, by TMA. (Through staging and TMA all
+// of them cost one of the loads' six stages: 713 us instead of 673.) At 32768 x 2048 -> 2 x 5504 the tensor core is busy for
+// about 60 % of the launch: the epilogue of a tile, two exponential-unit operations and four conversions an element, fills most
+// of the time that the next tile's products take. Product and activation apart took 555 + 331 us, and a and b crossed memory
 // twice (1.4 GB).
 struct SwigluShared {
   float rows[4][3][BM];  // [strip][a, b, g][row]
@@ -198,6 +199,10 @@ struct PairOf<__half> {
   }
   static __device__ __forceinline__ float2 get(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 };
+__device__ __forceinline__ void store32(uint8_t* p, const uint32_t (&w)[8]) {  // 32-byte aligned
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
 __device__ __forceinline__ float finite_or_nan(float v) { return fabsf(v) == INFINITY ? NAN : v; }
 // 16 pairs of a row: the largest finite magnitude; infinities become NaN
 template <typename S>
@@ -415,7 +420,7 @@ __global__ void __launch_bounds__((Cfg<BN, PAIR, S>::THREADS), 1)
   } else if constexpr (SWIGLU) {
     // ---------------- SwiGLU epilogue ----------------
     const int quarter = warp & 3, strip = (warp - 2) >> 2, r = quarter * 32 + lane;
-    uint8_t* const buf = smem_c + (warp - 2) * F::C_STAGE;  // 32 rows (of a, then of g; of b) and 32 columns of 32 bytes
+    uint8_t* const buf = smem_c + (warp - 2) * F::C_STAGE;  // 32 columns of 32 bytes
     SwigluShared& sh = *reinterpret_cast<SwigluShared*>(smem_c + F::EPI_WARPS * F::C_STAGE);
     const Gemm8Problem& q = p.q[0];
     const int nhb = q.N / 256, nmb = (q.M + 127) / 128;
@@ -466,38 +471,22 @@ __global__ void __launch_bounds__((Cfg<BN, PAIR, S>::THREADS), 1)
         return scale_inv(byte);
       };
       const int m0 = mb * BM + quarter * 32, h0 = hb * 128 + 32 * strip;
-      const bool rows_there = m0 < q.M;
-      auto send = [&](const CUtensorMap* map, uint8_t* from, int x, int y) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_3d(map, from, x, y, 0);
-          bulk_commit_group();
-        }
+      const bool row_there = mb * BM + r < q.M;
+      // a row's 32 codes of this strip: one sector, straight from the registers
+      auto put = [&](const Side& o, int col, const uint32_t(&w)[8]) {
+        if (row_there) store32(o.codes + (long long)(mb * BM + r) * o.width + col, w);
       };
-      // half i of a row's 32 bytes, in the 32-byte swizzle of the maps
-      auto half = [&](uint8_t* to, int i) { return reinterpret_cast<uint4*>(to + lane * 32 + ((i ^ ((lane >> 2) & 1)) << 4)); };
-      auto put_pairs = [&](uint8_t* to, const uint32_t(&u)[16], float inv) {
+      auto put_pairs = [&](int col, const uint32_t(&u)[16], float inv) {
         const float2 s = make_float2(inv, inv);
+        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t w[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-            w[n] = codes4(mul2(PairOf<S>::get(u[8 * i + 2 * n]), s), mul2(PairOf<S>::get(u[8 * i + 2 * n + 1]), s));
-          *half(to, i) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        for (int n = 0; n < 8; ++n) w[n] = codes4(mul2(PairOf<S>::get(u[2 * n]), s), mul2(PairOf<S>::get(u[2 * n + 1]), s));
+        put(sw.ck, col, w);
       };
-      if (lane == 0) bulk_wait_group_read<0>();
-      __syncwarp();
       if (sw.ck.codes != nullptr) {
         const float inv_a = row_scale(0, sw.ck, hb, 2 * nhb), inv_b = row_scale(1, sw.ck, nhb + hb, 2 * nhb);
-        if (rows_there) {
-          put_pairs(buf, pa, inv_a);
-          send(&sw.ck_map, buf, h0, m0);
-          put_pairs(buf + 1024, pb, inv_b);
-          send(&sw.ck_map, buf + 1024, q.N / 2 + h0, m0);
-        }
+        put_pairs(h0, pa, inv_a);
+        put_pairs(q.N / 2 + h0, pb, inv_b);
       }
       float g[32];
       float mg = 0.f;
@@ -538,7 +527,9 @@ __global__ void __launch_bounds__((Cfg<BN, PAIR, S>::THREADS), 1)
       }
       asm volatile("bar.sync 1, 512;" ::: "memory");  // the scales of g's columns are there
       if (sw.g8t.codes != nullptr && m0 < nmb * BM) {
-        uint8_t* to = buf + 2048 + lane;
+        if (lane == 0) bulk_wait_group_read<0>();
+        __syncwarp();
+        uint8_t* to = buf + lane;
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
           const float2 k = *reinterpret_cast<const float2*>(&sh.inv[32 * strip + j]);
@@ -546,27 +537,19 @@ __global__ void __launch_bounds__((Cfg<BN, PAIR, S>::THREADS), 1)
           to[j * 32] = (uint8_t)w;
           to[(j + 1) * 32] = (uint8_t)(w >> 8);
         }
-        send(&sw.g8t_map, buf + 2048, m0, h0);
-      }
-      if (rows_there) {
-        if (lane == 0) {  // a's codes are out of the buffer; those of b and of g's columns may not be
-          if (sw.g8t.codes != nullptr) bulk_wait_group_read<2>();
-          else bulk_wait_group_read<1>();
-        }
+        fence_proxy_async_smem();
         __syncwarp();
-        const float2 s = make_float2(inv_g, inv_g);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t w[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const float* v = &g[16 * i + 4 * n];
-            w[n] = codes4(mul2(make_float2(v[0], v[1]), s), mul2(make_float2(v[2], v[3]), s));
-          }
-          *half(buf, i) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (lane == 0) {
+          tma_store_3d(&sw.g8t_map, buf, m0, h0, 0);
+          bulk_commit_group();
         }
-        send(&sw.g8_map, buf, h0, m0);
       }
+      uint32_t w[8];
+      const float2 s = make_float2(inv_g, inv_g);
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+        w[n] = codes4(mul2(make_float2(g[4 * n], g[4 * n + 1]), s), mul2(make_float2(g[4 * n + 2], g[4 * n + 3]), s));
+      put(sw.g8, h0, w);
     }
     if (lane == 0) bulk_wait_group_all();
   } else {
@@ -675,7 +658,7 @@ template <int BN, bool PAIR, typename S = void>
 cudaError_t launch(const Gemm8Maps& t, Gemm8Params& p, const SwigluOf<S>& sw, Gemm8Tile tile, cudaStream_t s) {
   using F = Cfg<BN, PAIR, S>;
   auto kern = gemm8_kernel<BN, PAIR, S>;
-  static_assert(F::SMEM + 1024 <= 232448, "dynamic + static shared memory");
+  static_assert(F::SMEM + 256 <= 232448, "dynamic + static shared memory");
   static std::atomic<uint64_t> set{0};  // bit d: done on device d
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -747,15 +730,14 @@ cudaError_t gemm8_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8Tile tile, cuda
 }
 
 cudaError_t gemm8_swiglu_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8SwigluOut o, cudaStream_t s) {
-  if (!valid(p) || p.n != 1 || p.q[0].N % 256 != 0 || p.q[0].bias != nullptr || o.g8 == nullptr) return cudaErrorInvalidValue;
+  if (!valid(p) || p.n != 1 || p.q[0].N % 256 != 0 || p.q[0].bias != nullptr || o.g8 == nullptr ||
+      (o.g8t != nullptr && o.g8t_map == nullptr)) return cudaErrorInvalidValue;
   const int H = p.q[0].N / 2, M = p.q[0].M;
   Gemm8Swiglu sw{};
   sw.ck = side(o.ck, o.ck_scales, M, 2 * H);
   sw.g8 = side(o.g8, o.g8_scales, M, H);
   sw.g8t = side(o.g8t, o.g8t_scales, H, M);
-  sw.ck_map = *o.ck_map;
-  sw.g8_map = *o.g8_map;
-  sw.g8t_map = *o.g8t_map;
+  if (o.g8t != nullptr) sw.g8t_map = *o.g8t_map;
   if (p.q[0].elem == ELEM_BF16) return launch<256, true, __nv_bfloat16>(t, p, sw, TILE_PAIR_256, s);
   if (p.q[0].elem == ELEM_F16) return launch<256, true, __half>(t, p, sw, TILE_PAIR_256, s);
   return cudaErrorInvalidValue;
