@@ -457,6 +457,20 @@ def test_mlp_of_one_weight_twice(before):
     assert ((one.grad.double() - want).abs() <= tol * 1.001).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K,N", [(900, 5), (900, 40009), (1100, 20011), (2048, 4800), (4500, 2400)])
+@pytest.mark.parametrize("M", [1, 8, 9, 16])
+def test_few_rows_against_wide_weights(M, K, N, dtype):
+    """Every number of row groups of a CTA, one wave and several, a last CTA of fewer groups and rows."""
+    x, w = rnd(M, K, seed=1, dtype=dtype), rnd(N, K, seed=2, std=K ** -0.5)
+    qx, qw, bias = held(x), held(w), torch.randn(N, device=DEV)
+    want = qx @ qw.t()
+    got = B8.linear_blocks(x, B8.quantize_blocks(w), bias)
+    # the bias joins in fp32: half a step of that sum, and of the output's type
+    more = (want + bias.double()).abs() * 2.0 ** -23 + bias.double().abs() * torch.finfo(dtype).eps
+    assert_within(got, want + bias.double(), product_tol(qx, qw, dtype, want + bias.double()) + more)
+
+
 # ----------------------------------------------------------------------------------------------------- streams, graphs
 def test_captured_and_replayed():
     lin = torch.nn.Linear(256, 384, device=DEV)

@@ -834,13 +834,13 @@ cudaError_t swiglu_bwd_typed(const Swiglu8BwdParams& p, cudaStream_t s) {
 
 // --------------------------------------------------------------------------------------------------------- few rows
 // y [M, N] = Q(x) W^T + bias for at most 16 rows of x (tokens of a serving step), in one launch: x is packed where it is used.
-// Reading W bounds it (N Kp bytes). A CTA owns 16 RT rows of W, each of up to 8 warps every eighth block of 128; a warp's loads
-// of a block are 16 bytes per lane and independent. e4m3 values are fp16 values, so the products run on mma.m16n8k16 (W rows
-// x tokens) with fp32 sums, after one conversion of two codes each; the order of k inside a block is free, so a lane's 16
+// Reading W bounds it (N Kp bytes) once it is large. e4m3 values are fp16 values, so the products run on mma.m16n8k16 (W rows x
+// tokens) with fp32 sums, after one conversion of two codes each; the order of k inside a block is free, so a lane's 16
 // consecutive bytes serve as its operands of four instructions, for W and for x alike. A block's sum is scaled in fp32, the
 // warps' sums are added in order.
-// One token 2048 -> 6144 (12.6 MB, 1.9 us at the copy rate): 5.3 us, of which a launch takes about 2; 6.0 with 4 warps, 6.6 with
-// 16 (two waves), 5.7 with the 8-bit form of the instruction.
+// W cold in L2: one token 2048 -> 6144 (12.6 MB, 1.9 us at the copy rate) 6.9 us, 2048 -> 11008 8.4, 5504 -> 2048 7.9, 4 tokens
+// 5504 -> 11008 18.6, 16 tokens 2048 -> 6144 9.5. A CTA of eight warps for each 32 rows, loads a block at a time: 7.5, 11.1,
+// 10.0, 26.0, 14.3 (x packed more often, half-filled second waves).
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   asm volatile(
@@ -854,39 +854,67 @@ __device__ __forceinline__ void halves(uint32_t codes, uint32_t& lo, uint32_t& h
       : "=r"(lo), "=r"(hi) : "r"(codes));
 }
 
-constexpr int FEW_WARPS = 8;
-template <typename T, int NT, int RT>  // NT: groups of eight rows of x
-__global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_kernel(const FewRowsParams p, bool vec) {
-  __shared__ float part[FEW_WARPS][16 * RT][8 * NT + 1];
+// A CTA owns a few groups of 16 rows of W, each of its warps some of the blocks of 128 along K: the warp packs x's part of a block
+// once and multiplies it with that block of each group. A ring in shared memory holds up to FEW_SLOTS - 1 of these pieces on
+// their way; each lane reads back what it asked for itself, and adds to sums that it alone keeps there, so no thread waits for
+// another before the last product.
+constexpr int FEW_SLOTS = 4, FEW_GROUPS = 8;  // groups of a CTA: at most this, half of it for more than eight rows of x
+struct FewSlot {
+  uint4 w[2][2][32];         // [row g + 8 r][half of the block][lane]
+  uint32_t scales[2][32];    // of four blocks, this one among them
+};
+__device__ __forceinline__ void cp_async16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+// bytes of shared memory of a warp
+__host__ __device__ constexpr int few_ring() { return FEW_SLOTS * (int)sizeof(FewSlot); }
+__host__ __device__ constexpr int few_sums(int groups, int nt) { return groups * nt * 32 * 16; }
+
+template <typename T, int NT, int WARPS>  // NT: groups of eight rows of x; WARPS: at most
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 2 : 1) few_rows_kernel(const FewRowsParams p, int groups, bool vec) {
+  extern __shared__ __align__(16) uint8_t raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int warps = blockDim.x >> 5;
+  FewSlot* const ring = reinterpret_cast<FewSlot*>(raw + warp * few_ring());
+  uint8_t* const all_sums = raw + warps * few_ring();
+  float4* const sums = reinterpret_cast<float4*>(all_sums + warp * few_sums(groups, NT)) + lane;  // [group][NT][lane]
   const int nb = (p.K + TILE - 1) / TILE, quads = (nb + 3) / 4;
   const long long width = (long long)nb * TILE;
-  const int n0 = blockIdx.x * 16 * RT;
+  const int n0 = blockIdx.x * 16 * groups, mine = min(groups, (p.N - n0 + 15) / 16);
   const T* x = static_cast<const T*>(p.x);
-  float acc[RT][NT][4];
+  for (int i = 0; i < groups * NT; ++i) sums[i * 32] = make_float4(0.f, 0.f, 0.f, 0.f);
+  int next_kb = warp, next = 0;  // the next piece that is asked for
+  auto fetch = [&](int slot) {
+    if (next_kb < nb) {
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int i = 0; i < NT; ++i) acc[r][i][0] = acc[r][i][1] = acc[r][i][2] = acc[r][i][3] = 0.f;
-  for (int kb = warp; kb < nb; kb += warps) {
-    uint4 w[2 * RT][2];  // [row g + 8 r][half of the block]
-    float ws[2 * RT];
-#pragma unroll
-    for (int r = 0; r < 2 * RT; ++r) {
-      const int n = min(n0 + g + 8 * r, p.N - 1);  // rows past the last: not written
-      const uint8_t* src = p.codes + n * width + kb * TILE + 16 * t;
-      w[r][0] = __ldg(reinterpret_cast<const uint4*>(src));
-      w[r][1] = __ldg(reinterpret_cast<const uint4*>(src + 64));
-      ws[r] = scale_of(__ldg(p.scales + scale_at(n, kb, quads)));
+      for (int r = 0; r < 2; ++r) {
+        const int n = min(n0 + 16 * next + g + 8 * r, p.N - 1);  // rows past the last: not written
+        const uint8_t* src = p.codes + n * width + next_kb * TILE + 16 * t;
+        cp_async16(&ring[slot].w[r][0][lane], src);
+        cp_async16(&ring[slot].w[r][1][lane], src + 64);
+        cp_async4(&ring[slot].scales[r][lane], p.scales + scale_at(n, next_kb & ~3, quads));
+      }
+      if (++next == mine) {
+        next = 0;
+        next_kb += warps;
+      }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int s = 0; s < FEW_SLOTS - 1; ++s) fetch(s);
+  int slot = 0;
+  for (int kb = warp; kb < nb; kb += warps) {
+    uint2 b[NT][2][4];    // x in fp16 values of its codes: [half of the block][instruction]
+    float s0[NT], s1[NT];  // scales of tokens 2 t and 2 t + 1
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int m = 8 * i + g;
       Eight<T> f[4];  // columns 16 t .. + 15 and 64 + 16 t .. + 15 of the block
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        const int c = kb * TILE + (h >> 1) * 64 + 16 * t + (h & 1) * 8;
+        const int c = kb * TILE + (h >> 1) * 64 + 16 * t + (h & 1) * 8, m = 8 * i + g;
         f[h].load(x + m * p.ldx + c, m < p.M ? max(0, min(8, p.K - c)) : 0, vec);
       }
       float tops[4];
@@ -896,73 +924,95 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_rows_kernel(const FewRowsP
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int byte = scale_byte(top);
       const float inv = scale_inv(byte);
-      float d[RT][4] = {};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint2 lo = codes8(f[2 * h], inv), hi = codes8(f[2 * h + 1], inv);
+        halves(lo.x, b[i][h][0].x, b[i][h][0].y);
+        halves(lo.y, b[i][h][1].x, b[i][h][1].y);
+        halves(hi.x, b[i][h][2].x, b[i][h][2].y);
+        halves(hi.y, b[i][h][3].x, b[i][h][3].y);
+      }
+      const float s = scale_of(byte);
+      s0[i] = __shfl_sync(0xffffffffu, s, 8 * t);
+      s1[i] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+    }
+#pragma unroll 1
+    for (int r = 0; r < mine; ++r) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(FEW_SLOTS - 2) : "memory");
+      fetch(slot == 0 ? FEW_SLOTS - 1 : slot - 1);  // into the slot whose values the last products have taken
+      const FewSlot& from = ring[slot];
+      slot = slot + 1 == FEW_SLOTS ? 0 : slot + 1;
+      const float w0 = scale_of((from.scales[0][lane] >> (8 * (kb & 3))) & 0xff);
+      const float w1 = scale_of((from.scales[1][lane] >> (8 * (kb & 3))) & 0xff);
+      float d[NT][4] = {};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 u = from.w[0][h][lane], v = from.w[1][h][lane];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          uint32_t b0, b1;
-          halves(q == 0 ? lo.x : q == 1 ? lo.y : q == 2 ? hi.x : hi.y, b0, b1);
+          uint32_t a0, a1, a2, a3;
+          halves(q == 0 ? u.x : q == 1 ? u.y : q == 2 ? u.z : u.w, a0, a2);
+          halves(q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w, a1, a3);
 #pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const uint4 &u = w[2 * r][h], &v = w[2 * r + 1][h];
-            uint32_t a0, a1, a2, a3;
-            halves(q == 0 ? u.x : q == 1 ? u.y : q == 2 ? u.z : u.w, a0, a2);
-            halves(q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w, a1, a3);
-            mma_f16(d[r], a0, a1, a2, a3, b0, b1);
-          }
+          for (int i = 0; i < NT; ++i) mma_f16(d[i], a0, a1, a2, a3, b[i][h][q].x, b[i][h][q].y);
         }
       }
-      // d: rows g, g + 8 of W, tokens 2 t, 2 t + 1, whose scales their own lanes hold
-      const float s = scale_of(byte);
-      const float s0 = __shfl_sync(0xffffffffu, s, 8 * t), s1 = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+      // d: rows g, g + 8 of W, tokens 2 t, 2 t + 1. The scales are powers of two: their product is exact, and out of range only
+      // where the result is
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        // powers of two: their product is exact, and out of range only where the result is
-        acc[r][i][0] += d[r][0] * (s0 * ws[2 * r]);
-        acc[r][i][1] += d[r][1] * (s1 * ws[2 * r]);
-        acc[r][i][2] += d[r][2] * (s0 * ws[2 * r + 1]);
-        acc[r][i][3] += d[r][3] * (s1 * ws[2 * r + 1]);
+      for (int i = 0; i < NT; ++i) {
+        float4 a = sums[(r * NT + i) * 32];
+        a.x += d[i][0] * (s0[i] * w0);
+        a.y += d[i][1] * (s1[i] * w0);
+        a.z += d[i][2] * (s0[i] * w1);
+        a.w += d[i][3] * (s1[i] * w1);
+        sums[(r * NT + i) * 32] = a;
       }
     }
   }
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      part[warp][16 * r + g][8 * i + 2 * t] = acc[r][i][0];
-      part[warp][16 * r + g][8 * i + 2 * t + 1] = acc[r][i][1];
-      part[warp][16 * r + g + 8][8 * i + 2 * t] = acc[r][i][2];
-      part[warp][16 * r + g + 8][8 * i + 2 * t + 1] = acc[r][i][3];
-    }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
+  // the warps' sums in order
   T* y = static_cast<T*>(p.y);
-  for (int at = threadIdx.x; at < 16 * RT * p.M; at += blockDim.x) {
-    const int m = at / (16 * RT), r = at % (16 * RT), n = n0 + r;
+  const float* part = reinterpret_cast<const float*>(all_sums);
+  for (int at = threadIdx.x; at < 16 * mine * p.M; at += blockDim.x) {
+    const int m = at / (16 * mine), rest = at % (16 * mine), n = n0 + rest;
     if (n >= p.N) continue;
+    // row rest % 16 = g or g + 8, token m % 8 = 2 t or 2 t + 1
+    const int row = rest & 15, l = (row & 7) * 4 + ((m & 7) >> 1), e = (row >> 3) * 2 + (m & 1);
+    const float* q = part + (((rest >> 4) * NT + (m >> 3)) * 32 + l) * 4 + e;
     float v = 0.f;
-    for (int k = 0; k < warps; ++k) v += part[k][r][m];
+    for (int k = 0; k < warps; ++k) v += q[k * (few_sums(groups, NT) / 4)];
     if (p.bias != nullptr) v += p.bias[n];
     y[(long long)m * p.N + n] = from_f<T>(v);
   }
 }
 
-template <typename T>
-cudaError_t few_rows_typed(const FewRowsParams& p, int sms, cudaStream_t s) {
-  const int nb = (p.K + TILE - 1) / TILE, threads = std::min(FEW_WARPS, nb) * 32;
-  const bool vec = p.K % 8 == 0 && aligned16(p.x, p.ldx * (long long)sizeof(T));
-  // 32 rows of W share a packed x where they still fill the GPU
-  if ((p.N + 31) / 32 >= sms) {
-    const int grid = (p.N + 31) / 32;
-    if (p.M <= 8) few_rows_kernel<T, 1, 2><<<grid, threads, 0, s>>>(p, vec);
-    else few_rows_kernel<T, 2, 2><<<grid, threads, 0, s>>>(p, vec);
-  } else {
-    const int grid = (p.N + 15) / 16;
-    if (p.M <= 8) few_rows_kernel<T, 1, 1><<<grid, threads, 0, s>>>(p, vec);
-    else few_rows_kernel<T, 2, 1><<<grid, threads, 0, s>>>(p, vec);
+template <typename T, int NT, int WARPS>
+cudaError_t few_rows(const FewRowsParams& p, int groups, bool vec, cudaStream_t s) {
+  static std::atomic<uint64_t> set{0};
+  auto kern = few_rows_kernel<T, NT, WARPS>;
+  const int warps = std::min(WARPS, (p.K + TILE - 1) / TILE);
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev > 63 || !((set.load(std::memory_order_relaxed) >> dev) & 1))) {  // once per device
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * (few_ring() + few_sums(FEW_GROUPS / NT, NT)));
+    if (e == cudaSuccess && dev <= 63) set.fetch_or(1ull << dev);
   }
+  if (e != cudaSuccess) return e;
+  const int grid = (p.N + 16 * groups - 1) / (16 * groups);
+  kern<<<grid, 32 * warps, warps * (few_ring() + few_sums(groups, NT)), s>>>(p, groups, vec);
   return cudaGetLastError();
+}
+template <typename T, int NT>
+cudaError_t few_rows_typed(const FewRowsParams& p, int sms, cudaStream_t s) {
+  const bool vec = p.K % 8 == 0 && aligned16(p.x, p.ldx * (long long)sizeof(T));
+  const int all = (p.N + 15) / 16;
+  // equal waves, one as far as shared memory goes: of CTAs of sixteen warps, one per SM, or, where rows have at most eight blocks,
+  // of eight, two per SM
+  const int slots = p.K > 8 * TILE ? sms : 2 * sms, waves = (all + slots * (FEW_GROUPS / NT) - 1) / (slots * (FEW_GROUPS / NT));
+  const int groups = (all + slots * waves - 1) / (slots * waves);
+  return p.K > 8 * TILE ? few_rows<T, NT, 16>(p, groups, vec, s) : few_rows<T, NT, 8>(p, groups, vec, s);
 }
 
 template <typename F>
@@ -1018,7 +1068,9 @@ cudaError_t unpack8_launch(const uint8_t* codes, const uint8_t* scales, int R, i
 }
 cudaError_t few_rows_launch(const FewRowsParams& p, int elem, cudaStream_t s) {
   if (p.M <= 0 || p.M > kFewRows || p.N <= 0 || p.K <= 0) return cudaErrorInvalidValue;
-  return by_type(elem, [&](auto t) { return few_rows_typed<decltype(t)>(p, num_sms(), s); });
+  return by_type(elem, [&](auto t) {
+    return p.M <= 8 ? few_rows_typed<decltype(t), 1>(p, num_sms(), s) : few_rows_typed<decltype(t), 2>(p, num_sms(), s);
+  });
 }
 cudaError_t swiglu8_fwd_launch(const Swiglu8Params& p, int elem, cudaStream_t s) {
   if (p.M <= 0 || p.H <= 0 || (p.g == nullptr) == (p.g8 == nullptr) || (p.g8t != nullptr && p.g8 == nullptr))
