@@ -471,6 +471,35 @@ def test_few_rows_against_wide_weights(M, K, N, dtype):
     assert_within(got, want + bias.double(), product_tol(qx, qw, dtype, want + bias.double()) + more)
 
 
+def test_more_than_2_31_values():
+    """Offsets past 31 bits: the last rows and columns of a matrix of 2.16e9 values are those of the slices by themselves."""
+    M, K = 33024, 65536
+    x = torch.randn(M, K, device=DEV, dtype=torch.bfloat16, generator=torch.Generator(device=DEV).manual_seed(1))
+    r, c = B8.quantize_blocks(x, "both")
+    tail, right = B8.quantize_blocks(x[-128:]), B8.quantize_blocks(x[:, -128:], "cols")
+    assert torch.equal(r.codes[-128:].view(torch.uint8), tail.codes.view(torch.uint8)) and torch.equal(r.scales[-1:], tail.scales)
+    assert torch.equal(c.codes[-128:].view(torch.uint8), right.codes.view(torch.uint8)) and torch.equal(c.scales[-1:], right.scales)
+    assert torch.equal(B8.dequantize_blocks(r)[-128:], B8.dequantize_blocks(tail))
+    v = x[:1].clone()
+    assert torch.equal(B8.linear_blocks(v, r)[:, -128:], B8.linear_blocks(v, tail))
+    few = B8.quantize_blocks(x[:64])
+    want = held(x[-128:]) @ held(x[:64]).t()
+    assert_within(B8.gemm_blocks(r, few)[-128:], want, product_tol(held(x[-128:]), held(x[:64]), torch.bfloat16, want))
+    assert_within(B8.gemm_blocks(few, r)[:, -128:], want.t(), product_tol(held(x[:64]), held(x[-128:]), torch.bfloat16, want.t()))
+    out = torch.empty(M, K, device=DEV, dtype=torch.bfloat16)  # an output of as many values
+    a, b = B8.quantize_blocks(x[:, :128].contiguous()), B8.quantize_blocks(x[:1, :].view(K // 128, 128).repeat(128, 1))
+    B8.gemm_blocks(a, b, out=out)
+    want = held(x[-128:, :128]) @ held(x[:1].view(K // 128, 128)).t()
+    tol = product_tol(held(x[-128:, :128]), held(x[:1].view(K // 128, 128)), torch.bfloat16, want)
+    assert_within(out[-128:, -K // 128:], want, tol)
+    del out, r, c
+    ab, dg = x.requires_grad_(), torch.ones(M, K // 2, device=DEV, dtype=torch.bfloat16)
+    end = x.detach()[-128:].clone().requires_grad_()
+    g, h = B8.swiglu_blocks(ab), B8.swiglu_blocks(end)
+    g.backward(dg), h.backward(dg[-128:])
+    assert torch.equal(g[-128:], h) and torch.equal(ab.grad[-128:], end.grad)
+
+
 # ----------------------------------------------------------------------------------------------------- streams, graphs
 def test_captured_and_replayed():
     lin = torch.nn.Linear(256, 384, device=DEV)
@@ -496,6 +525,42 @@ def test_captured_and_replayed():
     want = train_linear(new_x, lin.weight, lin.bias, new_dy)
     assert torch.equal(y.detach(), want[0])
     assert all(torch.equal(a, b) for a, b in zip(got, want[1:]))
+
+
+@pytest.mark.parametrize("op", ["mlp", "swiglu", "few", "many"])
+def test_two_graphs_of_the_other_operators(op):
+    """Two captured graphs, replayed in turn and on other inputs, give what eager calls give."""
+    w1, w2 = rnd(512, 192, seed=1, std=192 ** -0.5, dtype=torch.float32), rnd(160, 256, seed=2, std=1 / 16, dtype=torch.float32)
+    held_w = B8.quantize_blocks(w1), B8.quantize_blocks(w2)
+
+    def run(x):
+        if op == "few" or op == "many":
+            with torch.no_grad():
+                return [B8.mlp_blocks(x, *held_w), B8.linear_blocks(x, held_w[0])]
+        leaves = [x] + [w.detach().requires_grad_() for w in ((w1, w2) if op == "mlp" else ())]
+        y = B8.mlp_blocks(*leaves) if op == "mlp" else B8.swiglu_blocks(x)
+        y.backward(y.detach())
+        return [y.detach()] + [t.grad for t in leaves]
+    rows = 9 if op == "few" else 300
+    xs = [rnd(rows, 192, seed=k).requires_grad_(op in ("mlp", "swiglu")) for k in (3, 4)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(xs[0].detach().clone().requires_grad_(xs[0].requires_grad))
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, got = [], []
+    for x in xs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(run(x))
+    with torch.no_grad():
+        for k, x in enumerate(xs):
+            x.copy_(rnd(rows, 192, seed=5 + k))
+    for k in (0, 1, 0):
+        graphs[k].replay()
+    for x, g in zip(xs, got):
+        want = run(x.detach().clone().requires_grad_(x.requires_grad))
+        assert len(want) == len(g) and all(torch.equal(a, b) for a, b in zip(g, want))
 
 
 def test_other_stream():
