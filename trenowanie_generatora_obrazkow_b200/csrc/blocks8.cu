@@ -506,8 +506,8 @@ __global__ void __launch_bounds__(256) swiglu8_bwd_kernel(const T* __restrict__ 
   }
 }
 
-// ---- the forms of the MLP: everything that is written is in 8 bits, both ways where a weight's gradient wants it (the forward
-// of 16-bit types has them in its product's epilogue but for few rows, which want g along the rows alone). One CTA of
+// ---- the forms of the MLP: everything that is written is in 8 bits, both ways where a weight's gradient wants it (the
+// forward of 16-bit types has them in its product's epilogue but for few rows, which want g along the rows alone). One CTA of
 // 512 threads per SM walks over tiles of 128 x 128; the tiles come by TMA, two ahead of the arithmetic (fp32: one), so no
 // registers and no address arithmetic go into loads. A thread holds 8 columns of 4 rows; the backward holds da and db at once
 // and takes each exponential once. What bounds them is the arithmetic: some 25 and 30 instructions an element.
