@@ -836,10 +836,11 @@ cudaError_t swiglu_bwd_typed(const Swiglu8BwdParams& p, cudaStream_t s) {
 // y [M, N] = Q(x) W^T + bias for at most 16 rows of x (tokens of a serving step), in one launch: x is packed where it is used.
 // Reading W bounds it (N Kp bytes) once it is large. e4m3 values are fp16 values, so the products run on mma.m16n8k16 (W rows x
 // tokens) with fp32 sums, after one conversion of two codes each; the order of k inside a block is free, so a lane's 16
-// consecutive bytes serve as its operands of four instructions, for W and for x alike. A block's sum is scaled in fp32, the
-// warps' sums are added in order.
+// consecutive bytes serve as its operands of four instructions, for W and for x alike. A block's sum d is scaled in fp32, by two
+// factors of about half the exponent each (scale_halves): the product of both scales may leave fp32's range where the sum's
+// place in y does not, as the largest values of x's and W's blocks need not meet. The warps' sums are added in order.
 // W cold in L2: one token 2048 -> 6144 (12.6 MB, 1.9 us at the copy rate) 6.9 us, 2048 -> 11008 8.4, 5504 -> 2048 7.9, 4 tokens
-// 5504 -> 11008 18.6, 16 tokens 2048 -> 6144 9.5. A CTA of eight warps for each 32 rows, loads a block at a time: 7.5, 11.1,
+// 5504 -> 11008 18.9, 16 tokens 2048 -> 6144 9.6. A CTA of eight warps for each 32 rows, loads a block at a time: 7.5, 11.1,
 // 10.0, 26.0, 14.3 (x packed more often, half-filled second waves).
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -908,7 +909,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 2 : 1) few_rows_kerne
   int slot = 0;
   for (int kb = warp; kb < nb; kb += warps) {
     uint2 b[NT][2][4];    // x in fp16 values of its codes: [half of the block][instruction]
-    float s0[NT], s1[NT];  // scales of tokens 2 t and 2 t + 1
+    float2 s0[NT], s1[NT];  // scales of tokens 2 t and 2 t + 1, as two factors
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       Eight<T> f[4];  // columns 16 t .. + 15 and 64 + 16 t .. + 15 of the block
@@ -932,9 +933,8 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 2 : 1) few_rows_kerne
         halves(hi.x, b[i][h][2].x, b[i][h][2].y);
         halves(hi.y, b[i][h][3].x, b[i][h][3].y);
       }
-      const float s = scale_of(byte);
-      s0[i] = __shfl_sync(0xffffffffu, s, 8 * t);
-      s1[i] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+      s0[i] = scale_halves(__shfl_sync(0xffffffffu, byte, 8 * t));
+      s1[i] = scale_halves(__shfl_sync(0xffffffffu, byte, 8 * t + 4));
     }
 #pragma unroll 1
     for (int r = 0; r < mine; ++r) {
@@ -942,8 +942,8 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 2 : 1) few_rows_kerne
       fetch(slot == 0 ? FEW_SLOTS - 1 : slot - 1);  // into the slot whose values the last products have taken
       const FewSlot& from = ring[slot];
       slot = slot + 1 == FEW_SLOTS ? 0 : slot + 1;
-      const float w0 = scale_of((from.scales[0][lane] >> (8 * (kb & 3))) & 0xff);
-      const float w1 = scale_of((from.scales[1][lane] >> (8 * (kb & 3))) & 0xff);
+      const float2 w0 = scale_halves((from.scales[0][lane] >> (8 * (kb & 3))) & 0xff);
+      const float2 w1 = scale_halves((from.scales[1][lane] >> (8 * (kb & 3))) & 0xff);
       float d[NT][4] = {};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -957,15 +957,15 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 2 : 1) few_rows_kerne
           for (int i = 0; i < NT; ++i) mma_f16(d[i], a0, a1, a2, a3, b[i][h][q].x, b[i][h][q].y);
         }
       }
-      // d: rows g, g + 8 of W, tokens 2 t, 2 t + 1. The scales are powers of two: their product is exact, and out of range only
-      // where the result is
+      // d: rows g, g + 8 of W, tokens 2 t, 2 t + 1
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
+        const float2 x0 = mul2(s0[i], w0), x1 = mul2(s1[i], w0), x2 = mul2(s0[i], w1), x3 = mul2(s1[i], w1);
         float4 a = sums[(r * NT + i) * 32];
-        a.x += d[i][0] * (s0[i] * w0);
-        a.y += d[i][1] * (s1[i] * w0);
-        a.z += d[i][2] * (s0[i] * w1);
-        a.w += d[i][3] * (s1[i] * w1);
+        a.x = fmaf(d[i][0] * x0.x, x0.y, a.x);
+        a.y = fmaf(d[i][1] * x1.x, x1.y, a.y);
+        a.z = fmaf(d[i][2] * x2.x, x2.y, a.z);
+        a.w = fmaf(d[i][3] * x3.x, x3.y, a.w);
         sums[(r * NT + i) * 32] = a;
       }
     }

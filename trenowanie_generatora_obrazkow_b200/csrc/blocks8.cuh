@@ -16,6 +16,12 @@ __device__ __forceinline__ float scale_inv(int byte) { return __uint_as_float((u
 __device__ __forceinline__ float scale_of(int byte) {                                                          // 2^e
   return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u);
 }
+// 2^e = x y with x = 2^floor(e / 2) or half of it, y = 2 or 4 x. d (x x') (y y') of two scales has no step that leaves fp32's range
+// upwards unless the result does (both factors are at least 1, or the first is less), nor downwards unless the result is less
+// than 2^-149 (|d| < 2^25 and x x' < 2^-108).
+__device__ __forceinline__ float2 scale_halves(int byte) {
+  return make_float2(__uint_as_float((uint32_t)((byte >> 1) + 63) << 23), __uint_as_float((uint32_t)((byte + 1 >> 1) + 64) << 23));
+}
 // offset of the scale byte of row r and block b; quads: atoms of a row tile, ceil(blocks / 4)
 __device__ __forceinline__ long long scale_at(int r, int b, int quads) {
   return ((long long)(r >> 7) * quads + (b >> 2)) * ATOM + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);

@@ -80,8 +80,8 @@ struct Gemm8SwigluOut {
 cudaError_t gemm8_swiglu_launch(const Gemm8Maps& t, Gemm8Params p, Gemm8SwigluOut o, cudaStream_t s);
 
 // y [M, N] = Q(x) W^T + bias for few rows, x packed on the way (one launch). Sixteen rows, W cold, against packing and product
-// apart: 2048 -> 6144 9.3 us (3.1 + 11.2), 5504 -> 2048 11.0 (3.0 + 18.7), 1280 -> 3456 6.4 (2.8 + 8.9), 640 -> 1920 4.3 (3.0 + 7.1),
-// 5504 -> 11008 32.6 (3.1 + 25.7).
+// apart: 2048 -> 6144 9.6 us (3.1 + 11.2), 5504 -> 2048 11.0 (3.0 + 18.7), 1280 -> 3456 6.4 (2.8 + 8.9), 640 -> 1920 4.3 (3.0 + 7.1),
+// 5504 -> 11008 32.9 (3.1 + 25.7).
 constexpr int kFewRows = 16;
 struct FewRowsParams {
   const void* x;            // [M, K], rows ldx apart
