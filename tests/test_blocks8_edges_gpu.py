@@ -1,7 +1,9 @@
-"""8-bit block operators at their edges on the GPU: scales far out."""
+"""8-bit block operators at their edges on the GPU: scales far out, blocks without a finite value."""
+import math
+
 import pytest
 import torch
-from test_blocks8_gpu import held
+from test_blocks8_gpu import TYPES, held, rnd
 
 from trenowanie_generatora_obrazkow_b200.ops import blocks8 as B8
 from trenowanie_generatora_obrazkow_b200.ops._ext import check_errors
@@ -46,3 +48,17 @@ def test_scales_whose_product_is_too_small(M, dtype, e):
     got = B8.linear_blocks(x, B8.quantize_blocks(w))
     want = torch.tensor([49 * 2.0 ** (18 + e), 0.0, 49 * 2.0 ** (18 + e)], device=DEV, dtype=torch.float64).to(dtype)
     assert torch.equal(got, want.expand(M, 3))
+
+
+# ------------------------------------------------------------------------------------------------- no finite value at all
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scale_bytes_of_blocks_without_a_finite_value(dtype):
+    x = rnd(300, 400, dtype=dtype, seed=3)
+    x[1, 128:256], x[2], x[3, 256:] = math.nan, -math.inf, math.inf
+    x[128:256, 7], x[:, 9], x[256:, 11] = math.nan, math.inf, -math.inf
+    x[4, 0:128:2], x[4, 1:128:2] = math.nan, math.inf
+    want = B8.quantize_blocks(x.cpu(), "both")
+    for got in (B8.quantize_blocks(x, "both"), (B8.quantize_blocks(x), B8.quantize_blocks(x, "cols"))):
+        for a, b in zip(got, want):
+            assert torch.equal(a.scales.cpu(), b.scales)
+            assert torch.equal(a.codes.cpu().view(torch.uint8) & 0x7f, b.codes.view(torch.uint8) & 0x7f)

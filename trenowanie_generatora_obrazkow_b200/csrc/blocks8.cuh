@@ -10,8 +10,11 @@ constexpr int TILE = 128;
 constexpr int ATOM = 512;
 
 // ---------------------------------------------------------------------------------------------------------- scales
-// With u the bits of A: the carry out of the mantissa's top bits is the step from m <= 1.75 to m > 1.75.
-__device__ __forceinline__ int scale_byte(float amax) { return max(0, (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8); }
+// With u the bits of A: the carry out of the mantissa's top bits is the step from m <= 1.75 to m > 1.75. A block without a finite
+// value has A = 0, which maxima that pass over NaN may show as NaN.
+__device__ __forceinline__ int scale_byte(float amax) {
+  return max(0, (int)((__float_as_uint(fmaxf(amax, 0.f)) + 0x1fffffu) >> 23) - 8);
+}
 __device__ __forceinline__ float scale_inv(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }  // 2^-e
 __device__ __forceinline__ float scale_of(int byte) {                                                          // 2^e
   return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u);
