@@ -1,4 +1,5 @@
-"""8-bit block operators at their edges on the GPU: scales far out, blocks without a finite value."""
+"""8-bit block operators at their edges on the GPU: scales far out, blocks without a finite value, weights that are frozen or
+released between forward and backward."""
 import math
 
 import pytest
@@ -62,3 +63,54 @@ def test_scale_bytes_of_blocks_without_a_finite_value(dtype):
         for a, b in zip(got, want):
             assert torch.equal(a.scales.cpu(), b.scales)
             assert torch.equal(a.codes.cpu().view(torch.uint8) & 0x7f, b.codes.view(torch.uint8) & 0x7f)
+
+
+# ---------------------------------------------------------------------------- weights frozen or released in between
+@pytest.mark.parametrize("op", ["linear", "mlp"])
+@pytest.mark.parametrize("late", [(1,), (2,), (1, 2)])
+@pytest.mark.parametrize("x_too", [False, True])
+def test_weights_released_after_the_forward_get_no_gradient(op, late, x_too):
+    """As everywhere in autograd, a tensor without requires_grad in the forward is not part of the graph."""
+    def tensors():
+        x, w = rnd(70, 128, seed=1), rnd(256, 128, seed=2, std=1 / 11, dtype=torch.float32)
+        return [x, w, rnd(256, seed=3, dtype=torch.float32) if op == "linear" else rnd(72, 128, seed=3, std=1 / 11, dtype=torch.float32)]
+    fn = B8.linear_blocks if op == "linear" else B8.mlp_blocks
+    dy = rnd(70, 256 if op == "linear" else 72, seed=4)
+
+    def run(release):
+        ts = tensors()
+        for i, t in enumerate(ts):
+            t.requires_grad_(x_too if i == 0 else i not in late)
+        y = fn(*ts)
+        if not y.requires_grad:
+            return None
+        if release:
+            for i in late:
+                ts[i].requires_grad_()
+        y.backward(dy)
+        return [t.grad for t in ts]
+    want, got = run(False), run(True)
+    if want is None:
+        assert late == (1, 2) and not x_too
+        return
+    for a, b in zip(got, want):
+        assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+    assert all(got[i] is None for i in late)
+
+
+@pytest.mark.parametrize("op", ["linear", "mlp"])
+@pytest.mark.parametrize("late", [(1,), (2,), (1, 2)])
+def test_weights_frozen_after_the_forward_get_no_gradient(op, late):
+    x, w = rnd(70, 128, seed=1), rnd(256, 128, seed=2, std=1 / 11, dtype=torch.float32)
+    v = rnd(256, seed=3, dtype=torch.float32) if op == "linear" else rnd(72, 128, seed=3, std=1 / 11, dtype=torch.float32)
+    fn = B8.linear_blocks if op == "linear" else B8.mlp_blocks
+    dy = rnd(70, 256 if op == "linear" else 72, seed=4)
+    full = [t.clone().requires_grad_() for t in (x, w, v)]
+    fn(*full).backward(dy)
+    ts = [t.clone().requires_grad_() for t in (x, w, v)]
+    y = fn(*ts)
+    for i in late:
+        ts[i].requires_grad_(False)
+    y.backward(dy)
+    for i, (a, b) in enumerate(zip(ts, full)):
+        assert a.grad is None if i in late else torch.equal(a.grad, b.grad)

@@ -417,8 +417,10 @@ struct Linear8Fn : public torch::autograd::Function<Linear8Fn> {
     const at::Tensor b32 = bias_f32(bias);
     product(xr, wr, y, ptr_f32(b32), false, err_word(err, x));
     ctx->save_for_backward({checkpoint});
-    ctx->saved_data["w"] = w;
-    if (given(bias)) ctx->saved_data["bias"] = *bias;
+    // a weight or bias that is no part of the graph now gets no gradient, whatever its flag is when the backward runs
+    if (dw) ctx->saved_data["w"] = w;
+    if (given(bias) && bias->requires_grad()) ctx->saved_data["bias"] = *bias;
+    ctx->saved_data["K"] = K;
     ctx->saved_data["err"] = err;
     ctx->saved_data["of"] = (dx ? 1 : 0) + (dw ? 2 : 0);
     return y;
@@ -433,7 +435,7 @@ struct Linear8Fn : public torch::autograd::Function<Linear8Fn> {
     const at::Tensor err = ctx->saved_data["err"].toTensor();
     int* const e = err_word(err, dy);
     const WeightGrad gw(ctx, "w"), gb(ctx, "bias");
-    const int64_t K = ctx->saved_data["w"].toTensor().size(1);
+    const int64_t K = ctx->saved_data["K"].toInt();
     Packed xt, wt, r, c;
     Arena before, now;
     if (of & 2) before.add(&xt, K, M);
@@ -670,8 +672,10 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
     at::Tensor y = fresh({M, N}, x.scalar_type(), x);
     product(g8, w2r, y, nullptr, false, e);
     ctx->save_for_backward({checkpoint});
-    ctx->saved_data["w1"] = w1;
-    ctx->saved_data["w2"] = w2;
+    if (of & 2) ctx->saved_data["w1"] = w1;  // as in Linear8Fn
+    if (of & 4) ctx->saved_data["w2"] = w2;
+    ctx->saved_data["K"] = K;
+    ctx->saved_data["H"] = H;
     ctx->saved_data["err"] = err;
     ctx->saved_data["of"] = of;
     return y;
@@ -682,8 +686,7 @@ struct Mlp8Fn : public torch::autograd::Function<Mlp8Fn> {
     const at::Tensor dy = rows_of(grads[0]);
     const c10::cuda::CUDAGuard guard(dy.device());
     const int64_t of = ctx->saved_data["of"].toInt();
-    const int64_t M = dy.size(0), N = dy.size(1), H = ctx->saved_data["w2"].toTensor().size(1),
-                  K = ctx->saved_data["w1"].toTensor().size(1);
+    const int64_t M = dy.size(0), N = dy.size(1), H = ctx->saved_data["H"].toInt(), K = ctx->saved_data["K"].toInt();
     const at::Tensor err = ctx->saved_data["err"].toTensor();
     int* const e = err_word(err, dy);
     const WeightGrad g1(ctx, "w1"), g2(ctx, "w2");
