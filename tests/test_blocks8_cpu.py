@@ -118,3 +118,16 @@ def test_serving_form_and_refusals():
     leaf = x.clone().requires_grad_()
     with pytest.raises(RuntimeError):
         torch.autograd.grad(torch.autograd.grad(B8.linear_blocks(leaf, w).sum(), leaf, create_graph=True)[0].sum(), leaf)
+
+
+def test_swiglu_of_sigmoids_below_the_range_of_fp32():
+    a = torch.tensor([-63.5, -64.5, -88.0, -96.0, -120.0, -160.0, -20.0, 0.0, 88.0]).repeat(15)[:128].expand(4, 128)
+    ab = torch.cat([a, torch.full((4, 128), 2.0 ** 118)], dim=1)
+    leaf = ab.clone().requires_grad_()
+    B8.swiglu_blocks(leaf).backward(torch.full((4, 128), 16.0))
+    a, b = (torch.stack([slow_held(r) for r in v]) for v in ab.chunk(2, dim=1))  # what the backward reads
+    s = torch.sigmoid(a)
+    low = 2.0 ** -126
+    assert torch.allclose(leaf.grad.double(), 16 * torch.cat([b * s * (1 + a * (1 - s)), a * s], dim=1), rtol=1e-5, atol=low)
+    a, b = ab.double().chunk(2, dim=1)
+    assert torch.allclose(B8.swiglu_blocks(ab).double(), a * torch.sigmoid(a) * b, rtol=1e-5, atol=low)

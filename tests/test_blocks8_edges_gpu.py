@@ -1,10 +1,11 @@
-"""8-bit block operators at their edges on the GPU: scales far out, blocks without a finite value, weights that are frozen or
-released between forward and backward."""
+"""8-bit block operators at their edges on the GPU: scales far out, sigmoids far out, blocks without a finite value, weights
+that are frozen or released between forward and backward."""
 import math
 
 import pytest
+import test_blocks8_gpu as plain
 import torch
-from test_blocks8_gpu import TYPES, held, rnd
+from test_blocks8_gpu import HALF, TYPES, held, rnd
 
 from trenowanie_generatora_obrazkow_b200.ops import blocks8 as B8
 from trenowanie_generatora_obrazkow_b200.ops._ext import check_errors
@@ -63,6 +64,67 @@ def test_scale_bytes_of_blocks_without_a_finite_value(dtype):
         for a, b in zip(got, want):
             assert torch.equal(a.scales.cpu(), b.scales)
             assert torch.equal(a.codes.cpu().view(torch.uint8) & 0x7f, b.codes.view(torch.uint8) & 0x7f)
+
+
+# ----------------------------------------------------------------------------------------------------------- far sigmoids
+FAR = [-88.0, -96.0, -104.0, -120.0, -144.0, -160.0, -80.0, 0.0, -1.0, -20.0, 88.0, 160.0]
+
+
+def far_activations(dtype):
+    """[256, 256]: a [256, 128], the first six of FAR in the rows of the first tile, all of them in those of the second, and b =
+    +-2^k with k falling along the columns. 8 bits hold each value, along the rows and along the columns."""
+    m = torch.arange(256, device=DEV)
+    a = torch.tensor(FAR, device=DEV)[torch.where(m < 128, m % 6, m % 12)][:, None].expand(256, 128)
+    k = torch.arange(128, device=DEV) % 8
+    return torch.cat([a, torch.exp2(118.0 - k) * (1 - 2 * (m % 2))[:, None]], 1).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+def test_swiglu_of_sigmoids_below_the_range_of_fp32(dtype):
+    """a down to -160 with b large enough for results in range. exp(-160) is 0 in fp32."""
+    ab = far_activations(dtype).requires_grad_()
+    assert all(torch.equal(held(v), v.double()) for v in (ab.detach()[:, :128], ab.detach()[:, 128:], ab.detach().t()))
+    dg = torch.full((256, 128), 2.0 ** 4, device=DEV, dtype=dtype)
+    g = B8.swiglu_blocks(ab)
+    g.backward(dg)
+    # exp(a / 2) from an argument rounded to 2^-24 of itself (|a| / 2 < 80: 2^-17.7) and two units in the last place, squared
+    fine = 2.0 ** -16
+    low = 2.0 ** -126  # below it bits go
+    want, d = plain.swiglu64(ab.detach()), plain.swiglu_grad64(ab.detach(), dg)
+    plain.assert_within(g, want, want.abs() * (HALF[dtype] + fine) + low)
+    a, b = ab.detach().double().chunk(2, 1)
+    s = torch.sigmoid(a)
+    parts = torch.cat([dg.double() * b * s * (1 + a.abs()), dg.double() * a * s], 1).abs()  # 1 + a (1 - s) may cancel
+    plain.assert_within(ab.grad, d, d.abs() * HALF[dtype] + parts * fine + low)
+    assert (want.abs() > 2.0 ** -60).double().mean() > 0.5
+
+
+def in_8_bits(got, want, dim):
+    """got are the held values of `want` up to 2^-14 of it: half a step of e4m3 or of the block's smallest step."""
+    w = want if dim == 1 else want.t()
+    top = w.abs().view(w.shape[0], -1, 128).amax(-1, keepdim=True).expand(-1, -1, 128).reshape(w.shape)
+    tol = torch.maximum(w.abs() * 2.0 ** -4, top / 224 * 2.0 ** -10) * (1 + 2.0 ** -8)
+    plain.assert_within(got, want, (tol if dim == 1 else tol.t()) + 2.0 ** -126)
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("held_w", [False, True])
+def test_mlp_of_sigmoids_below_the_range_of_fp32(dtype, held_w):
+    """x and W2 the identity: y is g in 8 bits, dW1 the gradient of [a | b] in 8 bits."""
+    ab, eye = far_activations(torch.float32), torch.eye(256, device=DEV)
+    x, w1, w2 = eye.to(dtype), ab.t().contiguous(), torch.eye(128, device=DEV)
+    want = plain.swiglu64(ab)
+    if held_w:
+        for rows in (256, 9):
+            y = B8.mlp_blocks(x[:rows], B8.quantize_blocks(w1), B8.quantize_blocks(w2))
+            in_8_bits(y.double(), want[:rows], 1)
+        return
+    leaves = [t.requires_grad_() for t in (x, w1, w2)]
+    dy = torch.full((256, 128), 2.0 ** 4, device=DEV, dtype=dtype)
+    y = B8.mlp_blocks(*leaves)
+    y.backward(dy)
+    in_8_bits(y.detach().double(), want, 1)
+    in_8_bits(leaves[1].grad.double().t(), plain.swiglu_grad64(ab, dy), 0)
 
 
 # ---------------------------------------------------------------------------- weights frozen or released in between

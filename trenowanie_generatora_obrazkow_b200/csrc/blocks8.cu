@@ -414,7 +414,7 @@ cudaError_t unpack_typed(const uint8_t* codes, const uint8_t* scales, int R, int
 
 // ----------------------------------------------------------------------------------------------------------- SwiGLU
 // g in ab's type, the checkpoint of ab in 8 bits. Rows alone: a thread holds 8 columns of ROW_R rows (two: enough warps to keep
-// the memory busy; at 32768 x 5504 the backward took 265 us with four, 212 with two). The checkpoint's blocks are those of a
+// the memory busy; at 32768 x 5504 the backward took 265 us with four, 212 with two, and 220 with sigmoids in two factors). The checkpoint's blocks are those of a
 // [M, 2 Hp] matrix: a's first, then b's. Rows past the last are read as the last one and not written.
 constexpr int ROW_R = 2;
 template <typename T, bool VEC, bool CK>
@@ -435,10 +435,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4)
   for (int i = 0; i < ROW_R; ++i) {
     Eight<T> o;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float2 x = a[i].pair(w), y = b[i].pair(w);
-      o.set(w, make_float2(x.x * sigmoid<sizeof(T) == 4>(x.x) * y.x, x.y * sigmoid<sizeof(T) == 4>(x.y) * y.y));
-    }
+    for (int w = 0; w < 4; ++w) o.set(w, swiglu<sizeof(T) == 4>(a[i].pair(w), b[i].pair(w)));
     if (r0 + i < M) o.store(g + (long long)(r0 + i) * H + c, n, vec_g);
   }
   if constexpr (CK) {
@@ -459,11 +456,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4)
 // dg, Q(a), Q(b) -> [da | db] in dg's type: da = dg b s (1 + a (1 - s)), db = dg a s with s = sigmoid(a)
 template <bool FINE>
 __device__ __forceinline__ void swiglu_grad(float2 a, float2 b, float2 dg, float2& da, float2& db) {
-  const float2 s = make_float2(sigmoid<FINE>(a.x), sigmoid<FINE>(a.y));
-  const float2 t = mul2(dg, s);
-  const float2 u = make_float2(fmaf(a.x, 1.f - s.x, 1.f), fmaf(a.y, 1.f - s.y, 1.f));
-  da = mul2(mul2(t, b), u);
-  db = mul2(t, a);
+  float2 p, q;
+  sigmoid<FINE>(a, p, q);
+  const float2 one = make_float2(1.f, 1.f), u = fma2(a, fma2(make_float2(-p.x, -p.y), q, one), one), t = mul2(dg, p);
+  da = mul2(mul2(t, mul2(b, q)), u);
+  db = mul2(t, mul2(a, q));
 }
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) swiglu8_bwd_kernel(const T* __restrict__ dg, long long ld, int M, int H, bool vec_d,
@@ -635,10 +632,7 @@ __global__ void __launch_bounds__(QT_THREADS, 1)
 #pragma unroll
     for (int i = 0; i < QT_R; ++i)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float2 x = a[i].pair(w);
-        v[i].set(w, mul2(mul2(x, make_float2(sigmoid<sizeof(T) == 4>(x.x), sigmoid<sizeof(T) == 4>(x.y))), b[i].pair(w)));
-      }
+      for (int w = 0; w < 4; ++w) v[i].set(w, swiglu<sizeof(T) == 4>(a[i].pair(w), b[i].pair(w)));
     if constexpr (CK) {
       qt_rows(a, ck, r0, hb, 2 * nhb, l16);
       qt_rows(b, ck, r0, nhb + hb, 2 * nhb, l16);

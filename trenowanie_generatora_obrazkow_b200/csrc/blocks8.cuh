@@ -1,4 +1,4 @@
-// Device helpers of the 8-bit block kernels (blocks8.cu, gemm8.cu): scales, conversions, the sigmoid, an output's place.
+// Device helpers of the 8-bit block kernels (blocks8.cu, gemm8.cu): scales, conversions, silu(a) b, an output's place.
 #pragma once
 #include <cuda_fp8.h>
 #include <stdint.h>
@@ -35,6 +35,13 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       "mov.b64 {%0, %1}, x;\n}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
 __device__ __forceinline__ uint32_t codes2(float a, float b) {  // a in the low byte
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(a), "f"(b));
@@ -54,19 +61,38 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // passes ov
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-
-// s = 1 / (1 + exp(-a)). For 16-bit types exp2 and the reciprocal are the hardware's approximations (an argument rounded to
-// 2^-24 of itself and two units in the last place), which the result's rounding hides; fp32 results take the library's.
+// s = 1 / (1 + exp(-a)) = p q. s leaves fp32's range below a = -87 while products of it may be far inside: with h = exp(min(a, 0) /
+// 2), p = h / (1 + exp(-|a|)) and q = h each operand of a product takes a factor and they stay there, x s y = (x p) (y q).
+// For 16-bit types exp2 and the reciprocal are the hardware's approximations: s is off by (1.25 |a| + 16) 2^-24 of itself at most
+// and taken as 0 below a = -174 (s < 2^-251). A result that is rounded to 16 bits hides that; one that goes to 8 bits from
+// fp32 takes the neighbouring code where it lies as near as that to a border, one in 2^-4 / 2^-20 = 2^16. fp32 takes the
+// library's, and s whole into p where that is in range (h squared is off by twice as much).
 template <bool FINE>
-__device__ __forceinline__ float sigmoid(float a) {
-  if constexpr (FINE) {
-    return 1.f / (1.f + expf(-a));
-  } else {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return r;
-  }
+__device__ __forceinline__ void sigmoid(float2 a, float2& p, float2& q) {
+  auto one = [](float v, float& x, float& y) {
+    if constexpr (FINE) {
+      const float e = expf(-fabsf(v));
+      y = 1.f;
+      if (v < -64.f) y = expf(0.5f * v);
+      x = (v >= 0.f ? 1.f : v < -64.f ? y : e) / (1.f + e);
+    } else {
+      float h, r;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(fabsf(v) * (-0.5f * 1.4426950408889634f)));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.f)));
+      y = v >= 0.f ? 1.f : h;
+      x = r;
+    }
+  };
+  one(a.x, p.x, q.x);
+  one(a.y, p.y, q.y);
+  if constexpr (!FINE) p = mul2(p, q);
+}
+// silu(a) b
+template <bool FINE>
+__device__ __forceinline__ float2 swiglu(float2 a, float2 b) {
+  float2 p, q;
+  sigmoid<FINE>(a, p, q);
+  return mul2(mul2(a, p), mul2(b, q));
 }
 
 struct Side {             // one 8-bit output

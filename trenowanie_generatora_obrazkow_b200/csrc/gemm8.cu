@@ -493,8 +493,7 @@ __global__ void __launch_bounds__((Cfg<BN, PAIR, S>::THREADS), 1)
       float mg = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const float2 a = PairOf<S>::get(pa[j]);
-        const float2 v = mul2(mul2(a, make_float2(sigmoid<false>(a.x), sigmoid<false>(a.y))), PairOf<S>::get(pb[j]));
+        const float2 v = swiglu<false>(PairOf<S>::get(pa[j]), PairOf<S>::get(pb[j]));
         g[2 * j] = v.x;
         g[2 * j + 1] = v.y;
         mg = max3(mg, fabsf(v.x), fabsf(v.y));

@@ -312,15 +312,24 @@ class LinearBlocks(torch.autograd.Function):
         return dx, dw, None if ctx.types[1] is None else dy.float().sum(0).to(ctx.types[1])
 
 
+def _far(a):
+    """Where a sigmoid leaves fp32's range or nears that (a < -64: it is exp(a) there), and exp(a / 2): a factor for each side of
+    a product, which may be far inside."""
+    return a < -64, torch.exp(a.clamp(max=0) / 2)
+
+
 def swiglu_f32(ab):
     a, b = ab.float().chunk(2, dim=-1)
-    return torch.nn.functional.silu(a) * b
+    far, h = _far(a)
+    return torch.where(far, (a * h) * (b * h), torch.nn.functional.silu(a) * b)
 
 
 def swiglu_grad_f32(ab, dg):
     a, b = ab.float().chunk(2, dim=-1)
     dg, s = dg.float(), torch.sigmoid(a)
-    return torch.cat([dg * b * s * (1 + a * (1 - s)), dg * a * s], dim=-1)
+    far, h = _far(a)
+    da = torch.where(far, (dg * h) * (b * h) * (1 + a), dg * b * s * (1 + a * (1 - s)))
+    return torch.cat([da, torch.where(far, (dg * h) * (a * h), dg * a * s)], dim=-1)
 
 
 class SwigluBlocks(torch.autograd.Function):
