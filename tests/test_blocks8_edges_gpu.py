@@ -1,11 +1,11 @@
-"""8-bit block operators at their edges on the GPU: scales far out, sigmoids far out, blocks without a finite value, weights
-that are frozen or released between forward and backward."""
+"""8-bit block operators at their edges on the GPU: scales and sigmoids far out, blocks without a finite value, weights that are
+frozen or released between forward and backward, sizes that give every unit several tiles."""
 import math
 
 import pytest
 import test_blocks8_gpu as plain
 import torch
-from test_blocks8_gpu import HALF, TYPES, held, rnd
+from test_blocks8_gpu import HALF, TYPES, held, held_t, rnd
 
 from trenowanie_generatora_obrazkow_b200.ops import blocks8 as B8
 from trenowanie_generatora_obrazkow_b200.ops._ext import check_errors
@@ -176,3 +176,37 @@ def test_weights_frozen_after_the_forward_get_no_gradient(op, late):
     y.backward(dy)
     for i, (a, b) in enumerate(zip(ts, full)):
         assert a.grad is None if i in late else torch.equal(a.grad, b.grad)
+
+
+# -------------------------------------------------------------------------------------------------- several tiles a unit
+@pytest.mark.parametrize("dtype", TYPES)
+def test_mlp_of_several_tiles_a_unit(dtype):
+    """17 x 22 tiles of 256 x 128 for 74 pairs of CTAs and 34 x 22 of 128 x 128 for 148 SMs, an odd last row: every unit's
+    accumulators, stages, maxima and staging are used again. Row by row and column by column."""
+    M, K, H, N = 4301, 192, 2816, 160
+    x, w1, w2 = rnd(M, K, seed=1, dtype=dtype), rnd(2 * H, K, seed=2, std=K ** -0.5, dtype=torch.float32, spread=0), \
+        rnd(N, H, seed=3, std=H ** -0.5, dtype=torch.float32, spread=0)
+    dy = rnd(M, N, seed=4, std=0.1, dtype=dtype)
+
+    def run(rows, wants=(1, 1, 1)):
+        leaves = [t.detach().clone().requires_grad_(bool(k)) for t, k in zip((x[rows], w1, w2), wants)]
+        y = B8.mlp_blocks(*leaves)
+        y.backward(dy[rows])
+        return [y.detach()] + [t.grad for t in leaves]
+    got = run(slice(None))
+    # rows of y and dx are their own sums, whatever is computed beside them
+    for lo, hi in ((0, 640), (1024, 2176), (4096, M), (4224, M)):
+        part = run(slice(lo, hi))
+        assert torch.equal(got[0][lo:hi], part[0]) and torch.equal(got[1][lo:hi], part[1])
+    # with and without the checkpoint, g along its columns, or weights that are packed in the call
+    for wants in ((1, 0, 0), (0, 1, 0), (0, 0, 1)):
+        for a, b in zip(run(slice(None), wants), got):
+            assert a is None or torch.equal(a, b)
+    assert torch.equal(got[0], B8.mlp_blocks(x, w1, w2))
+    assert torch.equal(got[0], B8.mlp_blocks(x, B8.quantize_blocks(w1), B8.quantize_blocks(w2)))
+    # Of the 160 to 5632 values that a row's or a column's results sum over, fewer than 2^-5 fall on the other side of a border
+    # of their 8 bits (2^-7 at most of all, and chance), by 2^-3 of themselves: 2^-3 2^-2.5 in the 2-norm, and a rounding
+    for g, w in zip(got, plain.mlp64(x, w1, w2, dy, dtype)):
+        for dim in (0, 1):
+            off = (g.double() - w).norm(dim=dim) / w.norm(dim=dim)
+            assert off.max().item() < 2.0 ** -5.5 + HALF[dtype], (tuple(g.shape), dim, off.argmax().item(), off.max().item())
