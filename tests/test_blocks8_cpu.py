@@ -131,3 +131,19 @@ def test_swiglu_of_sigmoids_below_the_range_of_fp32():
     assert torch.allclose(leaf.grad.double(), 16 * torch.cat([b * s * (1 + a * (1 - s)), a * s], dim=1), rtol=1e-5, atol=low)
     a, b = ab.double().chunk(2, dim=1)
     assert torch.allclose(B8.swiglu_blocks(ab).double(), a * torch.sigmoid(a) * b, rtol=1e-5, atol=low)
+
+
+def test_no_rows():
+    r, c = B8.quantize_blocks(torch.empty(0, 300), "both")
+    assert r.shape == (0, 300) and c.shape == (300, 0)
+    assert B8.dequantize_blocks(r).shape == (0, 300) and B8.dequantize_blocks(c).shape == (300, 0)
+    w, b, w1, w2 = (torch.randn(s).requires_grad_() for s in ((12, 300), (12,), (256, 300), (8, 128)))
+    for fn, ws, n in ((B8.linear_blocks, (w, b), 12), (B8.mlp_blocks, (w1, w2), 8)):
+        x = torch.empty(2, 0, 300, requires_grad=True)
+        y = fn(x, *ws)
+        y.sum().backward()
+        assert y.shape == (2, 0, n) and x.grad.shape == x.shape and all((t.grad == 0).all() for t in ws)
+    ab = torch.empty(0, 256, requires_grad=True)
+    B8.swiglu_blocks(ab).sum().backward()
+    assert ab.grad.shape == (0, 256)
+    assert B8.linear_blocks(torch.empty(0, 300), B8.quantize_blocks(w.detach())).shape == (0, 12)

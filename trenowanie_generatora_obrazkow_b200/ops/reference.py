@@ -270,15 +270,16 @@ def quantize_blocks(x):
     """x [M, K] -> (codes e4m3 [M, Kp], scales uint8 [ceil(M / 128), ceil(Kp / 512), 32, 4, 4]): see ops/blocks8.py."""
     M, K = x.shape
     nb, rt = -(-K // 128), -(-M // 128)
+    quads = -(-nb // 4)
     f = torch.nn.functional.pad(x.detach().float(), (0, nb * 128 - K)).view(M, nb, 128)
     finite = f.isfinite()
     top = torch.where(finite, f.abs(), 0.0).amax(-1)
     m, e = torch.frexp(top)  # top = m 2^e, 1/2 <= m < 1; 448 = 7/8 2^9
     e = torch.where(top > 0, torch.where(m <= 0.875, e - 9, e - 8).clamp_min(-127), -127)
     q = torch.where(finite, torch.ldexp(f, -e[..., None]), math.nan).to(torch.float8_e4m3fn)
-    scales = torch.zeros(rt * 128, -(-nb // 4) * 4, dtype=torch.uint8, device=x.device)
+    scales = torch.zeros(rt * 128, quads * 4, dtype=torch.uint8, device=x.device)
     scales[:M, :nb] = (e + 127).to(torch.uint8)
-    return q.view(M, nb * 128), scales.view(rt, 4, 32, -1, 4).permute(0, 3, 2, 1, 4).contiguous()
+    return q.view(M, nb * 128), scales.view(rt, 4, 32, quads, 4).permute(0, 3, 2, 1, 4).contiguous()
 
 
 def dequantize_blocks(codes, scales, cols):
@@ -286,7 +287,7 @@ def dequantize_blocks(codes, scales, cols):
     M, width = codes.shape
     rt, quads = scales.shape[:2]
     e = scales.permute(0, 3, 2, 1, 4).reshape(rt * 128, quads * 4)[:M, :width // 128].int() - 127
-    return torch.ldexp(codes.float().view(M, -1, 128), e[..., None]).view(M, width)[:, :cols]
+    return torch.ldexp(codes.float().view(M, width // 128, 128), e[..., None]).view(M, width)[:, :cols]
 
 
 def in_blocks(x):
