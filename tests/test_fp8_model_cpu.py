@@ -106,6 +106,19 @@ def test_block_linear():
     m.load_state_dict(state)
 
 
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.type(torch.float32),
+                                  lambda m: m.to("cpu", torch.float32), lambda m: m.to("meta").to_empty(device="cpu")])
+def test_block_linear_keeps_its_codes_when_a_module_is_cast(cast):
+    m = quantize(torch.nn.Sequential(torch.nn.Linear(130, 64)), "fp8_block")
+    x, codes, scales = torch.randn(3, 130), m[0].w.clone(), m[0].s.clone()
+    state = {k: v.clone() for k, v in m.state_dict().items()}
+    assert cast(m) is m and m[0].w.dtype == torch.float8_e4m3fn and m[0].s.dtype == torch.uint8
+    if not all(p.device.type == "cpu" and torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in ((m[0].w, codes), (m[0].s, scales))):
+        m.load_state_dict(state)  # emptied on the way
+    x, bias = x.to(m[0].bias.dtype if m[0].bias.dtype != torch.float64 else torch.float32), m[0].bias.detach()
+    assert torch.equal(m[0](x), B8.linear_blocks(x, B8.Blocks8(codes, scales, 130), bias))
+
+
 @pytest.mark.parametrize("flags", [["--fp8"], ["--act-checkpoint", "fp8"], ["--fp8", "--act-checkpoint", "fp8"]])
 def test_train_command(tmp_path, flags):
     r = subprocess.run([sys.executable, "train.py", "--synthetic", "16", "--out", str(tmp_path / "run"), "--size", "nano",

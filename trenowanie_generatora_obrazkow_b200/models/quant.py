@@ -95,6 +95,13 @@ class BlockLinear(nn.Module):
         self.bias = lin.bias
         self.in_features, self.out_features = lin.in_features, lin.out_features
 
+    def _apply(self, fn, recurse=True):
+        """Codes and scale bytes move, but are no numbers to convert (``module.to(torch.bfloat16)``)."""
+        held = self.w, self.s
+        super()._apply(fn, recurse)
+        self.w, self.s = (new if new.dtype == old.dtype else old.to(new.device) for new, old in zip((self.w, self.s), held))
+        return self
+
     @torch.no_grad()
     def forward(self, x):
         return B8.linear_blocks(x, B8.Blocks8(self.w, self.s, self.in_features), self.bias)
