@@ -119,6 +119,47 @@ def test_block_linear_keeps_its_codes_when_a_module_is_cast(cast):
     assert torch.equal(m[0](x), B8.linear_blocks(x, B8.Blocks8(codes, scales, 130), bias))
 
 
+@pytest.mark.parametrize("kind", ["int8", "fp8", "w8a8", "fp8_block"])
+@pytest.mark.parametrize("model", ["dit", "moe", "routed"])
+def test_quantized_models(kind, model):
+    """The framework's own models with every layer but the routers quantized."""
+    from trenowanie_generatora_obrazkow_b200.models.moe import moe_denoiser
+    from trenowanie_generatora_obrazkow_b200.models.routed import RoutedConfig, RoutedDenoiser
+    g = torch.Generator().manual_seed(1)
+    if model == "routed":
+        torch.manual_seed(0)
+        nets = [RoutedDenoiser(RoutedConfig(latent_channels=8, dim=128, depth=2, heads=2, kv_heads=2, axes=(16, 24, 24), text_dim=64,
+                                            experts=8, top_k=2, expert_hidden=128, groups=2, top_groups=1))]
+        z, t, text = torch.randn(2, 8, 2, 4, 4, generator=g), torch.rand(2, generator=g), torch.randn(2, 5, 64, generator=g)
+        run = lambda: nets[0](z, t, text)  # noqa: E731
+    else:
+        nets = _model()
+        if model == "moe":
+            moe_denoiser(nets[1], 4, 2, 128)
+        x, t, st = torch.randn(2, 128, 4, 4, generator=g), torch.rand(2, generator=g), torch.randn(2, 16, 64, generator=g)
+
+        def run():
+            text, valid = nets[0](lm_states=st)
+            return nets[1](x, t, text, valid)
+    with torch.no_grad():
+        plain = run()
+        for net in nets:
+            quantize(net, kind)
+            linears = [n for n, m in net.named_modules() if type(m) is torch.nn.Linear]
+            assert all(n.endswith(".router") for n in linears) and (model == "dit" or net is not nets[-1] or linears)
+        # a value's error is at most 2^-4 of it (less for the kinds of finer steps); products of many add up like noise
+        assert 0 < ((run() - plain).norm() / plain.norm()).item() < 0.1
+
+
+def test_quantized_blocks_are_the_marked_blocks():
+    g = torch.Generator().manual_seed(1)
+    x, t, text = torch.randn(2, 128, 4, 4, generator=g), torch.rand(2, generator=g), torch.randn(2, 9, 128, generator=g)
+    marked, held = _model()[1], _model()[1]
+    use_fp8(marked), quantize(held.blocks, "fp8_block")
+    with torch.no_grad():
+        assert torch.equal(marked(x, t, text), held(x, t, text))
+
+
 @pytest.mark.parametrize("flags", [["--fp8"], ["--act-checkpoint", "fp8"], ["--fp8", "--act-checkpoint", "fp8"]])
 def test_train_command(tmp_path, flags):
     r = subprocess.run([sys.executable, "train.py", "--synthetic", "16", "--out", str(tmp_path / "run"), "--size", "nano",

@@ -168,6 +168,34 @@ def test_block_linear_and_marked_layers():
     assert torch.equal(quantize(m, "fp8_block")(x), marked)
 
 
+@pytest.mark.parametrize("kind", ["int8", "fp8", "w8a8", "fp8_block"])
+def test_quantized_dit(kind):
+    from trenowanie_generatora_obrazkow_b200.models.quant import quantize, use_fp8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(4, 128, 16, 16, device="cuda", generator=g)
+    t = torch.rand(4, device="cuda", generator=g)
+    st = torch.randn(4, 32, 256, device="cuda", generator=g).bfloat16()
+
+    def run(te, den):
+        text, valid = te(lm_states=st)
+        return den(x, t, text, valid).float()
+    with torch.no_grad():
+        te, den = _model()
+        plain = run(te, den)
+        if kind == "fp8_block":
+            use_fp8(te), use_fp8(den)
+            marked = run(te, den)
+            te, den = _model()
+            quantize(te.blocks, kind), quantize(den.blocks, kind)
+            # the same products but for g, which is rounded to bf16 before it is packed: one value in 2^-9 / 2^-4 = 2^5 takes its
+            # neighbour, 2^-4 of it on average, 1.1 % of a branch's norm in each of two blocks
+            assert ((run(te, den) - marked).norm() / marked.norm()).item() < 0.023
+            te, den = _model()
+        quantize(te, kind), quantize(den, kind)  # time_mlp and ada take the form of few rows
+        assert 0 < ((run(te, den) - plain).norm() / plain.norm()).item() < 0.1
+    check_errors("cuda")
+
+
 @pytest.mark.parametrize("M", [3, 40])
 def test_far_scales(M):
     """Large activations against small weights: the product is in range, and so is the result."""

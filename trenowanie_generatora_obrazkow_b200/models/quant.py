@@ -12,7 +12,8 @@ framework's own blocks.
 * ``BlockLinear``: e4m3 weights with a power-of-two scale for each 128 inputs, activations packed the same way in the call
   (``ops.blocks8``): one launch for up to 16 rows, the block-scaled tcgen05 product above. No gradient.
 * ``quantize(module, kind)``: replaces every ``nn.Linear`` below ``module`` in place (kind "int8", "fp8", "fp8_block" or
-  "w8a8"; w8a8 only where both feature counts are multiples of 8, as the int8 GEMM requires).
+  "w8a8"; w8a8 only where both feature counts are multiples of 8, as the int8 GEMM requires) but the routers of experts,
+  whose scores are computed from their weights in fp32. Plain modules, and this framework's own models for inference.
 * ``use_fp8(module)``: the linear layers of every DiT and text block below ``module`` run on 8-bit products, in training
   forward and backward (fp32 master weights and gradients, ``ops.blocks8.linear_blocks`` / ``mlp_blocks``), without
   gradients with weights packed once per version. Parameters and checkpoints keep their names and types.
@@ -119,8 +120,12 @@ def use_fp8(module: nn.Module, on: bool = True) -> nn.Module:
 
 
 def quantize(module: nn.Module, kind: str) -> nn.Module:
+    from .moe import MoEMLP
+    from .routed import RoutedMLP
     for name, child in list(module.named_children()):
         if isinstance(child, nn.Linear):
+            if name == "router" and isinstance(module, (MoEMLP, RoutedMLP)):
+                continue
             if kind == "fp8_block":
                 setattr(module, name, BlockLinear(child))
             elif kind == "w8a8":

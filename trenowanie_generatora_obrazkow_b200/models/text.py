@@ -175,11 +175,11 @@ class LMTextEncoder(nn.Module):
         _, h = Fz.adanorm(h.contiguous(), None, None, self.in_norm.weight)
         if is_null is not None:
             h = torch.where(is_null.to(h.device)[:, None, None], self.null.to(h.dtype).expand_as(h), h)
-        if isinstance(self.in_proj, nn.Linear):
+        if not isinstance(self.in_proj, nn.Identity):  # also a quantized layer
             h = Fz.linear(h, self.in_proj)
         cos, sin = self.rope(L, h.device)
         h = _run_blocks(self.blocks, h, lens, cos, sin, self.norm, self.checkpoint_blocks)
-        if isinstance(self.out_proj, nn.Linear):
+        if not isinstance(self.out_proj, nn.Identity):
             h = Fz.linear(h, self.out_proj)
         return h, valid
 

@@ -108,8 +108,10 @@ def mlp_fp8(x, in_proj, out_proj):
 
 
 def up_swiglu(x, layer):
-    """silu(x Wg^T) * (x Wu^T) for an nn.Linear of (2H, D) gate | up rows. On CUDA without autograd (sampling) and
-    H % 128 == 0: one GEMM whose epilogue applies the SwiGLU (the (M, 2H) product never reaches memory)."""
+    """silu(x Wg^T) * (x Wu^T) for an nn.Linear (or a quantized layer) of (2H, D) gate | up rows. On CUDA without autograd
+    (sampling) and H % 128 == 0: one GEMM whose epilogue applies the SwiGLU (the (M, 2H) product never reaches memory)."""
+    if not isinstance(layer, torch.nn.Linear):
+        return swiglu(linear(x, layer))
     w = layer.weight
     H = w.shape[0] // 2
     if x.is_cuda and not marked_fp8(layer) and not (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)) and H % 128 == 0:
@@ -341,13 +343,16 @@ class _LinearFn(torch.autograd.Function):
 
 
 def linear(x, layer_or_weight, bias=None):
-    """y = x @ W^T (+ b). Accepts an ``nn.Linear`` (its weight and bias) or a weight tensor."""
+    """y = x @ W^T (+ b). Accepts an ``nn.Linear`` (its weight and bias), a weight tensor or a quantized layer
+    (``models.quant.quantize``), which is called."""
     if isinstance(layer_or_weight, torch.nn.Linear):
         weight, bias = layer_or_weight.weight, layer_or_weight.bias
         if marked_fp8(layer_or_weight):
             if x.is_cuda and x.dtype != torch.bfloat16:
                 x = x.to(torch.bfloat16)
             return B8.linear_blocks(x, weight if _trains(x, weight, bias) else fp8_weight(weight), bias)
+    elif isinstance(layer_or_weight, torch.nn.Module):
+        return layer_or_weight(x.to(torch.bfloat16)).to(torch.bfloat16) if x.is_cuda else layer_or_weight(x)
     else:
         weight = layer_or_weight
     if not x.is_cuda:
