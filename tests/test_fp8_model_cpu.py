@@ -106,6 +106,16 @@ def test_block_linear():
     m.load_state_dict(state)
 
 
+def test_block_linear_refuses_an_input_that_wants_a_gradient():
+    m = quantize(torch.nn.Sequential(torch.nn.Linear(130, 64)), "fp8_block")
+    x = torch.randn(3, 130)
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        m(leaf)
+    with torch.no_grad():
+        assert torch.equal(m(leaf), m(x))
+
+
 @pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.type(torch.float32),
                                   lambda m: m.to("cpu", torch.float32), lambda m: m.to("meta").to_empty(device="cpu")])
 def test_block_linear_keeps_its_codes_when_a_module_is_cast(cast):

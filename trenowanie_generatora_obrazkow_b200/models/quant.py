@@ -103,8 +103,13 @@ class BlockLinear(nn.Module):
         self.w, self.s = (new if new.dtype == old.dtype else old.to(new.device) for new, old in zip((self.w, self.s), held))
         return self
 
-    @torch.no_grad()
     def forward(self, x):
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("BlockLinear: a weight held in 8 bits passes no gradient on (use torch.no_grad() or detach x)")
+        return self._forward(x)
+
+    @torch.no_grad()
+    def _forward(self, x):
         return B8.linear_blocks(x, B8.Blocks8(self.w, self.s, self.in_features), self.bias)
 
 
