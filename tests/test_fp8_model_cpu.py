@@ -66,6 +66,33 @@ def test_marked_blocks_run_on_8_bit_products():
     assert torch.equal(_step(*_model())[0], plain)
 
 
+def test_marked_routed_blocks():
+    from trenowanie_generatora_obrazkow_b200.models.routed import RoutedConfig, RoutedDenoiser
+    torch.manual_seed(0)
+    net = RoutedDenoiser(RoutedConfig(latent_channels=8, dim=128, depth=2, heads=2, kv_heads=2, axes=(16, 24, 24), text_dim=64,
+                                      experts=8, top_k=2, expert_hidden=128, groups=2, top_groups=1, capacity_factor=8.0))
+    z, t, text = torch.randn(2, 8, 2, 4, 4), torch.rand(2), torch.randn(2, 5, 64)
+
+    def step():
+        net.zero_grad()
+        out = net(z, t, text)
+        out.square().mean().backward()
+        return out.detach(), torch.cat([p.grad.flatten() for p in net.parameters()])
+    plain, grads = step()
+    use_fp8(net)
+    assert all(m.fp8 for b in net.blocks for m in (b.qkv, b.out, b.cross.q, b.cross.kv, b.cross.out))
+    calls = []
+    real, B8.linear_blocks = B8.linear_blocks, lambda *a: calls.append(a) or real(*a)
+    try:
+        out, g8 = step()
+    finally:
+        B8.linear_blocks = real
+    assert len(calls) == 10
+    # a value's error is at most 2^-4 of it; products of many add up like noise (a token at a border may take another expert)
+    assert 0 < ((out - plain).norm() / plain.norm()).item() < 0.2
+    assert g8.shape == grads.shape and g8.isfinite().all()
+
+
 def test_held_weights_give_the_training_forward():
     lin = torch.nn.Linear(130, 48)
     lin.fp8 = True

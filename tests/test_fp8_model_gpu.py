@@ -196,6 +196,34 @@ def test_quantized_dit(kind):
     check_errors("cuda")
 
 
+def test_marked_routed_blocks():
+    from trenowanie_generatora_obrazkow_b200.models.quant import use_fp8
+    from trenowanie_generatora_obrazkow_b200.models.routed import RoutedConfig, RoutedDenoiser
+    torch.manual_seed(0)
+    net = RoutedDenoiser(RoutedConfig(latent_channels=8, dim=256, depth=2, heads=2, kv_heads=2, axes=(32, 48, 48), text_dim=64,
+                                      experts=8, top_k=2, expert_hidden=128, groups=2, top_groups=1, capacity_factor=8.0)).cuda()
+    z, t, text = torch.randn(2, 8, 3, 7, 9, device="cuda"), torch.rand(2, device="cuda"), torch.randn(2, 5, 64, device="cuda")
+
+    def step():
+        net.zero_grad()
+        out = net(z, t, text)
+        out.float().square().mean().backward()
+        return out.detach().float(), [p.grad for p in net.parameters()]
+    plain, _ = step()
+    use_fp8(net)
+    out, grads = step()
+    # a value's error is at most 2^-4 of it; products of many add up like noise (a token at a border may take another expert)
+    assert 0 < ((out - plain).norm() / plain.norm()).item() < 0.2
+    assert all(g is not None and g.isfinite().all() for g in grads)
+    with torch.no_grad():
+        net(z, t, text)
+        kept = [net.blocks[1].cross.kv.weight._tgo_fp8, net.blocks[0].qkv.weight._tgo_fp8]
+        held = net(z, t, text).float()
+    assert kept[0] is net.blocks[1].cross.kv.weight._tgo_fp8 and kept[1] is net.blocks[0].qkv.weight._tgo_fp8
+    assert ((held - out).norm() / out.norm()).item() < 0.2
+    check_errors("cuda")
+
+
 @pytest.mark.parametrize("M", [3, 40])
 def test_far_scales(M):
     """Large activations against small weights: the product is in range, and so is the result."""

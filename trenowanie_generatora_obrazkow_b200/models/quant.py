@@ -14,8 +14,8 @@ framework's own blocks.
 * ``quantize(module, kind)``: replaces every ``nn.Linear`` below ``module`` in place (kind "int8", "fp8", "fp8_block" or
   "w8a8"; w8a8 only where both feature counts are multiples of 8, as the int8 GEMM requires) but the routers of experts,
   whose scores are computed from their weights in fp32. Plain modules, and this framework's own models for inference.
-* ``use_fp8(module)``: the linear layers of every DiT and text block below ``module`` run on 8-bit products, in training
-  forward and backward (fp32 master weights and gradients, ``ops.blocks8.linear_blocks`` / ``mlp_blocks``), without
+* ``use_fp8(module)``: the linear layers of every DiT, routed and text block below ``module`` (not the routed experts, nor
+  the routers, whose scores stay fp32) run on 8-bit products, in training forward and backward (fp32 master weights and gradients, ``ops.blocks8.linear_blocks`` / ``mlp_blocks``), without
   gradients with weights packed once per version. Parameters and checkpoints keep their names and types.
 """
 import torch
@@ -115,9 +115,10 @@ class BlockLinear(nn.Module):
 
 def use_fp8(module: nn.Module, on: bool = True) -> nn.Module:
     from .dit import DenoiserBlock
+    from .routed import RoutedBlock
     from .text import TextBlock
     for block in module.modules():
-        if isinstance(block, (DenoiserBlock, TextBlock)):
+        if isinstance(block, (DenoiserBlock, RoutedBlock, TextBlock)):
             for lin in block.modules():
                 if isinstance(lin, nn.Linear):
                     lin.fp8 = on
