@@ -65,8 +65,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // passes ov
 // 2), p = h / (1 + exp(-|a|)) and q = h each operand of a product takes a factor and they stay there, x s y = (x p) (y q).
 // For 16-bit types exp2 and the reciprocal are the hardware's approximations: s is off by (1.25 |a| + 16) 2^-24 of itself at most
 // and taken as 0 below a = -174 (s < 2^-251). A result that is rounded to 16 bits hides that; one that goes to 8 bits from
-// fp32 takes the neighbouring code where it lies as near as that to a border, one in 2^-4 / 2^-20 = 2^16. fp32 takes the
-// library's, and s whole into p where that is in range (h squared is off by twice as much).
+// fp32 takes the neighbouring code where it lies as near as that to a border, one in 2^-4 / 2^-20 = 2^16. Measured in the MLP
+// against 64-bit sums and sigmoids, y of 3000 x 1024 x 2048 in fp16 is off by 1.6e-4 (1.2e-4 with the library's; the rest is the
+// rounding of [a | b] after sums in another order), in bf16 by the same with either. The library's took 335 us instead of 220
+// in swiglu_blocks' backward at 32768 x 5504, 553 instead of 356 in the MLP's. fp32 takes the library's, and s whole into p
+// where that is in range (h squared is off by twice as much).
 template <bool FINE>
 __device__ __forceinline__ void sigmoid(float2 a, float2& p, float2& q) {
   auto one = [](float v, float& x, float& y) {
