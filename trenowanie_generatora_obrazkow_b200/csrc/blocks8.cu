@@ -414,7 +414,7 @@ cudaError_t unpack_typed(const uint8_t* codes, const uint8_t* scales, int R, int
 
 // ----------------------------------------------------------------------------------------------------------- SwiGLU
 // g in ab's type, the checkpoint of ab in 8 bits. Rows alone: a thread holds 8 columns of ROW_R rows (two: enough warps to keep
-// the memory busy; at 32768 x 5504 the backward took 265 us with four, 212 with two, and 220 with sigmoids in two factors). The checkpoint's blocks are those of a
+// the memory busy; at 32768 x 5504 the backward took 265 us with four, 212 with two; 219 with sigmoids in two factors). The checkpoint's blocks are those of a
 // [M, 2 Hp] matrix: a's first, then b's. Rows past the last are read as the last one and not written.
 constexpr int ROW_R = 2;
 template <typename T, bool VEC, bool CK>
@@ -457,7 +457,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4)
 template <bool FINE>
 __device__ __forceinline__ void swiglu_grad(float2 a, float2 b, float2 dg, float2& da, float2& db) {
   float2 p, q;
-  sigmoid<FINE>(a, p, q);
+  sigmoid<FINE>(a.x, p.x, q.x);
+  sigmoid<FINE>(a.y, p.y, q.y);
   const float2 one = make_float2(1.f, 1.f), u = fma2(a, fma2(make_float2(-p.x, -p.y), q, one), one), t = mul2(dg, p);
   da = mul2(mul2(t, mul2(b, q)), u);
   db = mul2(t, mul2(a, q));

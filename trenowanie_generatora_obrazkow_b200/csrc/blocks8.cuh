@@ -61,40 +61,33 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // passes ov
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// s = 1 / (1 + exp(-a)) = p q. s leaves fp32's range below a = -87 while products of it may be far inside: with h = exp(min(a, 0) /
-// 2), p = h / (1 + exp(-|a|)) and q = h each operand of a product takes a factor and they stay there, x s y = (x p) (y q).
+// s = 1 / (1 + exp(-a)) = p q. s leaves fp32's range below a = -87 while products of it may be far inside: there s = exp(a), and p = q
+// = 1 / (1 + exp(-a / 2)) = exp(a / 2) (to 2^-62 of it); each operand of a product takes a factor, x s y = (x p) (y q).
 // For 16-bit types exp2 and the reciprocal are the hardware's approximations: s is off by (1.25 |a| + 16) 2^-24 of itself at most
 // and taken as 0 below a = -174 (s < 2^-251). A result that is rounded to 16 bits hides that; one that goes to 8 bits from
 // fp32 takes the neighbouring code where it lies as near as that to a border, one in 2^-4 / 2^-20 = 2^16. Measured in the MLP
 // against 64-bit sums and sigmoids, y of 3000 x 1024 x 2048 in fp16 is off by 1.6e-4 (1.2e-4 with the library's; the rest is the
-// rounding of [a | b] after sums in another order), in bf16 by the same with either. The library's took 335 us instead of 220
-// in swiglu_blocks' backward at 32768 x 5504, 553 instead of 356 in the MLP's. fp32 takes the library's, and s whole into p
-// where that is in range (h squared is off by twice as much).
+// rounding of [a | b] after sums in another order), in bf16 by the same with either. The library's took 335 us instead of 219
+// in swiglu_blocks' backward at 32768 x 5504, 553 instead of 353 in the MLP's. fp32 results take the library's.
 template <bool FINE>
-__device__ __forceinline__ void sigmoid(float2 a, float2& p, float2& q) {
-  auto one = [](float v, float& x, float& y) {
-    if constexpr (FINE) {
-      const float e = expf(-fabsf(v));
-      y = 1.f;
-      if (v < -64.f) y = expf(0.5f * v);
-      x = (v >= 0.f ? 1.f : v < -64.f ? y : e) / (1.f + e);
-    } else {
-      float h, r;
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(fabsf(v) * (-0.5f * 1.4426950408889634f)));
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.f)));
-      y = v >= 0.f ? 1.f : h;
-      x = r;
-    }
-  };
-  one(a.x, p.x, q.x);
-  one(a.y, p.y, q.y);
-  if constexpr (!FINE) p = mul2(p, q);
+__device__ __forceinline__ void sigmoid(float a, float& p, float& q) {
+  const bool far = a < -87.f;
+  if constexpr (FINE) {
+    p = 1.f / (1.f + expf(far ? -0.5f * a : -a));
+  } else {
+    float t = a * -1.4426950408889634f;
+    if (far) t *= 0.5f;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(t));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(1.f + t));
+  }
+  q = far ? p : 1.f;
 }
 // silu(a) b
 template <bool FINE>
 __device__ __forceinline__ float2 swiglu(float2 a, float2 b) {
   float2 p, q;
-  sigmoid<FINE>(a, p, q);
+  sigmoid<FINE>(a.x, p.x, q.x);
+  sigmoid<FINE>(a.y, p.y, q.y);
   return mul2(mul2(a, p), mul2(b, q));
 }
 
