@@ -19,9 +19,9 @@ __device__ __forceinline__ float scale_inv(int byte) { return __uint_as_float((u
 __device__ __forceinline__ float scale_of(int byte) {                                                          // 2^e
   return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u);
 }
-// 2^e = x y with x = 2^floor(e / 2) or half of it, y = 2 or 4 x. d (x x') (y y') of two scales has no step that leaves fp32's range
-// upwards unless the result does (both factors are at least 1, or the first is less), nor downwards unless the result is less
-// than 2^-149 (|d| < 2^25 and x x' < 2^-108).
+// 2^e = x y with x = 2^floor(e / 2) or half of it, y = 2 or 4 x. d (x x') (y y') of two scales has no step that leaves fp32's
+// range upwards unless the result does (both factors are at least 1, or the first is less), nor downwards unless the result
+// is less than 2^-149 (|d| < 2^25 and x x' < 2^-108).
 __device__ __forceinline__ float2 scale_halves(int byte) {
   return make_float2(__uint_as_float((uint32_t)((byte >> 1) + 63) << 23), __uint_as_float((uint32_t)((byte + 1 >> 1) + 64) << 23));
 }
@@ -61,8 +61,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // passes ov
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// s = 1 / (1 + exp(-a)) = p q. s leaves fp32's range below a = -87 while products of it may be far inside: there s = exp(a), and p = q
-// = 1 / (1 + exp(-a / 2)) = exp(a / 2) (to 2^-62 of it); each operand of a product takes a factor, x s y = (x p) (y q).
+// s = 1 / (1 + exp(-a)) = p q. s leaves fp32's range below a = -87 while products of it may be far inside: there s = exp(a), and p
+// = q = 1 / (1 + exp(-a / 2)) = exp(a / 2) (to 2^-62 of it); each operand of a product takes a factor, x s y = (x p) (y q).
 // For 16-bit types exp2 and the reciprocal are the hardware's approximations: s is off by (1.25 |a| + 16) 2^-24 of itself at most
 // and taken as 0 below a = -174 (s < 2^-251). A result that is rounded to 16 bits hides that; one that goes to 8 bits from
 // fp32 takes the neighbouring code where it lies as near as that to a border, one in 2^-4 / 2^-20 = 2^16. Measured in the MLP

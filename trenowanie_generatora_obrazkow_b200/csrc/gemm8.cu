@@ -167,10 +167,10 @@ struct Schedule {
 // strip (32 columns), what two blocks' values and a third in fp32 leave room for in registers. The strips of a row meet in
 // shared memory, as do the quarters of a column, whose maximum over a warp's rows is one integer reduction. Codes of rows
 // leave from the registers, 32 bytes a store; those of columns through 1 KB of staging a warp, by TMA. (Through staging and
-// TMA all of them cost one of the loads' six stages: 713 us instead of 673.) At 32768 x 2048 -> 2 x 5504 a tile takes 13.7 k
-// cycles, the tensor core is busy for 60 % of them: 3.1 k go by until the shared columns are read, 1.3 k in waits for loads,
-// the rest is put down to the epilogue's traffic in shared memory beside the operands' (11.8 k without checkpoint and g's
-// columns).
+// TMA all of them cost one of the loads' six stages: 713 us instead of 673; 680 with sigmoids in two factors.) At 32768 x 2048
+// -> 2 x 5504 a tile takes 13.7 k cycles, the tensor core is busy for 55 to 60 % of them: 3.1 k go by until the shared columns
+// are read, 1.3 k in waits for loads, the rest is put down to the epilogue's traffic in shared memory beside the operands' (11.8
+// k without checkpoint and g's columns).
 // Product and activation apart took 555 + 331 us, and a and b crossed memory twice (1.4 GB).
 struct SwigluShared {
   float rows[4][3][BM];  // [strip][a, b, g][row]

@@ -18,7 +18,8 @@ operand of the weight's gradient, one byte a value. Sums are fp32; the gradients
 
 Differentiable once. The gradients of fp32 leaves (weights, biases) are accumulated in place into their ``.grad`` like those
 of ``fused.linear`` (``torch.autograd.grad`` does not return them, tensor hooks on them do not run); other weights get theirs
-from autograd in their own type. CUDA tensors run the sm_100a kernels, CPU tensors the definitions of ``reference.py``.
+from autograd in their own type. A weight or bias that requires no gradient in the forward gets none, nor does one that is
+frozen by the time of the backward. CUDA tensors run the sm_100a kernels, CPU tensors the definitions of ``reference.py``.
 """
 from typing import NamedTuple
 
