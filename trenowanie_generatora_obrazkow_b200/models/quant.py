@@ -10,13 +10,15 @@ framework's own blocks.
   applied in its epilogue (``ext().quantize_rows_i8``, ``ext().gemm_i8``); elsewhere ``torch._int_mm``. Used for
   frozen teachers only.
 * ``BlockLinear``: e4m3 weights with a power-of-two scale for each 128 inputs, activations packed the same way in the call
-  (``ops.blocks8``): one launch for up to 16 rows, the block-scaled tcgen05 product above. No gradient.
+  (``ops.blocks8``): one launch for up to 16 rows, the block-scaled tcgen05 product above. No gradient: an input that wants
+  one is refused.
 * ``quantize(module, kind)``: replaces every ``nn.Linear`` below ``module`` in place (kind "int8", "fp8", "fp8_block" or
   "w8a8"; w8a8 only where both feature counts are multiples of 8, as the int8 GEMM requires) but the routers of experts,
   whose scores are computed from their weights in fp32. Plain modules, and this framework's own models for inference.
 * ``use_fp8(module)``: the linear layers of every DiT, routed and text block below ``module`` (not the routed experts, nor
-  the routers, whose scores stay fp32) run on 8-bit products, in training forward and backward (fp32 master weights and gradients, ``ops.blocks8.linear_blocks`` / ``mlp_blocks``), without
-  gradients with weights packed once per version. Parameters and checkpoints keep their names and types.
+  the routers, whose scores stay fp32) run on 8-bit products, in training forward and backward (fp32 master weights and
+  gradients, ``ops.blocks8.linear_blocks`` / ``mlp_blocks``), without gradients with weights packed once per version.
+  Parameters and checkpoints keep their names and types.
 """
 import torch
 import torch.nn as nn
